@@ -338,7 +338,8 @@ def _own_rope(s):
     tokens, hq, hk, d = case["tokens"], case["q_heads"], case["k_heads"], case["head_dim"]
     desc = api.RopeDesc(_code(api, "PRECISION", case["dtype"]), _code(api, "ROPE", case["layout"]), case["axes"],
                         tokens, hq, hk, d, case["rotary_dim"], s["freqs"].shape[0],
-                        q_strides=(q.stride(0), q.stride(1)), k_strides=(k.stride(0), k.stride(1)), q_out_strides=(hq * d, d), k_out_strides=(hk * d, d))
+                        q_strides=(q.stride(0), q.stride(1)), k_strides=(k.stride(0), k.stride(1)),
+                        q_out_strides=(hq * d, d), k_out_strides=(hk * d, d))
     if not case["backward"]:
         q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(
             k, memory_format=torch.contiguous_format)
