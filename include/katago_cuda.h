@@ -224,6 +224,98 @@ int kc_gpool_fc(const float* d_x, const float* d_mask, int n, int c, const float
 int kc_gpool_fc_noalloc(const float* d_x, const float* d_mask, int n, int c, const float* d_w, int oc, float* d_out,
                         void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Standalone operators on board tokens: rows of consecutive channels, one row per point (channels last), in
+ * float32, f16 or bf16 (KC_PRECISION_F32 / F16 / BF16), with 32-bit statistics and sums. They have no counterpart in
+ * the reference's graph; the neighbours there are its merged batch norm with activation and mask
+ * (tools/bin2onnx/bin2onnx.py bn_act_mask, trunk_tip_rmsnorm :1440-1463) and its 2D rotary positions (:449-484,
+ * :1388-1396), whose table layouts and activations they keep.
+ *
+ * All pointers are device pointers of one device, aligned to their element (speed wants 16 bytes, and strides that
+ * are multiples of 16 bytes). Work is enqueued on `stream` (a cudaStream_t of that device, NULL = its legacy default
+ * stream) without a host wait or an allocation, so that calls can be captured into a CUDA graph; the device need not
+ * be current. Strides are in elements and not negative; rows of an output must not share memory. An output may be
+ * the input of its own shape (same pointer and strides: in place); any other overlap of an output is refused.
+ * `d_workspace` (256-byte aligned, contents not kept) must not be used by two calls that can overlap on the GPU, nor
+ * be freed before a graph that captured it. Calls on different streams are otherwise independent. Results do not
+ * depend on timing: the same call gives the same bits.
+ * --------------------------------------------------------------------------------------------------------------- */
+#define KC_ACT_IDENTITY 0
+#define KC_ACT_RELU 1
+#define KC_ACT_MISH 2
+#define KC_ACT_SILU 3
+
+/* Group norm of n boards of `points` rows of `channels`, in `groups` groups of channels / groups neighbours. */
+typedef struct kc_group_norm_desc {
+  int32_t dtype; /* KC_PRECISION_* of x, y, dy and dx */
+  int32_t act;   /* KC_ACT_* */
+  int32_t n, points, channels, groups; /* n and points may be 0 */
+  float eps;     /* >= 0 */
+  int32_t reserved; /* 0 */
+  int64_t x_board_stride, x_row_stride; /* x and dx */
+  int64_t y_board_stride, y_row_stride; /* y and dy */
+  int64_t mask_board_stride;
+} kc_group_norm_desc;
+
+/* Bytes of workspace a call needs (0: d_workspace may be NULL). backward: 0 kc_group_norm_act, 1 its backward. */
+int kc_group_norm_act_workspace(const kc_group_norm_desc* desc, int backward, size_t* bytes);
+
+/* y = act((x - mean) * rstd * weight[c] + bias[c]) at the points whose mask is not 0, 0 at the others, where mean and
+ * rstd = 1 / sqrt(variance + eps) are those of the point's board and channel group over the points that are on
+ * (whatever x holds at the others, NaN and infinities too, has no effect). d_mask: [n][points] float32 rows at
+ * mask_board_stride, NULL = every point; d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not
+ * wanted): [n][groups][2] float32 mean and rstd, both 0 for a board without points. */
+int kc_group_norm_act(const kc_group_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
+                      const float* d_bias, void* d_y, float* d_stats, void* d_workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* The gradients by x, weight and bias, given dy and the forward pass's x and d_stats: dx (0 at points that are off),
+ * d_dweight and d_dbias [channels] float32 (sums over all boards, overwritten; each may be NULL). relu has slope 0
+ * at 0. */
+int kc_group_norm_act_backward(const kc_group_norm_desc* desc, const void* d_x, const float* d_mask,
+                               const float* d_weight, const float* d_bias, const float* d_stats, const void* d_dy,
+                               void* d_dx, float* d_dweight, float* d_dbias, void* d_workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Rotary positions with several axes, on Q and K heads. Pair j of a head, j < rotary_dim / 2, is turned by
+ * angle[t][table][j] = sum over axes a of pos[t][a] * freqs[table][j][a]; head dimensions from rotary_dim on pass
+ * unchanged. The frequencies are the reference's learned table layout (bin2onnx.py :1388-1396: [kv_heads][pairs][2]
+ * with the axes x, y); kc_rope_axes_freqs makes fixed ones. */
+#define KC_ROPE_HALVES 0 /* pair j = dimensions j and j + rotary_dim / 2 */
+#define KC_ROPE_PAIRS 1  /* pair j = dimensions 2 j and 2 j + 1 */
+#define KC_ROPE_MAX_AXES 4
+typedef struct kc_rope_desc {
+  int32_t dtype;   /* KC_PRECISION_* of q, k and their outputs and gradients */
+  int32_t layout;  /* KC_ROPE_* */
+  int32_t axes;    /* 1 .. KC_ROPE_MAX_AXES */
+  int32_t q_heads, k_heads; /* k_heads 0: no k (all k pointers are ignored) */
+  int32_t head_dim, rotary_dim; /* rotary_dim even, 2 .. head_dim; head_dim <= 1024 */
+  int32_t tables;  /* 1, or a divisor of q_heads and k_heads: head h of H uses table h / (H / tables) */
+  int64_t tokens;  /* may be 0 */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+} kc_rope_desc;
+
+/* The frequencies of fixed rotary positions, into the host array freqs [rotary_dim / 2][axes]: axis a turns
+ * sections[a] pairs (the sections add up to rotary_dim / 2; axis 0 has the first ones), pair i of its section by
+ * theta^(-i / sections[a]) per step. No device is used. */
+int kc_rope_axes_freqs(int axes, const int32_t* sections, double theta, int rotary_dim, float* freqs);
+
+/* Turns q and k: q_out[t][h] = R(angle) q[t][h]. d_pos: [tokens][axes] int32 (any sign), d_freqs:
+ * [tables][rotary_dim / 2][axes] float32. Angles are held in 64 bits: positions keep their full resolution. */
+int kc_rope_axes(const kc_rope_desc* desc, const void* d_q, const void* d_k, const int32_t* d_pos,
+                 const float* d_freqs, void* d_q_out, void* d_k_out, void* stream);
+
+/* The gradients by q and k (turned back by the same angles), and by the frequencies when d_dfreqs is not NULL:
+ * d_dq_out, d_dk_out are the gradients of kc_rope_axes' outputs (at q_out's and k_out's strides), d_q and d_k its
+ * inputs (only read for d_dfreqs, may be NULL otherwise), d_dq and d_dk the results (at q's and k's strides; in place
+ * of d_dq_out / d_dk_out where those strides are the same), d_dfreqs [tables][rotary_dim / 2][axes] float32
+ * (overwritten). The workspace is for d_dfreqs only. */
+int kc_rope_axes_backward_workspace(const kc_rope_desc* desc, size_t* bytes);
+int kc_rope_axes_backward(const kc_rope_desc* desc, const void* d_dq_out, const void* d_dk_out, const void* d_q,
+                          const void* d_k, const int32_t* d_pos, const float* d_freqs, void* d_dq, void* d_dk,
+                          float* d_dfreqs, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* Failure-detection self-test. Every spin-wait in this library's kernels is bounded: when a wait runs out, the
  * kernel records an error code in the handle's device error word, releases what it holds and returns, and the next
  * kc_wait / kc_synchronize reports KC_ERR_DEVICE (the handle stays usable). This enqueues on the handle's stream

@@ -18,6 +18,9 @@ PKG = os.path.dirname(os.path.dirname(HERE))  # katago-rs_b200/
 HEADER = os.path.join(os.path.dirname(PKG), "include", "katago_cuda.h")
 
 PRECISION_F32, PRECISION_F16, PRECISION_BF16, PRECISION_AUTO = 0, 1, 2, 3
+ACT_IDENTITY, ACT_RELU, ACT_MISH, ACT_SILU = range(4)
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_MAX_AXES = 4
 KC_OK, KC_ERR_INVALID, KC_ERR_PARSE, KC_ERR_CUDA, KC_ERR_TIMEOUT, KC_ERR_DEVICE, KC_ERR_NO_DEVICE = range(7)
 
 _LIB = None
@@ -59,6 +62,64 @@ class Desc(ctypes.Structure):
     ]
 
 
+class GroupNormDesc(ctypes.Structure):
+    """kc_group_norm_desc. dtype: PRECISION_*, act: ACT_*; x_strides, y_strides: (board, row) strides in elements,
+    None = contiguous; mask_stride: elements from one board's mask to the next, None = points."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("points", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("x_board_stride", ctypes.c_int64),
+        ("x_row_stride", ctypes.c_int64),
+        ("y_board_stride", ctypes.c_int64),
+        ("y_row_stride", ctypes.c_int64),
+        ("mask_board_stride", ctypes.c_int64),
+    ]
+
+    def __init__(self, dtype, act, n, points, channels, groups, eps, x_strides=None, y_strides=None,
+                 mask_stride=None):
+        whole = (points * channels, channels)
+        super().__init__(dtype, act, n, points, channels, groups, eps, 0, *(x_strides or whole),
+                         *(y_strides or whole), points if mask_stride is None else mask_stride)
+
+
+class RopeDesc(ctypes.Structure):
+    """kc_rope_desc. dtype: PRECISION_*, layout: ROPE_*; the strides are (token, head) in elements, None =
+    contiguous [tokens][heads][head_dim]."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("tables", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("q_out_token_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_token_stride", ctypes.c_int64),
+        ("k_out_head_stride", ctypes.c_int64),
+    ]
+
+    def __init__(self, dtype, layout, axes, tokens, q_heads, k_heads, head_dim, rotary_dim, tables=1, q_strides=None,
+                 k_strides=None, q_out_strides=None, k_out_strides=None):
+        q, k = (q_heads * head_dim, head_dim), (k_heads * head_dim, head_dim)
+        super().__init__(dtype, layout, axes, q_heads, k_heads, head_dim, rotary_dim, tables, tokens,
+                         *(q_strides or q), *(k_strides or k), *(q_out_strides or q), *(k_out_strides or k))
+
+
 P = ctypes.c_void_p
 I = ctypes.c_int
 FP = ctypes.POINTER(ctypes.c_float)
@@ -90,6 +151,13 @@ _SIGS = {
     "kc_copy_with_symmetry": ([FP, FP, I, I, I, I, I, I], I),
     "kc_gpool_fc": ([P, P, I, I, P, I, P, P], I),
     "kc_gpool_fc_noalloc": ([P, P, I, I, P, I, P, P], I),
+    "kc_group_norm_act_workspace": ([ctypes.POINTER(GroupNormDesc), I, ctypes.POINTER(ctypes.c_size_t)], I),
+    "kc_group_norm_act": ([ctypes.POINTER(GroupNormDesc), P, P, P, P, P, P, P, ctypes.c_size_t, P], I),
+    "kc_group_norm_act_backward": ([ctypes.POINTER(GroupNormDesc)] + [P] * 10 + [ctypes.c_size_t, P], I),
+    "kc_rope_axes_freqs": ([I, ctypes.POINTER(ctypes.c_int32), ctypes.c_double, I, FP], I),
+    "kc_rope_axes": ([ctypes.POINTER(RopeDesc), P, P, P, P, P, P, P], I),
+    "kc_rope_axes_backward_workspace": ([ctypes.POINTER(RopeDesc), ctypes.POINTER(ctypes.c_size_t)], I),
+    "kc_rope_axes_backward": ([ctypes.POINTER(RopeDesc)] + [P] * 10 + [ctypes.c_size_t, P], I),
     "kc_selftest_device_timeout": ([P, I], I),
     "kc_handle_packed_input_ptrs": ([P, ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32)), FPP, FPP,
                                      ctypes.POINTER(ctypes.POINTER(ctypes.c_int32)), FPP], I),
@@ -337,6 +405,57 @@ def gpool_fc(d_x: int, d_mask: int, n: int, c: int, d_w: int, oc: int, d_out: in
 def gpool_fc_noalloc(d_x: int, d_mask: int, n: int, c: int, d_w: int, oc: int, d_out: int, stream: int = 0):
     """kc_gpool_fc_noalloc: the same operator with its scratch in a fixed device array (no allocation)."""
     _check(lib().kc_gpool_fc_noalloc(d_x, d_mask, n, c, d_w, oc, d_out, stream or None))
+
+
+def group_norm_act_workspace(desc: GroupNormDesc, backward: bool) -> int:
+    """kc_group_norm_act_workspace: bytes of device workspace a forward or backward call needs."""
+    n = ctypes.c_size_t()
+    _check(lib().kc_group_norm_act_workspace(desc, backward, n))
+    return n.value
+
+
+def group_norm_act(desc: GroupNormDesc, d_x: int, d_mask: int, d_weight: int, d_bias: int, d_y: int, d_stats: int = 0,
+                   d_workspace: int = 0, workspace_bytes: int = 0, stream: int = 0):
+    """kc_group_norm_act on device pointers (masked group norm and activation, channels last; 0 = not given)."""
+    _check(lib().kc_group_norm_act(desc, d_x, d_mask, d_weight, d_bias, d_y, d_stats, d_workspace, workspace_bytes,
+                                   stream))
+
+
+def group_norm_act_backward(desc: GroupNormDesc, d_x: int, d_mask: int, d_weight: int, d_bias: int, d_stats: int,
+                            d_dy: int, d_dx: int, d_dweight: int = 0, d_dbias: int = 0, d_workspace: int = 0,
+                            workspace_bytes: int = 0, stream: int = 0):
+    """kc_group_norm_act_backward on device pointers: the gradients by x, weight and bias."""
+    _check(lib().kc_group_norm_act_backward(desc, d_x, d_mask, d_weight, d_bias, d_stats, d_dy, d_dx, d_dweight,
+                                            d_dbias, d_workspace, workspace_bytes, stream))
+
+
+def rope_axes_freqs(sections: Sequence[int], theta: float, rotary_dim: int) -> np.ndarray:
+    """kc_rope_axes_freqs: fixed rotary frequencies [rotary_dim / 2, axes] float32, axis a turning sections[a] pairs."""
+    axes = len(sections)
+    out = np.zeros((max(0, rotary_dim // 2), axes), np.float32)
+    _check(lib().kc_rope_axes_freqs(axes, (ctypes.c_int32 * axes)(*sections), theta, rotary_dim, _fp(out)))
+    return out
+
+
+def rope_axes(desc: RopeDesc, d_q: int, d_k: int, d_pos: int, d_freqs: int, d_q_out: int, d_k_out: int,
+              stream: int = 0):
+    """kc_rope_axes on device pointers: Q and K heads turned by their positions on several axes."""
+    _check(lib().kc_rope_axes(desc, d_q, d_k, d_pos, d_freqs, d_q_out, d_k_out, stream))
+
+
+def rope_axes_backward_workspace(desc: RopeDesc) -> int:
+    """kc_rope_axes_backward_workspace: bytes of device workspace a backward call with d_dfreqs needs."""
+    n = ctypes.c_size_t()
+    _check(lib().kc_rope_axes_backward_workspace(desc, n))
+    return n.value
+
+
+def rope_axes_backward(desc: RopeDesc, d_dq_out: int, d_dk_out: int, d_q: int, d_k: int, d_pos: int, d_freqs: int,
+                       d_dq: int, d_dk: int, d_dfreqs: int = 0, d_workspace: int = 0, workspace_bytes: int = 0,
+                       stream: int = 0):
+    """kc_rope_axes_backward on device pointers: the gradients by q, k and (d_dfreqs) the frequencies."""
+    _check(lib().kc_rope_axes_backward(desc, d_dq_out, d_dk_out, d_q, d_k, d_pos, d_freqs, d_dq, d_dk, d_dfreqs,
+                                       d_workspace, workspace_bytes, stream))
 
 
 def pack_spatial(planes: np.ndarray) -> np.ndarray:

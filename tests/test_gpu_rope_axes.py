@@ -1,0 +1,230 @@
+"""kc_rope_axes and its backward pass against float64.
+
+Tolerances. y = x1 cos - x2 sin: one rounding to the type, and in float32 the sine and cosine are off by at most
+2^-21 (angle reduced in 64 bits to half a turn, rounded to 24 bits: 2 pi 2^-26; 2 half steps of 2^-24 more from the
+function; sine and cosine of 2-byte types may come from the fast functions, off by 2^-21 more), two products and a sum
+by 2 half steps: S = 2^-20 of |x1| + |x2| covers both. The angle itself is a float64 sum: off by 2^-51 of its size.
+The frequencies' gradient adds terms pos * d angle, each off by 2 S of its size, over chains of below 128 float32
+additions (128 * 2^-24 = 2^-17)."""
+
+import pytest
+import torch
+
+import token_ops as t
+from katago_cuda import api
+
+pytestmark = pytest.mark.gpu
+
+S = 2.0**-20
+
+
+def make(tokens, hq, hk, hd, rd, axes, tables, dtype, seed, far=361):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    wide = torch.empty(tokens, hq + 2 * hk, hd, device="cuda").normal_(generator=g).to(t.DTYPES[dtype])
+    q, k = wide[:, :hq], wide[:, hq:hq + hk] if hk else None
+    pos = torch.randint(-far, far, (tokens, axes), device="cuda", generator=g, dtype=torch.int32)
+    freqs = torch.empty(tables, rd // 2, axes, device="cuda").normal_(0, 0.5, generator=g)
+    return wide, q, k, pos, freqs, g
+
+
+def check(got, x, pos, freqs, rd, layout, back=False):
+    want, size = t.turn64(x, pos, freqs, rd, layout, back)
+    half, tiny = t.half_step(x.dtype)
+    angle = torch.einsum("ta,hja->thj", pos.double().abs(), freqs.double().abs()).amax()
+    t.within(got, want, half * want.abs() + torch.where(size > 0, tiny, 0.0) + (S + angle * 2.0**-51) * size)
+    assert torch.equal(got[..., rd:], x[..., rd:])
+
+
+CASES = [
+    # tokens, q heads, k heads, head dim, rotary dim, axes, tables
+    (1, 6, 6, 64, 64, 2, 1), (1, 1, 0, 2, 2, 1, 1), (722, 6, 2, 64, 64, 2, 2), (361, 12, 12, 64, 32, 3, 12),
+    (100, 16, 4, 128, 96, 3, 1), (33, 4, 4, 102, 102, 2, 4), (50, 3, 1, 30, 10, 4, 1), (17, 8, 2, 16, 16, 1, 2),
+    (4099, 2, 1, 64, 48, 3, 1), (9, 2, 2, 1024, 1024, 2, 1), (65, 36, 12, 32, 32, 3, 12), (5, 7, 7, 18, 18, 2, 7),
+    (3000, 1, 1, 8, 6, 2, 1), (40, 64, 8, 128, 128, 3, 1),
+]
+
+
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens,hq,hk,hd,rd,axes,tables", CASES)
+def test_forward_and_backward(tokens, hq, hk, hd, rd, axes, tables, dtype, layout):
+    wide, q, k, pos, freqs, g = make(tokens, hq, hk, hd, rd, axes, tables, dtype, tokens)
+    q_out, k_out = t.rope_forward(q, k, pos, freqs, rd, layout)
+    check(q_out, q, pos, freqs, rd, layout)
+    dq_out = torch.randn(q.shape, device="cuda", generator=g).to(q.dtype)
+    dk_out = None
+    if k is not None:
+        check(k_out, k, pos, freqs, rd, layout)
+        dk_out = torch.randn(k.shape, device="cuda", generator=g).to(q.dtype)
+    for learned in (True, False):
+        grads = torch.full_like(wide, 3.0)
+        dq, dk, df = t.rope_backward(dq_out, dk_out, q, k, pos, freqs, rd, layout, dq=grads[:, :hq],
+                                     dk=None if k is None else grads[:, hq:hq + hk], learned=learned)
+        check(dq, dq_out, pos, freqs, rd, layout, back=True)
+        if k is not None:
+            check(dk, dk_out, pos, freqs, rd, layout, back=True)
+            assert grads[:, hq + hk:].eq(3).all()
+        if learned:
+            want, size = t.freqs_back64(dq_out, q, dk_out, k, pos, freqs, rd, layout)
+            t.within(df, want, (2 * S + 2.0**-17) * size)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+def test_strides_in_place_and_one_buffer(dtype, layout):
+    tokens, hq, hk, hd, rd = 77, 6, 2, 64, 48
+    wide, q, k, pos, freqs, g = make(tokens, hq, hk, hd, rd, 2, 2, dtype, 3)
+    want = t.rope_forward(q, k, pos, freqs, rd, layout)
+    # head-major outputs
+    qo, ko = (torch.full((h, tokens, hd), 5.0, device="cuda").to(q.dtype).transpose(0, 1) for h in (hq, hk))
+    t.rope_forward(q, k, pos, freqs, rd, layout, qo, ko)
+    assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
+    # outputs side by side in one buffer with a guard behind each head
+    buf = torch.full((tokens, hq + hk, hd + 8), 5.0, device="cuda").to(q.dtype)
+    t.rope_forward(q, k, pos, freqs, rd, layout, buf[:, :hq, :hd], buf[:, hq:, :hd])
+    assert torch.equal(buf[:, :hq, :hd], want[0]) and torch.equal(buf[:, hq:, :hd], want[1])
+    assert buf[:, :, hd:].eq(5).all()
+    # rows behind the last token stay as they were
+    buf = torch.full((tokens + 3, hq + hk, hd), 5.0, device="cuda").to(q.dtype)
+    t.rope_forward(q, k, pos, freqs, rd, layout, buf[:tokens, :hq], buf[:tokens, hq:])
+    assert buf[tokens:].eq(5).all()
+    # an odd element offset
+    flat = torch.zeros(wide.numel() + 8, device="cuda").to(q.dtype)
+    off = flat[3:3 + wide.numel()].view_as(wide)
+    off.copy_(wide)
+    got = t.rope_forward(off[:, :hq], off[:, hq:hq + hk], pos, freqs, rd, layout)
+    check(got[0], q, pos, freqs, rd, layout)
+    check(got[1], k, pos, freqs, rd, layout)
+    # in place, V columns untouched; and the gradient in place
+    v = wide[:, hq + hk:].clone()
+    dq_out, dk_out = want[0].clone(), want[1].clone()
+    q0, k0 = q.clone(), k.clone()
+    back = t.rope_backward(dq_out, dk_out, q0, k0, pos, freqs, rd, layout)
+    t.rope_forward(q, k, pos, freqs, rd, layout, q, k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(wide[:, hq + hk:], v)
+    got = t.rope_backward(dq_out, dk_out, q0, k0, pos, freqs, rd, layout, dq=dq_out, dk=dk_out)
+    assert all(torch.equal(a, b) for a, b in zip(got, back))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_far_positions(dtype):
+    """Positions up to the ends of int32 keep the resolution of one step."""
+    tokens = 64
+    wide, q, k, pos, freqs, g = make(tokens, 2, 2, 64, 64, 2, 1, dtype, 7, far=2**31 - 1)
+    pos[0] = -2**31
+    pos[1] = 2**31 - 1
+    q_out, k_out = t.rope_forward(q, k, pos, freqs, 64, "halves")
+    check(q_out, q, pos, freqs, 64, "halves")
+    check(k_out, k, pos, freqs, 64, "halves")
+    # one axis with a frequency of 1: a step at 10^6 turns by what a step at 0 does
+    near = torch.arange(8, device="cuda", dtype=torch.int32)[:, None]
+    one = torch.ones(1, 1, 1, device="cuda")
+    x = torch.ones(8, 1, 2, device="cuda")
+    a, _ = t.rope_forward(x, None, near + 1000000, one, 2, "pairs")
+    check(a, x, near + 1000000, one, 2, "pairs")
+
+
+def test_same_as_the_engine_on_a_board():
+    """Two axes with the reference's fixed table on a 19x19 board, halves layout: the rotation of the engine's float32
+    tier (tables rounded to float32 from float32 angles: 18 * 2^-24 + 2^-24 off)."""
+    pos = torch.stack([torch.arange(361) // 19, torch.arange(361) % 19], 1).int().cuda()
+    freqs = torch.from_numpy(api.rope_axes_freqs([16, 16], 100.0, 64)).cuda()[None]
+    q = torch.randn(361, 6, 64, device="cuda")
+    got, _ = t.rope_forward(q, None, pos, freqs, 64, "halves")
+    angle = (pos.float()[:, None, :] * freqs).sum(2)[:, None, :]
+    c, s = torch.cos(angle), torch.sin(angle)
+    want = torch.cat([q[..., :32] * c - q[..., 32:] * s, q[..., :32] * s + q[..., 32:] * c], 2)
+    assert (got - want).abs().max() <= 2 * (19 * 2.0**-24 + S) * q.abs().max()
+
+
+def test_gradient_of_frequencies_is_the_difference_quotient():
+    """sum(g * y) along a random direction of the frequencies, in float64: the quotient's error is h^2 / 6 of a third
+    derivative, |pos|^2 h^2 / 6 (below 1e-7 at |pos| <= 20, h = 3e-5) of the terms' size."""
+    for layout in t.LAYOUTS:
+        wide, q, k, pos, freqs, g = make(300, 4, 2, 32, 24, 3, 2, "f32", 13, far=20)
+        dq_out, dk_out = (torch.randn(v.shape, device="cuda", generator=g) for v in (q, k))
+        _, _, df = t.rope_backward(dq_out, dk_out, q, k, pos, freqs, 24, layout)
+        v = torch.randn(freqs.shape, device="cuda", generator=g).double()
+
+        def loss(h):
+            f = freqs.double() + h * v
+            return sum((t.turn64(x, pos, f, 24, layout)[0] * o.double()).sum().item() for x, o in ((q, dq_out), (k, dk_out)))
+
+        h = 3e-5
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        _, size = t.freqs_back64(dq_out, q, dk_out, k, pos, freqs, 24, layout)
+        assert abs((df.double() * v).sum().item() - slope) <= (2 * S + 2.0**-17 + 1e-6) * (size * v.abs()).sum().item()
+
+
+def test_turned_back_is_the_input():
+    """The backward pass undoes the rotation: two roundings and 2 S of |x1| + |x2|."""
+    wide, q, k, pos, freqs, g = make(500, 6, 6, 64, 64, 2, 6, "f32", 23)
+    q_out, k_out = t.rope_forward(q, k, pos, freqs, 64, "halves")
+    dq, dk, _ = t.rope_backward(q_out, k_out, q, k, pos, freqs, 64, "halves", learned=False)
+    assert (dq - q).abs().max() <= 8 * S * q.abs().max() and (dk - k).abs().max() <= 8 * S * k.abs().max()
+
+
+def test_same_bits_again_on_other_streams_and_in_graphs():
+    wide, q, k, pos, freqs, g = make(2000, 6, 2, 64, 64, 2, 2, "bf16", 29)
+    dq_out, dk_out = (torch.randn(v.shape, device="cuda", generator=g).bfloat16() for v in (q, k))
+
+    def both():
+        return t.rope_forward(q, k, pos, freqs, 64, "halves") + t.rope_backward(dq_out, dk_out, q, k, pos, freqs, 64,
+                                                                                "halves")
+
+    want = both()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(both())
+    torch.cuda.synchronize()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            r = both()
+        graphs.append((gr, r))
+    for _ in range(3):
+        for gr, r in graphs:
+            for v in r:
+                v.fill_(9)
+        torch.cuda.synchronize()
+        for s, (gr, r) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                gr.replay()
+        torch.cuda.synchronize()
+        for gr, r in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
+def test_offsets_past_32_bits():
+    far = (1 << 31) + 64
+    wide, q, k, pos, freqs, g = make(3, 2, 1, 64, 64, 2, 1, "f16", 31)
+    want = t.rope_forward(q, k, pos, freqs, 64, "pairs")
+    buf = torch.empty(2 * far + 256, dtype=torch.float16, device="cuda")
+    qf, kf = buf.as_strided((3, 2, 64), (far, 64, 1)), buf[128:].as_strided((3, 1, 64), (far, 64, 1))
+    qf.copy_(q)
+    kf.copy_(k)
+    t.rope_forward(qf, kf, pos, freqs, 64, "pairs", qf, kf)
+    assert torch.equal(qf, want[0]) and torch.equal(kf, want[1])
+
+
+def test_no_tokens():
+    d = api.RopeDesc(api.PRECISION_F16, api.ROPE_HALVES, 2, 0, 6, 2, 64, 64, 2)
+    df = torch.full((2, 32, 2), 5.0, device="cuda")
+    api.rope_axes_backward(d, 0, 0, 0, 0, 0, 0, 0, 0, df.data_ptr(), 0, 0, t.stream())
+    assert df.eq(0).all()
+
+
+def test_host_memory_is_refused():
+    wide, q, k, pos, freqs, g = make(4, 2, 2, 16, 16, 2, 1, "f32", 37)
+    d = t.rope_desc(q, k, q, k, 16, "halves", 2, 1)
+    with pytest.raises(api.KcError) as e:
+        api.rope_axes(d, q.data_ptr(), k.data_ptr(), pos.cpu().data_ptr(), freqs.data_ptr(), q.data_ptr(), k.data_ptr(),
+                      t.stream())
+    assert e.value.status == api.KC_ERR_INVALID and "device memory" in str(e.value)
