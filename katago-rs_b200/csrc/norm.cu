@@ -14,11 +14,12 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
 #include "../../include/katago_cuda.h"
-#include "gemm.cuh"
+#include "gemm_pair.cuh"
 #include "ops_common.h"
 
 namespace kc {
@@ -26,6 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTiles = 64;
+constexpr int kMaxSmem = 227 * 1024;  // of a block
 
 struct NormParams {
   const void* x;
@@ -102,6 +104,632 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 #pragma unroll
   for (int j = 0; j < VEC; j++) u.v[j] = from_f<T>(v[j]);
   *reinterpret_cast<Pack<T, VEC>*>(p) = u;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The resident path: a chunk of whole groups (V column vectors of VEC channels) of one board is read once and stays
+// in the shared memory of a block, or of a cluster of blocks that share the board's points, until it is written. A
+// thread owns `slots` vectors of one column vector: rows ty, ty + R, ... of its block's points, R = threads / V; it
+// copies them in itself (cp.async), so that no barrier stands between the copy and the statistics.
+// U neighbouring channels of a vector lie in one group (VEC, 4 or 1 of them), so that a thread's statistics are
+// VEC / U triples of (count, mean, sum of squares around it).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kMaxSlots = 32;  // a thread's rows are bits of one word
+
+struct ResShape {
+  int cw;      // channels of a chunk (the last one of a row may have fewer)
+  int cs, cs_log2;  // blocks of a cluster
+  int rows;    // points per block
+  int threads;
+  int R;       // rows at once
+  int slots;
+  int spec;    // copies x before the mask is known (few blocks: latency counts, not bytes)
+  int wvec;    // weight and bias may be read as 16-byte vectors
+};
+
+// A vector as pairs of floats (one channel: the second is 0).
+template <typename T, int VEC>
+struct Vec {
+  static constexpr int NP = (VEC + 1) / 2;
+  static constexpr int BYTES = VEC * (int)sizeof(T);
+  using Raw = typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2,
+              typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type;
+
+  __device__ static __forceinline__ f32x2 word(uint32_t w) {  // two 2-byte values
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      return {f.x, f.y};
+    }
+  }
+  __device__ static __forceinline__ void unpack(Raw r, f32x2 (&v)[NP]) {
+    if constexpr (VEC == 1) {
+      v[0] = {to_f<T>(*reinterpret_cast<const T*>(&r)), 0.0f};
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        if constexpr (sizeof(T) == 4) v[i] = {__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])};
+        else v[i] = word(w[i]);
+      }
+    }
+  }
+  __device__ static __forceinline__ Raw pack(const f32x2 (&v)[NP]) {
+    Raw r;
+    if constexpr (VEC == 1) {
+      *reinterpret_cast<T*>(&r) = from_f<T>(v[0].x);
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        if constexpr (sizeof(T) == 4) {
+          w[2 * i] = __float_as_uint(v[i].x);
+          w[2 * i + 1] = __float_as_uint(v[i].y);
+        } else {
+          w[i] = pack2<T>(v[i].x, v[i].y);
+        }
+      }
+    }
+    return r;
+  }
+  // global -> shared; complete for the issuing thread after copies_done()
+  __device__ static __forceinline__ void copy_in(Raw* dst, const T* src) {
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else if constexpr (BYTES >= 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+    else
+      *dst = *reinterpret_cast<const Raw*>(src);
+  }
+};
+
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ float2 ld_cluster(const float2* p, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster(const int* p, uint32_t rank) {
+  int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// act of two elements. One reciprocal serves both: the divisors' product stays below 2^127 (mish: (e^40 + ..)^2;
+// silu: exp(-z) is held to 2^60, where z sigma(z) is below 2^-53).
+template <int ACT>
+__device__ __forceinline__ f32x2 act2(f32x2 z) {
+  if constexpr (ACT == KC_ACT_RELU) {
+    return {z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y};
+  } else if constexpr (ACT == KC_ACT_MISH) {
+    const f32x2 t = mul2(z, {kLog2e, kLog2e});
+    const f32x2 e = {ex2(fminf(t.x, 20.0f * kLog2e)), ex2(fminf(t.y, 20.0f * kLog2e))};
+    const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
+    const f32x2 d = add2(n, {2.0f, 2.0f});
+    const float r = rcp(d.x * d.y);
+    return mul2(z, mul2(n, mul2({d.y, d.x}, {r, r})));
+  } else if constexpr (ACT == KC_ACT_SILU) {
+    const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
+    const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
+    const float r = rcp(d.x * d.y);
+    return mul2(z, mul2({d.y, d.x}, {r, r}));
+  } else {
+    return z;
+  }
+}
+
+// act' of two elements (relu apart: relu_on).
+// mish = z n / d with e = exp(z), n = e^2 + 2 e, d = n + 2: mish' = n / d + z 4 e (e + 1) / d^2 (above 20: 1).
+// silu' = s (1 + z (1 - s)), s = 1 / (1 + exp(-z)).
+template <int ACT>
+__device__ __forceinline__ f32x2 slope2(f32x2 z) {
+  if constexpr (ACT == KC_ACT_MISH) {
+    const f32x2 t = mul2(z, {kLog2e, kLog2e});
+    const f32x2 e = {ex2(fminf(t.x, 20.0f * kLog2e)), ex2(fminf(t.y, 20.0f * kLog2e))};
+    const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
+    const f32x2 d = add2(n, {2.0f, 2.0f});
+    const float r = rcp(d.x * d.y);
+    const f32x2 rd = mul2({d.y, d.x}, {r, r});
+    const f32x2 er = mul2(e, rd);                                 // e / d
+    const f32x2 k = mul2({4.0f, 4.0f}, mul2(er, add2(er, rd)));   // 4 e (e + 1) / d^2
+    return fma2(z, k, mul2(n, rd));
+  } else if constexpr (ACT == KC_ACT_SILU) {
+    const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
+    const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
+    const float r = rcp(d.x * d.y);
+    const f32x2 s = mul2({d.y, d.x}, {r, r});
+    const f32x2 u = fma2({-s.x, -s.y}, z, z);                     // z (1 - s)
+    return fma2(s, u, s);
+  } else {
+    return {1.0f, 1.0f};
+  }
+}
+
+// a / b of small non-negative integers (a < 2^20): the quotient's fraction is at least 1 / (2 b) off a border.
+__device__ __forceinline__ int small_div(int a, int b) { return (int)(((float)a + 0.5f) / (float)b); }
+
+struct ResIds {
+  int b, rank, c0, tx, ty, V;
+  int first, count;  // the thread's first point and how many (first + i R)
+};
+
+template <int VEC>
+__device__ __forceinline__ ResIds res_ids(const NormParams& p, const ResShape& s) {
+  ResIds t;
+  t.b = blockIdx.z * 65535 + blockIdx.y;
+  t.rank = blockIdx.x & (s.cs - 1);
+  t.c0 = (blockIdx.x >> s.cs_log2) * s.cw;
+  const int vfull = s.cw / VEC;
+  t.V = min(s.cw, p.C - t.c0) / VEC;
+  t.ty = small_div(threadIdx.x, vfull);
+  t.tx = threadIdx.x - t.ty * vfull;
+  const int r0 = t.rank * s.rows, r1 = min(p.points, r0 + s.rows);
+  t.first = r0 + t.ty;
+  t.count = t.ty < s.R && t.tx < t.V && t.first < r1 ? small_div(r1 - t.first + s.R - 1, s.R) : 0;
+  return t;
+}
+
+__device__ __forceinline__ uint32_t low_bits(int k) { return k >= 32 ? 0xffffffffu : (1u << k) - 1; }
+
+// Which of the thread's rows are on, as bits.
+__device__ __forceinline__ uint32_t on_bits(const NormParams& p, const ResShape& s, const ResIds& t) {
+  if (!p.mask) return low_bits(t.count);
+  const float* m = p.mask + (int64_t)t.b * p.mb + t.first;
+  uint32_t on = 0;
+#pragma unroll 4
+  for (int i = 0; i < t.count; i++, m += s.R)
+    if (__ldg(m) != 0.0f) on |= 1u << i;
+  return on;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_rows(const T* x, int64_t stride, const ResShape& s, const ResIds& t, uint32_t which,
+                                          typename Vec<T, VEC>::Raw* slot) {
+  x += t.first * stride;
+  stride *= s.R;
+#pragma unroll 4
+  for (int i = 0; i < t.count; i++, which >>= 1, x += stride, slot += s.threads)
+    if (which & 1) Vec<T, VEC>::copy_in(slot, x);
+}
+
+// f(vector) of the rows that are on.
+template <typename T, int VEC, typename F>
+__device__ __forceinline__ void each_on(const typename Vec<T, VEC>::Raw* slot, int threads, int count, uint32_t on, F&& f) {
+#pragma unroll 4
+  for (int i = 0; i < count; i++, on >>= 1, slot += threads)
+    if (on & 1) {
+      f32x2 v[Vec<T, VEC>::NP];
+      Vec<T, VEC>::unpack(*slot, v);
+      f(v);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_params(const float* w, float other, bool vec, int col,
+                                            f32x2 (&o)[(VEC + 1) / 2]) {
+  if (!w) {
+#pragma unroll
+    for (int j = 0; j < (VEC + 1) / 2; j++) o[j] = {other, other};
+  } else if (VEC % 4 == 0 && vec) {
+#pragma unroll
+    for (int j = 0; j < VEC / 4; j++) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(w + col) + j);
+      o[2 * j] = {f.x, f.y};
+      o[2 * j + 1] = {f.z, f.w};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < (VEC + 1) / 2; j++)
+      o[j] = {__ldg(w + col + 2 * j), VEC > 1 ? __ldg(w + col + 2 * j + 1) : other};
+  }
+}
+
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void apply_rows(const ResShape& s, const ResIds& t, uint32_t on,
+                                           const typename Vec<T, VEC>::Raw* slot, T* y, int64_t stride,
+                                           const f32x2 (&neg_mean)[Vec<T, VEC>::NP], const f32x2 (&a)[Vec<T, VEC>::NP],
+                                           const f32x2 (&b)[Vec<T, VEC>::NP]) {
+  using V = Vec<T, VEC>;
+  y += t.first * stride;
+  stride *= s.R;
+#pragma unroll 2
+  for (int i = 0; i < t.count; i++, on >>= 1, y += stride, slot += s.threads) {
+    f32x2 v[V::NP] = {};
+    if (on & 1) {
+      V::unpack(*slot, v);
+#pragma unroll
+      for (int j = 0; j < V::NP; j++) v[j] = act2<ACT>(fma2(add2(v[j], neg_mean[j]), a[j], b[j]));
+    }
+    *reinterpret_cast<typename V::Raw*>(y) = V::pack(v);
+  }
+}
+
+extern __shared__ __align__(16) unsigned char norm_smem[];
+
+template <typename T, int VEC, int U>
+__global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constant__ NormParams p,
+                                                            const __grid_constant__ ResShape sh) {
+  using V = Vec<T, VEC>;
+  constexpr int NU = VEC / U, NP = V::NP;
+  const ResIds t = res_ids<VEC>(p, sh);
+  if (t.b >= p.n) return;
+  const int units = sh.cw / U;  // of a row of the chunk
+  typename V::Raw* slot = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;
+  float2* part = reinterpret_cast<float2*>(norm_smem + (size_t)sh.slots * sh.threads * V::BYTES);
+  float2* mine = part + sh.R * units;  // the block's (mean, M2) of each group
+  int* cnt_s = reinterpret_cast<int*>(mine + sh.cw / p.cg);
+  int* cnt_block = cnt_s + sh.R;
+  const int col = t.c0 + t.tx * VEC;
+  const T* x = static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + col;
+  if (sh.spec) copy_rows<T, VEC>(x, p.xr, sh, t, 0xffffffffu, slot);
+  const uint32_t on = on_bits(p, sh, t);
+  if (!sh.spec) copy_rows<T, VEC>(x, p.xr, sh, t, on, slot);
+  f32x2 a[NP], bias[NP];
+  if (t.count) {
+    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, a);
+    load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
+  }
+  copies_done();
+
+  // the thread's shares: sums by channel pair, folded into units, then squares around the unit's mean
+  if (t.ty < sh.R && t.tx < t.V) {
+    const int cnt = __popc(on);
+    f32x2 acc[NP], neg[NP];
+#pragma unroll
+    for (int j = 0; j < NP; j++) acc[j] = {0.0f, 0.0f};
+    each_on<T, VEC>(slot, sh.threads, t.count, on, [&](const f32x2 (&v)[NP]) {
+#pragma unroll
+      for (int j = 0; j < NP; j++) acc[j] = add2(acc[j], v[j]);
+    });
+    const float icnt = cnt ? 1.0f / (float)(cnt * U) : 0.0f;
+    float mean[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < U; j++) s += (u * U + j) % 2 ? acc[(u * U + j) / 2].y : acc[(u * U + j) / 2].x;
+      mean[u] = s * icnt;
+    }
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+      neg[j] = {-mean[2 * j / U], VEC > 1 ? -mean[(2 * j + 1) / U] : 0.0f};
+      acc[j] = {0.0f, 0.0f};
+    }
+    each_on<T, VEC>(slot, sh.threads, t.count, on, [&](const f32x2 (&v)[NP]) {
+#pragma unroll
+      for (int j = 0; j < NP; j++) {
+        const f32x2 d = add2(v[j], neg[j]);
+        acc[j] = fma2(d, d, acc[j]);
+      }
+    });
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      float q = 0.0f;
+#pragma unroll
+      for (int j = 0; j < U; j++) q += (u * U + j) % 2 ? acc[(u * U + j) / 2].y : acc[(u * U + j) / 2].x;
+      part[t.ty * units + t.tx * NU + u] = make_float2(mean[u], q);
+    }
+    if (t.tx == 0) cnt_s[t.ty] = cnt;
+  }
+  __syncthreads();
+
+  // merged by group, a warp per group; means are added as distances from one share's mean, which are of the size of
+  // the spread, so that a large mean costs the sums nothing
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
+  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg);
+  int rows_on = 0;
+  for (int i = lane; i < sh.R; i += 32) rows_on += cnt_s[i];
+  for (int o = 16; o > 0; o >>= 1) rows_on += __shfl_xor_sync(0xffffffffu, rows_on, o);
+  const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
+  const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
+  float2* stats = p.stats ? p.stats + (int64_t)t.b * p.G + small_div(t.c0, p.cg) : nullptr;
+  for (int g = warp; g < groups; g += warps) {
+    const float2* gp = part + g * upg;
+    const float ref = gp[0].x;
+    float s = 0.0f, q = 0.0f;
+    for (int y = y0, u = u0; y < sh.R;) {
+      s += (float)(cnt_s[y] * U) * (gp[y * units + u].x - ref);
+      y += dy;
+      u += du;
+      if (u >= upg) u -= upg, y++;
+    }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float delta = s * inv;
+    for (int y = y0, u = u0; y < sh.R;) {
+      const float2 v = gp[y * units + u];
+      const float k = (float)(cnt_s[y] * U), d = v.x - ref - delta;
+      q += k != 0.0f ? v.y + k * d * d : 0.0f;
+      y += dy;
+      u += du;
+      if (u >= upg) u -= upg, y++;
+    }
+    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    if (lane == 0) {
+      float2 st = make_float2(ref + delta, q);
+      if (sh.cs == 1) {
+        st = rows_on ? make_float2(st.x, 1.0f / sqrtf(q * inv + p.eps)) : make_float2(0.0f, 0.0f);
+        if (stats) stats[g] = st;
+      }
+      mine[g] = st;
+    }
+  }
+  const float2* fin = mine;  // (mean, rstd)
+  __syncwarp();
+  if (sh.cs > 1) {
+    if (threadIdx.x == 0) *cnt_block = rows_on;
+    __syncwarp();
+    cluster_sync();
+    for (int g = threadIdx.x; g < groups; g += sh.threads) {
+      const float ref = mine[g].x;
+      float n = 0.0f, s = 0.0f, q = 0.0f;
+      for (int k = 0; k < sh.cs; k++) {
+        const float c = (float)ld_cluster(cnt_block, k);
+        n += c;
+        if (c != 0.0f) s += c * (ld_cluster(mine + g, k).x - ref);
+      }
+      const float delta = n != 0.0f ? s / n : 0.0f;
+      for (int k = 0; k < sh.cs; k++) {
+        const float c = (float)ld_cluster(cnt_block, k) * (float)p.cg;
+        const float2 v = ld_cluster(mine + g, k);
+        const float d = v.x - ref - delta;
+        if (c != 0.0f) q += v.y + c * d * d;
+      }
+      const float2 st = n != 0.0f ? make_float2(ref + delta, 1.0f / sqrtf(q / (n * (float)p.cg) + p.eps))
+                                  : make_float2(0.0f, 0.0f);
+      part[g] = st;
+      if (stats && t.rank == 0) stats[g] = st;
+    }
+    fin = part;
+  }
+  __syncthreads();
+
+  if (t.count) {
+    T* y = static_cast<T*>(p.y) + (int64_t)t.b * p.yb + col;
+    f32x2 neg[NP];
+    float2 st[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) st[u] = fin[small_div(t.tx * VEC + u * U, p.cg)];
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+      const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : lo;
+      neg[j] = {-lo.x, -hi.x};
+      a[j] = mul2(a[j], {lo.y, hi.y});
+    }
+    if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(sh, t, on, slot, y, p.yr, neg, a, bias);
+    else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(sh, t, on, slot, y, p.yr, neg, a, bias);
+    else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(sh, t, on, slot, y, p.yr, neg, a, bias);
+    else apply_rows<T, VEC, KC_ACT_IDENTITY>(sh, t, on, slot, y, p.yr, neg, a, bias);
+  }
+  if (sh.cs > 1) {  // a block's shared memory stays until the others have read it
+    __syncwarp();
+    cluster_sync();
+  }
+}
+
+// Backward: x in one slot of 16 bytes, dy in a second one that gz (float32, so two planes for 2-byte types) replaces
+// when the thread has read it. The channels' sums go over rows first, then over the cluster, then into their groups.
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void back_sums(const ResShape& s, uint32_t on, int count, const typename Vec<T, VEC>::Raw* xs,
+                                          unsigned char* gs, size_t plane, const f32x2 (&neg_mean)[Vec<T, VEC>::NP],
+                                          const f32x2 (&rstd)[Vec<T, VEC>::NP], const f32x2 (&w)[Vec<T, VEC>::NP],
+                                          const f32x2 (&b)[Vec<T, VEC>::NP], f32x2 (&s1)[Vec<T, VEC>::NP],
+                                          f32x2 (&s2)[Vec<T, VEC>::NP]) {
+  using V = Vec<T, VEC>;
+  using G = Vec<float, VEC < 4 ? VEC : 4>;
+#pragma unroll 2
+  for (int i = 0; i < count; i++, on >>= 1, xs += s.threads, gs += (size_t)s.threads * sizeof(typename G::Raw)) {
+    if (!(on & 1)) continue;
+    f32x2 x[V::NP], g[V::NP];
+    V::unpack(*xs, x);
+    V::unpack(*reinterpret_cast<const typename V::Raw*>(gs), g);
+#pragma unroll
+    for (int j = 0; j < V::NP; j++) {
+      const f32x2 xh = mul2(add2(x[j], neg_mean[j]), rstd[j]);
+      const f32x2 z = fma2(xh, w[j], b[j]);
+      if constexpr (ACT == KC_ACT_RELU) {
+        g[j].x = relu_on(z.x, x[j].x, -neg_mean[j].x, rstd[j].x, w[j].x, b[j].x) ? g[j].x : 0.0f;
+        g[j].y = relu_on(z.y, x[j].y, -neg_mean[j].y, rstd[j].y, w[j].y, b[j].y) ? g[j].y : 0.0f;
+      } else {
+        g[j] = mul2(g[j], slope2<ACT>(z));
+      }
+      s1[j] = add2(s1[j], g[j]);
+      s2[j] = fma2(g[j], xh, s2[j]);
+    }
+#pragma unroll
+    for (int k = 0; k < V::NP / G::NP; k++) {
+      f32x2 h[G::NP];
+#pragma unroll
+      for (int j = 0; j < G::NP; j++) h[j] = g[k * G::NP + j];
+      *reinterpret_cast<typename G::Raw*>(gs + k * plane) = G::pack(h);
+    }
+  }
+}
+
+template <typename T, int VEC, int U>
+__global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_constant__ NormParams p,
+                                                                 const __grid_constant__ ResShape sh) {
+  using V = Vec<T, VEC>;
+  using G = Vec<float, VEC < 4 ? VEC : 4>;
+  constexpr int NU = VEC / U, NP = V::NP;
+  const ResIds t = res_ids<VEC>(p, sh);
+  if (t.b >= p.n) return;
+  const size_t plane = (size_t)sh.slots * sh.threads * sizeof(typename G::Raw);
+  typename V::Raw* xs = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;
+  unsigned char* planes = norm_smem + (size_t)sh.slots * sh.threads * V::BYTES;
+  unsigned char* gs = planes + threadIdx.x * sizeof(typename G::Raw);
+  float2* red = reinterpret_cast<float2*>(planes + plane * (V::NP / G::NP));  // [R][cw], then [parts][cw]
+  float2* mine = red + sh.R * sh.cw;  // the block's channel sums
+  float2* coef = mine + sh.cw;        // the groups' (c1, c2)
+  int* cnt_s = reinterpret_cast<int*>(coef + sh.cw / p.cg);
+  int* cnt_block = cnt_s + sh.R;
+  const int col = t.c0 + t.tx * VEC, g0 = small_div(t.c0, p.cg);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + col;
+  const T* dy = static_cast<const T*>(p.dy) + (int64_t)t.b * p.yb + col;
+  static_assert(sizeof(typename V::Raw) <= sizeof(typename G::Raw), "dy waits in the first plane of gz");
+
+  const uint32_t on = on_bits(p, sh, t);
+  copy_rows<T, VEC>(x, p.xr, sh, t, on, xs);
+  {
+    const T* src = dy + t.first * p.yr;
+    unsigned char* dst = gs;
+    uint32_t which = on;
+#pragma unroll 4
+    for (int i = 0; i < t.count; i++, which >>= 1, src += p.yr * sh.R, dst += (size_t)sh.threads * sizeof(typename G::Raw))
+      if (which & 1) V::copy_in(reinterpret_cast<typename V::Raw*>(dst), src);
+  }
+  f32x2 w[NP], neg[NP], rstd[NP], s1[NP], s2[NP];
+#pragma unroll
+  for (int j = 0; j < NP; j++) s1[j] = s2[j] = {0.0f, 0.0f};
+  float2 st[NU];
+  if (t.count) {
+    f32x2 bias[NP];
+    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, w);
+    load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
+    if (VEC == 1) w[0].y = 0.0f;
+    const float2* stats = p.stats + (int64_t)t.b * p.G + g0;
+#pragma unroll
+    for (int u = 0; u < NU; u++) st[u] = stats[small_div(t.tx * VEC + u * U, p.cg)];
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+      const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : make_float2(0.0f, 0.0f);
+      neg[j] = {-lo.x, -hi.x};
+      rstd[j] = {lo.y, hi.y};
+    }
+    copies_done();
+    if (p.act == KC_ACT_MISH) back_sums<T, VEC, KC_ACT_MISH>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
+    else if (p.act == KC_ACT_SILU) back_sums<T, VEC, KC_ACT_SILU>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
+    else if (p.act == KC_ACT_RELU) back_sums<T, VEC, KC_ACT_RELU>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
+    else back_sums<T, VEC, KC_ACT_IDENTITY>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
+  }
+  if (t.ty < sh.R && t.tx < t.V) {
+    float2* o = red + t.ty * sh.cw + t.tx * VEC;
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+      o[2 * j] = make_float2(s1[j].x, s2[j].x);
+      if (VEC > 1) o[2 * j + 1] = make_float2(s1[j].y, s2[j].y);
+    }
+    if (t.tx == 0) cnt_s[t.ty] = __popc(on);
+  }
+  __syncthreads();
+
+  // channel sums: rows ty of `parts` threads per channel, then those
+  const int cw = t.V * VEC, warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
+  const int parts = max(1, small_div(sh.threads, sh.cw));
+  const int part = parts > 1 ? small_div(threadIdx.x, sh.cw) : 0;
+  for (int c = threadIdx.x - part * sh.cw; part < parts && c < cw; c += parts > 1 ? sh.cw : sh.threads) {
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int y = part; y < sh.R; y += parts) {
+      const float2 v = red[y * sh.cw + c];
+      s.x += v.x;
+      s.y += v.y;
+    }
+    red[part * sh.cw + c] = s;  // row `part` of this column is this thread's alone
+  }
+  int rows_on = 0;
+  for (int i = lane; i < sh.R; i += 32) rows_on += cnt_s[i];
+  for (int o = 16; o > 0; o >>= 1) rows_on += __shfl_xor_sync(0xffffffffu, rows_on, o);
+  if (threadIdx.x == 0) *cnt_block = rows_on;
+  __syncthreads();
+  const int used = min(parts, sh.R);
+  for (int c = threadIdx.x; c < cw; c += sh.threads) {
+    float2 s = red[c];
+    for (int k = 1; k < used; k++) {
+      s.x += red[k * sh.cw + c].x;
+      s.y += red[k * sh.cw + c].y;
+    }
+    mine[c] = s;
+  }
+  float2* total = mine;
+  if (sh.cs > 1) {
+    __syncwarp();
+    cluster_sync();
+    total = red;
+    rows_on = 0;
+    for (int k = 0; k < sh.cs; k++) rows_on += ld_cluster(cnt_block, k);
+    for (int c = threadIdx.x; c < cw; c += sh.threads) {
+      float2 s = ld_cluster(mine + c, 0);
+      for (int k = 1; k < sh.cs; k++) {
+        const float2 v = ld_cluster(mine + c, k);
+        s.x += v.x;
+        s.y += v.y;
+      }
+      total[c] = s;
+    }
+  }
+  __syncthreads();
+  if (p.sums && t.rank == 0)
+    for (int c = threadIdx.x; c < cw; c += sh.threads) p.sums[(int64_t)t.b * p.C + t.c0 + c] = total[c];
+  const int groups = small_div(cw, p.cg);
+  const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
+  for (int g = warp; g < groups; g += warps) {
+    float c1 = 0.0f, c2 = 0.0f;
+    for (int i = lane; i < p.cg; i += 32) {
+      const float wc = p.weight ? __ldg(p.weight + t.c0 + g * p.cg + i) : 1.0f;
+      const float2 s = total[g * p.cg + i];
+      c1 += wc * s.x;
+      c2 += wc * s.y;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      c1 += __shfl_xor_sync(0xffffffffu, c1, o);
+      c2 += __shfl_xor_sync(0xffffffffu, c2, o);
+    }
+    if (lane == 0) coef[g] = make_float2(c1 * inv, c2 * inv);
+  }
+  __syncthreads();
+
+  if (t.count) {
+    T* dx = static_cast<T*>(p.y) + (int64_t)t.b * p.xb + col + t.first * p.xr;
+    f32x2 k1[NP], k2[NP];  // dx = gz (rstd w) - rstd c1 - xh (rstd c2)
+    float2 co[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) co[u] = coef[small_div(t.tx * VEC + u * U, p.cg)];
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+      const float2 lo = co[2 * j / U], hi = VEC > 1 ? co[(2 * j + 1) / U] : lo;
+      w[j] = mul2(w[j], rstd[j]);
+      k1[j] = mul2({-lo.x, -hi.x}, rstd[j]);
+      k2[j] = mul2({-lo.y, -hi.y}, rstd[j]);
+    }
+    uint32_t which = on;
+#pragma unroll 2
+    for (int i = 0; i < t.count; i++, which >>= 1, dx += p.xr * sh.R, xs += sh.threads,
+             gs += (size_t)sh.threads * sizeof(typename G::Raw)) {
+      f32x2 o[NP] = {};
+      if (which & 1) {
+        V::unpack(*xs, o);
+#pragma unroll
+        for (int k = 0; k < V::NP / G::NP; k++) {
+          f32x2 g[G::NP];
+          G::unpack(*reinterpret_cast<const typename G::Raw*>(gs + k * plane), g);
+#pragma unroll
+          for (int j = 0; j < G::NP; j++) {
+            const int c = k * G::NP + j;
+            const f32x2 xh = mul2(add2(o[c], neg[c]), rstd[c]);
+            o[c] = fma2(g[j], w[c], fma2(xh, k2[c], k1[c]));
+          }
+        }
+      }
+      *reinterpret_cast<typename V::Raw*>(dx) = V::pack(o);
+    }
+  }
+  if (sh.cs > 1) {
+    __syncwarp();
+    cluster_sync();
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -468,6 +1096,59 @@ void split_shape(const kc_group_norm_desc& d, int& tiles, int& tile_rows) {
   tiles = (d.points + tile_rows - 1) / std::max(1, tile_rows);
 }
 
+// ---- resident path ----
+int lcm_of(int a, int b) {
+  int x = a, y = b;
+  while (y) {
+    const int r = x % y;
+    x = y;
+    y = r;
+  }
+  return (int)std::min<int64_t>((int64_t)a / x * b, 1 << 30);
+}
+
+// Shared memory of a block.
+size_t resident_smem(const ResShape& s, int vec, int unit, int es, int cg, bool backward) {
+  const size_t slots = (size_t)s.slots * s.threads, groups = s.cw / cg, ints = (s.R + 1) * sizeof(int);
+  if (!backward) return slots * vec * es + ((size_t)s.R * (s.cw / unit) + groups) * sizeof(float2) + ints;
+  return slots * vec * (es + 4) + ((size_t)(s.R + 1) * s.cw + groups) * sizeof(float2) + ints;
+}
+
+// Channels of a vector that are sure to lie in one group.
+int unit_of(int vec, int cg) { return vec >= 4 && cg % vec == 0 ? vec : vec >= 4 && cg % 4 == 0 ? 4 : 1; }
+
+// The chunk, cluster and block of a resident launch; false where a board's group does not fit 8 blocks.
+bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShape& s) {
+  const int es = dtype_bytes(d.dtype), cg = d.channels / d.groups, unit = unit_of(vec, cg);
+  const int base = lcm_of(cg, vec);
+  if (d.channels > 1 << 20 || base > d.channels || base / vec > 512) return false;  // small_div's range
+  // whole 64-byte pieces of a row
+  int k = 1;
+  while (base * k * es < 64 && base * k < d.channels) k++;
+  s.cw = std::min(d.channels, base * k);
+  if (s.cw / vec > 512) return false;
+  const int64_t chunks = (d.channels + s.cw - 1) / s.cw;
+  auto fits = [&](int threads, int cs, int most) {
+    s.threads = threads;
+    s.cs = cs;
+    if (s.cw / vec > threads) return false;
+    s.R = threads / (s.cw / vec);
+    s.rows = (d.points + cs - 1) / cs;
+    s.slots = (s.rows + s.R - 1) / s.R;
+    return s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
+  };
+  bool ok = false;
+  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 18);
+  for (int cs = 2; cs <= 8 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots);
+  if (!ok) ok = fits(512, 8, kMaxSlots);
+  if (!ok) return false;
+  // few boards: spread one over more SMs
+  while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < 148) fits(s.threads, s.cs * 2, kMaxSlots);
+  s.cs_log2 = s.cs == 8 ? 3 : s.cs == 4 ? 2 : s.cs == 2 ? 1 : 0;
+  s.spec = (int64_t)d.n * chunks * s.cs <= 2 * 148;
+  return chunks * s.cs <= 0x7fffffff;
+}
+
 struct Layout {
   size_t part = 0, part_n = 0, coef = 0, sums = 0, total = 0;
 };
@@ -476,18 +1157,26 @@ size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 Layout workspace_layout(const kc_group_norm_desc& d, bool backward) {
   Layout l;
   if (d.n == 0 || d.points == 0) return l;
-  int tiles, tile_rows;
-  split_shape(d, tiles, tile_rows);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += round256(bytes);
     return here;
   };
+  if (backward) l.sums = take((size_t)d.n * d.channels * sizeof(float2));
+  l.total = at;
+  // the split path's, unless the call is resident whatever its tensors' alignment
+  bool resident = true;
+  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2) {
+    ResShape s;
+    if (d.channels % v == 0) resident = resident && resident_shape(d, v, backward, s);
+  }
+  if (resident) return l;
+  int tiles, tile_rows;
+  split_shape(d, tiles, tile_rows);
   l.part = take((size_t)d.n * tiles * d.channels * sizeof(float2));
   l.part_n = take((size_t)d.n * tiles * sizeof(int));
   l.coef = take((size_t)d.n * d.groups * sizeof(float2));
-  if (backward) l.sums = take((size_t)d.n * d.channels * sizeof(float2));
   l.total = at;
   return l;
 }
@@ -531,18 +1220,60 @@ void split_backward(const NormParams& p, cudaStream_t st) {
   KC_CUDA(cudaGetLastError());
 }
 
+template <auto kernel>
+void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed[2];  // devices on which this kernel may take more than 48 KB
+  int dev = 0;
+  KC_CUDA(cudaGetDevice(&dev));
+  if (dev >= 128) bad("device index above 127");
+  if (!(allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1)) {
+    KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.C + s.cw - 1) / s.cw * s.cs), (unsigned)std::min(p.n, 65535),
+                     (unsigned)((p.n + 65534) / 65535));
+  cfg.blockDim = dim3((unsigned)s.threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)s.cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s.cs > 1 ? 1 : 0;
+  KC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, s));
+}
+
+template <typename T, int VEC, int U>
+void run_resident(const NormParams& p, const ResShape& s, bool backward, cudaStream_t st) {
+  const size_t smem = resident_smem(s, VEC, U, sizeof(T), p.cg, backward);
+  if (backward) launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, smem, st);
+  else launch_resident<norm_resident_kernel<T, VEC, U>>(p, s, smem, st);
+}
+
 template <typename T, int VEC>
-void run_vec(const NormParams& p, bool backward, cudaStream_t st) {
+void run_vec(const kc_group_norm_desc& d, const NormParams& p, bool backward, cudaStream_t st) {
+  ResShape s;
+  if (resident_shape(d, VEC, backward, s)) {
+    s.wvec = aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
+    const int unit = unit_of(VEC, p.cg);
+    if constexpr (VEC == 8)
+      if (unit == 8) return run_resident<T, VEC, 8>(p, s, backward, st);
+    if constexpr (VEC >= 4)
+      if (unit == 4) return run_resident<T, VEC, 4>(p, s, backward, st);
+    return run_resident<T, VEC, 1>(p, s, backward, st);
+  }
   backward ? split_backward<T, VEC>(p, st) : split_forward<T, VEC>(p, st);
 }
 
 template <typename T>
-void run_type(const NormParams& p, int vec, bool backward, cudaStream_t st) {
+void run_type(const kc_group_norm_desc& d, const NormParams& p, int vec, bool backward, cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (vec == 8) return run_vec<T, 8>(p, backward, st);
-  if (vec == 4) return run_vec<T, 4>(p, backward, st);
-  if (vec == 2) return run_vec<T, 2>(p, backward, st);
-  run_vec<T, 1>(p, backward, st);
+    if (vec == 8) return run_vec<T, 8>(d, p, backward, st);
+  if (vec == 4) return run_vec<T, 4>(d, p, backward, st);
+  if (vec == 2) return run_vec<T, 2>(d, p, backward, st);
+  run_vec<T, 1>(d, p, backward, st);
 }
 
 void run(const kc_group_norm_desc& d, NormParams p, int vec, bool backward, void* workspace, cudaStream_t st) {
@@ -565,9 +1296,9 @@ void run(const kc_group_norm_desc& d, NormParams p, int vec, bool backward, void
   p.part_n = reinterpret_cast<int*>(ws + l.part_n);
   p.coef = reinterpret_cast<float2*>(ws + l.coef);
   p.sums = reinterpret_cast<float2*>(ws + l.sums);
-  if (d.dtype == KC_PRECISION_F32) run_type<float>(p, vec, backward, st);
-  else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, vec, backward, st);
-  else run_type<__nv_bfloat16>(p, vec, backward, st);
+  if (d.dtype == KC_PRECISION_F32) run_type<float>(d, p, vec, backward, st);
+  else if (d.dtype == KC_PRECISION_F16) run_type<__half>(d, p, vec, backward, st);
+  else run_type<__nv_bfloat16>(d, p, vec, backward, st);
 }
 
 void check_tensors(const kc_group_norm_desc& d, std::initializer_list<Rows> rows, const float* mask,
