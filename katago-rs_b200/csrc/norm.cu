@@ -109,12 +109,13 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 // ---------------------------------------------------------------------------------------------------------------
 // The resident path: a chunk of whole groups (V column vectors of VEC channels) of one board is read once and stays
 // in the shared memory of a block, or of a cluster of blocks that share the board's points, until it is written. A
-// thread owns `slots` vectors of one column vector: rows ty, ty + R, ... of its block's points, R = threads / V; it
-// copies them in itself (cp.async), so that no barrier stands between the copy and the statistics.
+// thread owns rows ty, ty + R, ... of its block's points at one column vector, R = threads / V; it copies those that
+// are on into its own run of `slots` (an odd number of vectors, so that 16-byte accesses of neighbouring threads hit
+// different banks) itself (cp.async), so that no barrier stands between the copy and the statistics.
 // U neighbouring channels of a vector lie in one group (VEC, 4 or 1 of them), so that a thread's statistics are
 // VEC / U triples of (count, mean, sum of squares around it).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kMaxSlots = 32;  // a thread's rows are bits of one word
+constexpr int kMaxSlots = 31;  // a thread's rows are bits of one word, and their number is odd
 
 struct ResShape {
   int cw;      // channels of a chunk (the last one of a row may have fewer)
@@ -122,8 +123,8 @@ struct ResShape {
   int rows;    // points per block
   int threads;
   int R;       // rows at once
-  int slots;
-  int spec;    // copies x before the mask is known (few blocks: latency counts, not bytes)
+  int slots;   // vectors a thread has room for
+  uint32_t vdiv;  // 2^20 / V + 1: (t * vdiv) >> 20 = t / V for t, V <= 512
   int wvec;    // weight and bias may be read as 16-byte vectors
 };
 
@@ -221,12 +222,12 @@ __device__ __forceinline__ f32x2 act2(f32x2 z) {
     const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
     const f32x2 d = add2(n, {2.0f, 2.0f});
     const float r = rcp(d.x * d.y);
-    return mul2(z, mul2(n, mul2({d.y, d.x}, {r, r})));
+    return mul2(z, mul2(n, {d.y * r, d.x * r}));
   } else if constexpr (ACT == KC_ACT_SILU) {
     const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
     const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
     const float r = rcp(d.x * d.y);
-    return mul2(z, mul2({d.y, d.x}, {r, r}));
+    return mul2(z, {d.y * r, d.x * r});
   } else {
     return z;
   }
@@ -243,7 +244,7 @@ __device__ __forceinline__ f32x2 slope2(f32x2 z) {
     const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
     const f32x2 d = add2(n, {2.0f, 2.0f});
     const float r = rcp(d.x * d.y);
-    const f32x2 rd = mul2({d.y, d.x}, {r, r});
+    const f32x2 rd = {d.y * r, d.x * r};
     const f32x2 er = mul2(e, rd);                                 // e / d
     const f32x2 k = mul2({4.0f, 4.0f}, mul2(er, add2(er, rd)));   // 4 e (e + 1) / d^2
     return fma2(z, k, mul2(n, rd));
@@ -251,7 +252,7 @@ __device__ __forceinline__ f32x2 slope2(f32x2 z) {
     const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
     const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
     const float r = rcp(d.x * d.y);
-    const f32x2 s = mul2({d.y, d.x}, {r, r});
+    const f32x2 s = {d.y * r, d.x * r};
     const f32x2 u = fma2({-s.x, -s.y}, z, z);                     // z (1 - s)
     return fma2(s, u, s);
   } else {
@@ -259,12 +260,16 @@ __device__ __forceinline__ f32x2 slope2(f32x2 z) {
   }
 }
 
-// a / b of small non-negative integers (a < 2^20): the quotient's fraction is at least 1 / (2 b) off a border.
+// a / b of non-negative integers, a < 2^19: (a + 1/2) / b is at least 1 / (2 b) from a whole number, the fast divide
+// off by at most 2^-21 of it.
 __device__ __forceinline__ int small_div(int a, int b) { return (int)(((float)a + 0.5f) / (float)b); }
+
+__host__ __device__ __forceinline__ size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 struct ResIds {
   int b, rank, c0, tx, ty, V;
-  int first, count;  // the thread's first point and how many (first + i R)
+  int r0, r1;  // the block's points; the thread's are r0 + ty + i R
+  bool here;   // the thread has a column vector and rows
 };
 
 template <int VEC>
@@ -275,47 +280,80 @@ __device__ __forceinline__ ResIds res_ids(const NormParams& p, const ResShape& s
   t.c0 = (blockIdx.x >> s.cs_log2) * s.cw;
   const int vfull = s.cw / VEC;
   t.V = min(s.cw, p.C - t.c0) / VEC;
-  t.ty = small_div(threadIdx.x, vfull);
+  t.ty = (int)((threadIdx.x * s.vdiv) >> 20);
   t.tx = threadIdx.x - t.ty * vfull;
-  const int r0 = t.rank * s.rows, r1 = min(p.points, r0 + s.rows);
-  t.first = r0 + t.ty;
-  t.count = t.ty < s.R && t.tx < t.V && t.first < r1 ? small_div(r1 - t.first + s.R - 1, s.R) : 0;
+  t.r0 = t.rank * s.rows;
+  t.r1 = min(p.points, t.r0 + s.rows);
+  t.here = t.ty < s.R && t.tx < t.V;
   return t;
 }
 
-__device__ __forceinline__ uint32_t low_bits(int k) { return k >= 32 ? 0xffffffffu : (1u << k) - 1; }
-
-// Which of the thread's rows are on, as bits.
-__device__ __forceinline__ uint32_t on_bits(const NormParams& p, const ResShape& s, const ResIds& t) {
-  if (!p.mask) return low_bits(t.count);
-  const float* m = p.mask + (int64_t)t.b * p.mb + t.first;
-  uint32_t on = 0;
-#pragma unroll 4
-  for (int i = 0; i < t.count; i++, m += s.R)
-    if (__ldg(m) != 0.0f) on |= 1u << i;
-  return on;
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void copy_rows(const T* x, int64_t stride, const ResShape& s, const ResIds& t, uint32_t which,
-                                          typename Vec<T, VEC>::Raw* slot) {
-  x += t.first * stride;
-  stride *= s.R;
-#pragma unroll 4
-  for (int i = 0; i < t.count; i++, which >>= 1, x += stride, slot += s.threads)
-    if (which & 1) Vec<T, VEC>::copy_in(slot, x);
-}
-
-// f(vector) of the rows that are on.
-template <typename T, int VEC, typename F>
-__device__ __forceinline__ void each_on(const typename Vec<T, VEC>::Raw* slot, int threads, int count, uint32_t on, F&& f) {
-#pragma unroll 4
-  for (int i = 0; i < count; i++, on >>= 1, slot += threads)
-    if (on & 1) {
-      f32x2 v[Vec<T, VEC>::NP];
-      Vec<T, VEC>::unpack(*slot, v);
-      f(v);
+// on[y]: which points of row lane y are on, valid[y]: which there are; bit i is point r0 + y + i R. A warp per row
+// lane, a lane per bit.
+__device__ __forceinline__ void on_bits(const NormParams& p, const ResShape& s, const ResIds& t, uint32_t* on) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = s.threads / 32;
+  const float* m = p.mask + (int64_t)t.b * p.mb;
+  constexpr int N = 4;  // loads in flight
+  for (int y0 = warp; y0 < s.R; y0 += N * warps) {
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const int y = y0 + k * warps, r = t.r0 + y + lane * s.R;
+      v[k] = y < s.R && r < t.r1 ? (p.mask ? __ldg(m + r) : 1.0f) : 0.0f;
     }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const uint32_t w = __ballot_sync(0xffffffffu, v[k] != 0.0f);
+      if (lane == 0 && y0 + k * warps < s.R) on[y0 + k * warps] = w;
+    }
+  }
+}
+
+// The bits of the points that there are in a row lane.
+__device__ __forceinline__ uint32_t all_bits(const ResShape& s, const ResIds& t) {
+  const int left = t.r1 - t.r0 - t.ty;
+  const int k = t.here && left > 0 ? small_div(left + s.R - 1, s.R) : 0;
+  return k >= 32 ? 0xffffffffu : (1u << k) - 1;
+}
+
+// Rows of a tensor as the thread meets them: its i-th point is i * step bytes behind its first one (the host sees to
+// it that step fits 32 bits: one wide multiply-add an address).
+template <typename P>
+__device__ __forceinline__ P* nth_row(P* first, int i, uint32_t step) {
+  using B = typename std::conditional<std::is_const<P>::value, const char, char>::type;
+  return reinterpret_cast<P*>(reinterpret_cast<B*>(first) + (uint64_t)(uint32_t)i * step);
+}
+
+// The rows that are on into consecutive slots.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_rows(const T* x, uint32_t step, uint32_t on, void* slots, int slot_bytes) {
+  char* slot = static_cast<char*>(slots);
+  while (on) {
+    const int i = __ffs(on) - 1;
+    on &= on - 1;
+    Vec<T, VEC>::copy_in(reinterpret_cast<typename Vec<T, VEC>::Raw*>(slot), nth_row(x, i, step));
+    slot += slot_bytes;
+  }
+}
+
+// f(i) of the rows that are on, N of them side by side (independent work hides the latency of a vector's chain).
+template <int N, typename F>
+__device__ __forceinline__ void each_on(uint32_t on, F&& f) {
+  int left = __popc(on);
+  for (; left >= N; left -= N) {
+    int i[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      i[k] = __ffs(on) - 1;
+      on &= on - 1;
+    }
+    f(i);
+  }
+  for (; N > 1 && left > 0; left--) {
+    const int i[1] = {__ffs(on) - 1};
+    on &= on - 1;
+    f(i);
+  }
 }
 
 template <int VEC>
@@ -339,23 +377,31 @@ __device__ __forceinline__ void load_params(const float* w, float other, bool ve
 }
 
 template <typename T, int VEC, int ACT>
-__device__ __forceinline__ void apply_rows(const ResShape& s, const ResIds& t, uint32_t on,
-                                           const typename Vec<T, VEC>::Raw* slot, T* y, int64_t stride,
+__device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VEC>::Raw* slot, T* y, uint32_t step,
                                            const f32x2 (&neg_mean)[Vec<T, VEC>::NP], const f32x2 (&a)[Vec<T, VEC>::NP],
                                            const f32x2 (&b)[Vec<T, VEC>::NP]) {
   using V = Vec<T, VEC>;
-  y += t.first * stride;
-  stride *= s.R;
-#pragma unroll 2
-  for (int i = 0; i < t.count; i++, on >>= 1, y += stride, slot += s.threads) {
-    f32x2 v[V::NP] = {};
-    if (on & 1) {
-      V::unpack(*slot, v);
+  each_on<2>(on, [&](const auto& i) {
+    constexpr int N = sizeof(i) / sizeof(int);
+    f32x2 v[N][V::NP];
 #pragma unroll
-      for (int j = 0; j < V::NP; j++) v[j] = act2<ACT>(fma2(add2(v[j], neg_mean[j]), a[j], b[j]));
-    }
-    *reinterpret_cast<typename V::Raw*>(y) = V::pack(v);
-  }
+    for (int k = 0; k < N; k++) V::unpack(slot[k], v[k]);
+    slot += N;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+      for (int j = 0; j < V::NP; j++) v[k][j] = act2<ACT>(fma2(add2(v[k][j], neg_mean[j]), a[j], b[j]));
+#pragma unroll
+    for (int k = 0; k < N; k++) *reinterpret_cast<typename V::Raw*>(nth_row(y, i[k], step)) = V::pack(v[k]);
+  });
+}
+
+// 0 in the rows of the bits.
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_rows(uint32_t which, T* y, uint32_t step) {
+  using V = Vec<T, VEC>;
+  const f32x2 v[V::NP] = {};
+  each_on<1>(which, [&](const auto& i) { *reinterpret_cast<typename V::Raw*>(nth_row(y, i[0], step)) = V::pack(v); });
 }
 
 extern __shared__ __align__(16) unsigned char norm_smem[];
@@ -368,62 +414,67 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   const ResIds t = res_ids<VEC>(p, sh);
   if (t.b >= p.n) return;
   const int units = sh.cw / U;  // of a row of the chunk
-  typename V::Raw* slot = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;
-  float2* part = reinterpret_cast<float2*>(norm_smem + (size_t)sh.slots * sh.threads * V::BYTES);
+  const typename V::Raw* slot = reinterpret_cast<const typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
+  float2* part = reinterpret_cast<float2*>(norm_smem + round16((size_t)sh.slots * sh.threads * V::BYTES));
   float2* mine = part + sh.R * units;  // the block's (mean, M2) of each group
-  int* cnt_s = reinterpret_cast<int*>(mine + sh.cw / p.cg);
-  int* cnt_block = cnt_s + sh.R;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + sh.cw / p.cg);
+  int* cnt_block = reinterpret_cast<int*>(bits + sh.R);
   const int col = t.c0 + t.tx * VEC;
-  const T* x = static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + col;
-  if (sh.spec) copy_rows<T, VEC>(x, p.xr, sh, t, 0xffffffffu, slot);
-  const uint32_t on = on_bits(p, sh, t);
-  if (!sh.spec) copy_rows<T, VEC>(x, p.xr, sh, t, on, slot);
+  on_bits(p, sh, t, bits);
+  __syncthreads();
+  const uint32_t on = t.here ? bits[t.ty] : 0;
+  copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + (int64_t)(t.r0 + t.ty) * p.xr + col,
+                    (uint32_t)(sh.R * p.xr * sizeof(T)), on, const_cast<typename V::Raw*>(slot), V::BYTES);
   f32x2 a[NP], bias[NP];
-  if (t.count) {
+  if (t.here) {
     load_params<VEC>(p.weight, 1.0f, sh.wvec, col, a);
     load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
   }
   copies_done();
 
-  // the thread's shares: sums by channel pair, folded into units, then squares around the unit's mean
-  if (t.ty < sh.R && t.tx < t.V) {
+  // the thread's shares, in one pass around a value of its first row: the squares around the mean are the squares
+  // around that value less its distance's, at most as many times larger as the share has values, since it is one of
+  // them
+  if (t.here) {
     const int cnt = __popc(on);
-    f32x2 acc[NP], neg[NP];
+    f32x2 neg[NP], sum[NP], sq[NP];
+    float ref[NU];
+    {
+      f32x2 v[NP] = {};
+      if (on) V::unpack(slot[0], v);
 #pragma unroll
-    for (int j = 0; j < NP; j++) acc[j] = {0.0f, 0.0f};
-    each_on<T, VEC>(slot, sh.threads, t.count, on, [&](const f32x2 (&v)[NP]) {
-#pragma unroll
-      for (int j = 0; j < NP; j++) acc[j] = add2(acc[j], v[j]);
-    });
-    const float icnt = cnt ? 1.0f / (float)(cnt * U) : 0.0f;
-    float mean[NU];
-#pragma unroll
-    for (int u = 0; u < NU; u++) {
-      float s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < U; j++) s += (u * U + j) % 2 ? acc[(u * U + j) / 2].y : acc[(u * U + j) / 2].x;
-      mean[u] = s * icnt;
+      for (int u = 0; u < NU; u++) ref[u] = u * U % 2 ? v[u * U / 2].y : v[u * U / 2].x;
     }
 #pragma unroll
     for (int j = 0; j < NP; j++) {
-      neg[j] = {-mean[2 * j / U], VEC > 1 ? -mean[(2 * j + 1) / U] : 0.0f};
-      acc[j] = {0.0f, 0.0f};
+      neg[j] = {-ref[2 * j / U], VEC > 1 ? -ref[(2 * j + 1) / U] : 0.0f};
+      sum[j] = sq[j] = {0.0f, 0.0f};
     }
-    each_on<T, VEC>(slot, sh.threads, t.count, on, [&](const f32x2 (&v)[NP]) {
+#pragma unroll 4
+    for (int k = 0; k < cnt; k++) {
+      f32x2 v[NP];
+      V::unpack(slot[k], v);
 #pragma unroll
       for (int j = 0; j < NP; j++) {
         const f32x2 d = add2(v[j], neg[j]);
-        acc[j] = fma2(d, d, acc[j]);
+        sum[j] = add2(sum[j], d);
+        sq[j] = fma2(d, d, sq[j]);
       }
-    });
+    }
+    const float inv_n = cnt ? __fdividef(1.0f / U, (float)cnt) : 0.0f;
+    auto lane_of = [](const f32x2 (&v)[NP], int c) { return c % 2 ? v[c / 2].y : v[c / 2].x; };
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-      float q = 0.0f;
+      float m = lane_of(sum, u * U), q = lane_of(sq, u * U);
 #pragma unroll
-      for (int j = 0; j < U; j++) q += (u * U + j) % 2 ? acc[(u * U + j) / 2].y : acc[(u * U + j) / 2].x;
-      part[t.ty * units + t.tx * NU + u] = make_float2(mean[u], q);
+      for (int j = 1; j < U; j++) {
+        m += lane_of(sum, u * U + j);
+        q += lane_of(sq, u * U + j);
+      }
+      const float d = m * inv_n;
+      q -= m * d;
+      part[t.ty * units + t.tx * NU + u] = make_float2(ref[u] + d, q < 0.0f ? 0.0f : q);
     }
-    if (t.tx == 0) cnt_s[t.ty] = cnt;
   }
   __syncthreads();
 
@@ -432,8 +483,8 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
   const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg);
   int rows_on = 0;
-  for (int i = lane; i < sh.R; i += 32) rows_on += cnt_s[i];
-  for (int o = 16; o > 0; o >>= 1) rows_on += __shfl_xor_sync(0xffffffffu, rows_on, o);
+  for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits[i]);
+  rows_on = __reduce_add_sync(0xffffffffu, rows_on);
   const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
   const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   float2* stats = p.stats ? p.stats + (int64_t)t.b * p.G + small_div(t.c0, p.cg) : nullptr;
@@ -442,7 +493,7 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
     const float ref = gp[0].x;
     float s = 0.0f, q = 0.0f;
     for (int y = y0, u = u0; y < sh.R;) {
-      s += (float)(cnt_s[y] * U) * (gp[y * units + u].x - ref);
+      s += (float)(__popc(bits[y]) * U) * (gp[y * units + u].x - ref);
       y += dy;
       u += du;
       if (u >= upg) u -= upg, y++;
@@ -451,7 +502,7 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
     const float delta = s * inv;
     for (int y = y0, u = u0; y < sh.R;) {
       const float2 v = gp[y * units + u];
-      const float k = (float)(cnt_s[y] * U), d = v.x - ref - delta;
+      const float k = (float)(__popc(bits[y]) * U), d = v.x - ref - delta;
       q += k != 0.0f ? v.y + k * d * d : 0.0f;
       y += dy;
       u += du;
@@ -497,8 +548,8 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   }
   __syncthreads();
 
-  if (t.count) {
-    T* y = static_cast<T*>(p.y) + (int64_t)t.b * p.yb + col;
+  if (t.here) {
+    T* y = static_cast<T*>(p.y) + (int64_t)t.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col;
     f32x2 neg[NP];
     float2 st[NU];
 #pragma unroll
@@ -509,10 +560,12 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
       neg[j] = {-lo.x, -hi.x};
       a[j] = mul2(a[j], {lo.y, hi.y});
     }
-    if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(sh, t, on, slot, y, p.yr, neg, a, bias);
-    else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(sh, t, on, slot, y, p.yr, neg, a, bias);
-    else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(sh, t, on, slot, y, p.yr, neg, a, bias);
-    else apply_rows<T, VEC, KC_ACT_IDENTITY>(sh, t, on, slot, y, p.yr, neg, a, bias);
+    const uint32_t step = (uint32_t)(sh.R * p.yr * sizeof(T));
+    if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(on, slot, y, step, neg, a, bias);
+    else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slot, y, step, neg, a, bias);
+    else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slot, y, step, neg, a, bias);
+    else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slot, y, step, neg, a, bias);
+    zero_rows<T, VEC>(all_bits(sh, t) & ~on, y, step);
   }
   if (sh.cs > 1) {  // a block's shared memory stays until the others have read it
     __syncwarp();
@@ -520,86 +573,124 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   }
 }
 
-// Backward: x in one slot of 16 bytes, dy in a second one that gz (float32, so two planes for 2-byte types) replaces
-// when the thread has read it. The channels' sums go over rows first, then over the cluster, then into their groups.
-template <typename T, int VEC, int ACT>
-__device__ __forceinline__ void back_sums(const ResShape& s, uint32_t on, int count, const typename Vec<T, VEC>::Raw* xs,
-                                          unsigned char* gs, size_t plane, const f32x2 (&neg_mean)[Vec<T, VEC>::NP],
+// Backward: x and dy of the rows that are on in slots of their own; gz (float32, so two planes of 16 bytes for eight
+// 2-byte channels) takes dy's place when the thread has read it. The channels' sums go over rows first, then over the
+// cluster, then into their groups.
+template <typename T, int VEC>
+struct BackSlots {
+  using V = Vec<T, VEC>;
+  using G = Vec<float, VEC < 4 ? VEC : 4>;
+  static constexpr int PLANES = V::NP / G::NP;
+  static_assert(sizeof(typename V::Raw) <= sizeof(typename G::Raw), "dy waits in the first plane of gz");
+  typename V::Raw* x;
+  typename G::Raw* g[PLANES];
+  __device__ __forceinline__ void next(int n) {
+    x += n;
+#pragma unroll
+    for (int h = 0; h < PLANES; h++) g[h] += n;
+  }
+  __device__ __forceinline__ void store_g(int k, const f32x2 (&v)[V::NP]) {
+#pragma unroll
+    for (int h = 0; h < PLANES; h++) {
+      f32x2 o[G::NP];
+#pragma unroll
+      for (int j = 0; j < G::NP; j++) o[j] = v[h * G::NP + j];
+      g[h][k] = G::pack(o);
+    }
+  }
+  __device__ __forceinline__ void load_g(int k, f32x2 (&v)[V::NP]) const {
+#pragma unroll
+    for (int h = 0; h < PLANES; h++) {
+      f32x2 o[G::NP];
+      G::unpack(g[h][k], o);
+#pragma unroll
+      for (int j = 0; j < G::NP; j++) v[h * G::NP + j] = o[j];
+    }
+  }
+};
+
+template <typename T, int VEC, int ACT, int N>
+__device__ __forceinline__ void back_rows(BackSlots<T, VEC>& sl, const f32x2 (&neg_mean)[Vec<T, VEC>::NP],
                                           const f32x2 (&rstd)[Vec<T, VEC>::NP], const f32x2 (&w)[Vec<T, VEC>::NP],
                                           const f32x2 (&b)[Vec<T, VEC>::NP], f32x2 (&s1)[Vec<T, VEC>::NP],
                                           f32x2 (&s2)[Vec<T, VEC>::NP]) {
   using V = Vec<T, VEC>;
-  using G = Vec<float, VEC < 4 ? VEC : 4>;
-#pragma unroll 2
-  for (int i = 0; i < count; i++, on >>= 1, xs += s.threads, gs += (size_t)s.threads * sizeof(typename G::Raw)) {
-    if (!(on & 1)) continue;
-    f32x2 x[V::NP], g[V::NP];
-    V::unpack(*xs, x);
-    V::unpack(*reinterpret_cast<const typename V::Raw*>(gs), g);
+  f32x2 x[N][V::NP], g[N][V::NP];
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    V::unpack(sl.x[k], x[k]);
+    V::unpack(*reinterpret_cast<const typename V::Raw*>(sl.g[0] + k), g[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < N; k++)
 #pragma unroll
     for (int j = 0; j < V::NP; j++) {
-      const f32x2 xh = mul2(add2(x[j], neg_mean[j]), rstd[j]);
+      const f32x2 xh = mul2(add2(x[k][j], neg_mean[j]), rstd[j]);
       const f32x2 z = fma2(xh, w[j], b[j]);
+      f32x2& gz = g[k][j];
       if constexpr (ACT == KC_ACT_RELU) {
-        g[j].x = relu_on(z.x, x[j].x, -neg_mean[j].x, rstd[j].x, w[j].x, b[j].x) ? g[j].x : 0.0f;
-        g[j].y = relu_on(z.y, x[j].y, -neg_mean[j].y, rstd[j].y, w[j].y, b[j].y) ? g[j].y : 0.0f;
+        gz.x = relu_on(z.x, x[k][j].x, -neg_mean[j].x, rstd[j].x, w[j].x, b[j].x) ? gz.x : 0.0f;
+        gz.y = relu_on(z.y, x[k][j].y, -neg_mean[j].y, rstd[j].y, w[j].y, b[j].y) ? gz.y : 0.0f;
       } else {
-        g[j] = mul2(g[j], slope2<ACT>(z));
+        gz = mul2(gz, slope2<ACT>(z));
       }
-      s1[j] = add2(s1[j], g[j]);
-      s2[j] = fma2(g[j], xh, s2[j]);
+      s1[j] = add2(s1[j], gz);
+      s2[j] = fma2(gz, xh, s2[j]);
     }
 #pragma unroll
-    for (int k = 0; k < V::NP / G::NP; k++) {
-      f32x2 h[G::NP];
-#pragma unroll
-      for (int j = 0; j < G::NP; j++) h[j] = g[k * G::NP + j];
-      *reinterpret_cast<typename G::Raw*>(gs + k * plane) = G::pack(h);
-    }
-  }
+  for (int k = 0; k < N; k++) sl.store_g(k, g[k]);
+  sl.next(N);
+}
+
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void back_sums(BackSlots<T, VEC> sl, int cnt, const f32x2 (&neg_mean)[Vec<T, VEC>::NP],
+                                          const f32x2 (&rstd)[Vec<T, VEC>::NP], const f32x2 (&w)[Vec<T, VEC>::NP],
+                                          const f32x2 (&b)[Vec<T, VEC>::NP], f32x2 (&s1)[Vec<T, VEC>::NP],
+                                          f32x2 (&s2)[Vec<T, VEC>::NP]) {
+  for (; cnt >= 2; cnt -= 2) back_rows<T, VEC, ACT, 2>(sl, neg_mean, rstd, w, b, s1, s2);
+  if (cnt) back_rows<T, VEC, ACT, 1>(sl, neg_mean, rstd, w, b, s1, s2);
 }
 
 template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_constant__ NormParams p,
                                                                  const __grid_constant__ ResShape sh) {
   using V = Vec<T, VEC>;
-  using G = Vec<float, VEC < 4 ? VEC : 4>;
+  using S = BackSlots<T, VEC>;
+  using G = typename S::G;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
   if (t.b >= p.n) return;
-  const size_t plane = (size_t)sh.slots * sh.threads * sizeof(typename G::Raw);
-  typename V::Raw* xs = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;
-  unsigned char* planes = norm_smem + (size_t)sh.slots * sh.threads * V::BYTES;
-  unsigned char* gs = planes + threadIdx.x * sizeof(typename G::Raw);
-  float2* red = reinterpret_cast<float2*>(planes + plane * (V::NP / G::NP));  // [R][cw], then [parts][cw]
+  const size_t vectors = (size_t)sh.slots * sh.threads, plane = vectors * sizeof(typename G::Raw);
+  unsigned char* planes = norm_smem + round16(vectors * V::BYTES);
+  S slots;
+  slots.x = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
+#pragma unroll
+  for (int h = 0; h < S::PLANES; h++)
+    slots.g[h] = reinterpret_cast<typename G::Raw*>(planes + h * plane) + threadIdx.x * sh.slots;
+  float2* red = reinterpret_cast<float2*>(planes + S::PLANES * plane);  // [R][cw], then [parts][cw]
   float2* mine = red + sh.R * sh.cw;  // the block's channel sums
   float2* coef = mine + sh.cw;        // the groups' (c1, c2)
-  int* cnt_s = reinterpret_cast<int*>(coef + sh.cw / p.cg);
-  int* cnt_block = cnt_s + sh.R;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(coef + sh.cw / p.cg);
+  int* cnt_block = reinterpret_cast<int*>(bits + sh.R);
   const int col = t.c0 + t.tx * VEC, g0 = small_div(t.c0, p.cg);
-  const T* x = static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + col;
-  const T* dy = static_cast<const T*>(p.dy) + (int64_t)t.b * p.yb + col;
-  static_assert(sizeof(typename V::Raw) <= sizeof(typename G::Raw), "dy waits in the first plane of gz");
+  const int64_t x_at = (int64_t)t.b * p.xb + (int64_t)(t.r0 + t.ty) * p.xr + col;
+  const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
 
-  const uint32_t on = on_bits(p, sh, t);
-  copy_rows<T, VEC>(x, p.xr, sh, t, on, xs);
-  {
-    const T* src = dy + t.first * p.yr;
-    unsigned char* dst = gs;
-    uint32_t which = on;
-#pragma unroll 4
-    for (int i = 0; i < t.count; i++, which >>= 1, src += p.yr * sh.R, dst += (size_t)sh.threads * sizeof(typename G::Raw))
-      if (which & 1) V::copy_in(reinterpret_cast<typename V::Raw*>(dst), src);
-  }
+  on_bits(p, sh, t, bits);
+  __syncthreads();
+  const uint32_t on = t.here ? bits[t.ty] : 0;
+  copy_rows<T, VEC>(static_cast<const T*>(p.x) + x_at, x_step, on, slots.x, V::BYTES);
+  copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)t.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col, y_step, on,
+                    slots.g[0], sizeof(typename G::Raw));
   f32x2 w[NP], neg[NP], rstd[NP], s1[NP], s2[NP];
 #pragma unroll
   for (int j = 0; j < NP; j++) s1[j] = s2[j] = {0.0f, 0.0f};
-  float2 st[NU];
-  if (t.count) {
+  if (t.here) {
     f32x2 bias[NP];
     load_params<VEC>(p.weight, 1.0f, sh.wvec, col, w);
     load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
     if (VEC == 1) w[0].y = 0.0f;
+    float2 st[NU];
     const float2* stats = p.stats + (int64_t)t.b * p.G + g0;
 #pragma unroll
     for (int u = 0; u < NU; u++) st[u] = stats[small_div(t.tx * VEC + u * U, p.cg)];
@@ -610,19 +701,19 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
       rstd[j] = {lo.y, hi.y};
     }
     copies_done();
-    if (p.act == KC_ACT_MISH) back_sums<T, VEC, KC_ACT_MISH>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
-    else if (p.act == KC_ACT_SILU) back_sums<T, VEC, KC_ACT_SILU>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
-    else if (p.act == KC_ACT_RELU) back_sums<T, VEC, KC_ACT_RELU>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
-    else back_sums<T, VEC, KC_ACT_IDENTITY>(sh, on, t.count, xs, gs, plane, neg, rstd, w, bias, s1, s2);
+    const int cnt = __popc(on);
+    if (p.act == KC_ACT_MISH) back_sums<T, VEC, KC_ACT_MISH>(slots, cnt, neg, rstd, w, bias, s1, s2);
+    else if (p.act == KC_ACT_SILU) back_sums<T, VEC, KC_ACT_SILU>(slots, cnt, neg, rstd, w, bias, s1, s2);
+    else if (p.act == KC_ACT_RELU) back_sums<T, VEC, KC_ACT_RELU>(slots, cnt, neg, rstd, w, bias, s1, s2);
+    else back_sums<T, VEC, KC_ACT_IDENTITY>(slots, cnt, neg, rstd, w, bias, s1, s2);
   }
-  if (t.ty < sh.R && t.tx < t.V) {
+  if (t.here) {
     float2* o = red + t.ty * sh.cw + t.tx * VEC;
 #pragma unroll
     for (int j = 0; j < NP; j++) {
       o[2 * j] = make_float2(s1[j].x, s2[j].x);
       if (VEC > 1) o[2 * j + 1] = make_float2(s1[j].y, s2[j].y);
     }
-    if (t.tx == 0) cnt_s[t.ty] = __popc(on);
   }
   __syncthreads();
 
@@ -640,8 +731,8 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
     red[part * sh.cw + c] = s;  // row `part` of this column is this thread's alone
   }
   int rows_on = 0;
-  for (int i = lane; i < sh.R; i += 32) rows_on += cnt_s[i];
-  for (int o = 16; o > 0; o >>= 1) rows_on += __shfl_xor_sync(0xffffffffu, rows_on, o);
+  for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits[i]);
+  rows_on = __reduce_add_sync(0xffffffffu, rows_on);
   if (threadIdx.x == 0) *cnt_block = rows_on;
   __syncthreads();
   const int used = min(parts, sh.R);
@@ -691,8 +782,8 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   }
   __syncthreads();
 
-  if (t.count) {
-    T* dx = static_cast<T*>(p.y) + (int64_t)t.b * p.xb + col + t.first * p.xr;
+  if (t.here) {
+    T* dx = static_cast<T*>(p.y) + x_at;
     f32x2 k1[NP], k2[NP];  // dx = gz (rstd w) - rstd c1 - xh (rstd c2)
     float2 co[NU];
 #pragma unroll
@@ -704,27 +795,26 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
       k1[j] = mul2({-lo.x, -hi.x}, rstd[j]);
       k2[j] = mul2({-lo.y, -hi.y}, rstd[j]);
     }
-    uint32_t which = on;
-#pragma unroll 2
-    for (int i = 0; i < t.count; i++, which >>= 1, dx += p.xr * sh.R, xs += sh.threads,
-             gs += (size_t)sh.threads * sizeof(typename G::Raw)) {
-      f32x2 o[NP] = {};
-      if (which & 1) {
-        V::unpack(*xs, o);
+    each_on<2>(on, [&](const auto& i) {
+      constexpr int N = sizeof(i) / sizeof(int);
+      f32x2 o[N][NP], g[N][NP];
 #pragma unroll
-        for (int k = 0; k < V::NP / G::NP; k++) {
-          f32x2 g[G::NP];
-          G::unpack(*reinterpret_cast<const typename G::Raw*>(gs + k * plane), g);
-#pragma unroll
-          for (int j = 0; j < G::NP; j++) {
-            const int c = k * G::NP + j;
-            const f32x2 xh = mul2(add2(o[c], neg[c]), rstd[c]);
-            o[c] = fma2(g[j], w[c], fma2(xh, k2[c], k1[c]));
-          }
-        }
+      for (int k = 0; k < N; k++) {
+        V::unpack(slots.x[k], o[k]);
+        slots.load_g(k, g[k]);
       }
-      *reinterpret_cast<typename V::Raw*>(dx) = V::pack(o);
-    }
+      slots.next(N);
+#pragma unroll
+      for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+          const f32x2 xh = mul2(add2(o[k][j], neg[j]), rstd[j]);
+          o[k][j] = fma2(g[k][j], w[j], fma2(xh, k2[j], k1[j]));
+        }
+#pragma unroll
+      for (int k = 0; k < N; k++) *reinterpret_cast<typename V::Raw*>(nth_row(dx, i[k], x_step)) = V::pack(o[k]);
+    });
+    zero_rows<T, VEC>(all_bits(sh, t) & ~on, dx, x_step);
   }
   if (sh.cs > 1) {
     __syncwarp();
@@ -1110,8 +1200,8 @@ int lcm_of(int a, int b) {
 // Shared memory of a block.
 size_t resident_smem(const ResShape& s, int vec, int unit, int es, int cg, bool backward) {
   const size_t slots = (size_t)s.slots * s.threads, groups = s.cw / cg, ints = (s.R + 1) * sizeof(int);
-  if (!backward) return slots * vec * es + ((size_t)s.R * (s.cw / unit) + groups) * sizeof(float2) + ints;
-  return slots * vec * (es + 4) + ((size_t)(s.R + 1) * s.cw + groups) * sizeof(float2) + ints;
+  if (!backward) return round16(slots * vec * es) + ((size_t)s.R * (s.cw / unit) + groups) * sizeof(float2) + ints;
+  return round16(slots * vec * es) + slots * vec * 4 + ((size_t)(s.R + 1) * s.cw + groups) * sizeof(float2) + ints;
 }
 
 // Channels of a vector that are sure to lie in one group.
@@ -1121,7 +1211,7 @@ int unit_of(int vec, int cg) { return vec >= 4 && cg % vec == 0 ? vec : vec >= 4
 bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShape& s) {
   const int es = dtype_bytes(d.dtype), cg = d.channels / d.groups, unit = unit_of(vec, cg);
   const int base = lcm_of(cg, vec);
-  if (d.channels > 1 << 20 || base > d.channels || base / vec > 512) return false;  // small_div's range
+  if (d.channels > 1 << 18 || base > d.channels || base / vec > 512) return false;  // small_div's range
   // whole 64-byte pieces of a row
   int k = 1;
   while (base * k * es < 64 && base * k < d.channels) k++;
@@ -1134,18 +1224,19 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
     if (s.cw / vec > threads) return false;
     s.R = threads / (s.cw / vec);
     s.rows = (d.points + cs - 1) / cs;
-    s.slots = (s.rows + s.R - 1) / s.R;
-    return s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
+    s.slots = ((s.rows + s.R - 1) / s.R) | 1;
+    const int64_t step = std::max(d.x_row_stride, d.y_row_stride) * s.R * es;  // nth_row's
+    return step <= 0xffffffffll && s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
   };
   bool ok = false;
-  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 18);
+  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 19);
   for (int cs = 2; cs <= 8 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots);
   if (!ok) ok = fits(512, 8, kMaxSlots);
   if (!ok) return false;
   // few boards: spread one over more SMs
   while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < 148) fits(s.threads, s.cs * 2, kMaxSlots);
+  s.vdiv = (1u << 20) / (uint32_t)(s.cw / vec) + 1;
   s.cs_log2 = s.cs == 8 ? 3 : s.cs == 4 ? 2 : s.cs == 2 ? 1 : 0;
-  s.spec = (int64_t)d.n * chunks * s.cs <= 2 * 148;
   return chunks * s.cs <= 0x7fffffff;
 }
 
