@@ -288,25 +288,33 @@ __device__ __forceinline__ ResIds res_ids(const NormParams& p, const ResShape& s
   return t;
 }
 
-// on[y]: which points of row lane y are on, valid[y]: which there are; bit i is point r0 + y + i R. A warp per row
-// lane, a lane per bit.
+// on[y]: which points of row lane y are on, bit i being point r0 + y + i R. Ends with a barrier.
 __device__ __forceinline__ void on_bits(const NormParams& p, const ResShape& s, const ResIds& t, uint32_t* on) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = s.threads / 32;
-  const float* m = p.mask + (int64_t)t.b * p.mb;
+  const int rows = t.r1 - t.r0;
+  if (!p.mask) {
+    for (int y = threadIdx.x; y < s.R; y += s.threads) {
+      const int k = y < rows ? small_div(rows - y + s.R - 1, s.R) : 0;
+      on[y] = k >= 32 ? 0xffffffffu : (1u << k) - 1;
+    }
+    __syncthreads();
+    return;
+  }
+  const float* m = p.mask + (int64_t)t.b * p.mb + t.r0;
+  for (int y = threadIdx.x; y < s.R; y += s.threads) on[y] = 0;
   constexpr int N = 4;  // loads in flight
-  for (int y0 = warp; y0 < s.R; y0 += N * warps) {
+  for (int r0 = threadIdx.x; r0 < rows + (int)threadIdx.x; r0 += N * s.threads) {
     float v[N];
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      const int y = y0 + k * warps, r = t.r0 + y + lane * s.R;
-      v[k] = y < s.R && r < t.r1 ? (p.mask ? __ldg(m + r) : 1.0f) : 0.0f;
-    }
+    for (int k = 0; k < N; k++) v[k] = r0 + k * s.threads < rows ? __ldg(m + r0 + k * s.threads) : 0.0f;
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      const uint32_t w = __ballot_sync(0xffffffffu, v[k] != 0.0f);
-      if (lane == 0 && y0 + k * warps < s.R) on[y0 + k * warps] = w;
-    }
+    for (int k = 0; k < N; k++)
+      if (v[k] != 0.0f) {
+        const int r = r0 + k * s.threads, i = small_div(r, s.R);
+        atomicOr(on + r - i * s.R, 1u << i);
+      }
   }
+  __syncthreads();
 }
 
 // The bits of the points that there are in a row lane.
@@ -322,18 +330,6 @@ template <typename P>
 __device__ __forceinline__ P* nth_row(P* first, int i, uint32_t step) {
   using B = typename std::conditional<std::is_const<P>::value, const char, char>::type;
   return reinterpret_cast<P*>(reinterpret_cast<B*>(first) + (uint64_t)(uint32_t)i * step);
-}
-
-// The rows that are on into consecutive slots.
-template <typename T, int VEC>
-__device__ __forceinline__ void copy_rows(const T* x, uint32_t step, uint32_t on, void* slots, int slot_bytes) {
-  char* slot = static_cast<char*>(slots);
-  while (on) {
-    const int i = __ffs(on) - 1;
-    on &= on - 1;
-    Vec<T, VEC>::copy_in(reinterpret_cast<typename Vec<T, VEC>::Raw*>(slot), nth_row(x, i, step));
-    slot += slot_bytes;
-  }
 }
 
 // f(i) of the rows that are on, N of them side by side (independent work hides the latency of a vector's chain).
@@ -354,6 +350,17 @@ __device__ __forceinline__ void each_on(uint32_t on, F&& f) {
     on &= on - 1;
     f(i);
   }
+}
+
+// The rows that are on into consecutive slots.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_rows(const T* x, uint32_t step, uint32_t on, void* slots, int slot_bytes) {
+  char* slot = static_cast<char*>(slots);
+  each_on<4>(on, [&](const auto& i) {
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(i) / sizeof(int)); k++, slot += slot_bytes)
+      Vec<T, VEC>::copy_in(reinterpret_cast<typename Vec<T, VEC>::Raw*>(slot), nth_row(x, i[k], step));
+  });
 }
 
 template <int VEC>
@@ -406,6 +413,17 @@ __device__ __forceinline__ void zero_rows(uint32_t which, T* y, uint32_t step) {
 
 extern __shared__ __align__(16) unsigned char norm_smem[];
 
+// A group's (mean, rstd), also into the statistics the caller wants. 1 / sqrt by the fast function (2^-22) and one
+// Newton step; a variance of 0 with eps 0 gives infinity.
+__device__ __forceinline__ float2 final_stats(float mean, float var, bool any, float eps, float2* stats, int g) {
+  const float v = (var < 0.0f ? 0.0f : var) + eps;
+  float r = rsqrtf(v);
+  if (v > 0.0f && v < 1e38f) r = r * (1.5f - 0.5f * v * r * r);
+  const float2 st = any ? make_float2(mean, r) : make_float2(0.0f, 0.0f);
+  if (stats) stats[g] = st;
+  return st;
+}
+
 template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constant__ NormParams p,
                                                             const __grid_constant__ ResShape sh) {
@@ -421,7 +439,6 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   int* cnt_block = reinterpret_cast<int*>(bits + sh.R);
   const int col = t.c0 + t.tx * VEC;
   on_bits(p, sh, t, bits);
-  __syncthreads();
   const uint32_t on = t.here ? bits[t.ty] : 0;
   copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + (int64_t)(t.r0 + t.ty) * p.xr + col,
                     (uint32_t)(sh.R * p.xr * sizeof(T)), on, const_cast<typename V::Raw*>(slot), V::BYTES);
@@ -478,44 +495,43 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   }
   __syncthreads();
 
-  // merged by group, a warp per group; means are added as distances from one share's mean, which are of the size of
-  // the spread, so that a large mean costs the sums nothing
+  // merged by group, a warp per group, around one share's mean: the correction by the mean's distance from it is at
+  // most as many times the result as there are shares, since that share is one of them
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
   const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg);
   int rows_on = 0;
   for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits[i]);
   rows_on = __reduce_add_sync(0xffffffffu, rows_on);
-  const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
+  int some = 0;  // a row lane with a point that is on
+  while (some < sh.R - 1 && !bits[some]) some++;
+  const float inv = rows_on ? __fdividef(1.0f, (float)rows_on * (float)p.cg) : 0.0f;
   const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   float2* stats = p.stats ? p.stats + (int64_t)t.b * p.G + small_div(t.c0, p.cg) : nullptr;
   for (int g = warp; g < groups; g += warps) {
     const float2* gp = part + g * upg;
-    const float ref = gp[0].x;
+    const float ref = gp[some * units].x;
     float s = 0.0f, q = 0.0f;
     for (int y = y0, u = u0; y < sh.R;) {
-      s += (float)(__popc(bits[y]) * U) * (gp[y * units + u].x - ref);
-      y += dy;
-      u += du;
-      if (u >= upg) u -= upg, y++;
-    }
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float delta = s * inv;
-    for (int y = y0, u = u0; y < sh.R;) {
       const float2 v = gp[y * units + u];
-      const float k = (float)(__popc(bits[y]) * U), d = v.x - ref - delta;
-      q += k != 0.0f ? v.y + k * d * d : 0.0f;
+      const float k = (float)(__popc(bits[y]) * U), d = v.x - ref;
+      if (k != 0.0f) {
+        s += k * d;
+        q += v.y + k * d * d;
+      }
       y += dy;
       u += du;
       if (u >= upg) u -= upg, y++;
     }
-    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
     if (lane == 0) {
-      float2 st = make_float2(ref + delta, q);
-      if (sh.cs == 1) {
-        st = rows_on ? make_float2(st.x, 1.0f / sqrtf(q * inv + p.eps)) : make_float2(0.0f, 0.0f);
-        if (stats) stats[g] = st;
-      }
-      mine[g] = st;
+      const float delta = s * inv;
+      q -= s * delta;
+      mine[g] = sh.cs == 1 ? final_stats(ref + delta, q * inv, rows_on, p.eps, stats, g)
+                           : make_float2(ref + delta, q < 0.0f ? 0.0f : q);
     }
   }
   const float2* fin = mine;  // (mean, rstd)
@@ -539,10 +555,8 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
         const float d = v.x - ref - delta;
         if (c != 0.0f) q += v.y + c * d * d;
       }
-      const float2 st = n != 0.0f ? make_float2(ref + delta, 1.0f / sqrtf(q / (n * (float)p.cg) + p.eps))
-                                  : make_float2(0.0f, 0.0f);
-      part[g] = st;
-      if (stats && t.rank == 0) stats[g] = st;
+      part[g] = final_stats(ref + delta, n != 0.0f ? q / (n * (float)p.cg) : 0.0f, n != 0.0f, p.eps,
+                            t.rank == 0 ? stats : nullptr, g);
     }
     fin = part;
   }
@@ -677,7 +691,6 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
 
   on_bits(p, sh, t, bits);
-  __syncthreads();
   const uint32_t on = t.here ? bits[t.ty] : 0;
   copy_rows<T, VEC>(static_cast<const T*>(p.x) + x_at, x_step, on, slots.x, V::BYTES);
   copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)t.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col, y_step, on,
