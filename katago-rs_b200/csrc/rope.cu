@@ -18,7 +18,7 @@
 #include <string>
 
 #include "../../include/katago_cuda.h"
-#include "gemm.cuh"
+#include "gemm_pair.cuh"
 #include "ops_common.h"
 
 namespace kc {
@@ -45,10 +45,8 @@ struct RopeParams {
   int tile, rounds;               // tokens of a tile, threads that share a table's heads (head i of one: i mod rounds)
   uint32_t by_token, by_table, by_head;  // magic() of a token's items, a table's, a head's
   // backward with the frequencies' gradient
-  int head_lanes;                 // threads that share a table's heads: lane l takes heads l, l + head_lanes, ...
-  int width, lanes;               // a block's columns (table, head lane, vector of a head) and tokens at once
+  int width, lanes;               // a block's columns (table, head i mod rounds, vector of a head) and tokens at once
   int columns;                    // of all blocks y
-  int shared;                     // the frequencies' fractions are staged in shared memory
   float* partial;                 // [blocks][tables][pairs][axes]
   float* dfreqs;
   int blocks;
@@ -80,14 +78,6 @@ __device__ __forceinline__ float cos_fast(float x) {
 // n / d by magic(d).
 __device__ __forceinline__ int quotient(int n, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)n, magic) : n; }
 
-struct Position {
-  int at[KC_ROPE_MAX_AXES];
-  __device__ __forceinline__ void load(const RopeParams& p, int64_t t) {
-#pragma unroll
-    for (int a = 0; a < KC_ROPE_MAX_AXES; a++) at[a] = a < p.axes ? __ldg(p.pos + t * p.axes + a) : 0;
-  }
-};
-
 // (cos, sin) of an angle of turns * 2^-64. float32 takes the accurate functions; for 2-byte results the fast ones on
 // half a turn either way (off by 2^-21) are far below the rounding.
 template <typename T>
@@ -104,11 +94,13 @@ __device__ __forceinline__ float2 turned(unsigned long long turns) {
   return r;
 }
 
-// sin and cos of VP pairs' angles at one token, from the fractions in shared memory ([pair of the vector][axis] rows
-// of `stride` columns, so that neighbouring threads read neighbouring words) or from the frequencies `f`.
-template <typename T, int VP, bool STAGED>
-__device__ __forceinline__ void angles(const RopeParams& p, const Position& at, const unsigned long long* g, int stride,
-                                       const float* f, float (&c)[VP], float (&s)[VP]) {
+// sin and cos of VP pairs' angles at one token, from the frequencies `f`.
+template <typename T, int VP>
+__device__ __forceinline__ void angles(const RopeParams& p, int64_t t, const float* f, float (&c)[VP], float (&s)[VP]) {
+  long long pos[KC_ROPE_MAX_AXES];
+#pragma unroll
+  for (int a = 0; a < KC_ROPE_MAX_AXES; a++)
+    pos[a] = a < p.axes ? (long long)__ldg(p.pos + t * p.axes + a) * p.sign : 0;
 #pragma unroll
   for (int j = 0; j < VP; j++) {
     unsigned long long turns = 0;
@@ -116,22 +108,13 @@ __device__ __forceinline__ void angles(const RopeParams& p, const Position& at, 
 #pragma unroll
     for (int a = 0; a < KC_ROPE_MAX_AXES; a++)
       if (a < p.axes) {
-        const unsigned long long n = (unsigned long long)((long long)at.at[a] * p.sign);
-        if constexpr (STAGED) {
-          turns += n * g[(j * p.axes + a) * stride];
-        } else {
-          const float fr = __ldg(f + j * p.axes + a);
-          bad += fr - fr;
-          turns += n * turn_fraction(fr);
-        }
+        const float fr = __ldg(f + j * p.axes + a);
+        bad += fr - fr;
+        turns += (unsigned long long)pos[a] * turn_fraction(fr);
       }
     const float2 cs = turned<T>(turns);
-    c[j] = cs.x;
-    s[j] = cs.y;
-    if constexpr (!STAGED) {
-      s[j] += bad;
-      c[j] += bad;
-    }
+    c[j] = cs.x + bad;
+    s[j] = cs.y + bad;
   }
 }
 
@@ -163,6 +146,24 @@ struct Pairs {
     a = to_f<T>(LAYOUT == KC_ROPE_HALVES ? u.v[j] : at(2 * j));
     b = to_f<T>(LAYOUT == KC_ROPE_HALVES ? v.v[j] : at(2 * j + 1));
   }
+  // all pairs, two to a register pair (one pair: the second is 0)
+  __device__ __forceinline__ void get2(f32x2 (&a)[(VP + 1) / 2], f32x2 (&b)[(VP + 1) / 2]) {
+#pragma unroll
+    for (int j = 0; j < VP; j += 2) {
+      float a0, b0, a1 = 0.0f, b1 = 0.0f;
+      get(j, a0, b0);
+      if (VP > 1) get(j + 1, a1, b1);
+      a[j / 2] = {a0, a1};
+      b[j / 2] = {b0, b1};
+    }
+  }
+  __device__ __forceinline__ void set2(const f32x2 (&a)[(VP + 1) / 2], const f32x2 (&b)[(VP + 1) / 2]) {
+#pragma unroll
+    for (int j = 0; j < VP; j += 2) {
+      set(j, a[j / 2].x, b[j / 2].x);
+      if (VP > 1) set(j + 1, a[j / 2].y, b[j / 2].y);
+    }
+  }
   __device__ __forceinline__ void set(int j, float a, float b) {
     if constexpr (LAYOUT == KC_ROPE_HALVES) {
       u.v[j] = from_f<T>(a);
@@ -174,101 +175,8 @@ struct Pairs {
   }
 };
 
-// A thread's place: columns are (table, head lane, vector of a head: first the pairs', then the unrotated rest's),
-// so that neighbouring threads read neighbouring memory of a token; the block's other threads take other tokens.
-struct Place {
-  int lane, table, head, col, pv;
-  bool here;
-};
-
-template <int VP>
-__device__ __forceinline__ Place place(const RopeParams& p) {
-  Place w;
-  w.pv = p.pairs / VP;
-  const int cols = w.pv + p.rest / VP, column = blockIdx.y * p.width + threadIdx.x % p.width;
-  w.lane = threadIdx.x / p.width;
-  w.here = w.lane < p.lanes && column < p.columns;
-  w.col = column % cols;
-  w.head = column / cols % p.head_lanes;
-  w.table = column / cols / p.head_lanes;
-  return w;
-}
-
-extern __shared__ __align__(16) unsigned long long rope_smem[];
-
-// The fractions of all frequencies into shared memory, as angles() reads them; false where they are not wanted there
-// or one is not finite.
-template <int VP>
-__device__ __forceinline__ bool stage_freqs(const RopeParams& p) {
-  if (!p.shared) return false;
-  const int row = VP * p.axes, vectors = p.tables * p.pairs / VP;
-  bool bad = false;
-  for (int i = threadIdx.x; i < row * vectors; i += kThreads) {
-    const float f = __ldg(p.freqs + i);
-    rope_smem[i % row * vectors + i / row] = turn_fraction(f);
-    bad = bad || !isfinite(f);
-  }
-  return !__syncthreads_or(bad);
-}
-
-// A thread's N heads: the addresses of its vector in each, moved from token to token. Head i of a table is one of its
-// Q heads or, behind them, K heads.
-template <typename T, int N, bool X>
-struct HeadPtrs {
-  const T* in[N];
-  T* out[N];
-  const T* x[X ? N : 1];
-  bool is_q[N];
-  int count;
-  // heads first, first + head_lanes, ..; first < heads
-  __device__ __forceinline__ HeadPtrs(const RopeParams& p, const Place& w, int first, int64_t t, int d) {
-    const int heads = p.q.per_table + p.k.per_table;
-    count = min(N, (heads - first + p.head_lanes - 1) / p.head_lanes);
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      const int i = min(first + k * p.head_lanes, heads - 1);
-      is_q[k] = i < p.q.per_table;
-      const Heads& h = is_q[k] ? p.q : p.k;
-      const int64_t n = (int64_t)w.table * h.per_table + (is_q[k] ? i : i - p.q.per_table);
-      in[k] = static_cast<const T*>(h.in) + t * h.in_t + n * h.in_h + d;
-      out[k] = static_cast<T*>(h.out) + t * h.out_t + n * h.out_h + d;
-      if constexpr (X) x[k] = static_cast<const T*>(h.x) + t * h.x_t + n * h.x_h + d;
-    }
-  }
-  __device__ __forceinline__ void next_in(const RopeParams& p, int64_t tokens) {
-    const int64_t sq = p.q.in_t * tokens, sk = p.k.in_t * tokens, xq = p.q.x_t * tokens, xk = p.k.x_t * tokens;
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      in[k] += is_q[k] ? sq : sk;
-      if constexpr (X) x[k] += is_q[k] ? xq : xk;
-    }
-  }
-  __device__ __forceinline__ void next_out(const RopeParams& p, int64_t tokens) {
-    const int64_t sq = p.q.out_t * tokens, sk = p.k.out_t * tokens;
-#pragma unroll
-    for (int k = 0; k < N; k++) out[k] += is_q[k] ? sq : sk;
-  }
-};
-
-// The unrotated rest of a thread's heads.
-template <typename T, int VP, int N>
-__device__ __forceinline__ void copy_rest(const RopeParams& p, const Place& w, int first, int64_t t0, int64_t step) {
-  HeadPtrs<T, N, false> h(p, w, first, t0, 2 * p.pairs + (w.col - w.pv) * VP);
-  for (int64_t t = t0; t < p.tokens; t += step) {
-    Pack<T, VP> v[N];
-#pragma unroll
-    for (int k = 0; k < N; k++)
-      if (k < h.count) v[k] = *reinterpret_cast<const Pack<T, VP>*>(h.in[k]);
-#pragma unroll
-    for (int k = 0; k < N; k++)
-      if (k < h.count && h.in[k] != h.out[k]) *reinterpret_cast<Pack<T, VP>*>(h.out[k]) = v[k];
-    h.next_in(p, step);
-    h.next_out(p, step);
-  }
-}
-
 // One vector of one head of one token to a thread, which makes its own angles: for few tokens, where a launch is
-// latency, and for tables too large for shared memory. grid.x threads over (token, table, head, vector).
+// latency, and for what the tiles cannot take. Threads over (token, table, head, vector).
 template <typename T, int VP, int LAYOUT>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeParams p) {
   const int heads = p.q.per_table + p.k.per_table, pv = p.pairs / VP, cols = pv + p.rest / VP;
@@ -288,10 +196,8 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   }
   Pairs<T, VP, LAYOUT> x;
   x.load(in, col * VP, p.pairs);
-  Position at;
-  at.load(p, t);
   float c[VP], s[VP];
-  angles<T, VP, false>(p, at, nullptr, 0, p.freqs + ((int64_t)table * p.pairs + col * VP) * p.axes, c, s);
+  angles<T, VP>(p, t, p.freqs + ((int64_t)table * p.pairs + col * VP) * p.axes, c, s);
 #pragma unroll
   for (int j = 0; j < VP; j++) {
     float a, b;
@@ -301,198 +207,319 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   x.store(out, col * VP, p.pairs);
 }
 
-// Sine and cosine of a tile's angles into shared memory: a thread keeps an entry's (table, pair) fractions and goes
-// over the tile's tokens. An entry's place: [chunk of two pairs of a vector][vector of the tile], (cos, sin) pairs, so
+// ---------------------------------------------------------------------------------------------------------------
+// Tiles of tokens. A block makes the sines and cosines of a tile's (token, table, pair) entries once, in shared
+// memory, and then streams the heads through them, two heads of a table to a thread, so that a vector's sines serve
+// two loads. Several blocks to an SM: one's trigonometry runs under the others' loads and stores.
+// ---------------------------------------------------------------------------------------------------------------
+extern __shared__ __align__(16) unsigned char rope_smem[];
+
+// A head's first vector at token 0 and the bytes from token to token.
+struct alignas(16) HeadAddr {
+  const char* in;
+  char* out;
+  const char* x;
+  uint32_t in_step, out_step;
+};
+
+// A tile's shared memory: the frequencies' fractions [axes][entries], the phase of positions' bias [entries], the
+// heads [tables][heads], and the sines: [chunk of two pairs of a vector][vector of the tile] (cos, cos, sin, sin), so
 // that neighbouring threads read neighbouring 16-byte chunks.
+template <int VP>
+struct Tile {
+  static constexpr int CH = VP < 2 ? 1 : 2, CHUNKS = VP / CH;
+  unsigned long long *fraction, *bias;
+  HeadAddr* heads;
+  float* sines;
+  int entries, vectors;
+  __host__ __device__ static size_t bytes(int64_t entries, int axes, int64_t heads, int64_t tile) {
+    return (size_t)heads * sizeof(HeadAddr) + (size_t)((entries * (axes + 1) + 1) / 2 * 16) +
+           (size_t)((entries / VP * tile) | 1) * VP * 8;
+  }
+  __device__ __forceinline__ explicit Tile(const RopeParams& p) {
+    entries = p.tables * p.pairs;
+    vectors = (entries / VP * p.tile) | 1;
+    heads = reinterpret_cast<HeadAddr*>(rope_smem);
+    fraction = reinterpret_cast<unsigned long long*>(heads + p.tables * (p.q.per_table + p.k.per_table));
+    bias = fraction + entries * p.axes;
+    sines = reinterpret_cast<float*>(fraction + (entries * (p.axes + 1) + 1) / 2 * 2);
+  }
+  // an entry's cosine in the tile (its sine is CH floats behind), and what the next token adds
+  __device__ __forceinline__ float* at(int e) const {
+    return sines + ((size_t)(e % VP / CH) * vectors + e / VP) * (2 * CH) + e % CH;
+  }
+  __device__ __forceinline__ int per_token() const { return entries / VP * (2 * CH); }
+  __device__ __forceinline__ void read(int vector, f32x2 (&c)[(VP + 1) / 2], f32x2 (&s)[(VP + 1) / 2]) const {
+#pragma unroll
+    for (int q = 0; q < CHUNKS; q++) {
+      const Pack<float, 2 * CH> v = *reinterpret_cast<const Pack<float, 2 * CH>*>(sines + ((size_t)q * vectors + vector) * (2 * CH));
+      c[q] = {v.v[0], CH == 2 ? v.v[1] : 0.0f};
+      s[q] = {v.v[CH], CH == 2 ? v.v[CH + 1] : 0.0f};
+    }
+  }
+};
+
+// Once per block. Positions enter the products as unsigned numbers, 2^31 higher; the bias takes that out again. False
+// where a frequency is not finite.
+template <typename T, int VP>
+__device__ __forceinline__ bool tile_setup(const RopeParams& p, const Tile<VP>& tile) {
+  bool bad = false;
+  for (int e = threadIdx.x; e < tile.entries; e += kThreads) {
+    unsigned long long sum = 0;
+    for (int a = 0; a < p.axes; a++) {
+      const float f = __ldg(p.freqs + (int64_t)e * p.axes + a);
+      const unsigned long long turn = turn_fraction(f);
+      tile.fraction[a * tile.entries + e] = p.sign < 0 ? 0 - turn : turn;
+      sum += tile.fraction[a * tile.entries + e];
+      bad = bad || !isfinite(f);
+    }
+    tile.bias[e] = 0 - (sum << 31);
+  }
+  const int per = p.q.per_table + p.k.per_table;
+  for (int i = threadIdx.x; i < p.tables * per; i += kThreads) {
+    const int table = i / per, h = i - table * per;
+    const bool is_q = h < p.q.per_table;
+    const Heads& hd = is_q ? p.q : p.k;
+    const int64_t n = (int64_t)table * hd.per_table + (is_q ? h : h - p.q.per_table);
+    HeadAddr& o = tile.heads[i];
+    o.in = reinterpret_cast<const char*>(static_cast<const T*>(hd.in) + n * hd.in_h);
+    o.out = reinterpret_cast<char*>(static_cast<T*>(hd.out) + n * hd.out_h);
+    o.x = reinterpret_cast<const char*>(static_cast<const T*>(hd.x) + n * hd.x_h);
+    o.in_step = (uint32_t)(hd.in_t * sizeof(T));
+    o.out_step = (uint32_t)(hd.out_t * sizeof(T));
+  }
+  return !__syncthreads_or(bad);
+}
+
+// The tile's sines: a thread keeps an entry's fractions and goes over the tokens.
 template <typename T, int VP, int AXES>
-__device__ __forceinline__ void tile_angles(const RopeParams& p, int64_t t0, int tokens, const unsigned long long* g,
-                                            int entries, int vectors, float2* table) {
-  constexpr int CH = VP < 2 ? 1 : 2;
-  const int width = min(entries, kThreads), groups = kThreads / width;
+__device__ __forceinline__ void tile_angles(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens) {
+  const int width = min(tile.entries, kThreads), groups = kThreads / width;
   const int first = threadIdx.x % width, group = threadIdx.x / width;
   if (group >= groups) return;
-  for (int e = first; e < entries; e += width) {
-    unsigned long long fr[AXES];
+  const int step = tile.per_token() * groups;
+  for (int e = first; e < tile.entries; e += width) {
+    uint32_t lo[AXES], hi[AXES];
 #pragma unroll
-    for (int a = 0; a < AXES; a++) fr[a] = g[a * entries + e];
-    const int j = e % VP;
-    float2* o = table + (j / CH * vectors + e / VP) * CH + j % CH;
-    const int* pos = p.pos + t0 * AXES;
-#pragma unroll 2
-    for (int tt = group; tt < tokens; tt += groups) {
-      unsigned long long turns = 0;
+    for (int a = 0; a < AXES; a++) {
+      const unsigned long long f = tile.fraction[a * tile.entries + e];
+      lo[a] = (uint32_t)f;
+      hi[a] = (uint32_t)(f >> 32);
+    }
+    const unsigned long long bias = tile.bias[e];
+    float* o = tile.at(e) + tile.per_token() * group;
+    const int* pos = p.pos + (t0 + group) * AXES;
+#pragma unroll 4
+    for (int tt = group; tt < tokens; tt += groups, o += step, pos += groups * AXES) {
+      unsigned long long turns = bias;
+      uint32_t high = 0;
 #pragma unroll
-      for (int a = 0; a < AXES; a++) turns += (unsigned long long)(long long)__ldg(pos + tt * AXES + a) * fr[a];
-      o[tt * (entries / VP) * CH] = turned<T>(turns);
+      for (int a = 0; a < AXES; a++) {
+        const uint32_t n = (uint32_t)__ldg(pos + a) ^ 0x80000000u;
+        turns += (unsigned long long)n * lo[a];
+        high += n * hi[a];
+      }
+      const float2 cs = turned<T>(turns + ((unsigned long long)high << 32));
+      o[0] = cs.x;
+      o[Tile<VP>::CH] = cs.y;
     }
   }
 }
 
-// Tiles of tokens: the block makes the sines and cosines of a tile once, in shared memory, and then streams the
-// heads through them, N heads of a table to a thread (so that a vector's sines serve N loads). Few registers and many
-// blocks to an SM: one block's trigonometry runs under the others' loads and stores.
-template <typename T, int VP, int LAYOUT, int N>
-__global__ void __launch_bounds__(kThreads, 4) rope_axes_tile_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int CH = VP < 2 ? 1 : 2, CHUNKS = VP / CH;
-  const int entries = p.tables * p.pairs, vectors = (entries / VP * p.tile) | 1;
-  unsigned long long* g = rope_smem;  // [axes][entries]
-  float2* table = reinterpret_cast<float2*>(g + entries * p.axes + (entries * p.axes & 1));
-  bool bad = false;
-  for (int i = threadIdx.x; i < entries * p.axes; i += kThreads) {
-    const float f = __ldg(p.freqs + i);
-    const unsigned long long turn = turn_fraction(f);
-    g[i % p.axes * entries + i / p.axes] = p.sign < 0 ? 0 - turn : turn;
-    bad = bad || !isfinite(f);
+template <typename T, int VP>
+__device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens, bool finite) {
+  if (p.axes == 1) tile_angles<T, VP, 1>(p, tile, t0, tokens);
+  else if (p.axes == 2) tile_angles<T, VP, 2>(p, tile, t0, tokens);
+  else if (p.axes == 3) tile_angles<T, VP, 3>(p, tile, t0, tokens);
+  else tile_angles<T, VP, 4>(p, tile, t0, tokens);
+  __syncthreads();
+  if (finite) return;
+  for (int i = threadIdx.x; i < tokens * tile.entries; i += kThreads) {  // NaN where a frequency is not finite
+    const int tt = i / tile.entries, e = i - tt * tile.entries;
+    float* o = tile.at(e) + tile.per_token() * tt;
+    for (int a = 0; a < p.axes; a++) {
+      const float f = __ldg(p.freqs + (int64_t)e * p.axes + a);
+      o[0] += f - f;
+      o[Tile<VP>::CH] += f - f;
+    }
   }
-  bad = __syncthreads_or(bad);
+  __syncthreads();
+}
+
+// (a, b) turned: a c - b s, a s + b c, two pairs at once.
+__device__ __forceinline__ void turn2(f32x2& a, f32x2& b, f32x2 c, f32x2 s, f32x2 neg_s) {
+  const f32x2 ya = fma2(b, neg_s, mul2(a, c));
+  b = fma2(a, s, mul2(b, c));
+  a = ya;
+}
+
+template <typename T, int VP, int LAYOUT>
+__global__ void __launch_bounds__(kThreads, 4) rope_axes_tile_kernel(const __grid_constant__ RopeParams p) {
+  using P = Pairs<T, VP, LAYOUT>;
+  constexpr int N = 2, NP = (VP + 1) / 2;
+  const Tile<VP> tile(p);
+  const bool finite = tile_setup<T, VP>(p, tile);
   const int heads = p.q.per_table + p.k.per_table, pv = p.pairs / VP, cols = pv + p.rest / VP;
   const int per_token = p.tables * p.rounds * cols;
   for (int64_t t0 = (int64_t)blockIdx.x * p.tile; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.tile) {
     const int tokens = (int)min((int64_t)p.tile, p.tokens - t0);
-    if (p.axes == 1) tile_angles<T, VP, 1>(p, t0, tokens, g, entries, vectors, table);
-    else if (p.axes == 2) tile_angles<T, VP, 2>(p, t0, tokens, g, entries, vectors, table);
-    else if (p.axes == 3) tile_angles<T, VP, 3>(p, t0, tokens, g, entries, vectors, table);
-    else tile_angles<T, VP, 4>(p, t0, tokens, g, entries, vectors, table);
-    __syncthreads();
-    if (bad) {  // NaN where a frequency is not finite
-      for (int i = threadIdx.x; i < tokens * entries; i += kThreads) {
-        const int tt = i / entries, e = i - tt * entries, j = e % VP;
-        float2* o = table + (j / CH * vectors + tt * (entries / VP) + e / VP) * CH + j % CH;
-        for (int a = 0; a < p.axes; a++) {
-          const float f = __ldg(p.freqs + (int64_t)e * p.axes + a);
-          o->x += f - f;
-          o->y += f - f;
-        }
-      }
-      __syncthreads();
-    }
+    tile_sines<T, VP>(p, tile, t0, tokens, finite);
     for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
       const int tt = quotient(i, p.by_token), r = i - tt * per_token;
-      const int tb = quotient(r, p.by_table), r2 = r - tb * (p.rounds * cols);
+      const int table = quotient(r, p.by_table), r2 = r - table * (p.rounds * cols);
       const int first = quotient(r2, p.by_head), col = r2 - first * cols;
-      const int64_t t = t0 + tt;
-      const T* in[N];
-      T* out[N];
-#pragma unroll
-      for (int k = 0; k < N; k++) {
-        const int h = min(first + k * p.rounds, heads - 1);
-        const bool is_q = h < p.q.per_table;
-        const Heads& hd = is_q ? p.q : p.k;
-        const int n = tb * hd.per_table + (is_q ? h : h - p.q.per_table);
-        in[k] = static_cast<const T*>(hd.in) + t * hd.in_t + n * hd.in_h;
-        out[k] = static_cast<T*>(hd.out) + t * hd.out_t + n * hd.out_h;
+      const uint32_t t = (uint32_t)t0 + tt;
+      const HeadAddr* h = tile.heads + table * heads + first;
+      const bool two = first + p.rounds < heads;
+      const char* in[N] = {h->in + (uint64_t)t * h->in_step, nullptr};
+      char* out[N] = {h->out + (uint64_t)t * h->out_step, nullptr};
+      if (two) {
+        h += p.rounds;
+        in[1] = h->in + (uint64_t)t * h->in_step;
+        out[1] = h->out + (uint64_t)t * h->out_step;
       }
       if (col >= pv) {
-        const int d = 2 * p.pairs + (col - pv) * VP;
+        const uint32_t d = (2 * p.pairs + (col - pv) * VP) * sizeof(T);
+        Pack<T, VP> v[N];
 #pragma unroll
         for (int k = 0; k < N; k++)
-          if (first + k * p.rounds < heads && in[k] != out[k])
-            *reinterpret_cast<Pack<T, VP>*>(out[k] + d) = *reinterpret_cast<const Pack<T, VP>*>(in[k] + d);
+          if (k == 0 || two) v[k] = *reinterpret_cast<const Pack<T, VP>*>(in[k] + d);
+#pragma unroll
+        for (int k = 0; k < N; k++)
+          if ((k == 0 || two) && in[k] != out[k]) *reinterpret_cast<Pack<T, VP>*>(out[k] + d) = v[k];
         continue;
       }
-      Pairs<T, VP, LAYOUT> x[N];
+      P x[N];
 #pragma unroll
       for (int k = 0; k < N; k++)
-        if (first + k * p.rounds < heads) x[k].load(in[k], col * VP, p.pairs);
-      Pack<float2, CH> cs[CHUNKS];
-      const int v = tt * (entries / VP) + tb * pv + col;
-#pragma unroll
-      for (int q = 0; q < CHUNKS; q++) cs[q] = *reinterpret_cast<const Pack<float2, CH>*>(table + (q * vectors + v) * CH);
+        if (k == 0 || two) x[k].load(reinterpret_cast<const T*>(in[k]), col * VP, p.pairs);
+      f32x2 c[NP], s[NP];
+      tile.read(tt * (tile.entries / VP) + table * pv + col, c, s);
 #pragma unroll
       for (int k = 0; k < N; k++)
-        if (first + k * p.rounds < heads) {
+        if (k == 0 || two) {
+          f32x2 a[NP], b[NP];
+          x[k].get2(a, b);
 #pragma unroll
-          for (int j = 0; j < VP; j++) {
-            float a, b;
-            x[k].get(j, a, b);
-            const float2 w = cs[j / CH].v[j % CH];
-            x[k].set(j, a * w.x - b * w.y, a * w.y + b * w.x);
-          }
-          x[k].store(out[k], col * VP, p.pairs);
+          for (int j = 0; j < NP; j++) turn2(a[j], b[j], c[j], s[j], f32x2{-s[j].x, -s[j].y});
+          x[k].set2(a, b);
+          x[k].store(reinterpret_cast<T*>(out[k]), col * VP, p.pairs);
         }
     }
     __syncthreads();
   }
 }
 
-// Backward with the frequencies' gradient: a thread also adds pos * d angle over its tokens in float32; the block's
-// threads of one (table, pair vector) are added in order into the block's partial sums.
-template <typename T, int VP, int LAYOUT, int N>
-__global__ void __launch_bounds__(kThreads) rope_axes_back_kernel(const __grid_constant__ RopeParams p) {
+// Backward with the frequencies' gradient: a thread keeps one column (table, head i mod rounds, pair vector) and goes
+// over tokens; it adds pos * d angle in float32, and the block's threads of one (table, pair vector) are added in
+// order into the block's partial sums. `rounds` threads share a table's heads: head h, h + rounds, ... to one.
+template <typename T, int VP, int LAYOUT>
+__global__ void __launch_bounds__(kThreads, 2) rope_axes_back_kernel(const __grid_constant__ RopeParams p) {
+  using P = Pairs<T, VP, LAYOUT>;
+  constexpr int NP = (VP + 1) / 2;
   __shared__ float red[kThreads * VP];
-  const bool staged = stage_freqs<VP>(p);
-  const Place w = place<VP>(p);
-  const int64_t t0 = (int64_t)blockIdx.x * p.lanes + w.lane, step = (int64_t)gridDim.x * p.lanes;
-  const int j0 = w.col * VP, vectors = p.tables * w.pv;
-  float acc[KC_ROPE_MAX_AXES][VP] = {};
-  // a block holds all head lanes of a table (its sums are the block's), so that many heads take several rounds
-  const int heads = w.here ? p.q.per_table + p.k.per_table : 0;
-  for (int first = w.head; first < heads; first += N * p.head_lanes) {
-    if (w.col >= w.pv) {
-      copy_rest<T, VP, N>(p, w, first, t0, step);
-      continue;
-    }
-    const unsigned long long* g = rope_smem + w.table * w.pv + w.col;
-    const float* f = p.freqs + ((int64_t)w.table * p.pairs + j0) * p.axes;
-    HeadPtrs<T, N, true> h(p, w, first, t0, 0);
-    for (int64_t t = t0; t < p.tokens; t += step) {
-      Pairs<T, VP, LAYOUT> dy[N], x[N];
-#pragma unroll
-      for (int k = 0; k < N; k++)
-        if (k < h.count) {
-          dy[k].load(h.in[k], j0, p.pairs);
-          x[k].load(h.x[k], j0, p.pairs);
+  const Tile<VP> tile(p);
+  const bool finite = tile_setup<T, VP>(p, tile);
+  const int heads = p.q.per_table + p.k.per_table, pv = p.pairs / VP, cols = pv + p.rest / VP;
+  const int column = blockIdx.y * p.width + threadIdx.x % p.width, lane = threadIdx.x / p.width;
+  const bool here = lane < p.lanes && column < p.columns;
+  const int col = column % cols, first = column / cols % p.rounds, table = here ? column / cols / p.rounds : 0;
+  f32x2 acc[KC_ROPE_MAX_AXES][NP] = {};
+  for (int64_t t0 = (int64_t)blockIdx.x * p.tile; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.tile) {
+    const int tokens = (int)min((int64_t)p.tile, p.tokens - t0);
+    tile_sines<T, VP>(p, tile, t0, tokens, finite);
+    for (int tt = lane; here && tt < tokens; tt += p.lanes) {
+      const uint32_t t = (uint32_t)t0 + tt;
+      if (col >= pv) {
+        const uint32_t d = (2 * p.pairs + (col - pv) * VP) * sizeof(T);
+        for (int i = first; i < heads; i += p.rounds) {
+          const HeadAddr& h = tile.heads[table * heads + i];
+          const char* in = h.in + (uint64_t)t * h.in_step;
+          char* out = h.out + (uint64_t)t * h.out_step;
+          if (in != out) *reinterpret_cast<Pack<T, VP>*>(out + d) = *reinterpret_cast<const Pack<T, VP>*>(in + d);
         }
-      Position at;
-      at.load(p, t);
-      float c[VP], s[VP], turn[VP] = {};
-      if (staged) angles<T, VP, true>(p, at, g, vectors, f, c, s);
-      else angles<T, VP, false>(p, at, g, vectors, f, c, s);
+        continue;
+      }
+      f32x2 c[NP], s[NP], turn[NP] = {};
+      tile.read(tt * (tile.entries / VP) + table * pv + col, c, s);
+#pragma unroll 2
+      for (int i = first; i < heads; i += p.rounds) {
+        const HeadAddr& h = tile.heads[table * heads + i];
+        P dy, x;
+        dy.load(reinterpret_cast<const T*>(h.in + (uint64_t)t * h.in_step), col * VP, p.pairs);
+        x.load(reinterpret_cast<const T*>(h.x + (uint64_t)t * h.out_step), col * VP, p.pairs);
+        f32x2 a[NP], b[NP], xa[NP], xb[NP];
+        dy.get2(a, b);
+        x.get2(xa, xb);
 #pragma unroll
-      for (int k = 0; k < N; k++) {
-        if (k < h.count) {
-#pragma unroll
-          for (int j = 0; j < VP; j++) {
-            float a, b, xa, xb;
-            dy[k].get(j, a, b);
-            x[k].get(j, xa, xb);
-            const float da = a * c[j] - b * s[j], db = a * s[j] + b * c[j];
-            turn[j] += db * xa - da * xb;
-            dy[k].set(j, da, db);
-          }
-          dy[k].store(h.out[k], j0, p.pairs);
+        for (int j = 0; j < NP; j++) {
+          turn2(a[j], b[j], c[j], s[j], f32x2{-s[j].x, -s[j].y});
+          const f32x2 neg = mul2(a[j], f32x2{-1.0f, -1.0f});
+          turn[j] = fma2(b[j], xa[j], fma2(neg, xb[j], turn[j]));
         }
+        dy.set2(a, b);
+        dy.store(reinterpret_cast<T*>(h.out + (uint64_t)t * h.out_step), col * VP, p.pairs);
       }
 #pragma unroll
       for (int a = 0; a < KC_ROPE_MAX_AXES; a++) {
         if (a >= p.axes) break;
-        const float pos = (float)at.at[a];
+        const float pos = (float)__ldg(p.pos + (int64_t)t * p.axes + a);
 #pragma unroll
-        for (int j = 0; j < VP; j++) acc[a][j] += pos * turn[j];
+        for (int j = 0; j < NP; j++) acc[a][j] = fma2(f32x2{pos, pos}, turn[j], acc[a][j]);
       }
-      h.next_in(p, step);
-      h.next_out(p, step);
     }
+    __syncthreads();
   }
-  const int cols = w.pv + p.rest / VP;
 #pragma unroll
   for (int a = 0; a < KC_ROPE_MAX_AXES; a++) {
     if (a >= p.axes) break;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < VP; j++) red[j * kThreads + threadIdx.x] = acc[a][j];
+    for (int j = 0; j < VP; j++) red[j * kThreads + threadIdx.x] = j % 2 ? acc[a][j / 2].y : acc[a][j / 2].x;
     __syncthreads();
-    if (w.here && w.lane == 0 && w.head == 0 && w.col < w.pv) {
-      float* o = p.partial + (((int64_t)blockIdx.x * p.tables + w.table) * p.pairs + j0) * p.axes + a;
+    if (here && lane == 0 && first == 0 && col < pv) {
+      float* o = p.partial + (((int64_t)blockIdx.x * p.tables + table) * p.pairs + col * VP) * p.axes + a;
 #pragma unroll
       for (int j = 0; j < VP; j++) {
         float v = 0.0f;
         for (int l = 0; l < p.lanes; l++)
-          for (int h = 0; h < p.head_lanes; h++) v += red[j * kThreads + l * p.width + threadIdx.x + h * cols];
+          for (int h = 0; h < p.rounds; h++) v += red[j * kThreads + l * p.width + threadIdx.x + h * cols];
         o[(int64_t)j * p.axes] = v;
       }
     }
   }
+}
+
+// The frequencies' gradient alone, for what the tiles cannot take (tables too large for shared memory, steps past 32
+// bits): a thread per (table, pair) entry, blocks x share the tokens.
+template <typename T, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) rope_freqs_direct_kernel(const __grid_constant__ RopeParams p) {
+  const int e = blockIdx.y * kThreads + threadIdx.x;
+  if (e >= p.tables * p.pairs) return;
+  const int table = e / p.pairs, j = e - table * p.pairs;
+  float acc[KC_ROPE_MAX_AXES] = {};
+  for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    float c[1], s[1], turn = 0.0f;
+    angles<T, 1>(p, t, p.freqs + (int64_t)e * p.axes, c, s);
+    for (int i = 0; i < p.q.per_table + p.k.per_table; i++) {
+      const bool is_q = i < p.q.per_table;
+      const Heads& h = is_q ? p.q : p.k;
+      const int64_t n = (int64_t)table * h.per_table + (is_q ? i : i - p.q.per_table);
+      Pairs<T, 1, LAYOUT> dy, x;
+      dy.load(static_cast<const T*>(h.in) + t * h.in_t + n * h.in_h, j, p.pairs);
+      x.load(static_cast<const T*>(h.x) + t * h.x_t + n * h.x_h, j, p.pairs);
+      float a, b, xa, xb;
+      dy.get(0, a, b);
+      x.get(0, xa, xb);
+      turn += (a * s[0] + b * c[0]) * xa - (a * c[0] - b * s[0]) * xb;
+    }
+#pragma unroll
+    for (int a = 0; a < KC_ROPE_MAX_AXES; a++)
+      if (a < p.axes) acc[a] += (float)__ldg(p.pos + t * p.axes + a) * turn;
+  }
+#pragma unroll
+  for (int a = 0; a < KC_ROPE_MAX_AXES; a++)
+    if (a < p.axes) p.partial[((int64_t)blockIdx.x * p.tables * p.pairs + e) * p.axes + a] = acc[a];
 }
 
 // dfreqs = the blocks' partial sums, in order and in 64 bits: 8 frequencies a block, 32 lanes of blocks each.
@@ -603,7 +630,7 @@ int vec_of(const kc_rope_desc& d, std::initializer_list<Rows> all) {
 }
 
 constexpr int kSms = 148;
-constexpr int kMaxFreqBytes = 64 * 1024;  // of shared memory for the frequencies' fractions
+constexpr int kMaxTileBytes = 100 * 1024;  // of shared memory a block of the tile kernels
 
 // Blocks of a backward pass with the frequencies' gradient: two to an SM (registers), each with its partial sums.
 int64_t back_blocks(const kc_rope_desc& d) {
@@ -646,7 +673,7 @@ void launch_kernel(const RopeParams& p, dim3 grid, size_t smem, cudaStream_t st)
     KC_CUDA(cudaGetDevice(&dev));
     if (dev >= 128) bad("device index above 127");
     if (!(allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1)) {
-      KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxFreqBytes));
+      KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxTileBytes));
       allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
     }
   }
@@ -657,21 +684,34 @@ void launch_kernel(const RopeParams& p, dim3 grid, size_t smem, cudaStream_t st)
 // n * magic >> 32 = n / d for n d < 2^32 (0 stands for d = 1)
 uint32_t magic(int64_t d) { return d == 1 ? 0 : (uint32_t)(0xffffffffu / d + 1); }
 
+// Steps the tile kernels can index with: a token's in 32 bits of bytes, tokens in 32 bits.
+bool small_steps(const RopeParams& p, int64_t es) {
+  const int64_t most = std::max({p.q.in_t, p.q.out_t, p.q.x_t, p.k.in_t, p.k.out_t, p.k.x_t});
+  return p.tokens <= 0x7fffffff && most * es <= 0xffffffffll;
+}
+
+// Backward with the frequencies' gradient: the columns of a block. A thread takes two heads of a table or more: the
+// sums over the threads that share a table's heads are a block's, so that it holds whole tables.
 template <typename T, int VP, int LAYOUT>
 void launch_back(RopeParams p, cudaStream_t st) {
   const int heads = p.q.per_table + p.k.per_table, cols = p.pairs / VP + p.rest / VP;
-  // a thread takes two heads of a table to its angles, one where there are too few tokens for that; the sums over a
-  // table's head lanes are a block's: it holds whole tables
-  const int per = p.tokens * p.tables * cols * ((heads + 1) / 2) >= kSms * 512 ? 2 : 1;
-  p.head_lanes = std::min((heads + per - 1) / per, std::max(1, kThreads / cols));
-  p.columns = p.tables * p.head_lanes * cols;
+  p.rounds = std::min((heads + 1) / 2, std::max(1, kThreads / cols));
+  p.columns = p.tables * p.rounds * cols;
   p.width = std::min(p.columns, kThreads);
-  if (p.head_lanes > 1) p.width = p.width / (p.head_lanes * cols) * (p.head_lanes * cols);
+  if (p.rounds > 1) p.width = p.width / (p.rounds * cols) * (p.rounds * cols);
   p.lanes = kThreads / p.width;
-  const size_t bytes = (size_t)p.tables * p.pairs * p.axes * sizeof(unsigned long long);
-  p.shared = bytes <= (size_t)kMaxFreqBytes && p.tokens >= (int64_t)p.blocks * p.lanes * 4;
-  launch_kernel<rope_axes_back_kernel<T, VP, LAYOUT, 2>>(
-      p, dim3((unsigned)p.blocks, (unsigned)((p.columns + p.width - 1) / p.width)), p.shared ? bytes : 0, st);
+  const int64_t entries = (int64_t)p.tables * p.pairs;
+  auto bytes = [&](int64_t tile) { return Tile<VP>::bytes(entries, p.axes, (int64_t)p.tables * heads, tile); };
+  const int64_t spread = (p.tokens + p.blocks - 1) / p.blocks, fit = 32 * 1024 / (entries * 8);
+  p.tile = (int)std::max<int64_t>(1, std::min<int64_t>({spread, fit, 64}));
+  if (bytes(p.tile) <= (size_t)kMaxTileBytes && small_steps(p, sizeof(T))) {
+    launch_kernel<rope_axes_back_kernel<T, VP, LAYOUT>>(
+        p, dim3((unsigned)p.blocks, (unsigned)((p.columns + p.width - 1) / p.width)), bytes(p.tile), st);
+  } else {  // before the gradients, which may take the place of what it reads
+    launch_kernel<rope_freqs_direct_kernel<T, LAYOUT>>(
+        p, dim3((unsigned)p.blocks, (unsigned)((entries + kThreads - 1) / kThreads)), 0, st);
+    launch_kernel<rope_axes_kernel<T, VP, LAYOUT>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
+  }
   const int count = p.tables * p.pairs * p.axes;
   rope_freqs_kernel<<<(count + 7) / 8, kThreads, 0, st>>>(p.partial, p.blocks, count, p.dfreqs);
   KC_CUDA(cudaGetLastError());
@@ -685,12 +725,12 @@ void launch(RopeParams p, cudaStream_t st) {
   // tiles of at most 32 KB of sines, not more tokens than leave every SM four blocks' work
   const int64_t fit = 32 * 1024 / (entries * 8), spread = p.tokens / (kSms * 4);
   p.tile = (int)std::max<int64_t>(1, std::min<int64_t>({fit, spread, 64}));
-  const int64_t n = heads > 1 ? 2 : 1;
-  p.rounds = (int)((heads + n - 1) / n);
+  p.rounds = (int)((heads + 1) / 2);
   const int64_t per_token = (int64_t)p.tables * p.rounds * cols;
-  const size_t smem = (size_t)(entries * p.axes + 1) / 2 * 16 + (size_t)((entries / VP * p.tile) | 1) * VP * 8;
-  const bool small = p.tokens * p.tables * heads * cols <= kSms * 2048;  // one wave of threads
-  if (small || smem > (size_t)kMaxFreqBytes || per_token * per_token * p.tile > 0xffffffffll) {
+  const size_t smem = Tile<VP>::bytes(entries, p.axes, p.tables * heads, p.tile);
+  const bool one_wave = p.tokens * p.tables * heads * cols <= kSms * 2048;  // of threads
+  if (one_wave || smem > (size_t)kMaxTileBytes || per_token * per_token * p.tile > 0xffffffffll ||
+      !small_steps(p, sizeof(T))) {
     launch_kernel<rope_axes_kernel<T, VP, LAYOUT>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
     return;
   }
@@ -698,9 +738,7 @@ void launch(RopeParams p, cudaStream_t st) {
   p.by_table = magic(p.rounds * cols);
   p.by_head = magic(cols);
   const int64_t tiles = (p.tokens + p.tile - 1) / p.tile;
-  const dim3 grid((unsigned)std::min<int64_t>(tiles, kSms * 8));
-  if (n == 2) launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT, 2>>(p, grid, smem, st);
-  else launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT, 1>>(p, grid, smem, st);
+  launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT>>(p, dim3((unsigned)std::min<int64_t>(tiles, kSms * 8)), smem, st);
 }
 
 template <typename T, int VP>
