@@ -25,6 +25,8 @@ namespace kc {
 namespace {
 
 constexpr int kThreads = 256;
+// Blocks of the tile kernels to an SM, forward and backward with the frequencies' gradient (registers).
+constexpr int kTileBlocks = 3, kBackBlocks = 2;
 
 struct Heads {
   const void* in;
@@ -146,23 +148,17 @@ struct Pairs {
     a = to_f<T>(LAYOUT == KC_ROPE_HALVES ? u.v[j] : at(2 * j));
     b = to_f<T>(LAYOUT == KC_ROPE_HALVES ? v.v[j] : at(2 * j + 1));
   }
-  // all pairs, two to a register pair (one pair: the second is 0)
-  __device__ __forceinline__ void get2(f32x2 (&a)[(VP + 1) / 2], f32x2 (&b)[(VP + 1) / 2]) {
-#pragma unroll
-    for (int j = 0; j < VP; j += 2) {
-      float a0, b0, a1 = 0.0f, b1 = 0.0f;
-      get(j, a0, b0);
-      if (VP > 1) get(j + 1, a1, b1);
-      a[j / 2] = {a0, a1};
-      b[j / 2] = {b0, b1};
-    }
+  // pairs j and j + 1 (j even; where a vector has one pair the second is 0)
+  __device__ __forceinline__ void get2(int j, f32x2& a, f32x2& b) {
+    float a0, b0, a1 = 0.0f, b1 = 0.0f;
+    get(j, a0, b0);
+    if (VP > 1) get(j + 1, a1, b1);
+    a = {a0, a1};
+    b = {b0, b1};
   }
-  __device__ __forceinline__ void set2(const f32x2 (&a)[(VP + 1) / 2], const f32x2 (&b)[(VP + 1) / 2]) {
-#pragma unroll
-    for (int j = 0; j < VP; j += 2) {
-      set(j, a[j / 2].x, b[j / 2].x);
-      if (VP > 1) set(j + 1, a[j / 2].y, b[j / 2].y);
-    }
+  __device__ __forceinline__ void set2(int j, f32x2 a, f32x2 b) {
+    set(j, a.x, b.x);
+    if (VP > 1) set(j + 1, a.y, b.y);
   }
   __device__ __forceinline__ void set(int j, float a, float b) {
     if constexpr (LAYOUT == KC_ROPE_HALVES) {
@@ -222,19 +218,20 @@ struct alignas(16) HeadAddr {
   uint32_t in_step, out_step;
 };
 
-// A tile's shared memory: the frequencies' fractions [axes][entries], the phase of positions' bias [entries], the
-// heads [tables][heads], and the sines: [chunk of two pairs of a vector][vector of the tile] (cos, cos, sin, sin), so
+// A tile's shared memory: the heads [tables][heads], the frequencies' fractions [axes][entries], the phase of the
+// positions' bias [entries], the tile's positions [tokens][axes], and the sines: [chunk of two pairs of a vector][vector of the tile] (cos, cos, sin, sin), so
 // that neighbouring threads read neighbouring 16-byte chunks.
 template <int VP>
 struct Tile {
   static constexpr int CH = VP < 2 ? 1 : 2, CHUNKS = VP / CH;
   unsigned long long *fraction, *bias;
   HeadAddr* heads;
+  uint32_t* pos;
   float* sines;
   int entries, vectors;
   __host__ __device__ static size_t bytes(int64_t entries, int axes, int64_t heads, int64_t tile) {
     return (size_t)heads * sizeof(HeadAddr) + (size_t)((entries * (axes + 1) + 1) / 2 * 16) +
-           (size_t)((entries / VP * tile) | 1) * VP * 8;
+           (size_t)((tile * axes + 3) / 4 * 16) + (size_t)((entries / VP * tile) | 1) * VP * 8;
   }
   __device__ __forceinline__ explicit Tile(const RopeParams& p) {
     entries = p.tables * p.pairs;
@@ -242,7 +239,8 @@ struct Tile {
     heads = reinterpret_cast<HeadAddr*>(rope_smem);
     fraction = reinterpret_cast<unsigned long long*>(heads + p.tables * (p.q.per_table + p.k.per_table));
     bias = fraction + entries * p.axes;
-    sines = reinterpret_cast<float*>(fraction + (entries * (p.axes + 1) + 1) / 2 * 2);
+    pos = reinterpret_cast<uint32_t*>(fraction + (entries * (p.axes + 1) + 1) / 2 * 2);
+    sines = reinterpret_cast<float*>(pos + (p.tile * p.axes + 3) / 4 * 4);
   }
   // an entry's cosine in the tile (its sine is CH floats behind), and what the next token adds
   __device__ __forceinline__ float* at(int e) const {
@@ -259,10 +257,18 @@ struct Tile {
   }
 };
 
-// Once per block. Positions enter the products as unsigned numbers, 2^31 higher; the bias takes that out again. False
-// where a frequency is not finite.
+// A tile's positions, as unsigned numbers 2^31 higher (fewer steps in the 64-bit product); the bias takes that out.
+template <int VP>
+__device__ __forceinline__ void tile_positions(const RopeParams& p, const Tile<VP>& tile, int64_t t0) {
+  if (t0 >= p.tokens) return;
+  const int n = (int)min((int64_t)p.tile, p.tokens - t0) * p.axes;
+  for (int i = threadIdx.x; i < n; i += kThreads) tile.pos[i] = (uint32_t)__ldg(p.pos + t0 * p.axes + i) ^ 0x80000000u;
+}
+
+// Once per block, with the first tile's positions. False where a frequency is not finite.
 template <typename T, int VP>
 __device__ __forceinline__ bool tile_setup(const RopeParams& p, const Tile<VP>& tile) {
+  tile_positions<VP>(p, tile, (int64_t)blockIdx.x * p.tile);
   bool bad = false;
   for (int e = threadIdx.x; e < tile.entries; e += kThreads) {
     unsigned long long sum = 0;
@@ -293,7 +299,7 @@ __device__ __forceinline__ bool tile_setup(const RopeParams& p, const Tile<VP>& 
 
 // The tile's sines: a thread keeps an entry's fractions and goes over the tokens.
 template <typename T, int VP, int AXES>
-__device__ __forceinline__ void tile_angles(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens) {
+__device__ __forceinline__ void tile_angles(const Tile<VP>& tile, int tokens) {
   const int width = min(tile.entries, kThreads), groups = kThreads / width;
   const int first = threadIdx.x % width, group = threadIdx.x / width;
   if (group >= groups) return;
@@ -308,16 +314,15 @@ __device__ __forceinline__ void tile_angles(const RopeParams& p, const Tile<VP>&
     }
     const unsigned long long bias = tile.bias[e];
     float* o = tile.at(e) + tile.per_token() * group;
-    const int* pos = p.pos + (t0 + group) * AXES;
+    const uint32_t* pos = tile.pos + group * AXES;
 #pragma unroll 4
     for (int tt = group; tt < tokens; tt += groups, o += step, pos += groups * AXES) {
       unsigned long long turns = bias;
       uint32_t high = 0;
 #pragma unroll
       for (int a = 0; a < AXES; a++) {
-        const uint32_t n = (uint32_t)__ldg(pos + a) ^ 0x80000000u;
-        turns += (unsigned long long)n * lo[a];
-        high += n * hi[a];
+        turns += (unsigned long long)pos[a] * lo[a];
+        high += pos[a] * hi[a];
       }
       const float2 cs = turned<T>(turns + ((unsigned long long)high << 32));
       o[0] = cs.x;
@@ -328,11 +333,12 @@ __device__ __forceinline__ void tile_angles(const RopeParams& p, const Tile<VP>&
 
 template <typename T, int VP>
 __device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens, bool finite) {
-  if (p.axes == 1) tile_angles<T, VP, 1>(p, tile, t0, tokens);
-  else if (p.axes == 2) tile_angles<T, VP, 2>(p, tile, t0, tokens);
-  else if (p.axes == 3) tile_angles<T, VP, 3>(p, tile, t0, tokens);
-  else tile_angles<T, VP, 4>(p, tile, t0, tokens);
+  if (p.axes == 1) tile_angles<T, VP, 1>(tile, tokens);
+  else if (p.axes == 2) tile_angles<T, VP, 2>(tile, tokens);
+  else if (p.axes == 3) tile_angles<T, VP, 3>(tile, tokens);
+  else tile_angles<T, VP, 4>(tile, tokens);
   __syncthreads();
+  tile_positions<VP>(p, tile, t0 + (int64_t)gridDim.x * p.tile);  // the next tile's, seen after the tile's last barrier
   if (finite) return;
   for (int i = threadIdx.x; i < tokens * tile.entries; i += kThreads) {  // NaN where a frequency is not finite
     const int tt = i / tile.entries, e = i - tt * tile.entries;
@@ -347,14 +353,14 @@ __device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& 
 }
 
 // (a, b) turned: a c - b s, a s + b c, two pairs at once.
-__device__ __forceinline__ void turn2(f32x2& a, f32x2& b, f32x2 c, f32x2 s, f32x2 neg_s) {
-  const f32x2 ya = fma2(b, neg_s, mul2(a, c));
+__device__ __forceinline__ void turn2(f32x2& a, f32x2& b, f32x2 c, f32x2 s) {
+  const f32x2 ya = fma2({-b.x, -b.y}, s, mul2(a, c));
   b = fma2(a, s, mul2(b, c));
   a = ya;
 }
 
 template <typename T, int VP, int LAYOUT>
-__global__ void __launch_bounds__(kThreads, 4) rope_axes_tile_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, kTileBlocks) rope_axes_tile_kernel(const __grid_constant__ RopeParams p) {
   using P = Pairs<T, VP, LAYOUT>;
   constexpr int N = 2, NP = (VP + 1) / 2;
   const Tile<VP> tile(p);
@@ -398,11 +404,13 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_tile_kernel(const __gri
 #pragma unroll
       for (int k = 0; k < N; k++)
         if (k == 0 || two) {
-          f32x2 a[NP], b[NP];
-          x[k].get2(a, b);
 #pragma unroll
-          for (int j = 0; j < NP; j++) turn2(a[j], b[j], c[j], s[j], f32x2{-s[j].x, -s[j].y});
-          x[k].set2(a, b);
+          for (int j = 0; j < NP; j++) {
+            f32x2 a, b;
+            x[k].get2(2 * j, a, b);
+            turn2(a, b, c[j], s[j]);
+            x[k].set2(2 * j, a, b);
+          }
           x[k].store(reinterpret_cast<T*>(out[k]), col * VP, p.pairs);
         }
     }
@@ -413,8 +421,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_tile_kernel(const __gri
 // Backward with the frequencies' gradient: a thread keeps one column (table, head i mod rounds, pair vector) and goes
 // over tokens; it adds pos * d angle in float32, and the block's threads of one (table, pair vector) are added in
 // order into the block's partial sums. `rounds` threads share a table's heads: head h, h + rounds, ... to one.
-template <typename T, int VP, int LAYOUT>
-__global__ void __launch_bounds__(kThreads, 2) rope_axes_back_kernel(const __grid_constant__ RopeParams p) {
+template <typename T, int VP, int LAYOUT, int AXES>  // AXES: at most
+__global__ void __launch_bounds__(kThreads, kBackBlocks) rope_axes_back_kernel(const __grid_constant__ RopeParams p) {
   using P = Pairs<T, VP, LAYOUT>;
   constexpr int NP = (VP + 1) / 2;
   __shared__ float red[kThreads * VP];
@@ -424,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 2) rope_axes_back_kernel(const __gri
   const int column = blockIdx.y * p.width + threadIdx.x % p.width, lane = threadIdx.x / p.width;
   const bool here = lane < p.lanes && column < p.columns;
   const int col = column % cols, first = column / cols % p.rounds, table = here ? column / cols / p.rounds : 0;
-  f32x2 acc[KC_ROPE_MAX_AXES][NP] = {};
+  f32x2 acc[AXES][NP] = {};
   for (int64_t t0 = (int64_t)blockIdx.x * p.tile; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.tile) {
     const int tokens = (int)min((int64_t)p.tile, p.tokens - t0);
     tile_sines<T, VP>(p, tile, t0, tokens, finite);
@@ -442,26 +450,34 @@ __global__ void __launch_bounds__(kThreads, 2) rope_axes_back_kernel(const __gri
       }
       f32x2 c[NP], s[NP], turn[NP] = {};
       tile.read(tt * (tile.entries / VP) + table * pv + col, c, s);
-#pragma unroll 2
-      for (int i = first; i < heads; i += p.rounds) {
-        const HeadAddr& h = tile.heads[table * heads + i];
-        P dy, x;
-        dy.load(reinterpret_cast<const T*>(h.in + (uint64_t)t * h.in_step), col * VP, p.pairs);
-        x.load(reinterpret_cast<const T*>(h.x + (uint64_t)t * h.out_step), col * VP, p.pairs);
-        f32x2 a[NP], b[NP], xa[NP], xb[NP];
-        dy.get2(a, b);
-        x.get2(xa, xb);
+      constexpr int N = 2;  // heads in flight
+      for (int i = first; i < heads; i += N * p.rounds) {
+        const HeadAddr* h = tile.heads + table * heads + i;
+        const bool two = i + p.rounds < heads;
+        P dy[N], x[N];
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-          turn2(a[j], b[j], c[j], s[j], f32x2{-s[j].x, -s[j].y});
-          const f32x2 neg = mul2(a[j], f32x2{-1.0f, -1.0f});
-          turn[j] = fma2(b[j], xa[j], fma2(neg, xb[j], turn[j]));
-        }
-        dy.set2(a, b);
-        dy.store(reinterpret_cast<T*>(h.out + (uint64_t)t * h.out_step), col * VP, p.pairs);
+        for (int k = 0; k < N; k++)
+          if (k == 0 || two) {
+            dy[k].load(reinterpret_cast<const T*>(h[k * p.rounds].in + (uint64_t)t * h[k * p.rounds].in_step), col * VP, p.pairs);
+            x[k].load(reinterpret_cast<const T*>(h[k * p.rounds].x + (uint64_t)t * h[k * p.rounds].out_step), col * VP, p.pairs);
+          }
+#pragma unroll
+        for (int k = 0; k < N; k++)
+          if (k == 0 || two) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+              f32x2 a, b, xa, xb;
+              dy[k].get2(2 * j, a, b);
+              x[k].get2(2 * j, xa, xb);
+              turn2(a, b, c[j], s[j]);
+              turn[j] = fma2(b, xa, fma2({-a.x, -a.y}, xb, turn[j]));
+              dy[k].set2(2 * j, a, b);
+            }
+            dy[k].store(reinterpret_cast<T*>(h[k * p.rounds].out + (uint64_t)t * h[k * p.rounds].out_step), col * VP, p.pairs);
+          }
       }
 #pragma unroll
-      for (int a = 0; a < KC_ROPE_MAX_AXES; a++) {
+      for (int a = 0; a < AXES; a++) {
         if (a >= p.axes) break;
         const float pos = (float)__ldg(p.pos + (int64_t)t * p.axes + a);
 #pragma unroll
@@ -471,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 2) rope_axes_back_kernel(const __gri
     __syncthreads();
   }
 #pragma unroll
-  for (int a = 0; a < KC_ROPE_MAX_AXES; a++) {
+  for (int a = 0; a < AXES; a++) {
     if (a >= p.axes) break;
     __syncthreads();
 #pragma unroll
@@ -632,9 +648,9 @@ int vec_of(const kc_rope_desc& d, std::initializer_list<Rows> all) {
 constexpr int kSms = 148;
 constexpr int kMaxTileBytes = 100 * 1024;  // of shared memory a block of the tile kernels
 
-// Blocks of a backward pass with the frequencies' gradient: two to an SM (registers), each with its partial sums.
+// Blocks of a backward pass with the frequencies' gradient: as many as fit the SMs (registers), each with its partial sums.
 int64_t back_blocks(const kc_rope_desc& d) {
-  return std::min<int64_t>(kSms * 2, std::max<int64_t>(1, d.tokens));
+  return std::min<int64_t>(kSms * kBackBlocks, std::max<int64_t>(1, d.tokens));
 }
 size_t back_bytes(const kc_rope_desc& d) {
   if (d.tokens == 0) return 0;
@@ -684,6 +700,12 @@ void launch_kernel(const RopeParams& p, dim3 grid, size_t smem, cudaStream_t st)
 // n * magic >> 32 = n / d for n d < 2^32 (0 stands for d = 1)
 uint32_t magic(int64_t d) { return d == 1 ? 0 : (uint32_t)(0xffffffffu / d + 1); }
 
+// Tokens of a tile, at most `most` (32 KB of sines): every block gets the same number of tiles.
+int tile_tokens(int64_t tokens, int64_t blocks, int64_t most) {
+  const int64_t share = (tokens + blocks - 1) / blocks, tiles = (share + std::max<int64_t>(1, most) - 1) / std::max<int64_t>(1, most);
+  return (int)((share + tiles - 1) / tiles);
+}
+
 // Steps the tile kernels can index with: a token's in 32 bits of bytes, tokens in 32 bits.
 bool small_steps(const RopeParams& p, int64_t es) {
   const int64_t most = std::max({p.q.in_t, p.q.out_t, p.q.x_t, p.k.in_t, p.k.out_t, p.k.x_t});
@@ -702,11 +724,11 @@ void launch_back(RopeParams p, cudaStream_t st) {
   p.lanes = kThreads / p.width;
   const int64_t entries = (int64_t)p.tables * p.pairs;
   auto bytes = [&](int64_t tile) { return Tile<VP>::bytes(entries, p.axes, (int64_t)p.tables * heads, tile); };
-  const int64_t spread = (p.tokens + p.blocks - 1) / p.blocks, fit = 32 * 1024 / (entries * 8);
-  p.tile = (int)std::max<int64_t>(1, std::min<int64_t>({spread, fit, 64}));
+  p.tile = tile_tokens(p.tokens, p.blocks, std::min<int64_t>(64, 32 * 1024 / (entries * 8)));
   if (bytes(p.tile) <= (size_t)kMaxTileBytes && small_steps(p, sizeof(T))) {
-    launch_kernel<rope_axes_back_kernel<T, VP, LAYOUT>>(
-        p, dim3((unsigned)p.blocks, (unsigned)((p.columns + p.width - 1) / p.width)), bytes(p.tile), st);
+    const dim3 grid((unsigned)p.blocks, (unsigned)((p.columns + p.width - 1) / p.width));
+    if (p.axes <= 2) launch_kernel<rope_axes_back_kernel<T, VP, LAYOUT, 2>>(p, grid, bytes(p.tile), st);
+    else launch_kernel<rope_axes_back_kernel<T, VP, LAYOUT, KC_ROPE_MAX_AXES>>(p, grid, bytes(p.tile), st);
   } else {  // before the gradients, which may take the place of what it reads
     launch_kernel<rope_freqs_direct_kernel<T, LAYOUT>>(
         p, dim3((unsigned)p.blocks, (unsigned)((entries + kThreads - 1) / kThreads)), 0, st);
@@ -722,9 +744,7 @@ void launch(RopeParams p, cudaStream_t st) {
   if (p.dfreqs) return launch_back<T, VP, LAYOUT>(p, st);
   const int64_t heads = p.q.per_table + p.k.per_table, cols = p.pairs / VP + p.rest / VP;
   const int64_t entries = (int64_t)p.tables * p.pairs;
-  // tiles of at most 32 KB of sines, not more tokens than leave every SM four blocks' work
-  const int64_t fit = 32 * 1024 / (entries * 8), spread = p.tokens / (kSms * 4);
-  p.tile = (int)std::max<int64_t>(1, std::min<int64_t>({fit, spread, 64}));
+  p.tile = tile_tokens(p.tokens, kSms * kTileBlocks, std::min<int64_t>(32, 32 * 1024 / (entries * 8)));
   p.rounds = (int)((heads + 1) / 2);
   const int64_t per_token = (int64_t)p.tables * p.rounds * cols;
   const size_t smem = Tile<VP>::bytes(entries, p.axes, p.tables * heads, p.tile);
@@ -738,7 +758,7 @@ void launch(RopeParams p, cudaStream_t st) {
   p.by_table = magic(p.rounds * cols);
   p.by_head = magic(cols);
   const int64_t tiles = (p.tokens + p.tile - 1) / p.tile;
-  launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT>>(p, dim3((unsigned)std::min<int64_t>(tiles, kSms * 8)), smem, st);
+  launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT>>(p, dim3((unsigned)std::min<int64_t>(tiles, kSms * kTileBlocks)), smem, st);
 }
 
 template <typename T, int VP>
