@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTiles = 64;
 constexpr int kMaxSmem = 227 * 1024;  // of a block
+constexpr int kSms = 148;
 
 struct NormParams {
   const void* x;
@@ -40,7 +41,9 @@ struct NormParams {
   float2* part;          // [n][tiles][channels]: forward (mean, M2), backward (S1, S2)
   int* part_n;           // [n][tiles] points on
   float2* coef;          // [n][groups]: forward (mean, rstd), backward (c1, c2)
-  float2* sums;          // [n][channels] backward (S1, S2) of a board
+  float2* sums;          // [rows][channels] backward (S1, S2): split path of a board, resident path of a block's boards
+  float* dweight;
+  float* dbias;
   int64_t xb, xr, yb, yr, mb;
   int n, points, C, G, cg, act;
   float eps;
@@ -125,6 +128,8 @@ struct ResShape {
   int R;       // rows at once
   int slots;   // vectors a thread has room for
   uint32_t vdiv;  // 2^20 / V + 1: (t * vdiv) >> 20 = t / V for t, V <= 512
+  int slot_bytes;  // backward: of all slots, and at least the channel sums'
+  int boards;  // blocks that share a chunk's boards
   int wvec;    // weight and bias may be read as 16-byte vectors
 };
 
@@ -266,8 +271,9 @@ __device__ __forceinline__ int small_div(int a, int b) { return (int)(((float)a 
 
 __host__ __device__ __forceinline__ size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 
+// What a block does for every board it takes: boards blockIdx.y, blockIdx.y + gridDim.y, ... of one chunk.
 struct ResIds {
-  int b, rank, c0, tx, ty, V;
+  int rank, c0, tx, ty, V;
   int r0, r1;  // the block's points; the thread's are r0 + ty + i R
   bool here;   // the thread has a column vector and rows
 };
@@ -275,46 +281,44 @@ struct ResIds {
 template <int VEC>
 __device__ __forceinline__ ResIds res_ids(const NormParams& p, const ResShape& s) {
   ResIds t;
-  t.b = blockIdx.z * 65535 + blockIdx.y;
   t.rank = blockIdx.x & (s.cs - 1);
   t.c0 = (blockIdx.x >> s.cs_log2) * s.cw;
   const int vfull = s.cw / VEC;
   t.V = min(s.cw, p.C - t.c0) / VEC;
   t.ty = (int)((threadIdx.x * s.vdiv) >> 20);
   t.tx = threadIdx.x - t.ty * vfull;
-  t.r0 = t.rank * s.rows;
+  t.r0 = min(p.points, t.rank * s.rows);
   t.r1 = min(p.points, t.r0 + s.rows);
   t.here = t.ty < s.R && t.tx < t.V;
   return t;
 }
 
-// on[y]: which points of row lane y are on, bit i being point r0 + y + i R. Ends with a barrier.
-__device__ __forceinline__ void on_bits(const NormParams& p, const ResShape& s, const ResIds& t, uint32_t* on) {
-  const int rows = t.r1 - t.r0;
-  if (!p.mask) {
-    for (int y = threadIdx.x; y < s.R; y += s.threads) {
-      const int k = y < rows ? small_div(rows - y + s.R - 1, s.R) : 0;
-      on[y] = k >= 32 ? 0xffffffffu : (1u << k) - 1;
-    }
-    __syncthreads();
-    return;
-  }
-  const float* m = p.mask + (int64_t)t.b * p.mb + t.r0;
-  for (int y = threadIdx.x; y < s.R; y += s.threads) on[y] = 0;
-  constexpr int N = 4;  // loads in flight
-  for (int r0 = threadIdx.x; r0 < rows + (int)threadIdx.x; r0 += N * s.threads) {
-    float v[N];
+// on[y]: which points of row lane y are on, bit i being point r0 + y + i R. The mask's values are loaded early (the
+// first MASKS a thread), set to bits between two barriers in words that were cleared before the first of them.
+constexpr int kMasks = 4;
+
+__device__ __forceinline__ void load_masks(const NormParams& p, const ResShape& s, const ResIds& t, int b,
+                                           float (&v)[kMasks]) {
+  const float* m = p.mask + (int64_t)b * p.mb + t.r0;
 #pragma unroll
-    for (int k = 0; k < N; k++) v[k] = r0 + k * s.threads < rows ? __ldg(m + r0 + k * s.threads) : 0.0f;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < N; k++)
-      if (v[k] != 0.0f) {
-        const int r = r0 + k * s.threads, i = small_div(r, s.R);
-        atomicOr(on + r - i * s.R, 1u << i);
-      }
+  for (int k = 0; k < kMasks; k++) {
+    const int r = threadIdx.x + k * s.threads;
+    v[k] = r < t.r1 - t.r0 ? __ldg(m + r) : 0.0f;
   }
-  __syncthreads();
+}
+
+__device__ __forceinline__ void set_bits(const NormParams& p, const ResShape& s, const ResIds& t, int b,
+                                         const float (&v)[kMasks], uint32_t* on) {
+  auto set = [&](int r) {
+    const int i = small_div(r, s.R);
+    atomicOr(on + r - i * s.R, 1u << i);
+  };
+#pragma unroll
+  for (int k = 0; k < kMasks; k++)
+    if (v[k] != 0.0f) set(threadIdx.x + k * s.threads);
+  const float* m = p.mask + (int64_t)b * p.mb + t.r0;
+  for (int r = threadIdx.x + kMasks * s.threads; r < t.r1 - t.r0; r += s.threads)
+    if (__ldg(m + r) != 0.0f) set(r);
 }
 
 // The bits of the points that there are in a row lane.
@@ -424,162 +428,188 @@ __device__ __forceinline__ float2 final_stats(float mean, float var, bool any, f
   return st;
 }
 
+// A block goes over its boards with two barriers each: the next board's rows are copied into the slots as soon as
+// the thread has written this one's, so that the copy runs under the other threads' work and the next mask is known
+// by then.
 template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constant__ NormParams p,
                                                             const __grid_constant__ ResShape sh) {
   using V = Vec<T, VEC>;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
-  if (t.b >= p.n) return;
   const int units = sh.cw / U;  // of a row of the chunk
-  const typename V::Raw* slot = reinterpret_cast<const typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
+  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg), all_groups = sh.cw / p.cg;
+  typename V::Raw* slots = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
   float2* part = reinterpret_cast<float2*>(norm_smem + round16((size_t)sh.slots * sh.threads * V::BYTES));
-  float2* mine = part + sh.R * units;  // the block's (mean, M2) of each group
-  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + sh.cw / p.cg);
-  int* cnt_block = reinterpret_cast<int*>(bits + sh.R);
+  float2* fin = part + sh.R * units;   // the groups' (mean, rstd)
+  float2* mine = fin + all_groups;     // [2][groups] the block's (mean, M2), of even and odd boards (cluster)
+  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + 2 * all_groups);  // [2][R]
+  int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);                // [2]
   const int col = t.c0 + t.tx * VEC;
-  on_bits(p, sh, t, bits);
-  const uint32_t on = t.here ? bits[t.ty] : 0;
-  copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)t.b * p.xb + (int64_t)(t.r0 + t.ty) * p.xr + col,
-                    (uint32_t)(sh.R * p.xr * sizeof(T)), on, const_cast<typename V::Raw*>(slot), V::BYTES);
-  f32x2 a[NP], bias[NP];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
+  const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
+  const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
+  const T* x = static_cast<const T*>(p.x) + (int64_t)(t.r0 + t.ty) * p.xr + col;
+  const uint32_t all = all_bits(sh, t);
+
+  float masks[kMasks];
+  for (int y = threadIdx.x; y < 2 * sh.R; y += sh.threads) bits[y] = 0;
+  if (p.mask) load_masks(p, sh, t, blockIdx.y, masks);
+  __syncthreads();
+  if (p.mask) {
+    set_bits(p, sh, t, blockIdx.y, masks, bits);
+  } else if (t.tx == 0 && t.ty < sh.R) {
+    bits[t.ty] = bits[sh.R + t.ty] = all;
+  }
+  __syncthreads();
+  uint32_t on = t.here ? bits[t.ty] : 0;
+  copy_rows<T, VEC>(x + (int64_t)blockIdx.y * p.xb, x_step, on, slots, V::BYTES);
+  f32x2 weight[NP], bias[NP];
   if (t.here) {
-    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, a);
+    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, weight);
     load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
   }
-  copies_done();
 
-  // the thread's shares, in one pass around a value of its first row: the squares around the mean are the squares
-  // around that value less its distance's, at most as many times larger as the share has values, since it is one of
-  // them
-  if (t.here) {
-    const int cnt = __popc(on);
-    f32x2 neg[NP], sum[NP], sq[NP];
-    float ref[NU];
-    {
-      f32x2 v[NP] = {};
-      if (on) V::unpack(slot[0], v);
+  int odd = 0;
+  for (int b = blockIdx.y; b < p.n; b += gridDim.y, odd ^= 1) {
+    const int next = b + gridDim.y;
+    const bool more = next < p.n;
+    const uint32_t* bits_now = bits + odd * sh.R;
+    uint32_t* bits_next = bits + (odd ^ 1) * sh.R;
+    if (p.mask && more) load_masks(p, sh, t, next, masks);
+    copies_done();
+
+    // the thread's shares, in one pass around a value of its first row: the squares around the mean are the squares
+    // around that value less its distance's, at most as many times larger as the share has values, since it is one
+    // of them
+    if (t.here) {
+      const int cnt = __popc(on);
+      f32x2 neg[NP], sum[NP], sq[NP];
+      float ref[NU];
+      {
+        f32x2 v[NP] = {};
+        if (on) V::unpack(slots[0], v);
 #pragma unroll
-      for (int u = 0; u < NU; u++) ref[u] = u * U % 2 ? v[u * U / 2].y : v[u * U / 2].x;
-    }
-#pragma unroll
-    for (int j = 0; j < NP; j++) {
-      neg[j] = {-ref[2 * j / U], VEC > 1 ? -ref[(2 * j + 1) / U] : 0.0f};
-      sum[j] = sq[j] = {0.0f, 0.0f};
-    }
-#pragma unroll 4
-    for (int k = 0; k < cnt; k++) {
-      f32x2 v[NP];
-      V::unpack(slot[k], v);
+        for (int u = 0; u < NU; u++) ref[u] = u * U % 2 ? v[u * U / 2].y : v[u * U / 2].x;
+      }
 #pragma unroll
       for (int j = 0; j < NP; j++) {
-        const f32x2 d = add2(v[j], neg[j]);
-        sum[j] = add2(sum[j], d);
-        sq[j] = fma2(d, d, sq[j]);
+        neg[j] = {-ref[2 * j / U], VEC > 1 ? -ref[(2 * j + 1) / U] : 0.0f};
+        sum[j] = sq[j] = {0.0f, 0.0f};
+      }
+#pragma unroll 4
+      for (int k = 0; k < cnt; k++) {
+        f32x2 v[NP];
+        V::unpack(slots[k], v);
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+          const f32x2 d = add2(v[j], neg[j]);
+          sum[j] = add2(sum[j], d);
+          sq[j] = fma2(d, d, sq[j]);
+        }
+      }
+      const float inv_n = cnt ? __fdividef(1.0f / U, (float)cnt) : 0.0f;
+      auto lane_of = [](const f32x2 (&v)[NP], int c) { return c % 2 ? v[c / 2].y : v[c / 2].x; };
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        float m = lane_of(sum, u * U), q = lane_of(sq, u * U);
+#pragma unroll
+        for (int j = 1; j < U; j++) {
+          m += lane_of(sum, u * U + j);
+          q += lane_of(sq, u * U + j);
+        }
+        const float d = m * inv_n;
+        q -= m * d;
+        part[t.ty * units + t.tx * NU + u] = make_float2(ref[u] + d, q < 0.0f ? 0.0f : q);
       }
     }
-    const float inv_n = cnt ? __fdividef(1.0f / U, (float)cnt) : 0.0f;
-    auto lane_of = [](const f32x2 (&v)[NP], int c) { return c % 2 ? v[c / 2].y : v[c / 2].x; };
-#pragma unroll
-    for (int u = 0; u < NU; u++) {
-      float m = lane_of(sum, u * U), q = lane_of(sq, u * U);
-#pragma unroll
-      for (int j = 1; j < U; j++) {
-        m += lane_of(sum, u * U + j);
-        q += lane_of(sq, u * U + j);
-      }
-      const float d = m * inv_n;
-      q -= m * d;
-      part[t.ty * units + t.tx * NU + u] = make_float2(ref[u] + d, q < 0.0f ? 0.0f : q);
-    }
-  }
-  __syncthreads();
+    if (p.mask)  // last read before the previous board's second barrier
+      for (int y = threadIdx.x; y < sh.R; y += sh.threads) bits_next[y] = 0;
+    __syncthreads();
 
-  // merged by group, a warp per group, around one share's mean: the correction by the mean's distance from it is at
-  // most as many times the result as there are shares, since that share is one of them
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
-  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg);
-  int rows_on = 0;
-  for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits[i]);
-  rows_on = __reduce_add_sync(0xffffffffu, rows_on);
-  int some = 0;  // a row lane with a point that is on
-  while (some < sh.R - 1 && !bits[some]) some++;
-  const float inv = rows_on ? __fdividef(1.0f, (float)rows_on * (float)p.cg) : 0.0f;
-  const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
-  float2* stats = p.stats ? p.stats + (int64_t)t.b * p.G + small_div(t.c0, p.cg) : nullptr;
-  for (int g = warp; g < groups; g += warps) {
-    const float2* gp = part + g * upg;
-    const float ref = gp[some * units].x;
-    float s = 0.0f, q = 0.0f;
-    for (int y = y0, u = u0; y < sh.R;) {
-      const float2 v = gp[y * units + u];
-      const float k = (float)(__popc(bits[y]) * U), d = v.x - ref;
-      if (k != 0.0f) {
-        s += k * d;
-        q += v.y + k * d * d;
+    // merged by group, a warp per group, around one share's mean: the correction by the mean's distance from it is
+    // at most as many times the result as there are shares, since that share is one of them
+    int rows_on = 0;
+    for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits_now[i]);
+    rows_on = __reduce_add_sync(0xffffffffu, rows_on);
+    int some = 0;  // a row lane with a point that is on
+    while (some < sh.R - 1 && !bits_now[some]) some++;
+    const float inv = rows_on ? __fdividef(1.0f, (float)rows_on * (float)p.cg) : 0.0f;
+    float2* stats = p.stats && t.rank == 0 ? p.stats + (int64_t)b * p.G + small_div(t.c0, p.cg) : nullptr;
+    float2* block_stats = mine + odd * all_groups;
+    for (int g = warp; g < groups; g += warps) {
+      const float2* gp = part + g * upg;
+      const float ref = gp[some * units].x;
+      float s = 0.0f, q = 0.0f;
+      for (int y = y0, u = u0; y < sh.R;) {
+        const float2 v = gp[y * units + u];
+        const float k = (float)(__popc(bits_now[y]) * U), d = v.x - ref;
+        if (k != 0.0f) {
+          s += k * d;
+          q += v.y + k * d * d;
+        }
+        y += dy;
+        u += du;
+        if (u >= upg) u -= upg, y++;
       }
-      y += dy;
-      u += du;
-      if (u >= upg) u -= upg, y++;
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      q += __shfl_xor_sync(0xffffffffu, q, o);
-    }
-    if (lane == 0) {
-      const float delta = s * inv;
-      q -= s * delta;
-      mine[g] = sh.cs == 1 ? final_stats(ref + delta, q * inv, rows_on, p.eps, stats, g)
-                           : make_float2(ref + delta, q < 0.0f ? 0.0f : q);
-    }
-  }
-  const float2* fin = mine;  // (mean, rstd)
-  __syncwarp();
-  if (sh.cs > 1) {
-    if (threadIdx.x == 0) *cnt_block = rows_on;
-    __syncwarp();
-    cluster_sync();
-    for (int g = threadIdx.x; g < groups; g += sh.threads) {
-      const float ref = mine[g].x;
-      float n = 0.0f, s = 0.0f, q = 0.0f;
-      for (int k = 0; k < sh.cs; k++) {
-        const float c = (float)ld_cluster(cnt_block, k);
-        n += c;
-        if (c != 0.0f) s += c * (ld_cluster(mine + g, k).x - ref);
+      for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        q += __shfl_xor_sync(0xffffffffu, q, o);
       }
-      const float delta = n != 0.0f ? s / n : 0.0f;
-      for (int k = 0; k < sh.cs; k++) {
-        const float c = (float)ld_cluster(cnt_block, k) * (float)p.cg;
-        const float2 v = ld_cluster(mine + g, k);
-        const float d = v.x - ref - delta;
-        if (c != 0.0f) q += v.y + c * d * d;
+      if (lane == 0) {
+        const float delta = s * inv;
+        q -= s * delta;
+        if (sh.cs == 1) fin[g] = final_stats(ref + delta, q * inv, rows_on, p.eps, stats, g);
+        else block_stats[g] = make_float2(ref + delta, q < 0.0f ? 0.0f : q);
       }
-      part[g] = final_stats(ref + delta, n != 0.0f ? q / (n * (float)p.cg) : 0.0f, n != 0.0f, p.eps,
-                            t.rank == 0 ? stats : nullptr, g);
     }
-    fin = part;
-  }
-  __syncthreads();
+    if (p.mask && more) set_bits(p, sh, t, next, masks, bits_next);
+    if (sh.cs > 1) {
+      if (threadIdx.x == 0) counts[odd] = rows_on;
+      __syncwarp();
+      cluster_sync();
+      for (int g = warp; g < groups; g += warps) {  // a lane per block of the cluster
+        const float c = lane < sh.cs ? (float)ld_cluster(counts + odd, lane) : 0.0f;
+        const float2 v = lane < sh.cs ? ld_cluster(block_stats + g, lane) : make_float2(0.0f, 0.0f);
+        const float ref = block_stats[g].x;
+        float n = c, s = c != 0.0f ? c * (v.x - ref) : 0.0f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+          n += __shfl_xor_sync(0xffffffffu, n, o);
+          s += __shfl_xor_sync(0xffffffffu, s, o);
+        }
+        const float delta = n != 0.0f ? s / n : 0.0f, d = v.x - ref - delta;
+        float q = c != 0.0f ? v.y + c * (float)p.cg * d * d : 0.0f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+        if (lane == 0)
+          fin[g] = final_stats(ref + delta, n != 0.0f ? q / (n * (float)p.cg) : 0.0f, n != 0.0f, p.eps, stats, g);
+      }
+    }
+    __syncthreads();
 
-  if (t.here) {
-    T* y = static_cast<T*>(p.y) + (int64_t)t.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col;
-    f32x2 neg[NP];
-    float2 st[NU];
+    const uint32_t on_next = t.here && more ? bits_next[t.ty] : 0;
+    if (t.here) {
+      T* y = static_cast<T*>(p.y) + (int64_t)b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col;
+      f32x2 neg[NP], a[NP];
+      float2 st[NU];
 #pragma unroll
-    for (int u = 0; u < NU; u++) st[u] = fin[small_div(t.tx * VEC + u * U, p.cg)];
+      for (int u = 0; u < NU; u++) st[u] = fin[small_div(t.tx * VEC + u * U, p.cg)];
 #pragma unroll
-    for (int j = 0; j < NP; j++) {
-      const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : lo;
-      neg[j] = {-lo.x, -hi.x};
-      a[j] = mul2(a[j], {lo.y, hi.y});
+      for (int j = 0; j < NP; j++) {
+        const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : lo;
+        neg[j] = {-lo.x, -hi.x};
+        a[j] = mul2(weight[j], {lo.y, hi.y});
+      }
+      if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(on, slots, y, y_step, neg, a, bias);
+      else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slots, y, y_step, neg, a, bias);
+      else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slots, y, y_step, neg, a, bias);
+      else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slots, y, y_step, neg, a, bias);
+      if (more) copy_rows<T, VEC>(x + (int64_t)next * p.xb, x_step, on_next, slots, V::BYTES);
+      zero_rows<T, VEC>(all & ~on, y, y_step);
     }
-    const uint32_t step = (uint32_t)(sh.R * p.yr * sizeof(T));
-    if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(on, slot, y, step, neg, a, bias);
-    else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slot, y, step, neg, a, bias);
-    else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slot, y, step, neg, a, bias);
-    else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slot, y, step, neg, a, bias);
-    zero_rows<T, VEC>(all_bits(sh, t) & ~on, y, step);
+    on = on_next;
   }
   if (sh.cs > 1) {  // a block's shared memory stays until the others have read it
     __syncwarp();
@@ -673,7 +703,8 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   using G = typename S::G;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
-  if (t.b >= p.n) return;
+  const int units = sh.cw / U;
+  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg), all_groups = sh.cw / p.cg, g0 = small_div(t.c0, p.cg);
   const size_t vectors = (size_t)sh.slots * sh.threads, plane = vectors * sizeof(typename G::Raw);
   unsigned char* planes = norm_smem + round16(vectors * V::BYTES);
   S slots;
@@ -681,157 +712,217 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
 #pragma unroll
   for (int h = 0; h < S::PLANES; h++)
     slots.g[h] = reinterpret_cast<typename G::Raw*>(planes + h * plane) + threadIdx.x * sh.slots;
-  float2* red = reinterpret_cast<float2*>(planes + S::PLANES * plane);  // [R][cw], then [parts][cw]
-  float2* mine = red + sh.R * sh.cw;  // the block's channel sums
-  float2* coef = mine + sh.cw;        // the groups' (c1, c2)
-  uint32_t* bits = reinterpret_cast<uint32_t*>(coef + sh.cw / p.cg);
-  int* cnt_block = reinterpret_cast<int*>(bits + sh.R);
-  const int col = t.c0 + t.tx * VEC, g0 = small_div(t.c0, p.cg);
-  const int64_t x_at = (int64_t)t.b * p.xb + (int64_t)(t.r0 + t.ty) * p.xr + col;
+  float2* red = reinterpret_cast<float2*>(norm_smem);  // [R][cw] channel sums, when the slots have served
+  float2* part = reinterpret_cast<float2*>(norm_smem + sh.slot_bytes);  // (ty, unit) sums of w gz, w gz xh
+  float2* coef = part + sh.R * units;  // the groups' (c1, c2)
+  float2* mine = coef + all_groups;    // [2][groups] the block's sums, of even and odd boards (cluster)
+  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + 2 * all_groups);
+  int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);
+  const int col = t.c0 + t.tx * VEC;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
+  const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
+  const int64_t x_at = (int64_t)(t.r0 + t.ty) * p.xr + col, y_at = (int64_t)(t.r0 + t.ty) * p.yr + col;
+  const uint32_t all = all_bits(sh, t);
+  auto copy_board = [&](int b, uint32_t on) {
+    copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x, V::BYTES);
+    copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)b * p.yb + y_at, y_step, on, slots.g[0],
+                      sizeof(typename G::Raw));
+  };
 
-  on_bits(p, sh, t, bits);
-  const uint32_t on = t.here ? bits[t.ty] : 0;
-  copy_rows<T, VEC>(static_cast<const T*>(p.x) + x_at, x_step, on, slots.x, V::BYTES);
-  copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)t.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col, y_step, on,
-                    slots.g[0], sizeof(typename G::Raw));
-  f32x2 w[NP], neg[NP], rstd[NP], s1[NP], s2[NP];
+  float masks[kMasks];
+  for (int y = threadIdx.x; y < 2 * sh.R; y += sh.threads) bits[y] = 0;
+  if (p.mask) load_masks(p, sh, t, blockIdx.y, masks);
+  __syncthreads();
+  if (p.mask) {
+    set_bits(p, sh, t, blockIdx.y, masks, bits);
+  } else if (t.tx == 0 && t.ty < sh.R) {
+    bits[t.ty] = bits[sh.R + t.ty] = all;
+  }
+  __syncthreads();
+  uint32_t on = t.here ? bits[t.ty] : 0;
+  copy_board(blockIdx.y, on);
+  f32x2 w[NP], bias[NP], sum1[NP], sum2[NP];  // sums over the block's boards
 #pragma unroll
-  for (int j = 0; j < NP; j++) s1[j] = s2[j] = {0.0f, 0.0f};
+  for (int j = 0; j < NP; j++) sum1[j] = sum2[j] = {0.0f, 0.0f};
   if (t.here) {
-    f32x2 bias[NP];
     load_params<VEC>(p.weight, 1.0f, sh.wvec, col, w);
     load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
     if (VEC == 1) w[0].y = 0.0f;
-    float2 st[NU];
-    const float2* stats = p.stats + (int64_t)t.b * p.G + g0;
-#pragma unroll
-    for (int u = 0; u < NU; u++) st[u] = stats[small_div(t.tx * VEC + u * U, p.cg)];
-#pragma unroll
-    for (int j = 0; j < NP; j++) {
-      const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : make_float2(0.0f, 0.0f);
-      neg[j] = {-lo.x, -hi.x};
-      rstd[j] = {lo.y, hi.y};
-    }
-    copies_done();
-    const int cnt = __popc(on);
-    if (p.act == KC_ACT_MISH) back_sums<T, VEC, KC_ACT_MISH>(slots, cnt, neg, rstd, w, bias, s1, s2);
-    else if (p.act == KC_ACT_SILU) back_sums<T, VEC, KC_ACT_SILU>(slots, cnt, neg, rstd, w, bias, s1, s2);
-    else if (p.act == KC_ACT_RELU) back_sums<T, VEC, KC_ACT_RELU>(slots, cnt, neg, rstd, w, bias, s1, s2);
-    else back_sums<T, VEC, KC_ACT_IDENTITY>(slots, cnt, neg, rstd, w, bias, s1, s2);
   }
+
+  int odd = 0;
+  for (int b = blockIdx.y; b < p.n; b += gridDim.y, odd ^= 1) {
+    const int next = b + gridDim.y;
+    const bool more = next < p.n;
+    const uint32_t* bits_now = bits + odd * sh.R;
+    uint32_t* bits_next = bits + (odd ^ 1) * sh.R;
+    if (p.mask && more) load_masks(p, sh, t, next, masks);
+    f32x2 neg[NP], rstd[NP];
+    if (t.here) {
+      const float2* stats = p.stats + (int64_t)b * p.G + g0;
+      float2 st[NU];
+#pragma unroll
+      for (int u = 0; u < NU; u++) st[u] = stats[small_div(t.tx * VEC + u * U, p.cg)];
+#pragma unroll
+      for (int j = 0; j < NP; j++) {
+        const float2 lo = st[2 * j / U], hi = VEC > 1 ? st[(2 * j + 1) / U] : make_float2(0.0f, 0.0f);
+        neg[j] = {-lo.x, -hi.x};
+        rstd[j] = {lo.y, hi.y};
+      }
+      copies_done();
+      f32x2 s1[NP], s2[NP];
+#pragma unroll
+      for (int j = 0; j < NP; j++) s1[j] = s2[j] = {0.0f, 0.0f};
+      const int cnt = __popc(on);
+      if (p.act == KC_ACT_MISH) back_sums<T, VEC, KC_ACT_MISH>(slots, cnt, neg, rstd, w, bias, s1, s2);
+      else if (p.act == KC_ACT_SILU) back_sums<T, VEC, KC_ACT_SILU>(slots, cnt, neg, rstd, w, bias, s1, s2);
+      else if (p.act == KC_ACT_RELU) back_sums<T, VEC, KC_ACT_RELU>(slots, cnt, neg, rstd, w, bias, s1, s2);
+      else back_sums<T, VEC, KC_ACT_IDENTITY>(slots, cnt, neg, rstd, w, bias, s1, s2);
+#pragma unroll
+      for (int j = 0; j < NP; j++) {
+        sum1[j] = add2(sum1[j], s1[j]);
+        sum2[j] = add2(sum2[j], s2[j]);
+        s1[j] = mul2(s1[j], w[j]);
+        s2[j] = mul2(s2[j], w[j]);
+      }
+      auto lane_of = [](const f32x2 (&v)[NP], int c) { return c % 2 ? v[c / 2].y : v[c / 2].x; };
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+          o.x += lane_of(s1, u * U + j);
+          o.y += lane_of(s2, u * U + j);
+        }
+        part[t.ty * units + t.tx * NU + u] = o;
+      }
+    }
+    if (p.mask)
+      for (int y = threadIdx.x; y < sh.R; y += sh.threads) bits_next[y] = 0;
+    __syncthreads();
+
+    // the groups' sums, a warp per group
+    int rows_on = 0;
+    for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits_now[i]);
+    rows_on = __reduce_add_sync(0xffffffffu, rows_on);
+    const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
+    float2* block_sums = mine + odd * all_groups;
+    for (int g = warp; g < groups; g += warps) {
+      const float2* gp = part + g * upg;
+      float c1 = 0.0f, c2 = 0.0f;
+      for (int y = y0, u = u0; y < sh.R;) {
+        const float2 v = gp[y * units + u];
+        c1 += v.x;
+        c2 += v.y;
+        y += dy;
+        u += du;
+        if (u >= upg) u -= upg, y++;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        c1 += __shfl_xor_sync(0xffffffffu, c1, o);
+        c2 += __shfl_xor_sync(0xffffffffu, c2, o);
+      }
+      if (lane == 0) {
+        if (sh.cs == 1) coef[g] = make_float2(c1 * inv, c2 * inv);
+        else block_sums[g] = make_float2(c1, c2);
+      }
+    }
+    if (p.mask && more) set_bits(p, sh, t, next, masks, bits_next);
+    if (sh.cs > 1) {
+      if (threadIdx.x == 0) counts[odd] = rows_on;
+      __syncwarp();
+      cluster_sync();
+      for (int g = warp; g < groups; g += warps) {  // a lane per block of the cluster
+        float n = lane < sh.cs ? (float)ld_cluster(counts + odd, lane) : 0.0f;
+        float2 c = lane < sh.cs ? ld_cluster(block_sums + g, lane) : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+          n += __shfl_xor_sync(0xffffffffu, n, o);
+          c.x += __shfl_xor_sync(0xffffffffu, c.x, o);
+          c.y += __shfl_xor_sync(0xffffffffu, c.y, o);
+        }
+        const float f = n != 0.0f ? 1.0f / (n * (float)p.cg) : 0.0f;
+        if (lane == 0) coef[g] = make_float2(c.x * f, c.y * f);
+      }
+    }
+    __syncthreads();
+
+    const uint32_t on_next = t.here && more ? bits_next[t.ty] : 0;
+    if (t.here) {
+      T* dx = static_cast<T*>(p.y) + (int64_t)b * p.xb + x_at;
+      f32x2 k1[NP], k2[NP], wr[NP];  // dx = gz (rstd w) - rstd c1 - xh (rstd c2)
+      float2 co[NU];
+#pragma unroll
+      for (int u = 0; u < NU; u++) co[u] = coef[small_div(t.tx * VEC + u * U, p.cg)];
+#pragma unroll
+      for (int j = 0; j < NP; j++) {
+        const float2 lo = co[2 * j / U], hi = VEC > 1 ? co[(2 * j + 1) / U] : lo;
+        wr[j] = mul2(w[j], rstd[j]);
+        k1[j] = mul2({-lo.x, -hi.x}, rstd[j]);
+        k2[j] = mul2({-lo.y, -hi.y}, rstd[j]);
+      }
+      S sl = slots;
+      each_on<2>(on, [&](const auto& i) {
+        constexpr int N = sizeof(i) / sizeof(int);
+        f32x2 o[N][NP], g[N][NP];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+          V::unpack(sl.x[k], o[k]);
+          sl.load_g(k, g[k]);
+        }
+        sl.next(N);
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+          for (int j = 0; j < NP; j++) {
+            const f32x2 xh = mul2(add2(o[k][j], neg[j]), rstd[j]);
+            o[k][j] = fma2(g[k][j], wr[j], fma2(xh, k2[j], k1[j]));
+          }
+#pragma unroll
+        for (int k = 0; k < N; k++) *reinterpret_cast<typename V::Raw*>(nth_row(dx, i[k], x_step)) = V::pack(o[k]);
+      });
+      if (more) copy_board(next, on_next);
+      zero_rows<T, VEC>(all & ~on, dx, x_step);
+    }
+    on = on_next;
+  }
+  if (sh.cs > 1) {
+    __syncwarp();
+    cluster_sync();
+  }
+  if (!p.sums) return;
+
+  // the channels' sums over the block's boards: rows ty by `parts` threads per channel, then those
+  __syncthreads();
   if (t.here) {
     float2* o = red + t.ty * sh.cw + t.tx * VEC;
 #pragma unroll
     for (int j = 0; j < NP; j++) {
-      o[2 * j] = make_float2(s1[j].x, s2[j].x);
-      if (VEC > 1) o[2 * j + 1] = make_float2(s1[j].y, s2[j].y);
+      o[2 * j] = make_float2(sum1[j].x, sum2[j].x);
+      if (VEC > 1) o[2 * j + 1] = make_float2(sum1[j].y, sum2[j].y);
     }
   }
   __syncthreads();
-
-  // channel sums: rows ty of `parts` threads per channel, then those
-  const int cw = t.V * VEC, warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
-  const int parts = max(1, small_div(sh.threads, sh.cw));
-  const int part = parts > 1 ? small_div(threadIdx.x, sh.cw) : 0;
-  for (int c = threadIdx.x - part * sh.cw; part < parts && c < cw; c += parts > 1 ? sh.cw : sh.threads) {
+  const int cw = t.V * VEC, parts = min(sh.R, max(1, small_div(sh.threads, sh.cw)));
+  const int mine_part = parts > 1 ? small_div(threadIdx.x, sh.cw) : 0;
+  for (int c = threadIdx.x - mine_part * sh.cw; mine_part < parts && c < cw; c += parts > 1 ? sh.cw : sh.threads) {
     float2 s = make_float2(0.0f, 0.0f);
-    for (int y = part; y < sh.R; y += parts) {
-      const float2 v = red[y * sh.cw + c];
-      s.x += v.x;
-      s.y += v.y;
+    for (int y = mine_part; y < sh.R; y += parts) {
+      s.x += red[y * sh.cw + c].x;
+      s.y += red[y * sh.cw + c].y;
     }
-    red[part * sh.cw + c] = s;  // row `part` of this column is this thread's alone
+    red[mine_part * sh.cw + c] = s;  // row `mine_part` of this column is this thread's alone
   }
-  int rows_on = 0;
-  for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits[i]);
-  rows_on = __reduce_add_sync(0xffffffffu, rows_on);
-  if (threadIdx.x == 0) *cnt_block = rows_on;
   __syncthreads();
-  const int used = min(parts, sh.R);
   for (int c = threadIdx.x; c < cw; c += sh.threads) {
     float2 s = red[c];
-    for (int k = 1; k < used; k++) {
+    for (int k = 1; k < parts; k++) {
       s.x += red[k * sh.cw + c].x;
       s.y += red[k * sh.cw + c].y;
     }
-    mine[c] = s;
-  }
-  float2* total = mine;
-  if (sh.cs > 1) {
-    __syncwarp();
-    cluster_sync();
-    total = red;
-    rows_on = 0;
-    for (int k = 0; k < sh.cs; k++) rows_on += ld_cluster(cnt_block, k);
-    for (int c = threadIdx.x; c < cw; c += sh.threads) {
-      float2 s = ld_cluster(mine + c, 0);
-      for (int k = 1; k < sh.cs; k++) {
-        const float2 v = ld_cluster(mine + c, k);
-        s.x += v.x;
-        s.y += v.y;
-      }
-      total[c] = s;
-    }
-  }
-  __syncthreads();
-  if (p.sums && t.rank == 0)
-    for (int c = threadIdx.x; c < cw; c += sh.threads) p.sums[(int64_t)t.b * p.C + t.c0 + c] = total[c];
-  const int groups = small_div(cw, p.cg);
-  const float inv = rows_on ? 1.0f / ((float)rows_on * (float)p.cg) : 0.0f;
-  for (int g = warp; g < groups; g += warps) {
-    float c1 = 0.0f, c2 = 0.0f;
-    for (int i = lane; i < p.cg; i += 32) {
-      const float wc = p.weight ? __ldg(p.weight + t.c0 + g * p.cg + i) : 1.0f;
-      const float2 s = total[g * p.cg + i];
-      c1 += wc * s.x;
-      c2 += wc * s.y;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      c1 += __shfl_xor_sync(0xffffffffu, c1, o);
-      c2 += __shfl_xor_sync(0xffffffffu, c2, o);
-    }
-    if (lane == 0) coef[g] = make_float2(c1 * inv, c2 * inv);
-  }
-  __syncthreads();
-
-  if (t.here) {
-    T* dx = static_cast<T*>(p.y) + x_at;
-    f32x2 k1[NP], k2[NP];  // dx = gz (rstd w) - rstd c1 - xh (rstd c2)
-    float2 co[NU];
-#pragma unroll
-    for (int u = 0; u < NU; u++) co[u] = coef[small_div(t.tx * VEC + u * U, p.cg)];
-#pragma unroll
-    for (int j = 0; j < NP; j++) {
-      const float2 lo = co[2 * j / U], hi = VEC > 1 ? co[(2 * j + 1) / U] : lo;
-      w[j] = mul2(w[j], rstd[j]);
-      k1[j] = mul2({-lo.x, -hi.x}, rstd[j]);
-      k2[j] = mul2({-lo.y, -hi.y}, rstd[j]);
-    }
-    each_on<2>(on, [&](const auto& i) {
-      constexpr int N = sizeof(i) / sizeof(int);
-      f32x2 o[N][NP], g[N][NP];
-#pragma unroll
-      for (int k = 0; k < N; k++) {
-        V::unpack(slots.x[k], o[k]);
-        slots.load_g(k, g[k]);
-      }
-      slots.next(N);
-#pragma unroll
-      for (int k = 0; k < N; k++)
-#pragma unroll
-        for (int j = 0; j < NP; j++) {
-          const f32x2 xh = mul2(add2(o[k][j], neg[j]), rstd[j]);
-          o[k][j] = fma2(g[k][j], w[j], fma2(xh, k2[j], k1[j]));
-        }
-#pragma unroll
-      for (int k = 0; k < N; k++) *reinterpret_cast<typename V::Raw*>(nth_row(dx, i[k], x_step)) = V::pack(o[k]);
-    });
-    zero_rows<T, VEC>(all_bits(sh, t) & ~on, dx, x_step);
-  }
-  if (sh.cs > 1) {
-    __syncwarp();
-    cluster_sync();
+    p.sums[((int64_t)blockIdx.y * sh.cs + t.rank) * p.C + t.c0 + c] = s;
   }
 }
 
@@ -1141,16 +1232,17 @@ __global__ void __launch_bounds__(kThreads) norm_tile_dx_kernel(const __grid_con
   }
 }
 
-// dbias, dweight [c] = the boards' sums in a fixed order: 32 channels a block, 8 board lanes each.
-__global__ void __launch_bounds__(kThreads) norm_boards_kernel(const float2* __restrict__ sums, int n, int C,
+// dbias, dweight [c] = the rows' sums in a fixed order and in 64 bits: 8 channels a block, 32 lanes of rows each.
+__global__ void __launch_bounds__(kThreads) norm_params_kernel(const float2* __restrict__ sums, int rows, int C,
                                                                float* __restrict__ dweight,
                                                                float* __restrict__ dbias) {
-  __shared__ double2 red[8][32];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x / 32;
-  const int c = blockIdx.x * 32 + tx;
+  __shared__ double2 red[32][8];
+  const int tx = threadIdx.x & 7, ty = threadIdx.x / 8;
+  const int c = blockIdx.x * 8 + tx;
   double2 s = make_double2(0.0, 0.0);
   if (c < C)
-    for (int b = ty; b < n; b += 8) {
+#pragma unroll 4
+    for (int b = ty; b < rows; b += 32) {
       const float2 u = sums[(int64_t)b * C + c];
       s.x += u.x;
       s.y += u.y;
@@ -1158,7 +1250,7 @@ __global__ void __launch_bounds__(kThreads) norm_boards_kernel(const float2* __r
   red[ty][tx] = s;
   __syncthreads();
   if (ty == 0 && c < C) {
-    for (int i = 1; i < 8; i++) {
+    for (int i = 1; i < 32; i++) {
       s.x += red[i][tx].x;
       s.y += red[i][tx].y;
     }
@@ -1210,11 +1302,13 @@ int lcm_of(int a, int b) {
   return (int)std::min<int64_t>((int64_t)a / x * b, 1 << 30);
 }
 
-// Shared memory of a block.
-size_t resident_smem(const ResShape& s, int vec, int unit, int es, int cg, bool backward) {
-  const size_t slots = (size_t)s.slots * s.threads, groups = s.cw / cg, ints = (s.R + 1) * sizeof(int);
-  if (!backward) return round16(slots * vec * es) + ((size_t)s.R * (s.cw / unit) + groups) * sizeof(float2) + ints;
-  return round16(slots * vec * es) + slots * vec * 4 + ((size_t)(s.R + 1) * s.cw + groups) * sizeof(float2) + ints;
+// Shared memory of a block; sets slot_bytes.
+size_t resident_smem(ResShape& s, int vec, int unit, int es, int cg, bool backward) {
+  const size_t slots = (size_t)s.slots * s.threads, groups = s.cw / cg;
+  size_t bytes = round16(slots * vec * es);
+  if (backward) bytes = round16(std::max(bytes + slots * vec * 4, (size_t)s.R * s.cw * sizeof(float2)));
+  s.slot_bytes = (int)bytes;
+  return bytes + ((size_t)s.R * (s.cw / unit) + 3 * groups) * sizeof(float2) + (2 * s.R + 2) * sizeof(int);
 }
 
 // Channels of a vector that are sure to lie in one group.
@@ -1247,14 +1341,22 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
   if (!ok) ok = fits(512, 8, kMaxSlots);
   if (!ok) return false;
   // few boards: spread one over more SMs
-  while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < 148) fits(s.threads, s.cs * 2, kMaxSlots);
+  while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < kSms) fits(s.threads, s.cs * 2, kMaxSlots);
   s.vdiv = (1u << 20) / (uint32_t)(s.cw / vec) + 1;
+  // blocks enough for every SM; the boards go evenly over them
+  const int64_t smem = resident_smem(s, vec, unit, es, cg, backward);
+  const int threads_sm = backward || (vec == 8 && unit == 1) ? 512 : 768;  // by registers
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(kMaxSmem / (smem + 1024), threads_sm / s.threads));
+  const int64_t most = std::max<int64_t>(1, kSms * per_sm / (chunks * s.cs));
+  const int64_t turns = (d.n + most - 1) / most;
+  s.boards = (int)std::min<int64_t>((d.n + turns - 1) / turns, 65535);
   s.cs_log2 = s.cs == 8 ? 3 : s.cs == 4 ? 2 : s.cs == 2 ? 1 : 0;
   return chunks * s.cs <= 0x7fffffff;
 }
 
 struct Layout {
   size_t part = 0, part_n = 0, coef = 0, sums = 0, total = 0;
+  bool resident = false;  // without the split path's parts
 };
 size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -1267,14 +1369,18 @@ Layout workspace_layout(const kc_group_norm_desc& d, bool backward) {
     at += round256(bytes);
     return here;
   };
-  if (backward) l.sums = take((size_t)d.n * d.channels * sizeof(float2));
-  l.total = at;
   // the split path's, unless the call is resident whatever its tensors' alignment
   bool resident = true;
+  int64_t rows = 0;
   for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2) {
     ResShape s;
-    if (d.channels % v == 0) resident = resident && resident_shape(d, v, backward, s);
+    if (d.channels % v != 0) continue;
+    if (resident_shape(d, v, backward, s)) rows = std::max<int64_t>(rows, (int64_t)s.boards * s.cs);
+    else resident = false, rows = std::max<int64_t>(rows, d.n);
   }
+  if (backward) l.sums = take((size_t)rows * d.channels * sizeof(float2));
+  l.total = at;
+  l.resident = resident;
   if (resident) return l;
   int tiles, tile_rows;
   split_shape(d, tiles, tile_rows);
@@ -1296,6 +1402,12 @@ int vec_of(const kc_group_norm_desc& d, std::initializer_list<const void*> ptrs)
     if (ok) return v;
   }
   return 1;
+}
+
+void launch_params(const NormParams& p, int rows, cudaStream_t st) {
+  if (!p.dweight && !p.dbias) return;
+  norm_params_kernel<<<(p.C + 7) / 8, kThreads, 0, st>>>(p.sums, rows, p.C, p.dweight, p.dbias);
+  KC_CUDA(cudaGetLastError());
 }
 
 template <typename T, int VEC>
@@ -1322,6 +1434,7 @@ void split_backward(const NormParams& p, cudaStream_t st) {
   KC_CUDA(cudaGetLastError());
   norm_tile_dx_kernel<T, VEC><<<grid, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
+  launch_params(p, p.n, st);
 }
 
 template <auto kernel>
@@ -1335,8 +1448,7 @@ void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaSt
     allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.C + s.cw - 1) / s.cw * s.cs), (unsigned)std::min(p.n, 65535),
-                     (unsigned)((p.n + 65534) / 65535));
+  cfg.gridDim = dim3((unsigned)((p.C + s.cw - 1) / s.cw * s.cs), (unsigned)s.boards);
   cfg.blockDim = dim3((unsigned)s.threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -1350,10 +1462,11 @@ void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaSt
 }
 
 template <typename T, int VEC, int U>
-void run_resident(const NormParams& p, const ResShape& s, bool backward, cudaStream_t st) {
+void run_resident(const NormParams& p, ResShape s, bool backward, cudaStream_t st) {
   const size_t smem = resident_smem(s, VEC, U, sizeof(T), p.cg, backward);
-  if (backward) launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, smem, st);
-  else launch_resident<norm_resident_kernel<T, VEC, U>>(p, s, smem, st);
+  if (!backward) return launch_resident<norm_resident_kernel<T, VEC, U>>(p, s, smem, st);
+  launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, smem, st);
+  launch_params(p, s.boards * s.cs, st);
 }
 
 template <typename T, int VEC>
@@ -1399,7 +1512,7 @@ void run(const kc_group_norm_desc& d, NormParams p, int vec, bool backward, void
   p.part = reinterpret_cast<float2*>(ws + l.part);
   p.part_n = reinterpret_cast<int*>(ws + l.part_n);
   p.coef = reinterpret_cast<float2*>(ws + l.coef);
-  p.sums = reinterpret_cast<float2*>(ws + l.sums);
+  p.sums = p.dweight || p.dbias || !l.resident ? reinterpret_cast<float2*>(ws + l.sums) : nullptr;
   if (d.dtype == KC_PRECISION_F32) run_type<float>(d, p, vec, backward, st);
   else if (d.dtype == KC_PRECISION_F16) run_type<__half>(d, p, vec, backward, st);
   else run_type<__nv_bfloat16>(d, p, vec, backward, st);
@@ -1528,12 +1641,8 @@ extern "C" int kc_group_norm_act_backward(const kc_group_norm_desc* desc, const 
     p.y = d_dx;
     p.dy = d_dy;
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(d_stats));
+    p.dweight = d_dweight;
+    p.dbias = d_dbias;
     run(d, p, vec_of(d, {d_x, d_dy, d_dx}), true, d_workspace, st);
-    if (d_dweight || d_dbias) {
-      const Layout l = workspace_layout(d, true);
-      norm_boards_kernel<<<(d.channels + 31) / 32, kThreads, 0, st>>>(
-          reinterpret_cast<const float2*>(static_cast<char*>(d_workspace) + l.sums), d.n, d.channels, d_dweight, d_dbias);
-      KC_CUDA(cudaGetLastError());
-    }
   });
 }
