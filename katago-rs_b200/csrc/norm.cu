@@ -113,12 +113,12 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 // The resident path: a chunk of whole groups (V column vectors of VEC channels) of one board is read once and stays
 // in the shared memory of a block, or of a cluster of blocks that share the board's points, until it is written. A
 // thread owns rows ty, ty + R, ... of its block's points at one column vector, R = threads / V; it copies those that
-// are on into its own run of `slots` (an odd number of vectors, so that 16-byte accesses of neighbouring threads hit
-// different banks) itself (cp.async), so that no barrier stands between the copy and the statistics.
+// are on into `slots` of its own (every threads-th vector of shared memory) itself (cp.async), so that no barrier
+// stands between the copy and the statistics.
 // U neighbouring channels of a vector lie in one group (VEC, 4 or 1 of them), so that a thread's statistics are
 // VEC / U triples of (count, mean, sum of squares around it).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kMaxSlots = 31;  // a thread's rows are bits of one word, and their number is odd
+constexpr int kMaxSlots = 32;  // a thread's rows are bits of one word
 
 struct ResShape {
   int cw;      // channels of a chunk (the last one of a row may have fewer)
@@ -215,49 +215,55 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// act of two elements. One reciprocal serves both: the divisors' product stays below 2^127 (mish: (e^40 + ..)^2;
-// silu: exp(-z) is held to 2^60, where z sigma(z) is below 2^-53).
-template <int ACT>
+// act of two elements.
+// mish = z f, f = tanh(log(1 + e)), e = exp(z). For float32 f = n / (n + 2), n = e^2 + 2 e, which keeps its digits
+// where f is small (e held to 2^60, where f is 1). For 2-byte results f = 1 - 2 / ((1 + e)^2 + 1): three instructions
+// less, no bound on e (at infinity the quotient is 0), and off by 2^-23 absolutely, far below the values' rounding but
+// for results below 2^-12.
+// silu = z / (1 + exp(-z)), 0 where exp(-z) overflows.
+template <typename T, int ACT>
 __device__ __forceinline__ f32x2 act2(f32x2 z) {
   if constexpr (ACT == KC_ACT_RELU) {
     return {z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y};
   } else if constexpr (ACT == KC_ACT_MISH) {
     const f32x2 t = mul2(z, {kLog2e, kLog2e});
-    const f32x2 e = {ex2(fminf(t.x, 20.0f * kLog2e)), ex2(fminf(t.y, 20.0f * kLog2e))};
-    const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
-    const f32x2 d = add2(n, {2.0f, 2.0f});
-    const float r = rcp(d.x * d.y);
-    return mul2(z, mul2(n, {d.y * r, d.x * r}));
+    if constexpr (sizeof(T) == 2) {
+      const f32x2 u = add2({ex2(t.x), ex2(t.y)}, {1.0f, 1.0f});
+      const f32x2 d = fma2(u, u, {1.0f, 1.0f});
+      return mul2(z, fma2({rcp(d.x), rcp(d.y)}, {-2.0f, -2.0f}, {1.0f, 1.0f}));
+    } else {
+      const f32x2 e = {ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))};
+      const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
+      const f32x2 d = add2(n, {2.0f, 2.0f});
+      return mul2(z, mul2(n, {rcp(d.x), rcp(d.y)}));
+    }
   } else if constexpr (ACT == KC_ACT_SILU) {
     const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
-    const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
-    const float r = rcp(d.x * d.y);
-    return mul2(z, {d.y * r, d.x * r});
+    const f32x2 d = add2({ex2(t.x), ex2(t.y)}, {1.0f, 1.0f});
+    return mul2(z, {rcp(d.x), rcp(d.y)});
   } else {
     return z;
   }
 }
 
 // act' of two elements (relu apart: relu_on).
-// mish = z n / d with e = exp(z), n = e^2 + 2 e, d = n + 2: mish' = n / d + z 4 e (e + 1) / d^2 (above 20: 1).
-// silu' = s (1 + z (1 - s)), s = 1 / (1 + exp(-z)).
+// mish = z n / d with e = exp(z), n = e^2 + 2 e, d = n + 2: mish' = n / d + z 4 e (e + 1) / d^2 (e held to 2^60).
+// silu' = s (1 + z (1 - s)), s = 1 / (1 + exp(-z)), exp(-z) held to 2^60.
 template <int ACT>
 __device__ __forceinline__ f32x2 slope2(f32x2 z) {
   if constexpr (ACT == KC_ACT_MISH) {
     const f32x2 t = mul2(z, {kLog2e, kLog2e});
-    const f32x2 e = {ex2(fminf(t.x, 20.0f * kLog2e)), ex2(fminf(t.y, 20.0f * kLog2e))};
+    const f32x2 e = {ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))};
     const f32x2 n = mul2(e, add2(e, {2.0f, 2.0f}));
     const f32x2 d = add2(n, {2.0f, 2.0f});
-    const float r = rcp(d.x * d.y);
-    const f32x2 rd = {d.y * r, d.x * r};
+    const f32x2 rd = {rcp(d.x), rcp(d.y)};
     const f32x2 er = mul2(e, rd);                                 // e / d
     const f32x2 k = mul2({4.0f, 4.0f}, mul2(er, add2(er, rd)));   // 4 e (e + 1) / d^2
     return fma2(z, k, mul2(n, rd));
   } else if constexpr (ACT == KC_ACT_SILU) {
     const f32x2 t = mul2(z, {-kLog2e, -kLog2e});
     const f32x2 d = add2({ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))}, {1.0f, 1.0f});
-    const float r = rcp(d.x * d.y);
-    const f32x2 s = {d.y * r, d.x * r};
+    const f32x2 s = {rcp(d.x), rcp(d.y)};
     const f32x2 u = fma2({-s.x, -s.y}, z, z);                     // z (1 - s)
     return fma2(s, u, s);
   } else {
@@ -267,7 +273,9 @@ __device__ __forceinline__ f32x2 slope2(f32x2 z) {
 
 // a / b of non-negative integers, a < 2^19: (a + 1/2) / b is at least 1 / (2 b) from a whole number, the fast divide
 // off by at most 2^-21 of it.
-__device__ __forceinline__ int small_div(int a, int b) { return (int)(((float)a + 0.5f) / (float)b); }
+__device__ __forceinline__ int small_div(int a, int b) {
+  return (int)__fdividef((float)a + 0.5f, (float)b);
+}
 
 __host__ __device__ __forceinline__ size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 
@@ -388,7 +396,7 @@ __device__ __forceinline__ void load_params(const float* w, float other, bool ve
 }
 
 template <typename T, int VEC, int ACT>
-__device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VEC>::Raw* slot, T* y, uint32_t step,
+__device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VEC>::Raw* slot, int slot_step, T* y, uint32_t step,
                                            const f32x2 (&neg_mean)[Vec<T, VEC>::NP], const f32x2 (&a)[Vec<T, VEC>::NP],
                                            const f32x2 (&b)[Vec<T, VEC>::NP]) {
   using V = Vec<T, VEC>;
@@ -396,12 +404,11 @@ __device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VE
     constexpr int N = sizeof(i) / sizeof(int);
     f32x2 v[N][V::NP];
 #pragma unroll
-    for (int k = 0; k < N; k++) V::unpack(slot[k], v[k]);
-    slot += N;
+    for (int k = 0; k < N; k++, slot += slot_step) V::unpack(*slot, v[k]);
 #pragma unroll
     for (int k = 0; k < N; k++)
 #pragma unroll
-      for (int j = 0; j < V::NP; j++) v[k][j] = act2<ACT>(fma2(add2(v[k][j], neg_mean[j]), a[j], b[j]));
+      for (int j = 0; j < V::NP; j++) v[k][j] = act2<T, ACT>(fma2(add2(v[k][j], neg_mean[j]), a[j], b[j]));
 #pragma unroll
     for (int k = 0; k < N; k++) *reinterpret_cast<typename V::Raw*>(nth_row(y, i[k], step)) = V::pack(v[k]);
   });
@@ -439,11 +446,11 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   const ResIds t = res_ids<VEC>(p, sh);
   const int units = sh.cw / U;  // of a row of the chunk
   const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg), all_groups = sh.cw / p.cg;
-  typename V::Raw* slots = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
+  typename V::Raw* slots = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;  // every threads-th
   float2* part = reinterpret_cast<float2*>(norm_smem + round16((size_t)sh.slots * sh.threads * V::BYTES));
   float2* fin = part + sh.R * units;   // the groups' (mean, rstd)
   float2* mine = fin + all_groups;     // [2][groups] the block's (mean, M2), of even and odd boards (cluster)
-  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + 2 * all_groups);  // [2][R]
+  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + (sh.cs > 1 ? 2 * all_groups : 0));  // [2][R]
   int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);                // [2]
   const int col = t.c0 + t.tx * VEC;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
@@ -463,7 +470,7 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
   }
   __syncthreads();
   uint32_t on = t.here ? bits[t.ty] : 0;
-  copy_rows<T, VEC>(x + (int64_t)blockIdx.y * p.xb, x_step, on, slots, V::BYTES);
+  copy_rows<T, VEC>(x + (int64_t)blockIdx.y * p.xb, x_step, on, slots, sh.threads * V::BYTES);
   f32x2 weight[NP], bias[NP];
   if (t.here) {
     load_params<VEC>(p.weight, 1.0f, sh.wvec, col, weight);
@@ -497,10 +504,11 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
         neg[j] = {-ref[2 * j / U], VEC > 1 ? -ref[(2 * j + 1) / U] : 0.0f};
         sum[j] = sq[j] = {0.0f, 0.0f};
       }
+      const typename V::Raw* slot = slots;
 #pragma unroll 4
-      for (int k = 0; k < cnt; k++) {
+      for (int k = 0; k < cnt; k++, slot += sh.threads) {
         f32x2 v[NP];
-        V::unpack(slots[k], v);
+        V::unpack(*slot, v);
 #pragma unroll
         for (int j = 0; j < NP; j++) {
           const f32x2 d = add2(v[j], neg[j]);
@@ -602,11 +610,11 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
         neg[j] = {-lo.x, -hi.x};
         a[j] = mul2(weight[j], {lo.y, hi.y});
       }
-      if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(on, slots, y, y_step, neg, a, bias);
-      else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slots, y, y_step, neg, a, bias);
-      else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slots, y, y_step, neg, a, bias);
-      else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slots, y, y_step, neg, a, bias);
-      if (more) copy_rows<T, VEC>(x + (int64_t)next * p.xb, x_step, on_next, slots, V::BYTES);
+      if (p.act == KC_ACT_MISH) apply_rows<T, VEC, KC_ACT_MISH>(on, slots, sh.threads, y, y_step, neg, a, bias);
+      else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slots, sh.threads, y, y_step, neg, a, bias);
+      else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slots, sh.threads, y, y_step, neg, a, bias);
+      else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slots, sh.threads, y, y_step, neg, a, bias);
+      if (more) copy_rows<T, VEC>(x + (int64_t)next * p.xb, x_step, on_next, slots, sh.threads * V::BYTES);
       zero_rows<T, VEC>(all & ~on, y, y_step);
     }
     on = on_next;
@@ -628,10 +636,11 @@ struct BackSlots {
   static_assert(sizeof(typename V::Raw) <= sizeof(typename G::Raw), "dy waits in the first plane of gz");
   typename V::Raw* x;
   typename G::Raw* g[PLANES];
+  int step;
   __device__ __forceinline__ void next(int n) {
-    x += n;
+    x += n * step;
 #pragma unroll
-    for (int h = 0; h < PLANES; h++) g[h] += n;
+    for (int h = 0; h < PLANES; h++) g[h] += n * step;
   }
   __device__ __forceinline__ void store_g(int k, const f32x2 (&v)[V::NP]) {
 #pragma unroll
@@ -639,14 +648,14 @@ struct BackSlots {
       f32x2 o[G::NP];
 #pragma unroll
       for (int j = 0; j < G::NP; j++) o[j] = v[h * G::NP + j];
-      g[h][k] = G::pack(o);
+      g[h][k * step] = G::pack(o);
     }
   }
   __device__ __forceinline__ void load_g(int k, f32x2 (&v)[V::NP]) const {
 #pragma unroll
     for (int h = 0; h < PLANES; h++) {
       f32x2 o[G::NP];
-      G::unpack(g[h][k], o);
+      G::unpack(g[h][k * step], o);
 #pragma unroll
       for (int j = 0; j < G::NP; j++) v[h * G::NP + j] = o[j];
     }
@@ -662,8 +671,8 @@ __device__ __forceinline__ void back_rows(BackSlots<T, VEC>& sl, const f32x2 (&n
   f32x2 x[N][V::NP], g[N][V::NP];
 #pragma unroll
   for (int k = 0; k < N; k++) {
-    V::unpack(sl.x[k], x[k]);
-    V::unpack(*reinterpret_cast<const typename V::Raw*>(sl.g[0] + k), g[k]);
+    V::unpack(sl.x[k * sl.step], x[k]);
+    V::unpack(*reinterpret_cast<const typename V::Raw*>(sl.g[0] + k * sl.step), g[k]);
   }
 #pragma unroll
   for (int k = 0; k < N; k++)
@@ -708,15 +717,16 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   const size_t vectors = (size_t)sh.slots * sh.threads, plane = vectors * sizeof(typename G::Raw);
   unsigned char* planes = norm_smem + round16(vectors * V::BYTES);
   S slots;
-  slots.x = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x * sh.slots;
+  slots.x = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;
+  slots.step = sh.threads;
 #pragma unroll
   for (int h = 0; h < S::PLANES; h++)
-    slots.g[h] = reinterpret_cast<typename G::Raw*>(planes + h * plane) + threadIdx.x * sh.slots;
+    slots.g[h] = reinterpret_cast<typename G::Raw*>(planes + h * plane) + threadIdx.x;
   float2* red = reinterpret_cast<float2*>(norm_smem);  // [R][cw] channel sums, when the slots have served
   float2* part = reinterpret_cast<float2*>(norm_smem + sh.slot_bytes);  // (ty, unit) sums of w gz, w gz xh
   float2* coef = part + sh.R * units;  // the groups' (c1, c2)
   float2* mine = coef + all_groups;    // [2][groups] the block's sums, of even and odd boards (cluster)
-  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + 2 * all_groups);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(mine + (sh.cs > 1 ? 2 * all_groups : 0));
   int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);
   const int col = t.c0 + t.tx * VEC;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
@@ -725,9 +735,9 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   const int64_t x_at = (int64_t)(t.r0 + t.ty) * p.xr + col, y_at = (int64_t)(t.r0 + t.ty) * p.yr + col;
   const uint32_t all = all_bits(sh, t);
   auto copy_board = [&](int b, uint32_t on) {
-    copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x, V::BYTES);
+    copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x, sh.threads * V::BYTES);
     copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)b * p.yb + y_at, y_step, on, slots.g[0],
-                      sizeof(typename G::Raw));
+                      sh.threads * (int)sizeof(typename G::Raw));
   };
 
   float masks[kMasks];
@@ -869,7 +879,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
         f32x2 o[N][NP], g[N][NP];
 #pragma unroll
         for (int k = 0; k < N; k++) {
-          V::unpack(sl.x[k], o[k]);
+          V::unpack(sl.x[k * sl.step], o[k]);
           sl.load_g(k, g[k]);
         }
         sl.next(N);
@@ -1308,7 +1318,7 @@ size_t resident_smem(ResShape& s, int vec, int unit, int es, int cg, bool backwa
   size_t bytes = round16(slots * vec * es);
   if (backward) bytes = round16(std::max(bytes + slots * vec * 4, (size_t)s.R * s.cw * sizeof(float2)));
   s.slot_bytes = (int)bytes;
-  return bytes + ((size_t)s.R * (s.cw / unit) + 3 * groups) * sizeof(float2) + (2 * s.R + 2) * sizeof(int);
+  return bytes + ((size_t)s.R * (s.cw / unit) + (s.cs > 1 ? 3 : 1) * groups) * sizeof(float2) + (2 * s.R + 2) * sizeof(int);
 }
 
 // Channels of a vector that are sure to lie in one group.
@@ -1331,12 +1341,12 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
     if (s.cw / vec > threads) return false;
     s.R = threads / (s.cw / vec);
     s.rows = (d.points + cs - 1) / cs;
-    s.slots = ((s.rows + s.R - 1) / s.R) | 1;
+    s.slots = (s.rows + s.R - 1) / s.R;
     const int64_t step = std::max(d.x_row_stride, d.y_row_stride) * s.R * es;  // nth_row's
     return step <= 0xffffffffll && s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
   };
   bool ok = false;
-  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 19);
+  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 18);
   for (int cs = 2; cs <= 8 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots);
   if (!ok) ok = fits(512, 8, kMaxSlots);
   if (!ok) return false;
@@ -1445,6 +1455,8 @@ void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaSt
   if (dev >= 128) bad("device index above 127");
   if (!(allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1)) {
     KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    // all of an SM's shared memory: the blocks that resident_shape counts on start together
+    KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
