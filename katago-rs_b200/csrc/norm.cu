@@ -129,7 +129,9 @@ struct ResShape {
   int slots;   // vectors a thread has room for
   uint32_t vdiv;  // 2^20 / V + 1: (t * vdiv) >> 20 = t / V for t, V <= 512
   int slot_bytes;  // backward: of all slots, and at least the channel sums'
-  int boards;  // blocks that share a chunk's boards
+  int boards;  // backward: blocks that share a chunk's boards
+  int chunks;  // of a board
+  int blocks, step_boards, step_chunks;  // forward: blocks (clusters), and their distance in boards and chunks
   int wvec;    // weight and bias may be read as 16-byte vectors
 };
 
@@ -279,27 +281,44 @@ __device__ __forceinline__ int small_div(int a, int b) {
 
 __host__ __device__ __forceinline__ size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 
-// What a block does for every board it takes: boards blockIdx.y, blockIdx.y + gridDim.y, ... of one chunk.
+// A thread's place in its block, for every chunk of every board.
 struct ResIds {
-  int rank, c0, tx, ty, V;
+  int rank, tx, ty;
   int r0, r1;  // the block's points; the thread's are r0 + ty + i R
-  bool here;   // the thread has a column vector and rows
 };
 
 template <int VEC>
 __device__ __forceinline__ ResIds res_ids(const NormParams& p, const ResShape& s) {
   ResIds t;
   t.rank = blockIdx.x & (s.cs - 1);
-  t.c0 = (blockIdx.x >> s.cs_log2) * s.cw;
-  const int vfull = s.cw / VEC;
-  t.V = min(s.cw, p.C - t.c0) / VEC;
   t.ty = (int)((threadIdx.x * s.vdiv) >> 20);
-  t.tx = threadIdx.x - t.ty * vfull;
+  t.tx = threadIdx.x - t.ty * (s.cw / VEC);
   t.r0 = min(p.points, t.rank * s.rows);
   t.r1 = min(p.points, t.r0 + s.rows);
-  t.here = t.ty < s.R && t.tx < t.V;
   return t;
 }
+
+// A chunk of a board.
+struct Chunk {
+  int b, index, c0;
+  int cw;         // its channels (the last one of a row may have fewer)
+  int col;        // the thread's first channel
+  bool here;      // the thread has a column vector and rows
+  uint32_t all;   // the points that there are in its row lane
+
+  template <int VEC>
+  __device__ __forceinline__ void set(const NormParams& p, const ResShape& s, const ResIds& t, int board, int chunk) {
+    b = board;
+    index = chunk;
+    c0 = chunk * s.cw;
+    cw = min(s.cw, p.C - c0);
+    col = c0 + t.tx * VEC;
+    here = t.ty < s.R && t.tx * VEC < cw;
+    const int left = t.r1 - t.r0 - t.ty;
+    const int k = here && left > 0 ? small_div(left + s.R - 1, s.R) : 0;
+    all = k >= 32 ? 0xffffffffu : (1u << k) - 1;
+  }
+};
 
 // on[y]: which points of row lane y are on, bit i being point r0 + y + i R. The mask's values are loaded early (the
 // first MASKS a thread), set to bits between two barriers in words that were cleared before the first of them.
@@ -327,13 +346,6 @@ __device__ __forceinline__ void set_bits(const NormParams& p, const ResShape& s,
   const float* m = p.mask + (int64_t)b * p.mb + t.r0;
   for (int r = threadIdx.x + kMasks * s.threads; r < t.r1 - t.r0; r += s.threads)
     if (__ldg(m + r) != 0.0f) set(r);
-}
-
-// The bits of the points that there are in a row lane.
-__device__ __forceinline__ uint32_t all_bits(const ResShape& s, const ResIds& t) {
-  const int left = t.r1 - t.r0 - t.ty;
-  const int k = t.here && left > 0 ? small_div(left + s.R - 1, s.R) : 0;
-  return k >= 32 ? 0xffffffffu : (1u << k) - 1;
 }
 
 // Rows of a tensor as the thread meets them: its i-th point is i * step bytes behind its first one (the host sees to
@@ -435,61 +447,68 @@ __device__ __forceinline__ float2 final_stats(float mean, float var, bool any, f
   return st;
 }
 
-// A block goes over its boards with two barriers each: the next board's rows are copied into the slots as soon as
-// the thread has written this one's, so that the copy runs under the other threads' work and the next mask is known
-// by then.
-template <typename T, int VEC, int U>
-__global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constant__ NormParams p,
+// A block goes over chunks of boards, gridDim.x / cs apart in the order of memory, with two barriers each: the next
+// chunk's rows are copied into the slots as soon as the thread has written this one's, so that the copy runs under the
+// other threads' work and the next mask is known by then.
+template <typename T, int VEC, int U, int THREADS>  // THREADS: at most; blocks of 128 run five to an SM
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 5 : 1) norm_resident_kernel(const __grid_constant__ NormParams p,
                                                             const __grid_constant__ ResShape sh) {
   using V = Vec<T, VEC>;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
   const int units = sh.cw / U;  // of a row of the chunk
-  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg), all_groups = sh.cw / p.cg;
+  const int upg = p.cg / U, all_groups = sh.cw / p.cg;
   typename V::Raw* slots = reinterpret_cast<typename V::Raw*>(norm_smem) + threadIdx.x;  // every threads-th
   float2* part = reinterpret_cast<float2*>(norm_smem + round16((size_t)sh.slots * sh.threads * V::BYTES));
   float2* fin = part + sh.R * units;   // the groups' (mean, rstd)
-  float2* mine = fin + all_groups;     // [2][groups] the block's (mean, M2), of even and odd boards (cluster)
+  float2* mine = fin + all_groups;     // [2][groups] the block's (mean, M2), of even and odd turns (cluster)
   uint32_t* bits = reinterpret_cast<uint32_t*>(mine + (sh.cs > 1 ? 2 * all_groups : 0));  // [2][R]
   int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);                // [2]
-  const int col = t.c0 + t.tx * VEC;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
   const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
-  const T* x = static_cast<const T*>(p.x) + (int64_t)(t.r0 + t.ty) * p.xr + col;
-  const uint32_t all = all_bits(sh, t);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)(t.r0 + t.ty) * p.xr;
+  Chunk now, next;
+  {
+    const int first = blockIdx.x >> sh.cs_log2;
+    now.set<VEC>(p, sh, t, first / sh.chunks, first % sh.chunks);
+  }
 
   float masks[kMasks];
   for (int y = threadIdx.x; y < 2 * sh.R; y += sh.threads) bits[y] = 0;
-  if (p.mask) load_masks(p, sh, t, blockIdx.y, masks);
+  if (p.mask) load_masks(p, sh, t, now.b, masks);
   __syncthreads();
   if (p.mask) {
-    set_bits(p, sh, t, blockIdx.y, masks, bits);
+    set_bits(p, sh, t, now.b, masks, bits);
   } else if (t.tx == 0 && t.ty < sh.R) {
-    bits[t.ty] = bits[sh.R + t.ty] = all;
+    bits[t.ty] = bits[sh.R + t.ty] = now.all;
   }
   __syncthreads();
-  uint32_t on = t.here ? bits[t.ty] : 0;
-  copy_rows<T, VEC>(x + (int64_t)blockIdx.y * p.xb, x_step, on, slots, sh.threads * V::BYTES);
+  uint32_t on = now.here ? bits[t.ty] : 0;
+  copy_rows<T, VEC>(x + (int64_t)now.b * p.xb + now.col, x_step, on, slots, sh.threads * V::BYTES);
   f32x2 weight[NP], bias[NP];
-  if (t.here) {
-    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, weight);
-    load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
-  }
+  int loaded = -1;  // the chunk whose weight and bias they are
 
-  int odd = 0;
-  for (int b = blockIdx.y; b < p.n; b += gridDim.y, odd ^= 1) {
-    const int next = b + gridDim.y;
-    const bool more = next < p.n;
+  for (int odd = 0;; odd ^= 1) {
+    int next_b = now.b + sh.step_boards, next_c = now.index + sh.step_chunks;
+    if (next_c >= sh.chunks) next_c -= sh.chunks, next_b++;
+    const bool more = next_b < p.n;
+    if (more) next.set<VEC>(p, sh, t, next_b, next_c);
+    const int groups = small_div(now.cw, p.cg);
     const uint32_t* bits_now = bits + odd * sh.R;
     uint32_t* bits_next = bits + (odd ^ 1) * sh.R;
-    if (p.mask && more) load_masks(p, sh, t, next, masks);
+    if (p.mask && more) load_masks(p, sh, t, next.b, masks);
+    if (loaded != now.index && now.here) {
+      load_params<VEC>(p.weight, 1.0f, sh.wvec, now.col, weight);
+      load_params<VEC>(p.bias, 0.0f, sh.wvec, now.col, bias);
+    }
+    loaded = now.index;
     copies_done();
 
     // the thread's shares, in one pass around a value of its first row: the squares around the mean are the squares
     // around that value less its distance's, at most as many times larger as the share has values, since it is one
     // of them
-    if (t.here) {
+    if (now.here) {
       const int cnt = __popc(on);
       f32x2 neg[NP], sum[NP], sq[NP];
       float ref[NU];
@@ -543,7 +562,7 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
     int some = 0;  // a row lane with a point that is on
     while (some < sh.R - 1 && !bits_now[some]) some++;
     const float inv = rows_on ? __fdividef(1.0f, (float)rows_on * (float)p.cg) : 0.0f;
-    float2* stats = p.stats && t.rank == 0 ? p.stats + (int64_t)b * p.G + small_div(t.c0, p.cg) : nullptr;
+    float2* stats = p.stats && t.rank == 0 ? p.stats + (int64_t)now.b * p.G + small_div(now.c0, p.cg) : nullptr;
     float2* block_stats = mine + odd * all_groups;
     for (int g = warp; g < groups; g += warps) {
       const float2* gp = part + g * upg;
@@ -572,7 +591,7 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
         else block_stats[g] = make_float2(ref + delta, q < 0.0f ? 0.0f : q);
       }
     }
-    if (p.mask && more) set_bits(p, sh, t, next, masks, bits_next);
+    if (p.mask && more) set_bits(p, sh, t, next.b, masks, bits_next);
     if (sh.cs > 1) {
       if (threadIdx.x == 0) counts[odd] = rows_on;
       __syncwarp();
@@ -583,23 +602,22 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
         const float ref = block_stats[g].x;
         float n = c, s = c != 0.0f ? c * (v.x - ref) : 0.0f;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
+        for (int o = 8; o > 0; o >>= 1) {
           n += __shfl_xor_sync(0xffffffffu, n, o);
           s += __shfl_xor_sync(0xffffffffu, s, o);
         }
         const float delta = n != 0.0f ? s / n : 0.0f, d = v.x - ref - delta;
         float q = c != 0.0f ? v.y + c * (float)p.cg * d * d : 0.0f;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+        for (int o = 8; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
         if (lane == 0)
           fin[g] = final_stats(ref + delta, n != 0.0f ? q / (n * (float)p.cg) : 0.0f, n != 0.0f, p.eps, stats, g);
       }
     }
     __syncthreads();
 
-    const uint32_t on_next = t.here && more ? bits_next[t.ty] : 0;
-    if (t.here) {
-      T* y = static_cast<T*>(p.y) + (int64_t)b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + col;
+    if (now.here) {
+      T* y = static_cast<T*>(p.y) + (int64_t)now.b * p.yb + (int64_t)(t.r0 + t.ty) * p.yr + now.col;
       f32x2 neg[NP], a[NP];
       float2 st[NU];
 #pragma unroll
@@ -614,10 +632,18 @@ __global__ void __launch_bounds__(512) norm_resident_kernel(const __grid_constan
       else if (p.act == KC_ACT_SILU) apply_rows<T, VEC, KC_ACT_SILU>(on, slots, sh.threads, y, y_step, neg, a, bias);
       else if (p.act == KC_ACT_RELU) apply_rows<T, VEC, KC_ACT_RELU>(on, slots, sh.threads, y, y_step, neg, a, bias);
       else apply_rows<T, VEC, KC_ACT_IDENTITY>(on, slots, sh.threads, y, y_step, neg, a, bias);
-      if (more) copy_rows<T, VEC>(x + (int64_t)next * p.xb, x_step, on_next, slots, sh.threads * V::BYTES);
-      zero_rows<T, VEC>(all & ~on, y, y_step);
+      // the slots have served; the zeros of the rows that are off can wait
+      if (more) {
+        const uint32_t on_next = next.here ? bits_next[t.ty] : 0;
+        copy_rows<T, VEC>(x + (int64_t)next.b * p.xb + next.col, x_step, on_next, slots, sh.threads * V::BYTES);
+      }
+      zero_rows<T, VEC>(now.all & ~on, y, y_step);
+    } else if (more && next.here) {
+      copy_rows<T, VEC>(x + (int64_t)next.b * p.xb + next.col, x_step, bits_next[t.ty], slots, sh.threads * V::BYTES);
     }
-    on = on_next;
+    if (!more) break;
+    on = next.here ? bits_next[t.ty] : 0;
+    now = next;
   }
   if (sh.cs > 1) {  // a block's shared memory stays until the others have read it
     __syncwarp();
@@ -704,6 +730,7 @@ __device__ __forceinline__ void back_sums(BackSlots<T, VEC> sl, int cnt, const f
   if (cnt) back_rows<T, VEC, ACT, 1>(sl, neg_mean, rstd, w, b, s1, s2);
 }
 
+// A block keeps one chunk and goes over boards blockIdx.y, blockIdx.y + gridDim.y, ..., as the forward kernel does.
 template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_constant__ NormParams p,
                                                                  const __grid_constant__ ResShape sh) {
@@ -712,8 +739,10 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   using G = typename S::G;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
+  Chunk at;
+  at.set<VEC>(p, sh, t, 0, blockIdx.x >> sh.cs_log2);
   const int units = sh.cw / U;
-  const int upg = p.cg / U, groups = small_div(t.V * VEC, p.cg), all_groups = sh.cw / p.cg, g0 = small_div(t.c0, p.cg);
+  const int upg = p.cg / U, groups = small_div(at.cw, p.cg), all_groups = sh.cw / p.cg, g0 = small_div(at.c0, p.cg);
   const size_t vectors = (size_t)sh.slots * sh.threads, plane = vectors * sizeof(typename G::Raw);
   unsigned char* planes = norm_smem + round16(vectors * V::BYTES);
   S slots;
@@ -728,12 +757,11 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   float2* mine = coef + all_groups;    // [2][groups] the block's sums, of even and odd boards (cluster)
   uint32_t* bits = reinterpret_cast<uint32_t*>(mine + (sh.cs > 1 ? 2 * all_groups : 0));
   int* counts = reinterpret_cast<int*>(bits + 2 * sh.R);
-  const int col = t.c0 + t.tx * VEC;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = sh.threads / 32;
   const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
-  const int64_t x_at = (int64_t)(t.r0 + t.ty) * p.xr + col, y_at = (int64_t)(t.r0 + t.ty) * p.yr + col;
-  const uint32_t all = all_bits(sh, t);
+  const int64_t x_at = (int64_t)(t.r0 + t.ty) * p.xr + at.col, y_at = (int64_t)(t.r0 + t.ty) * p.yr + at.col;
+  const uint32_t all = at.all;
   auto copy_board = [&](int b, uint32_t on) {
     copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x, sh.threads * V::BYTES);
     copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)b * p.yb + y_at, y_step, on, slots.g[0],
@@ -750,14 +778,14 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
     bits[t.ty] = bits[sh.R + t.ty] = all;
   }
   __syncthreads();
-  uint32_t on = t.here ? bits[t.ty] : 0;
+  uint32_t on = at.here ? bits[t.ty] : 0;
   copy_board(blockIdx.y, on);
   f32x2 w[NP], bias[NP], sum1[NP], sum2[NP];  // sums over the block's boards
 #pragma unroll
   for (int j = 0; j < NP; j++) sum1[j] = sum2[j] = {0.0f, 0.0f};
-  if (t.here) {
-    load_params<VEC>(p.weight, 1.0f, sh.wvec, col, w);
-    load_params<VEC>(p.bias, 0.0f, sh.wvec, col, bias);
+  if (at.here) {
+    load_params<VEC>(p.weight, 1.0f, sh.wvec, at.col, w);
+    load_params<VEC>(p.bias, 0.0f, sh.wvec, at.col, bias);
     if (VEC == 1) w[0].y = 0.0f;
   }
 
@@ -769,7 +797,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
     uint32_t* bits_next = bits + (odd ^ 1) * sh.R;
     if (p.mask && more) load_masks(p, sh, t, next, masks);
     f32x2 neg[NP], rstd[NP];
-    if (t.here) {
+    if (at.here) {
       const float2* stats = p.stats + (int64_t)b * p.G + g0;
       float2 st[NU];
 #pragma unroll
@@ -848,7 +876,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
         float n = lane < sh.cs ? (float)ld_cluster(counts + odd, lane) : 0.0f;
         float2 c = lane < sh.cs ? ld_cluster(block_sums + g, lane) : make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
+        for (int o = 8; o > 0; o >>= 1) {
           n += __shfl_xor_sync(0xffffffffu, n, o);
           c.x += __shfl_xor_sync(0xffffffffu, c.x, o);
           c.y += __shfl_xor_sync(0xffffffffu, c.y, o);
@@ -859,8 +887,8 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
     }
     __syncthreads();
 
-    const uint32_t on_next = t.here && more ? bits_next[t.ty] : 0;
-    if (t.here) {
+    const uint32_t on_next = at.here && more ? bits_next[t.ty] : 0;
+    if (at.here) {
       T* dx = static_cast<T*>(p.y) + (int64_t)b * p.xb + x_at;
       f32x2 k1[NP], k2[NP], wr[NP];  // dx = gz (rstd w) - rstd c1 - xh (rstd c2)
       float2 co[NU];
@@ -906,7 +934,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
 
   // the channels' sums over the block's boards: rows ty by `parts` threads per channel, then those
   __syncthreads();
-  if (t.here) {
+  if (at.here) {
     float2* o = red + t.ty * sh.cw + t.tx * VEC;
 #pragma unroll
     for (int j = 0; j < NP; j++) {
@@ -915,7 +943,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
     }
   }
   __syncthreads();
-  const int cw = t.V * VEC, parts = min(sh.R, max(1, small_div(sh.threads, sh.cw)));
+  const int cw = at.cw, parts = min(sh.R, max(1, small_div(sh.threads, sh.cw)));
   const int mine_part = parts > 1 ? small_div(threadIdx.x, sh.cw) : 0;
   for (int c = threadIdx.x - mine_part * sh.cw; mine_part < parts && c < cw; c += parts > 1 ? sh.cw : sh.threads) {
     float2 s = make_float2(0.0f, 0.0f);
@@ -932,7 +960,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
       s.x += red[k * sh.cw + c].x;
       s.y += red[k * sh.cw + c].y;
     }
-    p.sums[((int64_t)blockIdx.y * sh.cs + t.rank) * p.C + t.c0 + c] = s;
+    p.sums[((int64_t)blockIdx.y * sh.cs + t.rank) * p.C + at.c0 + c] = s;
   }
 }
 
@@ -1347,20 +1375,31 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
   };
   bool ok = false;
   for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 18);
-  for (int cs = 2; cs <= 8 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots);
-  if (!ok) ok = fits(512, 8, kMaxSlots);
+  // larger boards: clusters of up to 16, where two blocks fit an SM before that where one does
+  for (int cs = 2; cs <= 16 && !ok; cs *= 2)
+    for (int threads = 256; threads <= 512 && !ok; threads *= 2)
+      ok = fits(threads, cs, kMaxSlots) && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem / 2 - 1024;
+  for (int cs = 2; cs <= 16 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots) || fits(512, cs, kMaxSlots);
   if (!ok) return false;
   // few boards: spread one over more SMs
   while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < kSms) fits(s.threads, s.cs * 2, kMaxSlots);
   s.vdiv = (1u << 20) / (uint32_t)(s.cw / vec) + 1;
-  // blocks enough for every SM; the boards go evenly over them
+  // blocks that run together, by shared memory and registers. A forward block takes any chunks; a backward one keeps
+  // its chunk (for the channels' sums) and the boards go evenly over them.
   const int64_t smem = resident_smem(s, vec, unit, es, cg, backward);
-  const int threads_sm = backward || (vec == 8 && unit == 1) ? 512 : 768;  // by registers
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(kMaxSmem / (smem + 1024), threads_sm / s.threads));
-  const int64_t most = std::max<int64_t>(1, kSms * per_sm / (chunks * s.cs));
-  const int64_t turns = (d.n + most - 1) / most;
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(kMaxSmem / (smem + 1024), !backward && s.threads == 128 ? 5 : 512 / s.threads));
+  s.chunks = (int)chunks;
+  s.blocks = (int)std::min<int64_t>(std::max<int64_t>(1, kSms * per_sm / s.cs), d.n * chunks);
+  if (s.cs > 1 && per_sm > 1) {  // clusters start together only where SMs have room: no more than the turns need
+    const int64_t tiles = d.n * chunks, turns = (tiles + s.blocks - 1) / s.blocks;
+    s.blocks = (int)((tiles + turns - 1) / turns);
+  }
+  s.step_boards = s.blocks / s.chunks;
+  s.step_chunks = s.blocks % s.chunks;
+  const int64_t most = std::max<int64_t>(1, kSms * per_sm / (chunks * s.cs)), turns = (d.n + most - 1) / most;
   s.boards = (int)std::min<int64_t>((d.n + turns - 1) / turns, 65535);
-  s.cs_log2 = s.cs == 8 ? 3 : s.cs == 4 ? 2 : s.cs == 2 ? 1 : 0;
+  s.cs_log2 = 0;
+  while (1 << s.cs_log2 < s.cs) s.cs_log2++;
   return chunks * s.cs <= 0x7fffffff;
 }
 
@@ -1448,19 +1487,20 @@ void split_backward(const NormParams& p, cudaStream_t st) {
 }
 
 template <auto kernel>
-void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaStream_t st) {
+void launch_resident(const NormParams& p, const ResShape& s, bool backward, size_t smem, cudaStream_t st) {
   static std::atomic<uint64_t> allowed[2];  // devices on which this kernel may take more than 48 KB
   int dev = 0;
   KC_CUDA(cudaGetDevice(&dev));
   if (dev >= 128) bad("device index above 127");
   if (!(allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1)) {
     KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));  // clusters of 16
     // all of an SM's shared memory: the blocks that resident_shape counts on start together
     KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.C + s.cw - 1) / s.cw * s.cs), (unsigned)s.boards);
+  cfg.gridDim = backward ? dim3((unsigned)(s.chunks * s.cs), (unsigned)s.boards) : dim3((unsigned)(s.blocks * s.cs));
   cfg.blockDim = dim3((unsigned)s.threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -1476,8 +1516,9 @@ void launch_resident(const NormParams& p, const ResShape& s, size_t smem, cudaSt
 template <typename T, int VEC, int U>
 void run_resident(const NormParams& p, ResShape s, bool backward, cudaStream_t st) {
   const size_t smem = resident_smem(s, VEC, U, sizeof(T), p.cg, backward);
-  if (!backward) return launch_resident<norm_resident_kernel<T, VEC, U>>(p, s, smem, st);
-  launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, smem, st);
+  if (!backward && s.threads == 128) return launch_resident<norm_resident_kernel<T, VEC, U, 128>>(p, s, false, smem, st);
+  if (!backward) return launch_resident<norm_resident_kernel<T, VEC, U, 512>>(p, s, false, smem, st);
+  launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, true, smem, st);
   launch_params(p, s.boards * s.cs, st);
 }
 
