@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -85,8 +86,10 @@ class GroupNormDesc(ctypes.Structure):
     def __init__(self, dtype, act, n, points, channels, groups, eps, x_strides=None, y_strides=None,
                  mask_stride=None):
         whole = (points * channels, channels)
-        super().__init__(dtype, act, n, points, channels, groups, eps, 0, *(x_strides or whole),
-                         *(y_strides or whole), points if mask_stride is None else mask_stride)
+        self._pack(self, 0, dtype, act, n, points, channels, groups, eps, 0, *(x_strides or whole),
+                   *(y_strides or whole), points if mask_stride is None else mask_stride)
+
+    _pack = struct.Struct("=6ifi5q").pack_into  # the fields in one go: made for every call of small batches
 
 
 class RopeDesc(ctypes.Structure):
@@ -116,8 +119,10 @@ class RopeDesc(ctypes.Structure):
     def __init__(self, dtype, layout, axes, tokens, q_heads, k_heads, head_dim, rotary_dim, tables=1, q_strides=None,
                  k_strides=None, q_out_strides=None, k_out_strides=None):
         q, k = (q_heads * head_dim, head_dim), (k_heads * head_dim, head_dim)
-        super().__init__(dtype, layout, axes, q_heads, k_heads, head_dim, rotary_dim, tables, tokens,
-                         *(q_strides or q), *(k_strides or k), *(q_out_strides or q), *(k_out_strides or k))
+        self._pack(self, 0, dtype, layout, axes, q_heads, k_heads, head_dim, rotary_dim, tables, tokens,
+                   *(q_strides or q), *(k_strides or k), *(q_out_strides or q), *(k_out_strides or k))
+
+    _pack = struct.Struct("=8i9q").pack_into
 
 
 P = ctypes.c_void_p
