@@ -1307,7 +1307,7 @@ void check_desc(const kc_group_norm_desc* d) {
   if (d->dtype != KC_PRECISION_F32 && d->dtype != KC_PRECISION_F16 && d->dtype != KC_PRECISION_BF16)
     bad("dtype must be KC_PRECISION_F32, F16 or BF16");
   if (d->act < KC_ACT_IDENTITY || d->act > KC_ACT_SILU) bad("unknown activation");
-  if (d->n < 0 || d->points < 0) bad("n and points must not be negative");
+  if (d->n < 0 || d->points < 0 || d->n > 1 << 30 || d->points > 1 << 30) bad("n and points must be 0 to 2^30");
   if (d->channels < 1 || d->groups < 1) bad("channels and groups must be positive");
   if (d->channels % d->groups != 0) bad("channels must be a multiple of groups");
   if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) bad("eps must be finite and not negative");

@@ -361,6 +361,79 @@ def test_host_memory_is_refused():
         assert e.value.status == api.KC_ERR_INVALID and "device memory" in str(e.value)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,points,channels,groups", [
+    (900, 361, 48, 4),      # many boards to a block
+    (300, 169, 200, 25),    # a narrower last chunk, blocks that change chunks
+    (70, 5776, 64, 8),      # clusters that go over several boards, more rows than the early mask loads
+    (45, 361, 768, 1),      # one group over a cluster of 16
+    (333, 20, 21, 3),       # single channels
+])
+def test_blocks_that_take_several_boards(n, points, channels, groups, dtype):
+    for act, kind in (("mish", "boards"), ("relu", "random"), ("silu", "none"), ("identity", "empty")):
+        _, x, w, b, g = make(n, points, channels, dtype, n)
+        mask = masks(kind, n, points, g)
+        y, stats = t.norm_forward(x, mask, w, b, groups, act)
+        check_forward(x, mask, w, b, groups, act, y, stats)
+        dy = torch.randn(x.shape, device="cuda", generator=g).to(x.dtype)
+        got = t.norm_backward(x, mask, w, b, stats, dy, groups, act)
+        check_backward(x, mask, w, b, stats, dy, groups, act, got)
+        z, _ = t.norm_forward(x, mask, w, b, groups, act, y=x)   # in place
+        assert torch.equal(z, y)
+
+
+def test_large_activations():
+    """z far outside the range of exp: mish and silu go to z and to 0, their slopes to 1 and 0."""
+    x = torch.linspace(-1, 1, 64, device="cuda").reshape(1, 64, 1).repeat(1, 1, 8)
+    on = torch.ones(1, 64, dtype=torch.bool, device="cuda")
+    b = torch.zeros(8, device="cuda")
+    for dtype in t.DTYPES.values():
+        for scale in (30.0, 200.0, 3e4):
+            w = torch.full((8,), scale, device="cuda")
+            for act in ("mish", "silu"):
+                xt = x.to(dtype)
+                y, stats = t.norm_forward(xt, None, w, b, 1, act)
+                want, _, _, xh, z = t.norm64(xt, on, w, b, 1, act)
+                half, tiny = t.half_step(dtype)
+                t.within(y, want, half * want.abs() + tiny + 1.1 * K24 * 3 * scale)
+                dy = torch.ones_like(xt)
+                got = t.norm_backward(xt, None, w, b, stats, dy, 1, act)
+                check_backward(xt, None, w, b, stats, dy, 1, act, got)
+
+
+def test_first_call_inside_a_capture():
+    """A fresh process whose first call of each operator is captured into a graph."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import token_ops as t
+x = torch.randn(4, 361, 64, device="cuda").bfloat16()
+w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+q = torch.randn(5000, 2, 64, device="cuda").bfloat16()
+pos = torch.zeros(5000, 2, dtype=torch.int32, device="cuda")
+freqs = torch.ones(1, 32, 2, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y, st = t.norm_forward(x, None, w, b, 8, "mish")
+    back = t.norm_backward(x, None, w, b, st, x, 8, "mish")
+    qo, _ = t.rope_forward(q, None, pos, freqs, 64, "halves")
+    dq = t.rope_backward(q, None, q, None, pos, freqs, 64, "halves")
+g.replay()
+torch.cuda.synchronize()
+y2, st2 = t.norm_forward(x, None, w, b, 8, "mish")
+assert torch.equal(y, y2) and torch.equal(st, st2) and torch.equal(qo, q)
+assert all(torch.equal(a, c) for a, c in zip(back, t.norm_backward(x, None, w, b, st, x, 8, "mish")))
+print("captured")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = code % (here, os.path.join(os.path.dirname(here), "katago-rs_b200", "python"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
 def test_many_shapes():
     """Random sizes, groups, strides, masks, types and directions."""
     import random

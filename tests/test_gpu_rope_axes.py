@@ -41,6 +41,9 @@ CASES = [
     (100, 16, 4, 128, 96, 3, 1), (33, 4, 4, 102, 102, 2, 4), (50, 3, 1, 30, 10, 4, 1), (17, 8, 2, 16, 16, 1, 2),
     (4099, 2, 1, 64, 48, 3, 1), (9, 2, 2, 1024, 1024, 2, 1), (65, 36, 12, 32, 32, 3, 12), (5, 7, 7, 18, 18, 2, 7),
     (3000, 1, 1, 8, 6, 2, 1), (40, 64, 8, 128, 128, 3, 1),
+    (20000, 6, 6, 64, 64, 2, 6), (30011, 8, 2, 64, 48, 4, 2),  # tiles of tokens
+    (300, 64, 64, 128, 128, 2, 64),                           # tables beyond shared memory
+    (9001, 3, 1, 34, 34, 1, 1), (7000, 5, 5, 20, 12, 3, 5),   # narrower vectors
 ]
 
 
@@ -106,10 +109,10 @@ def test_strides_in_place_and_one_buffer(dtype, layout):
     assert all(torch.equal(a, b) for a, b in zip(got, back))
 
 
+@pytest.mark.parametrize("tokens", [64, 60000])
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_far_positions(dtype):
+def test_far_positions(dtype, tokens):
     """Positions up to the ends of int32 keep the resolution of one step."""
-    tokens = 64
     wide, q, k, pos, freqs, g = make(tokens, 2, 2, 64, 64, 2, 1, dtype, 7, far=2**31 - 1)
     pos[0] = -2**31
     pos[1] = 2**31 - 1
@@ -210,8 +213,33 @@ def test_offsets_past_32_bits():
     qf, kf = buf.as_strided((3, 2, 64), (far, 64, 1)), buf[128:].as_strided((3, 1, 64), (far, 64, 1))
     qf.copy_(q)
     kf.copy_(k)
+    dq_out, dk_out = (torch.randn(v.shape, device="cuda", generator=g).half() for v in (q, k))
+    dq, dk, df = t.rope_backward(dq_out, dk_out, q, k, pos, freqs, 64, "pairs")
+    check(dq, dq_out, pos, freqs, 64, "pairs", back=True)
+    wantf, size = t.freqs_back64(dq_out, q, dk_out, k, pos, freqs, 64, "pairs")
+    far_grads = torch.empty(2 * far + 256, dtype=torch.float16, device="cuda")
+    gq, gk = far_grads.as_strided((3, 2, 64), (far, 64, 1)), far_grads[128:].as_strided((3, 1, 64), (far, 64, 1))
+    _, _, df = t.rope_backward(dq_out, dk_out, qf, kf, pos, freqs, 64, "pairs", dq=gq, dk=gk)
+    assert torch.equal(gq, dq) and torch.equal(gk, dk)
+    t.within(df, wantf, (2 * S + 2.0**-17) * size)
     t.rope_forward(qf, kf, pos, freqs, 64, "pairs", qf, kf)
     assert torch.equal(qf, want[0]) and torch.equal(kf, want[1])
+
+
+@pytest.mark.parametrize("tokens", [50, 40000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_frequencies_that_are_not_finite(tokens, bad):
+    """They make their own pairs NaN and nothing else."""
+    wide, q, k, pos, freqs, g = make(tokens, 4, 2, 32, 32, 2, 2, "bf16", 41)
+    want = t.rope_forward(q, k, pos, freqs, 32, "halves")
+    freqs[1, 5, 0] = bad
+    got = t.rope_forward(q, k, pos, freqs, 32, "halves")
+    for a, w, per in zip(got, want, (2, 1)):
+        hit = torch.zeros(w.shape[1:], dtype=torch.bool, device="cuda")
+        hit[per:, 5] = hit[per:, 21] = True
+        assert torch.isnan(a[:, hit]).all() and torch.equal(a[:, ~hit], w[:, ~hit])
+    dq, dk, df = t.rope_backward(want[0], want[1], q, k, pos, freqs, 32, "halves")
+    assert torch.isnan(df[1, 5]).all() and torch.isfinite(df[0]).all() and torch.isfinite(df[1, 6:]).all()
 
 
 def test_no_tokens():

@@ -34,7 +34,7 @@ def refused(f, *args, **kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(dtype=3), dict(dtype=-1), dict(act=4), dict(act=-1), dict(n=-1), dict(points=-1), dict(channels=0),
+    dict(dtype=3), dict(dtype=-1), dict(act=4), dict(act=-1), dict(n=-1), dict(points=-1), dict(n=(1 << 30) + 1), dict(points=(1 << 30) + 1), dict(channels=0),
     dict(groups=0), dict(groups=7), dict(groups=385), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
     dict(x_strides=(-384, 384)), dict(x_strides=(361 * 384, -1)), dict(y_strides=(361 * 384, 383)),
     dict(y_strides=(0, 384)), dict(y_strides=(361 * 384 - 1, 384)), dict(y_strides=(1 << 50, 384)),
@@ -114,6 +114,7 @@ def rotate_back(d, dqo=QO, dko=KO, q=Q, k=K, pos=POS, fr=FR, dq=DX, dk=DY, df=DF
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=3), dict(layout=2), dict(axes=0), dict(axes=5), dict(tokens=-1), dict(q_heads=0), dict(k_heads=-1),
+    dict(q_heads=4098), dict(k_heads=4098),
     dict(head_dim=1), dict(head_dim=1026, rotary_dim=2), dict(rotary_dim=0), dict(rotary_dim=3), dict(rotary_dim=66),
     dict(tables=0), dict(tables=3), dict(tables=6), dict(q_strides=(-1, 64)), dict(k_strides=(64, -64)),
     dict(q_out_strides=(383, 64)), dict(q_out_strides=(0, 64)), dict(k_out_strides=(128, 63)),
