@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 5 : 1) norm_resident
   const int y0 = small_div(lane, upg), u0 = lane - y0 * upg, dy = small_div(32, upg), du = 32 - dy * upg;
   const uint32_t x_step = (uint32_t)(sh.R * p.xr * sizeof(T)), y_step = (uint32_t)(sh.R * p.yr * sizeof(T));
   const T* x = static_cast<const T*>(p.x) + (int64_t)(t.r0 + t.ty) * p.xr;
-  Chunk now, next;
+  Chunk now = {}, next = {};
   {
     const int first = blockIdx.x >> sh.cs_log2;
     now.set<VEC>(p, sh, t, first / sh.chunks, first % sh.chunks);
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   using G = typename S::G;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
-  Chunk at;
+  Chunk at = {};
   at.set<VEC>(p, sh, t, 0, blockIdx.x >> sh.cs_log2);
   const int units = sh.cw / U;
   const int upg = p.cg / U, groups = small_div(at.cw, p.cg), all_groups = sh.cw / p.cg, g0 = small_div(at.c0, p.cg);
