@@ -7,8 +7,23 @@
 //   c1 = sum_{c of the group} w S1 / M, c2 = sum w S2 / M, dx = rstd (gz w - c1 - xh c2) where on,
 //   dbias = sum over boards of S1, dweight = of S2
 //
-// Statistics and sums are float32 (means are merged in float64). A thread's share of a mean and of a sum of squares
-// is taken around its own mean and shares are merged by count, so that a large mean costs no digits of the variance.
+// Statistics and sums are float32 (split path: merged in float64). A thread's share of a mean and of a sum of squares
+// is taken around a value of its own and shares are merged by count as distances from one of them, so that a large
+// mean costs no digits of the variance.
+//
+// What bounds it: HBM, once reading and writing the tensor is all the traffic there is; each element also costs about
+// 12 instructions forward (mish) and 25 backward, which takes nearly as long. So a board's chunk of channels is read
+// once into shared memory and stays there (resident path). Measured on a B200 (6,554 GB/s copy), bytes that have to
+// move / time:
+//   forward, 256 boards x 361 points x 384 channels, 32 groups, bf16, mish, mixed board sizes: 119 MB in 32.6 us,
+//     3,660 GB/s (the split path's three launches with two reads: 178 us). 53% of the issue slots; 16 warps to an SM
+//     (96 registers, 39 KB of slots a block), which wait for their own arithmetic and two barriers a chunk
+//   1,024 of those boards: 477 MB in 111 us, 4,310 GB/s
+//   backward, 512 such boards: 334 MB in 110 us, 3,030 GB/s (split path: 426 us); 128 registers and 115 KB of slots
+//     leave two blocks of 256 to an SM
+//   forward, 64 boards x 361 x 768, one group, float32, silu: 119 MB in 52 us, 2,290 GB/s: a board fills a cluster of
+//     16 blocks, all boards in four turns of all SMs that load, reduce and store in step
+//   forward, 32 x 5,776 x 256, 32 groups, bf16, silu: 189 MB in 56 us, 3,380 GB/s (clusters of 4)
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -117,6 +132,12 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 // stands between the copy and the statistics.
 // U neighbouring channels of a vector lie in one group (VEC, 4 or 1 of them), so that a thread's statistics are
 // VEC / U triples of (count, mean, sum of squares around it).
+//
+// Why this shape: shared memory and not registers, since vectors in registers had to be unrolled and unpacked floats
+// stayed live across the passes (206 registers, one block to an SM: 152 us for the 256 boards above). Chunks of at
+// least 64 bytes of a row: with 48 bytes the fixed work of a chunk weighs more (42 us), with 128 bytes clusters
+// are needed (54 us). Blocks of 128 with up to 18 rows a thread forward: the fixed work of a chunk (about 500
+// instructions a warp) is spread over more rows than with 256 (36 us). Only rows that are on are read.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSlots = 32;  // a thread's rows are bits of one word
 
@@ -196,7 +217,8 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 
 __device__ __forceinline__ float2 ld_cluster(const float2* p, uint32_t rank) {
   float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
   return v;
 }
 __device__ __forceinline__ int ld_cluster(const int* p, uint32_t rank) {
@@ -408,7 +430,8 @@ __device__ __forceinline__ void load_params(const float* w, float other, bool ve
 }
 
 template <typename T, int VEC, int ACT>
-__device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VEC>::Raw* slot, int slot_step, T* y, uint32_t step,
+__device__ __forceinline__ void apply_rows(uint32_t on, const typename Vec<T, VEC>::Raw* slot, int slot_step, T* y,
+                                           uint32_t step,
                                            const f32x2 (&neg_mean)[Vec<T, VEC>::NP], const f32x2 (&a)[Vec<T, VEC>::NP],
                                            const f32x2 (&b)[Vec<T, VEC>::NP]) {
   using V = Vec<T, VEC>;
@@ -451,8 +474,8 @@ __device__ __forceinline__ float2 final_stats(float mean, float var, bool any, f
 // chunk's rows are copied into the slots as soon as the thread has written this one's, so that the copy runs under the
 // other threads' work and the next mask is known by then.
 template <typename T, int VEC, int U, int THREADS>  // THREADS: at most; blocks of 128 run five to an SM
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 5 : 1) norm_resident_kernel(const __grid_constant__ NormParams p,
-                                                            const __grid_constant__ ResShape sh) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 5 : 1)
+    norm_resident_kernel(const __grid_constant__ NormParams p, const __grid_constant__ ResShape sh) {
   using V = Vec<T, VEC>;
   constexpr int NU = VEC / U, NP = V::NP;
   const ResIds t = res_ids<VEC>(p, sh);
@@ -763,7 +786,8 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
   const int64_t x_at = (int64_t)(t.r0 + t.ty) * p.xr + at.col, y_at = (int64_t)(t.r0 + t.ty) * p.yr + at.col;
   const uint32_t all = at.all;
   auto copy_board = [&](int b, uint32_t on) {
-    copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x, sh.threads * V::BYTES);
+    copy_rows<T, VEC>(static_cast<const T*>(p.x) + (int64_t)b * p.xb + x_at, x_step, on, slots.x,
+                      sh.threads * V::BYTES);
     copy_rows<T, VEC>(static_cast<const T*>(p.dy) + (int64_t)b * p.yb + y_at, y_step, on, slots.g[0],
                       sh.threads * (int)sizeof(typename G::Raw));
   };
@@ -1033,7 +1057,8 @@ __global__ void __launch_bounds__(kThreads) norm_tile_stats_kernel(const __grid_
     }
     if (t.active) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) red[(t.ty * VEC + j) * (kThreads / t.rows_at_once) + t.tx] = make_float2(mean[j], m2[j]);
+      for (int j = 0; j < VEC; j++)
+        red[(t.ty * VEC + j) * (kThreads / t.rows_at_once) + t.tx] = make_float2(mean[j], m2[j]);
       if (t.tx == 0) red_n[t.ty] = cnt;
     }
     __syncthreads();
@@ -1189,7 +1214,8 @@ __global__ void __launch_bounds__(kThreads) norm_tile_back_kernel(const __grid_c
     }
     if (t.active) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) red[(t.ty * VEC + j) * (kThreads / t.rows_at_once) + t.tx] = make_float2(s1[j], s2[j]);
+      for (int j = 0; j < VEC; j++)
+        red[(t.ty * VEC + j) * (kThreads / t.rows_at_once) + t.tx] = make_float2(s1[j], s2[j]);
       if (t.tx == 0) red_n[t.ty] = cnt;
     }
     __syncthreads();
@@ -1346,7 +1372,8 @@ size_t resident_smem(ResShape& s, int vec, int unit, int es, int cg, bool backwa
   size_t bytes = round16(slots * vec * es);
   if (backward) bytes = round16(std::max(bytes + slots * vec * 4, (size_t)s.R * s.cw * sizeof(float2)));
   s.slot_bytes = (int)bytes;
-  return bytes + ((size_t)s.R * (s.cw / unit) + (s.cs > 1 ? 3 : 1) * groups) * sizeof(float2) + (2 * s.R + 2) * sizeof(int);
+  return bytes + ((size_t)s.R * (s.cw / unit) + (s.cs > 1 ? 3 : 1) * groups) * sizeof(float2) +
+         (2 * s.R + 2) * sizeof(int);
 }
 
 // Channels of a vector that are sure to lie in one group.
@@ -1387,7 +1414,8 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
   // blocks that run together, by shared memory and registers. A forward block takes any chunks; a backward one keeps
   // its chunk (for the channels' sums) and the boards go evenly over them.
   const int64_t smem = resident_smem(s, vec, unit, es, cg, backward);
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(kMaxSmem / (smem + 1024), !backward && s.threads == 128 ? 5 : 512 / s.threads));
+  const int by_registers = !backward && s.threads == 128 ? 5 : 512 / s.threads;
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(kMaxSmem / (smem + 1024), by_registers));
   s.chunks = (int)chunks;
   s.blocks = (int)std::min<int64_t>(std::max<int64_t>(1, kSms * per_sm / s.cs), d.n * chunks);
   if (s.cs > 1 && per_sm > 1) {  // clusters start together only where SMs have room: no more than the turns need
@@ -1496,7 +1524,8 @@ void launch_resident(const NormParams& p, const ResShape& s, bool backward, size
     KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
     KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));  // clusters of 16
     // all of an SM's shared memory: the blocks that resident_shape counts on start together
-    KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared));
     allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
@@ -1516,7 +1545,8 @@ void launch_resident(const NormParams& p, const ResShape& s, bool backward, size
 template <typename T, int VEC, int U>
 void run_resident(const NormParams& p, ResShape s, bool backward, cudaStream_t st) {
   const size_t smem = resident_smem(s, VEC, U, sizeof(T), p.cg, backward);
-  if (!backward && s.threads == 128) return launch_resident<norm_resident_kernel<T, VEC, U, 128>>(p, s, false, smem, st);
+  if (!backward && s.threads == 128)
+    return launch_resident<norm_resident_kernel<T, VEC, U, 128>>(p, s, false, smem, st);
   if (!backward) return launch_resident<norm_resident_kernel<T, VEC, U, 512>>(p, s, false, smem, st);
   launch_resident<norm_resident_back_kernel<T, VEC, U>>(p, s, true, smem, st);
   launch_params(p, s.boards * s.cs, st);
@@ -1584,11 +1614,6 @@ void check_tensors(const kc_group_norm_desc& d, std::initializer_list<Rows> rows
 }
 
 // Outputs share no memory with each other or with an input; only a tensor may be its own output.
-struct Range {
-  const void* p;
-  int64_t bytes;
-};
-
 void check_outputs(const kc_group_norm_desc& d, const Rows& out, std::initializer_list<Rows> ins, const float* mask,
                    std::initializer_list<Range> small_in, std::initializer_list<Range> small_out) {
   if (!rows_distinct(out)) bad("rows of the output share memory");
@@ -1597,13 +1622,13 @@ void check_outputs(const kc_group_norm_desc& d, const Rows& out, std::initialize
   const Rows m{mask, d.n, 1, d.points, d.mask_board_stride, 0, 4};
   if (rows_overlap(out, m)) bad("the output overlaps the mask");
   for (const Range& s : small_in)
-    if (ranges_meet(s.p, s.bytes, out)) bad("the output overlaps another tensor of the call");
+    if (ranges_meet(s, out)) bad("the output overlaps another tensor of the call");
   for (const Range* o = small_out.begin(); o != small_out.end(); o++) {
-    bool meets = ranges_meet(o->p, o->bytes, out) || ranges_meet(o->p, o->bytes, m);
-    for (const Rows& i : ins) meets = meets || ranges_meet(o->p, o->bytes, i);
-    for (const Range& s : small_in) meets = meets || ranges_meet(o->p, o->bytes, {s.p, 1, 1, s.bytes, 0, 0, s.p ? 1 : 0});
+    bool meets = ranges_meet(*o, out) || ranges_meet(*o, m);
+    for (const Rows& i : ins) meets = meets || ranges_meet(*o, i);
+    for (const Range& s : small_in) meets = meets || ranges_meet(*o, s);
     for (const Range* q = o + 1; q != small_out.end(); q++)
-      meets = meets || ranges_meet(o->p, o->bytes, {q->p, 1, 1, q->bytes, 0, 0, q->p ? 1 : 0});
+      meets = meets || ranges_meet(*o, *q);
     if (meets) bad("the statistics, parameter gradients or workspace overlap another tensor of the call");
   }
 }

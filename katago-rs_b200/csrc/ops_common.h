@@ -34,8 +34,9 @@ int guard_entry(F&& f) noexcept {
 
 inline int dtype_bytes(int dtype) { return dtype == KC_PRECISION_F32 ? 4 : 2; }
 
-// Makes the device that holds the operator's tensors current for the launch, and the caller's device again after it. Every pointer (null ones are skipped) has to be device or managed memory of one device. A stream of another
-// device makes the launch fail (a stream cannot be asked for its device while it is captured).
+// Makes the device that holds the operator's tensors current for the launch, and the caller's device again after it.
+// Every pointer (null ones are skipped) has to be device or managed memory of one device. A stream of another device
+// makes the launch fail (a stream cannot be asked for its device while it is captured).
 class TensorDevice {
  public:
   TensorDevice(const char* op, std::initializer_list<const void*> ptrs) {
@@ -127,10 +128,17 @@ inline bool rows_in_range(const Rows& a) {
 
 inline bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-inline bool ranges_meet(const void* a, int64_t na, const Rows& r) {
-  if (!a || na <= 0 || r.empty()) return false;
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(a);
-  return lo < r.hi() && r.lo() < lo + (uintptr_t)na;
+// A plain array.
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+
+inline bool ranges_meet(const Range& a, const Rows& r) {
+  if (!a.p || a.bytes <= 0 || r.empty()) return false;
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(a.p);
+  return lo < r.hi() && r.lo() < lo + (uintptr_t)a.bytes;
 }
+inline bool ranges_meet(const Range& a, const Range& b) { return ranges_meet(a, Rows{b.p, 1, 1, b.bytes, 0, 0, 1}); }
 
 }  // namespace kc

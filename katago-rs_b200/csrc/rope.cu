@@ -6,9 +6,19 @@
 //
 // Angles are held in turns, as 64-bit fractions: a frequency is freq / (2 pi) mod 1 scaled by 2^64 (from float64, so
 // 53 bits of freq / (2 pi)), and whole turns of pos * frequency drop out of the 64-bit product by themselves. The
-// error is that of freq / (2 pi), 2^-53 of the angle; far positions keep their digits, at three integer
-// multiply-adds an axis.
+// error is that of freq / (2 pi), 2^-53 of the angle; far positions keep their digits, at two integer multiply-adds
+// an axis (float64 angles reduced with rint were 3 to 4 times the instructions).
 //
+// What bounds it: HBM for a table shared by all heads; with a table per key head the angles (17.7 million for 256
+// boards, about 28 instructions each) take as long as the transfers. Measured on a B200 (6,554 GB/s copy), bytes that
+// have to move / time:
+//   256 boards x 361 tokens, 6 + 6 heads of 64, f16: 284 MB in 53 us (5,300 GB/s) with one table, in 66.7 us
+//     (4,270 GB/s) with a table per key head; a thread per pair vector with its own float64 angles: 86 us
+//   57,767 tokens, 16 + 4 heads of 128, 96 of them turned, 3 axes, bf16: 592 MB in 119.5 us, 4,960 GB/s
+//   backward with the frequencies' gradient, 34,656 tokens, 12 + 4 heads of 64, 4 tables, bf16: 213 MB in 54.3 us,
+//     3,930 GB/s: 24 warps to an SM (80 registers), most of the time waiting for their loads
+//   backward without it, 4,099 tokens, 12 + 12 heads of 64, float32: 50 MB in 12 us
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -219,8 +229,8 @@ struct alignas(16) HeadAddr {
 };
 
 // A tile's shared memory: the heads [tables][heads], the frequencies' fractions [axes][entries], the phase of the
-// positions' bias [entries], the tile's positions [tokens][axes], and the sines: [chunk of two pairs of a vector][vector of the tile] (cos, cos, sin, sin), so
-// that neighbouring threads read neighbouring 16-byte chunks.
+// positions' bias [entries], the tile's positions [tokens][axes], and the sines: [chunk of two pairs of a vector]
+// [vector of the tile] (cos, cos, sin, sin), so that neighbouring threads read neighbouring 16-byte chunks.
 template <int VP>
 struct Tile {
   static constexpr int CH = VP < 2 ? 1 : 2, CHUNKS = VP / CH;
@@ -250,7 +260,8 @@ struct Tile {
   __device__ __forceinline__ void read(int vector, f32x2 (&c)[(VP + 1) / 2], f32x2 (&s)[(VP + 1) / 2]) const {
 #pragma unroll
     for (int q = 0; q < CHUNKS; q++) {
-      const Pack<float, 2 * CH> v = *reinterpret_cast<const Pack<float, 2 * CH>*>(sines + ((size_t)q * vectors + vector) * (2 * CH));
+      const float* chunk = sines + ((size_t)q * vectors + vector) * (2 * CH);
+      const Pack<float, 2 * CH> v = *reinterpret_cast<const Pack<float, 2 * CH>*>(chunk);
       c[q] = {v.v[0], CH == 2 ? v.v[1] : 0.0f};
       s[q] = {v.v[CH], CH == 2 ? v.v[CH + 1] : 0.0f};
     }
@@ -332,7 +343,8 @@ __device__ __forceinline__ void tile_angles(const Tile<VP>& tile, int tokens) {
 }
 
 template <typename T, int VP>
-__device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens, bool finite) {
+__device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& tile, int64_t t0, int tokens,
+                                           bool finite) {
   if (p.axes == 1) tile_angles<T, VP, 1>(tile, tokens);
   else if (p.axes == 2) tile_angles<T, VP, 2>(tile, tokens);
   else if (p.axes == 3) tile_angles<T, VP, 3>(tile, tokens);
@@ -458,8 +470,10 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) rope_axes_back_kernel(c
 #pragma unroll
         for (int k = 0; k < N; k++)
           if (k == 0 || two) {
-            dy[k].load(reinterpret_cast<const T*>(h[k * p.rounds].in + (uint64_t)t * h[k * p.rounds].in_step), col * VP, p.pairs);
-            x[k].load(reinterpret_cast<const T*>(h[k * p.rounds].x + (uint64_t)t * h[k * p.rounds].out_step), col * VP, p.pairs);
+            // x lies at the gradient's strides
+            const HeadAddr& hk = h[k * p.rounds];
+            dy[k].load(reinterpret_cast<const T*>(hk.in + (uint64_t)t * hk.in_step), col * VP, p.pairs);
+            x[k].load(reinterpret_cast<const T*>(hk.x + (uint64_t)t * hk.out_step), col * VP, p.pairs);
           }
 #pragma unroll
         for (int k = 0; k < N; k++)
@@ -473,7 +487,8 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) rope_axes_back_kernel(c
               turn[j] = fma2(b, xa, fma2({-a.x, -a.y}, xb, turn[j]));
               dy[k].set2(2 * j, a, b);
             }
-            dy[k].store(reinterpret_cast<T*>(h[k * p.rounds].out + (uint64_t)t * h[k * p.rounds].out_step), col * VP, p.pairs);
+            const HeadAddr& hk = h[k * p.rounds];
+            dy[k].store(reinterpret_cast<T*>(hk.out + (uint64_t)t * hk.out_step), col * VP, p.pairs);
           }
       }
 #pragma unroll
@@ -589,11 +604,6 @@ Rows k_out(const kc_rope_desc& d, const void* p) {
   return rows(d, p, d.k_heads, d.k_out_token_stride, d.k_out_head_stride);
 }
 
-struct Range {
-  const void* p;
-  int64_t bytes;
-};
-
 // The outputs' own memory, and what each of them may meet: only its own input, in place.
 void check_tensors(const kc_rope_desc& d, const Rows (&in)[2], const Rows (&out)[2], std::initializer_list<Rows> more,
                    std::initializer_list<Range> small_in, std::initializer_list<Range> small_out) {
@@ -615,17 +625,17 @@ void check_tensors(const kc_rope_desc& d, const Rows (&in)[2], const Rows (&out)
     for (const Rows& r : more)
       if (rows_overlap(out[i], r)) bad("an output overlaps an input");
     for (const Range& r : small_in)
-      if (ranges_meet(r.p, r.bytes, out[i])) bad("an output overlaps the positions or frequencies");
+      if (ranges_meet(r, out[i])) bad("an output overlaps the positions or frequencies");
     for (const Range& r : small_out)
-      if (ranges_meet(r.p, r.bytes, out[i])) bad("an output overlaps the frequencies' gradient or the workspace");
+      if (ranges_meet(r, out[i])) bad("an output overlaps the frequencies' gradient or the workspace");
   }
   if (rows_overlap(out[0], out[1])) bad("the outputs overlap");
   for (const Range* o = small_out.begin(); o != small_out.end(); o++) {
-    bool meets = ranges_meet(o->p, o->bytes, in[0]) || ranges_meet(o->p, o->bytes, in[1]);
-    for (const Rows& r : more) meets = meets || ranges_meet(o->p, o->bytes, r);
-    for (const Range& r : small_in) meets = meets || ranges_meet(o->p, o->bytes, {r.p, 1, 1, r.bytes, 0, 0, r.p ? 1 : 0});
+    bool meets = ranges_meet(*o, in[0]) || ranges_meet(*o, in[1]);
+    for (const Rows& r : more) meets = meets || ranges_meet(*o, r);
+    for (const Range& r : small_in) meets = meets || ranges_meet(*o, r);
     for (const Range* q = o + 1; q != small_out.end(); q++)
-      meets = meets || ranges_meet(o->p, o->bytes, {q->p, 1, 1, q->bytes, 0, 0, q->p ? 1 : 0});
+      meets = meets || ranges_meet(*o, *q);
     if (meets) bad("the frequencies' gradient or the workspace overlaps another tensor of the call");
   }
 }
@@ -648,7 +658,7 @@ int vec_of(const kc_rope_desc& d, std::initializer_list<Rows> all) {
 constexpr int kSms = 148;
 constexpr int kMaxTileBytes = 100 * 1024;  // of shared memory a block of the tile kernels
 
-// Blocks of a backward pass with the frequencies' gradient: as many as fit the SMs (registers), each with its partial sums.
+// Blocks of a backward pass with the frequencies' gradient, each with its partial sums: as many as the SMs hold.
 int64_t back_blocks(const kc_rope_desc& d) {
   return std::min<int64_t>(kSms * kBackBlocks, std::max<int64_t>(1, d.tokens));
 }
@@ -702,7 +712,8 @@ uint32_t magic(int64_t d) { return d == 1 ? 0 : (uint32_t)(0xffffffffu / d + 1);
 
 // Tokens of a tile, at most `most` (32 KB of sines): every block gets the same number of tiles.
 int tile_tokens(int64_t tokens, int64_t blocks, int64_t most) {
-  const int64_t share = (tokens + blocks - 1) / blocks, tiles = (share + std::max<int64_t>(1, most) - 1) / std::max<int64_t>(1, most);
+  const int64_t share = (tokens + blocks - 1) / blocks, cap = std::max<int64_t>(1, most);
+  const int64_t tiles = (share + cap - 1) / cap;
   return (int)((share + tiles - 1) / tiles);
 }
 
@@ -760,7 +771,8 @@ void launch(RopeParams p, cudaStream_t st) {
   p.by_table = magic(p.rounds * cols);
   p.by_head = magic(cols);
   const int64_t tiles = (p.tokens + p.tile - 1) / p.tile;
-  launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT>>(p, dim3((unsigned)std::min<int64_t>(tiles, kSms * kTileBlocks)), smem, st);
+  const dim3 grid((unsigned)std::min<int64_t>(tiles, kSms * kTileBlocks));
+  launch_kernel<rope_axes_tile_kernel<T, VP, LAYOUT>>(p, grid, smem, st);
 }
 
 template <typename T, int VP>

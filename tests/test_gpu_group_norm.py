@@ -219,7 +219,11 @@ def check_backward(x, mask, w, b, stats, dy, groups, act, got):
     dz = (xh * w.double().abs() + b.double().abs()) * dyd if act in ("mish", "silu") else torch.zeros_like(dyd)
     wd = w.double().abs()
     count = (on.sum(1) * cg).double().clamp(min=1)[:, None]
-    share = lambda v: ((v.sum(1) * wd).reshape(x.shape[0], groups, cg).sum(2) / count).repeat_interleave(cg, 1)[:, None]  # noqa: E731
+
+    def share(v):
+        s = (v.sum(1) * wd).reshape(x.shape[0], groups, cg).sum(2) / count
+        return s.repeat_interleave(cg, 1)[:, None]
+
     more = r * (dz * wd + share(dz) + xh * share(dz * xh))
     t.within(got[0], dx, torch.where(on[:, :, None], half * dx.abs() + tiny + K24 * (size + more + r * dyd * wd), 0.0))
     t.within(got[1], dw, K24 * (wsize + (dz * xh).sum((0, 1)) + (dyd * xh).sum((0, 1))))
@@ -380,6 +384,18 @@ def test_blocks_that_take_several_boards(n, points, channels, groups, dtype):
         check_backward(x, mask, w, b, stats, dy, groups, act, got)
         z, _ = t.norm_forward(x, mask, w, b, groups, act, y=x)   # in place
         assert torch.equal(z, y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n,points,channels,groups", [(2, 30000, 256, 1), (1, 90000, 24, 3), (3, 4000, 1000, 5)])
+def test_boards_beyond_a_cluster(n, points, channels, groups, dtype):
+    for act, kind in (("mish", "boards"), ("relu", "none"), ("silu", "empty")):
+        _, x, w, b, g = make(n, points, channels, dtype, n)
+        mask = masks(kind, n, points, g)
+        y, stats = t.norm_forward(x, mask, w, b, groups, act)
+        check_forward(x, mask, w, b, groups, act, y, stats)
+        dy = torch.randn(x.shape, device="cuda", generator=g).to(x.dtype)
+        check_backward(x, mask, w, b, stats, dy, groups, act, t.norm_backward(x, mask, w, b, stats, dy, groups, act))
 
 
 def test_large_activations():

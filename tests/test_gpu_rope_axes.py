@@ -151,7 +151,8 @@ def test_gradient_of_frequencies_is_the_difference_quotient():
 
         def loss(h):
             f = freqs.double() + h * v
-            return sum((t.turn64(x, pos, f, 24, layout)[0] * o.double()).sum().item() for x, o in ((q, dq_out), (k, dk_out)))
+            turned = [t.turn64(x, pos, f, 24, layout)[0] for x in (q, k)]
+            return sum((y * o.double()).sum().item() for y, o in zip(turned, (dq_out, dk_out)))
 
         h = 3e-5
         slope = (loss(h) - loss(-h)) / (2 * h)

@@ -55,7 +55,8 @@ def test_block(act):
     (dqkv,) = torch.autograd.grad(out, leaf, do)
     dqkv = dqkv.reshape(n * points, -1, hd).contiguous()
     dq, dk = dqkv[:, :hq], dqkv[:, hq:hq + hk]
-    _, _, dfreqs = t.rope_backward(dq, dk, before[:, :hq], before[:, hq:hq + hk], pos, freqs, hd, "halves", dq=dq, dk=dk)
+    _, _, dfreqs = t.rope_backward(dq, dk, before[:, :hq], before[:, hq:hq + hk], pos, freqs, hd, "halves", dq=dq,
+                                   dk=dk)
     dy = (dqkv.reshape(n * points, -1) @ wqkv.T).view(n, points, channels)
     dx, dw, db = t.norm_backward(x, mask, w, b, stats, dy, groups, act)
 

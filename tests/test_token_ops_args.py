@@ -34,7 +34,8 @@ def refused(f, *args, **kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(dtype=3), dict(dtype=-1), dict(act=4), dict(act=-1), dict(n=-1), dict(points=-1), dict(n=(1 << 30) + 1), dict(points=(1 << 30) + 1), dict(channels=0),
+    dict(dtype=3), dict(dtype=-1), dict(act=4), dict(act=-1), dict(n=-1), dict(points=-1), dict(n=(1 << 30) + 1),
+    dict(points=(1 << 30) + 1), dict(channels=0),
     dict(groups=0), dict(groups=7), dict(groups=385), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
     dict(x_strides=(-384, 384)), dict(x_strides=(361 * 384, -1)), dict(y_strides=(361 * 384, 383)),
     dict(y_strides=(0, 384)), dict(y_strides=(361 * 384 - 1, 384)), dict(y_strides=(1 << 50, 384)),
