@@ -7,7 +7,7 @@
 //   c1 = sum_{c of the group} w S1 / M, c2 = sum w S2 / M, dx = rstd (gz w - c1 - xh c2) where on,
 //   dbias = sum over boards of S1, dweight = of S2
 //
-// Statistics and sums are float32 (split path: merged in float64). A thread's share of a mean and of a sum of squares
+// Statistics and sums are float32. A thread's share of a mean and of a sum of squares
 // is taken around a value of its own and shares are merged by count as distances from one of them, so that a large
 // mean costs no digits of the variance.
 //
@@ -64,10 +64,6 @@ struct NormParams {
   float eps;
   int tiles, tile_rows;
 };
-
-__device__ __forceinline__ bool point_on(const NormParams& p, int b, int r) {
-  return p.mask == nullptr || __ldg(p.mask + (int64_t)b * p.mb + r) != 0.0f;
-}
 
 // relu keeps a NaN, as the other activations do
 __device__ __forceinline__ float norm_act(float z, int act) {
@@ -461,7 +457,7 @@ extern __shared__ __align__(16) unsigned char norm_smem[];
 
 // A group's (mean, rstd), also into the statistics the caller wants. 1 / sqrt by the fast function (2^-22) and one
 // Newton step; a variance of 0 with eps 0 gives infinity.
-__device__ __forceinline__ float2 final_stats(float mean, float var, bool any, float eps, float2* stats, int g) {
+__device__ __forceinline__ float2 final_stats(float mean, float var, bool any, float eps, float2* stats, int64_t g) {
   const float v = (var < 0.0f ? 0.0f : var) + eps;
   float r = rsqrtf(v);
   if (v > 0.0f && v < 1e38f) r = r * (1.5f - 0.5f * v * r * r);
@@ -992,6 +988,12 @@ __global__ void __launch_bounds__(512) norm_resident_back_kernel(const __grid_co
 // The split path, for boards too large for one cluster of blocks: column vectors of VEC channels (lanes tx) by rows
 // (ty), a tile of rows per block. grid (tiles * column blocks, boards modulo grid.y).
 // ---------------------------------------------------------------------------------------------------------------
+// Column vectors of a block: at most 64, the same number for every block.
+__host__ __device__ __forceinline__ int tile_columns(int V) {
+  const int blocks = (V + 63) / 64;
+  return (V + blocks - 1) / blocks;
+}
+
 struct TileIds {
   int tile, col0, tx, ty, rows_at_once;
   bool active;
@@ -999,7 +1001,7 @@ struct TileIds {
 
 template <int VEC>
 __device__ __forceinline__ TileIds tile_ids(const NormParams& p) {
-  const int V = p.C / VEC, vc = V < 64 ? V : 64;  // column vectors of a block
+  const int V = p.C / VEC, vc = tile_columns(V);
   TileIds t;
   t.tile = blockIdx.x % p.tiles;
   t.tx = threadIdx.x % vc;
@@ -1009,6 +1011,21 @@ __device__ __forceinline__ TileIds tile_ids(const NormParams& p) {
   t.col0 = cv * VEC;
   t.active = t.ty < t.rows_at_once && cv < V;
   return t;
+}
+
+// Which of the next N rows of a thread are there and on; their masks are loaded before any of them is waited for.
+// Backward fewer rows: they come in twos, with twice the constants.
+constexpr int kRowsAhead = 4, kBackRows = 2;
+template <int N>
+__device__ __forceinline__ void rows_ahead(const NormParams& p, int b, int r, int step, int r1, bool (&on)[N]) {
+  float m[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int ri = r + i * step;
+    m[i] = ri < r1 ? (p.mask ? __ldg(p.mask + (int64_t)b * p.mb + ri) : 1.0f) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) on[i] = m[i] != 0.0f;
 }
 
 template <typename T, int VEC>
@@ -1022,29 +1039,27 @@ __global__ void __launch_bounds__(kThreads) norm_tile_stats_kernel(const __grid_
     float mean[VEC] = {}, m2[VEC] = {};
     int cnt = 0;
     if (t.active) {
-      for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += 4 * t.rows_at_once) {
-        float v[4][VEC];
-        bool on[4];
+      for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += kRowsAhead * t.rows_at_once) {
+        float v[kRowsAhead][VEC];
+        bool on[kRowsAhead];
         int k = 0;
+        rows_ahead(p, b, r, t.rows_at_once, r1, on);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int ri = r + i * t.rows_at_once;
-          on[i] = ri < r1 && point_on(p, b, ri);
+        for (int i = 0; i < kRowsAhead; i++)
           if (on[i]) {
-            load_pack<T, VEC>(x + (int64_t)ri * p.xr, v[i]);
+            load_pack<T, VEC>(x + (int64_t)(r + i * t.rows_at_once) * p.xr, v[i]);
             k++;
           }
-        }
         if (!k) continue;
         const float ik = 1.0f / (float)k, share = (float)k / (float)(cnt + k);
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
           float s = 0.0f, q = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; i++) s += on[i] ? v[i][j] : 0.0f;
+          for (int i = 0; i < kRowsAhead; i++) s += on[i] ? v[i][j] : 0.0f;
           s *= ik;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
+          for (int i = 0; i < kRowsAhead; i++) {
             const float d = on[i] ? v[i][j] - s : 0.0f;
             q += d * d;
           }
@@ -1062,64 +1077,84 @@ __global__ void __launch_bounds__(kThreads) norm_tile_stats_kernel(const __grid_
       if (t.tx == 0) red_n[t.ty] = cnt;
     }
     __syncthreads();
-    if (t.active && t.ty == 0) {
-      int N = 0;
-      for (int i = 0; i < t.rows_at_once; i++) N += red_n[i];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        double s = 0.0;
-        for (int i = 0; i < t.rows_at_once; i++)
-          s += (double)red_n[i] * red[(i * VEC + j) * (kThreads / t.rows_at_once) + t.tx].x;
-        const double mu = N ? s / N : 0.0;
-        float q = 0.0f;
-        for (int i = 0; i < t.rows_at_once; i++) {
-          const float2 u = red[(i * VEC + j) * (kThreads / t.rows_at_once) + t.tx];
-          const float d = (float)(u.x - mu);
-          q += red_n[i] ? u.y + d * d * (float)red_n[i] : 0.0f;
-        }
-        p.part[((int64_t)b * p.tiles + t.tile) * p.C + t.col0 + j] = make_float2((float)mu, q);
-      }
-      if (t.col0 == 0) p.part_n[(int64_t)b * p.tiles + t.tile] = N;
+    // a thread per channel; means as distances from one of them
+    const int stride = kThreads / t.rows_at_once, first = t.col0 - t.tx * VEC;
+    int N = 0, some = 0;
+    for (int i = t.rows_at_once - 1; i >= 0; i--) {
+      N += red_n[i];
+      if (red_n[i]) some = i;
     }
+    for (int c = threadIdx.x; c < tile_columns(p.C / VEC) * VEC && first + c < p.C; c += kThreads) {
+      const int j = c % VEC, tx = c / VEC;
+      const float ref = red[(some * VEC + j) * stride + tx].x;
+      float s = 0.0f, q = 0.0f;
+      for (int i = 0; i < t.rows_at_once; i++)
+        if (red_n[i]) s += (float)red_n[i] * (red[(i * VEC + j) * stride + tx].x - ref);
+      const float delta = N ? s / (float)N : 0.0f;
+      for (int i = 0; i < t.rows_at_once; i++) {
+        const float2 u = red[(i * VEC + j) * stride + tx];
+        const float d = u.x - ref - delta;
+        if (red_n[i]) q += u.y + d * d * (float)red_n[i];
+      }
+      p.part[((int64_t)b * p.tiles + t.tile) * p.C + first + c] = make_float2(N ? ref + delta : 0.0f, q);
+    }
+    if (first == 0 && threadIdx.x == 0) p.part_n[(int64_t)b * p.tiles + t.tile] = N;
     __syncthreads();
   }
 }
 
-// Merges the tiles and channels of one group: a warp per (board, group).
-__global__ void __launch_bounds__(kThreads) norm_merge_stats_kernel(const __grid_constant__ NormParams p) {
-  const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  if (id >= (int64_t)p.n * p.G) return;
+// Sum over the threads of a block of whole warps, the same for all of them.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < blockDim.x / 32 ? red[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Merges the tiles and channels of one group: a block per (board, group), its threads over the channels of all tiles.
+__global__ void __launch_bounds__(1024) norm_merge_stats_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float red[32];
+  __shared__ int count[kMaxTiles];
+  const int64_t id = blockIdx.x;
   const int b = (int)(id / p.G), g = (int)(id % p.G);
   const float2* part = p.part + (int64_t)b * p.tiles * p.C + (int64_t)g * p.cg;
-  const int* pn = p.part_n + (int64_t)b * p.tiles;
-  const int64_t items = (int64_t)p.tiles * p.cg;
-  double s = 0.0, N = 0.0;
-  for (int64_t i = lane; i < items; i += 32) {
-    const int t = (int)(i / p.cg);
-    const int k = pn[t];
-    N += k;
-    s += (double)k * part[(int64_t)t * p.C + i % p.cg].x;
+  for (int t = threadIdx.x; t < p.tiles; t += blockDim.x) count[t] = p.part_n[(int64_t)b * p.tiles + t];
+  __syncthreads();
+  float N = 0.0f;
+  int some = 0;
+  for (int t = p.tiles - 1; t >= 0; t--) {
+    N += (float)count[t];
+    if (count[t]) some = t;
   }
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    N += __shfl_xor_sync(0xffffffffu, N, o);
-  }
-  const double mu = N > 0.0 ? s / N : 0.0;
-  double q = 0.0;
-  for (int64_t i = lane; i < items; i += 32) {
-    const int t = (int)(i / p.cg);
-    const int k = pn[t];
-    const float2 u = part[(int64_t)t * p.C + i % p.cg];
-    const float d = (float)(u.x - mu);
-    if (k) q += u.y + d * d * (float)k;
-  }
-  for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-  if (lane == 0) {
-    const float2 st = N > 0.0 ? make_float2((float)mu, 1.0f / sqrtf((float)(q / N) + p.eps)) : make_float2(0.0f, 0.0f);
-    p.coef[id] = st;
-    if (p.stats) p.stats[id] = st;
-  }
+  N *= (float)p.cg;
+  const float ref = part[(int64_t)some * p.C].x;
+  // thread -> (tile, channel) with the step of a block's threads
+  const int lanes = min(p.cg, (int)blockDim.x), c0 = threadIdx.x % lanes, t0 = threadIdx.x / lanes;
+  const int tiles_at_once = blockDim.x / lanes;
+  float s = 0.0f;
+  for (int t = t0; t < p.tiles && t0 < tiles_at_once; t += tiles_at_once)
+    if (count[t])
+#pragma unroll 4
+      for (int c = c0; c < p.cg; c += lanes) s += (float)count[t] * (part[(int64_t)t * p.C + c].x - ref);
+  s = block_sum(s, red);
+  const float delta = N > 0.0f ? s / N : 0.0f;
+  float q = 0.0f;
+  for (int t = t0; t < p.tiles && t0 < tiles_at_once; t += tiles_at_once)
+    if (count[t])
+#pragma unroll 4
+      for (int c = c0; c < p.cg; c += lanes) {
+        const float2 u = part[(int64_t)t * p.C + c];
+        const float d = u.x - ref - delta;
+        q += u.y + d * d * (float)count[t];
+      }
+  q = block_sum(q, red);
+  if (threadIdx.x == 0)
+    p.coef[id] = final_stats(ref + delta, N > 0.0f ? q / N : 0.0f, N > 0.0f, p.eps, p.stats, id);
 }
 
 template <typename T, int VEC>
@@ -1138,14 +1173,23 @@ __global__ void __launch_bounds__(kThreads) norm_tile_apply_kernel(const __grid_
       a[j] = st.y * (p.weight ? __ldg(p.weight + t.col0 + j) : 1.0f);
       bias[j] = p.bias ? __ldg(p.bias + t.col0 + j) : 0.0f;
     }
-    for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += t.rows_at_once) {
-      float v[VEC] = {};
-      if (point_on(p, b, r)) {
-        load_pack<T, VEC>(x + (int64_t)r * p.xr, v);
+    for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += kRowsAhead * t.rows_at_once) {
+      float v[kRowsAhead][VEC] = {};
+      bool on[kRowsAhead];
+      rows_ahead(p, b, r, t.rows_at_once, r1, on);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = norm_act((v[j] - mean[j]) * a[j] + bias[j], p.act);
+      for (int i = 0; i < kRowsAhead; i++)
+        if (on[i]) load_pack<T, VEC>(x + (int64_t)(r + i * t.rows_at_once) * p.xr, v[i]);
+#pragma unroll
+      for (int i = 0; i < kRowsAhead; i++) {
+        const int ri = r + i * t.rows_at_once;
+        if (ri >= r1) break;
+        if (on[i]) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) v[i][j] = norm_act((v[i][j] - mean[j]) * a[j] + bias[j], p.act);
+        }
+        store_pack<T, VEC>(y + (int64_t)ri * p.yr, v[i]);
       }
-      store_pack<T, VEC>(y + (int64_t)r * p.yr, v);
     }
   }
 }
@@ -1198,17 +1242,26 @@ __global__ void __launch_bounds__(kThreads) norm_tile_back_kernel(const __grid_c
       const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.xb + t.col0;
       const T* dy = static_cast<const T*>(p.dy) + (int64_t)b * p.yb + t.col0;
       const Channel<VEC> c = load_channel<VEC>(p, b, t.col0);
-      for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += t.rows_at_once) {
-        if (!point_on(p, b, r)) continue;
-        float v[VEC], g[VEC];
-        load_pack<T, VEC>(x + (int64_t)r * p.xr, v);
-        load_pack<T, VEC>(dy + (int64_t)r * p.yr, g);
-        back_vec<VEC>(c, p.act, v, g);
-        cnt++;
+      for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += kBackRows * t.rows_at_once) {
+        float v[kBackRows][VEC], g[kBackRows][VEC];
+        bool on[kBackRows];
+        rows_ahead(p, b, r, t.rows_at_once, r1, on);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          s1[j] += g[j];
-          s2[j] += g[j] * v[j];
+        for (int i = 0; i < kBackRows; i++)
+          if (on[i]) {
+            load_pack<T, VEC>(x + (int64_t)(r + i * t.rows_at_once) * p.xr, v[i]);
+            load_pack<T, VEC>(dy + (int64_t)(r + i * t.rows_at_once) * p.yr, g[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < kBackRows; i++) {
+          if (!on[i]) continue;
+          back_vec<VEC>(c, p.act, v[i], g[i]);
+          cnt++;
+#pragma unroll
+          for (int j = 0; j < VEC; j++) {
+            s1[j] += g[i][j];
+            s2[j] += g[i][j] * v[i][j];
+          }
         }
       }
     }
@@ -1219,54 +1272,53 @@ __global__ void __launch_bounds__(kThreads) norm_tile_back_kernel(const __grid_c
       if (t.tx == 0) red_n[t.ty] = cnt;
     }
     __syncthreads();
-    if (t.active && t.ty == 0) {
+    const int stride = kThreads / t.rows_at_once, first = t.col0 - t.tx * VEC;
+    // a thread per channel
+    for (int c = threadIdx.x; c < tile_columns(p.C / VEC) * VEC && first + c < p.C; c += kThreads) {
+      float2 s = make_float2(0.0f, 0.0f);
+      for (int i = 0; i < t.rows_at_once; i++) {
+        const float2 u = red[(i * VEC + c % VEC) * stride + c / VEC];
+        s.x += u.x;
+        s.y += u.y;
+      }
+      p.part[((int64_t)b * p.tiles + t.tile) * p.C + first + c] = s;
+    }
+    if (first == 0 && threadIdx.x == 0) {
       int N = 0;
       for (int i = 0; i < t.rows_at_once; i++) N += red_n[i];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int i = 0; i < t.rows_at_once; i++) {
-          const float2 u = red[(i * VEC + j) * (kThreads / t.rows_at_once) + t.tx];
-          s.x += u.x;
-          s.y += u.y;
-        }
-        p.part[((int64_t)b * p.tiles + t.tile) * p.C + t.col0 + j] = s;
-      }
-      if (t.col0 == 0) p.part_n[(int64_t)b * p.tiles + t.tile] = N;
+      p.part_n[(int64_t)b * p.tiles + t.tile] = N;
     }
     __syncthreads();
   }
 }
 
-// Adds the tiles of one group's channels and makes its c1, c2: a warp per (board, group).
-__global__ void __launch_bounds__(kThreads) norm_merge_back_kernel(const __grid_constant__ NormParams p) {
-  const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  if (id >= (int64_t)p.n * p.G) return;
+// Adds the tiles of one group's channels and makes its c1, c2: a block per (board, group), its threads over channels.
+__global__ void __launch_bounds__(1024) norm_merge_back_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float red[32];
+  const int64_t id = blockIdx.x;
   const int b = (int)(id / p.G), g = (int)(id % p.G);
-  const int* pn = p.part_n + (int64_t)b * p.tiles;
-  double N = 0.0;
-  for (int t = 0; t < p.tiles; t++) N += pn[t];
-  N *= p.cg;
-  double c1 = 0.0, c2 = 0.0;
-  for (int i = lane; i < p.cg; i += 32) {
+  float N = 0.0f;
+  for (int t = 0; t < p.tiles; t++) N += (float)p.part_n[(int64_t)b * p.tiles + t];
+  N *= (float)p.cg;
+  float c1 = 0.0f, c2 = 0.0f;
+  for (int i = threadIdx.x; i < p.cg; i += blockDim.x) {
     const int c = g * p.cg + i;
+    const float2* part = p.part + (int64_t)b * p.tiles * p.C + c;
     float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll 8
     for (int t = 0; t < p.tiles; t++) {
-      const float2 u = p.part[((int64_t)b * p.tiles + t) * p.C + c];
+      const float2 u = part[(int64_t)t * p.C];
       s.x += u.x;
       s.y += u.y;
     }
     p.sums[(int64_t)b * p.C + c] = s;
     const float w = p.weight ? __ldg(p.weight + c) : 1.0f;
-    c1 += (double)w * s.x;
-    c2 += (double)w * s.y;
+    c1 += w * s.x;
+    c2 += w * s.y;
   }
-  for (int o = 16; o > 0; o >>= 1) {
-    c1 += __shfl_xor_sync(0xffffffffu, c1, o);
-    c2 += __shfl_xor_sync(0xffffffffu, c2, o);
-  }
-  if (lane == 0) p.coef[id] = N > 0.0 ? make_float2((float)(c1 / N), (float)(c2 / N)) : make_float2(0.0f, 0.0f);
+  c1 = block_sum(c1, red);
+  c2 = block_sum(c2, red);
+  if (threadIdx.x == 0) p.coef[id] = N > 0.0f ? make_float2(c1 / N, c2 / N) : make_float2(0.0f, 0.0f);
 }
 
 template <typename T, int VEC>
@@ -1282,16 +1334,28 @@ __global__ void __launch_bounds__(kThreads) norm_tile_dx_kernel(const __grid_con
     float2 k[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) k[j] = p.coef[(int64_t)b * p.G + (t.col0 + j) / p.cg];
-    for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += t.rows_at_once) {
-      float v[VEC], g[VEC], o[VEC] = {};
-      if (point_on(p, b, r)) {
-        load_pack<T, VEC>(x + (int64_t)r * p.xr, v);
-        load_pack<T, VEC>(dy + (int64_t)r * p.yr, g);
-        back_vec<VEC>(c, p.act, v, g);
+    for (int r = t.tile * p.tile_rows + t.ty; r < r1; r += kBackRows * t.rows_at_once) {
+      float v[kBackRows][VEC], g[kBackRows][VEC];
+      bool on[kBackRows];
+      rows_ahead(p, b, r, t.rows_at_once, r1, on);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) o[j] = (g[j] * c.w[j] - k[j].x - v[j] * k[j].y) * c.rstd[j];
+      for (int i = 0; i < kBackRows; i++)
+        if (on[i]) {
+          load_pack<T, VEC>(x + (int64_t)(r + i * t.rows_at_once) * p.xr, v[i]);
+          load_pack<T, VEC>(dy + (int64_t)(r + i * t.rows_at_once) * p.yr, g[i]);
+        }
+#pragma unroll
+      for (int i = 0; i < kBackRows; i++) {
+        const int ri = r + i * t.rows_at_once;
+        if (ri >= r1) break;
+        float o[VEC] = {};
+        if (on[i]) {
+          back_vec<VEC>(c, p.act, v[i], g[i]);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) o[j] = (g[i][j] * c.w[j] - k[j].x - v[i][j] * k[j].y) * c.rstd[j];
+        }
+        store_pack<T, VEC>(dx + (int64_t)ri * p.xr, o);
       }
-      store_pack<T, VEC>(dx + (int64_t)r * p.xr, o);
     }
   }
 }
@@ -1408,6 +1472,9 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
       ok = fits(threads, cs, kMaxSlots) && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem / 2 - 1024;
   for (int cs = 2; cs <= 16 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots) || fits(512, cs, kMaxSlots);
   if (!ok) return false;
+  // narrow vectors hold little each: many turns of large clusters, where tiles of rows take fewer (40 boards of 5,000 x
+  // 99 channels, f16: 228 us in clusters of 16, 100 us in tiles)
+  if (vec * es < 8 && s.cs > 4) return false;
   // few boards: spread one over more SMs
   while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < kSms) fits(s.threads, s.cs * 2, kMaxSlots);
   s.vdiv = (1u << 20) / (uint32_t)(s.cw / vec) + 1;
@@ -1487,14 +1554,20 @@ void launch_params(const NormParams& p, int rows, cudaStream_t st) {
   KC_CUDA(cudaGetLastError());
 }
 
+// A block per (board, group), of threads for its items.
+unsigned merge_blocks(const NormParams& p) {
+  if ((int64_t)p.n * p.G > 0x7fffffff) bad("more groups than one launch takes");
+  return (unsigned)((int64_t)p.n * p.G);
+}
+unsigned merge_threads(int64_t items) { return (unsigned)std::min<int64_t>(1024, (items + 31) / 32 * 32); }
+
 template <typename T, int VEC>
 void split_forward(const NormParams& p, cudaStream_t st) {
-  const int V = p.C / VEC, vc = std::min(V, 64);
+  const int V = p.C / VEC, vc = tile_columns(V);
   const dim3 grid((unsigned)(p.tiles * ((V + vc - 1) / vc)), (unsigned)std::min(p.n, 65535));
-  const unsigned warps = (unsigned)(((int64_t)p.n * p.G + kThreads / 32 - 1) / (kThreads / 32));
   norm_tile_stats_kernel<T, VEC><<<grid, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
-  norm_merge_stats_kernel<<<warps, kThreads, 0, st>>>(p);
+  norm_merge_stats_kernel<<<merge_blocks(p), merge_threads((int64_t)p.cg * p.tiles), 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
   norm_tile_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
@@ -1502,12 +1575,11 @@ void split_forward(const NormParams& p, cudaStream_t st) {
 
 template <typename T, int VEC>
 void split_backward(const NormParams& p, cudaStream_t st) {
-  const int V = p.C / VEC, vc = std::min(V, 64);
+  const int V = p.C / VEC, vc = tile_columns(V);
   const dim3 grid((unsigned)(p.tiles * ((V + vc - 1) / vc)), (unsigned)std::min(p.n, 65535));
-  const unsigned warps = (unsigned)(((int64_t)p.n * p.G + kThreads / 32 - 1) / (kThreads / 32));
   norm_tile_back_kernel<T, VEC><<<grid, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
-  norm_merge_back_kernel<<<warps, kThreads, 0, st>>>(p);
+  norm_merge_back_kernel<<<merge_blocks(p), merge_threads(p.cg), 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
   norm_tile_dx_kernel<T, VEC><<<grid, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
