@@ -1443,7 +1443,7 @@ size_t resident_smem(ResShape& s, int vec, int unit, int es, int cg, bool backwa
 // Channels of a vector that are sure to lie in one group.
 int unit_of(int vec, int cg) { return vec >= 4 && cg % vec == 0 ? vec : vec >= 4 && cg % 4 == 0 ? 4 : 1; }
 
-// The chunk, cluster and block of a resident launch; false where a board's group does not fit 8 blocks.
+// The chunk, cluster and block of a resident launch; false where a board's group does not fit 16 blocks.
 bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShape& s) {
   const int es = dtype_bytes(d.dtype), cg = d.channels / d.groups, unit = unit_of(vec, cg);
   const int base = lcm_of(cg, vec);
