@@ -236,7 +236,7 @@ int kc_gpool_fc_noalloc(const float* d_x, const float* d_mask, int n, int c, con
  * stream) without a host wait or an allocation, so that calls can be captured into a CUDA graph; the device need not
  * be current. Strides are in elements and not negative; rows of an output must not share memory. An output may be
  * the input of its own shape (same pointer and strides: in place); any other overlap of an output is refused.
- * `d_workspace` (256-byte aligned, contents not kept) must not be used by two calls that can overlap on the GPU, nor
+ * `d_workspace` (16-byte aligned, contents not kept) must not be used by two calls that can overlap on the GPU, nor
  * be freed before a graph that captured it. Calls on different streams are otherwise independent. Results do not
  * depend on timing: the same call gives the same bits.
  * --------------------------------------------------------------------------------------------------------------- */
