@@ -86,3 +86,37 @@ def test_single_token_serving():
     for i in range(tokens):
         got = t.rope_forward(q[i:i + 1], k[i:i + 1], pos[i:i + 1], freqs, hd, "pairs")
         assert torch.equal(got[0][0], want[0][i]) and torch.equal(got[1][0], want[1][i])
+
+
+def test_host_threads_on_streams_of_their_own():
+    """Four host threads, each on its own stream, while the others call too: the same bits as alone."""
+    import threading
+
+    def work(seed, out):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(20, 361, 48 + 24 * seed, device="cuda", generator=g).bfloat16()
+        w, b = torch.ones(x.shape[2], device="cuda"), torch.zeros(x.shape[2], device="cuda")
+        q = torch.randn(4000, 4, 64, device="cuda", generator=g).bfloat16()
+        pos = torch.randint(0, 361, (4000, 2), device="cuda", generator=g, dtype=torch.int32)
+        freqs = torch.randn(2, 32, 2, device="cuda", generator=g)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                y, stats = t.norm_forward(x, None, w, b, 6, "mish")
+                r = (y, stats) + t.norm_backward(x, None, w, b, stats, x, 6, "mish")
+                r += t.rope_forward(q, q, pos, freqs, 64, "halves")
+                r += t.rope_backward(q, q, q, q, pos, freqs, 64, "halves")
+        stream.synchronize()
+        out[seed] = r
+
+    alone, together = {}, {}
+    for seed in range(4):
+        work(seed, alone)
+    threads = [threading.Thread(target=work, args=(seed, together)) for seed in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for seed in range(4):
+        assert all(torch.equal(a, c) for a, c in zip(alone[seed], together[seed]))
