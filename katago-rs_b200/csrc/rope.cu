@@ -693,8 +693,8 @@ unsigned grid_of(int64_t threads) {
 
 template <auto kernel>
 void launch_kernel(const RopeParams& p, dim3 grid, size_t smem, cudaStream_t st) {
-  if (smem > 48 * 1024) {
-    static std::atomic<uint64_t> allowed[2];  // devices on which this kernel may take more than 48 KB
+  if (smem > 0) {  // what a block gets unasked, 48 KB, has to hold the kernel's own shared memory too
+    static std::atomic<uint64_t> allowed[2];  // devices on which this kernel may take more
     int dev = 0;
     KC_CUDA(cudaGetDevice(&dev));
     if (dev >= 128) bad("device index above 127");

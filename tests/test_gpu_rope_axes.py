@@ -257,3 +257,30 @@ def test_host_memory_is_refused():
         api.rope_axes(d, q.data_ptr(), k.data_ptr(), pos.cpu().data_ptr(), freqs.data_ptr(), q.data_ptr(), k.data_ptr(),
                       t.stream())
     assert e.value.status == api.KC_ERR_INVALID and "device memory" in str(e.value)
+
+
+def learned_backward(tokens, hq, hk, hd, axes, tables, dtype):
+    """One backward pass with the frequencies' gradient, against float64."""
+    wide, q, k, pos, freqs, g = make(tokens, hq, hk, hd, hd, axes, tables, dtype, 43)
+    dq_out, dk_out = (torch.randn(v.shape, device="cuda", generator=g).to(q.dtype) for v in (q, k))
+    dq, dk, df = t.rope_backward(dq_out, dk_out, q, k, pos, freqs, hd, "halves")
+    check(dq, dq_out, pos, freqs, hd, "halves", back=True)
+    check(dk, dk_out, pos, freqs, hd, "halves", back=True)
+    want, size = t.freqs_back64(dq_out, q, dk_out, k, pos, freqs, hd, "halves")
+    t.within(df, want, (2 * S + 2.0**-17) * size)
+
+
+@pytest.mark.parametrize("tokens,hq,hk,hd,axes,tables,dtype", [
+    (4440, 12, 12, 64, 4, 12, "bf16"), (13804, 12, 12, 96, 2, 12, "bf16"), (20000, 12, 12, 64, 4, 12, "f16")])
+def test_first_call_with_tiles_near_48_kb(tokens, hq, hk, hd, axes, tables, dtype):
+    """The tiles alone stay below the 48 KB that a block gets unasked, with the kernel's own shared memory they pass
+    it. A fresh process each: an earlier call of the same kernel may have raised its limit."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import sys; sys.path[:0] = %r; import test_gpu_rope_axes as m; m.learned_backward%r" % (
+        [here, os.path.join(os.path.dirname(here), "katago-rs_b200", "python")],
+        (tokens, hq, hk, hd, axes, tables, dtype))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
