@@ -262,10 +262,11 @@ int kc_group_norm_act_workspace(const kc_group_norm_desc* desc, int backward, si
 
 /* y = act((x - mean) * rstd * weight[c] + bias[c]) at the points whose mask is not 0, 0 at the others, where mean and
  * rstd = 1 / sqrt(variance + eps) are those of the point's board and channel group over the points that are on
- * (whatever x holds at the others, NaN and infinities too, has no effect). Squares are float32: where x lies
- * 1e19 or more from the mean its group's results are not numbers. d_mask: [n][points] float32 rows at
- * mask_board_stride, NULL = every point; d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not
- * wanted): [n][groups][2] float32 mean and rstd, both 0 for a board without points. */
+ * (whatever x holds at the others, NaN and infinities too, has no effect). Squares are summed in float32: where a
+ * group's sum of squared distances from one of its values passes 3.4e38 (distances of 2.8e17 in 361 points x 12
+ * channels) its y and rstd are NaN. d_mask: [n][points] float32 rows at mask_board_stride, NULL = every point;
+ * d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not wanted): [n][groups][2] float32 mean and
+ * rstd, both 0 for a board without points. */
 int kc_group_norm_act(const kc_group_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
                       const float* d_bias, void* d_y, float* d_stats, void* d_workspace, size_t workspace_bytes,
                       void* stream);

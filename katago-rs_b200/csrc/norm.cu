@@ -456,10 +456,11 @@ __device__ __forceinline__ void zero_rows(uint32_t which, T* y, uint32_t step) {
 extern __shared__ __align__(16) unsigned char norm_smem[];
 
 // A group's (mean, rstd), also into the statistics the caller wants. 1 / sqrt by the fast function (2^-22) and one
-// Newton step; a variance of 0 with eps 0 gives infinity.
+// Newton step; a variance of 0 with eps 0 gives infinity, one whose squares passed float32's range NaN (1 / sqrt would
+// be 0, and the outputs those of a board of equal values).
 __device__ __forceinline__ float2 final_stats(float mean, float var, bool any, float eps, float2* stats, int64_t g) {
   const float v = (var < 0.0f ? 0.0f : var) + eps;
-  float r = rsqrtf(v);
+  float r = v <= 3.402823466e38f ? rsqrtf(v) : __int_as_float(0x7fc00000);
   if (v > 0.0f && v < 1e38f) r = r * (1.5f - 0.5f * v * r * r);
   const float2 st = any ? make_float2(mean, r) : make_float2(0.0f, 0.0f);
   if (stats) stats[g] = st;

@@ -467,3 +467,27 @@ def test_many_shapes():
         dy = torch.randn(x.shape, device="cuda", generator=g).to(x.dtype)
         got = t.norm_backward(x, mask, w, b, stats, dy, groups, act)
         check_backward(x, mask, w, b, stats, dy, groups, act, got)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,points,channels,groups", [(3, 361, 64, 8), (2, 361, 21, 7), (2, 9000, 64, 8),
+                                                      (2, 60000, 24, 8), (2, 20000, 512, 2), (3, 6, 64, 8)])
+def test_squares_beyond_float32(n, points, channels, groups, dtype):
+    """Where a group's sum of squares passes float32's range its results are not numbers, never those of another
+    variance; other groups and boards, and values whose squares stay within it, are as ever."""
+    cg = channels // groups
+    _, x, w, b, g = make(n, points, channels, dtype, 61, scale=1.0, shift=0.0)
+    mask = masks("boards", n, points, g)
+    on = (mask != 0)[:, :, None]
+    x[1, :, cg:2 * cg] = (x[1, :, cg:2 * cg].float() * 4e19).to(x.dtype)
+    for act in t.ACTS:
+        y, stats = t.norm_forward(x, mask, w, b, groups, act)
+        hit = torch.zeros_like(y, dtype=torch.bool)
+        hit[1, :, cg:2 * cg] = True
+        assert torch.isnan(y[hit & on]).all() and torch.isfinite(y[~hit | ~on]).all() and y[~on.expand_as(y)].eq(0).all()
+        assert torch.isnan(stats[1, 1, 1]) and torch.isnan(stats).sum() <= 2
+        dx, _, _ = t.norm_backward(x, mask, w, b, stats, torch.ones_like(x), groups, act)
+        assert torch.isnan(dx[hit & on]).all() and torch.isfinite(dx[~hit | ~on]).all()
+    x[1, :, cg:2 * cg] = (torch.randn(points, cg, device="cuda", generator=g) * 1e16).to(x.dtype)
+    y, stats = t.norm_forward(x, mask, w, b, groups, "identity")
+    check_forward(x, mask, w, b, groups, "identity", y, stats)
