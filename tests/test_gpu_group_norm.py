@@ -491,3 +491,23 @@ def test_squares_beyond_float32(n, points, channels, groups, dtype):
     x[1, :, cg:2 * cg] = (torch.randn(points, cg, device="cuda", generator=g) * 1e16).to(x.dtype)
     y, stats = t.norm_forward(x, mask, w, b, groups, "identity")
     check_forward(x, mask, w, b, groups, "identity", y, stats)
+
+
+@pytest.mark.parametrize("act", ["mish", "silu"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("points,channels", [(64, 8), (361, 384), (9000, 64), (9000, 384)])
+def test_tails_keep_their_digits(points, channels, dtype, act):
+    """z from -12.4 to 8.4. Below -5 |y'(z) / y| is at most 1, so that an error of z, K24 of its terms, is a relative
+    error of y; exponential, products and quotient add less than another K24 of y: the type's rounding is what is
+    left in the 2-byte types."""
+    x = torch.linspace(-1, 1, points, device="cuda")[None, :, None].repeat(2, 1, channels).to(t.DTYPES[dtype])
+    w, b = torch.full((channels,), 6.0, device="cuda"), torch.full((channels,), -2.0, device="cuda")
+    on = torch.ones(2, points, dtype=torch.bool, device="cuda")
+    y, stats = t.norm_forward(x, None, w, b, 1, act)
+    want, mean, rstd, xh, z = t.norm64(x, on, w, b, 1, act)
+    half, tiny = t.half_step(x.dtype)
+    zsize = (xh.abs() + rstd.max()) * 6 + 2
+    tail = z < -5
+    assert z.min() < -12 and tail.any()
+    tol = want.abs() * (half + K24 * (1 + zsize)) * 1.01 + tiny
+    t.within(y[tail], want[tail], tol[tail])
