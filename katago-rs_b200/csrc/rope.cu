@@ -69,11 +69,12 @@ struct alignas(N * sizeof(T)) Pack {
   T v[N];
 };
 
-// freq / (2 pi) mod 1, times 2^64. A frequency that is not finite gives 0 here; its angle is made NaN apart.
+// freq / (2 pi) mod 1, times 2^64. The distance from the nearest whole turn, exact in float64, keeps the digits of a
+// small frequency of either sign (from the turn below, a negative one's would be 1 less them). Half a turn saturates
+// to 2^-64 below it. A frequency that is not finite gives no angle; its sines are made NaN apart.
 __device__ __forceinline__ unsigned long long turn_fraction(float freq) {
   const double t = (double)freq * 0.15915494309189533577;  // 1 / (2 pi)
-  const double f = t - floor(t);
-  return f >= 0.0 && f < 1.0 ? (unsigned long long)(f * 18446744073709551616.0) : 0ull;
+  return (unsigned long long)__double2ll_rz((t - rint(t)) * 18446744073709551616.0);
 }
 
 __device__ __forceinline__ float sin_fast(float x) {

@@ -284,3 +284,18 @@ def test_first_call_with_tiles_near_48_kb(tokens, hq, hk, hd, axes, tables, dtyp
         (tokens, hq, hk, hd, axes, tables, dtype))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("tokens", [64, 60000])
+def test_far_positions_with_small_frequencies(tokens, sign):
+    """Frequencies of either sign keep their digits at the far end of int32. The rotated (1, 0) is (cos, sin): the
+    angle is off by the rounding of half a turn to 24 bits, pi 2^-25, and 3e-9 of the fraction and the float64
+    reference; the function by 2^-24, the result's rounding by 2^-24 and the sum's by another: below 2^-21 in all."""
+    g = torch.Generator(device="cuda").manual_seed(47)
+    pos = torch.randint(2**30, 2**31 - 1, (tokens, 1), device="cuda", generator=g, dtype=torch.int32)
+    freqs = sign * torch.empty(1, 32, 1, device="cuda").uniform_(1e-4, 1e-2, generator=g)
+    x = torch.cat([torch.ones(tokens, 2, 32, device="cuda"), torch.zeros(tokens, 2, 32, device="cuda")], 2)
+    q_out, _ = t.rope_forward(x, None, pos, freqs, 64, "halves")
+    want, _ = t.turn64(x, pos, freqs, 64, "halves")
+    t.within(q_out, want, 2.0**-21)
