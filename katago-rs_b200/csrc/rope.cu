@@ -91,16 +91,31 @@ __device__ __forceinline__ float cos_fast(float x) {
 // n / d by magic(d).
 __device__ __forceinline__ int quotient(int n, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)n, magic) : n; }
 
-// (cos, sin) of an angle of turns * 2^-64. float32 takes the accurate functions; for 2-byte results the fast ones on
-// half a turn either way (off by 2^-21) are far below the rounding.
+// (cos, sin) of an angle of turns * 2^-64, for results of T. 2-byte results take the fast functions on half a turn either
+// way (off by 2^-21, far below the rounding). float32 ones, the frequencies' gradient among them whatever the heads'
+// type, take polynomials in an eighth of a turn either way from the nearest quarter, y = 8 * angle / turn in [-1, 1]:
+// sin(y pi / 4) = y (pi / 4 + y^2 P(y^2)), cos(y pi / 4) = 1 + y^2 Q(y^2), P and Q with the least largest error (2e-9
+// and 5e-11 of the result, by weighted least squares), pi / 4 in two floats. Off by at most 7.5e-8.
 template <typename T>
 __device__ __forceinline__ float2 turned(unsigned long long turns) {
-  const float part = (float)(int)(turns >> 32);  // in 2^-32 turns, [-2^31, 2^31)
+  const uint32_t part = (uint32_t)(turns >> 32);  // in 2^-32 turns
   float2 r;
   if constexpr (sizeof(T) == 4) {
-    sincospif(part * 4.656612873077393e-10f, &r.y, &r.x);  // 2^-31
+    const uint32_t q = part + 0x20000000u;  // the nearest quarter in the upper two bits
+    const float y = (float)(int)(part - (q & 0xc0000000u)) * 0x1p-29f, z = y * y;
+    float u = fmaf(z, -3.59389829e-05f, 2.48998965e-03f);
+    u = fmaf(u, z, -8.07454347e-02f);
+    u = fmaf(u, z, -2.18556941e-08f);
+    float v = fmaf(z, 3.53132860e-06f, -3.25941998e-04f);
+    v = fmaf(v, z, 1.58543277e-02f);
+    v = fmaf(v, z, -3.08425136e-01f);
+    u = fmaf(y, 0.785398185f, y * u);
+    v = fmaf(v, z, 1.0f);
+    const bool odd = q & 0x40000000u;
+    r.x = __uint_as_float(__float_as_uint(odd ? u : v) ^ ((q + 0x40000000u) & 0x80000000u));
+    r.y = __uint_as_float(__float_as_uint(odd ? v : u) ^ (q & 0x80000000u));
   } else {
-    const float x = part * 1.4629180792671596e-09f;  // 2 pi 2^-32
+    const float x = (float)(int)part * 1.4629180792671596e-09f;  // 2 pi 2^-32
     r.x = cos_fast(x);
     r.y = sin_fast(x);
   }
@@ -183,8 +198,9 @@ struct Pairs {
 };
 
 // One vector of one head of one token to a thread, which makes its own angles: for few tokens, where a launch is
-// latency, and for what the tiles cannot take. Threads over (token, table, head, vector).
-template <typename T, int VP, int LAYOUT>
+// latency, and for what the tiles cannot take. Threads over (token, table, head, vector). S: the type that the sines
+// are good for.
+template <typename T, int VP, int LAYOUT, typename S>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeParams p) {
   const int heads = p.q.per_table + p.k.per_table, pv = p.pairs / VP, cols = pv + p.rest / VP;
   const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, per_token = (int64_t)p.tables * heads * cols;
@@ -204,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   Pairs<T, VP, LAYOUT> x;
   x.load(in, col * VP, p.pairs);
   float c[VP], s[VP];
-  angles<T, VP>(p, t, p.freqs + ((int64_t)table * p.pairs + col * VP) * p.axes, c, s);
+  angles<S, VP>(p, t, p.freqs + ((int64_t)table * p.pairs + col * VP) * p.axes, c, s);
 #pragma unroll
   for (int j = 0; j < VP; j++) {
     float a, b;
@@ -448,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) rope_axes_back_kernel(c
   f32x2 acc[AXES][NP] = {};
   for (int64_t t0 = (int64_t)blockIdx.x * p.tile; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.tile) {
     const int tokens = (int)min((int64_t)p.tile, p.tokens - t0);
-    tile_sines<T, VP>(p, tile, t0, tokens, finite);
+    tile_sines<float, VP>(p, tile, t0, tokens, finite);
     for (int tt = lane; here && tt < tokens; tt += p.lanes) {
       const uint32_t t = (uint32_t)t0 + tt;
       if (col >= pv) {
@@ -532,7 +548,7 @@ __global__ void __launch_bounds__(kThreads) rope_freqs_direct_kernel(const __gri
   float acc[KC_ROPE_MAX_AXES] = {};
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     float c[1], s[1], turn = 0.0f;
-    angles<T, 1>(p, t, p.freqs + (int64_t)e * p.axes, c, s);
+    angles<float, 1>(p, t, p.freqs + (int64_t)e * p.axes, c, s);
     for (int i = 0; i < p.q.per_table + p.k.per_table; i++) {
       const bool is_q = i < p.q.per_table;
       const Heads& h = is_q ? p.q : p.k;
@@ -744,7 +760,7 @@ void launch_back(RopeParams p, cudaStream_t st) {
   } else {  // before the gradients, which may take the place of what it reads
     launch_kernel<rope_freqs_direct_kernel<T, LAYOUT>>(
         p, dim3((unsigned)p.blocks, (unsigned)((entries + kThreads - 1) / kThreads)), 0, st);
-    launch_kernel<rope_axes_kernel<T, VP, LAYOUT>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
+    launch_kernel<rope_axes_kernel<T, VP, LAYOUT, float>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
   }
   const int count = p.tables * p.pairs * p.axes;
   rope_freqs_kernel<<<(count + 7) / 8, kThreads, 0, st>>>(p.partial, p.blocks, count, p.dfreqs);
@@ -765,7 +781,7 @@ void launch(RopeParams p, cudaStream_t st) {
   const bool one_wave = p.tokens * p.tables * heads * cols <= kSms * 2048;  // of threads
   if (one_wave || smem > (size_t)kMaxTileBytes || per_token * per_token * p.tile > 0xffffffffll ||
       !small_steps(p, sizeof(T))) {
-    launch_kernel<rope_axes_kernel<T, VP, LAYOUT>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
+    launch_kernel<rope_axes_kernel<T, VP, LAYOUT, T>>(p, dim3(grid_of(p.tokens * p.tables * heads * cols)), 0, st);
     return;
   }
   p.by_token = magic(per_token);

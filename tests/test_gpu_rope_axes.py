@@ -299,3 +299,19 @@ def test_far_positions_with_small_frequencies(tokens, sign):
     q_out, _ = t.rope_forward(x, None, pos, freqs, 64, "halves")
     want, _ = t.turn64(x, pos, freqs, 64, "halves")
     t.within(q_out, want, 2.0**-21)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,tables,hd", [(1, 1, 1024), (2, 2, 256), (64, 64, 128)])  # (64: beyond shared memory)
+def test_gradient_of_frequencies_has_float32_sines(heads, tables, hd, dtype):
+    """It is float32 whatever the heads' type. One token at position 1 with x = (1, 0): the gradient is cos for
+    g = (0, 1) and sin for g = (-1, 0), every product and sum of it exact. The angle is off by pi 2^-25 (half a turn
+    in 24 bits) and 2^-52 more, sine and cosine by 2^-24: below 2^-22."""
+    g = torch.Generator(device="cuda").manual_seed(53)
+    freqs = torch.empty(tables, hd // 2, 1, device="cuda").uniform_(-3.1, 3.1, generator=g)
+    pos = torch.ones(1, 1, dtype=torch.int32, device="cuda")
+    x = torch.cat([torch.ones(1, heads, hd // 2, device="cuda"), torch.zeros(1, heads, hd // 2, device="cuda")], 2)
+    x = x.to(t.DTYPES[dtype])
+    for dy, want in ((x.roll(hd // 2, 2), torch.cos(freqs.double())), (-x, torch.sin(freqs.double()))):
+        _, _, df = t.rope_backward(dy, None, x, None, pos, freqs, hd, "halves")
+        t.within(df, want, 2.0**-22)
