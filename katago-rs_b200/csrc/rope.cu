@@ -197,6 +197,14 @@ struct Pairs {
   }
 };
 
+// (a, b) turned: a c - b s, a s + b c, two pairs at once, with the same roundings in every kernel: one token at a
+// time gives the bits of the whole sequence.
+__device__ __forceinline__ void turn2(f32x2& a, f32x2& b, f32x2 c, f32x2 s) {
+  const f32x2 ya = fma2({-b.x, -b.y}, s, mul2(a, c));
+  b = fma2(a, s, mul2(b, c));
+  a = ya;
+}
+
 // One vector of one head of one token to a thread, which makes its own angles: for few tokens, where a launch is
 // latency, and for what the tiles cannot take. Threads over (token, table, head, vector). S: the type that the sines
 // are good for.
@@ -222,10 +230,12 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   float c[VP], s[VP];
   angles<S, VP>(p, t, p.freqs + ((int64_t)table * p.pairs + col * VP) * p.axes, c, s);
 #pragma unroll
-  for (int j = 0; j < VP; j++) {
-    float a, b;
-    x.get(j, a, b);
-    x.set(j, a * c[j] - b * s[j], a * s[j] + b * c[j]);
+  for (int j = 0; j < VP; j += 2) {
+    f32x2 a, b;
+    x.get2(j, a, b);
+    if constexpr (VP > 1) turn2(a, b, {c[j], c[j + 1]}, {s[j], s[j + 1]});
+    else turn2(a, b, {c[j], 0.0f}, {s[j], 0.0f});
+    x.set2(j, a, b);
   }
   x.store(out, col * VP, p.pairs);
 }
@@ -379,13 +389,6 @@ __device__ __forceinline__ void tile_sines(const RopeParams& p, const Tile<VP>& 
     }
   }
   __syncthreads();
-}
-
-// (a, b) turned: a c - b s, a s + b c, two pairs at once.
-__device__ __forceinline__ void turn2(f32x2& a, f32x2& b, f32x2 c, f32x2 s) {
-  const f32x2 ya = fma2({-b.x, -b.y}, s, mul2(a, c));
-  b = fma2(a, s, mul2(b, c));
-  a = ya;
 }
 
 template <typename T, int VP, int LAYOUT>

@@ -120,3 +120,20 @@ def test_host_threads_on_streams_of_their_own():
         th.join()
     for seed in range(4):
         assert all(torch.equal(a, c) for a, c in zip(alone[seed], together[seed]))
+
+
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_single_token_is_the_long_sequence(dtype, layout):
+    """One token at a time gives the bits of a sequence long enough for the kernel that goes over tiles of tokens."""
+    tokens, hq, hk, hd = 20000, 6, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(59)
+    q, k = (torch.randn(tokens, h, hd, device="cuda", generator=g).to(t.DTYPES[dtype]) for h in (hq, hk))
+    pos = torch.randint(-400, 400, (tokens, 3), device="cuda", generator=g, dtype=torch.int32)
+    freqs = torch.randn(hk, hd // 2, 3, device="cuda", generator=g)
+    want = t.rope_forward(q, k, pos, freqs, hd, layout)
+    for i in range(0, tokens, 397):
+        got = t.rope_forward(q[i:i + 1], k[i:i + 1], pos[i:i + 1], freqs, hd, layout)
+        assert torch.equal(got[0][0], want[0][i]) and torch.equal(got[1][0], want[1][i])
+    few = t.rope_forward(q[:40], k[:40], pos[:40], freqs, hd, layout)
+    assert torch.equal(few[0], want[0][:40]) and torch.equal(few[1], want[1][:40])
