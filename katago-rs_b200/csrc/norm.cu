@@ -1386,23 +1386,25 @@ __global__ void __launch_bounds__(kThreads) norm_params_kernel(const float2* __r
 // ---------------------------------------------------------------------------------------------------------------
 [[noreturn]] void bad(const std::string& m) { fail(KC_ERR_INVALID, "CUDA backend: group norm: " + m); }
 
+Rows x_rows(const kc_group_norm_desc& d, const void* p) {
+  return {p, d.n, d.points, d.channels, d.x_board_stride, d.x_row_stride, dtype_bytes(d.dtype)};
+}
+Rows y_rows(const kc_group_norm_desc& d, const void* p) {
+  return {p, d.n, d.points, d.channels, d.y_board_stride, d.y_row_stride, dtype_bytes(d.dtype)};
+}
+
+// What the workspace query and the calls refuse alike: sizes that the arithmetic of either cannot hold.
 void check_desc(const kc_group_norm_desc* d) {
   if (!d) bad("null descriptor");
   if (d->dtype != KC_PRECISION_F32 && d->dtype != KC_PRECISION_F16 && d->dtype != KC_PRECISION_BF16)
     bad("dtype must be KC_PRECISION_F32, F16 or BF16");
   if (d->act < KC_ACT_IDENTITY || d->act > KC_ACT_SILU) bad("unknown activation");
   if (d->n < 0 || d->points < 0 || d->n > 1 << 30 || d->points > 1 << 30) bad("n and points must be 0 to 2^30");
-  if (d->channels < 1 || d->groups < 1) bad("channels and groups must be positive");
+  if (d->channels < 1 || d->groups < 1 || d->channels > 1 << 30) bad("channels must be 1 to 2^30, groups positive");
   if (d->channels % d->groups != 0) bad("channels must be a multiple of groups");
+  if ((int64_t)d->n * d->channels > (int64_t)1 << 46) bad("n * channels must be at most 2^46");
   if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) bad("eps must be finite and not negative");
   if (d->reserved != 0) bad("reserved must be 0");
-}
-
-Rows x_rows(const kc_group_norm_desc& d, const void* p) {
-  return {p, d.n, d.points, d.channels, d.x_board_stride, d.x_row_stride, dtype_bytes(d.dtype)};
-}
-Rows y_rows(const kc_group_norm_desc& d, const void* p) {
-  return {p, d.n, d.points, d.channels, d.y_board_stride, d.y_row_stride, dtype_bytes(d.dtype)};
 }
 
 // Tiles of rows of the split path: enough blocks for every SM several times over, of at least 32 rows.

@@ -89,6 +89,16 @@ def test_group_norm_of_nothing(n, points):
     backward(d, x=0, dy=0, dx=0, st=0, mask=0, dw=0, db=0, ws=0, size=0)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(dtype=3), dict(act=4), dict(n=-1), dict(points=(1 << 30) + 1), dict(channels=0), dict(groups=7),
+    dict(eps=-1.0), dict(channels=(1 << 30) + 32), dict(channels=(1 << 31) - 1, groups=1), dict(n=1 << 30, points=0, channels=1 << 20)])
+@pytest.mark.parametrize("backward", [False, True])
+def test_workspace_query_refuses_what_the_calls_refuse(kw, backward):
+    d = desc(**kw)
+    refused(api.group_norm_act_workspace, d, backward)
+    refused(forward, d)
+
+
 def test_workspace_null_result():
     assert api.lib().kc_group_norm_act_workspace(desc(), 0, None) == api.KC_ERR_INVALID
     assert api.lib().kc_rope_axes_backward_workspace(rdesc(), None) == api.KC_ERR_INVALID
