@@ -257,7 +257,8 @@ typedef struct kc_group_norm_desc {
   int64_t mask_board_stride;
 } kc_group_norm_desc;
 
-/* Bytes of workspace a call needs (0: d_workspace may be NULL). backward: 0 kc_group_norm_act, 1 its backward. */
+/* Bytes of workspace a call needs (0: d_workspace may be NULL). backward: 0 kc_group_norm_act, 1 its backward. A
+ * descriptor whose sizes or strides the calls refuse is refused here too. */
 int kc_group_norm_act_workspace(const kc_group_norm_desc* desc, int backward, size_t* bytes);
 
 /* y = act((x - mean) * rstd * weight[c] + bias[c]) at the points whose mask is not 0, 0 at the others, where mean and

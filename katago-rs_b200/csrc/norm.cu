@@ -1393,7 +1393,7 @@ Rows y_rows(const kc_group_norm_desc& d, const void* p) {
   return {p, d.n, d.points, d.channels, d.y_board_stride, d.y_row_stride, dtype_bytes(d.dtype)};
 }
 
-// What the workspace query and the calls refuse alike: sizes that the arithmetic of either cannot hold.
+// What the workspace query and the calls refuse alike: sizes and strides that the arithmetic of either cannot hold.
 void check_desc(const kc_group_norm_desc* d) {
   if (!d) bad("null descriptor");
   if (d->dtype != KC_PRECISION_F32 && d->dtype != KC_PRECISION_F16 && d->dtype != KC_PRECISION_BF16)
@@ -1405,6 +1405,8 @@ void check_desc(const kc_group_norm_desc* d) {
   if ((int64_t)d->n * d->channels > (int64_t)1 << 46) bad("n * channels must be at most 2^46");
   if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) bad("eps must be finite and not negative");
   if (d->reserved != 0) bad("reserved must be 0");
+  if (!rows_in_range(x_rows(*d, nullptr)) || !rows_in_range(y_rows(*d, nullptr)))
+    bad("strides must not be negative, nor reach past 2^46 elements");
 }
 
 // Tiles of rows of the split path: enough blocks for every SM several times over, of at least 32 rows.
@@ -1673,10 +1675,8 @@ void check_tensors(const kc_group_norm_desc& d, std::initializer_list<Rows> rows
                    std::initializer_list<const void*> small) {
   const Rows m{mask, d.n, 1, d.points, d.mask_board_stride, 0, 4};
   if (mask && !rows_in_range(m)) bad("mask stride out of range");
-  for (const Rows& r : rows) {
-    if (!rows_in_range(r)) bad("strides must not be negative, nor reach past 2^46 elements");
+  for (const Rows& r : rows)
     if (!aligned_to(r.p, r.bytes)) bad("a tensor is not aligned to its element");
-  }
   for (const void* s : small)
     if (!aligned_to(s, 4)) bad("a float32 tensor is not aligned to its element");
 }

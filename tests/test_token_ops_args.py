@@ -91,7 +91,9 @@ def test_group_norm_of_nothing(n, points):
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=3), dict(act=4), dict(n=-1), dict(points=(1 << 30) + 1), dict(channels=0), dict(groups=7),
-    dict(eps=-1.0), dict(channels=(1 << 30) + 32), dict(channels=(1 << 31) - 1, groups=1), dict(n=1 << 30, points=0, channels=1 << 20)])
+    dict(eps=-1.0), dict(x_strides=(-384, 384)), dict(x_strides=(361 * 384, -1)), dict(y_strides=(361 * 384, -384)),
+    dict(y_strides=(1 << 50, 384)), dict(x_strides=(361 * 384, 1 << 62)), dict(y_strides=((1 << 63) - 1, 384)),
+    dict(channels=(1 << 30) + 32), dict(channels=(1 << 31) - 1, groups=1), dict(n=1 << 30, points=0, channels=1 << 20)])
 @pytest.mark.parametrize("backward", [False, True])
 def test_workspace_query_refuses_what_the_calls_refuse(kw, backward):
     d = desc(**kw)
