@@ -249,7 +249,9 @@ int kc_gpool_fc_noalloc(const float* d_x, const float* d_mask, int n, int c, con
 typedef struct kc_group_norm_desc {
   int32_t dtype; /* KC_PRECISION_* of x, y, dy and dx */
   int32_t act;   /* KC_ACT_* */
-  int32_t n, points, channels, groups; /* n and points 0 .. 2^30, channels 1 .. 2^30, n * channels at most 2^46 */
+  int32_t n, points, channels, groups; /* n and points 0 .. 2^30, channels 1 .. 2^30, n * channels at most 2^46; where
+                                          a group or a board is too large for a cluster of 16 blocks, n * groups
+                                          below 2^31 */
   float eps;     /* >= 0 */
   int32_t reserved; /* 0 */
   int64_t x_board_stride, x_row_stride; /* x and dx */

@@ -1524,6 +1524,7 @@ Layout workspace_layout(const kc_group_norm_desc& d, bool backward) {
   l.total = at;
   l.resident = resident;
   if (resident) return l;
+  if ((int64_t)d.n * d.groups > 0x7fffffff) bad("n * groups above 2^31 - 1");  // a block each in the split path's merge
   int tiles, tile_rows;
   split_shape(d, tiles, tile_rows);
   l.part = take((size_t)d.n * tiles * d.channels * sizeof(float2));
@@ -1553,10 +1554,7 @@ void launch_params(const NormParams& p, int rows, cudaStream_t st) {
 }
 
 // A block per (board, group), of threads for its items.
-unsigned merge_blocks(const NormParams& p) {
-  if ((int64_t)p.n * p.G > 0x7fffffff) bad("more groups than one launch takes");
-  return (unsigned)((int64_t)p.n * p.G);
-}
+unsigned merge_blocks(const NormParams& p) { return (unsigned)((int64_t)p.n * p.G); }  // workspace_layout: below 2^31
 unsigned merge_threads(int64_t items) { return (unsigned)std::min<int64_t>(1024, (items + 31) / 32 * 32); }
 
 template <typename T, int VEC>

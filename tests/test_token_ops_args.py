@@ -101,6 +101,14 @@ def test_workspace_query_refuses_what_the_calls_refuse(kw, backward):
     refused(forward, d)
 
 
+def test_more_groups_than_a_launch():
+    """Refused before anything is launched: boards of more channels than a cluster's tables hold, a group a channel."""
+    d = desc(n=8192, points=1, channels=(1 << 18) + 8, groups=(1 << 18) + 8)
+    assert "n * groups" in refused(api.group_norm_act_workspace, d, False)
+    far = [(1 << 42) + (i << 38) for i in range(8)]
+    assert "n * groups" in refused(forward, d, *far[:6], 1 << 45, 1 << 44)
+
+
 def test_workspace_null_result():
     assert api.lib().kc_group_norm_act_workspace(desc(), 0, None) == api.KC_ERR_INVALID
     assert api.lib().kc_rope_axes_backward_workspace(rdesc(), None) == api.KC_ERR_INVALID
