@@ -1452,6 +1452,7 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
   s.cw = std::min(d.channels, base * k);
   if (s.cw / vec > 512) return false;
   const int64_t chunks = (d.channels + s.cw - 1) / s.cw;
+  const int64_t row_step = d.points > 1 ? std::max(d.x_row_stride, d.y_row_stride) : 0;  // one row has no step
   auto fits = [&](int threads, int cs, int most) {
     s.threads = threads;
     s.cs = cs;
@@ -1459,7 +1460,7 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
     s.R = threads / (s.cw / vec);
     s.rows = (d.points + cs - 1) / cs;
     s.slots = (s.rows + s.R - 1) / s.R;
-    const int64_t step = std::max(d.x_row_stride, d.y_row_stride) * s.R * es;  // nth_row's
+    const int64_t step = row_step * s.R * es;  // nth_row's
     return step <= 0xffffffffll && s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
   };
   bool ok = false;
@@ -1653,9 +1654,9 @@ void run(const kc_group_norm_desc& d, NormParams p, int vec, bool backward, void
   p.act = d.act;
   p.eps = d.eps;
   p.xb = d.x_board_stride;
-  p.xr = d.x_row_stride;
+  p.xr = d.points > 1 ? d.x_row_stride : 0;
   p.yb = d.y_board_stride;
-  p.yr = d.y_row_stride;
+  p.yr = d.points > 1 ? d.y_row_stride : 0;
   p.mb = d.mask_board_stride;
   split_shape(d, p.tiles, p.tile_rows);
   const Layout l = workspace_layout(d, backward);

@@ -109,6 +109,14 @@ def test_more_groups_than_a_launch():
     assert "n * groups" in refused(forward, d, *far[:6], 1 << 45, 1 << 44)
 
 
+@pytest.mark.parametrize("backward", [False, True])
+def test_strides_of_one_row_play_no_part(backward):
+    """Boards of one point: whatever the row stride says, the call is the one of contiguous rows."""
+    want = api.group_norm_act_workspace(desc(points=1), backward)
+    for far in (1 << 34, 1 << 62, (1 << 63) - 1):
+        assert api.group_norm_act_workspace(desc(points=1, x_strides=(384, far), y_strides=(384, far)), backward) == want
+
+
 def test_workspace_null_result():
     assert api.lib().kc_group_norm_act_workspace(desc(), 0, None) == api.KC_ERR_INVALID
     assert api.lib().kc_rope_axes_backward_workspace(rdesc(), None) == api.KC_ERR_INVALID
