@@ -35,8 +35,9 @@ int guard_entry(F&& f) noexcept {
 inline int dtype_bytes(int dtype) { return dtype == KC_PRECISION_F32 ? 4 : 2; }
 
 // Makes the device that holds the operator's tensors current for the launch, and the caller's device again after it.
-// Every pointer (null ones are skipped) has to be device or managed memory of one device. A stream of another device
-// makes the launch fail (a stream cannot be asked for its device while it is captured).
+// Every pointer (null ones are skipped) has to be device memory of one device, or managed memory, which any device can
+// use: the caller's where there is nothing else. A stream of another device makes the launch fail (a stream cannot be
+// asked for its device while it is captured).
 class TensorDevice {
  public:
   TensorDevice(const char* op, std::initializer_list<const void*> ptrs) {
@@ -47,10 +48,10 @@ class TensorDevice {
       KC_CUDA(cudaPointerGetAttributes(&a, p));
       if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
         fail(KC_ERR_INVALID, std::string("CUDA backend: ") + op + ": a tensor is not in device memory");
-      const int d = a.type == cudaMemoryTypeManaged ? (dev_ < 0 ? saved_ : dev_) : a.device;
-      if (dev_ >= 0 && d != dev_)
+      if (a.type == cudaMemoryTypeManaged) continue;
+      if (dev_ >= 0 && a.device != dev_)
         fail(KC_ERR_INVALID, std::string("CUDA backend: ") + op + ": tensors on different devices");
-      dev_ = d;
+      dev_ = a.device;
     }
     if (dev_ < 0) dev_ = saved_;
     if (dev_ != saved_) KC_CUDA(cudaSetDevice(dev_));
