@@ -67,9 +67,19 @@ int managed_memory() {
   return 0;
 }
 
+// An error of a CUDA call belongs to the call of the operator that it failed, not to the next launch's check.
+int failed_call() {
+  const int rc = kc::guard_entry([] { KC_CUDA(pending = cudaErrorInvalidConfiguration); });
+  EXPECT(rc == KC_ERR_CUDA && !message.empty());
+  EXPECT(kc::guard_entry([] { KC_CUDA(cudaGetLastError()); }) == KC_OK);
+  EXPECT(kc::guard_entry([] { kc::TensorDevice dev("op", {reinterpret_cast<const void*>(4096)}); }) == KC_ERR_CUDA);
+  EXPECT(kc::guard_entry([] { KC_CUDA(cudaGetLastError()); }) == KC_OK);
+  return 0;
+}
 }  // namespace
 
 int main(int argc, char** argv) {
   if (argc == 2 && !std::strcmp(argv[1], "managed_memory")) return managed_memory();
+  if (argc == 2 && !std::strcmp(argv[1], "failed_call")) return failed_call();
   return 2;
 }
