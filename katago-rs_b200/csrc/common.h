@@ -24,6 +24,7 @@ struct Error : std::runtime_error {
 
 inline void cuda_check(cudaError_t e, const char* what, const char* file, int line) {
   if (e != cudaSuccess) {
+    (void)cudaGetLastError();  // the runtime keeps it otherwise, for the check after the next launch of a right call
     char buf[512];
     std::snprintf(buf, sizeof(buf), "CUDA backend: %s failed: %s (%s:%d)", what, cudaGetErrorString(e), file, line);
     throw Error(KC_ERR_CUDA, buf);

@@ -13,8 +13,7 @@
 
 namespace kc {
 
-// Runs an entry point's body; nothing thrown in it crosses the C boundary. The error of a failed CUDA call is reported
-// here and taken from the runtime, whose next launch check (of a call that is right) would report it again.
+// Runs an entry point's body; nothing thrown in it crosses the C boundary.
 template <typename F>
 int guard_entry(F&& f) noexcept {
   try {
@@ -22,7 +21,6 @@ int guard_entry(F&& f) noexcept {
     set_last_error("");
     return KC_OK;
   } catch (const Error& e) {
-    if (e.status == KC_ERR_CUDA) (void)cudaGetLastError();
     try { set_last_error(e.what()); } catch (...) {}
     return e.status;
   } catch (const std::exception& e) {
