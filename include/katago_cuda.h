@@ -293,7 +293,8 @@ typedef struct kc_rope_desc {
   int32_t dtype;   /* KC_PRECISION_* of q, k and their outputs and gradients */
   int32_t layout;  /* KC_ROPE_* */
   int32_t axes;    /* 1 .. KC_ROPE_MAX_AXES */
-  int32_t q_heads, k_heads; /* 1 .. 4096, 0 .. 4096; k_heads 0: no k (all k pointers are ignored) */
+  int32_t q_heads, k_heads; /* 1 .. 4096, 0 .. 4096; k_heads 0: no k (all k pointers and strides are
+                               ignored) */
   int32_t head_dim, rotary_dim; /* rotary_dim even, 2 .. head_dim; head_dim <= 1024 */
   int32_t tables;  /* 1, or a divisor of q_heads and k_heads: head h of H uses table h / (H / tables) */
   int64_t tokens;  /* may be 0 */

@@ -613,7 +613,8 @@ void check_desc(const kc_rope_desc* d) {
 }
 
 Rows rows(const kc_rope_desc& d, const void* p, int heads, int64_t ts, int64_t hs) {
-  return {heads ? p : nullptr, d.tokens, heads, d.head_dim, ts, hs, dtype_bytes(d.dtype)};
+  if (!heads) return {nullptr, d.tokens, 0, d.head_dim, 0, 0, dtype_bytes(d.dtype)};
+  return {p, d.tokens, heads, d.head_dim, ts, hs, dtype_bytes(d.dtype)};
 }
 Rows q_in(const kc_rope_desc& d, const void* p) { return rows(d, p, d.q_heads, d.q_token_stride, d.q_head_stride); }
 Rows k_in(const kc_rope_desc& d, const void* p) { return rows(d, p, d.k_heads, d.k_token_stride, d.k_head_stride); }
@@ -700,9 +701,12 @@ RopeParams params(const kc_rope_desc& d, const int32_t* pos, const float* freqs,
   return p;
 }
 
+// The strides of one token and of one head, which no address needs, are 0.
 Heads heads(const Rows& in, const Rows& out, const Rows& x, int tables) {
-  return {in.p, const_cast<void*>(out.p), x.p, in.outer_stride, in.inner_stride, out.outer_stride, out.inner_stride,
-          x.outer_stride, x.inner_stride, (int)(in.inner / tables)};
+  auto token = [](const Rows& r) { return r.outer > 1 ? r.outer_stride : 0; };
+  auto head = [](const Rows& r) { return r.inner > 1 ? r.inner_stride : 0; };
+  return {in.p, const_cast<void*>(out.p), x.p, token(in), head(in), token(out), head(out), token(x), head(x),
+          (int)(in.inner / tables)};
 }
 
 unsigned grid_of(int64_t threads) {

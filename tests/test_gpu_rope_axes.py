@@ -315,3 +315,23 @@ def test_gradient_of_frequencies_has_float32_sines(heads, tables, hd, dtype):
     for dy, want in ((x.roll(hd // 2, 2), torch.cos(freqs.double())), (-x, torch.sin(freqs.double()))):
         _, _, df = t.rope_backward(dy, None, x, None, pos, freqs, hd, "halves")
         t.within(df, want, 2.0**-22)
+
+
+def test_strides_that_no_address_needs():
+    """One token, one head, no k: the strides between tokens, heads and k heads may be any."""
+    for tokens, hq in ((1, 4), (5000, 1)):
+        wide, q, _, pos, freqs, g = make(tokens, hq, 0, 64, 64, 2, 1, "bf16", 67)
+        q = q.contiguous()
+        dq_out = torch.randn(q.shape, device="cuda", generator=g).bfloat16()
+        want = t.rope_forward(q, None, pos, freqs, 64, "halves")
+        back = t.rope_backward(dq_out, None, q, None, pos, freqs, 64, "halves")
+        st = (hq * 64 if tokens > 1 else 1 << 62, 64 if hq > 1 else (1 << 63) - 1)
+        d = api.RopeDesc(api.PRECISION_BF16, api.ROPE_HALVES, 2, tokens, hq, 0, 64, 64, 1, q_strides=st,
+                         k_strides=(1 << 62, -1), q_out_strides=st, k_out_strides=(-1, 1 << 62))
+        y, dq, df = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(freqs)
+        api.rope_axes(d, q.data_ptr(), 0, pos.data_ptr(), freqs.data_ptr(), y.data_ptr(), 0, t.stream())
+        size = api.rope_axes_backward_workspace(d)
+        ws = t.workspace(size, q.device)
+        api.rope_axes_backward(d, dq_out.data_ptr(), 0, q.data_ptr(), 0, pos.data_ptr(), freqs.data_ptr(),
+                               dq.data_ptr(), 0, df.data_ptr(), t.ptr(ws), size, t.stream())
+        assert torch.equal(y, want[0]) and torch.equal(dq, back[0]) and torch.equal(df, back[2])

@@ -193,6 +193,12 @@ def test_rotary_of_nothing():
     rotate_back(d, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
+def test_rotary_strides_of_absent_heads_play_no_part():
+    d = rdesc(tokens=0, k_heads=0, k_strides=(-1, 1 << 62), k_out_strides=(1 << 62, -64))
+    rotate(d, 0, 0, 0, 0, 0, 0)
+    rotate_back(d, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+
+
 def test_rotary_frequencies():
     f = api.rope_axes_freqs([8, 12, 12], 100.0, 64)
     want = np.zeros((32, 3))
