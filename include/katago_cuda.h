@@ -297,7 +297,7 @@ typedef struct kc_rope_desc {
                                ignored) */
   int32_t head_dim, rotary_dim; /* rotary_dim even, 2 .. head_dim; head_dim <= 1024 */
   int32_t tables;  /* 1, or a divisor of q_heads and k_heads: head h of H uses table h / (H / tables) */
-  int64_t tokens;  /* may be 0 */
+  int64_t tokens;  /* 0 .. 2^46 */
   int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
   int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
 } kc_rope_desc;

@@ -602,7 +602,7 @@ void check_desc(const kc_rope_desc* d) {
     bad("dtype must be KC_PRECISION_F32, F16 or BF16");
   if (d->layout != KC_ROPE_HALVES && d->layout != KC_ROPE_PAIRS) bad("unknown layout");
   if (d->axes < 1 || d->axes > KC_ROPE_MAX_AXES) bad("1 to " + std::to_string(KC_ROPE_MAX_AXES) + " axes");
-  if (d->tokens < 0) bad("tokens must not be negative");
+  if (d->tokens < 0 || d->tokens > (int64_t)1 << 46) bad("tokens must be 0 to 2^46");
   if (d->q_heads < 1 || d->k_heads < 0 || d->q_heads > 4096 || d->k_heads > 4096)
     bad("1 to 4096 q heads, 0 to 4096 k heads");
   if (d->head_dim < 2 || d->head_dim > 1024) bad("head_dim must be 2 to 1024");

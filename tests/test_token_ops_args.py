@@ -193,6 +193,12 @@ def test_rotary_of_nothing():
     rotate_back(d, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
+def test_rotary_workspace_query_refuses_what_the_calls_refuse():
+    for kw in (dict(tokens=(1 << 46) + 1), dict(tokens=(1 << 63) - 1), dict(axes=5), dict(tables=3)):
+        refused(api.rope_axes_backward_workspace, rdesc(**kw))
+        refused(rotate, rdesc(**kw))
+
+
 def test_rotary_strides_of_absent_heads_play_no_part():
     d = rdesc(tokens=0, k_heads=0, k_strides=(-1, 1 << 62), k_out_strides=(1 << 62, -64))
     rotate(d, 0, 0, 0, 0, 0, 0)
