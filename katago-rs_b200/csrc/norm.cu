@@ -237,8 +237,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // act of two elements.
 // mish = z f, f = tanh(log(1 + e)) = n / (n + 2), n = e^2 + 2 e, e = exp(z) (held to 2^60, where f is 1), which keeps
-// its digits where f is small. 1 - 2 / ((1 + e)^2 + 1) takes three instructions less (32.6 us where this takes 34.3, 256
-// boards x 361 x 384, bf16), but has lost half an f16 step already where the result is 2^-8, and 12 of them at z = -12.
+// its digits where f is small. 1 - 2 / ((1 + e)^2 + 1) takes three instructions less (32.6 us where this takes 34.3,
+// 256 boards x 361 x 384, bf16), but has lost half an f16 step already where the result is 2^-8, 12 of them at z = -12.
 // silu = z / (1 + exp(-z)), 0 where exp(-z) overflows.
 template <int ACT>
 __device__ __forceinline__ f32x2 act2(f32x2 z) {

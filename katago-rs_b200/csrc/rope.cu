@@ -91,9 +91,9 @@ __device__ __forceinline__ float cos_fast(float x) {
 // n / d by magic(d).
 __device__ __forceinline__ int quotient(int n, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)n, magic) : n; }
 
-// (cos, sin) of an angle of turns * 2^-64, for results of T. 2-byte results take the fast functions on half a turn either
-// way (off by 2^-21, far below the rounding). float32 ones, the frequencies' gradient among them whatever the heads'
-// type, take polynomials in an eighth of a turn either way from the nearest quarter, y = 8 * angle / turn in [-1, 1]:
+// (cos, sin) of an angle of turns * 2^-64, for results of T. 2-byte results take the fast functions on half a turn
+// either way (off by 2^-21, far below the rounding). float32 ones, the frequencies' gradient among them whatever the
+// heads' type, take polynomials in an eighth of a turn either way from the nearest quarter, y = 8 angle / turn:
 // sin(y pi / 4) = y (pi / 4 + y^2 P(y^2)), cos(y pi / 4) = 1 + y^2 Q(y^2), P and Q with the least largest error (2e-9
 // and 5e-11 of the result, by weighted least squares), pi / 4 in two floats. Off by at most 7.5e-8.
 template <typename T>

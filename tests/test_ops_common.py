@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 @pytest.fixture(scope="module")
 def program(tmp_path_factory):
     exe = str(tmp_path_factory.mktemp("ops") / "ops_common_check")
-    subprocess.check_call(["g++", "-std=c++17", "-O1", "-I" + os.path.join(os.environ.get("CUDA", "/usr/local/cuda"), "include"),
+    cuda = os.environ.get("CUDA", "/usr/local/cuda")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-I" + os.path.join(cuda, "include"),
                            "-I" + os.path.join(os.path.dirname(HERE), "katago-rs_b200", "csrc"), "-o", exe,
                            os.path.join(HERE, "ops_common_check.cpp")])
     return exe

@@ -114,7 +114,8 @@ def test_strides_of_one_row_play_no_part(backward):
     """Boards of one point: whatever the row stride says, the call is the one of contiguous rows."""
     want = api.group_norm_act_workspace(desc(points=1), backward)
     for far in (1 << 34, 1 << 62, (1 << 63) - 1):
-        assert api.group_norm_act_workspace(desc(points=1, x_strides=(384, far), y_strides=(384, far)), backward) == want
+        d = desc(points=1, x_strides=(384, far), y_strides=(384, far))
+        assert api.group_norm_act_workspace(d, backward) == want
 
 
 def test_workspace_null_result():
