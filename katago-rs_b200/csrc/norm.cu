@@ -132,8 +132,9 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 // Why this shape: shared memory and not registers, since vectors in registers had to be unrolled and unpacked floats
 // stayed live across the passes (206 registers, one block to an SM: 152 us for the 256 boards above). Chunks of at
 // least 64 bytes of a row: with 48 bytes the fixed work of a chunk weighs more (42 us), with 128 bytes clusters
-// are needed (54 us). Blocks of 128 with up to 18 rows a thread forward: the fixed work of a chunk (about 500
-// instructions a warp) is spread over more rows than with 256 (36 us). Only rows that are on are read.
+// are needed (54 us). Blocks of 128 forward: the fixed work of a chunk (about 500 instructions a warp) is spread over
+// more rows a thread than with 256 (36 us). Only rows that are on are read. (Times of the 256 boards with a mish of
+// three instructions less, which took 32.6 us in this shape.)
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSlots = 32;  // a thread's rows are bits of one word
 
@@ -1453,7 +1454,7 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
   if (s.cw / vec > 512) return false;
   const int64_t chunks = (d.channels + s.cw - 1) / s.cw;
   const int64_t row_step = d.points > 1 ? std::max(d.x_row_stride, d.y_row_stride) : 0;  // one row has no step
-  auto fits = [&](int threads, int cs, int most) {
+  auto fits = [&](int threads, int cs) {
     s.threads = threads;
     s.cs = cs;
     if (s.cw / vec > threads) return false;
@@ -1461,21 +1462,28 @@ bool resident_shape(const kc_group_norm_desc& d, int vec, bool backward, ResShap
     s.rows = (d.points + cs - 1) / cs;
     s.slots = (s.rows + s.R - 1) / s.R;
     const int64_t step = row_step * s.R * es;  // nth_row's
-    return step <= 0xffffffffll && s.slots <= most && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
+    return step <= 0xffffffffll && s.slots <= kMaxSlots &&
+           resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem;
   };
   bool ok = false;
-  for (int cs = 1; cs <= 8 && !ok; cs *= 2) ok = fits(backward ? 256 : 128, cs, backward ? 9 : 18);
+  // the fewest blocks whose rows leave room for as many of them on an SM as their registers do: five of 128 threads
+  // forward, two of 256 backward. (A limit of 18 and 9 rows a thread, which is that of 16-byte vectors at 361 points,
+  // put 400 points into clusters of two: 256 boards x 400 x 384, bf16, 51 us instead of 37.5; 400 boards x 700 x 30,
+  // bf16, 48 instead of 23 us, backward 78 instead of 30.)
+  const size_t share = kMaxSmem / (backward ? 2 : 5) - 1024;
+  for (int cs = 1; cs <= 8 && !ok; cs *= 2)
+    ok = fits(backward ? 256 : 128, cs) && resident_smem(s, vec, unit, es, cg, backward) <= share;
   // larger boards: clusters of up to 16, where two blocks fit an SM before that where one does
   for (int cs = 2; cs <= 16 && !ok; cs *= 2)
     for (int threads = 256; threads <= 512 && !ok; threads *= 2)
-      ok = fits(threads, cs, kMaxSlots) && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem / 2 - 1024;
-  for (int cs = 2; cs <= 16 && !ok; cs *= 2) ok = fits(256, cs, kMaxSlots) || fits(512, cs, kMaxSlots);
+      ok = fits(threads, cs) && resident_smem(s, vec, unit, es, cg, backward) <= (size_t)kMaxSmem / 2 - 1024;
+  for (int cs = 2; cs <= 16 && !ok; cs *= 2) ok = fits(256, cs) || fits(512, cs);
   if (!ok) return false;
   // narrow vectors hold little each: many turns of large clusters, where tiles of rows take fewer (40 boards of 5,000 x
   // 99 channels, f16: 228 us in clusters of 16, 100 us in tiles)
   if (vec * es < 8 && s.cs > 4) return false;
   // few boards: spread one over more SMs
-  while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < kSms) fits(s.threads, s.cs * 2, kMaxSlots);
+  while (s.cs < 8 && s.slots > 3 && (int64_t)d.n * chunks * s.cs < kSms) fits(s.threads, s.cs * 2);
   s.vdiv = (1u << 20) / (uint32_t)(s.cw / vec) + 1;
   // blocks that run together, by shared memory and registers. A forward block takes any chunks; a backward one keeps
   // its chunk (for the channels' sums) and the boards go evenly over them.

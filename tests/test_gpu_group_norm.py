@@ -535,3 +535,17 @@ def test_row_strides_of_boards_of_one_point():
                                         t.stream())
     assert torch.equal(y, want[0]) and torch.equal(stats, want[1])
     assert all(torch.equal(a, c) for a, c in zip((dx, dw, db), back))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("points", [361, 400, 420, 421, 460])
+@pytest.mark.parametrize("channels,groups", [(96, 8), (30, 6), (21, 3)])
+def test_boards_around_what_one_block_holds(points, channels, groups, dtype):
+    n = 40
+    for act, kind in (("mish", "boards"), ("silu", "none")):
+        _, x, w, b, g = make(n, points, channels, dtype, points)
+        mask = masks(kind, n, points, g)
+        y, stats = t.norm_forward(x, mask, w, b, groups, act)
+        check_forward(x, mask, w, b, groups, act, y, stats)
+        dy = torch.randn(x.shape, device="cuda", generator=g).to(x.dtype)
+        check_backward(x, mask, w, b, stats, dy, groups, act, t.norm_backward(x, mask, w, b, stats, dy, groups, act))
