@@ -11,16 +11,17 @@
 // is taken around a value of its own and shares are merged by count as distances from one of them, so that a large
 // mean costs no digits of the variance.
 //
-// What bounds it: HBM, once reading and writing the tensor is all the traffic there is; each element also costs about
-// 12 instructions forward (mish) and 25 backward, which takes nearly as long. So a board's chunk of channels is read
-// once into shared memory and stays there (resident path). Measured on a B200 (6,554 GB/s copy), bytes that have to
-// move / time:
-//   forward, 256 boards x 361 points x 384 channels, 32 groups, bf16, mish, mixed board sizes: 119 MB in 32.6 us,
-//     3,660 GB/s (the split path's three launches with two reads: 178 us). 53% of the issue slots; 16 warps to an SM
-//     (96 registers, 39 KB of slots a block), which wait for their own arithmetic and two barriers a chunk
-//   1,024 of those boards: 477 MB in 111 us, 4,310 GB/s
-//   backward, 512 such boards: 334 MB in 110 us, 3,030 GB/s (split path: 426 us); 128 registers and 115 KB of slots
-//     leave two blocks of 256 to an SM
+// What bounds it: HBM, once reading and writing the tensor is all the traffic there is; each element that is on also
+// costs about 24 instructions forward (mish) and 37 backward, which takes as long. So a board's chunk of channels is
+// read once into shared memory and stays there (resident path). Measured on a B200 (6,554 GB/s copy), bytes that have
+// to move / time:
+//   forward, 256 boards x 361 points x 384 channels, 32 groups, bf16, mish, mixed board sizes: 119 MB in 34.3 us,
+//     3,480 GB/s (the split path's three launches with two reads: 178 us). 54% of the issue slots, 18 us of bytes:
+//     transfers and arithmetic follow each other. 20 warps to an SM (96 registers, 39 KB of slots a block; 17 active on
+//     average), which wait for their own arithmetic and two barriers a chunk
+//   1,024 of those boards: 477 MB in 114 us, 4,180 GB/s
+//   backward, 512 such boards: 334 MB in 110.6 us, 3,020 GB/s (split path: 426 us), 49% of the issue slots; 128
+//     registers and 113 KB of shared memory leave two blocks of 256 to an SM
 //   forward, 64 boards x 361 x 768, one group, float32, silu: 119 MB in 52 us, 2,290 GB/s: a board fills a cluster of
 //     16 blocks, all boards in four turns of all SMs that load, reduce and store in step
 //   forward, 32 x 5,776 x 256, 32 groups, bf16, silu: 189 MB in 56 us, 3,380 GB/s (clusters of 4)

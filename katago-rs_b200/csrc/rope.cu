@@ -12,12 +12,13 @@
 // What bounds it: HBM for a table shared by all heads; with a table per key head the angles (17.7 million for 256
 // boards, about 28 instructions each) take as long as the transfers. Measured on a B200 (6,554 GB/s copy), bytes that
 // have to move / time:
-//   256 boards x 361 tokens, 6 + 6 heads of 64, f16: 284 MB in 53 us (5,300 GB/s) with one table, in 66.7 us
-//     (4,270 GB/s) with a table per key head; a thread per pair vector with its own float64 angles: 86 us
+//   256 boards x 361 tokens, 6 + 6 heads of 64, f16: 284 MB in 53.7 us (5,300 GB/s) with one table, in 66.9 us
+//     (4,255 GB/s) with a table per key head; a thread per pair vector with its own float64 angles: 86 us
 //   57,767 tokens, 16 + 4 heads of 128, 96 of them turned, 3 axes, bf16: 592 MB in 119.5 us, 4,960 GB/s
-//   backward with the frequencies' gradient, 34,656 tokens, 12 + 4 heads of 64, 4 tables, bf16: 213 MB in 54.3 us,
-//     3,930 GB/s: 24 warps to an SM (80 registers), most of the time waiting for their loads
-//   backward without it, 4,099 tokens, 12 + 12 heads of 64, float32: 50 MB in 12 us
+//   backward with the frequencies' gradient, 34,656 tokens, 12 + 4 heads of 64, 4 tables, bf16: 213 MB in 55.9 us,
+//     3,810 GB/s: 24 warps to an SM (80 registers), most of the time waiting for their loads; 1.6 us of it are the
+//     sines of a float32 result
+//   backward without it, 4,099 tokens, 12 + 12 heads of 64, float32: 50 MB in 11.9 us
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -776,7 +777,7 @@ void launch_back(RopeParams p, cudaStream_t st) {
 
 template <typename T, int VP, int LAYOUT>
 void launch(RopeParams p, cudaStream_t st) {
-  // backward 8-byte vectors, whose registers let three blocks run on an SM: 53.7 us against 71 us with 16 bytes and
+  // backward 8-byte vectors, whose registers let three blocks run on an SM: 55.4 us against 72.3 us with 16 bytes and
   // two blocks (34,656 tokens, 12 + 4 heads of 64, bf16)
   if (p.dfreqs) return launch_back<T, VP == 8 ? 4 : VP, LAYOUT>(p, st);
   const int64_t heads = p.q.per_table + p.k.per_table, cols = p.pairs / VP + p.rest / VP;
