@@ -570,7 +570,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 5 : 1)
     __syncthreads();
 
     // merged by group, a warp per group, around one share's mean: the correction by the mean's distance from it is
-    // at most as many times the result as there are shares, since that share is one of them
+    // at most as many times the result as there are shares, since that share is one of them. (4 of 768 float32
+    // channels 1e4 off the rest, one group: rstd off by 4.4e-6 of itself. A pass for the mean and one for the squares
+    // leave 3e-8, but take 5% longer with one group a board and 22% with one channel a group.)
     int rows_on = 0;
     for (int i = lane; i < sh.R; i += 32) rows_on += __popc(bits_now[i]);
     rows_on = __reduce_add_sync(0xffffffffu, rows_on);
