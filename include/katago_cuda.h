@@ -322,6 +322,36 @@ int kc_rope_axes_backward(const kc_rope_desc* desc, const void* d_dq_out, const 
                           const void* d_k, const int32_t* d_pos, const float* d_freqs, void* d_dq, void* d_dk,
                           float* d_dfreqs, void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* Norm of each token's row: n boards of `points` rows of `channels`. The transformer blocks of the nets use the RMS form
+ * (bin2onnx.py transformer_rmsnorm :1330-1340), which the engine has inside its forward pass. */
+#define KC_NORM_LAYER 0 /* mean and variance of the row */
+#define KC_NORM_RMS 1   /* root of the mean square, no mean */
+typedef struct kc_layer_norm_desc {
+  int32_t dtype; /* KC_PRECISION_* of x, y, dy and dx */
+  int32_t kind;  /* KC_NORM_* */
+  int32_t n, points, channels; /* n and points 0 .. 2^30, channels 1 .. 2^30 */
+  float eps;     /* >= 0 */
+  int64_t x_board_stride, x_row_stride; /* x and dx */
+  int64_t y_board_stride, y_row_stride; /* y and dy */
+  int64_t mask_board_stride;
+} kc_layer_norm_desc;
+
+/* y = (x - mean) * rstd * weight[c] + bias[c] at the tokens whose mask is not 0, 0 at the others (whatever x holds there
+ * has no effect), with the mean (0 for RMS) and rstd = 1 / sqrt(mean square distance from it + eps) of the token's row.
+ * Squares are summed in float32: a row whose sum passes 3.4e38 has NaN in y and rstd. d_mask: [n][points] float32 rows at
+ * mask_board_stride, NULL = every token; d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not
+ * wanted): [n][points][2] float32 mean and rstd, both 0 where the token is off. */
+int kc_layer_norm(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
+                  const float* d_bias, void* d_y, float* d_stats, void* stream);
+
+/* The gradients by x, weight and bias, given dy and the forward pass's x and d_stats: dx (0 at tokens that are off; in
+ * place of x, or of dy where the strides are the same), d_dweight and d_dbias [channels] float32 (sums over all tokens,
+ * overwritten; each may be NULL). The workspace is for d_dweight and d_dbias only. */
+int kc_layer_norm_backward_workspace(const kc_layer_norm_desc* desc, size_t* bytes);
+int kc_layer_norm_backward(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
+                           const float* d_stats, const void* d_dy, void* d_dx, float* d_dweight, float* d_dbias,
+                           void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* Failure-detection self-test. Every spin-wait in this library's kernels is bounded: when a wait runs out, the
  * kernel records an error code in the handle's device error word, releases what it holds and returns, and the next
  * kc_wait / kc_synchronize reports KC_ERR_DEVICE (the handle stays usable). This enqueues on the handle's stream

@@ -1,0 +1,716 @@
+// Norm of each token's row of channels (layer norm and RMS norm) on channels-last board tokens, forward and backward
+// (kc_layer_norm, kc_layer_norm_backward).
+//
+//   mean = sum x / C (RMS: 0), var = sum (x - mean)^2 / C, rstd = 1 / sqrt(var + eps), xh = (x - mean) rstd,
+//   y = xh w + b where the token is on, 0 elsewhere
+//   g = dy w, c1 = sum g / C (RMS: 0), c2 = sum g xh / C, dx = rstd (g - c1 - xh c2) where on,
+//   dweight = sum over tokens of dy xh, dbias = of dy
+//
+// A row stays in the registers of a group of lanes (2 to 32 of a warp, or a block) between the sums and the output:
+// one read, one write. The variance is taken around the float32 mean of the first pass, whose own error the second
+// pass finds (the sum of the distances), so that a large mean costs neither digits of the variance nor of x - mean.
+// Backward, a block goes over many rows and keeps the channels' sums in registers; a second launch adds the blocks' in
+// their order. Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read
+// again for each pass.
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "../../include/katago_cuda.h"
+#include "rows.cuh"
+
+namespace kc {
+namespace {
+
+[[noreturn]] void bad(const std::string& what) { fail(KC_ERR_INVALID, "CUDA backend: layer norm: " + what); }
+
+constexpr int kThreads = 256;
+constexpr int kLongThreads = 512;
+
+struct LayerParams {
+  const void* x;
+  const float* mask;
+  const float* weight;
+  const float* bias;
+  void* y;         // forward: y; backward: dx
+  const void* dy;
+  float2* stats;   // (mean, rstd) of a token: written by the forward pass (may be null), read by the backward
+  float* part;     // backward: [blocks][2][C] sums of dy xh and of dy
+  float* dweight;
+  float* dbias;
+  RowMap xm, ym, mm;
+  int64_t rows;
+  int C, lanes;
+  int kind;
+  int wide;        // weight and bias are 16-byte aligned
+  float eps;
+};
+
+__device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) {
+  return !p.mask || __ldg(p.mask + p.mm(r)) != 0.0f;
+}
+
+// 1 / sqrt(var + eps) of a sum of squares around a value that is `delta` from the mean; NaN where the squares passed
+// float32's range.
+__device__ __forceinline__ float rstd_of(float squares, float inv, float delta, float eps) {
+  const float var = squares * inv - delta * delta;
+  if (!(squares <= 3.402823466e38f)) return __int_as_float(0x7fffffff);
+  return __frsqrt_rn(fmaxf(var, 0.0f) + eps);
+}
+
+// A row's lanes: `lanes` neighbours of a warp, or a block.
+template <bool BLOCK>
+struct Group {
+  int lane, lanes;
+  int64_t first, step;
+  __device__ __forceinline__ explicit Group(int row_lanes) {
+    if (BLOCK) {
+      lanes = blockDim.x;
+      lane = threadIdx.x;
+      first = blockIdx.x;
+      step = gridDim.x;
+    } else {
+      lanes = row_lanes;
+      lane = threadIdx.x & (row_lanes - 1);
+      const int per = kThreads / row_lanes;
+      first = (int64_t)blockIdx.x * per + threadIdx.x / row_lanes;
+      step = (int64_t)gridDim.x * per;
+    }
+  }
+  __device__ __forceinline__ float2 sum(float2 v, float2* red) const {
+    return BLOCK ? block_sum(v, red) : lanes_sum(v, lanes);
+  }
+};
+
+// A warp's lanes stay together for the sums: a group behind the last row takes part with nothing.
+template <bool BLOCK>
+__device__ __forceinline__ bool rows_left(int64_t r, int64_t rows) {
+  return BLOCK ? r < rows : __any_sync(0xffffffffu, r < rows);
+}
+
+template <typename T, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : kThreads) layer_norm_kernel(const LayerParams p) {
+  using V = RowVec<T, VEC>;
+  __shared__ float2 red[2][32];
+  const Group<BLOCK> g(p.lanes);
+  const int nvec = p.C / VEC;
+  const float inv = 1.0f / (float)p.C;
+  int turn = 0;  // a block's sums in a row take turns with `red`
+  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step) {
+    const bool here = r < p.rows, on = here && token_on(p, r);
+    float v[NV][VEC];
+    float2 s = make_float2(0.0f, 0.0f);
+    if (on) {
+      const T* row = static_cast<const T*>(p.x) + p.xm(r);
+      typename V::Raw raw[NV];
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (g.lane + i * g.lanes < nvec) raw[i] = V::load(row + (g.lane + i * g.lanes) * VEC);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        if (g.lane + i * g.lanes >= nvec) continue;
+        V::unpack(raw[i], v[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) s.x += v[i][j];
+      }
+    }
+    float m0 = 0.0f;
+    if (p.kind == KC_NORM_LAYER) m0 = g.sum(s, red[turn ^= 1]).x * inv;
+    s = make_float2(0.0f, 0.0f);
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        if (g.lane + i * g.lanes >= nvec) continue;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          v[i][j] -= m0;
+          s.x += v[i][j];
+          s.y = fmaf(v[i][j], v[i][j], s.y);
+        }
+      }
+    }
+    s = g.sum(s, red[turn ^= 1]);
+    if (!here) continue;
+    const float delta = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f;
+    const float rstd = rstd_of(s.y, inv, delta, p.eps);
+    if (p.stats && g.lane == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
+    T* out = static_cast<T*>(p.y) + p.ym(r);
+    const float shift = -delta * rstd;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = (g.lane + i * g.lanes) * VEC;
+      if (g.lane + i * g.lanes >= nvec) continue;
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) o[j] = 0.0f;
+      if (on) {
+        float w[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o[j] = fmaf(v[i][j], rstd, shift);
+        if (p.weight) {
+          load_params<VEC>(p.weight + c, p.wide, w);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) o[j] *= w[j];
+        }
+        if (p.bias) {
+          load_params<VEC>(p.bias + c, p.wide, w);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) o[j] += w[j];
+        }
+      }
+      V::store(out + c, V::pack(o));
+    }
+  }
+}
+
+template <typename T, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel(const LayerParams p) {
+  using V = RowVec<T, VEC>;
+  __shared__ float2 red[2][32];
+  extern __shared__ float sums[];  // a warp's rows in lanes: [2][C]
+  const Group<BLOCK> g(p.lanes);
+  const int nvec = p.C / VEC;
+  const float inv = 1.0f / (float)p.C;
+  float aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+#pragma unroll
+    for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f;
+  int turn = 0;
+  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1) {
+    const bool here = r < p.rows, on = here && token_on(p, r);
+    typename V::Raw xr[NV], dr[NV];
+    float2 s = make_float2(0.0f, 0.0f), st = s;
+    if (on) {
+      const T* x = static_cast<const T*>(p.x) + p.xm(r);
+      const T* dy = static_cast<const T*>(p.dy) + p.ym(r);
+      st = p.stats[r];
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int c = (g.lane + i * g.lanes) * VEC;
+        if (g.lane + i * g.lanes < nvec) xr[i] = V::load(x + c), dr[i] = V::load(dy + c);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        if (g.lane + i * g.lanes >= nvec) continue;
+        float a[VEC], d[VEC], w[VEC];
+        V::unpack(xr[i], a);
+        V::unpack(dr[i], d);
+        if (p.weight) load_params<VEC>(p.weight + (g.lane + i * g.lanes) * VEC, p.wide, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          const float xh = (a[j] - st.x) * st.y;
+          const float gw = p.weight ? d[j] * w[j] : d[j];
+          s.x += gw;
+          s.y = fmaf(gw, xh, s.y);
+          aw[i][j] = fmaf(d[j], xh, aw[i][j]);
+          ab[i][j] += d[j];
+        }
+      }
+    }
+    s = g.sum(s, red[turn]);
+    if (!here) continue;
+    const float c1 = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f, c2 = s.y * inv;
+    T* out = static_cast<T*>(p.y) + p.xm(r);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = (g.lane + i * g.lanes) * VEC;
+      if (g.lane + i * g.lanes >= nvec) continue;
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) o[j] = 0.0f;
+      if (on) {
+        float a[VEC], d[VEC], w[VEC];
+        V::unpack(xr[i], a);
+        V::unpack(dr[i], d);
+        if (p.weight) load_params<VEC>(p.weight + c, p.wide, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          const float xh = (a[j] - st.x) * st.y;
+          const float gw = p.weight ? d[j] * w[j] : d[j];
+          o[j] = st.y * (gw - fmaf(xh, c2, c1));
+        }
+      }
+      V::store(out + c, V::pack(o));
+    }
+  }
+  if (!p.part) return;
+  float* part = p.part + (size_t)blockIdx.x * 2 * p.C;
+  if (BLOCK) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = (g.lane + i * g.lanes) * VEC;
+      if (g.lane + i * g.lanes >= nvec) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; j++) part[c + j] = aw[i][j], part[p.C + c + j] = ab[i][j];
+    }
+  } else {
+    // a warp's groups in registers, then warp after warp in shared memory
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (o >= g.lanes) {
+            aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
+            ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
+          }
+    for (int w = 0; w < kThreads / 32; w++) {
+      if (threadIdx.x / 32 == w && threadIdx.x % 32 < g.lanes) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+          const int c = (g.lane + i * g.lanes) * VEC;
+          if (g.lane + i * g.lanes >= nvec) continue;
+#pragma unroll
+          for (int j = 0; j < VEC; j++) {
+            sums[c + j] = w ? sums[c + j] + aw[i][j] : aw[i][j];
+            sums[p.C + c + j] = w ? sums[p.C + c + j] + ab[i][j] : ab[i][j];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * p.C; c += kThreads) part[c] = sums[c];
+  }
+}
+
+// Rows that registers do not hold: a block to a row, read again for each pass.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kLongThreads) layer_norm_long_kernel(const LayerParams p) {
+  using V = RowVec<T, VEC>;
+  __shared__ float2 red[2][32];
+  const float inv = 1.0f / (float)p.C;
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const bool on = token_on(p, r);
+    const T* row = static_cast<const T*>(p.x) + p.xm(r);
+    float2 s = make_float2(0.0f, 0.0f);
+    float m0 = 0.0f;
+    if (on && p.kind == KC_NORM_LAYER) {
+      for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
+        float v[VEC];
+        V::unpack(V::load(row + c), v);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) s.x += v[j];
+      }
+      m0 = block_sum(s, red[0]).x * inv;
+    }
+    s = make_float2(0.0f, 0.0f);
+    if (on)
+      for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
+        float v[VEC];
+        V::unpack(V::load(row + c), v);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          v[j] -= m0;
+          s.x += v[j];
+          s.y = fmaf(v[j], v[j], s.y);
+        }
+      }
+    s = block_sum(s, red[1]);
+    const float delta = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f;
+    const float rstd = rstd_of(s.y, inv, delta, p.eps);
+    if (p.stats && threadIdx.x == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
+    T* out = static_cast<T*>(p.y) + p.ym(r);
+    for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
+      float o[VEC], w[VEC], b[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) o[j] = 0.0f, w[j] = 1.0f, b[j] = 0.0f;
+      if (on) {
+        V::unpack(V::load(row + c), o);
+        if (p.weight) load_params<VEC>(p.weight + c, p.wide, w);
+        if (p.bias) load_params<VEC>(p.bias + c, p.wide, b);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o[j] = fmaf((o[j] - m0 - delta) * rstd, w[j], b[j]);
+      }
+      V::store(out + c, V::pack(o));
+    }
+    __syncthreads();  // red
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kLongThreads) layer_norm_long_back_kernel(const LayerParams p) {
+  using V = RowVec<T, VEC>;
+  __shared__ float2 red[32];
+  const float inv = 1.0f / (float)p.C;
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const bool on = token_on(p, r);
+    const T* x = static_cast<const T*>(p.x) + p.xm(r);
+    const T* dy = static_cast<const T*>(p.dy) + p.ym(r);
+    float2 s = make_float2(0.0f, 0.0f), st = s;
+    if (on) {
+      st = p.stats[r];
+      for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
+        float a[VEC], d[VEC], w[VEC];
+        V::unpack(V::load(x + c), a);
+        V::unpack(V::load(dy + c), d);
+        if (p.weight) load_params<VEC>(p.weight + c, p.wide, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          const float gw = p.weight ? d[j] * w[j] : d[j];
+          s.x += gw;
+          s.y = fmaf(gw, (a[j] - st.x) * st.y, s.y);
+        }
+      }
+    }
+    s = block_sum(s, red);
+    const float c1 = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f, c2 = s.y * inv;
+    T* out = static_cast<T*>(p.y) + p.xm(r);
+    for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) o[j] = 0.0f;
+      if (on) {
+        float a[VEC], d[VEC], w[VEC];
+        V::unpack(V::load(x + c), a);
+        V::unpack(V::load(dy + c), d);
+        if (p.weight) load_params<VEC>(p.weight + c, p.wide, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          const float gw = p.weight ? d[j] * w[j] : d[j];
+          o[j] = st.y * (gw - fmaf((a[j] - st.x) * st.y, c2, c1));
+        }
+      }
+      V::store(out + c, V::pack(o));
+    }
+    __syncthreads();  // red
+  }
+}
+
+// The channels' sums of long rows: a block to 32 channels and a share of the rows (before dx may take x's place).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) layer_norm_long_sums_kernel(const LayerParams p) {
+  __shared__ float2 red[kThreads / 32][32];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < p.C; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t c = c0 + tx;
+    float2 s = make_float2(0.0f, 0.0f);
+    if (c < p.C)
+      for (int64_t r = (int64_t)blockIdx.y * (kThreads / 32) + ty; r < p.rows; r += (int64_t)gridDim.y * (kThreads / 32)) {
+        if (!token_on(p, r)) continue;
+        const float2 st = p.stats[r];
+        const float d = to_f<T>(static_cast<const T*>(p.dy)[p.ym(r) + c]);
+        s.x = fmaf(d, (to_f<T>(static_cast<const T*>(p.x)[p.xm(r) + c]) - st.x) * st.y, s.x);
+        s.y += d;
+      }
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < p.C) {
+      for (int i = 1; i < kThreads / 32; i++) s.x += red[i][tx].x, s.y += red[i][tx].y;
+      p.part[(size_t)blockIdx.y * 2 * p.C + c] = s.x;
+      p.part[(size_t)blockIdx.y * 2 * p.C + p.C + c] = s.y;
+    }
+    __syncthreads();
+  }
+}
+
+// dweight and dbias from the blocks' sums, in the blocks' order. 32 channels to a block, 32 threads share the blocks.
+__global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* part, int blocks, int C, float* dweight,
+                                                                 float* dbias) {
+  pdl_wait();
+  __shared__ float red[32][33];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t cols = 2 * (int64_t)C;
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t c = c0 + tx;
+    float s = 0.0f;
+    if (c < cols)
+#pragma unroll 8
+      for (int b = ty; b < blocks; b += 32) s += part[(size_t)b * cols + c];
+    red[ty][tx] = s;
+    __syncthreads();
+    // thread (tx, ty) adds lane tx's sum of channel ty
+    float v = red[tx][ty];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int64_t at = c0 + ty;
+    if (tx == 0 && at < cols) {
+      if (at < C) {
+        if (dweight) dweight[at] = v;
+      } else if (dbias) {
+        dbias[at - C] = v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+
+// How a call goes over its rows.
+struct Shape {
+  int vec, nv;
+  bool block;    // a block to a row, otherwise `lanes` lanes of a warp
+  bool is_long;
+  int threads, lanes;
+  int64_t blocks;
+};
+
+constexpr int kNvs[] = {1, 2, 3, 4, 6, 8};
+
+// Registers of a warp's lane: 32 elements forward, 24 backward (with both tensors and both sums).
+bool nv_built(int vec, int nv, bool backward) {
+  if (vec <= 2) return nv == 2 || nv == 8;
+  return vec * nv <= (backward ? 24 : 32);
+}
+
+Shape shape_of(int64_t rows, int C, int vec, bool backward) {
+  Shape s{};
+  s.vec = vec;
+  const int64_t nvec = C / vec;
+  // the fewest lanes in a row that leave no more than an eighth of them idle, with as many vectors each as are built:
+  // few shuffles for a sum, many loads in flight
+  int64_t best = -1;
+  for (int lanes = 2; lanes <= 32; lanes *= 2)
+    for (int nv : kNvs) {
+      if (!nv_built(vec, nv, backward) || (int64_t)lanes * nv < nvec) continue;
+      const int64_t waste = (int64_t)lanes * nv * 8 - nvec * 8 > nvec ? (int64_t)lanes * nv - nvec : 0;
+      const int64_t cost = waste * 64 + lanes;
+      if (best < 0 || cost < best) best = cost, s.lanes = lanes, s.nv = nv;
+    }
+  if (best >= 0) {
+    s.threads = kThreads;
+    const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
+    s.blocks = std::min<int64_t>(all, backward ? 2 * kSmCount : 1 << 20);
+    return s;
+  }
+  s.block = true;
+  s.nv = vec == 8 ? 2 : 4;
+  const int64_t threads = ((nvec + s.nv - 1) / s.nv + 31) / 32 * 32;
+  if (threads <= (backward ? 512 : 1024)) {
+    s.threads = (int)threads;
+    s.blocks = std::min<int64_t>(rows, backward ? (int64_t)kSmCount * (512 / threads) : 1 << 20);
+    return s;
+  }
+  s.is_long = true;
+  s.threads = kLongThreads;
+  s.blocks = std::min<int64_t>(rows, 1 << 20);
+  return s;
+}
+
+// Shares of the rows in the long rows' channel sums.
+int64_t long_shares(int64_t rows, int C) {
+  const int64_t most = std::max<int64_t>(1, 8 * kSmCount / ((C + 31) / 32));
+  return std::max<int64_t>(1, std::min<int64_t>(most, rows / 8));
+}
+
+int64_t part_blocks(const Shape& s, int64_t rows, int C) { return s.is_long ? long_shares(rows, C) : s.blocks; }
+
+template <typename T, int VEC, int NV, bool BLOCK>
+void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
+  if (backward) {
+    if constexpr (BLOCK || NV * VEC <= 24)
+      layer_norm_back_kernel<T, VEC, NV, BLOCK>
+          <<<(unsigned)s.blocks, s.threads, BLOCK ? 0 : 2 * p.C * sizeof(float), st>>>(p);
+  } else {
+    layer_norm_kernel<T, VEC, NV, BLOCK><<<(unsigned)s.blocks, s.threads, 0, st>>>(p);
+  }
+  KC_CUDA(cudaGetLastError());
+}
+
+template <typename T, int VEC>
+void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
+  if (s.is_long) {
+    if (!backward) {
+      layer_norm_long_kernel<T, VEC><<<(unsigned)s.blocks, kLongThreads, 0, st>>>(p);
+    } else {
+      if (p.part) {
+        const dim3 grid((unsigned)std::min<int64_t>((p.C + 31) / 32, 1 << 20), (unsigned)long_shares(p.rows, p.C));
+        layer_norm_long_sums_kernel<T><<<grid, kThreads, 0, st>>>(p);
+        KC_CUDA(cudaGetLastError());
+      }
+      layer_norm_long_back_kernel<T, VEC><<<(unsigned)s.blocks, kLongThreads, 0, st>>>(p);
+    }
+    KC_CUDA(cudaGetLastError());
+  } else if (s.block) {
+    launch_rows<T, VEC, VEC == 8 ? 2 : 4, true>(p, s, backward, st);
+  } else if constexpr (VEC <= 2) {
+    s.nv == 2 ? launch_rows<T, VEC, 2, false>(p, s, backward, st) : launch_rows<T, VEC, 8, false>(p, s, backward, st);
+  } else {
+    switch (s.nv) {
+      case 1: return launch_rows<T, VEC, 1, false>(p, s, backward, st);
+      case 2: return launch_rows<T, VEC, 2, false>(p, s, backward, st);
+      case 3: return launch_rows<T, VEC, 3, false>(p, s, backward, st);
+      case 4: return launch_rows<T, VEC, 4, false>(p, s, backward, st);
+      case 6: if constexpr (VEC == 4) return launch_rows<T, VEC, 6, false>(p, s, backward, st); break;
+      case 8: if constexpr (VEC == 4) return launch_rows<T, VEC, 8, false>(p, s, backward, st); break;
+    }
+  }
+}
+
+template <typename T>
+void run_type(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (s.vec == 8) return run_vec<T, 8>(p, s, backward, st);
+  if (s.vec == 4) return run_vec<T, 4>(p, s, backward, st);
+  if (s.vec == 2) return run_vec<T, 2>(p, s, backward, st);
+  run_vec<T, 1>(p, s, backward, st);
+}
+
+void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cudaStream_t st) {
+  p.rows = (int64_t)d.n * d.points;
+  p.C = d.channels;
+  p.kind = d.kind;
+  p.eps = d.eps;
+  p.wide = aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
+  p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
+  p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);
+  p.mm = row_map(d.n, d.points, d.mask_board_stride, 1);
+  const Shape s = shape_of(p.rows, p.C, vec, backward);
+  p.lanes = s.lanes;
+  if (d.dtype == KC_PRECISION_F32) run_type<float>(p, s, backward, st);
+  else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, s, backward, st);
+  else run_type<__nv_bfloat16>(p, s, backward, st);
+  if (!p.part) return;
+  launch_after(layer_norm_params_kernel, dim3((unsigned)std::min<int64_t>((2 * (int64_t)p.C + 31) / 32, 1 << 20)),
+               dim3(1024), 0, st, (const float*)p.part, (int)part_blocks(s, p.rows, p.C), p.C, p.dweight, p.dbias);
+}
+
+Rows x_rows(const kc_layer_norm_desc& d, const void* p) {
+  return {p, d.n, d.points, d.channels, d.n > 1 ? d.x_board_stride : 0, d.points > 1 ? d.x_row_stride : 0,
+          dtype_bytes(d.dtype)};
+}
+Rows y_rows(const kc_layer_norm_desc& d, const void* p) {
+  return {p, d.n, d.points, d.channels, d.n > 1 ? d.y_board_stride : 0, d.points > 1 ? d.y_row_stride : 0,
+          dtype_bytes(d.dtype)};
+}
+Rows mask_rows(const kc_layer_norm_desc& d, const void* p) {
+  return {p, d.n, 1, d.points, d.n > 1 ? d.mask_board_stride : 0, 0, 4};
+}
+
+void check_desc(const kc_layer_norm_desc* d) {
+  if (!d) bad("null descriptor");
+  if (d->dtype < KC_PRECISION_F32 || d->dtype > KC_PRECISION_BF16) bad("unknown dtype");
+  if (d->kind != KC_NORM_LAYER && d->kind != KC_NORM_RMS) bad("unknown kind");
+  if (d->n < 0 || d->points < 0 || d->n > 1 << 30 || d->points > 1 << 30) bad("n and points must be 0 to 2^30");
+  if (d->channels < 1 || d->channels > 1 << 30) bad("channels must be 1 to 2^30");
+  if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) bad("eps must be finite and not negative");
+  for (const Rows& r : {x_rows(*d, d), y_rows(*d, d), mask_rows(*d, d)})
+    if (!rows_in_range(r)) bad("strides must not be negative, nor reach elements beyond 2^46");
+}
+
+int vec_of(const kc_layer_norm_desc& d, std::initializer_list<const void*> ptrs) {
+  const int es = dtype_bytes(d.dtype);
+  for (int v = 16 / es; v > 1; v /= 2) {
+    const bool board = d.n == 1 || (d.x_board_stride % v == 0 && d.y_board_stride % v == 0);
+    const bool row = d.points == 1 || (d.x_row_stride % v == 0 && d.y_row_stride % v == 0);
+    bool ok = d.channels % v == 0 && board && row;
+    for (const void* p : ptrs) ok = ok && aligned_to(p, (size_t)v * es);
+    if (ok) return v;
+  }
+  return 1;
+}
+
+// Of the parameter gradients' sums, whatever the tensors' alignment.
+size_t back_workspace(const kc_layer_norm_desc& d) {
+  const int64_t rows = (int64_t)d.n * d.points;
+  if (rows == 0) return 0;
+  int64_t blocks = 0;
+  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2)
+    if (d.channels % v == 0) blocks = std::max(blocks, part_blocks(shape_of(rows, d.channels, v, true), rows, d.channels));
+  return ((size_t)blocks * 2 * d.channels * sizeof(float) + 255) / 256 * 256;
+}
+
+// Outputs share no memory with each other or with an input; only a tensor may be its own output.
+void check_outputs(const Rows& out, std::initializer_list<Rows> ins, const Rows& mask,
+                   std::initializer_list<Range> small_in, std::initializer_list<Range> small_out) {
+  if (!rows_distinct(out)) bad("rows of the output share memory");
+  for (const Rows& i : ins)
+    if (rows_overlap(out, i) && !out.same(i)) bad("the output overlaps an input it does not match");
+  if (rows_overlap(out, mask)) bad("the output overlaps the mask");
+  for (const Range& s : small_in)
+    if (ranges_meet(s, out)) bad("the output overlaps another tensor of the call");
+  for (const Range* o = small_out.begin(); o != small_out.end(); o++) {
+    bool meets = ranges_meet(*o, out) || ranges_meet(*o, mask);
+    for (const Rows& i : ins) meets = meets || ranges_meet(*o, i);
+    for (const Range& s : small_in) meets = meets || ranges_meet(*o, s);
+    for (const Range* q = o + 1; q != small_out.end(); q++) meets = meets || ranges_meet(*o, *q);
+    if (meets) bad("the statistics, parameter gradients or workspace overlap another tensor of the call");
+  }
+}
+
+void check_aligned(std::initializer_list<Rows> rows, std::initializer_list<const void*> small, const void* stats) {
+  for (const Rows& r : rows)
+    if (!aligned_to(r.p, r.bytes)) bad("a tensor is not aligned to its element");
+  for (const void* s : small)
+    if (!aligned_to(s, 4)) bad("a float32 tensor is not aligned to its element");
+  if (!aligned_to(stats, 8)) bad("the statistics must be 8-byte aligned");
+}
+
+}  // namespace
+}  // namespace kc
+
+extern "C" int kc_layer_norm(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask,
+                             const float* d_weight, const float* d_bias, void* d_y, float* d_stats, void* stream) {
+  return kc::guard_entry([&] {
+    using namespace kc;
+    check_desc(desc);
+    const kc_layer_norm_desc d = *desc;
+    if (d.n == 0 || d.points == 0) return;
+    if (!d_x || !d_y) bad("null tensor");
+    const Rows x = x_rows(d, d_x), y = y_rows(d, d_y);
+    const int64_t ch = 4 * (int64_t)d.channels, sb = 8 * (int64_t)d.n * d.points;
+    check_aligned({x, y}, {d_mask, d_weight, d_bias}, d_stats);
+    check_outputs(y, {x}, mask_rows(d, d_mask), {{d_weight, ch}, {d_bias, ch}}, {{d_stats, sb}});
+    TensorDevice dev("layer norm", {d_x, d_mask, d_weight, d_bias, d_y, d_stats});
+    LayerParams p{};
+    p.x = d_x;
+    p.mask = d_mask;
+    p.weight = d_weight;
+    p.bias = d_bias;
+    p.y = d_y;
+    p.stats = reinterpret_cast<float2*>(d_stats);
+    run(d, p, vec_of(d, {d_x, d_y}), false, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int kc_layer_norm_backward_workspace(const kc_layer_norm_desc* desc, size_t* bytes) {
+  return kc::guard_entry([&] {
+    kc::check_desc(desc);
+    if (!bytes) kc::bad("null result");
+    *bytes = kc::back_workspace(*desc);
+  });
+}
+
+extern "C" int kc_layer_norm_backward(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask,
+                                      const float* d_weight, const float* d_stats, const void* d_dy, void* d_dx,
+                                      float* d_dweight, float* d_dbias, void* d_workspace, size_t workspace_bytes,
+                                      void* stream) {
+  return kc::guard_entry([&] {
+    using namespace kc;
+    check_desc(desc);
+    const kc_layer_norm_desc d = *desc;
+    const bool none = d.n == 0 || d.points == 0, params = d_dweight || d_dbias;
+    if (!none && (!d_x || !d_dy || !d_dx || !d_stats)) bad("null tensor");
+    const Rows x = x_rows(d, d_x), dy = y_rows(d, d_dy), dx = x_rows(d, d_dx);
+    const int64_t ch = 4 * (int64_t)d.channels, sb = 8 * (int64_t)d.n * d.points;
+    const size_t need = params ? back_workspace(d) : 0;
+    check_aligned({x, dy, dx}, {d_mask, d_weight, d_dweight, d_dbias}, d_stats);
+    check_outputs(dx, {x, dy}, mask_rows(d, d_mask), {{d_weight, ch}, {d_stats, sb}},
+                  {{d_dweight, ch}, {d_dbias, ch}, {need ? d_workspace : nullptr, (int64_t)need}});
+    if (need && (!d_workspace || workspace_bytes < need)) bad("workspace of " + std::to_string(need) + " bytes needed");
+    if (need && !aligned_to(d_workspace, 16)) bad("the workspace must be 16-byte aligned");
+    if (none && !params) return;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    TensorDevice dev("layer norm", {d_x, d_mask, d_weight, d_stats, d_dy, d_dx, d_dweight, d_dbias,
+                                    need ? d_workspace : nullptr});
+    if (none) {
+      if (d_dweight) KC_CUDA(cudaMemsetAsync(d_dweight, 0, (size_t)ch, st));
+      if (d_dbias) KC_CUDA(cudaMemsetAsync(d_dbias, 0, (size_t)ch, st));
+      return;
+    }
+    LayerParams p{};
+    p.x = d_x;
+    p.mask = d_mask;
+    p.weight = d_weight;
+    p.y = d_dx;
+    p.dy = d_dy;
+    p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(d_stats));
+    p.part = need ? static_cast<float*>(d_workspace) : nullptr;
+    p.dweight = d_dweight;
+    p.dbias = d_dbias;
+    run(d, p, vec_of(d, {d_x, d_dy, d_dx}), true, st);
+  });
+}

@@ -1,0 +1,137 @@
+// What the kernels over rows of consecutive elements share: vectors of 1 to 16 bytes of float32, f16 or bf16, sums over
+// the lanes of a warp and over a block, and the addresses of rows that lie in boards.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+#include <utility>
+
+#include "gemm_pair.cuh"
+#include "ops_common.h"
+
+namespace kc {
+
+// VEC neighbouring elements as one load or store.
+template <typename T, int VEC>
+struct RowVec {
+  static constexpr int BYTES = VEC * (int)sizeof(T);
+  using Raw = typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2,
+              typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type;
+
+  __device__ static __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  __device__ static __forceinline__ void store(T* p, Raw r) { *reinterpret_cast<Raw*>(p) = r; }
+  __device__ static __forceinline__ void unpack(const Raw& r, float (&v)[VEC]) {
+    if constexpr (BYTES == 2) {
+      v[0] = to_f<T>(*reinterpret_cast<const T*>(&r));
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+      if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = __uint_as_float(w[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) {
+          if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+          }
+        }
+      }
+    }
+  }
+  __device__ static __forceinline__ Raw pack(const float (&v)[VEC]) {
+    Raw r;
+    if constexpr (BYTES == 2) {
+      *reinterpret_cast<T*>(&r) = from_f<T>(v[0]);
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+      if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) w[i] = __float_as_uint(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+      }
+    }
+    return r;
+  }
+};
+
+// VEC float32 parameters; `wide`: the array is 16-byte aligned, and `p` as far into it as VEC allows.
+template <int VEC>
+__device__ __forceinline__ void load_params(const float* p, bool wide, float (&v)[VEC]) {
+  if (VEC % 4 == 0 && wide) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; i++) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+      v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) v[i] = __ldg(p + i);
+  }
+}
+
+// Sums over groups of `lanes` neighbouring lanes of a warp (a power of two; every lane of the warp takes part).
+__device__ __forceinline__ float2 lanes_sum(float2 v, int lanes) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+  return v;
+}
+
+// Sum over a block of whole warps. `red` holds a value per warp; two calls in a row take different ones.
+__device__ __forceinline__ float2 block_sum(float2 v, float2* red) {
+  v = lanes_sum(v, 32);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
+  return lanes_sum(lane < warps ? red[lane] : make_float2(0.0f, 0.0f), 32);
+}
+
+// Rows of `points` to a board. Boards whose rows go on at one stride are one long row of rows (points 0).
+struct RowMap {
+  int64_t points, board_stride, row_stride;
+  __device__ __forceinline__ int64_t operator()(int64_t r) const {
+    if (points == 0) return r * row_stride;
+    int64_t b;
+    if ((uint64_t)r <= 0xffffffffu) b = (uint32_t)r / (uint32_t)points;
+    else b = r / points;
+    return b * board_stride + (r - b * points) * row_stride;
+  }
+};
+inline RowMap row_map(int64_t n, int64_t points, int64_t board_stride, int64_t row_stride) {
+  if (n == 1) return {0, 0, row_stride};
+  if (points == 1) return {0, 0, board_stride};
+  if ((__int128)points * row_stride == board_stride) return {0, 0, row_stride};
+  return {points, board_stride, row_stride};
+}
+
+// A launch that may start while the stream's last kernel ends; it waits (pdl_wait) before it reads what that one wrote.
+template <typename... KArgs, typename... Args>
+void launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  KC_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+constexpr int kSmCount = 148;
+
+}  // namespace kc

@@ -22,6 +22,7 @@ PRECISION_F32, PRECISION_F16, PRECISION_BF16, PRECISION_AUTO = 0, 1, 2, 3
 ACT_IDENTITY, ACT_RELU, ACT_MISH, ACT_SILU = range(4)
 ROPE_HALVES, ROPE_PAIRS = 0, 1
 ROPE_MAX_AXES = 4
+NORM_LAYER, NORM_RMS = 0, 1
 KC_OK, KC_ERR_INVALID, KC_ERR_PARSE, KC_ERR_CUDA, KC_ERR_TIMEOUT, KC_ERR_DEVICE, KC_ERR_NO_DEVICE = range(7)
 
 _LIB = None
@@ -90,6 +91,31 @@ class GroupNormDesc(ctypes.Structure):
                    *(y_strides or whole), points if mask_stride is None else mask_stride)
 
     _pack = struct.Struct("=6ifi5q").pack_into  # the fields in one go: made for every call of small batches
+
+
+class LayerNormDesc(ctypes.Structure):
+    """kc_layer_norm_desc. dtype: PRECISION_*, kind: NORM_*; strides as GroupNormDesc's."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("kind", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("points", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x_board_stride", ctypes.c_int64),
+        ("x_row_stride", ctypes.c_int64),
+        ("y_board_stride", ctypes.c_int64),
+        ("y_row_stride", ctypes.c_int64),
+        ("mask_board_stride", ctypes.c_int64),
+    ]
+
+    def __init__(self, dtype, kind, n, points, channels, eps, x_strides=None, y_strides=None, mask_stride=None):
+        whole = (points * channels, channels)
+        self._pack(self, 0, dtype, kind, n, points, channels, eps, *(x_strides or whole), *(y_strides or whole),
+                   points if mask_stride is None else mask_stride)
+
+    _pack = struct.Struct("=5if5q").pack_into
 
 
 class RopeDesc(ctypes.Structure):
@@ -163,6 +189,9 @@ _SIGS = {
     "kc_rope_axes": ([ctypes.POINTER(RopeDesc), P, P, P, P, P, P, P], I),
     "kc_rope_axes_backward_workspace": ([ctypes.POINTER(RopeDesc), ctypes.POINTER(ctypes.c_size_t)], I),
     "kc_rope_axes_backward": ([ctypes.POINTER(RopeDesc)] + [P] * 10 + [ctypes.c_size_t, P], I),
+    "kc_layer_norm": ([ctypes.POINTER(LayerNormDesc)] + [P] * 7, I),
+    "kc_layer_norm_backward_workspace": ([ctypes.POINTER(LayerNormDesc), ctypes.POINTER(ctypes.c_size_t)], I),
+    "kc_layer_norm_backward": ([ctypes.POINTER(LayerNormDesc)] + [P] * 9 + [ctypes.c_size_t, P], I),
     "kc_selftest_device_timeout": ([P, I], I),
     "kc_handle_packed_input_ptrs": ([P, ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32)), FPP, FPP,
                                      ctypes.POINTER(ctypes.POINTER(ctypes.c_int32)), FPP], I),
@@ -461,6 +490,27 @@ def rope_axes_backward(desc: RopeDesc, d_dq_out: int, d_dk_out: int, d_q: int, d
     """kc_rope_axes_backward on device pointers: the gradients by q, k and (d_dfreqs) the frequencies."""
     _check(lib().kc_rope_axes_backward(desc, d_dq_out, d_dk_out, d_q, d_k, d_pos, d_freqs, d_dq, d_dk, d_dfreqs,
                                        d_workspace, workspace_bytes, stream))
+
+
+def layer_norm(desc: LayerNormDesc, d_x: int, d_mask: int, d_weight: int, d_bias: int, d_y: int, d_stats: int = 0,
+               stream: int = 0):
+    """kc_layer_norm on device pointers (layer or RMS norm of each token's row; 0 = not given)."""
+    _check(lib().kc_layer_norm(desc, d_x, d_mask, d_weight, d_bias, d_y, d_stats, stream))
+
+
+def layer_norm_backward_workspace(desc: LayerNormDesc) -> int:
+    """kc_layer_norm_backward_workspace: bytes of device workspace a backward call with parameter gradients needs."""
+    n = ctypes.c_size_t()
+    _check(lib().kc_layer_norm_backward_workspace(desc, n))
+    return n.value
+
+
+def layer_norm_backward(desc: LayerNormDesc, d_x: int, d_mask: int, d_weight: int, d_stats: int, d_dy: int, d_dx: int,
+                        d_dweight: int = 0, d_dbias: int = 0, d_workspace: int = 0, workspace_bytes: int = 0,
+                        stream: int = 0):
+    """kc_layer_norm_backward on device pointers: the gradients by x, weight and bias."""
+    _check(lib().kc_layer_norm_backward(desc, d_x, d_mask, d_weight, d_stats, d_dy, d_dx, d_dweight, d_dbias,
+                                        d_workspace, workspace_bytes, stream))
 
 
 def pack_spatial(planes: np.ndarray) -> np.ndarray:
