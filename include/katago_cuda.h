@@ -352,6 +352,59 @@ int kc_layer_norm_backward(const kc_layer_norm_desc* desc, const void* d_x, cons
                            const float* d_stats, const void* d_dy, void* d_dx, float* d_dweight, float* d_dbias,
                            void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* Learned rows looked up by token: y[t] = x[t] + scale * table[id[t]]. Points, moves or states of a token, the learned
+ * counterpart of rotary positions. */
+typedef struct kc_embed_desc {
+  int32_t dtype;      /* KC_PRECISION_* of table, x, y and dy */
+  int32_t channels;   /* 1 .. 2^20 */
+  int64_t tokens;     /* 0 .. 2^30 */
+  int64_t table_rows; /* 1 .. 2^30 */
+  float scale;        /* finite */
+  int32_t reserved;   /* 0 */
+  int64_t table_stride, x_stride, y_stride; /* elements from one row to the next; y_stride is dy's too */
+} kc_embed_desc;
+
+/* d_ids: [tokens] int32. An id outside 0 .. table_rows - 1 (padding) adds nothing: y[t] = x[t]. d_x NULL = 0; y may be
+ * x (same pointer and stride). The gradient by x is dy itself. */
+int kc_embed_rows(const kc_embed_desc* desc, const int32_t* d_ids, const void* d_table, const void* d_x, void* d_y,
+                  void* stream);
+
+/* The table's gradient, d_dtable [table_rows][channels] float32 (overwritten): scale times the sum of dy over the tokens
+ * that have the row's id, added in the tokens' order within pieces of a fixed length; 0 for a row that none has.
+ * table_stride and x_stride are ignored. */
+int kc_embed_rows_backward_workspace(const kc_embed_desc* desc, size_t* bytes);
+int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* d_ids, const void* d_dy, float* d_dtable,
+                           void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation: the loss of a student's logits (policy rows of 362 moves, or any classes) against a teacher's top
+ * logits. With q = softmax(logits / T) and p[j] = exp(top_logits[j] / T - L) over the row's entries j,
+ *   loss = T^2 * sum over j of p[j] * (log p[j] - log q[id[j]]),
+ * L = the entries' own log sum of exp(top_logits / T) (p adds up to 1), or d_teacher_log_sum[row], the teacher's over all
+ * its classes (p adds up to what the entries hold of it; the rest of the teacher's distribution is left out). */
+typedef struct kc_distill_desc {
+  int32_t dtype;     /* KC_PRECISION_* of logits and dlogits */
+  int32_t classes;   /* 1 .. 2^30 */
+  int64_t rows;      /* 0 .. 2^30 */
+  int32_t top;       /* 1 .. 1024 entries of a row */
+  float temperature; /* T, 2^-20 .. 2^20 */
+  int64_t logits_stride, dlogits_stride; /* elements from one row to the next */
+  int64_t top_stride;                    /* of d_ids and of d_top_logits */
+} kc_distill_desc;
+
+/* d_ids: [rows][top] int32, d_top_logits: [rows][top] float32. An entry whose id is outside 0 .. classes - 1 or whose
+ * logit is -inf is absent; entries of one class add up. A row without entries has loss 0 and gradient 0, whatever its
+ * logits hold. Logits of -inf (illegal moves) have probability 0: an entry there makes the loss infinite. NaN among a
+ * row's logits, +inf, or nothing but -inf make its loss NaN. d_loss: [rows] float32. d_stats (NULL = not wanted):
+ * [rows][2] float32, the row's largest logit and the sum of exp((logit - largest) / T), both 0 without entries. */
+int kc_distill_top(const kc_distill_desc* desc, const void* d_logits, const int32_t* d_ids, const float* d_top_logits,
+                   const float* d_teacher_log_sum, float* d_loss, float* d_stats, void* stream);
+
+/* The gradient by the logits, dlogits[i] = dloss * T * (q[i] * sum of p - sum of p[j] at id[j] = i), given the forward
+ * pass's inputs and d_stats. d_dloss: [rows] float32, NULL = 1. dlogits may be the logits (same pointer and stride). */
+int kc_distill_top_backward(const kc_distill_desc* desc, const void* d_logits, const int32_t* d_ids,
+                            const float* d_top_logits, const float* d_teacher_log_sum, const float* d_stats,
+                            const float* d_dloss, void* d_dlogits, void* stream);
+
 /* Failure-detection self-test. Every spin-wait in this library's kernels is bounded: when a wait runs out, the
  * kernel records an error code in the handle's device error word, releases what it holds and returns, and the next
  * kc_wait / kc_synchronize reports KC_ERR_DEVICE (the handle stays usable). This enqueues on the handle's stream

@@ -1,0 +1,611 @@
+// Learned rows looked up by token, and the gradient of their table (kc_embed_rows, kc_embed_rows_backward).
+//
+//   y[t] = x[t] + scale table[id[t]]            (x may be absent; an id outside the table adds nothing)
+//   dtable[v] = scale sum_{t: id[t] = v} dy[t]  (0 for rows that no token has)
+//
+// Forward, a few lanes of a warp take a token's row. Backward, the tokens are sorted by id (a stable radix sort of the
+// ids, so that a row's sum has the tokens' order whatever the timing) and the sorted list is cut into equal pieces
+// whatever the rows' shares of it, so that a row that most tokens have costs no more than many rows that few have: a
+// group of lanes sums its piece run by run, writes the runs that lie inside it, and leaves its first and last run to its
+// block, which joins those of its pieces; a last launch joins runs over blocks. Sums are float32: chains of at most a
+// piece, then the pieces of a block, then the blocks.
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "../../include/katago_cuda.h"
+#include "rows.cuh"
+
+namespace kc {
+namespace {
+
+[[noreturn]] void bad(const std::string& what) { fail(KC_ERR_INVALID, "CUDA backend: looked-up rows: " + what); }
+
+constexpr int kThreads = 256;
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kMaxBits = 9;          // of a digit: no more digits than threads; 16 warps x 512 counts are 32 KB
+constexpr int kTile = 2048;          // tokens of a block of the sort, at least
+constexpr int kUnroll = 8;           // tokens whose rows a lane has in flight
+
+struct EmbedParams {
+  const int32_t* ids;
+  const void* table;
+  const void* x;
+  void* y;
+  int64_t tokens, table_rows;
+  int64_t ts, xs, ys;
+  int C, lanes;
+  float scale;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) embed_kernel(const EmbedParams p) {
+  using V = RowVec<T, VEC>;
+  const int lane = threadIdx.x & (p.lanes - 1), per = kThreads / p.lanes, nvec = p.C / VEC;
+  for (int64_t t = (int64_t)blockIdx.x * per + threadIdx.x / p.lanes; t < p.tokens; t += (int64_t)gridDim.x * per) {
+    const int id = __ldg(p.ids + t);
+    const bool there = id >= 0 && id < p.table_rows;
+    const T* row = static_cast<const T*>(p.table) + (there ? id * p.ts : 0);
+    const T* x = p.x ? static_cast<const T*>(p.x) + t * p.xs : nullptr;
+    T* y = static_cast<T*>(p.y) + t * p.ys;
+    for (int v0 = lane; v0 < nvec; v0 += 4 * p.lanes) {
+      typename V::Raw a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int v = v0 + i * p.lanes;
+        if (v >= nvec) continue;
+        if (there) a[i] = V::load(row + v * VEC);
+        if (x) b[i] = V::load(x + v * VEC);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int v = v0 + i * p.lanes;
+        if (v >= nvec) continue;
+        float f[VEC], o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o[j] = 0.0f;
+        if (x) V::unpack(b[i], o);
+        if (there) {
+          V::unpack(a[i], f);
+#pragma unroll
+          for (int j = 0; j < VEC; j++) o[j] = fmaf(f[j], p.scale, o[j]);
+        }
+        V::store(y + v * VEC, V::pack(o));
+      }
+    }
+  }
+}
+
+// ---- tokens sorted by id -----------------------------------------------------------------------------------------
+// Entries are (key, token); the key of an id outside the table is table_rows, behind all rows. Each pass orders by one
+// digit and keeps the order of equal ones.
+struct SortParams {
+  const int32_t* ids;  // the first pass's input, otherwise `in`
+  const int2* in;
+  int2* out;
+  int* hist;           // [tiles][1 << bits]
+  int tokens, rows;
+  int shift, bits;
+  int tiles, tile;     // tokens of a tile
+};
+
+__device__ __forceinline__ int2 sort_entry(const SortParams& p, int i) {
+  if (!p.ids) return p.in[i];
+  const int id = p.ids[i];
+  return make_int2(id >= 0 && id < p.rows ? id : p.rows, i);
+}
+
+__global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortParams p) {
+  __shared__ int count[1 << kMaxBits];
+  pdl_wait();
+  pdl_trigger();
+  const int bins = 1 << p.bits;
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) count[b] = 0;
+  __syncthreads();
+  const int i0 = blockIdx.x * p.tile, i1 = min(p.tokens, i0 + p.tile);
+  for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
+    const int d = sort_entry(p, i).x >> p.shift & (bins - 1);
+    const uint32_t peers = __match_any_sync(__activemask(), d);
+    if (threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&count[d], __popc(peers));
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) p.hist[(size_t)blockIdx.x * bins + b] = count[b];
+}
+
+// Places the tile's entries. Each warp owns a share of consecutive entries: it counts its digits, takes its places
+// behind those of the tiles and warps before it, and goes over them again.
+__device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* count, int* scan) {
+  const int bins = 1 << p.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) count[b] = 0;
+  __syncthreads();
+  const int i0 = tile * p.tile, i1 = min(p.tokens, i0 + p.tile);
+  const int share = ((i1 - i0 + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int w0 = i0 + warp * share, w1 = min(i1, w0 + share);
+  int* mine = count + warp * bins;
+  for (int i = w0 + lane; i - lane < w1; i += 32) {
+    const int d = i < w1 ? sort_entry(p, i).x >> p.shift & (bins - 1) : bins;
+    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    if (d < bins && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  // thread b: digit b's places
+  int before = 0, total = 0;
+  if (threadIdx.x < bins) {
+    if (p.tiles > 1) {
+#pragma unroll 8
+      for (int t = 0; t < p.tiles; t++) {
+        const int h = p.hist[(size_t)t * bins + threadIdx.x];
+        if (t < tile) before += h;
+        total += h;
+      }
+    } else {
+      for (int w = 0; w < kSortWarps; w++) total += count[w * bins + threadIdx.x];
+    }
+  }
+  // exclusive sums of the totals over the digits
+  int sum = total;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) scan[warp] = sum;
+  __syncthreads();
+  int at = sum - total + before;
+  for (int w = 0; w < warp; w++) at += scan[w];
+  if (threadIdx.x < bins)
+    for (int w = 0; w < kSortWarps; w++) {
+      const int n = count[w * bins + threadIdx.x];
+      count[w * bins + threadIdx.x] = at;
+      at += n;
+    }
+  __syncthreads();
+  for (int i = w0 + lane; i - lane < w1; i += 32) {
+    const int2 e = i < w1 ? sort_entry(p, i) : make_int2(0, 0);
+    const int d = i < w1 ? e.x >> p.shift & (bins - 1) : bins;
+    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    if (d < bins) p.out[mine[d] + __popc(peers & ((1u << lane) - 1))] = e;
+    __syncwarp();
+    if (d < bins && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    __syncwarp();
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) embed_place_kernel(const SortParams p) {
+  extern __shared__ int count[];
+  __shared__ int scan[kSortWarps];
+  pdl_wait();
+  pdl_trigger();
+  place_tile(p, blockIdx.x, count, scan);
+}
+
+// All passes of a list that one block sorts.
+__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p, int passes, int2* a, int2* b) {
+  extern __shared__ int count[];
+  __shared__ int scan[kSortWarps];
+  pdl_trigger();
+  for (int i = 0; i < passes; i++) {
+    p.out = (passes - i) % 2 ? a : b;  // the last pass ends in a
+    p.shift = i * p.bits;
+    place_tile(p, 0, count, scan);
+    __syncthreads();
+    p.ids = nullptr;
+    p.in = p.out;
+  }
+}
+
+// ---- sums of sorted rows -----------------------------------------------------------------------------------------
+struct SumParams {
+  const int2* list;  // sorted entries
+  const void* dy;
+  float* dtable;
+  float* part;       // [blocks][2][C]: the first and last run of a block's pieces
+  int2* part_ids;    // [blocks]: their keys; y = -1 where one run is all
+  int64_t ys;
+  int tokens, rows, C, lanes;
+  int piece;         // entries of a group's piece, a multiple of kUnroll
+  int blocks;        // over the list; those behind them write the rows that no token has
+  int wide;          // dtable's rows are 16-byte aligned
+  float scale;
+};
+
+template <int VEC>
+__device__ __forceinline__ void store_row(const SumParams& p, int id, int c, const float (&v)[VEC]) {
+  if (id >= p.rows) return;
+  float* out = p.dtable + (size_t)id * p.C + c;
+  if (VEC % 4 == 0 && p.wide) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; i++)
+      reinterpret_cast<float4*>(out)[i] = make_float4(v[4 * i] * p.scale, v[4 * i + 1] * p.scale,
+                                                      v[4 * i + 2] * p.scale, v[4 * i + 3] * p.scale);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) out[i] = v[i] * p.scale;
+  }
+}
+
+// The rows from `row0` on that the list lacks, a thread looking for each, then all writing them.
+__device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int columns, int* absent) {
+  __shared__ int n;
+  if (threadIdx.x == 0) n = 0;
+  __syncthreads();
+  const int row = row0 + threadIdx.x;
+  if (row < p.rows) {
+    int lo = 0, hi = p.tokens;  // the first entry whose key is not below row
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (p.list[mid].x < row) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo == p.tokens || p.list[lo].x != row) absent[atomicAdd(&n, 1)] = row;
+  }
+  __syncthreads();
+  const int c0 = blockIdx.y * columns, c1 = min(p.C, c0 + columns);
+  const int width = p.wide ? (c1 - c0) / 4 : c1 - c0;
+  for (int i = threadIdx.x; i < n * width; i += kThreads) {
+    float* out = p.dtable + (size_t)absent[i / width] * p.C + c0;
+    if (p.wide) reinterpret_cast<float4*>(out)[i % width] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    else out[i % width] = 0.0f;
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) embed_sum_kernel(const SumParams p) {
+  using V = RowVec<T, VEC>;
+  __shared__ float slot[2][kThreads * VEC];  // [first, last][group][lane][VEC]
+  __shared__ int key[2][kThreads / 2];
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, p.lanes * VEC, key[0]);
+  const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kThreads / lanes;
+  const int v = blockIdx.y * lanes + lane, c = v * VEC;
+  const bool here = v < p.C / VEC;
+  const T* dy = static_cast<const T*>(p.dy) + c;
+  const int64_t i0 = ((int64_t)blockIdx.x * groups + group) * p.piece;
+  float acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
+  int cur = -1, first = -1;  // the run at hand, and the piece's first one once it is over
+  for (int e0 = 0; e0 < p.piece; e0 += kUnroll) {
+    int2 e[kUnroll];
+    typename V::Raw raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) e[u] = i0 + e0 + u < p.tokens ? p.list[i0 + e0 + u] : make_int2(p.rows, 0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++)
+      if (here && e[u].x < p.rows) raw[u] = V::load(dy + e[u].y * p.ys);
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      if (e[u].x != cur) {
+        if (cur >= 0) {
+          if (first < 0) {
+            first = cur;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) slot[0][threadIdx.x * VEC + j] = acc[j];
+          } else if (here) {
+            store_row<VEC>(p, cur, c, acc);
+          }
+        }
+        cur = e[u].x;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
+      }
+      if (here && cur < p.rows) {
+        float f[VEC];
+        V::unpack(raw[u], f);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) acc[j] += f[j];
+      }
+    }
+  }
+  const int last = first < 0 ? 0 : 1;
+#pragma unroll
+  for (int j = 0; j < VEC; j++) slot[last][threadIdx.x * VEC + j] = acc[j];
+  if (lane == 0) {
+    key[0][group] = first < 0 ? cur : first;
+    key[1][group] = first < 0 ? -1 : cur;
+  }
+  __syncthreads();
+  // the groups' first and last runs in order, a thread to a channel
+  const int width = lanes * VEC;
+  for (int j = threadIdx.x; j < width; j += kThreads) {
+    const int col = blockIdx.y * width + j;
+    if (col >= p.C) continue;
+    float* part = p.part + (size_t)blockIdx.x * 2 * p.C + col;
+    float sum = 0.0f;
+    int run = key[0][0], head = -1;
+    for (int g = 0; g < groups; g++)
+      for (int k = 0; k < 2; k++) {
+        const int id = key[k][g];
+        if (id < 0) continue;
+        if (id != run) {
+          if (head < 0) head = run, part[0] = sum;
+          else if (run < p.rows) p.dtable[(size_t)run * p.C + col] = sum * p.scale;
+          run = id;
+          sum = 0.0f;
+        }
+        sum += slot[k][g * width + j];
+      }
+    part[head < 0 ? 0 : p.C] = sum;
+    if (col == 0) p.part_ids[blockIdx.x] = make_int2(head < 0 ? run : head, head < 0 ? -1 : run);
+  }
+}
+
+// Runs over blocks. Block i of the list takes those that start in its first run (where the block before ends with
+// another key) and in its last one: the sum of that and of the first runs behind it with the same key. A block to 32
+// channels, 8 threads share a run's blocks.
+__global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumParams p) {
+  __shared__ float red[kThreads / 32][33];
+  __shared__ int stop;
+  pdl_wait();
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c = blockIdx.y * 32 + tx;
+  const int2 own = p.part_ids[blockIdx.x];
+  int2 prev = make_int2(-1, -1);
+  if (blockIdx.x > 0) prev = p.part_ids[blockIdx.x - 1];
+  for (int k = 0; k < 2; k++) {
+    const int id = k ? own.y : own.x;
+    if (id < 0 || id >= p.rows) continue;
+    if (k == 0 && id == (prev.y < 0 ? prev.x : prev.y)) continue;
+    // blocks [blockIdx.x + 1, stop) begin with the run; it goes beyond this block only if it is its last one
+    int end = blockIdx.x + 1;
+    if (k == 1 || own.y < 0) {
+      for (bool more = true; more; end += kThreads) {
+        if (threadIdx.x == 0) stop = kThreads;
+        __syncthreads();
+        const int j = end + threadIdx.x;
+        int2 q = make_int2(-1, -1);
+        if (j < p.blocks) q = p.part_ids[j];
+        const bool begins = j < p.blocks && q.x == id;
+        if (!begins || q.y >= 0) atomicMin(&stop, (int)threadIdx.x + (begins ? 1 : 0));
+        __syncthreads();
+        more = stop == kThreads;
+        if (!more) end += stop - kThreads;
+        // a run that ends with the last block looked at goes on there as nothing: the next round stops at once
+        __syncthreads();
+      }
+    }
+    float s = 0.0f;
+    if (c < p.C)
+#pragma unroll 4
+      for (int j = blockIdx.x + 1 + ty; j < end; j += kThreads / 32) s += p.part[(size_t)j * 2 * p.C + c];
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < p.C) {
+      s = p.part[(size_t)blockIdx.x * 2 * p.C + k * p.C + c];
+      for (int i = 0; i < kThreads / 32; i++) s += red[i][tx];
+      p.dtable[(size_t)id * p.C + c] = s * p.scale;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+
+// Lanes of a row: the widest group that leaves at most an eighth of its lanes idle.
+int lanes_of(int nvec) {
+  for (int lanes = 32; lanes > 2; lanes /= 2)
+    if (((nvec + lanes - 1) / lanes * lanes - nvec) * 8 <= nvec) return lanes;
+  return 2;
+}
+
+struct SumShape {
+  int lanes, chunks, piece, blocks;
+};
+SumShape sum_shape(int64_t tokens, int C, int vec) {
+  SumShape s;
+  const int nvec = C / vec;
+  s.lanes = lanes_of(nvec);
+  s.chunks = (nvec + s.lanes - 1) / s.lanes;
+  const int groups = kThreads / s.lanes;
+  // four blocks to an SM, of pieces of 16 to 256 entries
+  const int64_t want = (tokens * s.chunks + (int64_t)4 * kSmCount * groups - 1) / ((int64_t)4 * kSmCount * groups);
+  s.piece = (int)std::min<int64_t>(256, std::max<int64_t>(16, (want + kUnroll - 1) / kUnroll * kUnroll));
+  s.blocks = (int)((tokens + (int64_t)s.piece * groups - 1) / ((int64_t)s.piece * groups));
+  return s;
+}
+
+struct SortShape {
+  int passes, bits, tiles, tile;
+};
+SortShape sort_shape(int64_t tokens, int64_t rows) {
+  SortShape s;
+  int bits = 1;  // of keys 0 .. rows
+  while (rows >> bits) bits++;
+  s.passes = (bits + kMaxBits - 1) / kMaxBits;
+  s.bits = (bits + s.passes - 1) / s.passes;
+  s.tiles = (int)std::min<int64_t>(kSmCount, (tokens + kTile - 1) / kTile);
+  s.tile = (int)((tokens + s.tiles - 1) / s.tiles);
+  s.tiles = (int)((tokens + s.tile - 1) / s.tile);
+  return s;
+}
+
+struct Layout {
+  size_t a = 0, b = 0, hist = 0, part = 0, ids = 0, total = 0;
+};
+Layout layout(const kc_embed_desc& d) {
+  Layout l;
+  if (d.tokens == 0) return l;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const SortShape s = sort_shape(d.tokens, d.table_rows);
+  int blocks = 0;
+  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2)
+    if (d.channels % v == 0) blocks = std::max(blocks, sum_shape(d.tokens, d.channels, v).blocks);
+  l.a = take((size_t)d.tokens * sizeof(int2));
+  if (s.passes > 1) l.b = take((size_t)d.tokens * sizeof(int2));
+  if (s.tiles > 1) l.hist = take(((size_t)s.tiles << s.bits) * sizeof(int));
+  l.part = take((size_t)blocks * 2 * d.channels * sizeof(float));
+  l.ids = take((size_t)blocks * sizeof(int2));
+  l.total = at;
+  return l;
+}
+
+void sort_tokens(const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, int* hist, cudaStream_t st) {
+  const SortShape s = sort_shape(d.tokens, d.table_rows);
+  SortParams p{ids, nullptr, nullptr, hist, (int)d.tokens, (int)d.table_rows, 0, s.bits, s.tiles, s.tile};
+  const size_t smem = ((size_t)kSortWarps << s.bits) * sizeof(int);
+  if (s.tiles == 1) {
+    embed_sort_kernel<<<1, kSortThreads, smem, st>>>(p, s.passes, a, b);
+    KC_CUDA(cudaGetLastError());
+    return;
+  }
+  for (int i = 0; i < s.passes; i++) {
+    p.out = (s.passes - i) % 2 ? a : b;  // the last pass ends in a
+    p.shift = i * s.bits;
+    if (i == 0) {
+      embed_count_kernel<<<s.tiles, kSortThreads, 0, st>>>(p);
+      KC_CUDA(cudaGetLastError());
+    } else {
+      launch_after(embed_count_kernel, dim3(s.tiles), dim3(kSortThreads), 0, st, p);
+    }
+    launch_after(embed_place_kernel, dim3(s.tiles), dim3(kSortThreads), smem, st, p);
+    p.ids = nullptr;
+    p.in = p.out;
+  }
+}
+
+template <typename T, int VEC>
+void launch_sum(const SumParams& p, const SumShape& s, cudaStream_t st) {
+  const unsigned absent = (unsigned)((p.rows + (int64_t)kThreads - 1) / kThreads);
+  launch_after(embed_sum_kernel<T, VEC>, dim3((unsigned)s.blocks + absent, (unsigned)s.chunks), dim3(kThreads), 0, st, p);
+  launch_after(embed_join_kernel, dim3((unsigned)s.blocks, (unsigned)((p.C + 31) / 32)), dim3(kThreads), 0, st, p);
+}
+
+template <typename T>
+void run_type(const EmbedParams& p, int vec, unsigned blocks, cudaStream_t st) {
+  if (vec == 8) {
+    if constexpr (sizeof(T) == 2) embed_kernel<T, 8><<<blocks, kThreads, 0, st>>>(p);
+  } else if (vec == 4) {
+    embed_kernel<T, 4><<<blocks, kThreads, 0, st>>>(p);
+  } else if (vec == 2) {
+    embed_kernel<T, 2><<<blocks, kThreads, 0, st>>>(p);
+  } else {
+    embed_kernel<T, 1><<<blocks, kThreads, 0, st>>>(p);
+  }
+  KC_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void sum_type(const SumParams& p, const SumShape& s, int vec, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return launch_sum<T, 8>(p, s, st);
+  if (vec == 4) return launch_sum<T, 4>(p, s, st);
+  if (vec == 2) return launch_sum<T, 2>(p, s, st);
+  launch_sum<T, 1>(p, s, st);
+}
+
+Rows rows_of(const kc_embed_desc& d, const void* p, int64_t count, int64_t stride) {
+  return {p, count, 1, d.channels, count > 1 ? stride : 0, 0, dtype_bytes(d.dtype)};
+}
+
+void check_desc(const kc_embed_desc* d) {
+  if (!d) bad("null descriptor");
+  if (d->dtype < KC_PRECISION_F32 || d->dtype > KC_PRECISION_BF16) bad("unknown dtype");
+  if (d->tokens < 0 || d->tokens > 1 << 30) bad("tokens must be 0 to 2^30");
+  if (d->table_rows < 1 || d->table_rows > 1 << 30) bad("table_rows must be 1 to 2^30");
+  if (d->channels < 1 || d->channels > 1 << 20) bad("channels must be 1 to 2^20");
+  if (!std::isfinite(d->scale)) bad("scale must be finite");
+}
+
+void check_rows(const Rows& r) {
+  if (!rows_in_range(r)) bad("strides must not be negative, nor reach elements beyond 2^46");
+  if (!aligned_to(r.p, r.bytes)) bad("a tensor is not aligned to its element");
+}
+
+int vec_of(const kc_embed_desc& d, std::initializer_list<Rows> rows) {
+  const int es = dtype_bytes(d.dtype);
+  for (int v = 16 / es; v > 1; v /= 2) {
+    bool ok = d.channels % v == 0;
+    for (const Rows& r : rows) ok = ok && aligned_to(r.p, (size_t)v * es) && r.outer_stride % v == 0;
+    if (ok) return v;
+  }
+  return 1;
+}
+
+}  // namespace
+}  // namespace kc
+
+extern "C" int kc_embed_rows(const kc_embed_desc* desc, const int32_t* d_ids, const void* d_table, const void* d_x,
+                             void* d_y, void* stream) {
+  return kc::guard_entry([&] {
+    using namespace kc;
+    check_desc(desc);
+    const kc_embed_desc d = *desc;
+    const Rows table = rows_of(d, d_table, d.table_rows, d.table_stride), x = rows_of(d, d_x, d.tokens, d.x_stride),
+               y = rows_of(d, d_y, d.tokens, d.y_stride);
+    check_rows(table);
+    if (d_x) check_rows(x);
+    check_rows(y);
+    if (d.tokens == 0) return;
+    if (!d_ids || !d_table || !d_y) bad("null tensor");
+    if (!aligned_to(d_ids, 4)) bad("the ids are not aligned to their element");
+    if (!rows_distinct(y)) bad("rows of the output share memory");
+    if (rows_overlap(y, table) || ranges_meet(Range{d_ids, 4 * d.tokens}, y)) bad("the output overlaps an input");
+    if (rows_overlap(y, x) && !y.same(x)) bad("the output overlaps an input it does not match");
+    TensorDevice dev("looked-up rows", {d_ids, d_table, d_x, d_y});
+    EmbedParams p{d_ids, d_table, d_x, d_y, d.tokens, d.table_rows, table.outer_stride, x.outer_stride,
+                  y.outer_stride, d.channels, 0, d.scale};
+    const int vec = d_x ? vec_of(d, {table, x, y}) : vec_of(d, {table, y});
+    p.lanes = lanes_of(d.channels / vec);
+    const int64_t per = kThreads / p.lanes;
+    const unsigned blocks = (unsigned)std::min<int64_t>((d.tokens + per - 1) / per, 1 << 20);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d.dtype == KC_PRECISION_F32) run_type<float>(p, vec, blocks, st);
+    else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, vec, blocks, st);
+    else run_type<__nv_bfloat16>(p, vec, blocks, st);
+  });
+}
+
+extern "C" int kc_embed_rows_backward_workspace(const kc_embed_desc* desc, size_t* bytes) {
+  return kc::guard_entry([&] {
+    kc::check_desc(desc);
+    if (!bytes) kc::bad("null result");
+    *bytes = kc::layout(*desc).total;
+  });
+}
+
+extern "C" int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* d_ids, const void* d_dy,
+                                      float* d_dtable, void* d_workspace, size_t workspace_bytes, void* stream) {
+  return kc::guard_entry([&] {
+    using namespace kc;
+    check_desc(desc);
+    const kc_embed_desc d = *desc;
+    const Rows dy = rows_of(d, d_dy, d.tokens, d.y_stride);
+    check_rows(dy);
+    if (!d_dtable || (d.tokens && (!d_ids || !d_dy))) bad("null tensor");
+    if (!aligned_to(d_ids, 4) || !aligned_to(d_dtable, 4)) bad("a tensor is not aligned to its element");
+    const Layout l = layout(d);
+    const Range table{d_dtable, 4 * d.table_rows * d.channels}, ids{d_ids, 4 * d.tokens},
+        space{l.total ? d_workspace : nullptr, (int64_t)l.total};
+    if (ranges_meet(table, dy) || ranges_meet(table, ids)) bad("the output overlaps an input");
+    if (ranges_meet(space, dy) || ranges_meet(space, ids) || ranges_meet(space, table))
+      bad("the workspace overlaps another tensor of the call");
+    if (l.total && (!d_workspace || workspace_bytes < l.total))
+      bad("workspace of " + std::to_string(l.total) + " bytes needed");
+    if (l.total && !aligned_to(d_workspace, 16)) bad("the workspace must be 16-byte aligned");
+    TensorDevice dev("looked-up rows", {d_ids, d_dy, d_dtable, space.p});
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d.tokens == 0) {
+      KC_CUDA(cudaMemsetAsync(d_dtable, 0, (size_t)table.bytes, st));
+      return;
+    }
+    char* ws = static_cast<char*>(d_workspace);
+    int2* list = reinterpret_cast<int2*>(ws + l.a);
+    sort_tokens(d, d_ids, list, reinterpret_cast<int2*>(ws + l.b), reinterpret_cast<int*>(ws + l.hist), st);
+    const int vec = vec_of(d, {dy});
+    const SumShape s = sum_shape(d.tokens, d.channels, vec);
+    const SumParams p{list, d_dy, d_dtable, reinterpret_cast<float*>(ws + l.part), reinterpret_cast<int2*>(ws + l.ids),
+                      dy.outer_stride, (int)d.tokens, (int)d.table_rows, d.channels, s.lanes, s.piece, s.blocks,
+                      d.channels % 4 == 0 && aligned_to(d_dtable, 16), d.scale};
+    if (d.dtype == KC_PRECISION_F32) sum_type<float>(p, s, vec, st);
+    else if (d.dtype == KC_PRECISION_F16) sum_type<__half>(p, s, vec, st);
+    else sum_type<__nv_bfloat16>(p, s, vec, st);
+  });
+}

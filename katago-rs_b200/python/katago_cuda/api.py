@@ -118,6 +118,51 @@ class LayerNormDesc(ctypes.Structure):
     _pack = struct.Struct("=5if5q").pack_into
 
 
+class EmbedDesc(ctypes.Structure):
+    """kc_embed_desc. dtype: PRECISION_*; strides in elements, None = contiguous rows."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+    def __init__(self, dtype, tokens, channels, table_rows, scale=1.0, table_stride=None, x_stride=None,
+                 y_stride=None):
+        strides = (channels if s is None else s for s in (table_stride, x_stride, y_stride))
+        self._pack(self, 0, dtype, channels, tokens, table_rows, scale, 0, *strides)
+
+    _pack = struct.Struct("=2i2qfi3q").pack_into
+
+
+class DistillDesc(ctypes.Structure):
+    """kc_distill_desc. dtype: PRECISION_*; strides in elements, None = contiguous rows."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("classes", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("top", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("logits_stride", ctypes.c_int64),
+        ("dlogits_stride", ctypes.c_int64),
+        ("top_stride", ctypes.c_int64),
+    ]
+
+    def __init__(self, dtype, rows, classes, top, temperature=1.0, logits_stride=None, dlogits_stride=None,
+                 top_stride=None):
+        self._pack(self, 0, dtype, classes, rows, top, temperature, classes if logits_stride is None else logits_stride,
+                   classes if dlogits_stride is None else dlogits_stride, top if top_stride is None else top_stride)
+
+    _pack = struct.Struct("=2iqif3q").pack_into
+
+
 class RopeDesc(ctypes.Structure):
     """kc_rope_desc. dtype: PRECISION_*, layout: ROPE_*; the strides are (token, head) in elements, None =
     contiguous [tokens][heads][head_dim]."""
@@ -192,6 +237,11 @@ _SIGS = {
     "kc_layer_norm": ([ctypes.POINTER(LayerNormDesc)] + [P] * 7, I),
     "kc_layer_norm_backward_workspace": ([ctypes.POINTER(LayerNormDesc), ctypes.POINTER(ctypes.c_size_t)], I),
     "kc_layer_norm_backward": ([ctypes.POINTER(LayerNormDesc)] + [P] * 9 + [ctypes.c_size_t, P], I),
+    "kc_embed_rows": ([ctypes.POINTER(EmbedDesc)] + [P] * 5, I),
+    "kc_embed_rows_backward_workspace": ([ctypes.POINTER(EmbedDesc), ctypes.POINTER(ctypes.c_size_t)], I),
+    "kc_embed_rows_backward": ([ctypes.POINTER(EmbedDesc)] + [P] * 4 + [ctypes.c_size_t, P], I),
+    "kc_distill_top": ([ctypes.POINTER(DistillDesc)] + [P] * 7, I),
+    "kc_distill_top_backward": ([ctypes.POINTER(DistillDesc)] + [P] * 8, I),
     "kc_selftest_device_timeout": ([P, I], I),
     "kc_handle_packed_input_ptrs": ([P, ctypes.POINTER(ctypes.POINTER(ctypes.c_uint32)), FPP, FPP,
                                      ctypes.POINTER(ctypes.POINTER(ctypes.c_int32)), FPP], I),
@@ -511,6 +561,37 @@ def layer_norm_backward(desc: LayerNormDesc, d_x: int, d_mask: int, d_weight: in
     """kc_layer_norm_backward on device pointers: the gradients by x, weight and bias."""
     _check(lib().kc_layer_norm_backward(desc, d_x, d_mask, d_weight, d_stats, d_dy, d_dx, d_dweight, d_dbias,
                                         d_workspace, workspace_bytes, stream))
+
+
+def embed_rows(desc: EmbedDesc, d_ids: int, d_table: int, d_x: int, d_y: int, stream: int = 0):
+    """kc_embed_rows on device pointers: y[t] = x[t] + scale * table[id[t]] (d_x 0: no x)."""
+    _check(lib().kc_embed_rows(desc, d_ids, d_table, d_x, d_y, stream))
+
+
+def embed_rows_backward_workspace(desc: EmbedDesc) -> int:
+    """kc_embed_rows_backward_workspace: bytes of device workspace a backward call needs."""
+    n = ctypes.c_size_t()
+    _check(lib().kc_embed_rows_backward_workspace(desc, n))
+    return n.value
+
+
+def embed_rows_backward(desc: EmbedDesc, d_ids: int, d_dy: int, d_dtable: int, d_workspace: int = 0,
+                        workspace_bytes: int = 0, stream: int = 0):
+    """kc_embed_rows_backward on device pointers: the table's gradient, float32."""
+    _check(lib().kc_embed_rows_backward(desc, d_ids, d_dy, d_dtable, d_workspace, workspace_bytes, stream))
+
+
+def distill_top(desc: DistillDesc, d_logits: int, d_ids: int, d_top_logits: int, d_teacher_log_sum: int, d_loss: int,
+                d_stats: int = 0, stream: int = 0):
+    """kc_distill_top on device pointers: each row's loss against a teacher's top logits (0 = not given)."""
+    _check(lib().kc_distill_top(desc, d_logits, d_ids, d_top_logits, d_teacher_log_sum, d_loss, d_stats, stream))
+
+
+def distill_top_backward(desc: DistillDesc, d_logits: int, d_ids: int, d_top_logits: int, d_teacher_log_sum: int,
+                         d_stats: int, d_dloss: int, d_dlogits: int, stream: int = 0):
+    """kc_distill_top_backward on device pointers: the gradient by the logits (d_dloss 0: 1 for every row)."""
+    _check(lib().kc_distill_top_backward(desc, d_logits, d_ids, d_top_logits, d_teacher_log_sum, d_stats, d_dloss,
+                                         d_dlogits, stream))
 
 
 def pack_spatial(planes: np.ndarray) -> np.ndarray:

@@ -84,3 +84,97 @@ def test_layer_norm_of_nothing(n, points):
     assert api.layer_norm_backward_workspace(d) == 0
     lforward(d, x=0, y=0, mask=0, st=0)
     lbackward(d, x=0, dy=0, dx=0, st=0, mask=0, dw=0, db=0, ws=0, size=0)
+
+
+IDS, TABLE, DT = (A + (i << 32) for i in range(20, 23))
+
+
+def edesc(**kw):
+    a = dict(dtype=api.PRECISION_BF16, tokens=722, channels=384, table_rows=362, scale=2.0)
+    strides = {k: kw.pop(k) for k in list(kw) if k.endswith("stride")}
+    a.update(kw)
+    return api.EmbedDesc(*a.values(), **strides)
+
+
+def look_up(d, ids=IDS, table=TABLE, x=X, y=Y):
+    api.embed_rows(d, ids, table, x, y, 0)
+
+
+def look_up_back(d, ids=IDS, dy=DY, dt=DT, ws=WS, size=1 << 30):
+    api.embed_rows_backward(d, ids, dy, dt, ws, size, 0)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=3), dict(dtype=-1), dict(tokens=-1), dict(tokens=(1 << 30) + 1), dict(channels=0),
+    dict(channels=(1 << 20) + 1), dict(table_rows=0), dict(table_rows=(1 << 30) + 1), dict(scale=float("inf")),
+    dict(scale=float("nan")), dict(y_stride=-1), dict(y_stride=1 << 50)])
+def test_looked_up_rows_refuses(kw):
+    refused(look_up, edesc(**kw))
+    refused(look_up_back, edesc(**kw))
+    if not any(k.endswith("stride") for k in kw):
+        refused(api.embed_rows_backward_workspace, edesc(**kw))
+
+
+def test_looked_up_rows_refuses_tensors_and_overlaps():
+    d = edesc()
+    for kw in (dict(ids=0), dict(table=0), dict(y=0), dict(ids=IDS + 1), dict(table=TABLE + 1), dict(x=X + 1),
+               dict(y=Y + 1), dict(y=TABLE), dict(y=IDS), dict(y=X + 768), dict(y=TABLE + 361 * 768)):
+        refused(look_up, d, **kw)
+    refused(look_up, None)
+    for kw in (dict(table_stride=-1), dict(x_stride=-1), dict(y_stride=383), dict(y_stride=0)):
+        refused(look_up, edesc(**kw))
+    refused(look_up, edesc(x_stride=400), y=X)
+    look_up(edesc(tokens=0), 0, 0, 0, 0)
+    for kw in (dict(ids=0), dict(dy=0), dict(dt=0), dict(ids=IDS + 2), dict(dy=DY + 1), dict(dt=DT + 2), dict(ws=0),
+               dict(ws=WS + 8), dict(dt=DY), dict(dt=IDS), dict(ws=DT), dict(ws=DY), dict(ws=IDS),
+               dict(size=api.embed_rows_backward_workspace(d) - 1)):
+        refused(look_up_back, d, **kw)
+    assert api.embed_rows_backward_workspace(edesc(tokens=0)) == 0
+    assert api.lib().kc_embed_rows_backward_workspace(d, None) == api.KC_ERR_INVALID
+
+
+LOG, TOP, WHOLE, LOSS, DL, DLOG = (A + (i << 33) for i in range(20, 26))
+
+
+def ddesc(**kw):
+    a = dict(dtype=api.PRECISION_F16, rows=256, classes=362, top=32, temperature=1.0)
+    strides = {k: kw.pop(k) for k in list(kw) if k.endswith("stride")}
+    a.update(kw)
+    return api.DistillDesc(*a.values(), **strides)
+
+
+def distill(d, z=LOG, ids=IDS, top=TOP, whole=WHOLE, loss=LOSS, st=ST):
+    api.distill_top(d, z, ids, top, whole, loss, st, 0)
+
+
+def distill_back(d, z=LOG, ids=IDS, top=TOP, whole=WHOLE, st=ST, dl=DL, dz=DLOG):
+    api.distill_top_backward(d, z, ids, top, whole, st, dl, dz, 0)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=3), dict(rows=-1), dict(rows=(1 << 30) + 1), dict(classes=0), dict(classes=(1 << 30) + 1), dict(top=0),
+    dict(top=1025), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
+    dict(temperature=float("inf")), dict(temperature=1e-7), dict(logits_stride=-1), dict(logits_stride=1 << 50),
+    dict(top_stride=-1)])
+def test_top_logits_refuses(kw):
+    refused(distill, ddesc(**kw))
+    refused(distill_back, ddesc(**kw))
+
+
+def test_top_logits_refuses_tensors_and_overlaps():
+    d = ddesc()
+    for kw in (dict(z=0), dict(ids=0), dict(top=0), dict(loss=0), dict(z=LOG + 1), dict(ids=IDS + 2), dict(top=TOP + 1),
+               dict(whole=WHOLE + 2), dict(loss=LOSS + 1), dict(st=ST + 4), dict(loss=LOG), dict(loss=ST), dict(st=TOP),
+               dict(st=IDS), dict(loss=WHOLE)):
+        refused(distill, d, **kw)
+    refused(distill, None)
+    for kw in (dict(z=0), dict(ids=0), dict(top=0), dict(st=0), dict(dz=0), dict(dz=DLOG + 1), dict(st=ST + 4),
+               dict(dl=DL + 1), dict(dz=LOG + 724), dict(dz=IDS), dict(dz=TOP), dict(dz=ST), dict(dz=DL),
+               dict(dz=WHOLE)):
+        refused(distill_back, d, **kw)
+    refused(distill_back, None)
+    for kw in (dict(dlogits_stride=361), dict(dlogits_stride=-1), dict(dlogits_stride=0)):
+        refused(distill_back, ddesc(**kw))
+    refused(distill_back, ddesc(dlogits_stride=400), dz=LOG)
+    distill(ddesc(rows=0), 0, 0, 0, 0, 0, 0)
+    distill_back(ddesc(rows=0), 0, 0, 0, 0, 0, 0, 0)
