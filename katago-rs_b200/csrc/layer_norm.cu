@@ -89,28 +89,90 @@ __device__ __forceinline__ bool rows_left(int64_t r, int64_t rows) {
   return BLOCK ? r < rows : __any_sync(0xffffffffu, r < rows);
 }
 
-template <typename T, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : kThreads) layer_norm_kernel(const LayerParams p) {
+// A thread's vectors of the next rows, on their way into shared memory of its own (kDepth rows, the one at hand among
+// them). Rows that are off are not copied.
+template <typename T, int VEC, int NV, bool BLOCK, int TENSORS>
+struct Ring {
   using V = RowVec<T, VEC>;
+  using Raw = typename V::Raw;
+  static constexpr int DEPTH = BLOCK ? 2 : TENSORS == 2 ? 3 : 4;
+  static size_t bytes(int threads) { return (size_t)DEPTH * TENSORS * NV * threads * sizeof(Raw); }
+
+  Raw* mine;
+  int stage = 0;      // of the row at hand
+  int64_t next;       // the row to copy next
+  bool next_on;
+  uint32_t on = 0;    // a bit for each stage
+
+  __device__ __forceinline__ Raw* at(int s, int tensor, int i) const {
+    return mine + ((s * TENSORS + tensor) * NV + i) * blockDim.x;
+  }
+  __device__ __forceinline__ void look(const LayerParams& p) { next_on = next < p.rows && token_on(p, next); }
+  __device__ __forceinline__ void fetch(const LayerParams& p, const Group<BLOCK>& g, int nvec, int s) {
+    on = (on & ~(1u << s)) | (next_on ? 1u << s : 0u);
+    if (next_on) {
+      const T* x = static_cast<const T*>(p.x) + p.xm(next);
+      const T* dy = TENSORS == 2 ? static_cast<const T*>(p.dy) + p.ym(next) : nullptr;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int v = g.lane + i * g.lanes;
+        if (v >= nvec) continue;
+        copy_vec<T, VEC>(at(s, 0, i), x + v * VEC);
+        if (TENSORS == 2) copy_vec<T, VEC>(at(s, 1, i), dy + v * VEC);
+      }
+    }
+    copy_commit();
+    next += g.step;
+    look(p);
+  }
+  __device__ __forceinline__ void start(const LayerParams& p, const Group<BLOCK>& g, int nvec, void* smem) {
+    mine = static_cast<Raw*>(smem) + threadIdx.x;
+    next = g.first;
+    look(p);
+#pragma unroll
+    for (int s = 0; s < DEPTH - 1; s++) fetch(p, g, nvec, s);
+  }
+  // The row at hand is there afterwards, and one more is on its way.
+  __device__ __forceinline__ bool arrive(const LayerParams& p, const Group<BLOCK>& g, int nvec) {
+    fetch(p, g, nvec, stage == 0 ? DEPTH - 1 : stage - 1);
+    copy_wait<DEPTH - 1>();
+    return on >> stage & 1;
+  }
+  __device__ __forceinline__ void leave() { stage = stage == DEPTH - 1 ? 0 : stage + 1; }
+};
+
+template <typename T, int VEC, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : kThreads, BLOCK ? 1 : 2) layer_norm_kernel(const LayerParams p) {
+  using V = RowVec<T, VEC>;
+  constexpr bool KEEP = !BLOCK && NV * VEC <= 24;  // weight and bias stay in registers
   __shared__ float2 red[2][32];
+  extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
   const int nvec = p.C / VEC;
   const float inv = 1.0f / (float)p.C;
+  Ring<T, VEC, NV, BLOCK, 1> ring;
+  ring.start(p, g, nvec, smem);
+  float w[KEEP ? NV : 1][VEC], b[KEEP ? NV : 1][VEC];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) w[i][j] = 1.0f, b[i][j] = 0.0f;
+      const int v = g.lane + i * g.lanes;
+      if (v < nvec && p.weight) load_params<VEC>(p.weight + v * VEC, p.wide, w[i]);
+      if (v < nvec && p.bias) load_params<VEC>(p.bias + v * VEC, p.wide, b[i]);
+    }
+  }
   int turn = 0;  // a block's sums in a row take turns with `red`
-  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step) {
-    const bool here = r < p.rows, on = here && token_on(p, r);
+  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, ring.leave()) {
+    const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
     float v[NV][VEC];
     float2 s = make_float2(0.0f, 0.0f);
     if (on) {
-      const T* row = static_cast<const T*>(p.x) + p.xm(r);
-      typename V::Raw raw[NV];
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (g.lane + i * g.lanes < nvec) raw[i] = V::load(row + (g.lane + i * g.lanes) * VEC);
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         if (g.lane + i * g.lanes >= nvec) continue;
-        V::unpack(raw[i], v[i]);
+        V::unpack(*ring.at(ring.stage, 0, i), v[i]);
 #pragma unroll
         for (int j = 0; j < VEC; j++) s.x += v[i][j];
       }
@@ -145,63 +207,67 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : kThreads) layer_norm_kernel(con
 #pragma unroll
       for (int j = 0; j < VEC; j++) o[j] = 0.0f;
       if (on) {
-        float w[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; j++) o[j] = fmaf(v[i][j], rstd, shift);
-        if (p.weight) {
-          load_params<VEC>(p.weight + c, p.wide, w);
+        if constexpr (KEEP) {
 #pragma unroll
-          for (int j = 0; j < VEC; j++) o[j] *= w[j];
-        }
-        if (p.bias) {
-          load_params<VEC>(p.bias + c, p.wide, w);
+          for (int j = 0; j < VEC; j++) o[j] = fmaf(o[j], w[i][j], b[i][j]);
+        } else {
+          if (p.weight) {
+            load_params<VEC>(p.weight + c, p.wide, w[0]);
 #pragma unroll
-          for (int j = 0; j < VEC; j++) o[j] += w[j];
+            for (int j = 0; j < VEC; j++) o[j] *= w[0][j];
+          }
+          if (p.bias) {
+            load_params<VEC>(p.bias + c, p.wide, b[0]);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) o[j] += b[0][j];
+          }
         }
       }
       V::store(out + c, V::pack(o));
     }
   }
+  copy_wait<0>();
 }
 
 template <typename T, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel(const LayerParams p) {
   using V = RowVec<T, VEC>;
   __shared__ float2 red[2][32];
-  extern __shared__ float sums[];  // a warp's rows in lanes: [2][C]
+  extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
   const int nvec = p.C / VEC;
   const float inv = 1.0f / (float)p.C;
-  float aw[NV][VEC], ab[NV][VEC];
+  pdl_trigger();
+  Ring<T, VEC, NV, BLOCK, 2> ring;
+  ring.start(p, g, nvec, smem);
+  float aw[NV][VEC], ab[NV][VEC], w[NV][VEC];
 #pragma unroll
-  for (int i = 0; i < NV; i++)
+  for (int i = 0; i < NV; i++) {
 #pragma unroll
-    for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f;
+    for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f, w[i][j] = 1.0f;
+    const int v = g.lane + i * g.lanes;
+    if (v < nvec && p.weight) load_params<VEC>(p.weight + v * VEC, p.wide, w[i]);
+  }
   int turn = 0;
-  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1) {
-    const bool here = r < p.rows, on = here && token_on(p, r);
-    typename V::Raw xr[NV], dr[NV];
-    float2 s = make_float2(0.0f, 0.0f), st = s;
+  float2 st_next = g.first < p.rows ? p.stats[g.first] : make_float2(0.0f, 0.0f);
+  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1, ring.leave()) {
+    const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
+    const float2 st = st_next;
+    if (r + g.step < p.rows) st_next = p.stats[r + g.step];
+    float2 s = make_float2(0.0f, 0.0f);
     if (on) {
-      const T* x = static_cast<const T*>(p.x) + p.xm(r);
-      const T* dy = static_cast<const T*>(p.dy) + p.ym(r);
-      st = p.stats[r];
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = (g.lane + i * g.lanes) * VEC;
-        if (g.lane + i * g.lanes < nvec) xr[i] = V::load(x + c), dr[i] = V::load(dy + c);
-      }
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         if (g.lane + i * g.lanes >= nvec) continue;
-        float a[VEC], d[VEC], w[VEC];
-        V::unpack(xr[i], a);
-        V::unpack(dr[i], d);
-        if (p.weight) load_params<VEC>(p.weight + (g.lane + i * g.lanes) * VEC, p.wide, w);
+        float a[VEC], d[VEC];
+        V::unpack(*ring.at(ring.stage, 0, i), a);
+        V::unpack(*ring.at(ring.stage, 1, i), d);
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
           const float xh = (a[j] - st.x) * st.y;
-          const float gw = p.weight ? d[j] * w[j] : d[j];
+          const float gw = d[j] * w[i][j];
           s.x += gw;
           s.y = fmaf(gw, xh, s.y);
           aw[i][j] = fmaf(d[j], xh, aw[i][j]);
@@ -221,20 +287,19 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel
 #pragma unroll
       for (int j = 0; j < VEC; j++) o[j] = 0.0f;
       if (on) {
-        float a[VEC], d[VEC], w[VEC];
-        V::unpack(xr[i], a);
-        V::unpack(dr[i], d);
-        if (p.weight) load_params<VEC>(p.weight + c, p.wide, w);
+        float a[VEC], d[VEC];
+        V::unpack(*ring.at(ring.stage, 0, i), a);
+        V::unpack(*ring.at(ring.stage, 1, i), d);
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
           const float xh = (a[j] - st.x) * st.y;
-          const float gw = p.weight ? d[j] * w[j] : d[j];
-          o[j] = st.y * (gw - fmaf(xh, c2, c1));
+          o[j] = st.y * (d[j] * w[i][j] - fmaf(xh, c2, c1));
         }
       }
       V::store(out + c, V::pack(o));
     }
   }
+  copy_wait<0>();
   if (!p.part) return;
   float* part = p.part + (size_t)blockIdx.x * 2 * p.C;
   if (BLOCK) {
@@ -257,7 +322,9 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel
             aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
             ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
           }
+    float* sums = reinterpret_cast<float*>(smem);  // [2][C], where the rows were
     for (int w = 0; w < kThreads / 32; w++) {
+      __syncthreads();
       if (threadIdx.x / 32 == w && threadIdx.x % 32 < g.lanes) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -270,8 +337,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel
           }
         }
       }
-      __syncthreads();
     }
+    __syncthreads();
     for (int c = threadIdx.x; c < 2 * p.C; c += kThreads) part[c] = sums[c];
   }
 }
@@ -473,7 +540,7 @@ Shape shape_of(int64_t rows, int C, int vec, bool backward) {
   if (best >= 0) {
     s.threads = kThreads;
     const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
-    s.blocks = std::min<int64_t>(all, backward ? 2 * kSmCount : 1 << 20);
+    s.blocks = std::min<int64_t>(all, 2 * kSmCount);
     return s;
   }
   s.block = true;
@@ -481,7 +548,7 @@ Shape shape_of(int64_t rows, int C, int vec, bool backward) {
   const int64_t threads = ((nvec + s.nv - 1) / s.nv + 31) / 32 * 32;
   if (threads <= (backward ? 512 : 1024)) {
     s.threads = (int)threads;
-    s.blocks = std::min<int64_t>(rows, backward ? (int64_t)kSmCount * (512 / threads) : 1 << 20);
+    s.blocks = std::min<int64_t>(rows, (int64_t)kSmCount * std::max<int64_t>(1, 512 / threads));
     return s;
   }
   s.is_long = true;
@@ -501,11 +568,16 @@ int64_t part_blocks(const Shape& s, int64_t rows, int C) { return s.is_long ? lo
 template <typename T, int VEC, int NV, bool BLOCK>
 void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
   if (backward) {
-    if constexpr (BLOCK || NV * VEC <= 24)
-      layer_norm_back_kernel<T, VEC, NV, BLOCK>
-          <<<(unsigned)s.blocks, s.threads, BLOCK ? 0 : 2 * p.C * sizeof(float), st>>>(p);
+    if constexpr (BLOCK || NV * VEC <= 24) {
+      // the ring, and in its place the channels' sums
+      const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2>::bytes(s.threads), BLOCK ? 0 : 2 * p.C * sizeof(float));
+      allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK>>();
+      layer_norm_back_kernel<T, VEC, NV, BLOCK><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
+    }
   } else {
-    layer_norm_kernel<T, VEC, NV, BLOCK><<<(unsigned)s.blocks, s.threads, 0, st>>>(p);
+    allow_block_smem<layer_norm_kernel<T, VEC, NV, BLOCK>>();
+    layer_norm_kernel<T, VEC, NV, BLOCK>
+        <<<(unsigned)s.blocks, s.threads, Ring<T, VEC, NV, BLOCK, 1>::bytes(s.threads), st>>>(p);
   }
   KC_CUDA(cudaGetLastError());
 }

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -62,6 +63,22 @@ struct RowVec {
     return r;
   }
 };
+
+// Copies of vectors into shared memory by the thread that reads them there: no barrier, and loads in flight that take no
+// registers. copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_vec(typename RowVec<T, VEC>::Raw* dst, const T* src) {
+  constexpr int BYTES = RowVec<T, VEC>::BYTES;
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else if constexpr (BYTES >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+  else
+    *dst = *reinterpret_cast<const uint16_t*>(src);
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // VEC float32 parameters; `wide`: the array is 16-byte aligned, and `p` as far into it as VEC allows.
 template <int VEC>
@@ -133,5 +150,19 @@ void launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, 
 }
 
 constexpr int kSmCount = 148;
+constexpr int kMaxBlockSmem = 227 * 1024;
+
+// Lets a kernel take more than 48 KB of shared memory, once per device.
+template <auto kernel>
+void allow_block_smem() {
+  static std::atomic<uint64_t> allowed[2];
+  int dev = 0;
+  KC_CUDA(cudaGetDevice(&dev));
+  if (dev >= 128) fail(KC_ERR_INVALID, "CUDA backend: device index above 127");
+  if (allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1) return;
+  KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlockSmem - 2048));
+  KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
+}
 
 }  // namespace kc
