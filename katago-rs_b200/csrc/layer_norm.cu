@@ -36,7 +36,7 @@ struct LayerParams {
   void* y;         // forward: y; backward: dx
   const void* dy;
   float2* stats;   // (mean, rstd) of a token: written by the forward pass (may be null), read by the backward
-  float* part;     // backward: [blocks][2][C] sums of dy xh and of dy
+  float* part;     // backward: the blocks' sums of dy xh and of dy, [blocks][2][slots] (PartShape)
   float* dweight;
   float* dbias;
   RowMap xm, ym, mm;
@@ -78,7 +78,8 @@ struct Group {
       step = (int64_t)gridDim.x * per;
     }
   }
-  __device__ __forceinline__ float2 sum(float2 v, float2* red) const {
+  template <typename F>
+  __device__ __forceinline__ F sum(F v, float2* red) const {
     return BLOCK ? block_sum(v, red) : lanes_sum(v, lanes);
   }
 };
@@ -144,96 +145,119 @@ struct Ring {
 template <typename T, int VEC, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : kThreads, BLOCK ? 1 : 2) layer_norm_kernel(const LayerParams p) {
   using V = RowVec<T, VEC>;
+  using Q = RowPairs<T, VEC>;
+  constexpr int N = Q::N;
   constexpr bool KEEP = !BLOCK && NV * VEC <= 24;  // weight and bias stay in registers
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
   const int nvec = p.C / VEC;
   const float inv = 1.0f / (float)p.C;
+  const bool layer = p.kind == KC_NORM_LAYER;
   Ring<T, VEC, NV, BLOCK, 1> ring;
   ring.start(p, g, nvec, smem);
-  float w[KEEP ? NV : 1][VEC], b[KEEP ? NV : 1][VEC];
+  f32x2 w[KEEP ? NV : 1][N], b[KEEP ? NV : 1][N];
   if constexpr (KEEP) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) w[i][j] = 1.0f, b[i][j] = 0.0f;
+      for (int j = 0; j < N; j++) w[i][j] = {1.0f, 1.0f}, b[i][j] = {0.0f, 0.0f};
       const int v = g.lane + i * g.lanes;
-      if (v < nvec && p.weight) load_params<VEC>(p.weight + v * VEC, p.wide, w[i]);
-      if (v < nvec && p.bias) load_params<VEC>(p.bias + v * VEC, p.wide, b[i]);
+      if (v < nvec && p.weight) load_param_pairs<VEC>(p.weight + v * VEC, p.wide, w[i]);
+      if (v < nvec && p.bias) load_param_pairs<VEC>(p.bias + v * VEC, p.wide, b[i]);
     }
   }
   int turn = 0;  // a block's sums in a row take turns with `red`
   for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, ring.leave()) {
     const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
-    float v[NV][VEC];
-    float2 s = make_float2(0.0f, 0.0f);
-    if (on) {
+    T* out = static_cast<T*>(p.y) + (here ? p.ym(r) : 0);
+    if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
+      if (!here) continue;
+      if (p.stats && g.lane == 0) p.stats[r] = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        if (g.lane + i * g.lanes >= nvec) continue;
-        V::unpack(*ring.at(ring.stage, 0, i), v[i]);
+      for (int i = 0; i < NV; i++)
+        if (g.lane + i * g.lanes < nvec) V::store(out + (g.lane + i * g.lanes) * VEC, Q::zero());
+      continue;
+    }
+    // a warp whose rows are on in part goes over all of them; what its other slots hold is dropped in the end
+    f32x2 v[NV][N], s1 = {0.0f, 0.0f}, s2 = {0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < VEC; j++) s.x += v[i][j];
-      }
+    for (int i = 0; i < NV; i++) {
+      if (g.lane + i * g.lanes >= nvec) continue;
+      Q::unpack(*ring.at(ring.stage, 0, i), v[i]);
+      if (layer)
+#pragma unroll
+        for (int j = 0; j < N; j++) s1 = add2(s1, v[i][j]);
     }
     float m0 = 0.0f;
-    if (p.kind == KC_NORM_LAYER) m0 = g.sum(s, red[turn ^= 1]).x * inv;
-    s = make_float2(0.0f, 0.0f);
-    if (on) {
+    if (layer) {
+      m0 = g.sum(s1.x + s1.y, red[turn ^= 1]) * inv;
+      s1 = {0.0f, 0.0f};
+      const f32x2 back = {-m0, VEC > 1 ? -m0 : 0.0f};
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         if (g.lane + i * g.lanes >= nvec) continue;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          v[i][j] -= m0;
-          s.x += v[i][j];
-          s.y = fmaf(v[i][j], v[i][j], s.y);
+        for (int j = 0; j < N; j++) {
+          v[i][j] = add2(v[i][j], back);
+          s1 = add2(s1, v[i][j]);
         }
       }
     }
-    s = g.sum(s, red[turn ^= 1]);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (g.lane + i * g.lanes >= nvec) continue;
+#pragma unroll
+      for (int j = 0; j < N; j++) s2 = fma2(v[i][j], v[i][j], s2);
+    }
+    float delta = 0.0f, squares;
+    if (layer) {
+      const float2 s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn ^= 1]);
+      delta = s.x * inv;
+      squares = s.y;
+    } else {
+      squares = g.sum(s2.x + s2.y, red[turn ^= 1]);
+    }
     if (!here) continue;
-    const float delta = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f;
-    const float rstd = rstd_of(s.y, inv, delta, p.eps);
+    const float rstd = rstd_of(squares, inv, delta, p.eps);
     if (p.stats && g.lane == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
-    T* out = static_cast<T*>(p.y) + p.ym(r);
-    const float shift = -delta * rstd;
+    const f32x2 scale = {rstd, rstd}, shift = {-delta * rstd, -delta * rstd};
+    const uint32_t keep = on ? 0xffffffffu : 0u;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int c = (g.lane + i * g.lanes) * VEC;
       if (g.lane + i * g.lanes >= nvec) continue;
-      float o[VEC];
+      f32x2 o[N];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) o[j] = 0.0f;
-      if (on) {
+      for (int j = 0; j < N; j++) o[j] = fma2(v[i][j], scale, shift);
+      if constexpr (KEEP) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) o[j] = fmaf(v[i][j], rstd, shift);
-        if constexpr (KEEP) {
+        for (int j = 0; j < N; j++) o[j] = fma2(o[j], w[i][j], b[i][j]);
+      } else {
+        if (p.weight) {
+          load_param_pairs<VEC>(p.weight + c, p.wide, w[0]);
 #pragma unroll
-          for (int j = 0; j < VEC; j++) o[j] = fmaf(o[j], w[i][j], b[i][j]);
-        } else {
-          if (p.weight) {
-            load_params<VEC>(p.weight + c, p.wide, w[0]);
+          for (int j = 0; j < N; j++) o[j] = mul2(o[j], w[0][j]);
+        }
+        if (p.bias) {
+          load_param_pairs<VEC>(p.bias + c, p.wide, b[0]);
 #pragma unroll
-            for (int j = 0; j < VEC; j++) o[j] *= w[0][j];
-          }
-          if (p.bias) {
-            load_params<VEC>(p.bias + c, p.wide, b[0]);
-#pragma unroll
-            for (int j = 0; j < VEC; j++) o[j] += b[0][j];
-          }
+          for (int j = 0; j < N; j++) o[j] = add2(o[j], b[0][j]);
         }
       }
-      V::store(out + c, V::pack(o));
+      V::store(out + c, Q::mask(Q::pack(o), keep));
     }
   }
   copy_wait<0>();
 }
 
-template <typename T, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel(const LayerParams p) {
+// LEAN: RMS norm without a bias, which needs no sum of g and none of dy.
+template <typename T, int VEC, int NV, bool BLOCK, bool LEAN>
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : 2) layer_norm_back_kernel(const LayerParams p) {
   using V = RowVec<T, VEC>;
+  using Q = RowPairs<T, VEC>;
+  constexpr int N = Q::N;
+  constexpr bool AGAIN = !LEAN && NV * VEC > 16;  // g is made twice where registers do not hold it
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
@@ -242,13 +266,13 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel
   pdl_trigger();
   Ring<T, VEC, NV, BLOCK, 2> ring;
   ring.start(p, g, nvec, smem);
-  float aw[NV][VEC], ab[NV][VEC], w[NV][VEC];
+  f32x2 aw[NV][N], ab[LEAN ? 1 : NV][N], w[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; i++) {
 #pragma unroll
-    for (int j = 0; j < VEC; j++) aw[i][j] = ab[i][j] = 0.0f, w[i][j] = 1.0f;
+    for (int j = 0; j < N; j++) aw[i][j] = ab[LEAN ? 0 : i][j] = {0.0f, 0.0f}, w[i][j] = {1.0f, 1.0f};
     const int v = g.lane + i * g.lanes;
-    if (v < nvec && p.weight) load_params<VEC>(p.weight + v * VEC, p.wide, w[i]);
+    if (v < nvec && p.weight) load_param_pairs<VEC>(p.weight + v * VEC, p.wide, w[i]);
   }
   int turn = 0;
   float2 st_next = g.first < p.rows ? p.stats[g.first] : make_float2(0.0f, 0.0f);
@@ -256,90 +280,101 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) layer_norm_back_kernel
     const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
     const float2 st = st_next;
     if (r + g.step < p.rows) st_next = p.stats[r + g.step];
-    float2 s = make_float2(0.0f, 0.0f);
+    T* out = static_cast<T*>(p.y) + (here ? p.xm(r) : 0);
+    if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
+      if (!here) continue;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (g.lane + i * g.lanes < nvec) V::store(out + (g.lane + i * g.lanes) * VEC, Q::zero());
+      continue;
+    }
+    // xh and g of the row, for its sums and then for dx
+    f32x2 xh[NV][N], gw[AGAIN ? 1 : NV][N], s1 = {0.0f, 0.0f}, s2 = {0.0f, 0.0f};
+    const f32x2 back = {-st.x, VEC > 1 ? -st.x : 0.0f}, scale = {st.y, st.y};
     if (on) {
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         if (g.lane + i * g.lanes >= nvec) continue;
-        float a[VEC], d[VEC];
-        V::unpack(*ring.at(ring.stage, 0, i), a);
-        V::unpack(*ring.at(ring.stage, 1, i), d);
+        f32x2 d[N];
+        Q::unpack(*ring.at(ring.stage, 0, i), xh[i]);
+        Q::unpack(*ring.at(ring.stage, 1, i), d);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          const float xh = (a[j] - st.x) * st.y;
-          const float gw = d[j] * w[i][j];
-          s.x += gw;
-          s.y = fmaf(gw, xh, s.y);
-          aw[i][j] = fmaf(d[j], xh, aw[i][j]);
-          ab[i][j] += d[j];
+        for (int j = 0; j < N; j++) {
+          xh[i][j] = mul2(add2(xh[i][j], back), scale);
+          const f32x2 gj = mul2(d[j], w[i][j]);
+          aw[i][j] = fma2(d[j], xh[i][j], aw[i][j]);
+          s2 = fma2(gj, xh[i][j], s2);
+          if constexpr (!LEAN) {
+            ab[i][j] = add2(ab[i][j], d[j]);
+            s1 = add2(s1, gj);
+          }
+          if constexpr (!AGAIN) gw[i][j] = gj;
         }
       }
     }
-    s = g.sum(s, red[turn]);
+    float2 s;
+    if constexpr (LEAN) s = make_float2(0.0f, g.sum(s2.x + s2.y, red[turn]));
+    else s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn]);
     if (!here) continue;
-    const float c1 = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f, c2 = s.y * inv;
-    T* out = static_cast<T*>(p.y) + p.xm(r);
+    // rstd (g - c1 - xh c2)
+    const float k1 = p.kind == KC_NORM_LAYER ? -s.x * inv * st.y : 0.0f, k2 = -s.y * inv * st.y;
+    const f32x2 c1 = {k1, k1}, c2 = {k2, k2};
+    const uint32_t keep = on ? 0xffffffffu : 0u;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (g.lane + i * g.lanes) * VEC;
       if (g.lane + i * g.lanes >= nvec) continue;
-      float o[VEC];
+      f32x2 o[N];
+      if constexpr (AGAIN) {
+        Q::unpack(*ring.at(ring.stage, 1, i), o);
 #pragma unroll
-      for (int j = 0; j < VEC; j++) o[j] = 0.0f;
-      if (on) {
-        float a[VEC], d[VEC];
-        V::unpack(*ring.at(ring.stage, 0, i), a);
-        V::unpack(*ring.at(ring.stage, 1, i), d);
+        for (int j = 0; j < N; j++) o[j] = fma2(mul2(o[j], w[i][j]), scale, fma2(xh[i][j], c2, c1));
+      } else {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          const float xh = (a[j] - st.x) * st.y;
-          o[j] = st.y * (d[j] * w[i][j] - fmaf(xh, c2, c1));
-        }
+        for (int j = 0; j < N; j++) o[j] = fma2(gw[i][j], scale, fma2(xh[i][j], c2, c1));
       }
-      V::store(out + c, V::pack(o));
+      V::store(out + (g.lane + i * g.lanes) * VEC, Q::mask(Q::pack(o), keep));
     }
   }
   copy_wait<0>();
   if (!p.part) return;
-  float* part = p.part + (size_t)blockIdx.x * 2 * p.C;
+  // slot (which, i, j, lane) holds the sum of channel (lane + i lanes) VEC + j
+  constexpr int E = NV * VEC;
+  const int slots = E * g.lanes;
+  float* part = p.part + (size_t)blockIdx.x * 2 * slots;
   if (BLOCK) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (g.lane + i * g.lanes) * VEC;
-      if (g.lane + i * g.lanes >= nvec) continue;
-#pragma unroll
-      for (int j = 0; j < VEC; j++) part[c + j] = aw[i][j], part[p.C + c + j] = ab[i][j];
+    for (int e = 0; e < E; e++) {
+      const f32x2 a = aw[e / VEC][e % VEC / 2], b = ab[LEAN ? 0 : e / VEC][e % VEC / 2];
+      part[e * g.lanes + g.lane] = e % VEC % 2 ? a.y : a.x;
+      part[slots + e * g.lanes + g.lane] = e % VEC % 2 ? b.y : b.x;
     }
-  } else {
-    // a warp's groups in registers, then warp after warp in shared memory
+    return;
+  }
+  // a warp's groups in registers, then the warps' sums in shared memory, where the rows were
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(smem);
+  const int warp = threadIdx.x / 32;
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+  for (int e = 0; e < E; e++) {
+    const f32x2 fa = aw[e / VEC][e % VEC / 2], fb = ab[LEAN ? 0 : e / VEC][e % VEC / 2];
+    float a = e % VEC % 2 ? fa.y : fa.x, b = e % VEC % 2 ? fb.y : fb.x;
 #pragma unroll
-      for (int j = 0; j < VEC; j++)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-          if (o >= g.lanes) {
-            aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
-            ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
-          }
-    float* sums = reinterpret_cast<float*>(smem);  // [2][C], where the rows were
-    for (int w = 0; w < kThreads / 32; w++) {
-      __syncthreads();
-      if (threadIdx.x / 32 == w && threadIdx.x % 32 < g.lanes) {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-          const int c = (g.lane + i * g.lanes) * VEC;
-          if (g.lane + i * g.lanes >= nvec) continue;
-#pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            sums[c + j] = w ? sums[c + j] + aw[i][j] : aw[i][j];
-            sums[p.C + c + j] = w ? sums[p.C + c + j] + ab[i][j] : ab[i][j];
-          }
-        }
+    for (int o = 16; o > 0; o >>= 1)
+      if (o >= g.lanes) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (!LEAN) b += __shfl_xor_sync(0xffffffffu, b, o);
       }
+    if (threadIdx.x % 32 < g.lanes) {
+      sums[(warp * 2 * E + e) * g.lanes + g.lane] = a;
+      if (!LEAN) sums[((warp * 2 + 1) * E + e) * g.lanes + g.lane] = b;
     }
-    __syncthreads();
-    for (int c = threadIdx.x; c < 2 * p.C; c += kThreads) part[c] = sums[c];
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < (LEAN ? 1 : 2) * slots; k += kThreads) {
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kThreads / 32; v++) s += sums[v * 2 * slots + k];
+    part[k] = s;
   }
 }
 
@@ -473,32 +508,35 @@ __global__ void __launch_bounds__(kThreads) layer_norm_long_sums_kernel(const La
   }
 }
 
-// dweight and dbias from the blocks' sums, in the blocks' order. 32 channels to a block, 32 threads share the blocks.
-__global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* part, int blocks, int C, float* dweight,
+// dweight and dbias from the blocks' sums, in the blocks' order. 32 slots to a block, 32 threads share the blocks.
+struct PartShape {
+  int blocks, slots;     // slots: of a block's sums of dy xh, those of dy behind them
+  int C, nv, vec, lanes; // slot (i, j, lane) is channel (lane + i lanes) vec + j
+};
+
+__global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* part, const PartShape s, float* dweight,
                                                                  float* dbias) {
-  pdl_wait();
   __shared__ float red[32][33];
+  pdl_wait();
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  const int64_t cols = 2 * (int64_t)C;
-  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
-    const int64_t c = c0 + tx;
-    float s = 0.0f;
-    if (c < cols)
+  const int64_t first = dweight ? 0 : s.slots, end = dbias ? 2 * (int64_t)s.slots : s.slots;
+  for (int64_t k0 = first + (int64_t)blockIdx.x * 32; k0 < end; k0 += (int64_t)gridDim.x * 32) {
+    const int64_t k = k0 + tx;
+    float sum = 0.0f;
+    if (k < end)
 #pragma unroll 8
-      for (int b = ty; b < blocks; b += 32) s += part[(size_t)b * cols + c];
-    red[ty][tx] = s;
+      for (int b = ty; b < s.blocks; b += 32) sum += part[(size_t)b * 2 * s.slots + k];
+    red[ty][tx] = sum;
     __syncthreads();
-    // thread (tx, ty) adds lane tx's sum of channel ty
+    // thread (tx, ty) adds lane tx's sum of slot ty
     float v = red[tx][ty];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int64_t at = c0 + ty;
-    if (tx == 0 && at < cols) {
-      if (at < C) {
-        if (dweight) dweight[at] = v;
-      } else if (dbias) {
-        dbias[at - C] = v;
-      }
+    const int64_t at = k0 + ty;
+    if (tx == 0 && at < end) {
+      const int slot = (int)(at < s.slots ? at : at - s.slots), e = slot / s.lanes;
+      const int c = (slot % s.lanes + e / s.vec * s.lanes) * s.vec + e % s.vec;
+      if (c < s.C) (at < s.slots ? dweight : dbias)[c] = v;
     }
     __syncthreads();
   }
@@ -563,16 +601,28 @@ int64_t long_shares(int64_t rows, int C) {
   return std::max<int64_t>(1, std::min<int64_t>(most, rows / 8));
 }
 
-int64_t part_blocks(const Shape& s, int64_t rows, int C) { return s.is_long ? long_shares(rows, C) : s.blocks; }
+// The blocks' sums; long rows have a slot to a channel.
+PartShape part_shape(const Shape& s, int64_t rows, int C) {
+  if (s.is_long) return {(int)long_shares(rows, C), C, C, 1, 1, C};
+  const int lanes = s.block ? s.threads : s.lanes;
+  return {(int)s.blocks, s.nv * s.vec * lanes, C, s.nv, s.vec, lanes};
+}
+
+template <typename T, int VEC, int NV, bool BLOCK, bool LEAN>
+void launch_back(const LayerParams& p, const Shape& s, cudaStream_t st) {
+  // the ring, and in its place the warps' sums
+  const size_t sums = BLOCK ? 0 : (size_t)kThreads / 32 * 2 * NV * VEC * s.lanes * sizeof(float);
+  const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2>::bytes(s.threads), sums);
+  allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK, LEAN>>();
+  layer_norm_back_kernel<T, VEC, NV, BLOCK, LEAN><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
+}
 
 template <typename T, int VEC, int NV, bool BLOCK>
 void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
   if (backward) {
     if constexpr (BLOCK || NV * VEC <= 24) {
-      // the ring, and in its place the channels' sums
-      const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2>::bytes(s.threads), BLOCK ? 0 : 2 * p.C * sizeof(float));
-      allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK>>();
-      layer_norm_back_kernel<T, VEC, NV, BLOCK><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
+      if (p.kind == KC_NORM_RMS && !p.dbias) launch_back<T, VEC, NV, BLOCK, true>(p, s, st);
+      else launch_back<T, VEC, NV, BLOCK, false>(p, s, st);
     }
   } else {
     allow_block_smem<layer_norm_kernel<T, VEC, NV, BLOCK>>();
@@ -636,8 +686,10 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, s, backward, st);
   else run_type<__nv_bfloat16>(p, s, backward, st);
   if (!p.part) return;
-  launch_after(layer_norm_params_kernel, dim3((unsigned)std::min<int64_t>((2 * (int64_t)p.C + 31) / 32, 1 << 20)),
-               dim3(1024), 0, st, (const float*)p.part, (int)part_blocks(s, p.rows, p.C), p.C, p.dweight, p.dbias);
+  const PartShape q = part_shape(s, p.rows, p.C);
+  const int64_t slots = (int64_t)q.slots * ((p.dweight ? 1 : 0) + (p.dbias ? 1 : 0));
+  launch_after(layer_norm_params_kernel, dim3((unsigned)std::min<int64_t>((slots + 31) / 32, 1 << 20)), dim3(1024), 0, st,
+               (const float*)p.part, q, p.dweight, p.dbias);
 }
 
 Rows x_rows(const kc_layer_norm_desc& d, const void* p) {
@@ -679,10 +731,13 @@ int vec_of(const kc_layer_norm_desc& d, std::initializer_list<const void*> ptrs)
 size_t back_workspace(const kc_layer_norm_desc& d) {
   const int64_t rows = (int64_t)d.n * d.points;
   if (rows == 0) return 0;
-  int64_t blocks = 0;
-  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2)
-    if (d.channels % v == 0) blocks = std::max(blocks, part_blocks(shape_of(rows, d.channels, v, true), rows, d.channels));
-  return ((size_t)blocks * 2 * d.channels * sizeof(float) + 255) / 256 * 256;
+  size_t floats = 0;
+  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2) {
+    if (d.channels % v != 0) continue;
+    const PartShape q = part_shape(shape_of(rows, d.channels, v, true), rows, d.channels);
+    floats = std::max(floats, (size_t)q.blocks * 2 * q.slots);
+  }
+  return (floats * sizeof(float) + 255) / 256 * 256;
 }
 
 // Outputs share no memory with each other or with an input; only a tensor may be its own output.

@@ -64,6 +64,37 @@ struct RowVec {
   }
 };
 
+// A vector as pairs of floats, for the two-lane float32 arithmetic (one element: the second of the pair is 0).
+template <typename T, int VEC>
+struct RowPairs {
+  static constexpr int N = (VEC + 1) / 2;
+  using Raw = typename RowVec<T, VEC>::Raw;
+  __device__ static __forceinline__ void unpack(const Raw& r, f32x2 (&v)[N]) {
+    float f[VEC];
+    RowVec<T, VEC>::unpack(r, f);
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = {f[2 * j], VEC > 1 ? f[VEC > 1 ? 2 * j + 1 : 0] : 0.0f};
+  }
+  __device__ static __forceinline__ Raw pack(const f32x2 (&v)[N]) {
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) f[j] = j % 2 ? v[j / 2].y : v[j / 2].x;
+    return RowVec<T, VEC>::pack(f);
+  }
+  __device__ static __forceinline__ Raw zero() { return Raw{}; }
+  // `r` where keep is all ones, zeros where it is 0
+  __device__ static __forceinline__ Raw mask(Raw r, uint32_t keep) {
+    if constexpr (sizeof(Raw) == 2) {
+      return r & (uint16_t)keep;
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(Raw) / 4; i++) w[i] &= keep;
+      return r;
+    }
+  }
+};
+
 // Copies of vectors into shared memory by the thread that reads them there: no barrier, and loads in flight that take no
 // registers. copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived.
 template <typename T, int VEC>
@@ -95,6 +126,14 @@ __device__ __forceinline__ void load_params(const float* p, bool wide, float (&v
   }
 }
 
+template <int VEC>
+__device__ __forceinline__ void load_param_pairs(const float* p, bool wide, f32x2 (&v)[(VEC + 1) / 2]) {
+  float f[VEC];
+  load_params<VEC>(p, wide, f);
+#pragma unroll
+  for (int j = 0; j < (VEC + 1) / 2; j++) v[j] = {f[2 * j], VEC > 1 ? f[VEC > 1 ? 2 * j + 1 : 0] : 0.0f};
+}
+
 // Sums over groups of `lanes` neighbouring lanes of a warp (a power of two; every lane of the warp takes part).
 __device__ __forceinline__ float2 lanes_sum(float2 v, int lanes) {
 #pragma unroll
@@ -106,6 +145,13 @@ __device__ __forceinline__ float2 lanes_sum(float2 v, int lanes) {
   return v;
 }
 
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Sum over a block of whole warps. `red` holds a value per warp; two calls in a row take different ones.
 __device__ __forceinline__ float2 block_sum(float2 v, float2* red) {
   v = lanes_sum(v, 32);
@@ -113,6 +159,14 @@ __device__ __forceinline__ float2 block_sum(float2 v, float2* red) {
   __syncthreads();
   const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
   return lanes_sum(lane < warps ? red[lane] : make_float2(0.0f, 0.0f), 32);
+}
+
+__device__ __forceinline__ float block_sum(float v, float2* red) {
+  v = lanes_sum(v, 32);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32].x = v;
+  __syncthreads();
+  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
+  return lanes_sum(lane < warps ? red[lane].x : 0.0f, 32);
 }
 
 // Rows of `points` to a board. Boards whose rows go on at one stride are one long row of rows (points 0).
