@@ -47,9 +47,10 @@ struct LayerParams {
   float eps;
 };
 
-__device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) {
-  return !p.mask || __ldg(p.mask + p.mm(r)) != 0.0f;
+__device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
+  return p.mask ? __ldg(p.mask + p.mm(r)) : 1.0f;
 }
+__device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) { return token_mask(p, r) != 0.0f; }
 
 // 1 / sqrt(var + eps) of a sum of squares around a value that is `delta` from the mean; NaN where the squares passed
 // float32's range.
@@ -90,44 +91,69 @@ __device__ __forceinline__ bool rows_left(int64_t r, int64_t rows) {
   return BLOCK ? r < rows : __any_sync(0xffffffffu, r < rows);
 }
 
-// A thread's vectors of the next rows, on their way into shared memory of its own (kDepth rows, the one at hand among
-// them). Rows that are off are not copied.
+// A thread's NV vectors as pairs of elements, for the two-lane float32 arithmetic: a unit is a vector, or two vectors of
+// one element. Pair j of unit u has elements 2 j and 2 j + 1 of both vectors' elements.
+template <int VEC, int NV>
+struct Units {
+  static_assert(NV * VEC % 2 == 0, "whole pairs");
+  static constexpr int U = VEC == 1 ? NV / 2 : NV, N = VEC == 1 ? 1 : VEC / 2;
+  f32x2 v[U][N];
+
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int j = 0; j < N; j++) v[u][j] = {f, f};
+  }
+  __device__ __forceinline__ float element(int e) const {
+    const f32x2 q = v[e / (2 * N)][e / 2 % N];
+    return e % 2 ? q.y : q.x;
+  }
+};
+
+// A thread's vectors of the next rows, on their way into shared memory of its own (DEPTH rows, the one at hand among
+// them; no more than what 512 threads of an SM have room for). Rows that are off are not copied.
 template <typename T, int VEC, int NV, bool BLOCK, int TENSORS>
 struct Ring {
-  using V = RowVec<T, VEC>;
-  using Raw = typename V::Raw;
-  static constexpr int DEPTH = BLOCK ? 2 : TENSORS == 2 ? 3 : 4;
-  static size_t bytes(int threads) { return (size_t)DEPTH * TENSORS * NV * threads * sizeof(Raw); }
+  using Copy = RowCopy<T, VEC>;
+  using Slot = typename Copy::Slot;
+  static constexpr int ROW = TENSORS * NV * (int)sizeof(Slot);
+  static constexpr int DEPTH = TENSORS == 1 && ROW * 4 <= 420 ? 4 : ROW * 3 <= 420 ? 3 : 2;
+  static size_t bytes(int threads) { return (size_t)DEPTH * ROW * threads; }
 
-  Raw* mine;
+  Slot* mine;
   int stage = 0;      // of the row at hand
   int64_t next;       // the row to copy next
-  bool next_on;
+  float next_mask;    // looked at a row later, when it has arrived
   uint32_t on = 0;    // a bit for each stage
+  uint32_t high[TENSORS] = {};  // a bit for each stage: the row begins in the upper half of 4 bytes
 
-  __device__ __forceinline__ Raw* at(int s, int tensor, int i) const {
+  __device__ __forceinline__ Slot* at(int s, int tensor, int i) const {
     return mine + ((s * TENSORS + tensor) * NV + i) * blockDim.x;
   }
-  __device__ __forceinline__ void look(const LayerParams& p) { next_on = next < p.rows && token_on(p, next); }
+  __device__ __forceinline__ void look(const LayerParams& p) { next_mask = next < p.rows ? token_mask(p, next) : 0.0f; }
+  __device__ __forceinline__ void fetch_row(const T* row, int tensor, const Group<BLOCK>& g, int nvec, int s) {
+    if constexpr (Copy::BYTES == 2)
+      high[tensor] = (high[tensor] & ~(1u << s)) | ((uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1u) << s;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int v = g.lane + i * g.lanes;
+      if (v < nvec) Copy::copy(at(s, tensor, i), row + v * VEC);
+    }
+  }
   __device__ __forceinline__ void fetch(const LayerParams& p, const Group<BLOCK>& g, int nvec, int s) {
+    const bool next_on = next_mask != 0.0f;
     on = (on & ~(1u << s)) | (next_on ? 1u << s : 0u);
     if (next_on) {
-      const T* x = static_cast<const T*>(p.x) + p.xm(next);
-      const T* dy = TENSORS == 2 ? static_cast<const T*>(p.dy) + p.ym(next) : nullptr;
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int v = g.lane + i * g.lanes;
-        if (v >= nvec) continue;
-        copy_vec<T, VEC>(at(s, 0, i), x + v * VEC);
-        if (TENSORS == 2) copy_vec<T, VEC>(at(s, 1, i), dy + v * VEC);
-      }
+      fetch_row(static_cast<const T*>(p.x) + p.xm(next), 0, g, nvec, s);
+      if (TENSORS == 2) fetch_row(static_cast<const T*>(p.dy) + p.ym(next), TENSORS - 1, g, nvec, s);
     }
     copy_commit();
     next += g.step;
     look(p);
   }
   __device__ __forceinline__ void start(const LayerParams& p, const Group<BLOCK>& g, int nvec, void* smem) {
-    mine = static_cast<Raw*>(smem) + threadIdx.x;
+    mine = static_cast<Slot*>(smem) + threadIdx.x;
     next = g.first;
     look(p);
 #pragma unroll
@@ -139,83 +165,142 @@ struct Ring {
     copy_wait<DEPTH - 1>();
     return on >> stage & 1;
   }
+  // unit u of the row at hand
+  __device__ __forceinline__ void get(int tensor, int u, const Group<BLOCK>& g, int nvec, f32x2 (&v)[Units<VEC, NV>::N]) const {
+    float f[VEC];
+    if constexpr (VEC == 1) {
+      float e[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int i = 2 * u + k, c = g.lane + i * g.lanes;
+        f[0] = 0.0f;
+        if (c < nvec) Copy::unpack(*at(stage, tensor, i), (high[tensor] >> stage ^ (uint32_t)c) & 1u, f);
+        e[k] = f[0];
+      }
+      v[0] = {e[0], e[1]};
+    } else {
+      Copy::unpack(*at(stage, tensor, u), 0u, f);
+#pragma unroll
+      for (int j = 0; j < VEC / 2; j++) v[j] = {f[2 * j], f[2 * j + 1]};
+    }
+  }
   __device__ __forceinline__ void leave() { stage = stage == DEPTH - 1 ? 0 : stage + 1; }
 };
 
+// A thread's place in a row: which of its units there are.
+template <int VEC, int NV, bool BLOCK>
+struct Place {
+  using U = Units<VEC, NV>;
+  const Group<BLOCK>& g;
+  int nvec;
+  __device__ __forceinline__ bool has(int i) const { return g.lane + i * g.lanes < nvec; }  // vector i
+  __device__ __forceinline__ bool has_unit(int u) const { return has(VEC == 1 ? 2 * u : u); }
+  // `f` in the elements of unit u that there are
+  __device__ __forceinline__ f32x2 both(int u, float f) const {
+    return {f, VEC > 1 || has(2 * u + 1) ? f : 0.0f};
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int u, const f32x2 (&v)[U::N], uint32_t keep) const {
+    using V = RowVec<T, VEC>;
+    if constexpr (VEC == 1) {
+      const float a[1] = {v[0].x}, b[1] = {v[0].y};
+      V::store(row + g.lane + 2 * u * g.lanes, masked(V::pack(a), keep));
+      if (has(2 * u + 1)) V::store(row + g.lane + (2 * u + 1) * g.lanes, masked(V::pack(b), keep));
+    } else {
+      float f[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) f[j] = j % 2 ? v[j / 2].y : v[j / 2].x;
+      V::store(row + (g.lane + u * g.lanes) * VEC, masked(V::pack(f), keep));
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void zero(T* row) const {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if (has(i)) RowVec<T, VEC>::store(row + (g.lane + i * g.lanes) * VEC, typename RowVec<T, VEC>::Raw{});
+  }
+  __device__ __forceinline__ void load(U& w, const float* p, float otherwise, bool wide) const {
+    w.fill(otherwise);
+    if (!p) return;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (!has(i)) continue;
+      float f[VEC];
+      load_params<VEC>(p + (g.lane + i * g.lanes) * VEC, wide, f);
+      if constexpr (VEC == 1) {
+        if (i % 2) w.v[i / 2][0].y = f[0];
+        else w.v[i / 2][0].x = f[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; j++) w.v[i][j] = {f[2 * j], f[2 * j + 1]};
+      }
+    }
+  }
+};
+
+constexpr int kBlockThreads = 512;  // of blocks that share a row, at most: 128 registers each
+
 template <typename T, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : kThreads, BLOCK ? 1 : 2) layer_norm_kernel(const LayerParams p) {
-  using V = RowVec<T, VEC>;
-  using Q = RowPairs<T, VEC>;
-  constexpr int N = Q::N;
-  constexpr bool KEEP = !BLOCK && NV * VEC <= 24;  // weight and bias stay in registers
+__global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 2)
+    layer_norm_kernel(const LayerParams p) {
+  using U = Units<VEC, NV>;
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
-  const int nvec = p.C / VEC;
+  const Place<VEC, NV, BLOCK> at{g, p.C / VEC};
   const float inv = 1.0f / (float)p.C;
   const bool layer = p.kind == KC_NORM_LAYER;
   Ring<T, VEC, NV, BLOCK, 1> ring;
-  ring.start(p, g, nvec, smem);
-  f32x2 w[KEEP ? NV : 1][N], b[KEEP ? NV : 1][N];
-  if constexpr (KEEP) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-#pragma unroll
-      for (int j = 0; j < N; j++) w[i][j] = {1.0f, 1.0f}, b[i][j] = {0.0f, 0.0f};
-      const int v = g.lane + i * g.lanes;
-      if (v < nvec && p.weight) load_param_pairs<VEC>(p.weight + v * VEC, p.wide, w[i]);
-      if (v < nvec && p.bias) load_param_pairs<VEC>(p.bias + v * VEC, p.wide, b[i]);
-    }
-  }
+  ring.start(p, g, at.nvec, smem);
+  U w, b;
+  at.load(w, p.weight, 1.0f, p.wide);
+  at.load(b, p.bias, 0.0f, p.wide);
   int turn = 0;  // a block's sums in a row take turns with `red`
   for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, ring.leave()) {
-    const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
+    const bool here = r < p.rows, on = ring.arrive(p, g, at.nvec);
     T* out = static_cast<T*>(p.y) + (here ? p.ym(r) : 0);
     if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
       if (!here) continue;
       if (p.stats && g.lane == 0) p.stats[r] = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (g.lane + i * g.lanes < nvec) V::store(out + (g.lane + i * g.lanes) * VEC, Q::zero());
+      at.zero(out);
       continue;
     }
     // a warp whose rows are on in part goes over all of them; what its other slots hold is dropped in the end
-    f32x2 v[NV][N], s1 = {0.0f, 0.0f}, s2 = {0.0f, 0.0f};
+    U x;
+    f32x2 s1 = {0.0f, 0.0f}, s2 = s1;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      if (g.lane + i * g.lanes >= nvec) continue;
-      Q::unpack(*ring.at(ring.stage, 0, i), v[i]);
+    for (int u = 0; u < U::U; u++) {
+      if (!at.has_unit(u)) continue;
+      ring.get(0, u, g, at.nvec, x.v[u]);
       if (layer)
 #pragma unroll
-        for (int j = 0; j < N; j++) s1 = add2(s1, v[i][j]);
+        for (int j = 0; j < U::N; j++) s1 = add2(s1, x.v[u][j]);
     }
-    float m0 = 0.0f;
+    float m0 = 0.0f, delta = 0.0f, squares;
     if (layer) {
       m0 = g.sum(s1.x + s1.y, red[turn ^= 1]) * inv;
       s1 = {0.0f, 0.0f};
-      const f32x2 back = {-m0, VEC > 1 ? -m0 : 0.0f};
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        if (g.lane + i * g.lanes >= nvec) continue;
+      for (int u = 0; u < U::U; u++) {
+        if (!at.has_unit(u)) continue;
+        const f32x2 back = at.both(u, -m0);
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-          v[i][j] = add2(v[i][j], back);
-          s1 = add2(s1, v[i][j]);
+        for (int j = 0; j < U::N; j++) {
+          x.v[u][j] = add2(x.v[u][j], back);
+          s1 = add2(s1, x.v[u][j]);
+          s2 = fma2(x.v[u][j], x.v[u][j], s2);
         }
       }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      if (g.lane + i * g.lanes >= nvec) continue;
-#pragma unroll
-      for (int j = 0; j < N; j++) s2 = fma2(v[i][j], v[i][j], s2);
-    }
-    float delta = 0.0f, squares;
-    if (layer) {
       const float2 s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn ^= 1]);
       delta = s.x * inv;
       squares = s.y;
     } else {
+#pragma unroll
+      for (int u = 0; u < U::U; u++) {
+        if (!at.has_unit(u)) continue;
+#pragma unroll
+        for (int j = 0; j < U::N; j++) s2 = fma2(x.v[u][j], x.v[u][j], s2);
+      }
       squares = g.sum(s2.x + s2.y, red[turn ^= 1]);
     }
     if (!here) continue;
@@ -224,28 +309,11 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : kThreads, BLOCK ? 1 : 2) layer_
     const f32x2 scale = {rstd, rstd}, shift = {-delta * rstd, -delta * rstd};
     const uint32_t keep = on ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (g.lane + i * g.lanes) * VEC;
-      if (g.lane + i * g.lanes >= nvec) continue;
-      f32x2 o[N];
+    for (int u = 0; u < U::U; u++) {
+      if (!at.has_unit(u)) continue;
 #pragma unroll
-      for (int j = 0; j < N; j++) o[j] = fma2(v[i][j], scale, shift);
-      if constexpr (KEEP) {
-#pragma unroll
-        for (int j = 0; j < N; j++) o[j] = fma2(o[j], w[i][j], b[i][j]);
-      } else {
-        if (p.weight) {
-          load_param_pairs<VEC>(p.weight + c, p.wide, w[0]);
-#pragma unroll
-          for (int j = 0; j < N; j++) o[j] = mul2(o[j], w[0][j]);
-        }
-        if (p.bias) {
-          load_param_pairs<VEC>(p.bias + c, p.wide, b[0]);
-#pragma unroll
-          for (int j = 0; j < N; j++) o[j] = add2(o[j], b[0][j]);
-        }
-      }
-      V::store(out + c, Q::mask(Q::pack(o), keep));
+      for (int j = 0; j < U::N; j++) x.v[u][j] = fma2(fma2(x.v[u][j], scale, shift), w.v[u][j], b.v[u][j]);
+      at.store(out, u, x.v[u], keep);
     }
   }
   copy_wait<0>();
@@ -253,62 +321,55 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : kThreads, BLOCK ? 1 : 2) layer_
 
 // LEAN: RMS norm without a bias, which needs no sum of g and none of dy.
 template <typename T, int VEC, int NV, bool BLOCK, bool LEAN>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : 2) layer_norm_back_kernel(const LayerParams p) {
-  using V = RowVec<T, VEC>;
-  using Q = RowPairs<T, VEC>;
-  constexpr int N = Q::N;
-  constexpr bool AGAIN = !LEAN && NV * VEC > 16;  // g is made twice where registers do not hold it
+__global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 2)
+    layer_norm_back_kernel(const LayerParams p) {
+  using U = Units<VEC, NV>;
+  constexpr bool AGAIN = !LEAN && (BLOCK || NV * VEC > 16);  // xh and g are made twice where registers do not hold them
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
-  const int nvec = p.C / VEC;
+  const Place<VEC, NV, BLOCK> at{g, p.C / VEC};
   const float inv = 1.0f / (float)p.C;
   pdl_trigger();
   Ring<T, VEC, NV, BLOCK, 2> ring;
-  ring.start(p, g, nvec, smem);
-  f32x2 aw[NV][N], ab[LEAN ? 1 : NV][N], w[NV][N];
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-#pragma unroll
-    for (int j = 0; j < N; j++) aw[i][j] = ab[LEAN ? 0 : i][j] = {0.0f, 0.0f}, w[i][j] = {1.0f, 1.0f};
-    const int v = g.lane + i * g.lanes;
-    if (v < nvec && p.weight) load_param_pairs<VEC>(p.weight + v * VEC, p.wide, w[i]);
-  }
+  ring.start(p, g, at.nvec, smem);
+  U aw, ab, w;
+  aw.fill(0.0f);
+  ab.fill(0.0f);
+  at.load(w, p.weight, 1.0f, p.wide);
   int turn = 0;
   float2 st_next = g.first < p.rows ? p.stats[g.first] : make_float2(0.0f, 0.0f);
   for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1, ring.leave()) {
-    const bool here = r < p.rows, on = ring.arrive(p, g, nvec);
+    const bool here = r < p.rows, on = ring.arrive(p, g, at.nvec);
     const float2 st = st_next;
     if (r + g.step < p.rows) st_next = p.stats[r + g.step];
     T* out = static_cast<T*>(p.y) + (here ? p.xm(r) : 0);
     if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
-      if (!here) continue;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (g.lane + i * g.lanes < nvec) V::store(out + (g.lane + i * g.lanes) * VEC, Q::zero());
+      if (here) at.zero(out);
       continue;
     }
-    // xh and g of the row, for its sums and then for dx
-    f32x2 xh[NV][N], gw[AGAIN ? 1 : NV][N], s1 = {0.0f, 0.0f}, s2 = {0.0f, 0.0f};
-    const f32x2 back = {-st.x, VEC > 1 ? -st.x : 0.0f}, scale = {st.y, st.y};
+    // xh and g of the row, for its sums and then for dx (where dy has no element it is 0, and xh plays no part)
+    U xh, gw;
+    f32x2 s1 = {0.0f, 0.0f}, s2 = s1;
+    const f32x2 back = {-st.x, -st.x}, scale = {st.y, st.y};
     if (on) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        if (g.lane + i * g.lanes >= nvec) continue;
-        f32x2 d[N];
-        Q::unpack(*ring.at(ring.stage, 0, i), xh[i]);
-        Q::unpack(*ring.at(ring.stage, 1, i), d);
+      for (int u = 0; u < U::U; u++) {
+        if (!at.has_unit(u)) continue;
+        ring.get(0, u, g, at.nvec, xh.v[u]);
+        f32x2 d[U::N];
+        ring.get(1, u, g, at.nvec, d);
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-          xh[i][j] = mul2(add2(xh[i][j], back), scale);
-          const f32x2 gj = mul2(d[j], w[i][j]);
-          aw[i][j] = fma2(d[j], xh[i][j], aw[i][j]);
-          s2 = fma2(gj, xh[i][j], s2);
+        for (int j = 0; j < U::N; j++) {
+          xh.v[u][j] = mul2(add2(xh.v[u][j], back), scale);
+          const f32x2 gj = mul2(d[j], w.v[u][j]);
+          aw.v[u][j] = fma2(d[j], xh.v[u][j], aw.v[u][j]);
+          s2 = fma2(gj, xh.v[u][j], s2);
           if constexpr (!LEAN) {
-            ab[i][j] = add2(ab[i][j], d[j]);
+            ab.v[u][j] = add2(ab.v[u][j], d[j]);
             s1 = add2(s1, gj);
           }
-          if constexpr (!AGAIN) gw[i][j] = gj;
+          if constexpr (!AGAIN) gw.v[u][j] = gj;
         }
       }
     }
@@ -320,33 +381,35 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : 2) layer_n
     const float k1 = p.kind == KC_NORM_LAYER ? -s.x * inv * st.y : 0.0f, k2 = -s.y * inv * st.y;
     const f32x2 c1 = {k1, k1}, c2 = {k2, k2};
     const uint32_t keep = on ? 0xffffffffu : 0u;
+    if constexpr (AGAIN) asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      if (g.lane + i * g.lanes >= nvec) continue;
-      f32x2 o[N];
+    for (int u = 0; u < U::U; u++) {
+      if (!at.has_unit(u)) continue;
+      f32x2 o[U::N];
       if constexpr (AGAIN) {
-        Q::unpack(*ring.at(ring.stage, 1, i), o);
-#pragma unroll
-        for (int j = 0; j < N; j++) o[j] = fma2(mul2(o[j], w[i][j]), scale, fma2(xh[i][j], c2, c1));
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; j++) o[j] = fma2(gw[i][j], scale, fma2(xh[i][j], c2, c1));
+        ring.get(1, u, g, at.nvec, o);
+        ring.get(0, u, g, at.nvec, xh.v[u]);
       }
-      V::store(out + (g.lane + i * g.lanes) * VEC, Q::mask(Q::pack(o), keep));
+#pragma unroll
+      for (int j = 0; j < U::N; j++) {
+        if (AGAIN) xh.v[u][j] = mul2(add2(xh.v[u][j], back), scale);
+        const f32x2 gj = AGAIN ? mul2(o[j], w.v[u][j]) : gw.v[u][j];
+        o[j] = fma2(gj, scale, fma2(xh.v[u][j], c2, c1));
+      }
+      at.store(out, u, o, keep);
     }
   }
   copy_wait<0>();
   if (!p.part) return;
-  // slot (which, i, j, lane) holds the sum of channel (lane + i lanes) VEC + j
+  // slot (which, i, j, lane) holds the sum of channel (lane + i lanes) VEC + j (element i VEC + j)
   constexpr int E = NV * VEC;
   const int slots = E * g.lanes;
   float* part = p.part + (size_t)blockIdx.x * 2 * slots;
   if (BLOCK) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const f32x2 a = aw[e / VEC][e % VEC / 2], b = ab[LEAN ? 0 : e / VEC][e % VEC / 2];
-      part[e * g.lanes + g.lane] = e % VEC % 2 ? a.y : a.x;
-      part[slots + e * g.lanes + g.lane] = e % VEC % 2 ? b.y : b.x;
+      part[e * g.lanes + g.lane] = aw.element(e);
+      if (!LEAN) part[slots + e * g.lanes + g.lane] = ab.element(e);
     }
     return;
   }
@@ -356,8 +419,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : 2) layer_n
   const int warp = threadIdx.x / 32;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const f32x2 fa = aw[e / VEC][e % VEC / 2], fb = ab[LEAN ? 0 : e / VEC][e % VEC / 2];
-    float a = e % VEC % 2 ? fa.y : fa.x, b = e % VEC % 2 ? fb.y : fb.x;
+    float a = aw.element(e), b = ab.element(e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       if (o >= g.lanes) {
@@ -553,12 +615,14 @@ struct Shape {
   int64_t blocks;
 };
 
-constexpr int kNvs[] = {1, 2, 3, 4, 6, 8};
-
-// Registers of a warp's lane: 32 elements forward, 24 backward (with both tensors and both sums).
-bool nv_built(int vec, int nv, bool backward) {
-  if (vec <= 2) return nv == 2 || nv == 8;
-  return vec * nv <= (backward ? 24 : 32);
+// Vectors of a warp's lane, for each width of vector: up to 24 elements (weight, bias and the row in registers, or
+// weight, row, gradient and the channels' sums). A block's thread has 16 or, forward, 32 elements.
+constexpr int kNvs[] = {1, 2, 3, 4, 6, 8, 12, 16, 24};
+constexpr bool warp_nv(int vec, int nv) {
+  if (vec == 8) return nv <= 3;
+  if (vec == 4) return nv == 1 || nv == 2 || nv == 3 || nv == 4 || nv == 6;
+  if (vec == 2) return nv == 1 || nv == 4 || nv == 8 || nv == 12;
+  return nv == 2 || nv == 8 || nv == 16 || nv == 24;
 }
 
 Shape shape_of(int64_t rows, int C, int vec, bool backward) {
@@ -570,7 +634,7 @@ Shape shape_of(int64_t rows, int C, int vec, bool backward) {
   int64_t best = -1;
   for (int lanes = 2; lanes <= 32; lanes *= 2)
     for (int nv : kNvs) {
-      if (!nv_built(vec, nv, backward) || (int64_t)lanes * nv < nvec) continue;
+      if (!warp_nv(vec, nv) || (int64_t)lanes * nv < nvec) continue;
       const int64_t waste = (int64_t)lanes * nv * 8 - nvec * 8 > nvec ? (int64_t)lanes * nv - nvec : 0;
       const int64_t cost = waste * 64 + lanes;
       if (best < 0 || cost < best) best = cost, s.lanes = lanes, s.nv = nv;
@@ -578,17 +642,19 @@ Shape shape_of(int64_t rows, int C, int vec, bool backward) {
   if (best >= 0) {
     s.threads = kThreads;
     const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
-    s.blocks = std::min<int64_t>(all, 2 * kSmCount);
+    s.blocks = std::min<int64_t>(all, (!backward && s.nv * vec <= 8 ? 4 : 2) * kSmCount);  // by registers
     return s;
   }
   s.block = true;
-  s.nv = vec == 8 ? 2 : 4;
-  const int64_t threads = ((nvec + s.nv - 1) / s.nv + 31) / 32 * 32;
-  if (threads <= (backward ? 512 : 1024)) {
+  for (int elements = 16; elements <= (backward ? 16 : 32); elements *= 2) {
+    s.nv = elements / vec;
+    const int64_t threads = ((nvec + s.nv - 1) / s.nv + 31) / 32 * 32;
+    if (threads > kBlockThreads) continue;
     s.threads = (int)threads;
-    s.blocks = std::min<int64_t>(rows, (int64_t)kSmCount * std::max<int64_t>(1, 512 / threads));
+    s.blocks = std::min<int64_t>(rows, kSmCount * (kBlockThreads / threads));
     return s;
   }
+  s.block = false;
   s.is_long = true;
   s.threads = kLongThreads;
   s.blocks = std::min<int64_t>(rows, 1 << 20);
@@ -620,7 +686,7 @@ void launch_back(const LayerParams& p, const Shape& s, cudaStream_t st) {
 template <typename T, int VEC, int NV, bool BLOCK>
 void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
   if (backward) {
-    if constexpr (BLOCK || NV * VEC <= 24) {
+    if constexpr (!BLOCK || NV * VEC <= 16) {
       if (p.kind == KC_NORM_RMS && !p.dbias) launch_back<T, VEC, NV, BLOCK, true>(p, s, st);
       else launch_back<T, VEC, NV, BLOCK, false>(p, s, st);
     }
@@ -632,6 +698,22 @@ void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream
   KC_CUDA(cudaGetLastError());
 }
 
+template <typename T, int VEC, int NV>
+bool launch_warp(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
+  if constexpr (warp_nv(VEC, NV)) {
+    if (s.nv != NV) return false;
+    launch_rows<T, VEC, NV, false>(p, s, backward, st);
+    return true;
+  }
+  return false;
+}
+
+template <typename T, int VEC, int... NVS>
+void launch_warps(std::integer_sequence<int, NVS...>, const LayerParams& p, const Shape& s, bool backward,
+                  cudaStream_t st) {
+  (launch_warp<T, VEC, NVS>(p, s, backward, st) || ...);
+}
+
 template <typename T, int VEC>
 void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
   if (s.is_long) {
@@ -639,7 +721,7 @@ void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t s
       layer_norm_long_kernel<T, VEC><<<(unsigned)s.blocks, kLongThreads, 0, st>>>(p);
     } else {
       if (p.part) {
-        const dim3 grid((unsigned)std::min<int64_t>((p.C + 31) / 32, 1 << 20), (unsigned)long_shares(p.rows, p.C));
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)p.C + 31) / 32, 1 << 20), (unsigned)long_shares(p.rows, p.C));
         layer_norm_long_sums_kernel<T><<<grid, kThreads, 0, st>>>(p);
         KC_CUDA(cudaGetLastError());
       }
@@ -647,18 +729,10 @@ void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t s
     }
     KC_CUDA(cudaGetLastError());
   } else if (s.block) {
-    launch_rows<T, VEC, VEC == 8 ? 2 : 4, true>(p, s, backward, st);
-  } else if constexpr (VEC <= 2) {
-    s.nv == 2 ? launch_rows<T, VEC, 2, false>(p, s, backward, st) : launch_rows<T, VEC, 8, false>(p, s, backward, st);
+    if (s.nv == 16 / VEC) launch_rows<T, VEC, 16 / VEC, true>(p, s, backward, st);
+    else launch_rows<T, VEC, 32 / VEC, true>(p, s, backward, st);
   } else {
-    switch (s.nv) {
-      case 1: return launch_rows<T, VEC, 1, false>(p, s, backward, st);
-      case 2: return launch_rows<T, VEC, 2, false>(p, s, backward, st);
-      case 3: return launch_rows<T, VEC, 3, false>(p, s, backward, st);
-      case 4: return launch_rows<T, VEC, 4, false>(p, s, backward, st);
-      case 6: if constexpr (VEC == 4) return launch_rows<T, VEC, 6, false>(p, s, backward, st); break;
-      case 8: if constexpr (VEC == 4) return launch_rows<T, VEC, 8, false>(p, s, backward, st); break;
-    }
+    launch_warps<T, VEC>(std::integer_sequence<int, 1, 2, 3, 4, 6, 8, 12, 16, 24>{}, p, s, backward, st);
   }
 }
 

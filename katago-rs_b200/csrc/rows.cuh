@@ -64,52 +64,50 @@ struct RowVec {
   }
 };
 
-// A vector as pairs of floats, for the two-lane float32 arithmetic (one element: the second of the pair is 0).
+// Copies into shared memory by the thread that reads them there: no barrier, and loads in flight that take no registers.
+// copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived. A single 2-byte
+// element comes with the 4 aligned bytes around it.
 template <typename T, int VEC>
-struct RowPairs {
-  static constexpr int N = (VEC + 1) / 2;
-  using Raw = typename RowVec<T, VEC>::Raw;
-  __device__ static __forceinline__ void unpack(const Raw& r, f32x2 (&v)[N]) {
-    float f[VEC];
-    RowVec<T, VEC>::unpack(r, f);
-#pragma unroll
-    for (int j = 0; j < N; j++) v[j] = {f[2 * j], VEC > 1 ? f[VEC > 1 ? 2 * j + 1 : 0] : 0.0f};
+struct RowCopy {
+  using V = RowVec<T, VEC>;
+  static constexpr int BYTES = V::BYTES;
+  using Slot = typename std::conditional<BYTES == 2, uint32_t, typename V::Raw>::type;
+  __device__ static __forceinline__ void copy(Slot* dst, const T* src) {
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else if constexpr (BYTES == 2)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                   ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)3) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
+                   ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
   }
-  __device__ static __forceinline__ Raw pack(const f32x2 (&v)[N]) {
-    float f[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = j % 2 ? v[j / 2].y : v[j / 2].x;
-    return RowVec<T, VEC>::pack(f);
-  }
-  __device__ static __forceinline__ Raw zero() { return Raw{}; }
-  // `r` where keep is all ones, zeros where it is 0
-  __device__ static __forceinline__ Raw mask(Raw r, uint32_t keep) {
-    if constexpr (sizeof(Raw) == 2) {
-      return r & (uint16_t)keep;
+  // `high`: a single 2-byte element was the upper half of its 4 bytes
+  __device__ static __forceinline__ void unpack(const Slot& s, uint32_t high, float (&v)[VEC]) {
+    if constexpr (BYTES == 2) {
+      const uint16_t h = (uint16_t)(high ? s >> 16 : s);
+      v[0] = to_f<T>(*reinterpret_cast<const T*>(&h));
     } else {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(Raw) / 4; i++) w[i] &= keep;
-      return r;
+      V::unpack(s, v);
     }
   }
 };
-
-// Copies of vectors into shared memory by the thread that reads them there: no barrier, and loads in flight that take no
-// registers. copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived.
-template <typename T, int VEC>
-__device__ __forceinline__ void copy_vec(typename RowVec<T, VEC>::Raw* dst, const T* src) {
-  constexpr int BYTES = RowVec<T, VEC>::BYTES;
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-  else if constexpr (BYTES >= 4)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
-  else
-    *dst = *reinterpret_cast<const uint16_t*>(src);
-}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// `r` where keep is all ones, zeros where it is 0
+template <typename Raw>
+__device__ __forceinline__ Raw masked(Raw r, uint32_t keep) {
+  if constexpr (sizeof(Raw) == 2) {
+    return r & (uint16_t)keep;
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(Raw) / 4; i++) w[i] &= keep;
+    return r;
+  }
+}
 
 // VEC float32 parameters; `wide`: the array is 16-byte aligned, and `p` as far into it as VEC allows.
 template <int VEC>
@@ -124,14 +122,6 @@ __device__ __forceinline__ void load_params(const float* p, bool wide, float (&v
 #pragma unroll
     for (int i = 0; i < VEC; i++) v[i] = __ldg(p + i);
   }
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_param_pairs(const float* p, bool wide, f32x2 (&v)[(VEC + 1) / 2]) {
-  float f[VEC];
-  load_params<VEC>(p, wide, f);
-#pragma unroll
-  for (int j = 0; j < (VEC + 1) / 2; j++) v[j] = {f[2 * j], VEC > 1 ? f[VEC > 1 ? 2 * j + 1 : 0] : 0.0f};
 }
 
 // Sums over groups of `lanes` neighbouring lanes of a warp (a power of two; every lane of the warp takes part).
@@ -152,21 +142,26 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
-// Sum over a block of whole warps. `red` holds a value per warp; two calls in a row take different ones.
+// Sum over a block of whole warps, the warps' sums in their order. `red` holds a value per warp; two calls in a row take
+// different ones.
 __device__ __forceinline__ float2 block_sum(float2 v, float2* red) {
   v = lanes_sum(v, 32);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
-  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
-  return lanes_sum(lane < warps ? red[lane] : make_float2(0.0f, 0.0f), 32);
+  v = red[0];
+#pragma unroll 8
+  for (int w = 1; w < blockDim.x / 32; w++) v.x += red[w].x, v.y += red[w].y;
+  return v;
 }
 
 __device__ __forceinline__ float block_sum(float v, float2* red) {
   v = lanes_sum(v, 32);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32].x = v;
   __syncthreads();
-  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
-  return lanes_sum(lane < warps ? red[lane].x : 0.0f, 32);
+  v = red[0].x;
+#pragma unroll 8
+  for (int w = 1; w < blockDim.x / 32; w++) v += red[w].x;
+  return v;
 }
 
 // Rows of `points` to a board. Boards whose rows go on at one stride are one long row of rows (points 0).
