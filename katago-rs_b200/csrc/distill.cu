@@ -5,10 +5,16 @@
 //   loss = T^2 sum_j p_j (log p_j - log q_{id_j})
 //   dz_i = dloss T (P q_i - sum_{j: id_j = i} p_j), P = sum_j p_j
 //
-// Forward, one pass over a row's logits keeps the largest and the sum of exp((z - largest) / T) in every thread and
-// merges them; the entries' terms, differences of logarithms, are in 64 bits. Backward, the saved pair makes each
-// element's gradient one exponential; a row's entries (their classes gathered before the row is written, so that the
-// gradient may take the logits' place) are written over it at the end. Rows without entries are not read.
+// The teacher's side of a row is a few entries, held by the threads that share the row: exponentials of differences taken
+// in 64 bits, and sums in 64 bits, since the loss is a difference of logarithms. With e_j = exp((t_j - max t) / T) the
+// loss is T^2 (sum e_j x_j / sum e_j + log(s / sum e_j)), x_j = ((t_j - max t) - (z_{id_j} - m)) / T, from the row's
+// largest logit m and s = sum exp((z - m) / T): one logarithm a row.
+// Backward, the saved (m, s) make each element's gradient one exponential; the entries' classes are gathered before the
+// row is written, so that the gradient may take the logits' place, and written over it at the end. Rows without entries
+// are not read.
+//
+// Rows of at most 2,048 classes are a warp's, which keeps the row in shared memory while the next one is on its way there;
+// longer ones a block's or, where rows are few, a cluster's (forward) or several blocks' (backward).
 
 #include <algorithm>
 #include <cmath>
@@ -23,9 +29,11 @@ namespace {
 [[noreturn]] void bad(const std::string& what) { fail(KC_ERR_INVALID, "CUDA backend: top logits: " + what); }
 
 constexpr int kThreads = 256;
-constexpr int kWarpClasses = 2048;  // rows up to this long are a warp's
-constexpr int kWarpTop = 128;       // entries that a warp of the backward pass keeps in shared memory
-constexpr int kMaxTop = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kHeld = 4;            // entries of a thread
+constexpr int kWarpClasses = 2048;  // rows up to this long, with up to 32 kHeld entries, are a warp's
+constexpr int kWarpTop = 32 * kHeld;
+constexpr int kMaxTop = kThreads * kHeld;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -42,6 +50,7 @@ struct DistillParams {
   int64_t rows;
   int classes, k;
   int splits, seg;  // blocks of a row, classes of each
+  int row_bytes;    // of a warp's row in shared memory
   double temperature;
   float c;          // log2(e) / T
 };
@@ -52,6 +61,25 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// exp of a 64-bit argument to float32's precision, 0 below -200
+__device__ __forceinline__ float exp_of(double x) {
+  x = x < -200.0 ? -200.0 : x;
+  const float hi = (float)x, e = expf(hi);
+  return fmaf(e, (float)(x - hi), e);
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float warp_sum(float v) { return lanes_sum(v, 32); }
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // The largest value m (-inf: none) and s = sum of exp((z - m) / T).
 struct Peak {
   float m, s;
@@ -60,159 +88,279 @@ struct Peak {
 // An exponent's base: 0 where there is only -inf, whose differences would be NaN.
 __device__ __forceinline__ float base_of(float m) { return m == -kInf ? 0.0f : m; }
 
-__device__ __forceinline__ Peak merge(Peak a, Peak b, float c) {
-  const float m = fmaxf(a.m, b.m), base = base_of(m);
-  return {m, a.s * ex2((a.m - base) * c) + b.s * ex2((b.m - base) * c)};
-}
-
-template <int N>
-__device__ __forceinline__ void add_values(Peak& a, const float (&v)[N], float c) {
-  float m = a.m;
-#pragma unroll
-  for (int j = 0; j < N; j++) m = fmaxf(m, v[j]);
-  const float base = base_of(m);
-  if (m != a.m) a.s *= ex2((a.m - base) * c);
-  a.m = m;
-#pragma unroll
-  for (int j = 0; j < N; j++) a.s += ex2((v[j] - base) * c);
-}
-
 __device__ __forceinline__ Peak warp_peak(Peak a, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = merge(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)}, c);
-  return a;
+  const float m = warp_max(a.m);
+  return {m, warp_sum(a.s * ex2((a.m - base_of(m)) * c))};
 }
 
-// z[0, n) over `threads` threads: whole 16-byte vectors from the first aligned address on, single elements around them.
+// 16 bytes of a row
 template <typename T>
-__device__ __forceinline__ Peak row_peak(const T* z, int n, int thread, int threads, float c) {
-  constexpr int VEC = 16 / sizeof(T);
+struct Chunk {
+  static constexpr int VEC = 16 / sizeof(T), N = VEC / 2;
   using V = RowVec<T, VEC>;
-  Peak a{-kInf, 0.0f};
-  const int head = min(n, (int)((16 - (uintptr_t)z % 16) % 16 / sizeof(T)));
-  const int nvec = (n - head) / VEC;
-  const T* zv = z + head;
-  int v = thread;
-  for (; v + 3 * threads < nvec; v += 4 * threads) {
-    typename V::Raw raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) raw[i] = V::load(zv + (int64_t)(v + i * threads) * VEC);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float f[VEC];
-      V::unpack(raw[i], f);
-      add_values(a, f, c);
+  __device__ static __forceinline__ float largest(const uint4& r) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+    if constexpr (std::is_same<T, float>::value) {
+      return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2* h = reinterpret_cast<const T2*>(&r);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(to_f<T>(m.x), to_f<T>(m.y));
     }
   }
-  for (; v < nvec; v += threads) {
+  // exp((z - base) / T) of the elements
+  __device__ static __forceinline__ void exps(const uint4& r, float base, float c, f32x2 (&e)[N]) {
     float f[VEC];
-    V::unpack(V::load(zv + (int64_t)v * VEC), f);
-    add_values(a, f, c);
+    V::unpack(r, f);
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const f32x2 x = mul2(add2({f[2 * j], f[2 * j + 1]}, {-base, -base}), {c, c});
+      e[j] = {ex2(x.x), ex2(x.y)};
+    }
   }
-  for (int i = thread; i < n - nvec * VEC; i += threads) {
-    const float f[1] = {to_f<T>(z[i < head ? i : i + nvec * VEC])};
-    add_values(a, f, c);
+  __device__ static __forceinline__ f32x2 sum(const uint4& r, float base, float c) {
+    f32x2 e[N];
+    exps(r, base, c, e);
+#pragma unroll
+    for (int o = N / 2; o > 0; o /= 2)
+#pragma unroll
+      for (int j = 0; j < o; j++) e[j] = add2(e[j], e[j + o]);
+    return e[0];
   }
-  return a;
-}
-
-// The teacher's entries of a row.
-struct Entries {
-  const int32_t* ids;
-  const float* top;
-  __device__ __forceinline__ Entries(const DistillParams& p, int64_t r) : ids(p.ids + r * p.ts), top(p.top + r * p.ts) {}
-  __device__ __forceinline__ bool there(const DistillParams& p, int j) const {
-    const int id = __ldg(ids + j);
-    return id >= 0 && id < p.classes && __ldg(top + j) != -kInf;
+  __device__ static __forceinline__ uint4 gradient(const uint4& r, float base, float c, float a) {
+    f32x2 e[N];
+    exps(r, base, c, e);
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const f32x2 v = mul2(e[j], {a, a});
+      f[2 * j] = v.x;
+      f[2 * j + 1] = v.y;
+    }
+    return V::pack(f);
   }
 };
 
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// L of a row, by a warp.
-__device__ __forceinline__ double teacher_log_sum(const DistillParams& p, const Entries& e, int64_t r) {
-  if (p.whole) return p.whole[r];
-  const int lane = threadIdx.x % 32;
-  float m = -kInf;
-  for (int j = lane; j < p.k; j += 32)
-    if (e.there(p, j)) m = fmaxf(m, __ldg(e.top + j));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  double s = 0.0;
-  for (int j = lane; j < p.k; j += 32)
-    if (e.there(p, j)) s += exp(((double)__ldg(e.top + j) - m) / p.temperature);
-  return m / p.temperature + log(warp_sum(s));
-}
-
-// The loss of a row by a warp, from its logits' (m, s).
+// Elements before an address that begin its 16 bytes.
 template <typename T>
-__device__ __forceinline__ double row_loss(const DistillParams& p, const Entries& e, int64_t r, const T* z, Peak a) {
-  const double log_sum = teacher_log_sum(p, e, r), log_s = log((double)a.s);
-  double loss = 0.0;
-  for (int j = threadIdx.x % 32; j < p.k; j += 32) {
-    if (!e.there(p, j)) continue;
-    const double log_p = __ldg(e.top + j) / p.temperature - log_sum, prob = exp(log_p);
-    const double log_q = ((double)to_f<T>(z[__ldg(e.ids + j)]) - a.m) / p.temperature - log_s;
-    if (prob != 0.0) loss += prob * (log_p - log_q);
-  }
-  return warp_sum(loss) * p.temperature * p.temperature;
+__device__ __forceinline__ int lead_of(const T* p) {
+  return (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
 }
 
-__device__ __forceinline__ void write_row(const DistillParams& p, int64_t r, double loss, Peak a) {
-  p.loss[r] = (float)loss;
+// ---- the teacher's entries ---------------------------------------------------------------------------------------
+// Entry thread + i threads of a row in register i; id -1 and logit -inf where there is none.
+struct Held {
+  int id[kHeld];
+  float t[kHeld];
+  __device__ __forceinline__ void load(const DistillParams& p, int64_t r, int thread, int threads) {
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) {
+      const int j = thread + i * threads;
+      id[i] = -1;
+      t[i] = -kInf;
+      if (j < p.k && r < p.rows) {
+        id[i] = __ldg(p.ids + r * p.ts + j);
+        t[i] = __ldg(p.top + r * p.ts + j);
+      }
+    }
+  }
+  // once they have arrived: whether the thread has any
+  __device__ __forceinline__ bool settle(const DistillParams& p) {
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) {
+      if (id[i] < 0 || id[i] >= p.classes || t[i] == -kInf) {
+        id[i] = -1;
+        t[i] = -kInf;
+      }
+      some |= id[i] >= 0;
+    }
+    return some;
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = t[0];
+#pragma unroll
+    for (int i = 1; i < kHeld; i++) m = fmaxf(m, t[i]);
+    return m;
+  }
+};
+
+// The entries' exponentials: of (t - largest) / T, or with the teacher's own log sum the probabilities themselves.
+struct Teacher {
+  double shift, inv;  // exp(t inv - shift)
+  __device__ __forceinline__ Teacher(const DistillParams& p, int64_t r, float largest) {
+    inv = 1.0 / p.temperature;
+    shift = p.whole ? (double)__ldg(p.whole + r) : largest * inv;
+  }
+  __device__ __forceinline__ double at(float t) const { return t * inv - shift; }
+};
+
+// A thread's share of sum e and of sum e x, where z are the entries' logits.
+__device__ __forceinline__ void loss_terms(const Held& h, const Teacher& teacher, const float (&z)[kHeld], float m,
+                                           double& se, double& sex) {
+  se = sex = 0.0;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) {
+    if (h.id[i] < 0) continue;
+    const double x = teacher.at(h.t[i]);
+    const double e = exp_of(x);
+    se += e;
+    if (e != 0.0) sex += e * (x - ((double)z[i] - (double)m) * teacher.inv);
+  }
+}
+__device__ __forceinline__ void write_loss(const DistillParams& p, int64_t r, double se, double sex, Peak a) {
+  const double loss = p.whole ? sex + se * log((double)a.s) : sex / se + log((double)a.s / se);
+  p.loss[r] = (float)(loss * p.temperature * p.temperature);
   if (p.stats) p.stats[r] = make_float2(a.m, a.s);
 }
+__device__ __forceinline__ void write_nothing(const DistillParams& p, int64_t r) {
+  p.loss[r] = 0.0f;
+  if (p.stats) p.stats[r] = make_float2(0.0f, 0.0f);
+}
+
+// ---- rows of a warp ----------------------------------------------------------------------------------------------
+// The aligned 16-byte pieces that hold a row, in shared memory (such a piece never leaves the allocation of the element in
+// it); the elements of the first and last one that are not the row's become -inf.
+template <typename T>
+struct WarpRow {
+  static constexpr int VEC = 16 / sizeof(T);
+  static int bytes(int classes) { return (int)((classes * sizeof(T) + 30) / 16 * 16); }
+  T* buf;
+  __device__ __forceinline__ static int pieces(int lead, int classes) { return (lead + classes + VEC - 1) / VEC; }
+  __device__ __forceinline__ void fetch(const T* z, int classes, int lane) const {
+    const int lead = lead_of(z), n = pieces(lead, classes);
+    const T* z0 = z - lead;
+    for (int v = lane; v < n; v += 32) RowCopy<T, VEC>::copy(reinterpret_cast<uint4*>(buf) + v, z0 + v * VEC);
+  }
+  __device__ __forceinline__ void close(int lead, int classes, int lane) const {
+    if (lane < lead) buf[lane] = from_f<T>(-kInf);
+    const int tail = lead + classes + lane;
+    if (tail < pieces(lead, classes) * VEC) buf[tail] = from_f<T>(-kInf);
+    __syncwarp();
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_warp_kernel(const DistillParams p) {
-  const int lane = threadIdx.x % 32;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; r < p.rows; r += step) {
-    const Entries e(p, r);
-    bool some = false;
-    for (int j = lane; j < p.k; j += 32) some |= e.there(p, j);
-    if (!__any_sync(0xffffffffu, some)) {
-      if (lane == 0) write_row(p, r, 0.0, {0.0f, 0.0f});
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  auto row = [&](int turn) { return WarpRow<T>{reinterpret_cast<T*>(smem + (warp * 2 + turn) * p.row_bytes)}; };
+  const int64_t step = (int64_t)gridDim.x * kWarps;
+  int64_t r = (int64_t)blockIdx.x * kWarps + warp;
+  const T* z = static_cast<const T*>(p.z);
+  Held next, later;  // the next row's entries, and those of the one behind it on their way
+  next.load(p, r, lane, 32);
+  bool some_next = __any_sync(0xffffffffu, next.settle(p));
+  if (some_next) row(0).fetch(z + r * p.zs, p.classes, lane);
+  copy_commit();
+  later.load(p, r + step, lane, 32);
+  for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
+    const Held h = next;
+    const bool some = some_next;
+    next = later;
+    some_next = __any_sync(0xffffffffu, next.settle(p));
+    if (some_next) row(turn ^ 1).fetch(z + (r + step) * p.zs, p.classes, lane);
+    copy_commit();
+    later.load(p, r + 2 * step, lane, 32);
+    if (!some) {
+      if (lane == 0) write_nothing(p, r);
       continue;
     }
-    const T* z = static_cast<const T*>(p.z) + r * p.zs;
-    const Peak a = warp_peak(row_peak(z, p.classes, lane, 32, p.c), p.c);
-    const double loss = row_loss(p, e, r, z, a);
-    if (lane == 0) write_row(p, r, loss, a);
+    copy_wait<1>();
+    __syncwarp();
+    const int lead = lead_of(z + r * p.zs), n = WarpRow<T>::pieces(lead, p.classes);
+    const WarpRow<T> at = row(turn);
+    at.close(lead, p.classes, lane);
+    const uint4* piece = reinterpret_cast<const uint4*>(at.buf);
+    float m = -kInf, zh[kHeld];
+    for (int v = lane; v < n; v += 32) m = fmaxf(m, Chunk<T>::largest(piece[v]));
+    m = warp_max(m);
+    const float base = base_of(m);
+    f32x2 s2 = {0.0f, 0.0f};
+    for (int v = lane; v < n; v += 32) s2 = add2(s2, Chunk<T>::sum(piece[v], base, p.c));
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) zh[i] = h.id[i] >= 0 ? to_f<T>(at.buf[lead + h.id[i]]) : 0.0f;
+    const Teacher teacher(p, r, warp_max(h.largest()));
+    double se, sex;
+    loss_terms(h, teacher, zh, m, se, sex);
+    const float s = warp_sum(s2.x + s2.y);
+    se = warp_sum(se);
+    sex = warp_sum(sex);
+    if (lane == 0) write_loss(p, r, se, sex, {m, s});
+    __syncwarp();  // the row's place is free
   }
+  copy_wait<0>();
 }
 
-// A block, or a cluster of `splits` blocks, to a row.
+// ---- rows of a block ---------------------------------------------------------------------------------------------
+// z[0, n) over a block's threads: whole 16-byte pieces from the first aligned address on, single elements around them.
+template <typename T>
+__device__ __forceinline__ Peak row_peak(const T* z, int n, float c) {
+  constexpr int VEC = 16 / sizeof(T);
+  Peak a{-kInf, 0.0f};
+  auto raise = [&](float m) {
+    m = fmaxf(a.m, m);
+    if (m != a.m) a.s *= ex2((a.m - base_of(m)) * c);
+    a.m = m;
+    return base_of(m);
+  };
+  const int lead = lead_of(z), head = min(n, lead ? VEC - lead : 0), pieces = (n - head) / VEC, threads = blockDim.x;
+  const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+  int v = threadIdx.x;
+  for (; v + 3 * threads < pieces; v += 4 * threads) {
+    uint4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) raw[i] = zv[v + i * threads];
+    const float base = raise(fmaxf(fmaxf(Chunk<T>::largest(raw[0]), Chunk<T>::largest(raw[1])),
+                                   fmaxf(Chunk<T>::largest(raw[2]), Chunk<T>::largest(raw[3]))));
+    f32x2 s = Chunk<T>::sum(raw[0], base, c);
+#pragma unroll
+    for (int i = 1; i < 4; i++) s = add2(s, Chunk<T>::sum(raw[i], base, c));
+    a.s += s.x + s.y;
+  }
+  for (; v < pieces; v += threads) {
+    const uint4 raw = zv[v];
+    const f32x2 s = Chunk<T>::sum(raw, raise(Chunk<T>::largest(raw)), c);
+    a.s += s.x + s.y;
+  }
+  for (int i = threadIdx.x; i < n - pieces * VEC; i += threads) {
+    const float f = to_f<T>(z[i < head ? i : i + pieces * VEC]), base = raise(f);
+    a.s += ex2((f - base) * c);
+  }
+  return a;
+}
+
+// A block, or a cluster of `splits` blocks, to a row; the first of them has the entries.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_block_kernel(const DistillParams p) {
-  __shared__ Peak red[kThreads / 32];
+  __shared__ Peak red[kWarps];
+  __shared__ float red_t[kWarps];
+  __shared__ double red_e[kWarps], red_x[kWarps];
   __shared__ Peak share;
   const int64_t r = blockIdx.x / p.splits;
-  const int rank = blockIdx.x % p.splits, lane = threadIdx.x % 32;
-  const Entries e(p, r);
-  bool some = false;
-  for (int j = threadIdx.x; j < p.k; j += kThreads) some |= e.there(p, j);
-  if (!__syncthreads_or(some)) {  // all blocks of the row see the same
-    if (rank == 0 && threadIdx.x == 0) write_row(p, r, 0.0, {0.0f, 0.0f});
+  const int rank = blockIdx.x % p.splits, lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  Held h;
+  h.load(p, r, threadIdx.x, blockDim.x);
+  if (!__syncthreads_or(h.settle(p))) {  // all blocks of the row see the same
+    if (rank == 0 && threadIdx.x == 0) write_nothing(p, r);
     return;
   }
   const T* z = static_cast<const T*>(p.z) + r * p.zs;
+  float zh[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) zh[i] = rank == 0 && h.id[i] >= 0 ? to_f<T>(z[h.id[i]]) : 0.0f;
   const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg), c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
-  Peak a = warp_peak(row_peak(z + c0, c1 - c0, threadIdx.x, kThreads, p.c), p.c);
-  if (lane == 0) red[threadIdx.x / 32] = a;
+  Peak a = warp_peak(row_peak(z + c0, c1 - c0, p.c), p.c);
+  const float mt = warp_max(h.largest());
+  if (lane == 0) red[warp] = a, red_t[warp] = mt;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    a = warp_peak(lane < kThreads / 32 ? red[lane] : Peak{-kInf, 0.0f}, p.c);
-    if (lane == 0) share = a;
-  }
+  // every warp joins the warps' peaks for itself
+  a = warp_peak(lane < warps ? red[lane] : Peak{-kInf, 0.0f}, p.c);
   if (p.splits > 1) {
+    if (threadIdx.x == 0) share = a;
     cluster_sync();
-    if (rank == 0 && threadIdx.x < 32) {
+    if (rank == 0) {
       a = {-kInf, 0.0f};
       if (lane < p.splits) {
         const uint32_t at = mapa_shared(smem_u32(&share), lane);
@@ -221,20 +369,29 @@ __global__ void __launch_bounds__(kThreads) distill_block_kernel(const DistillPa
       a = warp_peak(a, p.c);
     }
     cluster_sync();
+    if (rank != 0) return;
   }
-  if (rank == 0 && threadIdx.x < 32) {
-    const double loss = row_loss(p, e, r, z, a);
-    if (lane == 0) write_row(p, r, loss, a);
+  const Teacher teacher(p, r, warp_max(lane < warps ? red_t[lane] : -kInf));
+  double se, sex;
+  loss_terms(h, teacher, zh, a.m, se, sex);
+  se = warp_sum(se);
+  sex = warp_sum(sex);
+  if (lane == 0) red_e[warp] = se, red_x[warp] = sex;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < warps; w++) se += red_e[w], sex += red_x[w];
+    write_loss(p, r, se, sex, a);
   }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------
-// The entries of a row in shared memory, held by a warp or a block.
-struct EntryStore {
-  int* id;          // -1: absent
-  float* p;         // probability, and in the end the gradient
-  float* total;     // of all entries of that class; negative where an earlier entry stands for it
-  uint32_t* seen;   // a bit for each class modulo `bits`
+// Where entries of one class find each other: a bit for each class modulo `bits`, the bits that two entries share, and
+// the entries for those that have to look.
+struct Meet {
+  uint32_t* seen;
+  uint32_t* twice;
+  int* id;
+  float* p;
   uint32_t bits;
 };
 
@@ -243,190 +400,265 @@ __device__ __forceinline__ void sync_rows() {
   if (BLOCK) __syncthreads();
   else __syncwarp();
 }
-
-// Entries of one class become one. A class whose bit is set before it is looked for among all entries.
 template <bool BLOCK>
-__device__ __forceinline__ void join_equal(const EntryStore& s, int k, int thread, int threads) {
-  for (uint32_t i = thread; i < s.bits / 32; i += threads) s.seen[i] = 0;
-  sync_rows<BLOCK>();
-  uint32_t again = 0;  // this thread's entries (at most 32) whose bit was set
-  for (int j = thread, n = 0; j < k; j += threads, n++) {
-    if (s.id[j] < 0) continue;
-    const uint32_t b = (uint32_t)s.id[j] & (s.bits - 1);
-    if (atomicOr(&s.seen[b / 32], 1u << b % 32) >> b % 32 & 1) again |= 1u << n;
-  }
-  for (int j = thread, n = 0; j < k; j += threads, n++) {
-    if (!(again >> n & 1)) continue;
-    int low = -1, count = 0;
-    float sum = 0.0f;
-    for (int i = 0; i < k; i++) {
-      if (s.id[i] != s.id[j]) continue;
-      if (low < 0) low = i;
-      sum += s.p[i];
-      count++;
+__device__ __forceinline__ bool any_rows(bool v) {
+  return BLOCK ? __syncthreads_or(v) : __any_sync(0xffffffffu, v);
+}
+
+template <bool BLOCK>
+__device__ __forceinline__ void clear(const Meet& s, int thread, int threads) {
+  for (uint32_t i = thread; i < s.bits / 32; i += threads) s.seen[i] = s.twice[i] = 0;
+}
+
+// `prob` of the first entry of a class becomes the sum over all of that class in their order, those of the others
+// negative. The bits are clear.
+template <bool BLOCK>
+__device__ __forceinline__ void join_equal(const Meet& s, const Held& h, float (&prob)[kHeld], int k, int thread,
+                                           int threads) {
+  bool again = false;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) {
+    if (h.id[i] < 0) continue;
+    const uint32_t b = (uint32_t)h.id[i] & (s.bits - 1), bit = 1u << b % 32;
+    if (atomicOr(&s.seen[b / 32], bit) & bit) {
+      atomicOr(&s.twice[b / 32], bit);
+      again = true;
     }
-    if (count > 1)  // all threads that come here for this class write the same
-      for (int i = low; i < k; i++)
-        if (s.id[i] == s.id[j]) s.total[i] = i == low ? sum : -1.0f;
   }
+  if (!any_rows<BLOCK>(again)) return;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (thread + i * threads < k) s.id[thread + i * threads] = h.id[i], s.p[thread + i * threads] = prob[i];
   sync_rows<BLOCK>();
-}
-
-// dz[0, n) = a exp((z - m) / T)
-template <typename T, int VEC>
-__device__ __forceinline__ void row_gradient(const T* z, T* dz, int n, int thread, int threads, float m, float c, float a) {
-  using V = RowVec<T, VEC>;
-  const int head = VEC == 1 ? 0 : min(n, (int)((16 - (uintptr_t)z % 16) % 16 / sizeof(T)));
-  const int nvec = (n - head) / VEC;
-  int v = thread;
-  auto one = [&](typename V::Raw raw, int at) {
-    float f[VEC];
-    V::unpack(raw, f);
 #pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = a * ex2((f[j] - m) * c);
-    V::store(dz + head + (int64_t)at * VEC, V::pack(f));
-  };
-  for (; v + 3 * threads < nvec; v += 4 * threads) {
-    typename V::Raw raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) raw[i] = V::load(z + head + (int64_t)(v + i * threads) * VEC);
-#pragma unroll
-    for (int i = 0; i < 4; i++) one(raw[i], v + i * threads);
-  }
-  for (; v < nvec; v += threads) one(V::load(z + head + (int64_t)v * VEC), v);
-  for (int i = thread; i < n - nvec * VEC; i += threads) {
-    const int at = i < head ? i : i + nvec * VEC;
-    dz[at] = from_f<T>(a * ex2((to_f<T>(z[at]) - m) * c));
+  for (int i = 0; i < kHeld; i++) {
+    if (h.id[i] < 0) continue;
+    const uint32_t b = (uint32_t)h.id[i] & (s.bits - 1);
+    if (!(s.twice[b / 32] >> b % 32 & 1)) continue;
+    float sum = 0.0f;
+    int low = -1;
+    for (int j = 0; j < k; j++) {
+      if (s.id[j] != h.id[i]) continue;
+      if (low < 0) low = j;
+      sum += s.p[j];
+    }
+    prob[i] = low == thread + i * threads ? sum : -1.0f;
   }
 }
 
-// A row's classes [c0, c1) by a warp or a block. `log_sum` and `prob` are the same in all its threads.
-template <typename T, int VEC, bool BLOCK>
-__device__ __forceinline__ void back_row(const DistillParams& p, int64_t r, int c0, int c1, const EntryStore& s,
-                                         int thread, int threads, double prob) {
-  const T* z = static_cast<const T*>(p.z) + r * p.zs;
-  T* dz = static_cast<T*>(p.dz) + r * p.ds;
-  join_equal<BLOCK>(s, p.k, thread, threads);
-  const float2 st = p.stats[r];
-  const double g = (p.dloss ? (double)p.dloss[r] : 1.0) * p.temperature, scale = prob / st.y;
-  const float base = base_of(st.x);
-  for (int j = thread; j < p.k; j += threads) {
-    const int id = s.id[j];
-    if (id < c0 || id >= c1) continue;
-    s.p[j] = (float)(g * (scale * exp(((double)to_f<T>(z[id]) - base) / p.temperature) - (double)s.total[j]));
+// dz[0, n) = a exp((z - base) / T) over a block's threads; VEC 1: z and dz are not equally far from 16 bytes
+template <typename T, bool WIDE>
+__device__ __forceinline__ void row_gradient(const T* z, T* dz, int n, float base, float c, float a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int threads = blockDim.x;
+  int head = n, pieces = 0;
+  if (WIDE) {
+    const int lead = lead_of(z);
+    head = min(n, lead ? VEC - lead : 0);
+    pieces = (n - head) / VEC;
+    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+    uint4* dv = reinterpret_cast<uint4*>(dz + head);
+    int v = threadIdx.x;
+    for (; v + 3 * threads < pieces; v += 4 * threads) {
+      uint4 raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) raw[i] = zv[v + i * threads];
+#pragma unroll
+      for (int i = 0; i < 4; i++) dv[v + i * threads] = Chunk<T>::gradient(raw[i], base, c, a);
+    }
+    for (; v < pieces; v += threads) dv[v] = Chunk<T>::gradient(zv[v], base, c, a);
   }
-  sync_rows<BLOCK>();
-  row_gradient<T, VEC>(z + c0, dz + c0, c1 - c0, thread, threads, base, p.c, (float)(g * scale));
-  sync_rows<BLOCK>();
-  for (int j = thread; j < p.k; j += threads) {
-    const int id = s.id[j];
-    if (id >= c0 && id < c1 && s.total[j] >= 0.0f) dz[id] = from_f<T>(s.p[j]);
+  for (int i = threadIdx.x; i < n - pieces * VEC; i += threads) {
+    const int at = i < head ? i : i + pieces * VEC;
+    dz[at] = from_f<T>(a * ex2((to_f<T>(z[at]) - base) * c));
   }
 }
 
-template <typename T, int VEC>
+template <typename T>
 __device__ __forceinline__ void zero_row(T* dz, int n, int thread, int threads) {
-  using V = RowVec<T, VEC>;
-  const int head = VEC == 1 ? 0 : min(n, (int)((16 - (uintptr_t)dz % 16) % 16 / sizeof(T)));
-  const int nvec = (n - head) / VEC;
-  for (int v = thread; v < nvec; v += threads) V::store(dz + head + (int64_t)v * VEC, typename V::Raw{});
-  for (int i = thread; i < n - nvec * VEC; i += threads) dz[i < head ? i : i + nvec * VEC] = from_f<T>(0.0f);
+  constexpr int VEC = 16 / sizeof(T);
+  const int lead = lead_of(dz), head = min(n, lead ? VEC - lead : 0), pieces = (n - head) / VEC;
+  for (int v = thread; v < pieces; v += threads) reinterpret_cast<uint4*>(dz + head)[v] = uint4{};
+  for (int i = thread; i < n - pieces * VEC; i += threads) dz[i < head ? i : i + pieces * VEC] = from_f<T>(0.0f);
 }
 
-// The entries and their probabilities into shared memory; the sum of these. Every warp finds L for itself.
-template <bool BLOCK>
-__device__ __forceinline__ double load_entries(const DistillParams& p, const Entries& e, int64_t r, const EntryStore& s,
-                                               int thread, int threads, double* red) {
-  const double log_sum = teacher_log_sum(p, e, r);
-  double sum = 0.0;
-  for (int j = thread; j < p.k; j += threads) {
-    const bool there = e.there(p, j);
-    const double prob = there ? exp(__ldg(e.top + j) / p.temperature - log_sum) : 0.0;
-    s.id[j] = there ? __ldg(e.ids + j) : -1;
-    s.p[j] = s.total[j] = (float)prob;
-    sum += prob;
+// The factors of a row's gradient: g (scale exp((z - base) / T) - p).
+struct Factors {
+  double g, scale;
+  float base;
+  __device__ __forceinline__ Factors(const DistillParams& p, int64_t r, double sum) {
+    const float2 st = p.stats[r];
+    g = (p.dloss ? (double)p.dloss[r] : 1.0) * p.temperature;
+    scale = sum / st.y;
+    base = base_of(st.x);
   }
-  sum = warp_sum(sum);
-  if (BLOCK) {
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = sum;
-    __syncthreads();
-    sum = 0.0;
-    for (int w = 0; w < kThreads / 32; w++) sum += red[w];
+  __device__ __forceinline__ float entry(float z, float prob, double inv) const {
+    return (float)(g * (scale * exp_of(((double)z - base) * inv) - prob));
   }
-  return sum;
-}
+};
 
-template <typename T, int VEC>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const DistillParams p) {
-  __shared__ int id[kThreads / 32][kWarpTop];
-  __shared__ float prob[kThreads / 32][kWarpTop], total[kThreads / 32][kWarpTop];
-  __shared__ uint32_t seen[kThreads / 32][kWarpClasses / 32];
+  constexpr int VEC = 16 / sizeof(T), WORDS = kWarpClasses / 32;
+  __shared__ uint32_t seen[kWarps][2][WORDS];
+  __shared__ int ids[kWarps][kWarpTop];
+  __shared__ float probs[kWarps][kWarpTop];
+  extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const EntryStore s{id[warp], prob[warp], total[warp], seen[warp], kWarpClasses};
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + warp; r < p.rows; r += step) {
-    const Entries e(p, r);
-    bool some = false;
-    for (int j = lane; j < p.k; j += 32) some |= e.there(p, j);
-    if (!__any_sync(0xffffffffu, some)) {
-      zero_row<T, VEC>(static_cast<T*>(p.dz) + r * p.ds, p.classes, lane, 32);
+  const Meet meet{seen[warp][0], seen[warp][1], ids[warp], probs[warp], kWarpClasses};
+  auto row = [&](int turn) { return WarpRow<T>{reinterpret_cast<T*>(smem + (warp * 2 + turn) * p.row_bytes)}; };
+  const int64_t step = (int64_t)gridDim.x * kWarps;
+  int64_t r = (int64_t)blockIdx.x * kWarps + warp;
+  const T* z = static_cast<const T*>(p.z);
+  Held next, later;
+  next.load(p, r, lane, 32);
+  bool some_next = __any_sync(0xffffffffu, next.settle(p));
+  if (some_next) row(0).fetch(z + r * p.zs, p.classes, lane);
+  copy_commit();
+  later.load(p, r + step, lane, 32);
+  for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
+    const Held h = next;
+    const bool some = some_next;
+    next = later;
+    some_next = __any_sync(0xffffffffu, next.settle(p));
+    if (some_next) row(turn ^ 1).fetch(z + (r + step) * p.zs, p.classes, lane);
+    copy_commit();
+    later.load(p, r + 2 * step, lane, 32);
+    T* dz = static_cast<T*>(p.dz) + r * p.ds;
+    if (!some) {
+      zero_row(dz, p.classes, lane, 32);
       continue;
     }
-    __syncwarp();  // the last row's entries have been written
-    const double sum = load_entries<false>(p, e, r, s, lane, 32, nullptr);
-    back_row<T, VEC, false>(p, r, 0, p.classes, s, lane, 32, sum);
+    clear<false>(meet, lane, 32);
+    const Teacher teacher(p, r, warp_max(h.largest()));
+    float prob[kHeld];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) {
+      prob[i] = h.id[i] >= 0 ? exp_of(teacher.at(h.t[i])) : 0.0f;
+      sum += prob[i];
+    }
+    sum = warp_sum(sum);
+    if (!p.whole) {
+#pragma unroll
+      for (int i = 0; i < kHeld; i++) prob[i] = (float)(prob[i] / sum);
+      sum = 1.0;
+    }
+    __syncwarp();
+    join_equal<false>(meet, h, prob, p.k, lane, 32);
+    const Factors f(p, r, sum);
+    const float a = (float)(f.g * f.scale);
+    copy_wait<1>();
+    __syncwarp();
+    const int lead = lead_of(z + r * p.zs), n = WarpRow<T>::pieces(lead, p.classes);
+    const T* buf = row(turn).buf;
+    // the pieces that are the row's alone as they are, the elements around them one at a time
+    const int v0 = !WIDE ? n : lead ? 1 : 0, v1 = !WIDE ? n : (lead + p.classes) / VEC;
+    for (int v = v0 + lane; v < v1; v += 32)
+      reinterpret_cast<uint4*>(dz - lead)[v] = Chunk<T>::gradient(reinterpret_cast<const uint4*>(buf)[v], f.base, p.c, a);
+    auto one = [&](int e) { dz[e] = from_f<T>(a * ex2((to_f<T>(buf[lead + e]) - f.base) * p.c)); };
+    if (WIDE && v0 <= v1) {
+      if (lead && lane < VEC - lead) one(lane);
+      const int e = v1 * VEC - lead + lane;
+      if (e < p.classes) one(e);
+    } else {
+      for (int e = lane; e < p.classes; e += 32) one(e);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kHeld; i++)
+      if (h.id[i] >= 0 && prob[i] >= 0.0f)
+        dz[h.id[i]] = from_f<T>(f.entry(to_f<T>(buf[lead + h.id[i]]), prob[i], teacher.inv));
+    __syncwarp();  // the row's place and the bits are free
   }
+  copy_wait<0>();
 }
 
-template <typename T, int VEC>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) distill_back_block_kernel(const DistillParams p) {
   constexpr int kBits = 32768;
-  __shared__ int id[kMaxTop];
-  __shared__ float prob[kMaxTop], total[kMaxTop];
-  __shared__ uint32_t seen[kBits / 32];
-  __shared__ double red[kThreads / 32];
+  __shared__ uint32_t seen[2][kBits / 32];
+  __shared__ int ids[kMaxTop];
+  __shared__ float probs[kMaxTop];
+  __shared__ float red_t[kWarps];
+  __shared__ double red_e[kWarps];
   const int64_t r = blockIdx.x / p.splits;
-  const int rank = (int)(blockIdx.x % p.splits);
+  const int rank = (int)(blockIdx.x % p.splits), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
   const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg), c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
-  const Entries e(p, r);
-  bool some = false;
-  for (int j = threadIdx.x; j < p.k; j += kThreads) some |= e.there(p, j);
-  if (!__syncthreads_or(some)) {
-    zero_row<T, VEC>(static_cast<T*>(p.dz) + r * p.ds + c0, c1 - c0, threadIdx.x, kThreads);
-    return;
+  const T* z = static_cast<const T*>(p.z) + r * p.zs;
+  T* dz = static_cast<T*>(p.dz) + r * p.ds;
+  const Meet meet{seen[0], seen[1], ids, probs, kBits};
+  Held h;
+  h.load(p, r, threadIdx.x, blockDim.x);
+  clear<true>(meet, threadIdx.x, blockDim.x);
+  const bool some = h.settle(p);
+  const float mt = warp_max(h.largest());
+  if (lane == 0) red_t[warp] = mt;
+  if (!__syncthreads_or(some)) return zero_row(dz + c0, c1 - c0, threadIdx.x, blockDim.x);
+  const Teacher teacher(p, r, warp_max(lane < warps ? red_t[lane] : -kInf));
+  float prob[kHeld], zh[kHeld];
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) {
+    // the logits of this block's classes, before they may be written over
+    zh[i] = h.id[i] >= c0 && h.id[i] < c1 ? to_f<T>(z[h.id[i]]) : 0.0f;
+    prob[i] = h.id[i] >= 0 ? exp_of(teacher.at(h.t[i])) : 0.0f;
+    sum += prob[i];
   }
-  const EntryStore s{id, prob, total, seen, kBits};
-  const double sum = load_entries<true>(p, e, r, s, threadIdx.x, kThreads, red);
-  back_row<T, VEC, true>(p, r, c0, c1, s, threadIdx.x, kThreads, sum);
+  sum = warp_sum(sum);
+  if (lane == 0) red_e[warp] = sum;
+  __syncthreads();
+  sum = red_e[0];
+  for (int w = 1; w < warps; w++) sum += red_e[w];
+  if (!p.whole) {
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) prob[i] = (float)(prob[i] / sum);
+    sum = 1.0;
+  }
+  join_equal<true>(meet, h, prob, p.k, threadIdx.x, blockDim.x);  // with a barrier: all logits are gathered
+  const Factors f(p, r, sum);
+  float entry[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) entry[i] = f.entry(zh[i], prob[i], teacher.inv);
+  row_gradient<T, WIDE>(z + c0, dz + c0, c1 - c0, f.base, p.c, (float)(f.g * f.scale));
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (h.id[i] >= c0 && h.id[i] < c1 && prob[i] >= 0.0f) dz[h.id[i]] = from_f<T>(entry[i]);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
 
-// Blocks to a row, so that few rows still fill the device: `most` of them, of 4,096 classes or more.
-void split_rows(DistillParams& p, int most) {
+// Blocks to a row, so that few rows still fill the device: `most` of them, of 4,096 classes or more. Returns the threads
+// of a block: as many as keep a few 16-byte pieces each, and hold the entries.
+int split_rows(DistillParams& p, int most, int bytes) {
   const int64_t want = (8 * kSmCount + p.rows - 1) / p.rows;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, p.classes / 4096}));
   int pow2 = 1;
   while (2 * pow2 <= p.splits) pow2 *= 2;
   p.splits = pow2;
   p.seg = (int)(((int64_t)p.classes + p.splits - 1) / p.splits + 63) / 64 * 64;
+  return (int64_t)p.seg * bytes <= 16384 && p.k <= kMaxTop / 2 ? kThreads / 2 : kThreads;
 }
 
-unsigned warp_blocks(int64_t rows) {
-  return (unsigned)std::min<int64_t>((rows + kThreads / 32 - 1) / (kThreads / 32), 1 << 20);
-}
+bool warp_rows(const DistillParams& p) { return p.classes <= kWarpClasses && p.k <= kWarpTop; }
+
+// Blocks of warps that go over the rows: four to an SM.
+unsigned warp_blocks(int64_t rows) { return (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 4 * kSmCount); }
 
 template <typename T>
 void forward(DistillParams p, cudaStream_t st) {
-  if (p.classes <= kWarpClasses) {
-    distill_warp_kernel<T><<<warp_blocks(p.rows), kThreads, 0, st>>>(p);
+  if (warp_rows(p)) {
+    p.row_bytes = WarpRow<T>::bytes(p.classes);
+    allow_block_smem<distill_warp_kernel<T>>();
+    distill_warp_kernel<T><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
     KC_CUDA(cudaGetLastError());
     return;
   }
-  split_rows(p, 8);
+  const int threads = split_rows(p, 8, sizeof(T));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * p.splits));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -437,22 +669,24 @@ void forward(DistillParams p, cudaStream_t st) {
   KC_CUDA(cudaLaunchKernelEx(&cfg, distill_block_kernel<T>, p));
 }
 
-template <typename T, int VEC>
+template <typename T, bool WIDE>
 void backward(DistillParams p, cudaStream_t st) {
-  if (p.classes <= kWarpClasses && p.k <= kWarpTop) {
-    distill_back_warp_kernel<T, VEC><<<warp_blocks(p.rows), kThreads, 0, st>>>(p);
+  if (warp_rows(p)) {
+    p.row_bytes = WarpRow<T>::bytes(p.classes);
+    allow_block_smem<distill_back_warp_kernel<T, WIDE>>();
+    distill_back_warp_kernel<T, WIDE><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
   } else {
-    split_rows(p, 256);
-    distill_back_block_kernel<T, VEC><<<(unsigned)(p.rows * p.splits), kThreads, 0, st>>>(p);
+    const int threads = split_rows(p, 256, sizeof(T));
+    distill_back_block_kernel<T, WIDE><<<(unsigned)(p.rows * p.splits), threads, 0, st>>>(p);
   }
   KC_CUDA(cudaGetLastError());
 }
 
 template <typename T>
 void run_backward(const DistillParams& p, cudaStream_t st) {
-  // vectors where a row's logits and gradient are equally far from 16 bytes
+  // 16-byte pieces where a row's logits and gradient are equally far from them
   const bool wide = ((uintptr_t)p.z - (uintptr_t)p.dz) % 16 == 0 && (p.rows == 1 || (p.zs - p.ds) * (int64_t)sizeof(T) % 16 == 0);
-  wide ? backward<T, 16 / sizeof(T)>(p, st) : backward<T, 1>(p, st);
+  wide ? backward<T, true>(p, st) : backward<T, false>(p, st);
 }
 
 Rows logit_rows(const kc_distill_desc& d, const void* p, int64_t stride) {

@@ -201,7 +201,7 @@ void launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, 
 constexpr int kSmCount = 148;
 constexpr int kMaxBlockSmem = 227 * 1024;
 
-// Lets a kernel take more than 48 KB of shared memory, once per device.
+// Lets a kernel take all of a block's shared memory, once per device.
 template <auto kernel>
 void allow_block_smem() {
   static std::atomic<uint64_t> allowed[2];
@@ -209,7 +209,10 @@ void allow_block_smem() {
   KC_CUDA(cudaGetDevice(&dev));
   if (dev >= 128) fail(KC_ERR_INVALID, "CUDA backend: device index above 127");
   if (allowed[dev / 64].load(std::memory_order_acquire) >> (dev % 64) & 1) return;
-  KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlockSmem - 2048));
+  cudaFuncAttributes attr;
+  KC_CUDA(cudaFuncGetAttributes(&attr, kernel));
+  KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kMaxBlockSmem - (int)attr.sharedSizeBytes));
   KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
 }
