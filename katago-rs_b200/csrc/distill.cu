@@ -30,10 +30,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeld = 4;            // entries of a thread
-constexpr int kWarpClasses = 2048;  // rows up to this long, with up to 32 kHeld entries, are a warp's
-constexpr int kWarpTop = 32 * kHeld;
-constexpr int kMaxTop = kThreads * kHeld;
+constexpr int kMostHeld = 4;        // entries of a thread (kernels are built for 1, 2 and 4)
+constexpr int kWarpClasses = 2048;  // rows up to this long, with up to 32 kMostHeld entries, are a warp's
+constexpr int kWarpTop = 32 * kMostHeld;
+constexpr int kMaxTop = kThreads * kMostHeld;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -51,7 +51,7 @@ struct DistillParams {
   int classes, k;
   int splits, seg;  // blocks of a row, classes of each
   int row_bytes;    // of a warp's row in shared memory
-  double temperature;
+  double temperature, inv;
   float c;          // log2(e) / T
 };
 
@@ -150,12 +150,13 @@ __device__ __forceinline__ int lead_of(const T* p) {
 
 // ---- the teacher's entries ---------------------------------------------------------------------------------------
 // Entry thread + i threads of a row in register i; id -1 and logit -inf where there is none.
+template <int HELD>
 struct Held {
-  int id[kHeld];
-  float t[kHeld];
+  int id[HELD];
+  float t[HELD];
   __device__ __forceinline__ void load(const DistillParams& p, int64_t r, int thread, int threads) {
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
+    for (int i = 0; i < HELD; i++) {
       const int j = thread + i * threads;
       id[i] = -1;
       t[i] = -kInf;
@@ -169,7 +170,7 @@ struct Held {
   __device__ __forceinline__ bool settle(const DistillParams& p) {
     bool some = false;
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
+    for (int i = 0; i < HELD; i++) {
       if (id[i] < 0 || id[i] >= p.classes || t[i] == -kInf) {
         id[i] = -1;
         t[i] = -kInf;
@@ -181,7 +182,7 @@ struct Held {
   __device__ __forceinline__ float largest() const {
     float m = t[0];
 #pragma unroll
-    for (int i = 1; i < kHeld; i++) m = fmaxf(m, t[i]);
+    for (int i = 1; i < HELD; i++) m = fmaxf(m, t[i]);
     return m;
   }
 };
@@ -189,19 +190,18 @@ struct Held {
 // The entries' exponentials: of (t - largest) / T, or with the teacher's own log sum the probabilities themselves.
 struct Teacher {
   double shift, inv;  // exp(t inv - shift)
-  __device__ __forceinline__ Teacher(const DistillParams& p, int64_t r, float largest) {
-    inv = 1.0 / p.temperature;
-    shift = p.whole ? (double)__ldg(p.whole + r) : largest * inv;
-  }
+  __device__ __forceinline__ Teacher(const DistillParams& p, int64_t r, float largest)
+      : shift(p.whole ? (double)__ldg(p.whole + r) : largest * p.inv), inv(p.inv) {}
   __device__ __forceinline__ double at(float t) const { return t * inv - shift; }
 };
 
 // A thread's share of sum e and of sum e x, where z are the entries' logits.
-__device__ __forceinline__ void loss_terms(const Held& h, const Teacher& teacher, const float (&z)[kHeld], float m,
+template <int HELD>
+__device__ __forceinline__ void loss_terms(const Held<HELD>& h, const Teacher& teacher, const float (&z)[HELD], float m,
                                            double& se, double& sex) {
   se = sex = 0.0;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) {
+  for (int i = 0; i < HELD; i++) {
     if (h.id[i] < 0) continue;
     const double x = teacher.at(h.t[i]);
     const double e = exp_of(x);
@@ -225,7 +225,7 @@ __device__ __forceinline__ void write_nothing(const DistillParams& p, int64_t r)
 template <typename T>
 struct WarpRow {
   static constexpr int VEC = 16 / sizeof(T);
-  static int bytes(int classes) { return (int)((classes * sizeof(T) + 30) / 16 * 16); }
+  static int bytes(int64_t classes) { return (int)std::min<int64_t>((classes * (int)sizeof(T) + 30) / 16 * 16, 1 << 16); }
   T* buf;
   __device__ __forceinline__ static int pieces(int lead, int classes) { return (lead + classes + VEC - 1) / VEC; }
   __device__ __forceinline__ void fetch(const T* z, int classes, int lane) const {
@@ -241,22 +241,27 @@ struct WarpRow {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_warp_kernel(const DistillParams p) {
+template <typename T, int HELD>
+__global__ void __launch_bounds__(kThreads, HELD == 1 ? 4 : 3) distill_warp_kernel(const DistillParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   auto row = [&](int turn) { return WarpRow<T>{reinterpret_cast<T*>(smem + (warp * 2 + turn) * p.row_bytes)}; };
   const int64_t step = (int64_t)gridDim.x * kWarps;
   int64_t r = (int64_t)blockIdx.x * kWarps + warp;
   const T* z = static_cast<const T*>(p.z);
-  Held next, later;  // the next row's entries, and those of the one behind it on their way
+  Held<HELD> next, later;  // the next row's entries, and those of the one behind it on their way
   next.load(p, r, lane, 32);
   bool some_next = __any_sync(0xffffffffu, next.settle(p));
   if (some_next) row(0).fetch(z + r * p.zs, p.classes, lane);
   copy_commit();
   later.load(p, r + step, lane, 32);
+  // lane i keeps what the loss of the i-th of 32 rows is made of; they are written together
+  int64_t own_r = -1;
+  double own_se = 1.0, own_sex = 0.0;
+  Peak own{0.0f, 0.0f};
+  int kept = 0;
   for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
-    const Held h = next;
+    const Held<HELD> h = next;
     const bool some = some_next;
     next = later;
     some_next = __any_sync(0xffffffffu, next.settle(p));
@@ -273,23 +278,29 @@ __global__ void __launch_bounds__(kThreads) distill_warp_kernel(const DistillPar
     const WarpRow<T> at = row(turn);
     at.close(lead, p.classes, lane);
     const uint4* piece = reinterpret_cast<const uint4*>(at.buf);
-    float m = -kInf, zh[kHeld];
+    float m = -kInf, zh[HELD];
     for (int v = lane; v < n; v += 32) m = fmaxf(m, Chunk<T>::largest(piece[v]));
     m = warp_max(m);
     const float base = base_of(m);
     f32x2 s2 = {0.0f, 0.0f};
     for (int v = lane; v < n; v += 32) s2 = add2(s2, Chunk<T>::sum(piece[v], base, p.c));
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) zh[i] = h.id[i] >= 0 ? to_f<T>(at.buf[lead + h.id[i]]) : 0.0f;
-    const Teacher teacher(p, r, warp_max(h.largest()));
+    for (int i = 0; i < HELD; i++) zh[i] = h.id[i] >= 0 ? to_f<T>(at.buf[lead + h.id[i]]) : 0.0f;
+    const Teacher teacher(p, r, p.whole ? 0.0f : warp_max(h.largest()));
     double se, sex;
     loss_terms(h, teacher, zh, m, se, sex);
     const float s = warp_sum(s2.x + s2.y);
     se = warp_sum(se);
     sex = warp_sum(sex);
-    if (lane == 0) write_loss(p, r, se, sex, {m, s});
+    if (lane == kept) own_r = r, own_se = se, own_sex = sex, own = {m, s};
+    if (++kept == 32) {
+      write_loss(p, own_r, own_se, own_sex, own);
+      own_r = -1;
+      kept = 0;
+    }
     __syncwarp();  // the row's place is free
   }
+  if (own_r >= 0) write_loss(p, own_r, own_se, own_sex, own);
   copy_wait<0>();
 }
 
@@ -332,24 +343,24 @@ __device__ __forceinline__ Peak row_peak(const T* z, int n, float c) {
 }
 
 // A block, or a cluster of `splits` blocks, to a row; the first of them has the entries.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_block_kernel(const DistillParams p) {
+template <typename T, int HELD>
+__global__ void __launch_bounds__(kThreads, 4) distill_block_kernel(const DistillParams p) {
   __shared__ Peak red[kWarps];
   __shared__ float red_t[kWarps];
   __shared__ double red_e[kWarps], red_x[kWarps];
   __shared__ Peak share;
   const int64_t r = blockIdx.x / p.splits;
   const int rank = blockIdx.x % p.splits, lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
-  Held h;
+  Held<HELD> h;
   h.load(p, r, threadIdx.x, blockDim.x);
   if (!__syncthreads_or(h.settle(p))) {  // all blocks of the row see the same
     if (rank == 0 && threadIdx.x == 0) write_nothing(p, r);
     return;
   }
   const T* z = static_cast<const T*>(p.z) + r * p.zs;
-  float zh[kHeld];
+  float zh[HELD];
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) zh[i] = rank == 0 && h.id[i] >= 0 ? to_f<T>(z[h.id[i]]) : 0.0f;
+  for (int i = 0; i < HELD; i++) zh[i] = rank == 0 && h.id[i] >= 0 ? to_f<T>(z[h.id[i]]) : 0.0f;
   const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg), c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
   Peak a = warp_peak(row_peak(z + c0, c1 - c0, p.c), p.c);
   const float mt = warp_max(h.largest());
@@ -412,12 +423,12 @@ __device__ __forceinline__ void clear(const Meet& s, int thread, int threads) {
 
 // `prob` of the first entry of a class becomes the sum over all of that class in their order, those of the others
 // negative. The bits are clear.
-template <bool BLOCK>
-__device__ __forceinline__ void join_equal(const Meet& s, const Held& h, float (&prob)[kHeld], int k, int thread,
+template <bool BLOCK, int HELD>
+__device__ __forceinline__ void join_equal(const Meet& s, const Held<HELD>& h, float (&prob)[HELD], int k, int thread,
                                            int threads) {
   bool again = false;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) {
+  for (int i = 0; i < HELD; i++) {
     if (h.id[i] < 0) continue;
     const uint32_t b = (uint32_t)h.id[i] & (s.bits - 1), bit = 1u << b % 32;
     if (atomicOr(&s.seen[b / 32], bit) & bit) {
@@ -427,11 +438,11 @@ __device__ __forceinline__ void join_equal(const Meet& s, const Held& h, float (
   }
   if (!any_rows<BLOCK>(again)) return;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++)
+  for (int i = 0; i < HELD; i++)
     if (thread + i * threads < k) s.id[thread + i * threads] = h.id[i], s.p[thread + i * threads] = prob[i];
   sync_rows<BLOCK>();
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) {
+  for (int i = 0; i < HELD; i++) {
     if (h.id[i] < 0) continue;
     const uint32_t b = (uint32_t)h.id[i] & (s.bits - 1);
     if (!(s.twice[b / 32] >> b % 32 & 1)) continue;
@@ -497,8 +508,8 @@ struct Factors {
   }
 };
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const DistillParams p) {
+template <typename T, bool WIDE, int HELD>
+__global__ void __launch_bounds__(kThreads, HELD == 1 ? 4 : 3) distill_back_warp_kernel(const DistillParams p) {
   constexpr int VEC = 16 / sizeof(T), WORDS = kWarpClasses / 32;
   __shared__ uint32_t seen[kWarps][2][WORDS];
   __shared__ int ids[kWarps][kWarpTop];
@@ -510,14 +521,14 @@ __global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const Disti
   const int64_t step = (int64_t)gridDim.x * kWarps;
   int64_t r = (int64_t)blockIdx.x * kWarps + warp;
   const T* z = static_cast<const T*>(p.z);
-  Held next, later;
+  Held<HELD> next, later;
   next.load(p, r, lane, 32);
   bool some_next = __any_sync(0xffffffffu, next.settle(p));
   if (some_next) row(0).fetch(z + r * p.zs, p.classes, lane);
   copy_commit();
   later.load(p, r + step, lane, 32);
   for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
-    const Held h = next;
+    const Held<HELD> h = next;
     const bool some = some_next;
     next = later;
     some_next = __any_sync(0xffffffffu, next.settle(p));
@@ -530,18 +541,18 @@ __global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const Disti
       continue;
     }
     clear<false>(meet, lane, 32);
-    const Teacher teacher(p, r, warp_max(h.largest()));
-    float prob[kHeld];
+    const Teacher teacher(p, r, p.whole ? 0.0f : warp_max(h.largest()));
+    float prob[HELD];
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
+    for (int i = 0; i < HELD; i++) {
       prob[i] = h.id[i] >= 0 ? exp_of(teacher.at(h.t[i])) : 0.0f;
       sum += prob[i];
     }
     sum = warp_sum(sum);
     if (!p.whole) {
 #pragma unroll
-      for (int i = 0; i < kHeld; i++) prob[i] = (float)(prob[i] / sum);
+      for (int i = 0; i < HELD; i++) prob[i] = (float)(prob[i] / sum);
       sum = 1.0;
     }
     __syncwarp();
@@ -566,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const Disti
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kHeld; i++)
+    for (int i = 0; i < HELD; i++)
       if (h.id[i] >= 0 && prob[i] >= 0.0f)
         dz[h.id[i]] = from_f<T>(f.entry(to_f<T>(buf[lead + h.id[i]]), prob[i], teacher.inv));
     __syncwarp();  // the row's place and the bits are free
@@ -574,8 +585,8 @@ __global__ void __launch_bounds__(kThreads) distill_back_warp_kernel(const Disti
   copy_wait<0>();
 }
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) distill_back_block_kernel(const DistillParams p) {
+template <typename T, bool WIDE, int HELD>
+__global__ void __launch_bounds__(kThreads, 4) distill_back_block_kernel(const DistillParams p) {
   constexpr int kBits = 32768;
   __shared__ uint32_t seen[2][kBits / 32];
   __shared__ int ids[kMaxTop];
@@ -588,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) distill_back_block_kernel(const Dist
   const T* z = static_cast<const T*>(p.z) + r * p.zs;
   T* dz = static_cast<T*>(p.dz) + r * p.ds;
   const Meet meet{seen[0], seen[1], ids, probs, kBits};
-  Held h;
+  Held<HELD> h;
   h.load(p, r, threadIdx.x, blockDim.x);
   clear<true>(meet, threadIdx.x, blockDim.x);
   const bool some = h.settle(p);
@@ -596,10 +607,10 @@ __global__ void __launch_bounds__(kThreads) distill_back_block_kernel(const Dist
   if (lane == 0) red_t[warp] = mt;
   if (!__syncthreads_or(some)) return zero_row(dz + c0, c1 - c0, threadIdx.x, blockDim.x);
   const Teacher teacher(p, r, warp_max(lane < warps ? red_t[lane] : -kInf));
-  float prob[kHeld], zh[kHeld];
+  float prob[HELD], zh[HELD];
   double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) {
+  for (int i = 0; i < HELD; i++) {
     // the logits of this block's classes, before they may be written over
     zh[i] = h.id[i] >= c0 && h.id[i] < c1 ? to_f<T>(z[h.id[i]]) : 0.0f;
     prob[i] = h.id[i] >= 0 ? exp_of(teacher.at(h.t[i])) : 0.0f;
@@ -612,18 +623,18 @@ __global__ void __launch_bounds__(kThreads) distill_back_block_kernel(const Dist
   for (int w = 1; w < warps; w++) sum += red_e[w];
   if (!p.whole) {
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) prob[i] = (float)(prob[i] / sum);
+    for (int i = 0; i < HELD; i++) prob[i] = (float)(prob[i] / sum);
     sum = 1.0;
   }
   join_equal<true>(meet, h, prob, p.k, threadIdx.x, blockDim.x);  // with a barrier: all logits are gathered
   const Factors f(p, r, sum);
-  float entry[kHeld];
+  float entry[HELD];
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) entry[i] = f.entry(zh[i], prob[i], teacher.inv);
+  for (int i = 0; i < HELD; i++) entry[i] = f.entry(zh[i], prob[i], teacher.inv);
   row_gradient<T, WIDE>(z + c0, dz + c0, c1 - c0, f.base, p.c, (float)(f.g * f.scale));
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kHeld; i++)
+  for (int i = 0; i < HELD; i++)
     if (h.id[i] >= c0 && h.id[i] < c1 && prob[i] >= 0.0f) dz[h.id[i]] = from_f<T>(entry[i]);
 }
 
@@ -646,16 +657,14 @@ bool warp_rows(const DistillParams& p) { return p.classes <= kWarpClasses && p.k
 // Blocks of warps that go over the rows: four to an SM.
 unsigned warp_blocks(int64_t rows) { return (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 4 * kSmCount); }
 
-template <typename T>
-void forward(DistillParams p, cudaStream_t st) {
+template <typename T, int HELD>
+void forward_held(const DistillParams& p, int threads, cudaStream_t st) {
   if (warp_rows(p)) {
-    p.row_bytes = WarpRow<T>::bytes(p.classes);
-    allow_block_smem<distill_warp_kernel<T>>();
-    distill_warp_kernel<T><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
+    allow_block_smem<distill_warp_kernel<T, HELD>>();
+    distill_warp_kernel<T, HELD><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
     KC_CUDA(cudaGetLastError());
     return;
   }
-  const int threads = split_rows(p, 8, sizeof(T));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * p.splits));
   cfg.blockDim = dim3(threads);
@@ -666,20 +675,36 @@ void forward(DistillParams p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  KC_CUDA(cudaLaunchKernelEx(&cfg, distill_block_kernel<T>, p));
+  KC_CUDA(cudaLaunchKernelEx(&cfg, distill_block_kernel<T, HELD>, p));
+}
+
+template <typename T, bool WIDE, int HELD>
+void backward_held(const DistillParams& p, int threads, cudaStream_t st) {
+  if (warp_rows(p)) {
+    allow_block_smem<distill_back_warp_kernel<T, WIDE, HELD>>();
+    distill_back_warp_kernel<T, WIDE, HELD><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
+  } else {
+    distill_back_block_kernel<T, WIDE, HELD><<<(unsigned)(p.rows * p.splits), threads, 0, st>>>(p);
+  }
+  KC_CUDA(cudaGetLastError());
+}
+
+template <typename T>
+void forward(DistillParams p, cudaStream_t st) {
+  p.row_bytes = WarpRow<T>::bytes(p.classes);
+  const int threads = warp_rows(p) ? 32 : split_rows(p, 8, sizeof(T));
+  if (p.k <= threads) forward_held<T, 1>(p, threads, st);
+  else if (p.k <= 2 * threads) forward_held<T, 2>(p, threads, st);
+  else forward_held<T, 4>(p, threads, st);
 }
 
 template <typename T, bool WIDE>
 void backward(DistillParams p, cudaStream_t st) {
-  if (warp_rows(p)) {
-    p.row_bytes = WarpRow<T>::bytes(p.classes);
-    allow_block_smem<distill_back_warp_kernel<T, WIDE>>();
-    distill_back_warp_kernel<T, WIDE><<<warp_blocks(p.rows), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
-  } else {
-    const int threads = split_rows(p, 256, sizeof(T));
-    distill_back_block_kernel<T, WIDE><<<(unsigned)(p.rows * p.splits), threads, 0, st>>>(p);
-  }
-  KC_CUDA(cudaGetLastError());
+  p.row_bytes = WarpRow<T>::bytes(p.classes);
+  const int threads = warp_rows(p) ? 32 : split_rows(p, 256, sizeof(T));
+  if (p.k <= threads) backward_held<T, WIDE, 1>(p, threads, st);
+  else if (p.k <= 2 * threads) backward_held<T, WIDE, 2>(p, threads, st);
+  else backward_held<T, WIDE, 4>(p, threads, st);
 }
 
 template <typename T>
@@ -719,6 +744,7 @@ DistillParams params_of(const kc_distill_desc& d) {
   p.ds = d.rows > 1 ? d.dlogits_stride : 0;
   p.ts = d.rows > 1 ? d.top_stride : 0;
   p.temperature = d.temperature;
+  p.inv = 1.0 / p.temperature;
   p.c = kLog2e / d.temperature;
   return p;
 }
