@@ -98,6 +98,10 @@ template <typename T>
 struct Chunk {
   static constexpr int VEC = 16 / sizeof(T), N = VEC / 2;
   using V = RowVec<T, VEC>;
+  __device__ static __forceinline__ uint4 nothing() {  // elements of -inf
+    const uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+  }
   __device__ static __forceinline__ float largest(const uint4& r) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
     if constexpr (std::is_same<T, float>::value) {
@@ -318,21 +322,16 @@ __device__ __forceinline__ Peak row_peak(const T* z, int n, float c) {
   };
   const int lead = lead_of(z), head = min(n, lead ? VEC - lead : 0), pieces = (n - head) / VEC, threads = blockDim.x;
   const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-  int v = threadIdx.x;
-  for (; v + 3 * threads < pieces; v += 4 * threads) {
+  for (int v = threadIdx.x; v < pieces; v += 4 * threads) {
     uint4 raw[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) raw[i] = zv[v + i * threads];
+    for (int i = 0; i < 4; i++) raw[i] = v + i * threads < pieces ? zv[v + i * threads] : Chunk<T>::nothing();
     const float base = raise(fmaxf(fmaxf(Chunk<T>::largest(raw[0]), Chunk<T>::largest(raw[1])),
                                    fmaxf(Chunk<T>::largest(raw[2]), Chunk<T>::largest(raw[3]))));
     f32x2 s = Chunk<T>::sum(raw[0], base, c);
 #pragma unroll
-    for (int i = 1; i < 4; i++) s = add2(s, Chunk<T>::sum(raw[i], base, c));
-    a.s += s.x + s.y;
-  }
-  for (; v < pieces; v += threads) {
-    const uint4 raw = zv[v];
-    const f32x2 s = Chunk<T>::sum(raw, raise(Chunk<T>::largest(raw)), c);
+    for (int i = 1; i < 4; i++)
+      if (v + i * threads < pieces) s = add2(s, Chunk<T>::sum(raw[i], base, c));
     a.s += s.x + s.y;
   }
   for (int i = threadIdx.x; i < n - pieces * VEC; i += threads) {
@@ -469,15 +468,15 @@ __device__ __forceinline__ void row_gradient(const T* z, T* dz, int n, float bas
     pieces = (n - head) / VEC;
     const uint4* zv = reinterpret_cast<const uint4*>(z + head);
     uint4* dv = reinterpret_cast<uint4*>(dz + head);
-    int v = threadIdx.x;
-    for (; v + 3 * threads < pieces; v += 4 * threads) {
+    for (int v = threadIdx.x; v < pieces; v += 4 * threads) {
       uint4 raw[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) raw[i] = zv[v + i * threads];
+      for (int i = 0; i < 4; i++)
+        if (v + i * threads < pieces) raw[i] = zv[v + i * threads];
 #pragma unroll
-      for (int i = 0; i < 4; i++) dv[v + i * threads] = Chunk<T>::gradient(raw[i], base, c, a);
+      for (int i = 0; i < 4; i++)
+        if (v + i * threads < pieces) dv[v + i * threads] = Chunk<T>::gradient(raw[i], base, c, a);
     }
-    for (; v < pieces; v += threads) dv[v] = Chunk<T>::gradient(zv[v], base, c, a);
   }
   for (int i = threadIdx.x; i < n - pieces * VEC; i += threads) {
     const int at = i < head ? i : i + pieces * VEC;
