@@ -23,11 +23,13 @@ namespace {
 [[noreturn]] void bad(const std::string& what) { fail(KC_ERR_INVALID, "CUDA backend: looked-up rows: " + what); }
 
 constexpr int kThreads = 256;
-constexpr int kSortThreads = 512;
+constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kMaxBits = 9;          // of a digit: no more digits than threads; 16 warps x 512 counts are 32 KB
+constexpr int kMaxBits = 9;          // of a digit: no more digits than threads; 32 warps x 512 counts are 64 KB
 constexpr int kTile = 2048;          // tokens of a block of the sort, at least
-constexpr int kUnroll = 8;           // tokens whose rows a lane has in flight
+constexpr int kClusterTokens = 1 << 19;  // sorted in one launch by a cluster of up to 16 blocks
+constexpr int kRounds = 8;           // entries of a lane of the sort that stay in registers between its two passes
+constexpr int kUnroll = 4;           // tokens whose rows a lane has in flight
 
 struct EmbedParams {
   const int32_t* ids;
@@ -92,8 +94,8 @@ struct SortParams {
 };
 
 __device__ __forceinline__ int2 sort_entry(const SortParams& p, int i) {
-  if (!p.ids) return p.in[i];
-  const int id = p.ids[i];
+  if (!p.ids) return __ldcg(p.in + i);  // other blocks' of the cluster
+  const int id = __ldg(p.ids + i);
   return make_int2(id >= 0 && id < p.rows ? id : p.rows, i);
 }
 
@@ -115,34 +117,75 @@ __global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortPar
 }
 
 // Places the tile's entries. Each warp owns a share of consecutive entries: it counts its digits, takes its places
-// behind those of the tiles and warps before it, and goes over them again.
-__device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* count, int* scan) {
+// behind those of the tiles and warps before it, and goes over them again. The tiles' counts are in p.hist; a cluster with
+// a block to each tile exchanges them (`totals`, [tiles][bins]).
+template <bool CLUSTER>
+__device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* count, int* scan, int* totals) {
   const int bins = 1 << p.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) count[b] = 0;
+  for (int b = threadIdx.x; b < kSortWarps * bins / 4; b += kSortThreads)
+    reinterpret_cast<int4*>(count)[b] = make_int4(0, 0, 0, 0);
   __syncthreads();
   const int i0 = tile * p.tile, i1 = min(p.tokens, i0 + p.tile);
-  const int share = ((i1 - i0 + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int share = ((max(i1 - i0, 0) + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
   const int w0 = i0 + warp * share, w1 = min(i1, w0 + share);
   int* mine = count + warp * bins;
-  for (int i = w0 + lane; i - lane < w1; i += 32) {
-    const int d = i < w1 ? sort_entry(p, i).x >> p.shift & (bins - 1) : bins;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    if (d < bins && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+  // an entry's place among those of its digit in the warp's share; a share of few rounds keeps its entries and places
+  auto place = [&](int d) {
+    // the lanes with this digit, a bit at a time (a match instruction takes an SM about 40 cycles: 92,416 tokens, 9 bits
+    // 17.7 us)
+    uint32_t peers = __ballot_sync(0xffffffffu, d < bins);
+    for (int b = 0; b < p.bits; b++) {
+      const uint32_t ones = __ballot_sync(0xffffffffu, d >> b & 1);
+      peers &= d >> b & 1 ? ones : ~ones;
+    }
+    int n = 0;
+    if (d < bins) n = mine[d];
     __syncwarp();
+    if (d < bins && lane == __ffs(peers) - 1) mine[d] = n + __popc(peers);
+    __syncwarp();
+    return n + __popc(peers & ((1u << lane) - 1));
+  };
+  auto digit = [&](int key, int i) { return i < w1 ? key >> p.shift & (bins - 1) : bins; };
+  const bool kept = share <= 32 * kRounds;
+  int2 e[kRounds];
+  int at_digit[kRounds];
+  for (int j = w0 + lane; j - lane < w1; j += 32 * kRounds) {
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry(p, j + 32 * k) : make_int2(0, 0);
+#pragma unroll
+    for (int k = 0; k < kRounds; k++)
+      if (j - lane + 32 * k < w1) at_digit[k] = place(digit(e[k].x, j + 32 * k));
   }
   __syncthreads();
   // thread b: digit b's places
   int before = 0, total = 0;
-  if (threadIdx.x < bins) {
-    if (p.tiles > 1) {
-#pragma unroll 8
-      for (int t = 0; t < p.tiles; t++) {
-        const int h = p.hist[(size_t)t * bins + threadIdx.x];
-        if (t < tile) before += h;
-        total += h;
-      }
-    } else {
+  if (CLUSTER) {
+    if (threadIdx.x < bins) {
+#pragma unroll
       for (int w = 0; w < kSortWarps; w++) total += count[w * bins + threadIdx.x];
+      if (p.tiles > 1)  // to all blocks of the cluster
+        for (int t = 0; t < p.tiles; t++)
+          asm volatile("st.shared::cluster.u32 [%0], %1;"
+                       ::"r"(mapa_shared(smem_u32(totals + tile * bins + threadIdx.x), t)), "r"(total) : "memory");
+    }
+    if (p.tiles > 1) {
+      cluster_sync();
+      total = 0;
+      if (threadIdx.x < bins) {
+#pragma unroll 8
+        for (int t = 0; t < p.tiles; t++) {
+          const int h = totals[t * bins + threadIdx.x];
+          if (t < tile) before += h;
+          total += h;
+        }
+      }
+    }
+  } else if (threadIdx.x < bins) {
+#pragma unroll 8
+    for (int t = 0; t < p.tiles; t++) {
+      const int h = p.hist[(size_t)t * bins + threadIdx.x];
+      if (t < tile) before += h;
+      total += h;
     }
   }
   // exclusive sums of the totals over the digits
@@ -154,44 +197,57 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   }
   if (lane == 31) scan[warp] = sum;
   __syncthreads();
-  int at = sum - total + before;
-  for (int w = 0; w < warp; w++) at += scan[w];
-  if (threadIdx.x < bins)
+  if (threadIdx.x < bins) {
+    int at = sum - total + before;
+    for (int w = 0; w < warp; w++) at += scan[w];
+#pragma unroll 8
     for (int w = 0; w < kSortWarps; w++) {
       const int n = count[w * bins + threadIdx.x];
       count[w * bins + threadIdx.x] = at;
       at += n;
     }
+  }
   __syncthreads();
-  for (int i = w0 + lane; i - lane < w1; i += 32) {
-    const int2 e = i < w1 ? sort_entry(p, i) : make_int2(0, 0);
-    const int d = i < w1 ? e.x >> p.shift & (bins - 1) : bins;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    if (d < bins) p.out[mine[d] + __popc(peers & ((1u << lane) - 1))] = e;
-    __syncwarp();
-    if (d < bins && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
-    __syncwarp();
+  if (kept) {
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) {
+      const int i = w0 + lane + 32 * k;
+      if (i < w1) p.out[mine[digit(e[k].x, i)] + at_digit[k]] = e[k];
+    }
+    return;
+  }
+  for (int j = w0 + lane; j - lane < w1; j += 32 * kRounds) {
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry(p, j + 32 * k) : make_int2(0, 0);
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) {
+      if (j - lane + 32 * k >= w1) continue;
+      const int n = place(digit(e[k].x, j + 32 * k));
+      if (j + 32 * k < w1) p.out[n] = e[k];
+    }
   }
 }
 
 __global__ void __launch_bounds__(kSortThreads) embed_place_kernel(const SortParams p) {
-  extern __shared__ int count[];
+  extern __shared__ __align__(16) int count[];
   __shared__ int scan[kSortWarps];
   pdl_wait();
   pdl_trigger();
-  place_tile(p, blockIdx.x, count, scan);
+  place_tile<false>(p, blockIdx.x, count, scan, nullptr);
 }
 
-// All passes of a list that one block sorts.
+// All passes of a list that a cluster sorts, a tile to a block.
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p, int passes, int2* a, int2* b) {
-  extern __shared__ int count[];
+  extern __shared__ __align__(16) int count[];
   __shared__ int scan[kSortWarps];
+  int* totals = count + (kSortWarps << p.bits);
   pdl_trigger();
   for (int i = 0; i < passes; i++) {
     p.out = (passes - i) % 2 ? a : b;  // the last pass ends in a
     p.shift = i * p.bits;
-    place_tile(p, 0, count, scan);
-    __syncthreads();
+    place_tile<true>(p, blockIdx.x, count, scan, totals);
+    if (p.tiles > 1) cluster_sync();  // the entries are written, and the totals have been read
+    else __syncthreads();
     p.ids = nullptr;
     p.in = p.out;
   }
@@ -253,7 +309,7 @@ __device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int co
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) embed_sum_kernel(const SumParams p) {
+__global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams p) {
   using V = RowVec<T, VEC>;
   __shared__ float slot[2][kThreads * VEC];  // [first, last][group][lane][VEC]
   __shared__ int key[2][kThreads / 2];
@@ -269,14 +325,22 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(const SumParams p) 
 #pragma unroll
   for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
   int cur = -1, first = -1;  // the run at hand, and the piece's first one once it is over
+  int2 later[kUnroll];  // the next entries, on their way while the rows of these are
+  auto look = [&](int e0) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++)
+      later[u] = e0 < p.piece && i0 + e0 + u < p.tokens ? p.list[i0 + e0 + u] : make_int2(p.rows, 0);
+  };
+  look(0);
   for (int e0 = 0; e0 < p.piece; e0 += kUnroll) {
     int2 e[kUnroll];
     typename V::Raw raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) e[u] = i0 + e0 + u < p.tokens ? p.list[i0 + e0 + u] : make_int2(p.rows, 0);
+    for (int u = 0; u < kUnroll; u++) e[u] = later[u];
 #pragma unroll
     for (int u = 0; u < kUnroll; u++)
       if (here && e[u].x < p.rows) raw[u] = V::load(dy + e[u].y * p.ys);
+    look(e0 + kUnroll);
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
       if (e[u].x != cur) {
@@ -386,9 +450,9 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumParams p)
 
 // Lanes of a row: the widest group that leaves at most an eighth of its lanes idle.
 int lanes_of(int nvec) {
-  for (int lanes = 32; lanes > 2; lanes /= 2)
+  for (int lanes = 32; lanes > 8; lanes /= 2)
     if (((nvec + lanes - 1) / lanes * lanes - nvec) * 8 <= nvec) return lanes;
-  return 2;
+  return 8;
 }
 
 struct SumShape {
@@ -400,15 +464,16 @@ SumShape sum_shape(int64_t tokens, int C, int vec) {
   s.lanes = lanes_of(nvec);
   s.chunks = (nvec + s.lanes - 1) / s.lanes;
   const int groups = kThreads / s.lanes;
-  // four blocks to an SM, of pieces of 16 to 256 entries
+  // four blocks to an SM, of pieces of up to 256 entries
   const int64_t want = (tokens * s.chunks + (int64_t)4 * kSmCount * groups - 1) / ((int64_t)4 * kSmCount * groups);
-  s.piece = (int)std::min<int64_t>(256, std::max<int64_t>(16, (want + kUnroll - 1) / kUnroll * kUnroll));
+  s.piece = (int)std::min<int64_t>(256, std::max<int64_t>(kUnroll, (want + kUnroll - 1) / kUnroll * kUnroll));
   s.blocks = (int)((tokens + (int64_t)s.piece * groups - 1) / ((int64_t)s.piece * groups));
   return s;
 }
 
 struct SortShape {
   int passes, bits, tiles, tile;
+  bool cluster;
 };
 SortShape sort_shape(int64_t tokens, int64_t rows) {
   SortShape s;
@@ -416,8 +481,14 @@ SortShape sort_shape(int64_t tokens, int64_t rows) {
   while (rows >> bits) bits++;
   s.passes = (bits + kMaxBits - 1) / kMaxBits;
   s.bits = (bits + s.passes - 1) / s.passes;
-  s.tiles = (int)std::min<int64_t>(kSmCount, (tokens + kTile - 1) / kTile);
-  s.tile = (int)((tokens + s.tiles - 1) / s.tiles);
+  s.cluster = tokens <= kClusterTokens;
+  if (s.cluster) {
+    s.tiles = 1;
+    while (s.tiles < 16 && (int64_t)s.tiles * kTile < tokens) s.tiles *= 2;
+    s.tile = (int)((tokens + s.tiles - 1) / s.tiles);
+    return s;
+  }
+  s.tile = (int)((tokens + kSmCount - 1) / kSmCount);
   s.tiles = (int)((tokens + s.tile - 1) / s.tile);
   return s;
 }
@@ -440,7 +511,7 @@ Layout layout(const kc_embed_desc& d) {
     if (d.channels % v == 0) blocks = std::max(blocks, sum_shape(d.tokens, d.channels, v).blocks);
   l.a = take((size_t)d.tokens * sizeof(int2));
   if (s.passes > 1) l.b = take((size_t)d.tokens * sizeof(int2));
-  if (s.tiles > 1) l.hist = take(((size_t)s.tiles << s.bits) * sizeof(int));
+  if (!s.cluster) l.hist = take(((size_t)s.tiles << s.bits) * sizeof(int));
   l.part = take((size_t)blocks * 2 * d.channels * sizeof(float));
   l.ids = take((size_t)blocks * sizeof(int2));
   l.total = at;
@@ -451,11 +522,23 @@ void sort_tokens(const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, i
   const SortShape s = sort_shape(d.tokens, d.table_rows);
   SortParams p{ids, nullptr, nullptr, hist, (int)d.tokens, (int)d.table_rows, 0, s.bits, s.tiles, s.tile};
   const size_t smem = ((size_t)kSortWarps << s.bits) * sizeof(int);
-  if (s.tiles == 1) {
-    embed_sort_kernel<<<1, kSortThreads, smem, st>>>(p, s.passes, a, b);
-    KC_CUDA(cudaGetLastError());
+  if (s.cluster) {
+    allow_block_smem<embed_sort_kernel, true>();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(s.tiles);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = smem + ((size_t)s.tiles << s.bits) * sizeof(int);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.tiles;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.tiles > 1 ? 1 : 0;
+    KC_CUDA(cudaLaunchKernelEx(&cfg, embed_sort_kernel, p, s.passes, a, b));
     return;
   }
+  allow_block_smem<embed_place_kernel>();
   for (int i = 0; i < s.passes; i++) {
     p.out = (s.passes - i) % 2 ? a : b;  // the last pass ends in a
     p.shift = i * s.bits;

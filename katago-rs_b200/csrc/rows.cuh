@@ -201,8 +201,8 @@ void launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, 
 constexpr int kSmCount = 148;
 constexpr int kMaxBlockSmem = 227 * 1024;
 
-// Lets a kernel take all of a block's shared memory, once per device.
-template <auto kernel>
+// Lets a kernel take all of a block's shared memory (and clusters of 16 blocks), once per device.
+template <auto kernel, bool CLUSTERS = false>
 void allow_block_smem() {
   static std::atomic<uint64_t> allowed[2];
   int dev = 0;
@@ -214,6 +214,7 @@ void allow_block_smem() {
   KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kMaxBlockSmem - (int)attr.sharedSizeBytes));
   KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (CLUSTERS) KC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   allowed[dev / 64].fetch_or(1ull << (dev % 64), std::memory_order_release);
 }
 
