@@ -27,8 +27,9 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 9;          // of a digit: no more digits than threads; 32 warps x 512 counts are 64 KB
 constexpr int kTile = 2048;          // tokens of a block of the sort, at least
-constexpr int kClusterTokens = 1 << 19;  // sorted in one launch by a cluster of up to 16 blocks
 constexpr int kRounds = 8;           // entries of a lane of the sort that stay in registers between its two passes
+// Sorted in one launch by a cluster of up to 16 blocks; more by two launches a digit over all SMs.
+constexpr int kClusterTokens = 16 * kSortThreads * kRounds;
 constexpr int kUnroll = 4;           // tokens whose rows a lane has in flight
 
 struct EmbedParams {
@@ -131,12 +132,14 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   int* mine = count + warp * bins;
   // an entry's place among those of its digit in the warp's share; a share of few rounds keeps its entries and places
   auto place = [&](int d) {
-    // the lanes with this digit, a bit at a time (a match instruction takes an SM about 40 cycles: 92,416 tokens, 9 bits
-    // 17.7 us)
+    // the lanes with this digit, a bit at a time
     uint32_t peers = __ballot_sync(0xffffffffu, d < bins);
-    for (int b = 0; b < p.bits; b++) {
-      const uint32_t ones = __ballot_sync(0xffffffffu, d >> b & 1);
-      peers &= d >> b & 1 ? ones : ~ones;
+#pragma unroll
+    for (int b = 0; b < kMaxBits; b++) {
+      if (b >= p.bits) break;
+      const bool one = d >> b & 1;
+      const uint32_t ones = __ballot_sync(0xffffffffu, one);
+      peers &= one ? ones : ~ones;
     }
     int n = 0;
     if (d < bins) n = mine[d];
@@ -488,7 +491,9 @@ SortShape sort_shape(int64_t tokens, int64_t rows) {
     s.tile = (int)((tokens + s.tiles - 1) / s.tiles);
     return s;
   }
-  s.tile = (int)((tokens + kSmCount - 1) / kSmCount);
+  // few tiles, so that a block soon has all their counts, of few entries, which go out one 32-byte sector each (400,000
+  // tokens, 17 bits: 79 us in all with a tile to each SM, 74 us in tiles of 8,192; 300,000, 2 bits: 52 and 57 us)
+  s.tile = (int)std::max<int64_t>(2 * kTile, (tokens + kSmCount - 1) / kSmCount);
   s.tiles = (int)((tokens + s.tile - 1) / s.tile);
   return s;
 }
