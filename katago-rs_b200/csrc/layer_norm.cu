@@ -126,20 +126,21 @@ struct Ring {
   int64_t next;       // the row to copy next
   float next_mask;    // looked at a row later, when it has arrived
   uint32_t on = 0;    // a bit for each stage
-  uint32_t high[TENSORS] = {};  // a bit for each stage: the row begins in the upper half of 4 bytes
+  // a bit for each stage: the thread's elements (its lanes are an even number apart) are the upper halves of 4 bytes
+  uint32_t high[TENSORS] = {};
 
   __device__ __forceinline__ Slot* at(int s, int tensor, int i) const {
-    return mine + ((s * TENSORS + tensor) * NV + i) * blockDim.x;
+    return mine + (s * TENSORS * NV + tensor * NV + i) * (BLOCK ? (int)blockDim.x : kThreads);
   }
   __device__ __forceinline__ void look(const LayerParams& p) { next_mask = next < p.rows ? token_mask(p, next) : 0.0f; }
   __device__ __forceinline__ void fetch_row(const T* row, int tensor, const Group<BLOCK>& g, int nvec, int s) {
+    const T* src = row + g.lane * VEC;
     if constexpr (Copy::BYTES == 2)
-      high[tensor] = (high[tensor] & ~(1u << s)) | ((uint32_t)(reinterpret_cast<uintptr_t>(row) >> 1) & 1u) << s;
+      high[tensor] = (high[tensor] & ~(1u << s)) | ((uint32_t)(reinterpret_cast<uintptr_t>(src) >> 1) & 1u) << s;
+    src = Copy::base(src);
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int v = g.lane + i * g.lanes;
-      if (v < nvec) Copy::copy(at(s, tensor, i), row + v * VEC);
-    }
+    for (int i = 0; i < NV; i++, src += g.lanes * VEC)
+      if (g.lane + i * g.lanes < nvec) Copy::copy(at(s, tensor, i), src);
   }
   __device__ __forceinline__ void fetch(const LayerParams& p, const Group<BLOCK>& g, int nvec, int s) {
     const bool next_on = next_mask != 0.0f;
@@ -174,12 +175,12 @@ struct Ring {
       for (int k = 0; k < 2; k++) {
         const int i = 2 * u + k, c = g.lane + i * g.lanes;
         f[0] = 0.0f;
-        if (c < nvec) Copy::unpack(*at(stage, tensor, i), (high[tensor] >> stage ^ (uint32_t)c) & 1u, f);
+        if (c < nvec) Copy::unpack(*at(stage, tensor, i), high[tensor] >> stage & 1, f);
         e[k] = f[0];
       }
       v[0] = {e[0], e[1]};
     } else {
-      Copy::unpack(*at(stage, tensor, u), 0u, f);
+      Copy::unpack(*at(stage, tensor, u), false, f);
 #pragma unroll
       for (int j = 0; j < VEC / 2; j++) v[j] = {f[2 * j], f[2 * j + 1]};
     }

@@ -66,27 +66,31 @@ struct RowVec {
 
 // Copies into shared memory by the thread that reads them there: no barrier, and loads in flight that take no registers.
 // copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived. A single 2-byte
-// element comes with the 4 aligned bytes around it.
+// element comes with the 4 aligned bytes around it (`src` is the address of those: base()).
 template <typename T, int VEC>
 struct RowCopy {
   using V = RowVec<T, VEC>;
   static constexpr int BYTES = V::BYTES;
   using Slot = typename std::conditional<BYTES == 2, uint32_t, typename V::Raw>::type;
+  __device__ static __forceinline__ const T* base(const T* p) {
+    return BYTES == 2 ? reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3) : p;
+  }
   __device__ static __forceinline__ void copy(Slot* dst, const T* src) {
     if constexpr (BYTES == 16)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-    else if constexpr (BYTES == 2)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                   ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)3) : "memory");
     else
       asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
-                   ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+                   ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES == 2 ? 4 : BYTES) : "memory");
   }
-  // `high`: a single 2-byte element was the upper half of its 4 bytes
-  __device__ static __forceinline__ void unpack(const Slot& s, uint32_t high, float (&v)[VEC]) {
+  // `high`: a single 2-byte element is the upper half of its 4 bytes
+  __device__ static __forceinline__ void unpack(const Slot& s, bool high, float (&v)[VEC]) {
     if constexpr (BYTES == 2) {
-      const uint16_t h = (uint16_t)(high ? s >> 16 : s);
-      v[0] = to_f<T>(*reinterpret_cast<const T*>(&h));
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        v[0] = __uint_as_float((high ? s : s << 16) & 0xffff0000u);
+      } else {
+        const uint16_t h = (uint16_t)(high ? s >> 16 : s);
+        v[0] = to_f<T>(*reinterpret_cast<const T*>(&h));
+      }
     } else {
       V::unpack(s, v);
     }
