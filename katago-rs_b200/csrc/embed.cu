@@ -30,6 +30,8 @@ constexpr int kTile = 2048;          // tokens of a block of the sort, at least
 constexpr int kRounds = 8;           // entries of a lane of the sort that stay in registers between its two passes
 // Sorted in one launch by a cluster of up to 16 blocks; more by two launches a digit over all SMs.
 constexpr int kClusterTokens = 16 * kSortThreads * kRounds;
+constexpr int kFewTokens = 2048;     // sorted and summed in one launch, with digits of up to 8 bits
+constexpr int kFewBits = 8;
 constexpr int kUnroll = 4;           // tokens whose rows a lane has in flight
 
 struct EmbedParams {
@@ -94,8 +96,11 @@ struct SortParams {
   int tiles, tile;     // tokens of a tile
 };
 
+enum class SortIn { kTiles, kCluster, kBlock };  // over launches, over a cluster, in a block's shared memory
+
+template <SortIn IN>
 __device__ __forceinline__ int2 sort_entry(const SortParams& p, int i) {
-  if (!p.ids) return __ldcg(p.in + i);  // other blocks' of the cluster
+  if (!p.ids) return IN == SortIn::kBlock ? p.in[i] : __ldcg(p.in + i);  // other blocks' of the cluster
   const int id = __ldg(p.ids + i);
   return make_int2(id >= 0 && id < p.rows ? id : p.rows, i);
 }
@@ -109,7 +114,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortPar
   __syncthreads();
   const int i0 = blockIdx.x * p.tile, i1 = min(p.tokens, i0 + p.tile);
   for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
-    const int d = sort_entry(p, i).x >> p.shift & (bins - 1);
+    const int d = sort_entry<SortIn::kTiles>(p, i).x >> p.shift & (bins - 1);
     const uint32_t peers = __match_any_sync(__activemask(), d);
     if (threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&count[d], __popc(peers));
   }
@@ -120,14 +125,15 @@ __global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortPar
 // Places the tile's entries. Each warp owns a share of consecutive entries: it counts its digits, takes its places
 // behind those of the tiles and warps before it, and goes over them again. The tiles' counts are in p.hist; a cluster with
 // a block to each tile exchanges them (`totals`, [tiles][bins]).
-template <bool CLUSTER>
+template <SortIn IN, int THREADS>
 __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* count, int* scan, int* totals) {
+  constexpr int WARPS = THREADS / 32;
   const int bins = 1 << p.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int b = threadIdx.x; b < kSortWarps * bins / 4; b += kSortThreads)
+  for (int b = threadIdx.x; b < WARPS * bins / 4; b += THREADS)
     reinterpret_cast<int4*>(count)[b] = make_int4(0, 0, 0, 0);
   __syncthreads();
   const int i0 = tile * p.tile, i1 = min(p.tokens, i0 + p.tile);
-  const int share = ((max(i1 - i0, 0) + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int share = ((max(i1 - i0, 0) + WARPS - 1) / WARPS + 31) / 32 * 32;
   const int w0 = i0 + warp * share, w1 = min(i1, w0 + share);
   int* mine = count + warp * bins;
   // an entry's place among those of its digit in the warp's share; a share of few rounds keeps its entries and places
@@ -154,7 +160,7 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   int at_digit[kRounds];
   for (int j = w0 + lane; j - lane < w1; j += 32 * kRounds) {
 #pragma unroll
-    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry(p, j + 32 * k) : make_int2(0, 0);
+    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry<IN>(p, j + 32 * k) : make_int2(0, 0);
 #pragma unroll
     for (int k = 0; k < kRounds; k++)
       if (j - lane + 32 * k < w1) at_digit[k] = place(digit(e[k].x, j + 32 * k));
@@ -162,10 +168,10 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   __syncthreads();
   // thread b: digit b's places
   int before = 0, total = 0;
-  if (CLUSTER) {
+  if (IN != SortIn::kTiles) {
     if (threadIdx.x < bins) {
 #pragma unroll
-      for (int w = 0; w < kSortWarps; w++) total += count[w * bins + threadIdx.x];
+      for (int w = 0; w < WARPS; w++) total += count[w * bins + threadIdx.x];
       if (p.tiles > 1)  // to all blocks of the cluster
         for (int t = 0; t < p.tiles; t++)
           asm volatile("st.shared::cluster.u32 [%0], %1;"
@@ -204,7 +210,7 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
     int at = sum - total + before;
     for (int w = 0; w < warp; w++) at += scan[w];
 #pragma unroll 8
-    for (int w = 0; w < kSortWarps; w++) {
+    for (int w = 0; w < WARPS; w++) {
       const int n = count[w * bins + threadIdx.x];
       count[w * bins + threadIdx.x] = at;
       at += n;
@@ -221,7 +227,7 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   }
   for (int j = w0 + lane; j - lane < w1; j += 32 * kRounds) {
 #pragma unroll
-    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry(p, j + 32 * k) : make_int2(0, 0);
+    for (int k = 0; k < kRounds; k++) e[k] = j + 32 * k < w1 ? sort_entry<IN>(p, j + 32 * k) : make_int2(0, 0);
 #pragma unroll
     for (int k = 0; k < kRounds; k++) {
       if (j - lane + 32 * k >= w1) continue;
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_place_kernel(const SortPar
   __shared__ int scan[kSortWarps];
   pdl_wait();
   pdl_trigger();
-  place_tile<false>(p, blockIdx.x, count, scan, nullptr);
+  place_tile<SortIn::kTiles, kSortThreads>(p, blockIdx.x, count, scan, nullptr);
 }
 
 // All passes of a list that a cluster sorts, a tile to a block.
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p, 
   for (int i = 0; i < passes; i++) {
     p.out = (passes - i) % 2 ? a : b;  // the last pass ends in a
     p.shift = i * p.bits;
-    place_tile<true>(p, blockIdx.x, count, scan, totals);
+    place_tile<SortIn::kCluster, kSortThreads>(p, blockIdx.x, count, scan, totals);
     if (p.tiles > 1) cluster_sync();  // the entries are written, and the totals have been read
     else __syncthreads();
     p.ids = nullptr;
@@ -286,7 +292,7 @@ __device__ __forceinline__ void store_row(const SumParams& p, int id, int c, con
   }
 }
 
-// The rows from `row0` on that the list lacks, a thread looking for each, then all writing them.
+// The kThreads rows from `row0` on that the list lacks: a thread looks for each, then all write them.
 __device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int columns, int* absent) {
   __shared__ int n;
   if (threadIdx.x == 0) n = 0;
@@ -311,24 +317,22 @@ __device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int co
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams p) {
+// The block's pieces of the list. WHOLE: they are all there is, and no run goes on in another block.
+// slot: [first, last][group][lane][VEC], key: [first, last][group]
+template <typename T, int VEC, bool WHOLE>
+__device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int (*key)[kThreads / 2]) {
   using V = RowVec<T, VEC>;
-  __shared__ float slot[2][kThreads * VEC];  // [first, last][group][lane][VEC]
-  __shared__ int key[2][kThreads / 2];
-  pdl_wait();
-  pdl_trigger();
-  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, p.lanes * VEC, key[0]);
+  constexpr int SLOTS = kThreads * VEC;
   const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kThreads / lanes;
   const int v = blockIdx.y * lanes + lane, c = v * VEC;
   const bool here = v < p.C / VEC;
   const T* dy = static_cast<const T*>(p.dy) + c;
-  const int64_t i0 = ((int64_t)blockIdx.x * groups + group) * p.piece;
+  const int64_t i0 = ((int64_t)(WHOLE ? 0 : blockIdx.x) * groups + group) * p.piece;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
   int cur = -1, first = -1;  // the run at hand, and the piece's first one once it is over
-  int2 later[kUnroll];  // the next entries, on their way while the rows of these are
+  int2 later[kUnroll];       // the next entries, on their way while the rows of these are
   auto look = [&](int e0) {
 #pragma unroll
     for (int u = 0; u < kUnroll; u++)
@@ -351,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams 
           if (first < 0) {
             first = cur;
 #pragma unroll
-            for (int j = 0; j < VEC; j++) slot[0][threadIdx.x * VEC + j] = acc[j];
+            for (int j = 0; j < VEC; j++) slot[threadIdx.x * VEC + j] = acc[j];
           } else if (here) {
             store_row<VEC>(p, cur, c, acc);
           }
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams 
   }
   const int last = first < 0 ? 0 : 1;
 #pragma unroll
-  for (int j = 0; j < VEC; j++) slot[last][threadIdx.x * VEC + j] = acc[j];
+  for (int j = 0; j < VEC; j++) slot[last * SLOTS + threadIdx.x * VEC + j] = acc[j];
   if (lane == 0) {
     key[0][group] = first < 0 ? cur : first;
     key[1][group] = first < 0 ? -1 : cur;
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams 
   for (int j = threadIdx.x; j < width; j += kThreads) {
     const int col = blockIdx.y * width + j;
     if (col >= p.C) continue;
-    float* part = p.part + (size_t)blockIdx.x * 2 * p.C + col;
+    float* part = WHOLE ? nullptr : p.part + (size_t)blockIdx.x * 2 * p.C + col;
     float sum = 0.0f;
     int run = key[0][0], head = -1;
     for (int g = 0; g < groups; g++)
@@ -389,15 +393,53 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams 
         const int id = key[k][g];
         if (id < 0) continue;
         if (id != run) {
-          if (head < 0) head = run, part[0] = sum;
+          if (!WHOLE && head < 0) head = run, part[0] = sum;
           else if (run < p.rows) p.dtable[(size_t)run * p.C + col] = sum * p.scale;
           run = id;
           sum = 0.0f;
         }
-        sum += slot[k][g * width + j];
+        sum += slot[k * SLOTS + g * width + j];
       }
-    part[head < 0 ? 0 : p.C] = sum;
-    if (col == 0) p.part_ids[blockIdx.x] = make_int2(head < 0 ? run : head, head < 0 ? -1 : run);
+    if (WHOLE) {
+      if (run < p.rows) p.dtable[(size_t)run * p.C + col] = sum * p.scale;
+    } else {
+      part[head < 0 ? 0 : p.C] = sum;
+      if (col == 0) p.part_ids[blockIdx.x] = make_int2(head < 0 ? run : head, head < 0 ? -1 : run);
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams p) {
+  __shared__ float slot[2 * kThreads * VEC];
+  __shared__ int key[2][kThreads / 2];
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, p.lanes * VEC, key[0]);
+  sum_pieces<T, VEC, false>(p, slot, key);
+}
+
+// Few tokens in one launch: every block sorts them in its shared memory, the first of each column of blocks sums, and all
+// share the rows that no token has.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) embed_few_kernel(SumParams p, SortParams q, int passes) {
+  __shared__ __align__(16) int2 list[2][kFewTokens];
+  __shared__ __align__(16) int count[kThreads / 32 << kFewBits];
+  __shared__ int scan[kThreads / 32], absent[kThreads], key[2][kThreads / 2];
+  static_assert(sizeof(list[1]) >= 2 * kThreads * VEC * sizeof(float), "the slots take the place of the other list");
+  for (int i = 0; i < passes; i++) {
+    q.out = list[(passes - i) % 2 ? 0 : 1];  // the last pass ends in list[0]
+    q.shift = i * q.bits;
+    place_tile<SortIn::kBlock, kThreads>(q, 0, count, scan, nullptr);
+    __syncthreads();
+    q.ids = nullptr;
+    q.in = q.out;
+  }
+  p.list = list[0];
+  if (blockIdx.x == 0) sum_pieces<T, VEC, true>(p, reinterpret_cast<float*>(list[1]), key);
+  for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < p.rows; row0 += (int64_t)gridDim.x * kThreads) {
+    absent_rows(p, (int)row0, p.lanes * VEC, absent);
+    __syncthreads();
   }
 }
 
@@ -580,13 +622,44 @@ void run_type(const EmbedParams& p, int vec, unsigned blocks, cudaStream_t st) {
   KC_CUDA(cudaGetLastError());
 }
 
+// One launch where a group of lanes with 64 bytes of a row each, 32 tokens to a group at most, has all tokens in a block
+// (361 tokens x 384, 362 rows, f16: 12.0 us in three launches).
+template <typename T, int VEC>
+bool launch_few(SumParams p, const int32_t* ids, cudaStream_t st) {
+  p.lanes = std::max(4, 64 / (VEC * (int)sizeof(T)));
+  const int groups = kThreads / p.lanes, chunks = (p.C / VEC + p.lanes - 1) / p.lanes;
+  if (p.tokens > std::min(kFewTokens, 32 * groups) || chunks > 2 * kSmCount) return false;
+  p.piece = (p.tokens + groups * kUnroll - 1) / (groups * kUnroll) * kUnroll;
+  int bits = 1;
+  while ((int64_t)p.rows >> bits) bits++;
+  const int passes = (bits + kFewBits - 1) / kFewBits;
+  const SortParams q{ids, nullptr, nullptr, nullptr, p.tokens, p.rows, 0, (bits + passes - 1) / passes, 1, p.tokens};
+  const int64_t rows = (p.rows + (int64_t)kThreads - 1) / kThreads, most = std::max(1, 4 * kSmCount / chunks);
+  embed_few_kernel<T, VEC><<<dim3((unsigned)std::min(rows, most), (unsigned)chunks), kThreads, 0, st>>>(p, q, passes);
+  KC_CUDA(cudaGetLastError());
+  return true;
+}
+
+template <typename T, int VEC>
+void sum_vec(SumParams p, const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, int* hist, cudaStream_t st) {
+  if (launch_few<T, VEC>(p, ids, st)) return;
+  sort_tokens(d, ids, a, b, hist, st);
+  const SumShape s = sum_shape(d.tokens, d.channels, VEC);
+  p.list = a;
+  p.lanes = s.lanes;
+  p.piece = s.piece;
+  p.blocks = s.blocks;
+  launch_sum<T, VEC>(p, s, st);
+}
+
 template <typename T>
-void sum_type(const SumParams& p, const SumShape& s, int vec, cudaStream_t st) {
+void sum_type(const SumParams& p, const kc_embed_desc& d, int vec, const int32_t* ids, int2* a, int2* b, int* hist,
+              cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (vec == 8) return launch_sum<T, 8>(p, s, st);
-  if (vec == 4) return launch_sum<T, 4>(p, s, st);
-  if (vec == 2) return launch_sum<T, 2>(p, s, st);
-  launch_sum<T, 1>(p, s, st);
+    if (vec == 8) return sum_vec<T, 8>(p, d, ids, a, b, hist, st);
+  if (vec == 4) return sum_vec<T, 4>(p, d, ids, a, b, hist, st);
+  if (vec == 2) return sum_vec<T, 2>(p, d, ids, a, b, hist, st);
+  sum_vec<T, 1>(p, d, ids, a, b, hist, st);
 }
 
 Rows rows_of(const kc_embed_desc& d, const void* p, int64_t count, int64_t stride) {
@@ -685,15 +758,22 @@ extern "C" int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* 
       return;
     }
     char* ws = static_cast<char*>(d_workspace);
-    int2* list = reinterpret_cast<int2*>(ws + l.a);
-    sort_tokens(d, d_ids, list, reinterpret_cast<int2*>(ws + l.b), reinterpret_cast<int*>(ws + l.hist), st);
+    int2 *a = reinterpret_cast<int2*>(ws + l.a), *b = reinterpret_cast<int2*>(ws + l.b);
+    int* hist = reinterpret_cast<int*>(ws + l.hist);
     const int vec = vec_of(d, {dy});
-    const SumShape s = sum_shape(d.tokens, d.channels, vec);
-    const SumParams p{list, d_dy, d_dtable, reinterpret_cast<float*>(ws + l.part), reinterpret_cast<int2*>(ws + l.ids),
-                      dy.outer_stride, (int)d.tokens, (int)d.table_rows, d.channels, s.lanes, s.piece, s.blocks,
-                      d.channels % 4 == 0 && aligned_to(d_dtable, 16), d.scale};
-    if (d.dtype == KC_PRECISION_F32) sum_type<float>(p, s, vec, st);
-    else if (d.dtype == KC_PRECISION_F16) sum_type<__half>(p, s, vec, st);
-    else sum_type<__nv_bfloat16>(p, s, vec, st);
+    SumParams p{};
+    p.dy = d_dy;
+    p.dtable = d_dtable;
+    p.part = reinterpret_cast<float*>(ws + l.part);
+    p.part_ids = reinterpret_cast<int2*>(ws + l.ids);
+    p.ys = dy.outer_stride;
+    p.tokens = (int)d.tokens;
+    p.rows = (int)d.table_rows;
+    p.C = d.channels;
+    p.wide = d.channels % 4 == 0 && aligned_to(d_dtable, 16);
+    p.scale = d.scale;
+    if (d.dtype == KC_PRECISION_F32) sum_type<float>(p, d, vec, d_ids, a, b, hist, st);
+    else if (d.dtype == KC_PRECISION_F16) sum_type<__half>(p, d, vec, d_ids, a, b, hist, st);
+    else sum_type<__nv_bfloat16>(p, d, vec, d_ids, a, b, hist, st);
   });
 }
