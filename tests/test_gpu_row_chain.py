@@ -1,0 +1,134 @@
+"""The operators in a row, as a distillation step of a small token net uses them: rows of moves and of points looked up and
+added, RMS norm, a linear, layer norm, a policy linear, the loss against a teacher's top logits; backward through all of
+it, against the same chain in float64."""
+
+import threading
+
+import pytest
+import torch
+
+import row_ops as r
+import token_ops as t
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def full_products():
+    before = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    yield
+    torch.backends.cuda.matmul.allow_tf32 = before
+
+
+def test_distillation_step():
+    """float32 throughout: each operator is within 2^-17 of its terms, and the linears and norms pass relative errors on
+    with factors of about 10: 1e-3 of the largest value is far above that and far below any wrong row, mask or weight."""
+    n, points, channels, classes, k, temp = 6, 361, 96, 362, 24, 2.0
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    moves, places = rand(classes + 1, channels) * 0.3, rand(points, channels) * 0.3
+    w1, w2, b2 = 1 + 0.2 * rand(channels), 1 + 0.2 * rand(channels), 0.2 * rand(channels)
+    lin, head = rand(channels, channels) / channels**0.5, rand(channels, classes) / channels**0.5 * 3
+    tokens = n * points
+    move_ids = torch.randint(-1, classes + 1, (tokens,), device="cuda", generator=g, dtype=torch.int32)
+    place_ids = (torch.arange(tokens, device="cuda") % points).int()
+    side = torch.tensor([19, 13, 9, 19, 13, 9], device="cuda")[:, None]
+    p = torch.arange(points, device="cuda")
+    mask = ((p % 19 < side) & (p // 19 < side)).float()
+    on = mask != 0
+    ids = rand(n, classes).argsort(1)[:, :k].int().contiguous()
+    ids[2] = -1
+    top, dloss = 2 * rand(n, k), rand(n).abs()
+
+    # the library's operators around torch's products
+    x0 = r.embed_forward(move_ids, moves, None, 2.0)
+    x0 = r.embed_forward(place_ids, places, x0, 1.0, y=x0).view(n, points, channels)
+    y1, st1 = r.layer_forward(x0, mask, w1, None, "rms")
+    h = (y1.view(-1, channels) @ lin).view(n, points, channels)
+    y2, st2 = r.layer_forward(h, mask, w2, b2, "layer")
+    pooled = y2.sum(1) / on.sum(1, keepdim=True)
+    logits = pooled @ head
+    loss, stats = r.distill_forward(logits, ids, top, None, temp)
+    dlogits = r.distill_backward(logits, ids, top, stats, None, temp, dloss)
+    dpooled = dlogits @ head.T / on.sum(1, keepdim=True)
+    dy2 = dpooled[:, None, :].expand(n, points, channels).contiguous()
+    dh, dw2, db2 = r.layer_backward(h, mask, w2, st2, dy2, "layer")
+    dy1 = (dh.view(-1, channels) @ lin.T).view(n, points, channels)
+    dx0, dw1, _ = r.layer_backward(x0, mask, w1, st1, dy1, "rms")
+    dx0 = dx0.view(tokens, channels)
+    dmoves, dplaces = r.embed_backward(move_ids, dx0, classes + 1, 2.0), r.embed_backward(place_ids, dx0, points)
+
+    # float64
+    leaves = [v.double().requires_grad_() for v in (moves, places, w1, w2, b2)]
+    md, pd, w1d, w2d, b2d = leaves
+    there = (move_ids >= 0)[:, None]
+    x = torch.where(there, md[move_ids.clamp(min=0).long()] * 2.0, 0.0) + pd[place_ids.long()]
+    y = r.layer64(x.view(n, points, channels), on, w1d, None, "rms")[0]
+    y = r.layer64((y.view(-1, channels) @ lin.double()).view(n, points, channels), on, w2d, b2d, "layer")[0]
+    z = (y.sum(1) / on.sum(1, keepdim=True)) @ head.double()
+    some = (ids >= 0).any(1)
+    tt = torch.where(some[:, None], top.double() / temp, 0.0)
+    lp = torch.log_softmax(tt, 1)
+    lq = torch.log_softmax(z / temp, 1).gather(1, ids.clamp(min=0).long())
+    want = torch.where(some, temp**2 * (lp.exp() * (lp - lq)).sum(1), 0.0)
+    grads = torch.autograd.grad((want * dloss.double()).sum(), leaves)
+    for got, ref in ((loss, want.detach()), (dmoves, grads[0]), (dplaces, grads[1]), (dw1, grads[2]), (dw2, grads[3]),
+                     (db2, grads[4])):
+        assert (got.double() - ref).abs().max() <= 1e-3 * ref.abs().max()
+    assert loss[2] == 0 and dlogits[2].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_one_token_at_a_time(dtype):
+    """A token alone gives the bits that it has in a sequence, through the lookup and the norms."""
+    tokens, channels, rows = 700, 384, 362
+    g = torch.Generator(device="cuda").manual_seed(5)
+    table = torch.randn(rows, channels, device="cuda", generator=g).to(t.DTYPES[dtype])
+    ids = torch.randint(-1, rows, (tokens,), device="cuda", generator=g, dtype=torch.int32)
+    w = torch.rand(channels, device="cuda", generator=g) + 0.5
+
+    def run(ids):
+        x = r.embed_forward(ids, table, None, 1.5)
+        y, _ = r.layer_forward(x[None], None, w, None, "rms")
+        return r.layer_forward(y, None, w, w, "layer")[0][0]
+
+    want = run(ids)
+    for i in range(0, tokens, 97):
+        assert torch.equal(run(ids[i:i + 1])[0], want[i])
+
+
+def test_host_threads_on_streams_of_their_own():
+    """Four host threads, each on its own stream, while the others call too: the same bits as alone."""
+
+    def work(seed, out):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+        x = rand(4, 361, 96 + 40 * seed).bfloat16()
+        w = rand(x.shape[2])
+        ids = torch.randint(0, 50, (4 * 361 * (1 + 2 * seed),), device="cuda", generator=g, dtype=torch.int32)
+        dy = rand(ids.shape[0], 64).half()
+        z, top = rand(30, 900 * (1 + 2 * seed)), rand(30, 20)
+        tid = torch.randint(0, 900, (30, 20), device="cuda", generator=g, dtype=torch.int32)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                y, st = r.layer_forward(x, None, w, w, "layer")
+                res = (y, st) + r.layer_backward(x, None, w, st, x, "layer")
+                res += (r.embed_backward(ids, dy, 50),)
+                loss, stats = r.distill_forward(z, tid, top)
+                res += (loss, stats, r.distill_backward(z, tid, top, stats))
+        stream.synchronize()
+        out[seed] = res
+
+    alone, together = {}, {}
+    for seed in range(4):
+        work(seed, alone)
+    threads = [threading.Thread(target=work, args=(seed, together)) for seed in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for seed in range(4):
+        assert all(torch.equal(a, c) for a, c in zip(alone[seed], together[seed]))
