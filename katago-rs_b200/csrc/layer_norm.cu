@@ -111,13 +111,32 @@ struct Units {
   }
 };
 
+// A vector that begins `bytes` (0 to 15, UP: 1 to 16) into 32 bytes; ELEMENT bytes divide it.
+template <int ELEMENT, bool UP>
+__device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32_t bytes) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int k = 0; k < 6; k++) w[k] = bytes & 8 ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; k++) w[k] = bytes & 4 ? w[k + 1] : w[k];
+  if (ELEMENT == 2) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(w[k], w[k + 1], (bytes & 2) * 8);
+  }
+  return UP && bytes & 16 ? hi : make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A thread's vectors of the next rows, on their way into shared memory of its own (DEPTH rows, the one at hand among
 // them; no more than what 512 threads of an SM have room for). Rows that are off are not copied.
-template <typename T, int VEC, int NV, bool BLOCK, int TENSORS>
+// SHIFT: rows that begin anywhere. The aligned 16-byte pieces that hold the row are copied (such a piece never leaves the
+// allocation of the element in it), and a vector is a window over its own piece and the next one, which a neighbour has;
+// its warp's lanes have to be done with a row before the next one takes its place.
+template <typename T, int VEC, int NV, bool BLOCK, int TENSORS, bool SHIFT>
 struct Ring {
   using Copy = RowCopy<T, VEC>;
   using Slot = typename Copy::Slot;
-  static constexpr int ROW = TENSORS * NV * (int)sizeof(Slot);
+  static constexpr int SLOTS = SHIFT ? NV + 1 : NV;  // of a tensor's row
+  static constexpr int ROW = TENSORS * SLOTS * (int)sizeof(Slot);
   static constexpr int DEPTH = TENSORS == 1 && ROW * 4 <= 420 ? 4 : ROW * 3 <= 420 ? 3 : 2;
   static size_t bytes(int threads) { return (size_t)DEPTH * ROW * threads; }
 
@@ -126,48 +145,60 @@ struct Ring {
   int64_t next;       // the row to copy next
   float next_mask;    // looked at a row later, when it has arrived
   uint32_t on = 0;    // a bit for each stage
-  // a bit for each stage: the thread's elements (its lanes are an even number apart) are the upper halves of 4 bytes
-  uint32_t high[TENSORS] = {};
+  // 4 bits for each stage: where the row begins in its first piece; or whether the thread's single 2-byte elements (its
+  // lanes are an even number apart) are the upper halves of 4 bytes
+  uint32_t begin[TENSORS] = {};
 
   __device__ __forceinline__ Slot* at(int s, int tensor, int i) const {
-    return mine + (s * TENSORS * NV + tensor * NV + i) * (BLOCK ? (int)blockDim.x : kThreads);
+    return mine + (s * TENSORS * SLOTS + tensor * SLOTS + i) * (BLOCK ? (int)blockDim.x : kThreads);
   }
   __device__ __forceinline__ void look(const LayerParams& p) { next_mask = next < p.rows ? token_mask(p, next) : 0.0f; }
-  __device__ __forceinline__ void fetch_row(const T* row, int tensor, const Group<BLOCK>& g, int nvec, int s) {
+  __device__ __forceinline__ void fetch_row(const T* row, int tensor, const Group<BLOCK>& g, int C, int s) {
     const T* src = row + g.lane * VEC;
-    if constexpr (Copy::BYTES == 2)
-      high[tensor] = (high[tensor] & ~(1u << s)) | ((uint32_t)(reinterpret_cast<uintptr_t>(src) >> 1) & 1u) << s;
+    int n = C / VEC;
+    if constexpr (SHIFT || Copy::BYTES == 2) {
+      const uint32_t low = SHIFT ? (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u
+                                 : (uint32_t)(reinterpret_cast<uintptr_t>(src) >> 1) & 1u;
+      begin[tensor] = (begin[tensor] & ~(15u << 4 * s)) | low << 4 * s;
+      if (SHIFT) {
+        src = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(row) - low) + g.lane * VEC;
+        n = (int)(low + C * sizeof(T) + 15) / 16;
+      }
+    }
     src = Copy::base(src);
 #pragma unroll
-    for (int i = 0; i < NV; i++, src += g.lanes * VEC)
-      if (g.lane + i * g.lanes < nvec) Copy::copy(at(s, tensor, i), src);
+    for (int i = 0; i < SLOTS; i++, src += g.lanes * VEC)
+      if (g.lane + i * g.lanes < n) Copy::copy(at(s, tensor, i), src);
   }
-  __device__ __forceinline__ void fetch(const LayerParams& p, const Group<BLOCK>& g, int nvec, int s) {
+  __device__ __forceinline__ void fetch(const LayerParams& p, const Group<BLOCK>& g, int s) {
     const bool next_on = next_mask != 0.0f;
     on = (on & ~(1u << s)) | (next_on ? 1u << s : 0u);
     if (next_on) {
-      fetch_row(static_cast<const T*>(p.x) + p.xm(next), 0, g, nvec, s);
-      if (TENSORS == 2) fetch_row(static_cast<const T*>(p.dy) + p.ym(next), TENSORS - 1, g, nvec, s);
+      fetch_row(static_cast<const T*>(p.x) + p.xm(next), 0, g, p.C, s);
+      if (TENSORS == 2) fetch_row(static_cast<const T*>(p.dy) + p.ym(next), TENSORS - 1, g, p.C, s);
     }
     copy_commit();
     next += g.step;
     look(p);
   }
-  __device__ __forceinline__ void start(const LayerParams& p, const Group<BLOCK>& g, int nvec, void* smem) {
+  __device__ __forceinline__ void start(const LayerParams& p, const Group<BLOCK>& g, void* smem) {
     mine = static_cast<Slot*>(smem) + threadIdx.x;
     next = g.first;
     look(p);
 #pragma unroll
-    for (int s = 0; s < DEPTH - 1; s++) fetch(p, g, nvec, s);
+    for (int s = 0; s < DEPTH - 1; s++) fetch(p, g, s);
   }
   // The row at hand is there afterwards, and one more is on its way.
-  __device__ __forceinline__ bool arrive(const LayerParams& p, const Group<BLOCK>& g, int nvec) {
-    fetch(p, g, nvec, stage == 0 ? DEPTH - 1 : stage - 1);
+  __device__ __forceinline__ bool arrive(const LayerParams& p, const Group<BLOCK>& g) {
+    if (SHIFT) __syncwarp();
+    fetch(p, g, stage == 0 ? DEPTH - 1 : stage - 1);
     copy_wait<DEPTH - 1>();
+    if (SHIFT) __syncwarp();
     return on >> stage & 1;
   }
-  // unit u of the row at hand
-  __device__ __forceinline__ void get(int tensor, int u, const Group<BLOCK>& g, int nvec, f32x2 (&v)[Units<VEC, NV>::N]) const {
+  // unit u of the row at hand; of a vector that ends behind the row, `rest` elements
+  __device__ __forceinline__ void get(int tensor, int u, const Group<BLOCK>& g, int nvec, int rest,
+                                      f32x2 (&v)[Units<VEC, NV>::N]) const {
     float f[VEC];
     if constexpr (VEC == 1) {
       float e[2];
@@ -175,12 +206,30 @@ struct Ring {
       for (int k = 0; k < 2; k++) {
         const int i = 2 * u + k, c = g.lane + i * g.lanes;
         f[0] = 0.0f;
-        if (c < nvec) Copy::unpack(*at(stage, tensor, i), high[tensor] >> stage & 1, f);
+        if (c < nvec) Copy::unpack(*at(stage, tensor, i), begin[tensor] >> 4 * stage & 1, f);
         e[k] = f[0];
       }
       v[0] = {e[0], e[1]};
+      return;
+    }
+    if constexpr (SHIFT) {
+      // the last of the group's lanes goes on at the first one's next slot
+      const Slot* own = at(stage, tensor, u);
+      const Slot* other = g.lane == g.lanes - 1 ? at(stage, tensor, u + 1) - (g.lanes - 1) : own + 1;
+      uint4 raw = window<sizeof(T), false>(*own, *other, begin[tensor] >> 4 * stage & 15);
+      if (rest && g.lane + u * g.lanes == nvec - 1) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int bytes = rest * (int)sizeof(T) - 4 * k;
+          w[k] = bytes >= 4 ? w[k] : bytes <= 0 ? 0u : w[k] & 0xffffu;
+        }
+      }
+      Copy::unpack(raw, false, f);
     } else {
       Copy::unpack(*at(stage, tensor, u), false, f);
+    }
+    if constexpr (VEC > 1) {
 #pragma unroll
       for (int j = 0; j < VEC / 2; j++) v[j] = {f[2 * j], f[2 * j + 1]};
     }
@@ -188,17 +237,29 @@ struct Ring {
   __device__ __forceinline__ void leave() { stage = stage == DEPTH - 1 ? 0 : stage + 1; }
 };
 
-// A thread's place in a row: which of its units there are.
-template <int VEC, int NV, bool BLOCK>
+// A thread's place in a row: which of its units there are, and their way out.
+template <int VEC, int NV, bool BLOCK, bool SHIFT>
 struct Place {
   using U = Units<VEC, NV>;
   const Group<BLOCK>& g;
-  int nvec;
+  int nvec, rest;  // vectors of the row; SHIFT: elements of the last one, 0 where it is whole
+  __device__ __forceinline__ Place(const Group<BLOCK>& group, int C)
+      : g(group), nvec(SHIFT ? (C + VEC - 1) / VEC : C / VEC), rest(SHIFT ? C % VEC : 0) {}
   __device__ __forceinline__ bool has(int i) const { return g.lane + i * g.lanes < nvec; }  // vector i
   __device__ __forceinline__ bool has_unit(int u) const { return has(VEC == 1 ? 2 * u : u); }
-  // `f` in the elements of unit u that there are
-  __device__ __forceinline__ f32x2 both(int u, float f) const {
-    return {f, VEC > 1 || has(2 * u + 1) ? f : 0.0f};
+  // `f` in the elements of pair j of unit u that there are
+  __device__ __forceinline__ f32x2 both(int u, int j, float f) const {
+    if (VEC == 1) return {f, has(2 * u + 1) ? f : 0.0f};
+    if (SHIFT && rest && g.lane + u * g.lanes == nvec - 1)
+      return {2 * j < rest ? f : 0.0f, 2 * j + 1 < rest ? f : 0.0f};
+    return {f, f};
+  }
+  template <typename T>
+  __device__ __forceinline__ static typename RowVec<T, VEC>::Raw pack(const f32x2 (&v)[U::N]) {
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) f[j] = j % 2 ? v[j / 2].y : v[j / 2].x;
+    return RowVec<T, VEC>::pack(f);
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, int u, const f32x2 (&v)[U::N], uint32_t keep) const {
@@ -208,10 +269,7 @@ struct Place {
       V::store(row + g.lane + 2 * u * g.lanes, masked(V::pack(a), keep));
       if (has(2 * u + 1)) V::store(row + g.lane + (2 * u + 1) * g.lanes, masked(V::pack(b), keep));
     } else {
-      float f[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) f[j] = j % 2 ? v[j / 2].y : v[j / 2].x;
-      V::store(row + (g.lane + u * g.lanes) * VEC, masked(V::pack(f), keep));
+      V::store(row + (g.lane + u * g.lanes) * VEC, masked(pack<T>(v), keep));
     }
   }
   template <typename T>
@@ -220,14 +278,50 @@ struct Place {
     for (int i = 0; i < NV; i++)
       if (has(i)) RowVec<T, VEC>::store(row + (g.lane + i * g.lanes) * VEC, typename RowVec<T, VEC>::Raw{});
   }
+  // SHIFT: all vectors of a row that begins anywhere, by all lanes of the warp: a piece is a window over the vector before
+  // and its own; the pieces that hold other rows' elements go out element by element. Nothing where `here` is false.
+  template <typename T>
+  __device__ __forceinline__ void store_shifted(T* row, int C, const uint4 (&raw)[NV], bool here) const {
+    const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+    const int skip = (int)(low / sizeof(T)), from = g.lane == 0 ? g.lanes - 1 : g.lane - 1;
+    const bool last = g.lane == g.lanes - 1;
+    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(row) - low);
+#pragma unroll
+    for (int i = 0; i <= NV; i++) {
+      const uint4 own = i < NV ? raw[i < NV ? i : 0] : uint4{};
+      const uint4 give = last && i > 0 ? raw[i > 0 ? i - 1 : 0] : own;
+      uint4 before;
+      before.x = __shfl_sync(0xffffffffu, give.x, from, g.lanes);
+      before.y = __shfl_sync(0xffffffffu, give.y, from, g.lanes);
+      before.z = __shfl_sync(0xffffffffu, give.z, from, g.lanes);
+      before.w = __shfl_sync(0xffffffffu, give.w, from, g.lanes);
+      const uint4 piece = window<sizeof(T), true>(before, own, 16 - low);
+      const int v = g.lane + i * g.lanes, c = v * VEC - skip;
+      if (!here || c >= C) continue;
+      if (c >= 0 && c + VEC <= C) {
+        out[v] = piece;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&piece);
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          if (c + j >= 0 && c + j < C) row[c + j] = e[j];
+      }
+    }
+  }
   __device__ __forceinline__ void load(U& w, const float* p, float otherwise, bool wide) const {
     w.fill(otherwise);
     if (!p) return;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       if (!has(i)) continue;
+      const float* q = p + (g.lane + i * g.lanes) * VEC;
       float f[VEC];
-      load_params<VEC>(p + (g.lane + i * g.lanes) * VEC, wide, f);
+      if (SHIFT && rest && g.lane + i * g.lanes == nvec - 1) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) f[j] = j < rest ? __ldg(q + j) : otherwise;
+      } else {
+        load_params<VEC>(q, wide, f);
+      }
       if constexpr (VEC == 1) {
         if (i % 2) w.v[i / 2][0].y = f[0];
         else w.v[i / 2][0].x = f[0];
@@ -241,29 +335,33 @@ struct Place {
 
 constexpr int kBlockThreads = 512;  // of blocks that share a row, at most: 128 registers each
 
-template <typename T, int VEC, int NV, bool BLOCK>
+template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 2)
     layer_norm_kernel(const LayerParams p) {
   using U = Units<VEC, NV>;
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
-  const Place<VEC, NV, BLOCK> at{g, p.C / VEC};
+  const Place<VEC, NV, BLOCK, SHIFT> at(g, p.C);
   const float inv = 1.0f / (float)p.C;
   const bool layer = p.kind == KC_NORM_LAYER;
-  Ring<T, VEC, NV, BLOCK, 1> ring;
-  ring.start(p, g, at.nvec, smem);
+  Ring<T, VEC, NV, BLOCK, 1, SHIFT> ring;
+  ring.start(p, g, smem);
   U w, b;
   at.load(w, p.weight, 1.0f, p.wide);
   at.load(b, p.bias, 0.0f, p.wide);
   int turn = 0;  // a block's sums in a row take turns with `red`
   for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, ring.leave()) {
-    const bool here = r < p.rows, on = ring.arrive(p, g, at.nvec);
+    const bool here = r < p.rows, on = ring.arrive(p, g);
     T* out = static_cast<T*>(p.y) + (here ? p.ym(r) : 0);
     if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
-      if (!here) continue;
-      if (p.stats && g.lane == 0) p.stats[r] = make_float2(0.0f, 0.0f);
-      at.zero(out);
+      if (here && p.stats && g.lane == 0) p.stats[r] = make_float2(0.0f, 0.0f);
+      if constexpr (SHIFT) {
+        const uint4 nothing[NV] = {};
+        at.store_shifted(out, p.C, nothing, here);
+      } else if (here) {
+        at.zero(out);
+      }
       continue;
     }
     // a warp whose rows are on in part goes over all of them; what its other slots hold is dropped in the end
@@ -272,7 +370,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
 #pragma unroll
     for (int u = 0; u < U::U; u++) {
       if (!at.has_unit(u)) continue;
-      ring.get(0, u, g, at.nvec, x.v[u]);
+      ring.get(0, u, g, at.nvec, at.rest, x.v[u]);
       if (layer)
 #pragma unroll
         for (int j = 0; j < U::N; j++) s1 = add2(s1, x.v[u][j]);
@@ -284,10 +382,9 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
 #pragma unroll
       for (int u = 0; u < U::U; u++) {
         if (!at.has_unit(u)) continue;
-        const f32x2 back = at.both(u, -m0);
 #pragma unroll
         for (int j = 0; j < U::N; j++) {
-          x.v[u][j] = add2(x.v[u][j], back);
+          x.v[u][j] = add2(x.v[u][j], at.both(u, j, -m0));
           s1 = add2(s1, x.v[u][j]);
           s2 = fma2(x.v[u][j], x.v[u][j], s2);
         }
@@ -304,24 +401,28 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
       }
       squares = g.sum(s2.x + s2.y, red[turn ^= 1]);
     }
-    if (!here) continue;
+    if (!SHIFT && !here) continue;
     const float rstd = rstd_of(squares, inv, delta, p.eps);
-    if (p.stats && g.lane == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
+    if (here && p.stats && g.lane == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
     const f32x2 scale = {rstd, rstd}, shift = {-delta * rstd, -delta * rstd};
     const uint32_t keep = on ? 0xffffffffu : 0u;
+    uint4 raw[SHIFT ? NV : 1];
 #pragma unroll
     for (int u = 0; u < U::U; u++) {
+      if constexpr (SHIFT) raw[u] = uint4{};
       if (!at.has_unit(u)) continue;
 #pragma unroll
       for (int j = 0; j < U::N; j++) x.v[u][j] = fma2(fma2(x.v[u][j], scale, shift), w.v[u][j], b.v[u][j]);
-      at.store(out, u, x.v[u], keep);
+      if constexpr (SHIFT) raw[u] = masked(at.template pack<T>(x.v[u]), keep);
+      else at.store(out, u, x.v[u], keep);
     }
+    if constexpr (SHIFT) at.store_shifted(out, p.C, raw, here);
   }
   copy_wait<0>();
 }
 
 // LEAN: RMS norm without a bias, which needs no sum of g and none of dy.
-template <typename T, int VEC, int NV, bool BLOCK, bool LEAN>
+template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT, bool LEAN>
 __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 2)
     layer_norm_back_kernel(const LayerParams p) {
   using U = Units<VEC, NV>;
@@ -329,11 +430,11 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
   __shared__ float2 red[2][32];
   extern __shared__ __align__(16) uint8_t smem[];
   const Group<BLOCK> g(p.lanes);
-  const Place<VEC, NV, BLOCK> at{g, p.C / VEC};
+  const Place<VEC, NV, BLOCK, SHIFT> at(g, p.C);
   const float inv = 1.0f / (float)p.C;
   pdl_trigger();
-  Ring<T, VEC, NV, BLOCK, 2> ring;
-  ring.start(p, g, at.nvec, smem);
+  Ring<T, VEC, NV, BLOCK, 2, SHIFT> ring;
+  ring.start(p, g, smem);
   U aw, ab, w;
   aw.fill(0.0f);
   ab.fill(0.0f);
@@ -341,12 +442,17 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
   int turn = 0;
   float2 st_next = g.first < p.rows ? p.stats[g.first] : make_float2(0.0f, 0.0f);
   for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1, ring.leave()) {
-    const bool here = r < p.rows, on = ring.arrive(p, g, at.nvec);
+    const bool here = r < p.rows, on = ring.arrive(p, g);
     const float2 st = st_next;
     if (r + g.step < p.rows) st_next = p.stats[r + g.step];
     T* out = static_cast<T*>(p.y) + (here ? p.xm(r) : 0);
     if (BLOCK ? !on : !__any_sync(0xffffffffu, on)) {
-      if (here) at.zero(out);
+      if constexpr (SHIFT) {
+        const uint4 nothing[NV] = {};
+        at.store_shifted(out, p.C, nothing, here);
+      } else if (here) {
+        at.zero(out);
+      }
       continue;
     }
     // xh and g of the row, for its sums and then for dx (where dy has no element it is 0, and xh plays no part)
@@ -357,9 +463,9 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
 #pragma unroll
       for (int u = 0; u < U::U; u++) {
         if (!at.has_unit(u)) continue;
-        ring.get(0, u, g, at.nvec, xh.v[u]);
+        ring.get(0, u, g, at.nvec, at.rest, xh.v[u]);
         f32x2 d[U::N];
-        ring.get(1, u, g, at.nvec, d);
+        ring.get(1, u, g, at.nvec, at.rest, d);
 #pragma unroll
         for (int j = 0; j < U::N; j++) {
           xh.v[u][j] = mul2(add2(xh.v[u][j], back), scale);
@@ -377,19 +483,21 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
     float2 s;
     if constexpr (LEAN) s = make_float2(0.0f, g.sum(s2.x + s2.y, red[turn]));
     else s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn]);
-    if (!here) continue;
+    if (!SHIFT && !here) continue;
     // rstd (g - c1 - xh c2)
     const float k1 = p.kind == KC_NORM_LAYER ? -s.x * inv * st.y : 0.0f, k2 = -s.y * inv * st.y;
     const f32x2 c1 = {k1, k1}, c2 = {k2, k2};
     const uint32_t keep = on ? 0xffffffffu : 0u;
     if constexpr (AGAIN) asm volatile("" ::: "memory");
+    uint4 raw[SHIFT ? NV : 1];
 #pragma unroll
     for (int u = 0; u < U::U; u++) {
+      if constexpr (SHIFT) raw[u] = uint4{};
       if (!at.has_unit(u)) continue;
       f32x2 o[U::N];
       if constexpr (AGAIN) {
-        ring.get(1, u, g, at.nvec, o);
-        ring.get(0, u, g, at.nvec, xh.v[u]);
+        ring.get(1, u, g, at.nvec, at.rest, o);
+        ring.get(0, u, g, at.nvec, at.rest, xh.v[u]);
       }
 #pragma unroll
       for (int j = 0; j < U::N; j++) {
@@ -397,8 +505,10 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
         const f32x2 gj = AGAIN ? mul2(o[j], w.v[u][j]) : gw.v[u][j];
         o[j] = fma2(gj, scale, fma2(xh.v[u][j], c2, c1));
       }
-      at.store(out, u, o, keep);
+      if constexpr (SHIFT) raw[u] = masked(at.template pack<T>(o), keep);
+      else at.store(out, u, o, keep);
     }
+    if constexpr (SHIFT) at.store_shifted(out, p.C, raw, here);
   }
   copy_wait<0>();
   if (!p.part) return;
@@ -610,32 +720,31 @@ __global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* pa
 // How a call goes over its rows.
 struct Shape {
   int vec, nv;
+  bool shift;    // rows that begin anywhere
   bool block;    // a block to a row, otherwise `lanes` lanes of a warp
   bool is_long;
   int threads, lanes;
   int64_t blocks;
 };
 
-// Vectors of a warp's lane, for each width of vector: up to 24 elements (weight, bias and the row in registers, or
-// weight, row, gradient and the channels' sums). A block's thread has 16 or, forward, 32 elements.
-constexpr int kNvs[] = {1, 2, 3, 4, 6, 8, 12, 16, 24};
-constexpr bool warp_nv(int vec, int nv) {
-  if (vec == 8) return nv <= 3;
-  if (vec == 4) return nv == 1 || nv == 2 || nv == 3 || nv == 4 || nv == 6;
-  if (vec == 2) return nv == 1 || nv == 4 || nv == 8 || nv == 12;
-  return nv == 2 || nv == 8 || nv == 16 || nv == 24;
-}
+// 16-byte vectors of a warp's lane: up to 24 elements (weight, bias and the row in registers, or weight, row, gradient and
+// the channels' sums). A block's thread has 16 or, forward, 32 elements.
+constexpr int kNvs[] = {1, 2, 3, 4, 6};
+constexpr bool warp_nv(int vec, int nv) { return vec * nv <= 24 && (vec == 4 || nv <= 3); }
 
-Shape shape_of(int64_t rows, int C, int vec, bool backward) {
+// `bytes` of an element; `vec`: the widest vectors to which channels, strides and addresses are aligned.
+Shape shape_of(int64_t rows, int C, int bytes, int vec, bool backward) {
   Shape s{};
-  s.vec = vec;
-  const int64_t nvec = C / vec;
+  const int whole = 16 / bytes;
+  s.vec = whole;
+  s.shift = vec < whole;
+  const int64_t nvec = ((int64_t)C + whole - 1) / whole;
   // the fewest lanes in a row that leave no more than an eighth of them idle, with as many vectors each as are built:
   // few shuffles for a sum, many loads in flight
   int64_t best = -1;
   for (int lanes = 2; lanes <= 32; lanes *= 2)
     for (int nv : kNvs) {
-      if (!warp_nv(vec, nv) || (int64_t)lanes * nv < nvec) continue;
+      if (!warp_nv(whole, nv) || (int64_t)lanes * nv < nvec) continue;
       const int64_t waste = (int64_t)lanes * nv * 8 - nvec * 8 > nvec ? (int64_t)lanes * nv - nvec : 0;
       const int64_t cost = waste * 64 + lanes;
       if (best < 0 || cost < best) best = cost, s.lanes = lanes, s.nv = nv;
@@ -643,16 +752,18 @@ Shape shape_of(int64_t rows, int C, int vec, bool backward) {
   if (best >= 0) {
     s.threads = kThreads;
     const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
-    s.blocks = std::min<int64_t>(all, (!backward && s.nv * vec <= 8 ? 4 : 2) * kSmCount);  // by registers
+    s.blocks = std::min<int64_t>(all, (!backward && s.nv * whole <= 8 ? s.shift ? 3 : 4 : 2) * kSmCount);  // by registers
     return s;
   }
+  s.shift = false;
+  s.vec = vec;
   s.block = true;
   for (int elements = 16; elements <= (backward ? 16 : 32); elements *= 2) {
     s.nv = elements / vec;
-    const int64_t threads = ((nvec + s.nv - 1) / s.nv + 31) / 32 * 32;
-    if (threads > kBlockThreads) continue;
-    s.threads = (int)threads;
-    s.blocks = std::min<int64_t>(rows, kSmCount * (kBlockThreads / threads));
+    const int64_t threads = ((int64_t)C / vec + s.nv - 1) / s.nv;
+    s.threads = (int)std::min<int64_t>((threads + 31) / 32 * 32, 1 << 20);
+    if (s.threads > kBlockThreads) continue;
+    s.blocks = std::min<int64_t>(rows, kSmCount * (kBlockThreads / s.threads));
     return s;
   }
   s.block = false;
@@ -675,44 +786,46 @@ PartShape part_shape(const Shape& s, int64_t rows, int C) {
   return {(int)s.blocks, s.nv * s.vec * lanes, C, s.nv, s.vec, lanes};
 }
 
-template <typename T, int VEC, int NV, bool BLOCK, bool LEAN>
+template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT, bool LEAN>
 void launch_back(const LayerParams& p, const Shape& s, cudaStream_t st) {
   // the ring, and in its place the warps' sums
   const size_t sums = BLOCK ? 0 : (size_t)kThreads / 32 * 2 * NV * VEC * s.lanes * sizeof(float);
-  const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2>::bytes(s.threads), sums);
-  allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK, LEAN>>();
-  layer_norm_back_kernel<T, VEC, NV, BLOCK, LEAN><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
+  const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2, SHIFT>::bytes(s.threads), sums);
+  allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN>>();
+  layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
 }
 
-template <typename T, int VEC, int NV, bool BLOCK>
+template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT>
 void launch_rows(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
   if (backward) {
     if constexpr (!BLOCK || NV * VEC <= 16) {
-      if (p.kind == KC_NORM_RMS && !p.dbias) launch_back<T, VEC, NV, BLOCK, true>(p, s, st);
-      else launch_back<T, VEC, NV, BLOCK, false>(p, s, st);
+      if (p.kind == KC_NORM_RMS && !p.dbias) launch_back<T, VEC, NV, BLOCK, SHIFT, true>(p, s, st);
+      else launch_back<T, VEC, NV, BLOCK, SHIFT, false>(p, s, st);
     }
   } else {
-    allow_block_smem<layer_norm_kernel<T, VEC, NV, BLOCK>>();
-    layer_norm_kernel<T, VEC, NV, BLOCK>
-        <<<(unsigned)s.blocks, s.threads, Ring<T, VEC, NV, BLOCK, 1>::bytes(s.threads), st>>>(p);
+    allow_block_smem<layer_norm_kernel<T, VEC, NV, BLOCK, SHIFT>>();
+    layer_norm_kernel<T, VEC, NV, BLOCK, SHIFT>
+        <<<(unsigned)s.blocks, s.threads, Ring<T, VEC, NV, BLOCK, 1, SHIFT>::bytes(s.threads), st>>>(p);
   }
   KC_CUDA(cudaGetLastError());
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int NV>
 bool launch_warp(const LayerParams& p, const Shape& s, bool backward, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
   if constexpr (warp_nv(VEC, NV)) {
     if (s.nv != NV) return false;
-    launch_rows<T, VEC, NV, false>(p, s, backward, st);
+    s.shift ? launch_rows<T, VEC, NV, false, true>(p, s, backward, st)
+            : launch_rows<T, VEC, NV, false, false>(p, s, backward, st);
     return true;
   }
   return false;
 }
 
-template <typename T, int VEC, int... NVS>
+template <typename T, int... NVS>
 void launch_warps(std::integer_sequence<int, NVS...>, const LayerParams& p, const Shape& s, bool backward,
                   cudaStream_t st) {
-  (launch_warp<T, VEC, NVS>(p, s, backward, st) || ...);
+  (launch_warp<T, NVS>(p, s, backward, st) || ...);
 }
 
 template <typename T, int VEC>
@@ -729,11 +842,12 @@ void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t s
       layer_norm_long_back_kernel<T, VEC><<<(unsigned)s.blocks, kLongThreads, 0, st>>>(p);
     }
     KC_CUDA(cudaGetLastError());
-  } else if (s.block) {
-    if (s.nv == 16 / VEC) launch_rows<T, VEC, 16 / VEC, true>(p, s, backward, st);
-    else launch_rows<T, VEC, 32 / VEC, true>(p, s, backward, st);
+  } else if (!s.block) {
+    launch_warps<T>(std::integer_sequence<int, 1, 2, 3, 4, 6>{}, p, s, backward, st);
+  } else if (s.nv == 16 / VEC) {
+    launch_rows<T, VEC, 16 / VEC, true, false>(p, s, backward, st);
   } else {
-    launch_warps<T, VEC>(std::integer_sequence<int, 1, 2, 3, 4, 6, 8, 12, 16, 24>{}, p, s, backward, st);
+    launch_rows<T, VEC, 32 / VEC, true, false>(p, s, backward, st);
   }
 }
 
@@ -755,7 +869,7 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
   p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);
   p.mm = row_map(d.n, d.points, d.mask_board_stride, 1);
-  const Shape s = shape_of(p.rows, p.C, vec, backward);
+  const Shape s = shape_of(p.rows, p.C, dtype_bytes(d.dtype), vec, backward);
   p.lanes = s.lanes;
   if (d.dtype == KC_PRECISION_F32) run_type<float>(p, s, backward, st);
   else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, s, backward, st);
@@ -809,7 +923,7 @@ size_t back_workspace(const kc_layer_norm_desc& d) {
   size_t floats = 0;
   for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2) {
     if (d.channels % v != 0) continue;
-    const PartShape q = part_shape(shape_of(rows, d.channels, v, true), rows, d.channels);
+    const PartShape q = part_shape(shape_of(rows, d.channels, dtype_bytes(d.dtype), v, true), rows, d.channels);
     floats = std::max(floats, (size_t)q.blocks * 2 * q.slots);
   }
   return (floats * sizeof(float) + 255) / 256 * 256;
