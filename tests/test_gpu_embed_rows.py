@@ -74,6 +74,16 @@ def test_many_tokens(kind):
     check_backward(r.embed_backward(ids, dy, 3000000 // 32, -0.5), ids, dy, 3000000 // 32, -0.5)
 
 
+@pytest.mark.parametrize("tokens", [1, 31, 32, 33, 255, 256, 511, 1024, 2047, 2048, 2049, 16383, 16384, 16385, 131072,
+                                    131073])
+@pytest.mark.parametrize("kind", ["skewed", "one", "padded"])
+def test_ends_of_the_ways_to_sort(tokens, kind):
+    """In a block's shared memory, by clusters of 1 to 16 blocks, by launches; digits of 1, 9 and 2 x 6 bits."""
+    for channels, rows, dtype in ((8, 1, "f32"), (16, 500, "bf16"), (4, 4000, "f16")):
+        ids, _, dy, _ = make(tokens, channels, rows, dtype, tokens, kind)
+        check_backward(r.embed_backward(ids, dy, rows, 1.5), ids, dy, rows, 1.5)
+
+
 def test_three_digits():
     ids, table, dy, _ = make(10000, 4, 1 << 20, "f32", 7, "padded")
     check_backward(r.embed_backward(ids, dy, 1 << 20), ids, dy, 1 << 20, 1.0)

@@ -71,6 +71,9 @@ CASES = [
     (1, 1000, 8, 0), (7, 3, 256, 8), (2, 19, 1024, 0), (1, 50, 1000, 0), (3, 5, 2048, 0), (2, 9, 1030, 0),
     (1, 6, 4096, 0), (2, 2, 4099, 0), (1, 3, 8192, 8), (1, 3, 16384, 0), (1, 2, 40000, 0), (2, 1, 20003, 0),
     (300, 40, 16, 0), (1, 5, 130, 0), (2, 70, 640, 1), (1, 17, 192, 0), (3, 2, 513, 0),
+    # rows that begin anywhere: whole and partial last vectors, as many vectors as a group of lanes holds
+    (3, 40, 768, 3), (2, 50, 767, 0), (3, 31, 384, 5), (2, 90, 24, 1), (1, 77, 8, 1), (2, 33, 760, 2), (1, 9, 769, 1),
+    (5, 60, 128, 7), (1, 300, 3, 0),
 ]
 
 

@@ -132,3 +132,51 @@ def test_host_threads_on_streams_of_their_own():
         th.join()
     for seed in range(4):
         assert all(torch.equal(a, c) for a, c in zip(alone[seed], together[seed]))
+
+
+def test_first_calls_in_a_capture():
+    """A fresh process whose first call of each kernel is captured into a graph."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import row_ops as r
+x = [torch.randn(40, 50, c, device="cuda").bfloat16() for c in (96, 2000, 20000)] + [
+    torch.randn(40, 50, 99, device="cuda")[:, :, 1:98]]
+w = [torch.ones(v.shape[2], device="cuda") for v in x]
+ids = [torch.arange(n, device="cuda").int() %% 300 for n in (500, 30000, 200000)]
+dy = [torch.randn(i.shape[0], 16, device="cuda") for i in ids]
+z = [torch.randn(n, c, device="cuda").half() for n, c in ((500, 362), (1300, 5000), (2, 90000))]
+tid = [torch.zeros(v.shape[0], 40, device="cuda").int() for v in z]
+top = [torch.zeros(v.shape[0], 40, device="cuda") for v in z]
+
+
+def everything():
+    out = []
+    for v, u in zip(x, w):
+        y, st = r.layer_forward(v, None, u, u, "layer")
+        out += [y, st, *r.layer_backward(v, None, u, st, y, "layer")]
+        y, st = r.layer_forward(v, None, u, None, "rms")
+        out += [y, st, *r.layer_backward(v, None, u, st, y, "rms")]
+    for i, d in zip(ids, dy):
+        out += [r.embed_forward(i, d[:300], d), r.embed_backward(i, d, 300)]
+    for v, i, t in zip(z, tid, top):
+        loss, st = r.distill_forward(v, i, t)
+        out += [loss, st, r.distill_backward(v, i, t, st)]
+    return out
+
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = everything()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, everything()))
+print("captured")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = code % (here, os.path.join(os.path.dirname(here), "katago-rs_b200", "python"))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
