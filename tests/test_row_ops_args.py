@@ -34,7 +34,8 @@ def lbackward(d, x=X, mask=MASK, w=W, st=ST, dy=DY, dx=DX, dw=DW, db=DB, ws=WS, 
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=3), dict(dtype=-1), dict(kind=2), dict(kind=-1), dict(n=-1), dict(points=-1), dict(n=(1 << 30) + 1),
-    dict(points=(1 << 30) + 1), dict(channels=0), dict(channels=(1 << 30) + 1), dict(eps=-1.0), dict(eps=float("nan")),
+    dict(points=(1 << 30) + 1), dict(n=1 << 30, points=1 << 30, x_strides=(0, 0), y_strides=(0, 0), mask_stride=0),
+    dict(channels=0), dict(channels=(1 << 30) + 1), dict(eps=-1.0), dict(eps=float("nan")),
     dict(eps=float("inf")), dict(x_strides=(-384, 384)), dict(x_strides=(361 * 384, -1)),
     dict(y_strides=(1 << 50, 384)), dict(mask_stride=-1), dict(mask_stride=1 << 62)])
 def test_layer_norm_refuses(kw):
