@@ -9,6 +9,15 @@
 // group of lanes sums its piece run by run, writes the runs that lie inside it, and leaves its first and last run to its
 // block, which joins those of its pieces; a last launch joins runs over blocks. Sums are float32: chains of at most a
 // piece, then the pieces of a block, then the blocks.
+//
+// What bounds it, measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
+//   forward, 57,767 tokens x 768 added to a sequence, bf16: 187 MB in 36.5 us, 5,110 GB/s (HBM)
+//   backward, 92,416 tokens x 384, 362 rows, bf16: 72 MB in 37.3 us: sort 15 us, sums 18 us (66% of the issue slots), joins
+//     6 us, the launches overlapping. The sort is 16 SMs' work: 5 us of ranks, 3 us for the exchange of the counts, 4 us
+//     to write 8-byte entries a sector each
+//   backward, 20,011 tokens x 512, 50,000 rows, float32: 143 MB in 48.0 us: sort 13 us, sums and zeros 26 us, joins 7 us
+// Not kept: zeros written by the SMs that the sort leaves idle (50.1 us), dy asked into L2 by them (45.8 us, but the
+// 92,416 tokens 40.2 us).
 
 #include <algorithm>
 #include <cmath>

@@ -12,6 +12,18 @@
 // Backward, a block goes over many rows and keeps the channels' sums in registers; a second launch adds the blocks' in
 // their order. Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read
 // again for each pass.
+//
+// What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an SM
+// that hold their rows, parameters and sums in registers. The rows behind the one at hand are on their way into shared
+// memory (loads straight into registers, one row at a time: 62 us where the ring takes 27); a mask is looked at a row
+// after it was asked for (34 us without). Measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
+//   forward, 256 boards x 361 x 384, layer norm, bf16, masked: 120 MB in 25.6 us, 4,680 GB/s
+//   forward, 64 x 361 x 768, layer norm, float32: 142 MB in 24.5 us, 5,800 GB/s
+//   backward, 128 x 361 x 768, RMS norm, bf16: 213 MB in 41.4 us, 5,160 GB/s
+//   backward, 256 x 361 x 384, layer norm, bf16, masked: 168 MB in 38.9 us, 4,310 GB/s
+// further from it: rows that begin anywhere (forward 256 x 361 x 384 of 387: 42.5 us, a window of 19 instructions each way
+// a vector), rows of a block (forward 9,000 x 4,096, bf16, RMS: 36.5 us of 22.5; barriers), single elements there (5,000 x
+// 4,099: 93 us of 12.5), rows read again (backward 1,000 x 20,000, float32: 150 us of 37).
 
 #include <algorithm>
 #include <cmath>
