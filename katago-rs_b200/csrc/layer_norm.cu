@@ -138,6 +138,9 @@ __device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32
   return UP && bytes & 16 ? hi : make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Rows of a ring, whose thread takes `row` bytes for each.
+constexpr int ring_depth(int row, bool backward) { return !backward && row * 4 <= 420 ? 4 : row * 3 <= 420 ? 3 : 2; }
+
 // A thread's vectors of the next rows, on their way into shared memory of its own (DEPTH rows, the one at hand among
 // them; no more than what 512 threads of an SM have room for). Rows that are off are not copied.
 // SHIFT: rows that begin anywhere. The aligned 16-byte pieces that hold the row are copied (such a piece never leaves the
@@ -149,7 +152,7 @@ struct Ring {
   using Slot = typename Copy::Slot;
   static constexpr int SLOTS = SHIFT ? NV + 1 : NV;  // of a tensor's row
   static constexpr int ROW = TENSORS * SLOTS * (int)sizeof(Slot);
-  static constexpr int DEPTH = TENSORS == 1 && ROW * 4 <= 420 ? 4 : ROW * 3 <= 420 ? 3 : 2;
+  static constexpr int DEPTH = ring_depth(ROW, TENSORS == 2);
   static size_t bytes(int threads) { return (size_t)DEPTH * ROW * threads; }
 
   Slot* mine;
@@ -813,9 +816,12 @@ Shape shape_of(int64_t rows, int C, int bytes, int vec, bool backward) {
   if (best >= 0) {
     s.threads = kThreads;
     const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
-    const int64_t per_sm = backward ? 2 : s.nv * whole <= 8 ? (s.shift ? 3 : 4)
-                                        : shared_params(s.vec, s.nv, false, s.shift) ? 3 : 2;  // by registers
-    s.blocks = std::min<int64_t>(all, per_sm * kSmCount);
+    // as many blocks as run at once, by registers and by the ring
+    const int by_registers = backward ? 2 : s.nv * whole <= 8 ? (s.shift ? 3 : 4)
+                                          : shared_params(s.vec, s.nv, false, s.shift) ? 3 : 2;
+    const int row = (backward ? 2 : 1) * (s.nv + (s.shift ? 1 : 0)) * 16;
+    const int by_ring = kMaxBlockSmem / (ring_depth(row, backward) * row * kThreads + 1024);
+    s.blocks = std::min<int64_t>(all, kSmCount * std::min(by_registers, by_ring));
     return s;
   }
   s.shift = false;
