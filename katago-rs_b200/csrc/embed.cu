@@ -290,14 +290,16 @@ template <int VEC>
 __device__ __forceinline__ void store_row(const SumParams& p, int id, int c, const float (&v)[VEC]) {
   if (id >= p.rows) return;
   float* out = p.dtable + (size_t)id * p.C + c;
-  if (VEC % 4 == 0 && p.wide) {
+  if (VEC % 4 == 0 && p.wide) {  // channels are a multiple of 4: whole float4s, of which the row may end behind one
 #pragma unroll
     for (int i = 0; i < VEC / 4; i++)
-      reinterpret_cast<float4*>(out)[i] = make_float4(v[4 * i] * p.scale, v[4 * i + 1] * p.scale,
-                                                      v[4 * i + 2] * p.scale, v[4 * i + 3] * p.scale);
+      if (c + 4 * i < p.C)
+        reinterpret_cast<float4*>(out)[i] = make_float4(v[4 * i] * p.scale, v[4 * i + 1] * p.scale,
+                                                        v[4 * i + 2] * p.scale, v[4 * i + 3] * p.scale);
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) out[i] = v[i] * p.scale;
+    for (int i = 0; i < VEC; i++)
+      if (c + i < p.C) out[i] = v[i] * p.scale;
   }
 }
 
@@ -327,15 +329,32 @@ __device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int co
 }
 
 // The block's pieces of the list. WHOLE: they are all there is, and no run goes on in another block.
+// SHIFT: rows of dy that begin anywhere. A lane reads an aligned 16-byte piece of the row (which never leaves the
+// allocation of the element in it); its vector is a window over that and the next lane's, so that the last lane of a group
+// has none. What lies behind the row's end is summed into channels that are not written.
 // slot: [first, last][group][lane][VEC], key: [first, last][group]
-template <typename T, int VEC, bool WHOLE>
+template <typename T, int VEC, bool SHIFT, bool WHOLE>
 __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int (*key)[kThreads / 2]) {
   using V = RowVec<T, VEC>;
   constexpr int SLOTS = kThreads * VEC;
   const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kThreads / lanes;
-  const int v = blockIdx.y * lanes + lane, c = v * VEC;
-  const bool here = v < p.C / VEC;
-  const T* dy = static_cast<const T*>(p.dy) + c;
+  const int per = SHIFT ? lanes - 1 : lanes;  // vectors of a group
+  const int v = blockIdx.y * per + lane, c = v * VEC;
+  const bool here = lane < per && c < p.C;
+  const T* dy = static_cast<const T*>(p.dy) + (SHIFT ? 0 : c);
+  // where a token's row begins in its first piece
+  auto begin = [&](int token) {
+    return ((uint32_t)reinterpret_cast<uintptr_t>(dy) + (uint32_t)token * (uint32_t)p.ys * (uint32_t)sizeof(T)) & 15u;
+  };
+  auto row = [&](int token) {
+    if constexpr (SHIFT) {
+      const uint32_t low = begin(token);
+      const T* piece = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(dy + token * p.ys) - low) + c;
+      return 16 * v < (int)(low + p.C * sizeof(T)) ? V::load(piece) : typename V::Raw{};
+    } else {
+      return here ? V::load(dy + token * p.ys) : typename V::Raw{};
+    }
+  };
   const int64_t i0 = ((int64_t)(WHOLE ? 0 : blockIdx.x) * groups + group) * p.piece;
   float acc[VEC];
 #pragma unroll
@@ -354,8 +373,7 @@ __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int 
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) e[u] = later[u];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++)
-      if (here && e[u].x < p.rows) raw[u] = V::load(dy + e[u].y * p.ys);
+    for (int u = 0; u < kUnroll; u++) raw[u] = e[u].x < p.rows ? row(e[u].y) : typename V::Raw{};
     look(e0 + kUnroll);
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
@@ -372,6 +390,14 @@ __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int 
         cur = e[u].x;
 #pragma unroll
         for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
+      }
+      if constexpr (SHIFT) {
+        uint4 next;
+        next.x = __shfl_down_sync(0xffffffffu, raw[u].x, 1, lanes);
+        next.y = __shfl_down_sync(0xffffffffu, raw[u].y, 1, lanes);
+        next.z = __shfl_down_sync(0xffffffffu, raw[u].z, 1, lanes);
+        next.w = __shfl_down_sync(0xffffffffu, raw[u].w, 1, lanes);
+        raw[u] = window<sizeof(T), false>(raw[u], next, begin(e[u].y));
       }
       if (here && cur < p.rows) {
         float f[VEC];
@@ -391,8 +417,8 @@ __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int 
   __syncthreads();
   // the groups' first and last runs in order, a thread to a channel
   const int width = lanes * VEC;
-  for (int j = threadIdx.x; j < width; j += kThreads) {
-    const int col = blockIdx.y * width + j;
+  for (int j = threadIdx.x; j < per * VEC; j += kThreads) {
+    const int col = blockIdx.y * per * VEC + j;
     if (col >= p.C) continue;
     float* part = WHOLE ? nullptr : p.part + (size_t)blockIdx.x * 2 * p.C + col;
     float sum = 0.0f;
@@ -418,19 +444,19 @@ __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int 
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFT>
 __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams p) {
   __shared__ float slot[2 * kThreads * VEC];
   __shared__ int key[2][kThreads / 2];
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, p.lanes * VEC, key[0]);
-  sum_pieces<T, VEC, false>(p, slot, key);
+  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, (p.lanes - SHIFT) * VEC, key[0]);
+  sum_pieces<T, VEC, SHIFT, false>(p, slot, key);
 }
 
 // Few tokens in one launch: every block sorts them in its shared memory, the first of each column of blocks sums, and all
 // share the rows that no token has.
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) embed_few_kernel(SumParams p, SortParams q, int passes) {
   __shared__ __align__(16) int2 list[2][kFewTokens];
   __shared__ __align__(16) int count[kThreads / 32 << kFewBits];
@@ -445,9 +471,9 @@ __global__ void __launch_bounds__(kThreads) embed_few_kernel(SumParams p, SortPa
     q.in = q.out;
   }
   p.list = list[0];
-  if (blockIdx.x == 0) sum_pieces<T, VEC, true>(p, reinterpret_cast<float*>(list[1]), key);
+  if (blockIdx.x == 0) sum_pieces<T, VEC, SHIFT, true>(p, reinterpret_cast<float*>(list[1]), key);
   for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < p.rows; row0 += (int64_t)gridDim.x * kThreads) {
-    absent_rows(p, (int)row0, p.lanes * VEC, absent);
+    absent_rows(p, (int)row0, (p.lanes - SHIFT) * VEC, absent);
     __syncthreads();
   }
 }
@@ -503,20 +529,24 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumParams p)
 // ---- host --------------------------------------------------------------------------------------------------------
 
 // Lanes of a row: the widest group that leaves at most an eighth of its lanes idle.
-int lanes_of(int nvec) {
-  for (int lanes = 32; lanes > 8; lanes /= 2)
-    if (((nvec + lanes - 1) / lanes * lanes - nvec) * 8 <= nvec) return lanes;
+// `shift`: one of them has no vector.
+int lanes_of(int nvec, bool shift) {
+  for (int lanes = 32; lanes > 8; lanes /= 2) {
+    const int per = lanes - shift;
+    if (((nvec + per - 1) / per * per - nvec) * 8 <= nvec) return lanes;
+  }
   return 8;
 }
 
 struct SumShape {
   int lanes, chunks, piece, blocks;
 };
-SumShape sum_shape(int64_t tokens, int C, int vec) {
+// `shift`: a group's last lane has no vector
+SumShape sum_shape(int64_t tokens, int C, int vec, bool shift) {
   SumShape s;
-  const int nvec = C / vec;
-  s.lanes = lanes_of(nvec);
-  s.chunks = (nvec + s.lanes - 1) / s.lanes;
+  const int nvec = (C + vec - 1) / vec;
+  s.lanes = lanes_of(nvec, shift);
+  s.chunks = (nvec + s.lanes - shift - 1) / (s.lanes - shift);
   const int groups = kThreads / s.lanes;
   // four blocks to an SM, of pieces of up to 256 entries
   const int64_t want = (tokens * s.chunks + (int64_t)4 * kSmCount * groups - 1) / ((int64_t)4 * kSmCount * groups);
@@ -563,8 +593,8 @@ Layout layout(const kc_embed_desc& d) {
   };
   const SortShape s = sort_shape(d.tokens, d.table_rows);
   int blocks = 0;
-  for (int v = 16 / dtype_bytes(d.dtype); v >= 1; v /= 2)
-    if (d.channels % v == 0) blocks = std::max(blocks, sum_shape(d.tokens, d.channels, v).blocks);
+  for (bool shift : {false, true})
+    blocks = std::max(blocks, sum_shape(d.tokens, d.channels, 16 / dtype_bytes(d.dtype), shift).blocks);
   l.a = take((size_t)d.tokens * sizeof(int2));
   if (s.passes > 1) l.b = take((size_t)d.tokens * sizeof(int2));
   if (!s.cluster) l.hist = take(((size_t)s.tiles << s.bits) * sizeof(int));
@@ -610,10 +640,10 @@ void sort_tokens(const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, i
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFT>
 void launch_sum(const SumParams& p, const SumShape& s, cudaStream_t st) {
   const unsigned absent = (unsigned)((p.rows + (int64_t)kThreads - 1) / kThreads);
-  launch_after(embed_sum_kernel<T, VEC>, dim3((unsigned)s.blocks + absent, (unsigned)s.chunks), dim3(kThreads), 0, st, p);
+  launch_after(embed_sum_kernel<T, VEC, SHIFT>, dim3((unsigned)s.blocks + absent, (unsigned)s.chunks), dim3(kThreads), 0, st, p);
   launch_after(embed_join_kernel, dim3((unsigned)s.blocks, (unsigned)((p.C + 31) / 32)), dim3(kThreads), 0, st, p);
 }
 
@@ -631,12 +661,13 @@ void run_type(const EmbedParams& p, int vec, unsigned blocks, cudaStream_t st) {
   KC_CUDA(cudaGetLastError());
 }
 
-// One launch where a group of lanes with 64 bytes of a row each, 32 tokens to a group at most, has all tokens in a block
-// (361 tokens x 384, 362 rows, f16: 12.0 us in three launches).
-template <typename T, int VEC>
+// One launch where groups of four lanes, 32 tokens to a group at most, have all tokens in a block (361 tokens x 384, 362
+// rows, f16: 13.7 us, 12.0 us in three launches, but 16 and 22 us with the calls' time on the host).
+template <typename T, int VEC, bool SHIFT>
 bool launch_few(SumParams p, const int32_t* ids, cudaStream_t st) {
-  p.lanes = std::max(4, 64 / (VEC * (int)sizeof(T)));
-  const int groups = kThreads / p.lanes, chunks = (p.C / VEC + p.lanes - 1) / p.lanes;
+  p.lanes = 4;
+  const int groups = kThreads / p.lanes, per = p.lanes - SHIFT, nvec = (p.C + VEC - 1) / VEC;
+  const int chunks = (nvec + per - 1) / per;
   if (p.tokens > std::min(kFewTokens, 32 * groups) || chunks > 2 * kSmCount) return false;
   p.piece = (p.tokens + groups * kUnroll - 1) / (groups * kUnroll) * kUnroll;
   int bits = 1;
@@ -644,31 +675,23 @@ bool launch_few(SumParams p, const int32_t* ids, cudaStream_t st) {
   const int passes = (bits + kFewBits - 1) / kFewBits;
   const SortParams q{ids, nullptr, nullptr, nullptr, p.tokens, p.rows, 0, (bits + passes - 1) / passes, 1, p.tokens};
   const int64_t rows = (p.rows + (int64_t)kThreads - 1) / kThreads, most = std::max(1, 4 * kSmCount / chunks);
-  embed_few_kernel<T, VEC><<<dim3((unsigned)std::min(rows, most), (unsigned)chunks), kThreads, 0, st>>>(p, q, passes);
+  const dim3 grid((unsigned)std::min(rows, most), (unsigned)chunks);
+  embed_few_kernel<T, VEC, SHIFT><<<grid, kThreads, 0, st>>>(p, q, passes);
   KC_CUDA(cudaGetLastError());
   return true;
 }
 
-template <typename T, int VEC>
-void sum_vec(SumParams p, const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, int* hist, cudaStream_t st) {
-  if (launch_few<T, VEC>(p, ids, st)) return;
+template <typename T, bool SHIFT>
+void sum_type(SumParams p, const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, int* hist, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (launch_few<T, VEC, SHIFT>(p, ids, st)) return;
   sort_tokens(d, ids, a, b, hist, st);
-  const SumShape s = sum_shape(d.tokens, d.channels, VEC);
+  const SumShape s = sum_shape(d.tokens, d.channels, VEC, SHIFT);
   p.list = a;
   p.lanes = s.lanes;
   p.piece = s.piece;
   p.blocks = s.blocks;
-  launch_sum<T, VEC>(p, s, st);
-}
-
-template <typename T>
-void sum_type(const SumParams& p, const kc_embed_desc& d, int vec, const int32_t* ids, int2* a, int2* b, int* hist,
-              cudaStream_t st) {
-  if constexpr (sizeof(T) == 2)
-    if (vec == 8) return sum_vec<T, 8>(p, d, ids, a, b, hist, st);
-  if (vec == 4) return sum_vec<T, 4>(p, d, ids, a, b, hist, st);
-  if (vec == 2) return sum_vec<T, 2>(p, d, ids, a, b, hist, st);
-  sum_vec<T, 1>(p, d, ids, a, b, hist, st);
+  launch_sum<T, VEC, SHIFT>(p, s, st);
 }
 
 Rows rows_of(const kc_embed_desc& d, const void* p, int64_t count, int64_t stride) {
@@ -723,7 +746,7 @@ extern "C" int kc_embed_rows(const kc_embed_desc* desc, const int32_t* d_ids, co
     EmbedParams p{d_ids, d_table, d_x, d_y, d.tokens, d.table_rows, table.outer_stride, x.outer_stride,
                   y.outer_stride, d.channels, 0, d.scale};
     const int vec = d_x ? vec_of(d, {table, x, y}) : vec_of(d, {table, y});
-    p.lanes = lanes_of(d.channels / vec);
+    p.lanes = lanes_of(d.channels / vec, false);
     const int64_t per = kThreads / p.lanes;
     const unsigned blocks = (unsigned)std::min<int64_t>((d.tokens + per - 1) / per, 1 << 20);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -769,7 +792,7 @@ extern "C" int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* 
     char* ws = static_cast<char*>(d_workspace);
     int2 *a = reinterpret_cast<int2*>(ws + l.a), *b = reinterpret_cast<int2*>(ws + l.b);
     int* hist = reinterpret_cast<int*>(ws + l.hist);
-    const int vec = vec_of(d, {dy});
+    const bool shift = vec_of(d, {dy}) * dy.bytes < 16;
     SumParams p{};
     p.dy = d_dy;
     p.dtable = d_dtable;
@@ -781,8 +804,12 @@ extern "C" int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* 
     p.C = d.channels;
     p.wide = d.channels % 4 == 0 && aligned_to(d_dtable, 16);
     p.scale = d.scale;
-    if (d.dtype == KC_PRECISION_F32) sum_type<float>(p, d, vec, d_ids, a, b, hist, st);
-    else if (d.dtype == KC_PRECISION_F16) sum_type<__half>(p, d, vec, d_ids, a, b, hist, st);
-    else sum_type<__nv_bfloat16>(p, d, vec, d_ids, a, b, hist, st);
+    auto run = [&](auto zero) {
+      using T = decltype(zero);
+      shift ? sum_type<T, true>(p, d, d_ids, a, b, hist, st) : sum_type<T, false>(p, d, d_ids, a, b, hist, st);
+    };
+    if (d.dtype == KC_PRECISION_F32) run(0.0f);
+    else if (d.dtype == KC_PRECISION_F16) run(__half{});
+    else run(__nv_bfloat16{});
   });
 }

@@ -123,21 +123,6 @@ struct Units {
   }
 };
 
-// A vector that begins `bytes` (0 to 15, UP: 1 to 16) into 32 bytes; ELEMENT bytes divide it.
-template <int ELEMENT, bool UP>
-__device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32_t bytes) {
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-  for (int k = 0; k < 6; k++) w[k] = bytes & 8 ? w[k + 2] : w[k];
-#pragma unroll
-  for (int k = 0; k < 5; k++) w[k] = bytes & 4 ? w[k + 1] : w[k];
-  if (ELEMENT == 2) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(w[k], w[k + 1], (bytes & 2) * 8);
-  }
-  return UP && bytes & 16 ? hi : make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Rows of a ring, whose thread takes `row` bytes for each.
 constexpr int ring_depth(int row, bool backward) { return !backward && row * 4 <= 420 ? 4 : row * 3 <= 420 ? 3 : 2; }
 

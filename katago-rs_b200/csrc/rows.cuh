@@ -128,6 +128,21 @@ __device__ __forceinline__ void load_params(const float* p, bool wide, float (&v
   }
 }
 
+// A vector that begins `bytes` (0 to 15, UP: 1 to 16) into 32 bytes; ELEMENT bytes divide it.
+template <int ELEMENT, bool UP>
+__device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32_t bytes) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int k = 0; k < 6; k++) w[k] = bytes & 8 ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; k++) w[k] = bytes & 4 ? w[k + 1] : w[k];
+  if (ELEMENT == 2) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(w[k], w[k + 1], (bytes & 2) * 8);
+  }
+  return UP && bytes & 16 ? hi : make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Sums over groups of `lanes` neighbouring lanes of a warp (a power of two; every lane of the warp takes part).
 __device__ __forceinline__ float2 lanes_sum(float2 v, int lanes) {
 #pragma unroll
