@@ -16,6 +16,8 @@
 //     6 us, the launches overlapping. The sort is 16 SMs' work: 5 us of ranks, 3 us for the exchange of the counts, 4 us
 //     to write 8-byte entries a sector each
 //   backward, 20,011 tokens x 512, 50,000 rows, float32: 143 MB in 48.0 us: sort 13 us, sums and zeros 26 us, joins 7 us
+//   rows that begin anywhere: forward, 57,767 x 768 of 771, bf16: 63 us (72 us an element or two at a time); backward,
+//     92,416 x 384 of 387, bf16: 52.5 us (75 us)
 // Not kept: zeros written by the SMs that the sort leaves idle (50.1 us), dy asked into L2 by them (45.8 us, but the
 // 92,416 tokens 40.2 us).
 
@@ -87,6 +89,72 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const EmbedParams p) {
           for (int j = 0; j < VEC; j++) o[j] = fmaf(f[j], p.scale, o[j]);
         }
         V::store(y + v * VEC, V::pack(o));
+      }
+    }
+  }
+}
+
+// The same for rows that begin anywhere: aligned 16-byte pieces of the rows are read and written, each by a lane; a
+// vector is a window over a lane's piece and the next lane's, and a piece to write one over the lane before's vector and
+// its own. So lanes 1 to lanes - 2 of a group write; lane 0 has the last vector of the pieces before. (In place, no piece
+// is read after its row's elements have been written.)
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embed_shift_kernel(const EmbedParams p) {
+  constexpr int VEC = 16 / sizeof(T), BATCH = 2;
+  using V = RowVec<T, VEC>;
+  const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1), per = kThreads / lanes, mine = lanes - 2;
+  const int pieces = (p.C + VEC - 1) / VEC + 1, bytes = p.C * (int)sizeof(T);
+  auto low_of = [](const void* q) { return (uint32_t)reinterpret_cast<uintptr_t>(q) & 15u; };
+  auto piece_of = [](const T* row, uint32_t low, int q) {
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) - low + 16 * (intptr_t)q);
+  };
+  auto from = [&](const uint4& w, int source) {
+    return make_uint4(__shfl_sync(0xffffffffu, w.x, source, lanes), __shfl_sync(0xffffffffu, w.y, source, lanes),
+                      __shfl_sync(0xffffffffu, w.z, source, lanes), __shfl_sync(0xffffffffu, w.w, source, lanes));
+  };
+  for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < p.tokens; t0 += (int64_t)gridDim.x * per) {
+    const int64_t t = t0 + threadIdx.x / lanes;
+    const bool here = t < p.tokens;
+    const int id = here ? __ldg(p.ids + t) : -1;
+    const bool there = id >= 0 && id < p.table_rows;
+    const T* row = static_cast<const T*>(p.table) + (there ? id * p.ts : 0);
+    const T* x = static_cast<const T*>(p.x) + (here ? t * p.xs : 0);
+    T* y = static_cast<T*>(p.y) + (here ? t * p.ys : 0);
+    const uint32_t low_t = low_of(row), low_x = low_of(x), low_y = low_of(y);
+    const int skip = (int)(low_y / sizeof(T));
+    uint4 carry{};
+    for (int v0 = 0; v0 < pieces; v0 += BATCH * mine) {
+      uint4 a[BATCH], b[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; k++) {
+        const int q = v0 + k * mine + lane - 1;
+        a[k] = there && lane > 0 && 16 * q < (int)low_t + bytes ? piece_of(row, low_t, q) : uint4{};
+        if (p.x) b[k] = here && lane > 0 && 16 * q < (int)low_x + bytes ? piece_of(x, low_x, q) : uint4{};
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; k++) {
+        const int q = v0 + k * mine + lane - 1;
+        float f[VEC], o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o[j] = 0.0f;
+        if (p.x) V::unpack(window<sizeof(T), false>(b[k], from(b[k], lane + 1), low_x), o);
+        V::unpack(window<sizeof(T), false>(a[k], from(a[k], lane + 1), low_t), f);
+        if (there)
+#pragma unroll
+          for (int j = 0; j < VEC; j++) o[j] = fmaf(f[j], p.scale, o[j]);
+        const uint4 vec = lane == 0 ? carry : V::pack(o);
+        carry = from(vec, lanes - 2);
+        const uint4 piece = window<sizeof(T), true>(from(vec, lane - 1), vec, 16 - low_y);
+        const int c = q * VEC - skip;
+        if (!here || lane == 0 || lane == lanes - 1 || c >= p.C) continue;
+        if (c >= 0 && c + VEC <= p.C) {
+          *reinterpret_cast<uint4*>(y + c) = piece;
+        } else {
+          const T* e = reinterpret_cast<const T*>(&piece);
+#pragma unroll
+          for (int j = 0; j < VEC; j++)
+            if (c + j >= 0 && c + j < p.C) y[c + j] = e[j];
+        }
       }
     }
   }
@@ -528,14 +596,14 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumParams p)
 
 // ---- host --------------------------------------------------------------------------------------------------------
 
-// Lanes of a row: the widest group that leaves at most an eighth of its lanes idle.
-// `shift`: one of them has no vector.
-int lanes_of(int nvec, bool shift) {
-  for (int lanes = 32; lanes > 8; lanes /= 2) {
-    const int per = lanes - shift;
-    if (((nvec + per - 1) / per * per - nvec) * 8 <= nvec) return lanes;
-  }
-  return 8;
+// Lanes of a row, `idle` of which have no vector: the groups that need the fewest lanes in all, the widest of them; the
+// narrowest of those with two idle lanes (60,000 tokens x 377, bf16, forward: 56 us with 32 lanes).
+int lanes_of(int nvec, int idle) {
+  int best = 32;
+  auto all = [&](int lanes) { return (int64_t)(nvec + lanes - idle - 1) / (lanes - idle) * lanes; };
+  for (int lanes = 16; lanes >= 8; lanes /= 2)
+    if (all(lanes) < all(best) || (idle == 2 && all(lanes) == all(best))) best = lanes;
+  return best;
 }
 
 struct SumShape {
@@ -648,16 +716,9 @@ void launch_sum(const SumParams& p, const SumShape& s, cudaStream_t st) {
 }
 
 template <typename T>
-void run_type(const EmbedParams& p, int vec, unsigned blocks, cudaStream_t st) {
-  if (vec == 8) {
-    if constexpr (sizeof(T) == 2) embed_kernel<T, 8><<<blocks, kThreads, 0, st>>>(p);
-  } else if (vec == 4) {
-    embed_kernel<T, 4><<<blocks, kThreads, 0, st>>>(p);
-  } else if (vec == 2) {
-    embed_kernel<T, 2><<<blocks, kThreads, 0, st>>>(p);
-  } else {
-    embed_kernel<T, 1><<<blocks, kThreads, 0, st>>>(p);
-  }
+void run_type(const EmbedParams& p, bool shift, unsigned blocks, cudaStream_t st) {
+  if (shift) embed_shift_kernel<T><<<blocks, kThreads, 0, st>>>(p);
+  else embed_kernel<T, 16 / sizeof(T)><<<blocks, kThreads, 0, st>>>(p);
   KC_CUDA(cudaGetLastError());
 }
 
@@ -745,14 +806,16 @@ extern "C" int kc_embed_rows(const kc_embed_desc* desc, const int32_t* d_ids, co
     TensorDevice dev("looked-up rows", {d_ids, d_table, d_x, d_y});
     EmbedParams p{d_ids, d_table, d_x, d_y, d.tokens, d.table_rows, table.outer_stride, x.outer_stride,
                   y.outer_stride, d.channels, 0, d.scale};
-    const int vec = d_x ? vec_of(d, {table, x, y}) : vec_of(d, {table, y});
-    p.lanes = lanes_of(d.channels / vec, false);
+    const int whole = 16 / dtype_bytes(d.dtype);
+    const bool shift = (d_x ? vec_of(d, {table, x, y}) : vec_of(d, {table, y})) < whole;
+    const int nvec = (d.channels + whole - 1) / whole;
+    p.lanes = lanes_of(shift ? nvec + 1 : nvec, shift ? 2 : 0);
     const int64_t per = kThreads / p.lanes;
     const unsigned blocks = (unsigned)std::min<int64_t>((d.tokens + per - 1) / per, 1 << 20);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (d.dtype == KC_PRECISION_F32) run_type<float>(p, vec, blocks, st);
-    else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, vec, blocks, st);
-    else run_type<__nv_bfloat16>(p, vec, blocks, st);
+    if (d.dtype == KC_PRECISION_F32) run_type<float>(p, shift, blocks, st);
+    else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, shift, blocks, st);
+    else run_type<__nv_bfloat16>(p, shift, blocks, st);
   });
 }
 

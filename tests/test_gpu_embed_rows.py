@@ -97,7 +97,7 @@ def test_three_digits():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("channels", [64, 100, 33])
+@pytest.mark.parametrize("channels", [64, 100, 33, 1, 1001, 2000])
 def test_strides_guards_and_in_place(dtype, channels):
     tokens, rows = 500, 40
     ids, table, x, g = make(tokens, channels, rows, dtype, 11)
