@@ -190,14 +190,21 @@ __global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortPar
   for (int b = threadIdx.x; b < bins; b += kSortThreads) count[b] = 0;
   __syncthreads();
   const int i0 = blockIdx.x * p.tile, i1 = min(p.tokens, i0 + p.tile);
-  for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
-    const int d = sort_entry<SortIn::kTiles>(p, i).x >> p.shift & (bins - 1);
-    const uint32_t peers = __match_any_sync(__activemask(), d);
-    if (threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&count[d], __popc(peers));
+  const int lane = threadIdx.x % 32;
+  for (int i = i0 + threadIdx.x; i - lane < i1; i += kSortThreads) {  // a warp's lanes stay together
+    const int d = i < i1 ? sort_entry<SortIn::kTiles>(p, i).x >> p.shift & (bins - 1) : bins;
+    const uint32_t peers = __match_any_sync(0xffffffffu, d);
+    if (d < bins && lane == __ffs(peers) - 1) atomicAdd(&count[d], __popc(peers));
   }
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kSortThreads) p.hist[(size_t)blockIdx.x * bins + b] = count[b];
 }
+
+// The two halves of cluster_sync.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Places the tile's entries. Each warp owns a share of consecutive entries: it counts its digits, takes its places
 // behind those of the tiles and warps before it, and goes over them again. The tiles' counts are in p.hist; a cluster with
@@ -246,6 +253,8 @@ __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* c
   // thread b: digit b's places
   int before = 0, total = 0;
   if (IN != SortIn::kTiles) {
+    // no block writes into another one's shared memory before that has started (embed_sort_kernel)
+    if (IN == SortIn::kCluster && p.ids && p.tiles > 1) cluster_wait();
     if (threadIdx.x < bins) {
 #pragma unroll
       for (int w = 0; w < WARPS; w++) total += count[w * bins + threadIdx.x];
@@ -328,6 +337,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p, 
   __shared__ int scan[kSortWarps];
   int* totals = count + (kSortWarps << p.bits);
   pdl_trigger();
+  if (p.tiles > 1) cluster_arrive();
   for (int i = 0; i < passes; i++) {
     p.out = (passes - i) % 2 ? a : b;  // the last pass ends in a
     p.shift = i * p.bits;

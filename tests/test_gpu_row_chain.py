@@ -180,3 +180,43 @@ print("captured")
     code = code % (here, os.path.join(os.path.dirname(here), "katago-rs_b200", "python"))
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
+
+
+def test_offsets_beyond_32_bits():
+    """Boards, table rows and logit rows 2^31 elements apart (and an odd number more). Lookups and losses have the bits of
+    single rows; norms are within 2^-10 of the value (half a step of f16 is 2^-11) and 2^-12 of a standard deviation."""
+    buf = torch.zeros(2**31 + 70000, device="cuda", dtype=torch.float16)
+    out = torch.zeros(2**31 + 70000, device="cuda", dtype=torch.float16)
+    for far in (2**31, 2**31 + 7):
+        g = torch.Generator(device="cuda").manual_seed(7)
+        v = torch.randn(2, 5, 384, device="cuda", generator=g).half()
+        w = torch.rand(384, device="cuda", generator=g)
+        x, y = (b.as_strided((2, 5, 384), (far, 384, 1)) for b in (buf, out))
+        x.copy_(v)
+        got = r.layer_forward(x, None, w, w, "layer", y=y)
+        on = torch.ones(2, 5, dtype=torch.bool, device="cuda")
+        want = r.layer64(v, on, w, w, "layer")[0]
+        assert ((y.double() - want).abs() <= 2.0**-10 * want.abs() + 2.0**-12).all()
+        dx = r.layer_backward(x, None, w, got[1], y, "layer", dx=buf.as_strided((2, 5, 384), (far, 384, 1)))[0]
+        want = r.layer_back64(v, on, w, got[1][..., 0], got[1][..., 1], y, "layer")[0]
+        assert ((dx.double() - want).abs() <= 2.0**-10 * want.abs() + 2.0**-12).all()
+
+        table, rows = (b.as_strided((2, 384), (far, 1)) for b in (buf, out))
+        table.copy_(v[:, 0])
+        ids = torch.tensor([1, 0], device="cuda", dtype=torch.int32)
+        r.embed_forward(ids, table, table, 1.0, y=rows)
+        assert torch.equal(rows, (v[:, 0].float().flip(0) + v[:, 0].float()).half())
+        grad = r.embed_backward(ids, rows, 2)
+        assert torch.equal(grad, rows.float().flip(0))
+
+        for classes in (362, 30000):
+            z = buf.as_strided((2, classes), (far, 1))
+            z.copy_(torch.randn(2, classes, device="cuda", generator=g))
+            tid = torch.randint(0, classes, (2, 9), device="cuda", generator=g, dtype=torch.int32)
+            top = torch.randn(2, 9, device="cuda", generator=g)
+            loss, st = r.distill_forward(z, tid, top)
+            dz = r.distill_backward(z, tid, top, st, dz=out.as_strided((2, classes), (far, 1)))
+            for i in range(2):
+                l1, s1 = r.distill_forward(z[i:i + 1], tid[i:i + 1], top[i:i + 1])
+                assert torch.equal(loss[i:i + 1], l1) and torch.equal(st[i:i + 1], s1)
+                assert torch.equal(dz[i:i + 1], r.distill_backward(z[i:i + 1], tid[i:i + 1], top[i:i + 1], s1))
