@@ -10,7 +10,7 @@
 // one read, one write. The variance is taken around the float32 mean of the first pass, whose own error the second
 // pass finds (the sum of the distances), so that a large mean costs neither digits of the variance nor of x - mean.
 // Backward, a block goes over many rows and keeps the channels' sums in registers; a second launch adds the blocks' in
-// their order. Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read
+// their order (few rows: a cluster adds its own). Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read
 // again for each pass.
 //
 // What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an SM
@@ -56,6 +56,7 @@ struct LayerParams {
   int C, lanes;
   int kind;
   int wide;        // weight and bias are 16-byte aligned
+  int cluster;     // backward: all blocks are one cluster of so many, which adds their sums itself; 0: `part`
   float eps;
 };
 
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
     if constexpr (SHIFT) at.store_shifted(out, p.C, raw, here);
   }
   copy_wait<0>();
-  if (!p.part) return;
+  if (!p.dweight && !p.dbias) return;
   // slot (which, i, j, lane) holds the sum of channel (lane + i lanes) VEC + j (element i VEC + j)
   constexpr int E = NV * VEC;
   const int slots = E * g.lanes;
@@ -592,12 +593,30 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
     }
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < (LEAN ? 1 : 2) * slots; k += kThreads) {
+  const int all = (LEAN ? 1 : 2) * slots;
+  for (int k = threadIdx.x; k < all; k += kThreads) {
     float s = 0.0f;
 #pragma unroll
     for (int v = 0; v < kThreads / 32; v++) s += sums[v * 2 * slots + k];
-    part[k] = s;
+    if (p.cluster) sums[k] = s;  // read by this thread alone so far
+    else part[k] = s;
   }
+  if (!p.cluster) return;
+  // each block of the cluster adds a share of the slots over all of them
+  cluster_sync();
+  for (int k = blockIdx.x * kThreads + threadIdx.x; k < all; k += p.cluster * kThreads) {
+    float s = 0.0f;
+    for (int t = 0; t < p.cluster; t++) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(sums + k), t)) : "memory");
+      s += v;
+    }
+    const int slot = k < slots ? k : k - slots, e = slot / g.lanes;
+    const int c = (slot % g.lanes + e / VEC * g.lanes) * VEC + e % VEC;
+    float* out = k < slots ? p.dweight : p.dbias;
+    if (out && c < p.C) out[c] = s;
+  }
+  cluster_sync();  // no block's shared memory goes before it has been read
 }
 
 // Rows that registers do not hold: a block to a row, read again for each pass.
@@ -845,8 +864,19 @@ void launch_back(const LayerParams& p, const Shape& s, cudaStream_t st) {
   // the ring, and in its place the warps' sums
   const size_t sums = BLOCK ? 0 : (size_t)kThreads / 32 * 2 * NV * VEC * s.lanes * sizeof(float);
   const size_t smem = std::max(Ring<T, VEC, NV, BLOCK, 2, SHIFT>::bytes(s.threads), sums);
-  allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN>>();
-  layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN><<<(unsigned)s.blocks, s.threads, smem, st>>>(p);
+  allow_block_smem<layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN>, !BLOCK>();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)s.blocks);
+  cfg.blockDim = dim3(s.threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster ? 1 : 0;
+  KC_CUDA(cudaLaunchKernelEx(&cfg, layer_norm_back_kernel<T, VEC, NV, BLOCK, SHIFT, LEAN>, p));
 }
 
 template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT>
@@ -924,12 +954,23 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
   p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);
   p.mm = row_map(d.n, d.points, d.mask_board_stride, 1);
-  const Shape s = shape_of(p.rows, p.C, dtype_bytes(d.dtype), vec, backward);
+  Shape s = shape_of(p.rows, p.C, dtype_bytes(d.dtype), vec, backward);
   p.lanes = s.lanes;
+  // few rows: one cluster of up to 16 blocks, whose groups of lanes have 4 rows each at most, and no second launch (361 x
+  // 384, RMS, bf16, with the call's time on the host: 21.0 us, 23.5 in two launches; 8.3 and 7.9 us on the device. With 16
+  // rows a group, 7,261 x 100, f16, took 29 us on the device, 10.5 over all SMs)
+  if (p.part && !s.block && !s.is_long) {
+    const int64_t groups = kThreads / s.lanes;
+    if (p.rows <= 16 * 4 * groups) {
+      p.cluster = 1;
+      while (p.cluster < 16 && p.cluster * groups < p.rows) p.cluster *= 2;
+      s.blocks = p.cluster;
+    }
+  }
   if (d.dtype == KC_PRECISION_F32) run_type<float>(p, s, backward, st);
   else if (d.dtype == KC_PRECISION_F16) run_type<__half>(p, s, backward, st);
   else run_type<__nv_bfloat16>(p, s, backward, st);
-  if (!p.part) return;
+  if (!p.part || p.cluster) return;
   const PartShape q = part_shape(s, p.rows, p.C);
   const int64_t slots = (int64_t)q.slots * ((p.dweight ? 1 : 0) + (p.dbias ? 1 : 0));
   launch_after(layer_norm_params_kernel, dim3((unsigned)std::min<int64_t>((slots + 31) / 32, 1 << 20)), dim3(1024), 0, st,

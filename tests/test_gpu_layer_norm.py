@@ -89,6 +89,17 @@ def test_forward_and_backward(n, points, channels, pad, dtype, kind):
         check_backward(x, mask, w, stats, dy, kind, dx, dw, db)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 16, 17, 64, 255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 8192, 8193])
+def test_ends_of_the_ways_to_add(rows, dtype):
+    """Parameter gradients by clusters of 1 to 16 blocks and by a second launch, of 4 to 128 rows to a block at once."""
+    for channels, pad in ((384, 0), (100, 3), (9, 0), (16, 0)):
+        x, dy, w, b, mask = make(1, rows, channels, dtype, rows, rows % 2 == 0, pad)
+        for kind in r.KINDS:
+            y, stats = r.layer_forward(x, mask, w, b, kind)
+            check_backward(x, mask, w, stats, dy, kind, *r.layer_backward(x, mask, w, stats, dy, kind))
+
+
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_many_rows(kind):
     """A block goes over many rows: 92,416 x 96 over at most 296 blocks of 16 rows or more, chains of 20."""
