@@ -238,7 +238,8 @@ int kc_gpool_fc_noalloc(const float* d_x, const float* d_mask, int n, int c, con
  * the input of its own shape (same pointer and strides: in place); any other overlap of an output is refused.
  * `d_workspace` (16-byte aligned, contents not kept) must not be used by two calls that can overlap on the GPU, nor
  * be freed before a graph that captured it. Calls on different streams are otherwise independent. Results do not
- * depend on timing: the same call gives the same bits.
+ * depend on timing: the same call gives the same bits. Rows that do not lie on 16 bytes may be read in the aligned
+ * 16-byte pieces that hold them; what else such a piece holds has no effect, and is not written.
  * --------------------------------------------------------------------------------------------------------------- */
 #define KC_ACT_IDENTITY 0
 #define KC_ACT_RELU 1
@@ -338,8 +339,8 @@ typedef struct kc_layer_norm_desc {
 
 /* y = (x - mean) * rstd * weight[c] + bias[c] at the tokens whose mask is not 0, 0 at the others (whatever x holds there
  * has no effect), with the mean (0 for RMS) and rstd = 1 / sqrt(mean square distance from it + eps) of the token's row.
- * Squares are summed in float32: a row whose sum passes 3.4e38 has NaN in y and rstd. d_mask: [n][points] float32 rows at
- * mask_board_stride, NULL = every token; d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not
+ * Squares are summed in float32: a row whose sum passes 3.4e38 has NaN in y and rstd. d_mask: [n][points] float32 rows
+ * at mask_board_stride, NULL = every token; d_weight, d_bias: [channels] float32, NULL = 1 and 0. d_stats (NULL = not
  * wanted): [n][points][2] float32 mean and rstd, both 0 where the token is off. */
 int kc_layer_norm(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
                   const float* d_bias, void* d_y, float* d_stats, void* stream);
@@ -379,8 +380,8 @@ int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* d_ids, cons
 /* Distillation: the loss of a student's logits (policy rows of 362 moves, or any classes) against a teacher's top
  * logits. With q = softmax(logits / T) and p[j] = exp(top_logits[j] / T - L) over the row's entries j,
  *   loss = T^2 * sum over j of p[j] * (log p[j] - log q[id[j]]),
- * L = the entries' own log sum of exp(top_logits / T) (p adds up to 1), or d_teacher_log_sum[row], the teacher's over all
- * its classes (p adds up to what the entries hold of it; the rest of the teacher's distribution is left out). */
+ * L = the entries' own log sum of exp(top_logits / T) (p adds up to 1), or d_teacher_log_sum[row], the teacher's over
+ * all its classes (p adds up to what the entries hold of it; the rest of the teacher's distribution is left out). */
 typedef struct kc_distill_desc {
   int32_t dtype;     /* KC_PRECISION_* of logits and dlogits */
   int32_t classes;   /* 1 .. 2^30 */

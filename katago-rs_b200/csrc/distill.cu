@@ -5,21 +5,23 @@
 //   loss = T^2 sum_j p_j (log p_j - log q_{id_j})
 //   dz_i = dloss T (P q_i - sum_{j: id_j = i} p_j), P = sum_j p_j
 //
-// The teacher's side of a row is a few entries, held by the threads that share the row: exponentials of differences taken
-// in 64 bits, and sums in 64 bits, since the loss is a difference of logarithms. With e_j = exp((t_j - max t) / T) the
-// loss is T^2 (sum e_j x_j / sum e_j + log(s / sum e_j)), x_j = ((t_j - max t) - (z_{id_j} - m)) / T, from the row's
-// largest logit m and s = sum exp((z - m) / T): one logarithm a row.
+// The teacher's side of a row is a few entries, held by the threads that share the row: exponentials of differences
+// taken in 64 bits, and sums in 64 bits, since the loss is a difference of logarithms. With e_j = exp((t_j - max t) /
+// T) the loss is T^2 (sum e_j x_j / sum e_j + log(s / sum e_j)), x_j = ((t_j - max t) - (z_{id_j} - m)) / T, from the
+// row's largest logit m and s = sum exp((z - m) / T): one logarithm a row.
 // Backward, the saved (m, s) make each element's gradient one exponential; the entries' classes are gathered before the
 // row is written, so that the gradient may take the logits' place, and written over it at the end. Rows without entries
 // are not read.
 //
-// Rows of at most 2,048 classes are a warp's, which keeps the row in shared memory while the next one is on its way there;
-// longer ones a block's or, where rows are few, a cluster's (forward) or several blocks' (backward).
+// Rows of at most 2,048 classes are a warp's, which keeps the row in shared memory while the next one is on its way
+// there; longer ones a block's or, where rows are few, a cluster's (forward) or several blocks' (backward).
 //
 // What bounds it, measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
-//   backward, 4,096 rows x 32,000, 128 entries, bf16: 513 MB in 91.7 us, 5,590 GB/s (HBM)
-//   forward, the same: 251 MB in 59.8 us, 4,200 GB/s: exponentials (16 a clock and SM: 29 us) and 51% of the issue slots
-//   backward, 16,384 rows x 362, 64 entries, bf16: 32 MB in 14.3 us: 580 warp instructions a row, most of them the entries'
+//   backward, 4,096 rows x 32,000, 128 entries, bf16: 513 MB in 91.0 us, 5,640 GB/s (HBM)
+//   forward, the same: 251 MB in 59.8 us, 4,200 GB/s: exponentials (16 a clock and SM: 29 us) and 51% of the issue
+//     slots
+//   backward, 16,384 rows x 362, 64 entries, bf16: 32 MB in 14.3 us: 580 warp instructions a row, most of them the
+//     entries'
 //   forward, 60,000 rows x 362, 32 entries, bf16: 57 MB in 32 us: 424 warp instructions a row, 75% of the issue slots
 // With loops over the entries in memory, all in 64 bits, these took 99, 67, 29 and 73 us.
 
@@ -108,13 +110,15 @@ struct Chunk {
   static constexpr int VEC = 16 / sizeof(T), N = VEC / 2;
   using V = RowVec<T, VEC>;
   __device__ static __forceinline__ uint4 nothing() {  // elements of -inf
-    const uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    const uint32_t w = std::is_same<T, float>::value ? 0xff800000u
+                       : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
     return make_uint4(w, w, w, w);
   }
   __device__ static __forceinline__ float largest(const uint4& r) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
     if constexpr (std::is_same<T, float>::value) {
-      return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+      return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                   fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
     } else {
       using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
       const T2* h = reinterpret_cast<const T2*>(&r);
@@ -233,12 +237,14 @@ __device__ __forceinline__ void write_nothing(const DistillParams& p, int64_t r)
 }
 
 // ---- rows of a warp ----------------------------------------------------------------------------------------------
-// The aligned 16-byte pieces that hold a row, in shared memory (such a piece never leaves the allocation of the element in
-// it); the elements of the first and last one that are not the row's become -inf.
+// The aligned 16-byte pieces that hold a row, in shared memory (such a piece never leaves the allocation of the element
+// in it); the elements of the first and last one that are not the row's become -inf.
 template <typename T>
 struct WarpRow {
   static constexpr int VEC = 16 / sizeof(T);
-  static int bytes(int64_t classes) { return (int)std::min<int64_t>((classes * (int)sizeof(T) + 30) / 16 * 16, 1 << 16); }
+  static int bytes(int64_t classes) {
+    return (int)std::min<int64_t>((classes * (int)sizeof(T) + 30) / 16 * 16, 1 << 16);
+  }
   T* buf;
   __device__ __forceinline__ static int pieces(int lead, int classes) { return (lead + classes + VEC - 1) / VEC; }
   __device__ __forceinline__ void fetch(const T* z, int classes, int lane) const {
@@ -369,7 +375,8 @@ __global__ void __launch_bounds__(kThreads, 4) distill_block_kernel(const Distil
   float zh[HELD];
 #pragma unroll
   for (int i = 0; i < HELD; i++) zh[i] = rank == 0 && h.id[i] >= 0 ? to_f<T>(z[h.id[i]]) : 0.0f;
-  const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg), c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
+  const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg);
+  const int c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
   Peak a = warp_peak(row_peak(z + c0, c1 - c0, p.c), p.c);
   const float mt = warp_max(h.largest());
   if (lane == 0) red[warp] = a, red_t[warp] = mt;
@@ -465,7 +472,7 @@ __device__ __forceinline__ void join_equal(const Meet& s, const Held<HELD>& h, f
   }
 }
 
-// dz[0, n) = a exp((z - base) / T) over a block's threads; VEC 1: z and dz are not equally far from 16 bytes
+// dz[0, n) = a exp((z - base) / T) over a block's threads; WIDE: z and dz are equally far from 16 bytes
 template <typename T, bool WIDE>
 __device__ __forceinline__ void row_gradient(const T* z, T* dz, int n, float base, float c, float a) {
   constexpr int VEC = 16 / sizeof(T);
@@ -575,7 +582,8 @@ __global__ void __launch_bounds__(kThreads, warp_kernel_blocks(HELD)) distill_ba
     // the pieces that are the row's alone as they are, the elements around them one at a time
     const int v0 = !WIDE ? n : lead ? 1 : 0, v1 = !WIDE ? n : (lead + p.classes) / VEC;
     for (int v = v0 + lane; v < v1; v += 32)
-      reinterpret_cast<uint4*>(dz - lead)[v] = Chunk<T>::gradient(reinterpret_cast<const uint4*>(buf)[v], f.base, p.c, a);
+      reinterpret_cast<uint4*>(dz - lead)[v] =
+          Chunk<T>::gradient(reinterpret_cast<const uint4*>(buf)[v], f.base, p.c, a);
     auto one = [&](int e) { dz[e] = from_f<T>(a * ex2((to_f<T>(buf[lead + e]) - f.base) * p.c)); };
     if (WIDE && v0 <= v1) {
       if (lead && lane < VEC - lead) one(lane);
@@ -603,8 +611,10 @@ __global__ void __launch_bounds__(kThreads, 4) distill_back_block_kernel(const D
   __shared__ float red_t[kWarps];
   __shared__ double red_e[kWarps];
   const int64_t r = blockIdx.x / p.splits;
-  const int rank = (int)(blockIdx.x % p.splits), lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
-  const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg), c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
+  const int rank = (int)(blockIdx.x % p.splits);
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int c0 = (int)min((int64_t)p.classes, (int64_t)rank * p.seg);
+  const int c1 = (int)min((int64_t)p.classes, (int64_t)c0 + p.seg);
   const T* z = static_cast<const T*>(p.z) + r * p.zs;
   T* dz = static_cast<T*>(p.dz) + r * p.ds;
   const Meet meet{seen[0], seen[1], ids, probs, kBits};
@@ -650,8 +660,8 @@ __global__ void __launch_bounds__(kThreads, 4) distill_back_block_kernel(const D
 
 // ---- host --------------------------------------------------------------------------------------------------------
 
-// Blocks to a row, so that few rows still fill the device: `most` of them, of 4,096 classes or more. Returns the threads
-// of a block: as many as keep a few 16-byte pieces each, and hold the entries.
+// Blocks to a row, so that few rows still fill the device: `most` of them, of 4,096 classes or more. Returns the
+// threads of a block: as many as keep a few 16-byte pieces each, and hold the entries.
 int split_rows(DistillParams& p, int most, int bytes) {
   const int64_t want = (8 * kSmCount + p.rows - 1) / p.rows;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, p.classes / 4096}));
@@ -664,7 +674,8 @@ int split_rows(DistillParams& p, int most, int bytes) {
 
 bool warp_rows(const DistillParams& p) { return p.classes <= kWarpClasses && p.k <= kWarpTop; }
 
-// Blocks of warps that go over the rows: as many as run at once, by registers and shared memory (16 KB for the entries).
+// Blocks of warps that go over the rows: as many as run at once, by registers and shared memory (16 KB for the
+// entries).
 unsigned warp_blocks(const DistillParams& p, int held) {
   const int by_rows = kMaxBlockSmem / (2 * kWarps * p.row_bytes + 16384);
   const int64_t most = (int64_t)kSmCount * std::max(1, std::min(warp_kernel_blocks(held), by_rows));
@@ -696,7 +707,8 @@ template <typename T, bool WIDE, int HELD>
 void backward_held(const DistillParams& p, int threads, cudaStream_t st) {
   if (warp_rows(p)) {
     allow_block_smem<distill_back_warp_kernel<T, WIDE, HELD>>();
-    distill_back_warp_kernel<T, WIDE, HELD><<<warp_blocks(p, HELD), kThreads, (size_t)2 * kWarps * p.row_bytes, st>>>(p);
+    const size_t smem = (size_t)2 * kWarps * p.row_bytes;
+    distill_back_warp_kernel<T, WIDE, HELD><<<warp_blocks(p, HELD), kThreads, smem, st>>>(p);
   } else {
     distill_back_block_kernel<T, WIDE, HELD><<<(unsigned)(p.rows * p.splits), threads, 0, st>>>(p);
   }
@@ -726,7 +738,8 @@ void backward(DistillParams p, cudaStream_t st) {
 template <typename T>
 void run_backward(const DistillParams& p, cudaStream_t st) {
   // 16-byte pieces where a row's logits and gradient are equally far from them
-  const bool wide = ((uintptr_t)p.z - (uintptr_t)p.dz) % 16 == 0 && (p.rows == 1 || (p.zs - p.ds) * (int64_t)sizeof(T) % 16 == 0);
+  const bool wide = ((uintptr_t)p.z - (uintptr_t)p.dz) % 16 == 0 &&
+                    (p.rows == 1 || (p.zs - p.ds) * (int64_t)sizeof(T) % 16 == 0);
   wide ? backward<T, true>(p, st) : backward<T, false>(p, st);
 }
 
@@ -820,7 +833,8 @@ extern "C" int kc_distill_top_backward(const kc_distill_desc* desc, const void* 
     if (!rows_distinct(dz)) bad("rows of the output share memory");
     if (rows_overlap(dz, z) && !dz.same(z)) bad("the output overlaps an input it does not match");
     if (rows_overlap(dz, ids) || rows_overlap(dz, top)) bad("the output overlaps an input");
-    for (const Range& s : {Range{d_stats, 8 * d.rows}, Range{d_dloss, 4 * d.rows}, Range{d_teacher_log_sum, 4 * d.rows}})
+    for (const Range& s :
+         {Range{d_stats, 8 * d.rows}, Range{d_dloss, 4 * d.rows}, Range{d_teacher_log_sum, 4 * d.rows}})
       if (ranges_meet(s, dz)) bad("the output overlaps an input");
     TensorDevice dev("top logits", {d_logits, d_ids, d_top_logits, d_teacher_log_sum, d_stats, d_dloss, d_dlogits});
     DistillParams p = params_of(d);

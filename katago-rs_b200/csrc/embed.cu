@@ -6,16 +6,17 @@
 // Forward, a few lanes of a warp take a token's row. Backward, the tokens are sorted by id (a stable radix sort of the
 // ids, so that a row's sum has the tokens' order whatever the timing) and the sorted list is cut into equal pieces
 // whatever the rows' shares of it, so that a row that most tokens have costs no more than many rows that few have: a
-// group of lanes sums its piece run by run, writes the runs that lie inside it, and leaves its first and last run to its
-// block, which joins those of its pieces; a last launch joins runs over blocks. Sums are float32: chains of at most a
-// piece, then the pieces of a block, then the blocks.
+// group of lanes sums its piece run by run, writes the runs that lie inside it, and leaves its first and last run to
+// its block, which joins those of its pieces; a last launch joins runs over blocks. Sums are float32: chains of at most
+// a piece, then the pieces of a block, then the blocks.
 //
 // What bounds it, measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
 //   forward, 57,767 tokens x 768 added to a sequence, bf16: 187 MB in 36.5 us, 5,110 GB/s (HBM)
-//   backward, 92,416 tokens x 384, 362 rows, bf16: 72 MB in 37.3 us: sort 15 us, sums 18 us (66% of the issue slots), joins
-//     6 us, the launches overlapping. The sort is 16 SMs' work: 5 us of ranks, 3 us for the exchange of the counts, 4 us
-//     to write 8-byte entries a sector each
-//   backward, 20,011 tokens x 512, 50,000 rows, float32: 143 MB in 48.0 us: sort 13 us, sums and zeros 26 us, joins 7 us
+//   backward, 92,416 tokens x 384, 362 rows, bf16: 72 MB in 38.2 us: sort 15 us, sums 18 us (66% of the issue slots),
+//     joins 6 us, the launches overlapping. The sort is 16 SMs' work: 5 us of ranks, 3 us for the exchange of the
+//     counts, 4 us to write 8-byte entries a sector each
+//   backward, 20,011 tokens x 512, 50,000 rows, float32: 143 MB in 48.0 us: sort 13 us, sums and zeros 26 us, joins 7
+//     us
 //   rows that begin anywhere: forward, 57,767 x 768 of 771, bf16: 63 us (72 us an element or two at a time); backward,
 //     92,416 x 384 of 387, bf16: 52.5 us (75 us)
 // Not kept: zeros written by the SMs that the sort leaves idle (50.1 us), dy asked into L2 by them (45.8 us, but the
@@ -95,9 +96,9 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const EmbedParams p) {
 }
 
 // The same for rows that begin anywhere: aligned 16-byte pieces of the rows are read and written, each by a lane; a
-// vector is a window over a lane's piece and the next lane's, and a piece to write one over the lane before's vector and
-// its own. So lanes 1 to lanes - 2 of a group write; lane 0 has the last vector of the pieces before. (In place, no piece
-// is read after its row's elements have been written.)
+// vector is a window over a lane's piece and the next lane's, and a piece to write one over the lane before's vector
+// and its own. So lanes 1 to lanes - 2 of a group write; lane 0 has the last vector of the pieces before. (In place, no
+// piece is read after its row's elements have been written.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) embed_shift_kernel(const EmbedParams p) {
   constexpr int VEC = 16 / sizeof(T), BATCH = 2;
@@ -207,8 +208,8 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Places the tile's entries. Each warp owns a share of consecutive entries: it counts its digits, takes its places
-// behind those of the tiles and warps before it, and goes over them again. The tiles' counts are in p.hist; a cluster with
-// a block to each tile exchanges them (`totals`, [tiles][bins]).
+// behind those of the tiles and warps before it, and goes over them again. The tiles' counts are in p.hist; a cluster
+// with a block to each tile exchanges them (`totals`, [tiles][bins]).
 template <SortIn IN, int THREADS>
 __device__ __forceinline__ void place_tile(const SortParams& p, int tile, int* count, int* scan, int* totals) {
   constexpr int WARPS = THREADS / 32;
@@ -408,8 +409,8 @@ __device__ __forceinline__ void absent_rows(const SumParams& p, int row0, int co
 
 // The block's pieces of the list. WHOLE: they are all there is, and no run goes on in another block.
 // SHIFT: rows of dy that begin anywhere. A lane reads an aligned 16-byte piece of the row (which never leaves the
-// allocation of the element in it); its vector is a window over that and the next lane's, so that the last lane of a group
-// has none. What lies behind the row's end is summed into channels that are not written.
+// allocation of the element in it); its vector is a window over that and the next lane's, so that the last lane of a
+// group has none. What lies behind the row's end is summed into channels that are not written.
 // slot: [first, last][group][lane][VEC], key: [first, last][group]
 template <typename T, int VEC, bool SHIFT, bool WHOLE>
 __device__ __forceinline__ void sum_pieces(const SumParams& p, float* slot, int (*key)[kThreads / 2]) {
@@ -528,12 +529,13 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumParams 
   __shared__ int key[2][kThreads / 2];
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x >= p.blocks) return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, (p.lanes - SHIFT) * VEC, key[0]);
+  if (blockIdx.x >= p.blocks)
+    return absent_rows(p, (blockIdx.x - p.blocks) * kThreads, (p.lanes - SHIFT) * VEC, key[0]);
   sum_pieces<T, VEC, SHIFT, false>(p, slot, key);
 }
 
-// Few tokens in one launch: every block sorts them in its shared memory, the first of each column of blocks sums, and all
-// share the rows that no token has.
+// Few tokens in one launch: every block sorts them in its shared memory, the first of each column of blocks sums, and
+// all share the rows that no token has.
 template <typename T, int VEC, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) embed_few_kernel(SumParams p, SortParams q, int passes) {
   __shared__ __align__(16) int2 list[2][kFewTokens];
@@ -721,7 +723,8 @@ void sort_tokens(const kc_embed_desc& d, const int32_t* ids, int2* a, int2* b, i
 template <typename T, int VEC, bool SHIFT>
 void launch_sum(const SumParams& p, const SumShape& s, cudaStream_t st) {
   const unsigned absent = (unsigned)((p.rows + (int64_t)kThreads - 1) / kThreads);
-  launch_after(embed_sum_kernel<T, VEC, SHIFT>, dim3((unsigned)s.blocks + absent, (unsigned)s.chunks), dim3(kThreads), 0, st, p);
+  const dim3 grid((unsigned)s.blocks + absent, (unsigned)s.chunks);
+  launch_after(embed_sum_kernel<T, VEC, SHIFT>, grid, dim3(kThreads), 0, st, p);
   launch_after(embed_join_kernel, dim3((unsigned)s.blocks, (unsigned)((p.C + 31) / 32)), dim3(kThreads), 0, st, p);
 }
 
@@ -732,8 +735,8 @@ void run_type(const EmbedParams& p, bool shift, unsigned blocks, cudaStream_t st
   KC_CUDA(cudaGetLastError());
 }
 
-// One launch where groups of four lanes, 32 tokens to a group at most, have all tokens in a block (361 tokens x 384, 362
-// rows, f16: 13.7 us, 12.0 us in three launches, but 16 and 22 us with the calls' time on the host).
+// One launch where groups of four lanes, 32 tokens to a group at most, have all tokens in a block (361 tokens x 384,
+// 362 rows, f16: 13.7 us, 12.0 us in three launches, but 16 and 22 us with the calls' time on the host).
 template <typename T, int VEC, bool SHIFT>
 bool launch_few(SumParams p, const int32_t* ids, cudaStream_t st) {
   p.lanes = 4;

@@ -10,20 +10,20 @@
 // one read, one write. The variance is taken around the float32 mean of the first pass, whose own error the second
 // pass finds (the sum of the distances), so that a large mean costs neither digits of the variance nor of x - mean.
 // Backward, a block goes over many rows and keeps the channels' sums in registers; a second launch adds the blocks' in
-// their order (few rows: a cluster adds its own). Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read
-// again for each pass.
+// their order (few rows: a cluster adds its own). Rows that registers do not hold (more than 16,384 channels forward,
+// 8,192 backward) are read again for each pass.
 //
-// What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an SM
-// that hold their rows, parameters and sums in registers. The rows behind the one at hand are on their way into shared
-// memory (loads straight into registers, one row at a time: 62 us where the ring takes 27); a mask is looked at a row
-// after it was asked for (34 us without). Measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
+// What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an
+// SM that hold their rows, parameters and sums in registers. The rows behind the one at hand are on their way into
+// shared memory (loads straight into registers, one row at a time: 62 us where the ring takes 27); a mask is looked at
+// a row after it was asked for (34 us without). Measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
 //   forward, 256 boards x 361 x 384, layer norm, bf16, masked: 120 MB in 25.6 us, 4,680 GB/s
 //   forward, 64 x 361 x 768, layer norm, float32: 142 MB in 24.5 us, 5,800 GB/s
 //   backward, 128 x 361 x 768, RMS norm, bf16: 213 MB in 41.4 us, 5,160 GB/s
 //   backward, 256 x 361 x 384, layer norm, bf16, masked: 168 MB in 38.9 us, 4,310 GB/s
-// further from it: rows that begin anywhere (forward 256 x 361 x 384 of 387: 42.5 us, a window of 19 instructions each way
-// a vector), rows of a block (forward 9,000 x 4,096, bf16, RMS: 36.5 us of 22.5; barriers), single elements there (5,000 x
-// 4,099: 93 us of 12.5), rows read again (backward 1,000 x 20,000, float32: 150 us of 37).
+// further from it: rows that begin anywhere (forward 256 x 361 x 384 of 387: 42.5 us, a window of 19 instructions each
+// way a vector), rows of a block (forward 9,000 x 4,096, bf16, RMS: 36.5 us of 22.5; barriers), single elements there
+// (5,000 x 4,099: 93 us of 12.5), rows read again (backward 1,000 x 20,000, float32: 150 us of 37).
 
 #include <algorithm>
 #include <cmath>
@@ -104,8 +104,8 @@ __device__ __forceinline__ bool rows_left(int64_t r, int64_t rows) {
   return BLOCK ? r < rows : __any_sync(0xffffffffu, r < rows);
 }
 
-// A thread's NV vectors as pairs of elements, for the two-lane float32 arithmetic: a unit is a vector, or two vectors of
-// one element. Pair j of unit u has elements 2 j and 2 j + 1 of both vectors' elements.
+// A thread's NV vectors as pairs of elements, for the two-lane float32 arithmetic: a unit is a vector, or two vectors
+// of one element. Pair j of unit u has elements 2 j and 2 j + 1 of both vectors' elements.
 template <int VEC, int NV>
 struct Units {
   static_assert(NV * VEC % 2 == 0, "whole pairs");
@@ -129,9 +129,9 @@ constexpr int ring_depth(int row, bool backward) { return !backward && row * 4 <
 
 // A thread's vectors of the next rows, on their way into shared memory of its own (DEPTH rows, the one at hand among
 // them; no more than what 512 threads of an SM have room for). Rows that are off are not copied.
-// SHIFT: rows that begin anywhere. The aligned 16-byte pieces that hold the row are copied (such a piece never leaves the
-// allocation of the element in it), and a vector is a window over its own piece and the next one, which a neighbour has;
-// its warp's lanes have to be done with a row before the next one takes its place.
+// SHIFT: rows that begin anywhere. The aligned 16-byte pieces that hold the row are copied (such a piece never leaves
+// the allocation of the element in it), and a vector is a window over its own piece and the next one, which a neighbour
+// has; its warp's lanes have to be done with a row before the next one takes its place.
 template <typename T, int VEC, int NV, bool BLOCK, int TENSORS, bool SHIFT>
 struct Ring {
   using Copy = RowCopy<T, VEC>;
@@ -279,8 +279,9 @@ struct Place {
     for (int i = 0; i < NV; i++)
       if (has(i)) RowVec<T, VEC>::store(row + (g.lane + i * g.lanes) * VEC, typename RowVec<T, VEC>::Raw{});
   }
-  // SHIFT: all vectors of a row that begins anywhere, by all lanes of the warp: a piece is a window over the vector before
-  // and its own; the pieces that hold other rows' elements go out element by element. Nothing where `here` is false.
+  // SHIFT: all vectors of a row that begins anywhere, by all lanes of the warp: a piece is a window over the vector
+  // before and its own; the pieces that hold other rows' elements go out element by element. Nothing where `here` is
+  // false.
   template <typename T>
   __device__ __forceinline__ void store_shifted(T* row, int C, const uint4 (&raw)[NV], bool here) const {
     const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
@@ -334,11 +335,11 @@ struct Place {
   }
 };
 
-// y = xh w + b of the units of a thread, with its weights and biases in registers or, SHARED, in the block's shared memory
-// (16-byte parts of all vectors side by side, each read without a conflict). Shared where that makes room for a third
-// block on an SM: 24 elements of 2 bytes a lane, 256 boards x 361 x 384 layer norm, bf16, 25.6 us and 27.2 in registers;
-// float32 rows, whose ring leaves room for two blocks, lose (64 x 361 x 768: 32.6 and 24.8 us), and so do 8 elements,
-// which registers let run four blocks at once (2,000,000 x 16, bf16: 40.7 and 33.1 us).
+// y = xh w + b of the units of a thread, with its weights and biases in registers or, SHARED, in the block's shared
+// memory (16-byte parts of all vectors side by side, each read without a conflict). Shared where that makes room for a
+// third block on an SM: 24 elements of 2 bytes a lane, 256 boards x 361 x 384 layer norm, bf16, 25.6 us and 27.2 in
+// registers; float32 rows, whose ring leaves room for two blocks, lose (64 x 361 x 768: 32.6 and 24.8 us), and so do 8
+// elements, which registers let run four blocks at once (2,000,000 x 16, bf16: 40.7 and 33.1 us).
 template <int VEC, int NV, bool BLOCK, bool SHIFT, bool SHARED>
 struct Affine {
   using At = Place<VEC, NV, BLOCK, SHIFT>;
@@ -380,7 +381,9 @@ struct Affine {
     }
   }
 };
-constexpr bool shared_params(int vec, int nv, bool block, bool shift) { return !block && !shift && vec == 8 && nv == 3; }
+constexpr bool shared_params(int vec, int nv, bool block, bool shift) {
+  return !block && !shift && vec == 8 && nv == 3;
+}
 
 constexpr int kBlockThreads = 512;  // of blocks that share a row, at most: 128 registers each
 
@@ -731,7 +734,8 @@ __global__ void __launch_bounds__(kThreads) layer_norm_long_sums_kernel(const La
     const int64_t c = c0 + tx;
     float2 s = make_float2(0.0f, 0.0f);
     if (c < p.C)
-      for (int64_t r = (int64_t)blockIdx.y * (kThreads / 32) + ty; r < p.rows; r += (int64_t)gridDim.y * (kThreads / 32)) {
+      for (int64_t r = (int64_t)blockIdx.y * (kThreads / 32) + ty; r < p.rows;
+           r += (int64_t)gridDim.y * (kThreads / 32)) {
         if (!token_on(p, r)) continue;
         const float2 st = p.stats[r];
         const float d = to_f<T>(static_cast<const T*>(p.dy)[p.ym(r) + c]);
@@ -795,8 +799,8 @@ struct Shape {
   int64_t blocks;
 };
 
-// 16-byte vectors of a warp's lane: up to 24 elements (weight, bias and the row in registers, or weight, row, gradient and
-// the channels' sums). A block's thread has 16 or, forward, 32 elements.
+// 16-byte vectors of a warp's lane: up to 24 elements (weight, bias and the row in registers, or weight, row, gradient
+// and the channels' sums). A block's thread has 16 or, forward, 32 elements.
 constexpr int kNvs[] = {1, 2, 3, 4, 6};
 constexpr bool warp_nv(int vec, int nv) { return vec * nv <= 24 && (vec == 4 || nv <= 3); }
 
@@ -920,7 +924,8 @@ void run_vec(const LayerParams& p, const Shape& s, bool backward, cudaStream_t s
       layer_norm_long_kernel<T, VEC><<<(unsigned)s.blocks, kLongThreads, 0, st>>>(p);
     } else {
       if (p.part) {
-        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)p.C + 31) / 32, 1 << 20), (unsigned)long_shares(p.rows, p.C));
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)p.C + 31) / 32, 1 << 20),
+                        (unsigned)long_shares(p.rows, p.C));
         layer_norm_long_sums_kernel<T><<<grid, kThreads, 0, st>>>(p);
         KC_CUDA(cudaGetLastError());
       }
@@ -956,9 +961,9 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.mm = row_map(d.n, d.points, d.mask_board_stride, 1);
   Shape s = shape_of(p.rows, p.C, dtype_bytes(d.dtype), vec, backward);
   p.lanes = s.lanes;
-  // few rows: one cluster of up to 16 blocks, whose groups of lanes have 4 rows each at most, and no second launch (361 x
-  // 384, RMS, bf16, with the call's time on the host: 21.0 us, 23.5 in two launches; 8.3 and 7.9 us on the device. With 16
-  // rows a group, 7,261 x 100, f16, took 29 us on the device, 10.5 over all SMs)
+  // few rows: one cluster of up to 16 blocks, whose groups of lanes have 4 rows each at most, and no second launch (361
+  // x 384, RMS, bf16, with the call's time on the host: 21.0 us, 23.5 in two launches; 8.3 and 7.9 us on the device.
+  // With 16 rows a group, 7,261 x 100, f16, took 29 us on the device, 10.5 over all SMs)
   if (p.part && !s.block && !s.is_long) {
     const int64_t groups = kThreads / s.lanes;
     if (p.rows <= 16 * 4 * groups) {
@@ -973,8 +978,8 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   if (!p.part || p.cluster) return;
   const PartShape q = part_shape(s, p.rows, p.C);
   const int64_t slots = (int64_t)q.slots * ((p.dweight ? 1 : 0) + (p.dbias ? 1 : 0));
-  launch_after(layer_norm_params_kernel, dim3((unsigned)std::min<int64_t>((slots + 31) / 32, 1 << 20)), dim3(1024), 0, st,
-               (const float*)p.part, q, p.dweight, p.dbias);
+  const dim3 grid((unsigned)std::min<int64_t>((slots + 31) / 32, 1 << 20));
+  launch_after(layer_norm_params_kernel, grid, dim3(1024), 0, st, (const float*)p.part, q, p.dweight, p.dbias);
 }
 
 Rows x_rows(const kc_layer_norm_desc& d, const void* p) {

@@ -64,9 +64,9 @@ struct RowVec {
   }
 };
 
-// Copies into shared memory by the thread that reads them there: no barrier, and loads in flight that take no registers.
-// copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived. A single 2-byte
-// element comes with the 4 aligned bytes around it (`src` is the address of those: base()).
+// Copies into shared memory by the thread that reads them there: no barrier, and loads in flight that take no
+// registers. copy_commit() closes a group; copy_wait<N>() returns when all but the last N groups have arrived. A single
+// 2-byte element comes with the 4 aligned bytes around it (`src` is the address of those: base()).
 template <typename T, int VEC>
 struct RowCopy {
   using V = RowVec<T, VEC>;
@@ -161,8 +161,8 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
-// Sum over a block of whole warps, the warps' sums in their order. `red` holds a value per warp; two calls in a row take
-// different ones.
+// Sum over a block of whole warps, the warps' sums in their order. `red` holds a value per warp; two calls in a row
+// take different ones.
 __device__ __forceinline__ float2 block_sum(float2 v, float2* red) {
   v = lanes_sum(v, 32);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
