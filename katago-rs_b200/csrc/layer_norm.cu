@@ -492,9 +492,9 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
   aw.fill(0.0f);
   ab.fill(0.0f);
   at.load(w, p.weight, 1.0f, p.wide);
-  int turn = 0;
+  int turn = 0;  // a block's sums of the rows that are on take turns with `red`
   float2 st_next = g.first < p.rows ? p.stats[g.first] : make_float2(0.0f, 0.0f);
-  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, turn ^= 1, ring.leave()) {
+  for (int64_t r = g.first; rows_left<BLOCK>(r, p.rows); r += g.step, ring.leave()) {
     const bool here = r < p.rows, on = ring.arrive(p, g);
     const float2 st = st_next;
     if (r + g.step < p.rows) st_next = p.stats[r + g.step];
@@ -534,8 +534,8 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
       }
     }
     float2 s;
-    if constexpr (LEAN) s = make_float2(0.0f, g.sum(s2.x + s2.y, red[turn]));
-    else s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn]);
+    if constexpr (LEAN) s = make_float2(0.0f, g.sum(s2.x + s2.y, red[turn ^= 1]));
+    else s = g.sum(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn ^= 1]);
     if (!SHIFT && !here) continue;
     // rstd (g - c1 - xh c2)
     const float k1 = p.kind == KC_NORM_LAYER ? -s.x * inv * st.y : 0.0f, k2 = -s.y * inv * st.y;

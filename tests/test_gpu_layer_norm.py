@@ -100,6 +100,25 @@ def test_ends_of_the_ways_to_add(rows, dtype):
             check_backward(x, mask, w, stats, dy, kind, *r.layer_backward(x, mask, w, stats, dy, kind))
 
 
+@pytest.mark.parametrize("channels,blocks", [(2000, 592), (4096, 296), (1500, 740), (1030, 296), (8192, 148)])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_blocks_whose_rows_are_on_in_turn(kind, channels, blocks):
+    """Every other row of a block is off, so that the sums of those that are on follow each other without what a row
+    between them would wait for: the bits of the rows that are on by themselves."""
+    rows = 9 * blocks
+    x, dy, w, b, _ = make(1, rows, channels, "bf16", 31, False)
+    mask = (torch.arange(rows, device="cuda") // blocks % 2 == 0).float()[None]
+    on = mask[0] != 0
+    y, stats = r.layer_forward(x, mask, w, b, kind)
+    alone, own = r.layer_forward(x[:, on].contiguous(), None, w, b, kind)
+    assert torch.equal(y[:, on], alone) and torch.equal(stats[:, on], own) and y[:, ~on].eq(0).all()
+    for _ in range(5):
+        dx, dw, db = r.layer_backward(x, mask, w, stats, dy, kind)
+        check_backward(x, mask, w, stats, dy, kind, dx, dw, db)
+        single = r.layer_backward(x[:, on].contiguous(), None, w, own, dy[:, on].contiguous(), kind)[0]
+        assert torch.equal(dx[:, on], single)
+
+
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_many_rows(kind):
     """A block goes over many rows: 92,416 x 96 over at most 296 blocks of 16 rows or more, chains of 20."""
