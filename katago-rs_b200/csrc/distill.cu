@@ -45,6 +45,10 @@ constexpr int kWarpTop = 32 * kMostHeld;
 constexpr int kMaxTop = kThreads * kMostHeld;
 // Blocks to an SM of the kernels that give a row to a warp: 64 registers, or 80 for more entries.
 constexpr int warp_kernel_blocks(int held) { return held <= 2 ? 4 : 3; }
+// The loss is T^2 times a difference of logarithms that shrinks like 1 / T^2 while their error, the float32 sums',
+// stays. Logits at distance 1 from the teacher's have a loss of 0.5, off by up to T^2 2^-18 (362 classes): 0.8% of it at
+// T = 32. The worst of 2,000 rows measured: 0.02% at T = 20, 0.05% at 32, 2.5% at 256, 35% at 1,024, 490% at 4,096.
+constexpr float kMostTemperature = 32.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -756,7 +760,7 @@ void check_desc(const kc_distill_desc* d) {
   if (d->rows < 0 || d->rows > 1 << 30) bad("rows must be 0 to 2^30");
   if (d->classes < 1 || d->classes > 1 << 30) bad("classes must be 1 to 2^30");
   if (d->top < 1 || d->top > kMaxTop) bad("top must be 1 to 1024");
-  if (!(d->temperature >= 0x1p-20f && d->temperature <= 0x1p20f)) bad("temperature must be 2^-20 to 2^20");
+  if (!(d->temperature >= 0x1p-20f && d->temperature <= kMostTemperature)) bad("temperature must be 2^-20 to 32");
 }
 
 void check_rows(const Rows& r) {

@@ -236,3 +236,55 @@ def test_same_bits_alone_on_streams_and_in_graphs():
             gr.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(u, v) for u, v in zip(out, want))
+
+
+NEAR = [(64, 362, 362), (64, 100, 100), (16, 1024, 1024), (200, 362, 120)]
+
+
+@pytest.mark.parametrize("temp", [1.0, 4.0, 20.0, 32.0])
+@pytest.mark.parametrize("rows,classes,k", NEAR)
+def test_student_near_its_teacher(rows, classes, k, temp):
+    """The loss is a small difference, about half the noise's variance at any temperature, and its error's bound T^2 P E
+    grows with T, to 1024 x 2^-18 = 4e-3 at the highest: 0.8% of a loss of 0.5. The gradient is a difference too, of g q
+    and g p, about g q / T: E of g q is T E = 1.3e-4 of it at the highest temperature."""
+    z, _, _, dloss = make(rows, classes, 1, "f32", 3, absent=False)
+    g = torch.Generator(device="cuda").manual_seed(41)
+    ids = torch.rand(z.shape, device="cuda", generator=g).argsort(1)[:, :k].int().contiguous()
+    top = z.gather(1, ids.long()) + torch.randn(rows, k, device="cuda", generator=g)
+    whole = None if k == classes else torch.logsumexp(torch.scatter(z, 1, ids.long(), top).double() / temp, 1).float()
+    loss, stats = r.distill_forward(z, ids, top, whole, temp)
+    want, _, _ = r.distill64(z, ids, top, whole, temp)
+    _, _, p, _ = r.teacher64(ids, top, whole, classes, temp)
+    bound = temp**2 * p.sum(1) * unit(classes, 32 if classes <= 2048 and k <= 128 else 128) + 2.0**-23 * want.abs()
+    t.within(loss, want, bound)
+    dz = r.distill_backward(z, ids, top, stats, whole, temp, dloss)
+    check_backward(z, ids, top, whole, temp, stats, dloss, dz)
+    if k == classes:
+        assert (bound / want).max() < 0.04 and loss.min() > 0
+        assert (bound / want).mean() < 0.011
+        exact = torch.stack(r.distill64(z, ids, top, None, temp)[1:], 1)
+        full = r.distill_back64(z, ids, top, None, temp, exact, dloss)[0]
+        assert (dz.double() - full).norm() <= 2e-4 * full.norm()
+
+
+@pytest.mark.parametrize("temp", [2.0**-20, 32.0])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,classes,k", [(40, 362, 30), (10, 362, 300), (6, 9001, 64)])
+def test_ends_of_the_temperature(rows, classes, k, dtype, temp):
+    """Weights are off by 2^-22 (expf) and a rounding: 2^-21 of the terms' sizes, twice with the division by the sum."""
+    z, ids, top, dloss = make(rows, classes, k, dtype, 29)
+    for scale in (1.0, temp):  # scaled by T: probabilities as at T = 1
+        zs, ts = (z.float() * scale).to(z.dtype), top * scale
+        loss, stats = r.distill_forward(zs, ids, ts, None, temp)
+        want, m, s = r.distill64(zs, ids, ts, None, temp)
+        there, _, p, _ = r.teacher64(ids, ts, None, classes, temp)
+        at = torch.where(there, ids, 0).long()
+        best = torch.where(there, ts.double(), NEG).amax(1, keepdim=True)
+        x = ((ts.double() - best) - (zs.double().gather(1, at) - m[:, None])) / temp
+        size = torch.where(p > 0, p * x.abs(), 0.0).sum(1)
+        e = unit(classes, 32 if classes <= 2048 else 128)
+        t.within(loss, want, temp**2 * (p.sum(1) * e + 2.0**-20 * size) + 2.0**-23 * want.abs())
+        assert torch.equal(stats[:, 0].double(), m)
+        t.within(stats[:, 1], s, e * s)
+        dz = r.distill_backward(zs, ids, ts, stats, None, temp, dloss)
+        check_backward(zs, ids, ts, None, temp, stats, dloss, dz)

@@ -179,3 +179,10 @@ def test_top_logits_refuses_tensors_and_overlaps():
     refused(distill_back, ddesc(dlogits_stride=400), dz=LOG)
     distill(ddesc(rows=0), 0, 0, 0, 0, 0, 0)
     distill_back(ddesc(rows=0), 0, 0, 0, 0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("temperature", [32.00001, 64.0, 1024.0, 2.0**20, 2.0**-20 * (1 - 2.0**-24)])
+def test_top_logits_refuses_temperatures(temperature):
+    """Beyond 32 the loss of a student near its teacher would be lost in the error of its float32 sums."""
+    assert "temperature" in refused(distill, ddesc(temperature=temperature))
+    assert "temperature" in refused(distill_back, ddesc(temperature=temperature))
