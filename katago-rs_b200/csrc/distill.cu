@@ -46,8 +46,8 @@ constexpr int kMaxTop = kThreads * kMostHeld;
 // Blocks to an SM of the kernels that give a row to a warp: 64 registers, or 80 for more entries.
 constexpr int warp_kernel_blocks(int held) { return held <= 2 ? 4 : 3; }
 // The loss is T^2 times a difference of logarithms that shrinks like 1 / T^2 while their error, the float32 sums',
-// stays. Logits at distance 1 from the teacher's have a loss of 0.5, off by up to T^2 2^-18 (362 classes): 0.8% of it at
-// T = 32. The worst of 2,000 rows measured: 0.02% at T = 20, 0.05% at 32, 2.5% at 256, 35% at 1,024, 490% at 4,096.
+// stays. Logits at distance 1 from the teacher's have a loss of 0.5, off by up to T^2 2^-18 (362 classes): 0.8% of it
+// at T = 32. The worst of 2,000 rows measured: 0.02% at T = 20, 0.05% at 32, 2.5% at 256, 35% at 1,024, 490% at 4,096.
 constexpr float kMostTemperature = 32.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
@@ -215,6 +215,10 @@ struct Teacher {
       : shift(p.whole ? (double)__ldg(p.whole + r) : largest * p.inv), inv(p.inv) {}
   __device__ __forceinline__ double at(float t) const { return t * inv - shift; }
 };
+
+// The sum of probabilities that were divided by their sum: 1, or NaN where an entry is NaN or +inf, which then is the
+// whole row's gradient.
+__device__ __forceinline__ double whole_of(double sum) { return (sum - sum) + 1.0; }
 
 // A thread's share of sum e and of sum e x, where z are the entries' logits.
 template <int HELD>
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, warp_kernel_blocks(HELD)) distill_ba
       const double share = 1.0 / sum;
 #pragma unroll
       for (int i = 0; i < HELD; i++) prob[i] = (float)(prob[i] * share);
-      sum = 1.0;
+      sum = whole_of(sum);
     }
     __syncwarp();
     join_equal<false>(meet, h, prob, p.k, lane, 32);
@@ -648,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_back_block_kernel(const D
     const double share = 1.0 / sum;
 #pragma unroll
     for (int i = 0; i < HELD; i++) prob[i] = (float)(prob[i] * share);
-    sum = 1.0;
+    sum = whole_of(sum);
   }
   join_equal<true>(meet, h, prob, p.k, threadIdx.x, blockDim.x);  // with a barrier: all logits are gathered
   const Factors f(p, r, sum);

@@ -288,3 +288,26 @@ def test_ends_of_the_temperature(rows, classes, k, dtype, temp):
         t.within(stats[:, 1], s, e * s)
         dz = r.distill_backward(zs, ids, ts, stats, None, temp, dloss)
         check_backward(zs, ids, ts, None, temp, stats, dloss, dz)
+
+
+@pytest.mark.parametrize("classes,k", [(362, 20), (362, 200), (9001, 40)])
+@pytest.mark.parametrize("given", [False, True])
+def test_teachers_that_are_not_finite(classes, k, given):
+    """NaN among a row's top logits, or +inf, or NaN as its log sum: loss and gradient of that row are NaN."""
+    z, ids, top, dloss = make(6, classes, k, "f32", 37, absent=False)
+    whole = torch.logsumexp(top.double(), 1).float() + 0.1 if given else None
+    want = r.distill_forward(z, ids, top, whole)
+    back = r.distill_backward(z, ids, top, want[1], whole, 1.0, dloss)
+    top[1, k // 2] = float("nan")
+    ids[2, 1] = ids[2, 0]  # that meet
+    top[2, 0] = float("nan")
+    top[3, 0] = float("inf")
+    if given:
+        whole[4] = float("nan")
+    else:
+        top[4] = float("nan")
+    loss, stats = r.distill_forward(z, ids, top, whole)
+    dz = r.distill_backward(z, ids, top, stats, whole, 1.0, dloss)
+    ok, bad = [0, 5], [1, 2, 3, 4]
+    assert loss[bad].isnan().all() and dz[bad].isnan().all()
+    assert torch.equal(loss[ok], want[0][ok]) and torch.equal(dz[ok], back[ok])
