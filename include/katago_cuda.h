@@ -397,10 +397,11 @@ typedef struct kc_distill_desc {
 
 /* d_ids: [rows][top] int32, d_top_logits: [rows][top] float32. An entry whose id is outside 0 .. classes - 1 or whose
  * logit is -inf is absent; entries of one class add up. A row without entries has loss 0 and gradient 0, whatever its
- * logits hold. Logits of -inf (illegal moves) have probability 0: an entry there makes the loss infinite. NaN among a
- * row's logits, +inf, or nothing but -inf make its loss NaN, and so does NaN or +inf as an entry's logit, with all of
- * the row's gradient. d_loss: [rows] float32. d_stats (NULL = not wanted): [rows][2] float32, the row's largest logit and
- * the sum of exp((logit - largest) / T), both 0 without entries. */
+ * logits hold. Logits of -inf (illegal moves) have probability 0: an entry there makes the loss infinite, unless its p
+ * is below about 1e-300, which counts as 0. NaN among a row's logits, +inf, or nothing but -inf make its loss NaN, and
+ * so does NaN or +inf as an entry's logit, with all of the row's gradient. d_loss: [rows] float32. d_stats (NULL = not
+ * wanted): [rows][2] float32, the row's largest logit and the sum of exp((logit - largest) / T), both 0 without
+ * entries. */
 int kc_distill_top(const kc_distill_desc* desc, const void* d_logits, const int32_t* d_ids, const float* d_top_logits,
                    const float* d_teacher_log_sum, float* d_loss, float* d_stats, void* stream);
 

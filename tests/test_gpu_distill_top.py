@@ -311,3 +311,25 @@ def test_teachers_that_are_not_finite(classes, k, given):
     ok, bad = [0, 5], [1, 2, 3, 4]
     assert loss[bad].isnan().all() and dz[bad].isnan().all()
     assert torch.equal(loss[ok], want[0][ok]) and torch.equal(dz[ok], back[ok])
+
+
+@pytest.mark.parametrize("classes,k", [(362, 20), (362, 200), (20011, 40)])
+@pytest.mark.parametrize("given", [False, True])
+def test_light_entries_at_classes_without_probability(classes, k, given):
+    """An entry at a logit of -inf makes the loss infinite as long as 64 bits hold its weight, float32 or not."""
+    z, ids, top, dloss = make(8, classes, k, "f32", 31, absent=False)
+    g = torch.Generator(device="cuda").manual_seed(43)
+    ids = torch.rand(8, classes, device="cuda", generator=g).argsort(1)[:, :k].int().contiguous()
+    temp = 0.1
+    top[:, 0] = top.amax(1) + 1.0
+    for i, below in enumerate((0.0, 5.0, 10.0, 10.5, 20.0, 60.0, 100.0)):  # T = 0.1: e^0 to e^-1000
+        top[i, 1] = top[i, 0] - below
+        z[i, ids[i, 1].long()] = NEG
+    whole = torch.logsumexp(top.double() / temp, 1).float() if given else None
+    loss, stats = r.distill_forward(z, ids, top, whole, temp)
+    assert loss[:6].eq(float("inf")).all() and loss[6:].isfinite().all()
+    want = r.distill64(z, ids, top, whole, temp)[0]
+    assert torch.equal(loss.isinf(), want.isinf())
+    dz = r.distill_backward(z, ids, top, stats, whole, temp, dloss)
+    assert dz.isfinite().all()
+    check_backward(z, ids, top, whole, temp, stats, dloss, dz)
