@@ -331,7 +331,7 @@ typedef struct kc_layer_norm_desc {
   int32_t dtype; /* KC_PRECISION_* of x, y, dy and dx */
   int32_t kind;  /* KC_NORM_* */
   int32_t n, points, channels; /* n and points 0 .. 2^30 (n * points at most 2^46), channels 1 .. 2^30 */
-  float eps;     /* >= 0; with 0 a row of equal values (RMS: of zeros) has NaN in y */
+  float eps;     /* >= 0; with 0 a row of equal values, to float32's rounding (RMS: of zeros), has NaN in y and rstd */
   int64_t x_board_stride, x_row_stride; /* x and dx */
   int64_t y_board_stride, y_row_stride; /* y and dy */
   int64_t mask_board_stride;

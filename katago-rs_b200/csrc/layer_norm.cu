@@ -58,6 +58,7 @@ struct LayerParams {
   int wide;        // weight and bias are 16-byte aligned
   int cluster;     // backward: all blocks are one cluster of so many, which adds their sums itself; 0: `part`
   float eps;
+  float flat;      // without an eps: variances up to this share of the squared distance from the first mean are 0
 };
 
 __device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
@@ -66,11 +67,13 @@ __device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
 __device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) { return token_mask(p, r) != 0.0f; }
 
 // 1 / sqrt(var + eps) of a sum of squares around a value that is `delta` from the mean; NaN where the squares passed
-// float32's range.
-__device__ __forceinline__ float rstd_of(float squares, float inv, float delta, float eps) {
+// float32's range, and where neither the variance nor eps is above 0. A row of equal values has the same distance from
+// its first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square (`flat`).
+__device__ __forceinline__ float rstd_of(const LayerParams& p, float squares, float inv, float delta) {
   const float var = squares * inv - delta * delta;
-  if (!(squares <= 3.402823466e38f)) return __int_as_float(0x7fffffff);
-  return __frsqrt_rn(fmaxf(var, 0.0f) + eps);
+  if (!(squares <= 3.402823466e38f) || (p.eps == 0.0f && !(var > p.flat * delta * delta)))
+    return __int_as_float(0x7fffffff);
+  return __frsqrt_rn(fmaxf(var, 0.0f) + p.eps);
 }
 
 // A row's lanes: `lanes` neighbours of a warp, or a block.
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads,
       squares = g.sum(s2.x + s2.y, red[turn ^= 1]);
     }
     if (!SHIFT && !here) continue;
-    const float rstd = rstd_of(squares, inv, delta, p.eps);
+    const float rstd = rstd_of(p, squares, inv, delta);
     if (here && p.stats && g.lane == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
     const f32x2 scale = {rstd, rstd}, shift = {-delta * rstd, -delta * rstd};
     const uint32_t keep = on ? 0xffffffffu : 0u;
@@ -656,7 +659,7 @@ __global__ void __launch_bounds__(kLongThreads) layer_norm_long_kernel(const Lay
       }
     s = block_sum(s, red[1]);
     const float delta = p.kind == KC_NORM_LAYER ? s.x * inv : 0.0f;
-    const float rstd = rstd_of(s.y, inv, delta, p.eps);
+    const float rstd = rstd_of(p, s.y, inv, delta);
     if (p.stats && threadIdx.x == 0) p.stats[r] = on ? make_float2(m0 + delta, rstd) : make_float2(0.0f, 0.0f);
     T* out = static_cast<T*>(p.y) + p.ym(r);
     for (int c = threadIdx.x * VEC; c < p.C; c += kLongThreads * VEC) {
@@ -955,6 +958,8 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.C = d.channels;
   p.kind = d.kind;
   p.eps = d.eps;
+  // a sum is made of at most 42 + C / 512 additions: three such errors and the products', each 2^-24
+  p.flat = (3.0f * (42.0f + (float)p.C / 512.0f) + 16.0f) * 0x1p-24f;
   p.wide = aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
   p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
   p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);

@@ -309,3 +309,30 @@ def test_same_bits_alone_in_batches_on_streams_and_in_graphs():
             gr.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(u, v) for u, v in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("channels", [1, 7, 100, 384, 767, 1000, 1031, 4096, 20000, 40000])
+def test_rows_of_equal_values_without_eps(dtype, channels):
+    """NaN with eps 0, whatever the first mean's rounding leaves; the other rows as ever. With an eps, the bias."""
+    values = torch.tensor([1.7, 0.1, -3e4, 1e-3, 0.0, 1.0, -7.3, 0.30001], device="cuda").to(t.DTYPES[dtype])
+    x, _, w, b, _ = make(1, 16, channels, dtype, channels, False)
+    x[0, ::2] = values[:, None]
+    for bias in (None, b):
+        y, stats = r.layer_forward(x, None, w, bias, "layer", eps=0.0)
+        assert y[0, ::2].isnan().all() and stats[0, ::2, 1].isnan().all()
+        if channels > 1:
+            check_forward(x[:, 1::2], None, w, bias, "layer", y[:, 1::2], stats[:, 1::2], eps=0.0)
+        y, stats = r.layer_forward(x, None, w, bias, "rms", eps=0.0)
+        assert y[0, 8].isnan().all() and stats[0, 8, 1].isnan()
+        keep = torch.arange(16, device="cuda") != 8
+        check_forward(x[:, keep], None, w, bias, "rms", y[:, keep], stats[:, keep], eps=0.0)
+        # with an eps: the first mean is off by E of the value, what is left of the distance from it by E of that
+        y, stats = r.layer_forward(x[:, ::2], None, w, bias, "layer")
+        want, mean, rstd, _ = r.layer64(x[:, ::2], on_of(x[:, ::2], None), w, bias, "layer")
+        left = unit(channels) ** 2 * mean.abs()
+        half, tiny = t.half_step(x.dtype)
+        add = 0.0 if bias is None else 2.0**-23 * b.double().abs()
+        t.within(y, want, half * want.abs() + tiny + (left * rstd)[:, :, None] * w.double() * 1.01 + add)
+        t.within(stats[..., 0], mean, 2.0**-24 * mean.abs() + left)
+        t.within(stats[..., 1], rstd, 2 * unit(channels) * rstd)
