@@ -524,7 +524,8 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
         ring.get(1, u, g, at.nvec, at.rest, d);
 #pragma unroll
         for (int j = 0; j < U::N; j++) {
-          xh.v[u][j] = mul2(add2(xh.v[u][j], back), scale);
+          // elements beside the row's last one stay 0: their distance from the mean, times rstd, may pass float32
+          xh.v[u][j] = mul2(add2(xh.v[u][j], LEAN || (VEC > 1 && !SHIFT) ? back : at.both(u, j, -st.x)), scale);
           const f32x2 gj = mul2(d[j], w.v[u][j]);
           aw.v[u][j] = fma2(d[j], xh.v[u][j], aw.v[u][j]);
           s2 = fma2(gj, xh.v[u][j], s2);

@@ -336,3 +336,14 @@ def test_rows_of_equal_values_without_eps(dtype, channels):
         t.within(y, want, half * want.abs() + tiny + (left * rstd)[:, :, None] * w.double() * 1.01 + add)
         t.within(stats[..., 0], mean, 2.0**-24 * mean.abs() + left)
         t.within(stats[..., 1], rstd, 2 * unit(channels) * rstd)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [1, 7, 99, 100, 383, 769, 1031, 4099, 384])
+def test_means_whose_quotient_by_the_spread_passes_float32(dtype, channels):
+    """mean x rstd beyond float32's range, where x - mean is 0: dx = rstd (g - mean of g), whatever stands beside the
+    row's last element in its vector."""
+    x, dy, w, _, _ = make(2, 5, channels, dtype, channels, False)
+    x.fill_(2.0**119)
+    stats = torch.tensor([2.0**119, 2.0**10], device="cuda").expand(2, 5, 2).contiguous()
+    check_backward(x, None, w, stats, dy, "layer", *r.layer_backward(x, None, w, stats, dy, "layer"))
