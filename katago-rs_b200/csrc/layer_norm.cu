@@ -58,7 +58,7 @@ struct LayerParams {
   int wide;        // weight and bias are 16-byte aligned
   int cluster;     // backward: all blocks are one cluster of so many, which adds their sums itself; 0: `part`
   float eps;
-  float flat;      // without an eps: variances up to this share of the squared distance from the first mean are 0
+  float flat;      // eps 0: a variance up to this share of the squared distance from the first mean is 0; otherwise 0
 };
 
 __device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
@@ -70,10 +70,8 @@ __device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) { retu
 // float32's range, and where neither the variance nor eps is above 0. A row of equal values has the same distance from
 // its first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square (`flat`).
 __device__ __forceinline__ float rstd_of(const LayerParams& p, float squares, float inv, float delta) {
-  const float var = squares * inv - delta * delta;
-  if (!(squares <= 3.402823466e38f) || (p.eps == 0.0f && !(var > p.flat * delta * delta)))
-    return __int_as_float(0x7fffffff);
-  return __frsqrt_rn(fmaxf(var, 0.0f) + p.eps);
+  const float var = fmaxf(squares * inv - delta * delta, 0.0f) + p.eps;
+  return squares <= 3.402823466e38f && var > p.flat * (delta * delta) ? __frsqrt_rn(var) : __int_as_float(0x7fffffff);
 }
 
 // A row's lanes: `lanes` neighbours of a warp, or a block.
@@ -960,7 +958,7 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.kind = d.kind;
   p.eps = d.eps;
   // a sum is made of at most 42 + C / 512 additions: three such errors and the products', each 2^-24
-  p.flat = (3.0f * (42.0f + (float)p.C / 512.0f) + 16.0f) * 0x1p-24f;
+  p.flat = p.eps > 0.0f ? 0.0f : (3.0f * (42.0f + (float)p.C / 512.0f) + 16.0f) * 0x1p-24f;
   p.wide = aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
   p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
   p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);
