@@ -7,11 +7,12 @@
 //   dweight = sum over tokens of dy xh, dbias = of dy
 //
 // A row stays in the registers of a group of lanes (2 to 32 of a warp, or a block) between the sums and the output:
-// one read, one write. The variance is taken around the float32 mean of the first pass, whose own error the second
-// pass finds (the sum of the distances), so that a large mean costs neither digits of the variance nor of x - mean.
-// Backward, a block goes over many rows and keeps the channels' sums in registers; a second launch adds the blocks' in
-// their order (few rows: a cluster adds its own). Rows that registers do not hold (more than 16,384 channels forward,
-// 8,192 backward) are read again for each pass.
+// one read, one write. Forward, the variance is taken around the float32 mean of the first pass, whose own error the
+// second pass finds (the sum of the distances), so that a large mean costs neither digits of the variance nor of
+// x - mean. Backward, x - mean is from the saved mean, one float32: xh is off by up to |mean| rstd 2^-24 in a whole row
+// (6e-4 under a mean of 10^4 times the spread), and dx and dweight with it. A block goes over many rows there and keeps
+// the channels' sums in registers; a second launch adds the blocks' in their order (few rows: a cluster adds its own).
+// Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read again for each pass.
 //
 // What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an
 // SM that hold their rows, parameters and sums in registers. The rows behind the one at hand are on their way into

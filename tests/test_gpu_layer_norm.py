@@ -347,3 +347,23 @@ def test_means_whose_quotient_by_the_spread_passes_float32(dtype, channels):
     x.fill_(2.0**119)
     stats = torch.tensor([2.0**119, 2.0**10], device="cuda").expand(2, 5, 2).contiguous()
     check_backward(x, None, w, stats, dy, "layer", *r.layer_backward(x, None, w, stats, dy, "layer"))
+
+
+@pytest.mark.parametrize("channels", [384, 767, 1500, 20000])
+def test_gradients_under_large_means(channels):
+    """Against float64 from float64 statistics. The saved mean is a float32, off by 2^-24 of itself: xh is off by
+    h = |mean| rstd 2^-24 in the whole row, besides what check_backward allows and rstd's own error."""
+    x, dy, w, b, _ = make(2, 10, channels, "f32", 19, False, shift=13000.0)
+    on = on_of(x, None)
+    _, stats = r.layer_forward(x, None, w, b, "layer")
+    _, mean, rstd, xh = r.layer64(x, on, w, b, "layer")
+    dx, dw, db = r.layer_backward(x, None, w, stats, dy, "layer")
+    want, ww, wb, size, sw, sb = r.layer_back64(x, on, w, mean, rstd, dy, "layer")
+    e = unit(channels)
+    h = (mean.abs() * rstd * 2.0**-24 + e)[:, :, None]
+    g = dy.double() * w.double()
+    c1, c2 = g.mean(2, keepdim=True).abs(), (g * xh).mean(2, keepdim=True).abs()
+    t.within(dx, want, 2.0**-24 * want.abs() + 2 * e * size + 6 * e * size
+             + rstd[:, :, None] * (h * c2 + xh.abs() * h * c1 + h * h * c1) * 1.01)
+    t.within(dw, ww, SUMS * sw + 2 * e * sw + (dy.double().abs() * h).sum((0, 1)))
+    t.within(db, wb, SUMS * sb)
