@@ -347,7 +347,7 @@ int kc_layer_norm(const kc_layer_norm_desc* desc, const void* d_x, const float* 
 
 /* The gradients by x, weight and bias, given dy and the forward pass's x and d_stats: dx (0 at tokens that are off; in
  * place of x, or of dy where the strides are the same), d_dweight and d_dbias [channels] float32 (sums over all tokens,
- * overwritten; each may be NULL). (x - mean) * rstd is taken from the saved float32 mean: it is off by
+ * added in float32, overwritten; each may be NULL). (x - mean) * rstd is taken from the saved float32 mean: it is off by
  * up to |mean| * rstd * 2^-24, the same in a whole row. The workspace is for d_dweight and d_dbias only. */
 int kc_layer_norm_backward_workspace(const kc_layer_norm_desc* desc, size_t* bytes);
 int kc_layer_norm_backward(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
@@ -372,8 +372,8 @@ int kc_embed_rows(const kc_embed_desc* desc, const int32_t* d_ids, const void* d
                   void* stream);
 
 /* The table's gradient, d_dtable [table_rows][channels] float32 (overwritten): scale times the sum of dy over the tokens
- * that have the row's id, added in the tokens' order within pieces of a fixed length; 0 for a row that none has.
- * table_stride and x_stride are ignored. */
+ * that have the row's id, added in float32, in the tokens' order within pieces of a fixed length; 0 for a row that none
+ * has. table_stride and x_stride are ignored. */
 int kc_embed_rows_backward_workspace(const kc_embed_desc* desc, size_t* bytes);
 int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* d_ids, const void* d_dy, float* d_dtable,
                            void* d_workspace, size_t workspace_bytes, void* stream);
