@@ -77,9 +77,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// exp of a 64-bit argument to float32's precision, 0 below -200
-__device__ __forceinline__ float exp_of(double x) {
-  x = x < -200.0 ? -200.0 : x;
+// exp of a 64-bit argument, or of `least`, to float32's precision; 0 below -104
+__device__ __forceinline__ float exp_of(double x, double least = -200.0) {
+  x = x < least ? least : x;
   const float hi = (float)x, e = expf(hi);
   return fmaf(e, (float)(x - hi), e);
 }
@@ -221,9 +221,8 @@ struct Teacher {
 // whole row's gradient.
 __device__ __forceinline__ double whole_of(double sum) { return (sum - sum) + 1.0; }
 
-// A thread's share of sum e and of sum e x, where z are the entries' logits. An entry whose e float32 does not hold
-// (below about -104) adds nothing, but at a class without probability its term is infinite all the same; one below
-// kLightest (e 10^-300) has no weight at all.
+// A thread's share of sum e and of sum e x, where z are the entries' logits. An e is float32's least numbers at least
+// (e^-100), so that at a class without probability its term is infinite; below kLightest (10^-300) it has no weight.
 template <int HELD>
 __device__ __forceinline__ void loss_terms(const Held<HELD>& h, const Teacher& teacher, const float (&z)[HELD], float m,
                                            double& se, double& sex) {
@@ -232,10 +231,9 @@ __device__ __forceinline__ void loss_terms(const Held<HELD>& h, const Teacher& t
   for (int i = 0; i < HELD; i++) {
     if (h.id[i] < 0) continue;
     const double x = teacher.at(h.t[i]);
-    const double e = exp_of(x);
+    const double e = exp_of(x, -100.0);
     se += e;
-    if (e != 0.0) sex += e * (x - ((double)z[i] - (double)m) * teacher.inv);
-    else if (z[i] == -kInf && x > kLightest) sex = kInf;
+    if (x > kLightest) sex += e * (x - ((double)z[i] - (double)m) * teacher.inv);
   }
 }
 __device__ __forceinline__ void write_loss(const DistillParams& p, int64_t r, double se, double sex, Peak a) {
