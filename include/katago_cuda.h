@@ -347,8 +347,8 @@ int kc_layer_norm(const kc_layer_norm_desc* desc, const void* d_x, const float* 
 
 /* The gradients by x, weight and bias, given dy and the forward pass's x and d_stats: dx (0 at tokens that are off; in
  * place of x, or of dy where the strides are the same), d_dweight and d_dbias [channels] float32 (sums over all tokens,
- * added in float32, overwritten; each may be NULL). (x - mean) * rstd is taken from the saved float32 mean: it is off by
- * up to |mean| * rstd * 2^-24, the same in a whole row. The workspace is for d_dweight and d_dbias only. */
+ * added in float32, overwritten; each may be NULL). (x - mean) * rstd is taken from the saved float32 mean: it is off
+ * by up to |mean| * rstd * 2^-24, the same in a whole row. The workspace is for d_dweight and d_dbias only. */
 int kc_layer_norm_backward_workspace(const kc_layer_norm_desc* desc, size_t* bytes);
 int kc_layer_norm_backward(const kc_layer_norm_desc* desc, const void* d_x, const float* d_mask, const float* d_weight,
                            const float* d_stats, const void* d_dy, void* d_dx, float* d_dweight, float* d_dbias,

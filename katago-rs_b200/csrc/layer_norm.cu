@@ -58,8 +58,7 @@ struct LayerParams {
   int kind;
   int wide;        // weight and bias are 16-byte aligned
   int cluster;     // backward: all blocks are one cluster of so many, which adds their sums itself; 0: `part`
-  float eps;
-  float flat;      // eps 0: a variance up to this share of the squared distance from the first mean is 0; otherwise 0
+  float eps, least, slack;  // rstd_of
 };
 
 __device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
@@ -68,11 +67,13 @@ __device__ __forceinline__ float token_mask(const LayerParams& p, int64_t r) {
 __device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) { return token_mask(p, r) != 0.0f; }
 
 // 1 / sqrt(var + eps) of a sum of squares around a value that is `delta` from the mean; NaN where the squares passed
-// float32's range, and where neither the variance nor eps is above 0. A row of equal values has the same distance from
-// its first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square (`flat`).
+// float32's range. Without an eps NaN too where the variance is 0. A row of equal values has the same distance from its
+// first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square: `slack` (1 with an
+// eps) makes that negative, and `least` (0 with an eps, otherwise -inf) leaves it so.
 __device__ __forceinline__ float rstd_of(const LayerParams& p, float squares, float inv, float delta) {
-  const float var = fmaxf(squares * inv - delta * delta, 0.0f) + p.eps;
-  return squares <= 3.402823466e38f && var > p.flat * (delta * delta) ? __frsqrt_rn(var) : __int_as_float(0x7fffffff);
+  const float var = squares * inv - delta * p.slack * delta;
+  if (!(squares <= 3.402823466e38f)) return __int_as_float(0x7fffffff);
+  return __frsqrt_rn(fmaxf(var, p.least) + p.eps);
 }
 
 // A row's lanes: `lanes` neighbours of a warp, or a block.
@@ -199,7 +200,8 @@ struct Ring {
     if (SHIFT) __syncwarp();
     return on >> stage & 1;
   }
-  // unit u of the row at hand; of a vector that ends behind the row, `rest` elements
+  // unit u of the row at hand; of a vector that ends behind the row, `rest` elements. What stands beside them is 0, but
+  // in the backward pass's x another element of the row: 0 is so far from a large mean that its xh may pass float32.
   __device__ __forceinline__ void get(int tensor, int u, const Group<BLOCK>& g, int nvec, int rest,
                                       f32x2 (&v)[Units<VEC, NV>::N]) const {
     float f[VEC];
@@ -208,7 +210,7 @@ struct Ring {
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         const int i = 2 * u + k, c = g.lane + i * g.lanes;
-        f[0] = 0.0f;
+        f[0] = k == 1 && TENSORS == 2 && tensor == 0 ? e[0] : 0.0f;
         if (c < nvec) Copy::unpack(*at(stage, tensor, i), begin[tensor] >> 4 * stage & 1, f);
         e[k] = f[0];
       }
@@ -222,10 +224,12 @@ struct Ring {
       uint4 raw = window<sizeof(T), false>(*own, *other, begin[tensor] >> 4 * stage & 15);
       if (rest && g.lane + u * g.lanes == nvec - 1) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+        const uint32_t first = sizeof(T) == 4 ? w[0] : w[0] << 16 | (w[0] & 0xffffu);
+        const uint32_t fill = TENSORS == 2 && tensor == 0 ? first : 0u;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int bytes = rest * (int)sizeof(T) - 4 * k;
-          w[k] = bytes >= 4 ? w[k] : bytes <= 0 ? 0u : w[k] & 0xffffu;
+          w[k] = bytes >= 4 ? w[k] : bytes <= 0 ? fill : (w[k] & 0xffffu) | (fill & 0xffff0000u);
         }
       }
       Copy::unpack(raw, false, f);
@@ -523,8 +527,7 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 
         ring.get(1, u, g, at.nvec, at.rest, d);
 #pragma unroll
         for (int j = 0; j < U::N; j++) {
-          // elements beside the row's last one stay 0: their distance from the mean, times rstd, may pass float32
-          xh.v[u][j] = mul2(add2(xh.v[u][j], LEAN || (VEC > 1 && !SHIFT) ? back : at.both(u, j, -st.x)), scale);
+          xh.v[u][j] = mul2(add2(xh.v[u][j], back), scale);
           const f32x2 gj = mul2(d[j], w.v[u][j]);
           aw.v[u][j] = fma2(d[j], xh.v[u][j], aw.v[u][j]);
           s2 = fma2(gj, xh.v[u][j], s2);
@@ -958,8 +961,14 @@ void run(const kc_layer_norm_desc& d, LayerParams p, int vec, bool backward, cud
   p.C = d.channels;
   p.kind = d.kind;
   p.eps = d.eps;
-  // a sum is made of at most 42 + C / 512 additions: three such errors and the products', each 2^-24
-  p.flat = p.eps > 0.0f ? 0.0f : (3.0f * (42.0f + (float)p.C / 512.0f) + 16.0f) * 0x1p-24f;
+  p.slack = 1.0f;
+  if (p.eps == 0.0f) {
+    // a sum is made of at most 42 + C / 512 additions: three such errors and the products', each 2^-24. The least
+    // negative number for an eps: a variance of 0 becomes NaN, others stay
+    p.slack += (3.0f * (42.0f + (float)p.C / 512.0f) + 16.0f) * 0x1p-24f;
+    p.least = -HUGE_VALF;
+    p.eps = -0x1p-149f;
+  }
   p.wide = aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
   p.xm = row_map(d.n, d.points, d.x_board_stride, d.x_row_stride);
   p.ym = row_map(d.n, d.points, d.y_board_stride, d.y_row_stride);
