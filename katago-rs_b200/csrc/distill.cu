@@ -18,11 +18,14 @@
 //
 // What bounds it, measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
 //   backward, 4,096 rows x 32,000, 128 entries, bf16: 513 MB in 91.0 us, 5,640 GB/s (HBM)
-//   forward, the same: 251 MB in 59.8 us, 4,200 GB/s: exponentials (16 a clock and SM: 29 us) and 51% of the issue
-//     slots
+//   forward, the same: 251 MB in 59.8 us, 4,200 GB/s. Neither the exponentials (16 a clock and SM: 29 us) nor issue
+//     (51% of the slots) is full: a block lives for one row, whose first loads wait for the entries and a barrier, and
+//     has nothing in flight while it ends
 //   backward, 16,384 rows x 362, 64 entries, bf16: 32 MB in 14.3 us: 580 warp instructions a row, most of them the
 //     entries'
 //   forward, 60,000 rows x 362, 32 entries, bf16: 57 MB in 32 us: 424 warp instructions a row, 75% of the issue slots
+//   more than 128 entries in rows of 362, which a block takes: 16,384 rows, 362 entries, bf16, forward 59 MB in 51.7
+//     us, backward 71 MB in 60.5 us: 2,740 warp instructions a row, the entries' and the clearing of 8 KB of bits
 // With loops over the entries in memory, all in 64 bits, these took 99, 67, 29 and 73 us.
 
 #include <algorithm>
@@ -685,7 +688,7 @@ int split_rows(DistillParams& p, int most, int bytes) {
 bool warp_rows(const DistillParams& p) { return p.classes <= kWarpClasses && p.k <= kWarpTop; }
 
 // Blocks of warps that go over the rows: as many as run at once, by registers and shared memory (16 KB for the
-// entries).
+// entries); one less than that backward in 2-byte types with more than 64 entries (60 and 64 registers).
 unsigned warp_blocks(const DistillParams& p, int held) {
   const int by_rows = kMaxBlockSmem / (2 * kWarps * p.row_bytes + 16384);
   const int64_t most = (int64_t)kSmCount * std::max(1, std::min(warp_kernel_blocks(held), by_rows));

@@ -14,17 +14,23 @@
 // the channels' sums in registers; a second launch adds the blocks' in their order (few rows: a cluster adds its own).
 // Rows that registers do not hold (more than 16,384 channels forward, 8,192 backward) are read again for each pass.
 //
-// What bounds it: HBM in the large, with 307 warp instructions a pair of rows of 384 next to it, of 16 to 24 warps an
-// SM that hold their rows, parameters and sums in registers. The rows behind the one at hand are on their way into
-// shared memory (loads straight into registers, one row at a time: 62 us where the ring takes 27); a mask is looked at
-// a row after it was asked for (34 us without). Measured on a B200 (6,549 GB/s copy), bytes that have to move / time:
-//   forward, 256 boards x 361 x 384, layer norm, bf16, masked: 120 MB in 25.6 us, 4,680 GB/s
+// What bounds it: HBM in the large, with 341 warp instructions a pair of rows of 384 next to it (62% of the issue
+// slots), of 16 to 24 warps an SM that hold their rows and sums in registers. The rows behind the one at hand are on
+// their way into shared memory (loads straight into registers, one row at a time: 62 us where the ring takes 27); a
+// mask is looked at a row after it was asked for (34 us without). Measured on a B200 (6,549 GB/s copy), bytes that have
+// to move / time:
+//   forward, 256 boards x 361 x 384, layer norm, masked: bf16 120 MB in 25.6 us, 4,680 GB/s; float32 239 MB in 43.1 us,
+//     5,540 GB/s
+//   the same, RMS norm, no mask: bf16 143 MB in 25.9 us, 5,510 GB/s; float32 285 MB in 50.4 us, 5,650 GB/s
 //   forward, 64 x 361 x 768, layer norm, float32: 142 MB in 24.5 us, 5,800 GB/s
 //   backward, 128 x 361 x 768, RMS norm, bf16: 213 MB in 41.4 us, 5,160 GB/s
-//   backward, 256 x 361 x 384, layer norm, bf16, masked: 168 MB in 38.9 us, 4,310 GB/s
-// further from it: rows that begin anywhere (forward 256 x 361 x 384 of 387: 42.5 us, a window of 19 instructions each
-// way a vector), rows of a block (forward 9,000 x 4,096, bf16, RMS: 36.5 us of 22.5; barriers), single elements there
-// (5,000 x 4,099: 93 us of 12.5), rows read again (backward 1,000 x 20,000, float32: 150 us of 37).
+//   backward, 256 x 361 x 384, RMS norm, float32: 427 MB in 74.5 us, 5,730 GB/s
+//   the same, layer norm, masked: bf16 168 MB in 39.2 us, 4,280 GB/s; float32 334 MB in 63.5 us, 5,260 GB/s
+// further from it: 2-byte rows of 16 elements a lane (forward, 256 x 361 x 128, 256 and 512, RMS norm, bf16: 12.0, 20.2
+// and 36.4 us of 7.3, 14.6 and 29.0), rows that begin anywhere (forward 256 x 361 x 384 of 387: 42.5 us, a window of 19
+// instructions each way a vector), rows of a block (forward 9,000 x 4,096, bf16, RMS: 36.5 us of 22.5; barriers),
+// single elements there (5,000 x 4,099: 93 us of 12.5), rows read again (backward 1,000 x 20,000, float32: 150 us of
+// 37).
 
 #include <algorithm>
 #include <cmath>
@@ -68,8 +74,8 @@ __device__ __forceinline__ bool token_on(const LayerParams& p, int64_t r) { retu
 
 // 1 / sqrt(var + eps) of a sum of squares around a value that is `delta` from the mean; NaN where the squares passed
 // float32's range. Without an eps NaN too where the variance is 0. A row of equal values has the same distance from its
-// first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square: `slack` (1 with an
-// eps) makes that negative, and `least` (0 with an eps, otherwise -inf) leaves it so.
+// first mean everywhere, mostly not 0, and a variance that is the rounding of two sums of its square: `slack` (1 with
+// an eps) makes that negative, and `least` (0 with an eps, otherwise -inf) leaves it so.
 __device__ __forceinline__ float rstd_of(const LayerParams& p, float squares, float inv, float delta) {
   const float var = squares * inv - delta * p.slack * delta;
   if (!(squares <= 3.402823466e38f)) return __int_as_float(0x7fffffff);
@@ -345,7 +351,9 @@ struct Place {
 // memory (16-byte parts of all vectors side by side, each read without a conflict). Shared where that makes room for a
 // third block on an SM: 24 elements of 2 bytes a lane, 256 boards x 361 x 384 layer norm, bf16, 25.6 us and 27.2 in
 // registers; float32 rows, whose ring leaves room for two blocks, lose (64 x 361 x 768: 32.6 and 24.8 us), and so do 8
-// elements, which registers let run four blocks at once (2,000,000 x 16, bf16: 40.7 and 33.1 us).
+// elements, which registers let run four blocks at once (2,000,000 x 16, bf16: 40.7 and 33.3 us). 16 elements of 2
+// bytes run two blocks from registers and would gain too, which is not made use of yet (256 boards x 361 x 128, 256 and
+// 512, layer norm, bf16, masked: 14.2, 22.9 and 40.5 us, from shared memory 12.9, 20.2 and 35.2).
 template <int VEC, int NV, bool BLOCK, bool SHIFT, bool SHARED>
 struct Affine {
   using At = Place<VEC, NV, BLOCK, SHIFT>;
@@ -481,6 +489,9 @@ __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads,
 }
 
 // LEAN: RMS norm without a bias, which needs no sum of g and none of dy.
+// 128 registers do not hold 24 elements a lane of rows that begin anywhere: LEAN spills 188 bytes a thread (2-byte
+// types; 128 x 361 x 767, bf16: 82.5 us of 32.5) or 452 (float32: 117 us of 65); without LEAN float32 spills 72 and,
+// with 16 elements, 88.
 template <typename T, int VEC, int NV, bool BLOCK, bool SHIFT, bool LEAN>
 __global__ void __launch_bounds__(BLOCK ? kBlockThreads : kThreads, BLOCK ? 1 : 2)
     layer_norm_back_kernel(const LayerParams p) {
@@ -830,7 +841,9 @@ Shape shape_of(int64_t rows, int C, int bytes, int vec, bool backward) {
   if (best >= 0) {
     s.threads = kThreads;
     const int64_t per = kThreads / s.lanes, all = (rows + per - 1) / per;
-    // as many blocks as run at once, by registers and by the ring
+    // about as many blocks as run at once, by registers and by the ring. Of float32 rows of 9 to 16 channels, and of
+    // 2-byte rows of up to 16 that begin anywhere, registers let one less to an SM run than are launched: the last ones
+    // wait (2,000,000 x 16 and x 13, float32: 58.3 and 94.7 us; 51.1 and 85.2 with a block less)
     const int by_registers = backward ? 2 : s.nv * whole <= 8 ? (s.shift ? 3 : 4)
                                           : shared_params(s.vec, s.nv, false, s.shift) ? 3 : 2;
     const int row = (backward ? 2 : 1) * (s.nv + (s.shift ? 1 : 0)) * 16;
