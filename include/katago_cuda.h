@@ -383,9 +383,9 @@ int kc_embed_rows_backward(const kc_embed_desc* desc, const int32_t* d_ids, cons
  *   loss = T^2 * sum over j of p[j] * (log p[j] - log q[id[j]]),
  * L = the entries' own log sum of exp(top_logits / T) (p adds up to 1), or d_teacher_log_sum[row], the teacher's over
  * all its classes (p adds up to what the entries hold of it; the rest of the teacher's distribution is left out).
- * Exponentials and their sums are float32, off by up to 2^-17 of themselves (rows of up to 131,072 classes): the loss
- * is off by up to that times T^2 * sum of p, the gradient by up to that times dloss * T * q. The loss of a student near
- * its teacher does not grow with T, hence the limit of T. */
+ * Exponentials and their sums are float32, off by up to 2^-16 of themselves (rows of up to 131,072 classes; 2^-18 up to
+ * 2,048): the loss is off by up to that times T^2 * sum of p, the gradient by up to that times dloss * T * (q + p). The
+ * loss of a student near its teacher does not grow with T, hence the limit of T. */
 typedef struct kc_distill_desc {
   int32_t dtype;     /* KC_PRECISION_* of logits and dlogits */
   int32_t classes;   /* 1 .. 2^30 */
